@@ -281,6 +281,118 @@ int mi_rotary_two(const mi_rotary_rows* rows, const void* cos, const void* sin, 
                   int32_t rot_dim, int64_t table_rows, int64_t seq_len_for_null_ids, int inverse, int interleaved, int dtype, int table_dtype, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Norms of queries and keys over each head with the rotary embedding in the same pass: attention.py:805-806 (norm_query, norm_key of
+ * key_query_norm: core/nn/norm/rms_norm.py:47-50 or layernorm.py:75-86 over head_dim) followed by :836-845 (rotary), for both tensors in one launch.
+ *   xh = x * rsqrt(mean(x^2) + eps)  (layer_norm: (x - mean) * rsqrt(var + eps)),  out = R(position) (xh * weight (+ bias))
+ * in fp32 with one rounding on store.  x: [n_tokens, heads, head_dim] by element strides (token, head), features contiguous; weight, bias:
+ * [head_dim] of the same type.  A head count of 0 leaves a tensor out (its pointers may be NULL).  rotary_cos NULL: no rotation.  Tables, position ids and
+ * their clamping as for mi_rotary (rot_dim features rotated, table_dtype the data type or fp32) and, with rotary_interleaved, as for mi_rotary_complex.
+ * head_dim up to 256; rows that are not whole 16-byte vectors are taken element by element.
+ * Algorithmic HBM bytes: fwd 2, bwd 3 * n_tokens * (n_q_heads + n_kv_heads) * head_dim * e, and the table rows touched.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct mi_norm_rotary_args {
+    const void* q;
+    const void* k;
+    void* q_out;
+    void* k_out;
+    const void* q_weight;
+    const void* k_weight;
+    const void* q_bias;                /* or NULL */
+    const void* k_bias;
+    const void* rotary_cos;
+    const void* rotary_sin;
+    const int64_t* position_ids;       /* [n_tokens] */
+    int64_t n_tokens, table_rows;
+    int64_t q_stride_token, q_stride_head, k_stride_token, k_stride_head;
+    int64_t q_out_stride_token, q_out_stride_head, k_out_stride_token, k_out_stride_head;
+    int32_t n_q_heads, n_kv_heads, head_dim, rot_dim, layer_norm, rotary_interleaved, dtype, table_dtype;
+    float eps;
+    void* stream;
+} mi_norm_rotary_args;
+int mi_norm_rotary_fwd(const mi_norm_rotary_args* args);
+
+/* Backward: from fwd.q, fwd.k (fwd.q_out, fwd.k_out and the biases are not looked at) and the gradients of the outputs
+ *   dn = R^T d_out,  dweight = sum dn * xh,  dbias = sum dn,  g = dn * weight,  dx = rstd * (g - xh * mean(g * xh) (- mean(g): layer_norm)).
+ * The statistics are recomputed.  dweight / dbias (in `dtype`; may be NULL) are sums of per-workgroup fp32 partial sums in `workspace`, in a fixed
+ * order (bit-reproducible).  n_tokens must not be 0. */
+typedef struct mi_norm_rotary_bwd_args {
+    mi_norm_rotary_args fwd;
+    const void* d_q_out;
+    const void* d_k_out;
+    void* dq;
+    void* dk;
+    void* dq_weight;
+    void* dk_weight;
+    void* dq_bias;
+    void* dk_bias;
+    int64_t d_q_out_stride_token, d_q_out_stride_head, d_k_out_stride_token, d_k_out_stride_head;
+    int64_t dq_stride_token, dq_stride_head, dk_stride_token, dk_stride_head;
+    void* workspace;
+    size_t workspace_bytes;
+} mi_norm_rotary_bwd_args;
+size_t mi_norm_rotary_bwd_workspace_bytes(int32_t head_dim);
+int mi_norm_rotary_bwd(const mi_norm_rotary_bwd_args* args);
+
+/* ------------------------------------------------------------------------------------------
+ * Paged KV cache.  The reference grows one cache per sequence by torch.cat (attention.py:852-869); here keys (post-rotary) and values of all
+ * sequences lie in pages [n_pages, page_size, n_kv_heads, head_dim] (element strides page / token / head, features contiguous, the same for K and V,
+ * page_size a multiple of 16), and page_table [batch, max_pages] (int32, row stride page_table_stride) names the pages of a sequence in the order of its
+ * positions.  New tokens of all sequences are packed: sequence b owns tokens cu_seqlens[b] .. cu_seqlens[b + 1], any number of them, none included.
+ * ctx_len[b] counts the keys of sequence b INCLUDING its new ones.  Tokens behind the last sequence belong to nobody.
+ *
+ * mi_paged_append stores the new tokens' keys and values at positions ctx_len[b] - new[b] .. ctx_len[b] - 1 of their sequences: rows.k, normed where
+ * rows.k_weight is given and rotated where rows.rotary_cos is, and v as it is; in the same launch q_out = the same of rows.q (n_q_heads 0: none).  A token
+ * whose position or page lies outside the page table or the cache is not stored.  rows.k_out is not looked at.  Two tokens must not share a slot.
+ * bf16 or f16.  Algorithmic HBM bytes: 2 * n_tokens * (n_q_heads + 2 n_kv_heads) * head_dim * e.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct mi_paged_append_args {
+    mi_norm_rotary_args rows;
+    const void* v;
+    void* k_pages;
+    void* v_pages;
+    const int32_t* page_table;
+    const int32_t* cu_seqlens;
+    const int32_t* ctx_len;
+    int64_t v_stride_token, v_stride_head;
+    int64_t page_stride, page_stride_token, page_stride_head;
+    int64_t page_table_stride;
+    int32_t batch, n_pages, page_size, max_pages;
+} mi_paged_append_args;
+int mi_paged_append(const mi_paged_append_args* args);
+
+/* Attention of the new tokens over the pages (mi_paged_append first): token i of the n of sequence b attends to its keys at positions u < ctx_len[b] and, when
+ * causal, u <= ctx_len[b] - n + i.  Softmax in fp32 of scores scaled by softmax_scale, probabilities rounded to `dtype` before P V as in mi_attn_fwd; a row
+ * without keys yields zeros.  q, o [total_q, n_q_heads, head_dim] by element strides; query head h reads KV head h / (n_q_heads / n_kv_heads).  Rows of o
+ * behind the last sequence are left as they are.  head_dim in {32, 64, 96, 128}, bf16 or f16, max_pages * page_size <= 2^30.
+ * max_q_len: an upper bound of the new tokens of a sequence, 0 if unknown (the launches for longer ones are then made too; sequences over the bound may be
+ * left out).  Lengths beyond the page table count its room; a page number outside the cache reads the nearest page inside.
+ * workspace: mi_paged_attn_workspace_bytes() bytes for calls of up to `tokens` tokens, 16-byte aligned, one call at a time; nothing in it has to be cleared.
+ * The key axis is cut by the lengths on the device, so that the work of a ragged batch is even; the order of the sums depends on the lengths of all
+ * sequences of the call, and on nothing else.
+ * Algorithmic work: 4 * head_dim * n_q_heads * pairs flop; HBM bytes 2 * sum ctx_len * n_kv_heads * head_dim * e + 2 * total_q * n_q_heads * head_dim * e. */
+typedef struct mi_paged_attn_args {
+    const void* q;
+    const void* k_pages;
+    const void* v_pages;
+    void* o;
+    const int32_t* page_table;
+    const int32_t* cu_seqlens;
+    const int32_t* ctx_len;
+    int64_t total_q;
+    int64_t q_stride_token, q_stride_head, o_stride_token, o_stride_head;
+    int64_t page_stride, page_stride_token, page_stride_head;
+    int64_t page_table_stride;
+    int32_t batch, n_pages, page_size, max_pages;
+    int32_t n_q_heads, n_kv_heads, head_dim, dtype, causal, max_q_len;
+    float softmax_scale;
+    void* workspace;
+    size_t workspace_bytes;
+    void* stream;
+} mi_paged_attn_args;
+size_t mi_paged_attn_workspace_bytes(int64_t tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim);
+int mi_paged_attn(const mi_paged_attn_args* args);
+
+/* ------------------------------------------------------------------------------------------
  * Attention core.  Replaces core/nn/attention/attention.py:108-213 (multi_head_attention) with
  * core/nn/masked_softmax/masked_softmax.py:14-34 as softmax and :76-105 as mask, plus repeat_kv
  * (:60-69) and, when cos/sin are given, the rotary call at :836-845.  Interface precedent for a

@@ -27,6 +27,8 @@ EXPORTS = (
     "mi_swiglu_fwd", "mi_swiglu_bwd", "mi_rotary", "mi_rotary_complex", "mi_rotary_two",
     "mi_attn_fwd", "mi_attn_bwd_workspace_bytes", "mi_attn_bwd_workspace_bytes_kv", "mi_attn_bwd_workspace_bytes_for", "mi_attn_bwd",
     "mi_gemm", "mi_gemm_workspace_bytes", "mi_gemm_with_workspace", "mi_rows_product", "mi_transpose16", "mi_column_sum", "mi_add_rmsnorm_bwd", "mi_add_layernorm_fwd", "mi_add_layernorm_bwd", "mi_attn_decode_workspace_bytes", "mi_attn_decode", "mi_attn_decode_with_tickets", "mi_fill_cache", "mi_attn_decode_static_scratch_bytes", "mi_attn_decode_static",
+    "mi_norm_rotary_fwd", "mi_norm_rotary_bwd_workspace_bytes", "mi_norm_rotary_bwd", "mi_paged_append",
+    "mi_paged_attn_workspace_bytes", "mi_paged_attn",
 )
 
 
@@ -102,6 +104,48 @@ class MiRowsArgs(Structure):
 class MiRotaryRows(Structure):
     _fields_ = [("x", c_void_p), ("out", c_void_p), ("x_stride_token", c_int64), ("x_stride_head", c_int64), ("out_stride_token", c_int64),
                 ("out_stride_head", c_int64), ("n_heads", c_int32)]
+
+
+class MiNormRotaryArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p), ("q_weight", c_void_p), ("k_weight", c_void_p),
+        ("q_bias", c_void_p), ("k_bias", c_void_p), ("rotary_cos", c_void_p), ("rotary_sin", c_void_p), ("position_ids", c_void_p),
+        ("n_tokens", c_int64), ("table_rows", c_int64),
+        ("q_stride_token", c_int64), ("q_stride_head", c_int64), ("k_stride_token", c_int64), ("k_stride_head", c_int64),
+        ("q_out_stride_token", c_int64), ("q_out_stride_head", c_int64), ("k_out_stride_token", c_int64), ("k_out_stride_head", c_int64),
+        ("n_q_heads", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32), ("rot_dim", c_int32), ("layer_norm", c_int32),
+        ("rotary_interleaved", c_int32), ("dtype", c_int32), ("table_dtype", c_int32), ("eps", c_float), ("stream", c_void_p),
+    ]
+
+
+class MiNormRotaryBwdArgs(Structure):
+    _fields_ = [
+        ("fwd", MiNormRotaryArgs), ("d_q_out", c_void_p), ("d_k_out", c_void_p), ("dq", c_void_p), ("dk", c_void_p),
+        ("dq_weight", c_void_p), ("dk_weight", c_void_p), ("dq_bias", c_void_p), ("dk_bias", c_void_p),
+        ("d_q_out_stride_token", c_int64), ("d_q_out_stride_head", c_int64), ("d_k_out_stride_token", c_int64), ("d_k_out_stride_head", c_int64),
+        ("dq_stride_token", c_int64), ("dq_stride_head", c_int64), ("dk_stride_token", c_int64), ("dk_stride_head", c_int64),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class MiPagedAppendArgs(Structure):
+    _fields_ = [
+        ("rows", MiNormRotaryArgs), ("v", c_void_p), ("k_pages", c_void_p), ("v_pages", c_void_p), ("page_table", c_void_p), ("cu_seqlens", c_void_p),
+        ("ctx_len", c_void_p), ("v_stride_token", c_int64), ("v_stride_head", c_int64), ("page_stride", c_int64), ("page_stride_token", c_int64),
+        ("page_stride_head", c_int64), ("page_table_stride", c_int64), ("batch", c_int32), ("n_pages", c_int32), ("page_size", c_int32),
+        ("max_pages", c_int32),
+    ]
+
+
+class MiPagedAttnArgs(Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k_pages", c_void_p), ("v_pages", c_void_p), ("o", c_void_p), ("page_table", c_void_p), ("cu_seqlens", c_void_p),
+        ("ctx_len", c_void_p), ("total_q", c_int64), ("q_stride_token", c_int64), ("q_stride_head", c_int64), ("o_stride_token", c_int64),
+        ("o_stride_head", c_int64), ("page_stride", c_int64), ("page_stride_token", c_int64), ("page_stride_head", c_int64),
+        ("page_table_stride", c_int64), ("batch", c_int32), ("n_pages", c_int32), ("page_size", c_int32), ("max_pages", c_int32),
+        ("n_q_heads", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32), ("dtype", c_int32), ("causal", c_int32), ("max_q_len", c_int32),
+        ("softmax_scale", c_float), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("stream", c_void_p),
+    ]
 
 
 _lib = None
@@ -185,6 +229,18 @@ def _declare(lib):
     lib.mi_add_layernorm_fwd.argtypes = [c_void_p] * 8 + [c_int64, c_int64, c_float, c_int, c_void_p]
     lib.mi_add_layernorm_bwd.restype = c_int
     lib.mi_add_layernorm_bwd.argtypes = [c_void_p] * 10 + [c_size_t, c_int64, c_int64, c_float, c_int, c_void_p]
+    lib.mi_norm_rotary_fwd.restype = c_int
+    lib.mi_norm_rotary_fwd.argtypes = [POINTER(MiNormRotaryArgs)]
+    lib.mi_norm_rotary_bwd_workspace_bytes.restype = c_size_t
+    lib.mi_norm_rotary_bwd_workspace_bytes.argtypes = [c_int32]
+    lib.mi_norm_rotary_bwd.restype = c_int
+    lib.mi_norm_rotary_bwd.argtypes = [POINTER(MiNormRotaryBwdArgs)]
+    lib.mi_paged_append.restype = c_int
+    lib.mi_paged_append.argtypes = [POINTER(MiPagedAppendArgs)]
+    lib.mi_paged_attn_workspace_bytes.restype = c_size_t
+    lib.mi_paged_attn_workspace_bytes.argtypes = [c_int64, c_int32, c_int32, c_int32]
+    lib.mi_paged_attn.restype = c_int
+    lib.mi_paged_attn.argtypes = [POINTER(MiPagedAttnArgs)]
     lib.mi_attn_fwd.restype = c_int
     lib.mi_attn_fwd.argtypes = [POINTER(MiAttnArgs)]
     lib.mi_attn_bwd_workspace_bytes.restype = c_size_t

@@ -1,0 +1,813 @@
+// Attention of ragged chunks of new tokens over a paged KV cache for gfx950.
+//
+// Two kernels share a call by the number of rows (new tokens x query heads of a group) of a sequence: `paged_rows` for up to kRowLimit of them (single
+// tokens, drafts), bound by the cache's bytes, and `paged_tiles` for chunks, bound by the matrix pipe.  Either cuts its work by paged_plan.h, which every
+// workgroup evaluates on the lengths by itself; partial results (running maximum, sum, unscaled output) of sequences with several splits go to the
+// workspace and are merged by `paged_merge`.
+//
+// Pages hold a multiple of 16 keys, so 16 neighbouring keys (what one row of an MFMA operand tile, or one wavefront's share of a tile's direct loads, needs)
+// have one page: its number is found once per 16 keys and wavefront, and a paged cache costs next to nothing against a contiguous one.
+#include "attn_common.h"
+#include "paged_plan.h"
+
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+
+namespace {
+
+constexpr int kRowLimit = 16;        // rows of a sequence up to which paged_rows computes it
+constexpr int kRowBlock = 16;
+constexpr int kRowChunk = 32;        // keys per wavefront and step of paged_rows
+constexpr int kRowWaves = 4;
+constexpr int kTileRows = 256;
+constexpr int kTileKeys = 64;
+constexpr float kRescaleGap = 8.0f;  // log2 units by which a row's maximum may lag before its output is rescaled
+
+struct PagedParams {
+    const elem_t *q, *kp, *vp;
+    elem_t* o;
+    const int32_t *table, *cu, *ctx;
+    int64_t table_stride, q_st, q_sh, o_st, o_sh, p_sp, p_st, p_sh;
+    int batch, total, n_pages, page, max_pages, capacity, nq, nkv, n_rep, causal;
+    uint32_t page_m, rep_m, nkv_m;
+    float scale_log2;
+    PagedPlan rows, tiles;
+    int rows_partials, tiles_partials;                // how many per KV head
+    float *rows_o, *rows_ml, *tiles_o, *tiles_ml;     // partial results: [partial][KV head][row of the block][feature], and (maximum in log2 units, sum)
+};
+
+__device__ __forceinline__ f32x4v mfma_16x16x32(elem8_t a, elem8_t b, f32x4v c) {
+#ifdef MI_ELEM_F16
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+#else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+#endif
+}
+
+// sums over lanes 0 .. this one
+__device__ __forceinline__ int prefix_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);      // row_shr 1, 2, 4, 8, then the last lanes of the rows in front
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return v;
+}
+
+// A sequence as one workgroup or row meets it; the same in every lane.
+struct Found {
+    int b;             // -1: none
+    int slot;          // of the sequence's blocks * splits, where it was looked for by a slot
+    int splits;
+    int partial;       // first partial result of the sequence (splits > 1)
+    PagedSeq seq;
+    PagedWork work;
+};
+
+// The sequence that `hit(first slot, slots, first partial result, partial results)` names, lane i looking at sequences i, i + 64, ...
+template <class Hit> __device__ __forceinline__ Found find_work(const PagedParams& p, const PagedPlan& plan, Hit hit) {
+    const int lane = threadIdx.x & 63;
+    PagedSeq seq{};
+    PagedWork work{};
+    auto look = [&](int base) {
+        const int b = base + lane, i = min(b, p.batch - 1);
+        seq = paged_seq(p.cu[i], p.cu[i + 1], p.ctx[i], p.total, p.capacity);
+        work = paged_work(plan, seq, p.n_rep);
+        if (b >= p.batch) work.blocks = seq.n = 0;
+    };
+    int64_t units = 0;
+    if (plan.target > 0) {
+        for (int base = 0; base < p.batch; base += 64) {
+            look(base);
+            units += (uint32_t)__builtin_amdgcn_readlane(prefix_sum(work.blocks * work.tiles), 63);
+        }
+    }
+    const int split_tiles = paged_split_tiles(plan, units);
+    int slots = 0, partials = 0;
+    Found f;
+    f.b = -1;
+    for (int base = 0; base < p.batch; base += 64) {
+        if (p.batch > 64 || plan.target == 0) look(base);
+        const int splits = paged_splits(work, split_tiles), n = work.blocks * splits, part = splits > 1 ? n : 0;
+        const int upto = slots + prefix_sum(n), part_upto = partials + prefix_sum(part);
+        const uint64_t found = __ballot(work.blocks > 0 && hit(upto - n, n, part_upto - part, part));
+        if (found != 0) {
+            const int l = __builtin_ctzll(found);
+            f.b = base + l;
+            f.slot = __builtin_amdgcn_readlane(upto - n, l);
+            f.splits = __builtin_amdgcn_readlane(splits, l);
+            f.partial = __builtin_amdgcn_readlane(part_upto - part, l);
+            f.seq.first = __builtin_amdgcn_readlane(seq.first, l);
+            f.seq.n = __builtin_amdgcn_readlane(seq.n, l);
+            f.seq.ctx = __builtin_amdgcn_readlane(seq.ctx, l);
+            f.seq.len = __builtin_amdgcn_readlane(seq.len, l);
+            f.work.blocks = __builtin_amdgcn_readlane(work.blocks, l);
+            f.work.tiles = __builtin_amdgcn_readlane(work.tiles, l);
+            return f;
+        }
+        slots = __builtin_amdgcn_readlane(upto, 63);
+        partials = __builtin_amdgcn_readlane(part_upto, 63);
+    }
+    return f;
+}
+
+// Page of the 16 keys from 16 * group on.  A number outside the cache is taken for the nearest inside.
+__device__ __forceinline__ int page_of(const PagedParams& p, const int32_t* table, int group) {
+    const int page = table[divide((uint32_t)group * 16u, p.page, p.page_m)];
+    return page < 0 ? 0 : (page >= p.n_pages ? p.n_pages - 1 : page);
+}
+// row of a page that the group starts at
+__device__ __forceinline__ int row_in_page(const PagedParams& p, int group) {
+    const int key = group * 16;
+    return key - divide((uint32_t)key, p.page, p.page_m) * p.page;
+}
+
+// ---- rows whose products met values that are not finite -----------------------------------------------------------------------------------------------
+// A matrix product multiplies a masked key's probability, zero, with whatever its value holds, and zero times infinity or NaN is NaN.  So a row that is not
+// finite and has fewer keys than its workgroup multiplies is computed anew from its own keys alone, by one wavefront: key by key with a lane each
+// for the scores, then feature by feature (2 lane, 2 lane + 1).  Nothing but such values pays for it.
+__device__ __forceinline__ bool not_finite(float x) {
+    uint32_t u = __float_as_uint(x);
+    asm("" : "+v"(u));                                     // a test of these bits as they are: one of a float is compiled without NaN
+    return (u & 0x7f800000u) == 0x7f800000u;
+}
+
+template <int D>
+__device__ __forceinline__ void own_keys_only(const PagedParams& p, const int32_t* table, int kvh, const elem_t* q, int k0, int limit, float& M, float& L, float& O0,
+                                              float& O1) {
+    const int lane = threadIdx.x & 63, d = 2 * lane;
+    M = -INFINITY;
+    L = O0 = O1 = 0.f;
+    for (int key0 = k0; key0 < limit; key0 += 64) {
+        const int key = min(key0 + lane, limit - 1), n = min(64, limit - key0);
+        const int64_t at = (int64_t)page_of(p, table, key >> 4) * p.p_sp + (int64_t)(row_in_page(p, key >> 4) + (key & 15)) * p.p_st + (int64_t)kvh * p.p_sh;
+        float s = 0.f;
+        for (int f = 0; f < D; f += 8) {
+            float a[8], b[8];
+            Elem<elem_t>::unpack(ld128(q + f), a);
+            Elem<elem_t>::unpack(ld128(p.kp + at + f), b);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += a[i] * b[i];
+        }
+        s = lane < n ? s * p.scale_log2 : -INFINITY;
+        const float m = fmaxf(M, group_max<64>(s)), use = m == -INFINITY ? 0.f : m, alpha = M == -INFINITY ? 0.f : fast_exp2(M - use);
+        const float e = lane < n ? fast_exp2(s - use) : 0.f, e_rounded = (float)(elem_t)e;
+        L = L * alpha + group_sum<64>(e);
+        O0 *= alpha;
+        O1 *= alpha;
+        M = m;
+        for (int j = 0; j < n; ++j) {
+            const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e_rounded), j));
+            const int64_t vj = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), j) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)at, j));
+            if (d < D) {
+                const uint32_t v = *reinterpret_cast<const uint32_t*>(p.vp + vj + d);
+                O0 += pj * elem_lo(v);
+                O1 += pj * elem_hi(v);
+            }
+        }
+    }
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------------------------------------------
+// One workgroup per (block of 16 rows, KV head, split); its wavefronts take chunks of 32 keys in turn:
+//     S^T[key][row] = K Q^T      v_mfma_f32_16x16x32, A = K rows straight from global memory in operand layout, B = Q^T
+//     online softmax over keys   a lane's column is a row: eight keys in the lane, two lane exchanges
+//     O^T[feature][row] += V^T P^T    V passes through a wavefront's own LDS and is read back transposed
+// Every cached element is read from memory once per block of rows.  The next chunk's loads are under way while a chunk is computed.
+template <int D>
+__global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const PagedParams p) {
+    constexpr int NWV = kRowWaves, kThreads = 64 * NWV;
+    constexpr int KS = D / 32, DT = D / 16;
+    constexpr int VSTR = 2 * D + 32;          // bytes per key row of a staged V chunk: transposed reads of 8 rows x 32 bytes hit 256 distinct bytes
+    constexpr int V_ITEMS = 8 * (D / 8);      // (four keys, eight features) of a chunk
+    constexpr int V_PER_LANE = (V_ITEMS + 63) / 64;
+    __shared__ __attribute__((aligned(16))) char v_lds[NWV][kRowChunk * VSTR];
+    __shared__ float wm_lds[NWV][16], wl_lds[NWV][16], wo_lds[NWV][16][D + 1];
+    __shared__ int redo_lds[16];
+
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, G = lane >> 4;
+    const int slot = divide(blockIdx.x, p.nkv, p.nkv_m), kvh = blockIdx.x - slot * p.nkv;
+    const Found f = find_work(p, p.rows, [&](int first, int n, int, int) { return slot >= first && slot < first + n; });
+    if (f.b < 0) return;
+    const int in = slot - f.slot, split = in / f.work.blocks, block = in - split * f.work.blocks;
+    if (split >= f.splits || (f.splits > 1 && (uint32_t)(f.partial + in) >= (uint32_t)p.rows_partials)) return;
+    int s0, s1;
+    paged_split_keys(p.rows, f.seq, f.work, f.splits, split, s0, s1);
+    const int n_rows = min(kRowBlock, f.seq.n * p.n_rep - block * kRowBlock);
+    // this lane's row
+    const int row = block * kRowBlock + min(l16, n_rows - 1), token = divide(row, p.n_rep, p.rep_m), head = kvh * p.n_rep + row - token * p.n_rep;
+    const int limit = l16 < n_rows ? min(paged_limit(f.seq, token, p.causal), s1) : 0;
+    const int end = group_max<16>(limit);                  // the same for the four groups of 16 lanes
+    const int n_iter = __builtin_amdgcn_readfirstlane(end > s0 ? (end - s0 + NWV * kRowChunk - 1) / (NWV * kRowChunk) : 0);
+    const int last = max(s1 - 1, 0), last_group = last >> 4;      // keys past the split repeat its last one
+
+    uint4 raw[KS];
+    {
+        const elem_t* qr = p.q + (int64_t)(f.seq.first + token) * p.q_st + (int64_t)head * p.q_sh + 8 * G;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) raw[ks] = ld128(qr + 32 * ks);
+    }
+    f32x4v o_acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o_acc[dt] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    float m_i = -INFINITY, l_i = 0.f;
+
+    const int32_t* table = p.table + (int64_t)f.b * p.table_stride;
+    const elem_t *kbase = p.kp + (int64_t)kvh * p.p_sh, *vbase = p.vp + (int64_t)kvh * p.p_sh;
+    char* vt = v_lds[wave];
+    const char* vt_lane = vt + (4 * G + (l16 >> 2)) * VSTR + 8 * (l16 & 3);
+    // lane i: pages of both groups of this wavefront's chunk i of the 64 from `ids_from` on
+    int ids[2], ids_from = 0;
+    auto look_up = [&](int from) {
+        ids_from = from;
+        const int group = (s0 + (NWV * (from + lane) + wave) * kRowChunk) >> 4;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) ids[t] = page_of(p, table, min(group + t, last_group));
+    };
+
+    struct ChunkRegs {
+        elem8_t kf[2][KS];
+        uint4 vraw[V_PER_LANE][4];
+    };
+    auto request = [&](ChunkRegs& c, int it) {
+        const int key0 = s0 + (NWV * it + wave) * kRowChunk;
+        int64_t at[2];                                     // of key 16 * group in the pages
+        int group[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            group[t] = min((key0 >> 4) + t, last_group);
+            at[t] = (int64_t)__builtin_amdgcn_readlane(ids[t], it - ids_from) * p.p_sp + (int64_t)row_in_page(p, group[t]) * p.p_st;
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int r = min(key0 + 16 * t + l16, last) - 16 * group[t];
+            const elem_t* kr = kbase + at[t] + (int64_t)r * p.p_st + 8 * G;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) c.kf[t][ks] = __builtin_bit_cast(elem8_t, ldg_nt(reinterpret_cast<const uint4*>(kr + 32 * ks)));
+        }
+#pragma unroll
+        for (int j = 0; j < V_PER_LANE; ++j) {
+            const int item = lane + 64 * j;
+            if (V_ITEMS % 64 != 0 && item >= V_ITEMS) break;
+            const int quad = item / (D / 8), dg = item % (D / 8);
+            const int g = quad < 4 ? group[0] : group[1];
+            const elem_t* vr = vbase + (quad < 4 ? at[0] : at[1]) + 8 * dg;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int rr = min(key0 + 4 * quad + r, last) - 16 * g;
+                c.vraw[j][r] = ldg_nt(reinterpret_cast<const uint4*>(vr + (int64_t)rr * p.p_st));
+            }
+        }
+    };
+    elem8_t qf[KS];
+    auto load_chunk = [&](ChunkRegs& c, int it) {
+        if (it >= n_iter) return;
+        if (it - ids_from >= 64) look_up(it);
+        request(c, it);
+    };
+    auto process_chunk = [&](ChunkRegs& c, int it) {
+        const int key0 = s0 + (NWV * it + wave) * kRowChunk;
+        const bool active = key0 < end;                    // wave-uniform
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        elem8_t pf;
+        float alpha = 1.f;
+        if (active) {
+            f32x4v s_acc[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                s_acc[t] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) s_acc[t] = mfma_16x16x32(c.kf[t][ks], qf[ks], s_acc[t]);
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (key0 + 16 * t + 4 * G + r >= limit) s_acc[t][r] = -INFINITY;
+                    mx = fmaxf(mx, s_acc[t][r]);
+                }
+            mx = quad_max(mx);
+            const float m_new = fmaxf(m_i, mx * p.scale_log2), m_use = m_new == -INFINITY ? 0.f : m_new;   // a row may have no key here, or none at all
+            alpha = fast_exp2(m_i - m_use);
+            m_i = m_new;
+            float rs = 0.f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float e = fast_exp2(s_acc[t][r] * p.scale_log2 - m_use);
+                    rs += e;
+                    pf[4 * t + r] = (elem_t)e;             // slot (G, i): key 16 * (i / 4) + 4 * G + i % 4
+                }
+            l_i = l_i * alpha + rs;
+#pragma unroll
+            for (int j = 0; j < V_PER_LANE; ++j) {
+                const int item = lane + 64 * j;
+                if (V_ITEMS % 64 != 0 && item >= V_ITEMS) break;
+                const int quad = item / (D / 8), dg = item % (D / 8);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) st128(vt + (4 * quad + r) * VSTR + 16 * dg, c.vraw[j][r]);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (active) {
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const elem8_t a = tr_pair(vt_lane + 32 * dt, vt_lane + 16 * VSTR + 32 * dt);
+                o_acc[dt] = o_acc[dt] * alpha;
+                o_acc[dt] = mfma_16x16x32(a, pf, o_acc[dt]);
+            }
+        }
+    };
+
+    ChunkRegs ra, rb;
+    if (n_iter > 0) {
+        look_up(0);
+        request(ra, 0);
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) qf[ks] = __builtin_bit_cast(elem8_t, raw[ks]);
+    for (int it = 0; it < n_iter; it += 2) {
+        load_chunk(rb, it + 1);
+        process_chunk(ra, it);
+        if (it + 1 < n_iter) {
+            load_chunk(ra, it + 2);
+            process_chunk(rb, it + 1);
+        }
+    }
+
+    // ---- the wavefronts' results together; of a single split the output, else a partial result ----
+    l_i = quad_sum(l_i);
+    if (G == 0) { wm_lds[wave][l16] = m_i; wl_lds[wave][l16] = l_i; }
+    if (tid < 16) redo_lds[tid] = 0;
+    const int filled = (s1 + kRowChunk - 1) & -kRowChunk;  // chunks are filled up to here: with keys that a row may not see, or with others once more
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) wo_lds[wave][l16][16 * dt + 4 * G + r] = o_acc[dt][r];
+    __syncthreads();
+    const auto emit = [&](int r, int d, float M, float L, float O0, float O1) {
+        if (f.splits == 1) {
+            const int rr = block * kRowBlock + r, i = divide(rr, p.n_rep, p.rep_m);
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            *reinterpret_cast<uint32_t*>(p.o + (int64_t)(f.seq.first + i) * p.o_st + (int64_t)(kvh * p.n_rep + rr - i * p.n_rep) * p.o_sh + d) = pack_elem2(O0 * inv, O1 * inv);
+        } else {
+            const int64_t at = ((int64_t)(f.partial + in) * p.nkv + kvh) * kRowBlock + r;
+            *reinterpret_cast<float2*>(p.rows_o + at * D + d) = make_float2(O0, O1);
+            if (d == 0) *reinterpret_cast<float2*>(p.rows_ml + at * 2) = make_float2(M, L);
+        }
+    };
+    for (int idx = tid; idx < n_rows * (D / 2); idx += kThreads) {
+        const int r = idx / (D / 2), d = 2 * (idx % (D / 2));
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < NWV; ++w) M = fmaxf(M, wm_lds[w][r]);
+        float L = 0.f, O0 = 0.f, O1 = 0.f;
+#pragma unroll
+        for (int w = 0; w < NWV; ++w) {
+            const float wm = wm_lds[w][r], scale = wm == -INFINITY ? 0.f : fast_exp2(wm - M);
+            L += scale * wl_lds[w][r];
+            O0 += scale * wo_lds[w][r][d];
+            O1 += scale * wo_lds[w][r][d + 1];
+        }
+        if (not_finite(O0) || not_finite(O1) || not_finite(L)) redo_lds[r] = 1;
+        emit(r, d, M, L, O0, O1);
+    }
+    if (__ballot(l16 < n_rows && limit < filled) == 0) return;     // the same for the workgroup
+    __syncthreads();
+    for (int r = wave; r < n_rows; r += NWV) {
+        const int lim = __builtin_amdgcn_readlane(limit, r);
+        if (redo_lds[r] == 0 || lim >= filled) continue;
+        const int rr = block * kRowBlock + r, i = divide(rr, p.n_rep, p.rep_m);
+        float M, L, O0, O1;
+        own_keys_only<D>(p, table, kvh, p.q + (int64_t)(f.seq.first + i) * p.q_st + (int64_t)(kvh * p.n_rep + rr - i * p.n_rep) * p.q_sh, s0, lim, M, L, O0, O1);
+        if (2 * lane < D) emit(r, 2 * lane, M, L, O0, O1);
+    }
+}
+
+// ---- chunks -------------------------------------------------------------------------------------------------------------------------------------------
+// Direct loads of this wavefront's 16 rows of a 64-key tile.
+template <int D> struct PageDma {
+    using T = LdsTile<D>;
+    static constexpr int COUNT = T::kInstrs / 4;
+    uint32_t off[COUNT];
+    int lw, lane;
+    __device__ __forceinline__ static void src_of(int n, int lw, int lane, int& row, int& unit_off) {
+        int unit;
+        T::dma_src(lw * COUNT + n, lane, row, unit);
+        if (D == 96 && unit >= D / 8) unit = 0;
+        row -= 16 * lw;
+        unit_off = 16 * unit;
+    }
+    __device__ __forceinline__ void init(int lw_, int lane_, int64_t tok_stride) {
+        lw = lw_;
+        lane = lane_;
+#pragma unroll
+        for (int j = 0; j < COUNT; ++j) {
+            int row, unit_off;
+            src_of(j, lw, lane, row, unit_off);
+            off[j] = (uint32_t)(row * (int)tok_stride * 2 + unit_off);
+        }
+    }
+    // base: key 16 * group of the wavefront's group (uniform); rows: how many of the 16 there are (further ones repeat the last)
+    __device__ __forceinline__ void issue(const elem_t* base, int64_t tok_stride, int rows, char* tile) const {
+        char* dst = tile + 1024 * COUNT * lw;
+        if (rows >= 16) {
+#pragma unroll
+            for (int j = 0; j < COUNT; ++j) DmaPlan<D, 1>::issue_one(off[j], base, dst + 1024 * j);
+        } else {
+            int l = lane;
+            asm volatile("" : "+v"(l));
+#pragma unroll
+            for (int j = 0; j < COUNT; ++j) {
+                int row, unit_off;
+                src_of(j, lw, l, row, unit_off);
+                DmaPlan<D, 1>::issue_one((uint32_t)(min(row, rows - 1) * (int)tok_stride * 2 + unit_off), base, dst + 1024 * j);
+            }
+        }
+    }
+};
+
+// One workgroup per (block of 256 rows, KV head, split): eight wavefronts of 32 rows.  Tiles of 64 keys stream through rings of four swizzled LDS stages,
+// K requested three tiles ahead by the second four wavefronts and V two by the first.  The two groups of four run half a tile apart (enforced by the
+// barriers), so on every SIMD one wavefront issues products while the other computes its softmax:
+//     S^T = K Q^T      A = K rows from LDS, B = Q in registers
+//     softmax          a lane's column is a row of the block; the maximum is raised only when it lags by 2^8, so most tiles rescale nothing
+//     O^T += V^T P^T   B = P^T as the accumulators of S^T hold it, A = V^T by transposing LDS reads
+template <int D>
+__global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p) {
+    constexpr int NW = 8, BN = kTileKeys;
+    constexpr int KS = D / 16, DT = D / 32, NS = 4;
+    using Tile = LdsTile<D>;
+    constexpr int RB = Tile::RB, TILE = Tile::kBytes, IPW = PageDma<D>::COUNT;
+    __shared__ __attribute__((aligned(1024))) char k_lds[NS * TILE];
+    __shared__ __attribute__((aligned(1024))) char v_lds[NS * TILE];
+    __shared__ int end_lds[NW];
+
+    const int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63, l32 = lane & 31, g = lane >> 5;
+    const int slot = divide(blockIdx.x, p.nkv, p.nkv_m), kvh = blockIdx.x - slot * p.nkv;
+    const Found f = find_work(p, p.tiles, [&](int first, int n, int, int) { return slot >= first && slot < first + n; });
+    if (f.b < 0) return;                                   // the same for the whole workgroup
+    const int in = slot - f.slot, split = in / f.work.blocks, block = f.work.blocks - 1 - (in - split * f.work.blocks);      // longest first
+    if (split >= f.splits || (f.splits > 1 && (uint32_t)(f.partial + in) >= (uint32_t)p.tiles_partials)) return;
+    int s0, s1;
+    paged_split_keys(p.tiles, f.seq, f.work, f.splits, split, s0, s1);
+
+    // ---- this lane's row, its keys [s0, limit), its part of Q ----
+    const int n_rows = f.seq.n * p.n_rep, row = block * kTileRows + wave * 32 + l32;
+    const int rr = min(row, n_rows - 1), token = divide(rr, p.n_rep, p.rep_m), head = kvh * p.n_rep + rr - token * p.n_rep;
+    const int limit = row < n_rows ? min(paged_limit(f.seq, token, p.causal), s1) : 0;
+    elem8_t qf[KS];
+    {
+        const elem_t* qrow = p.q + (int64_t)(f.seq.first + token) * p.q_st + (int64_t)head * p.q_sh + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = __builtin_bit_cast(elem8_t, ld128(qrow + 16 * ks));
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));     // in registers before the loop: waited for here, not behind the loop's loads
+    const int wmax = group_max<64>(limit);
+    if (lane == 0) end_lds[wave] = wmax;
+    __syncthreads();
+    int end = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) end = max(end, end_lds[w]);
+    const int n_tiles = __builtin_amdgcn_readfirstlane(end > s0 ? (end - s0 + BN - 1) / BN : 0);
+
+    f32x16_t o_acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o_acc[dt][r] = 0.f;
+    float m_i = -INFINITY, l_i = 0.f;
+
+    // ---- direct loads: wavefronts 0 - 3 of V, 4 - 7 of K; wavefront lw of either of keys 16 lw .. + 15 of a tile ----
+    const bool v_role = wave < 4;
+    const int lw = wave & 3, grp = wave >> 2;
+    const int32_t* table = p.table + (int64_t)f.b * p.table_stride;
+    const elem_t* base = (v_role ? p.vp : p.kp) + (int64_t)kvh * p.p_sh;
+    char* ring = v_role ? v_lds : k_lds;
+    const int last = max(s1 - 1, 0), last_group = last >> 4;
+    PageDma<D> dma;
+    dma.init(lw, lane, p.p_st);
+    int ids = 0;                                           // lane i: page of this wavefront's keys in tile i of the current 64
+    auto load_tile = [&](int tile) {
+        if (tile >= n_tiles) return;
+        const int group0 = (s0 >> 4) + lw;
+        if ((tile & 63) == 0) ids = page_of(p, table, min(group0 + 4 * (tile + lane), last_group));
+        const int group = min(group0 + 4 * tile, last_group);
+        const int page = __builtin_amdgcn_readlane(ids, tile & 63);
+        const elem_t* from = base + (int64_t)page * p.p_sp + (int64_t)row_in_page(p, group) * p.p_st;
+        dma.issue(from, p.p_st, last - 16 * group + 1, ring + (tile % NS) * TILE);
+    };
+    auto n_issued = [&](int a, int b) { return IPW * max(0, min(b, n_tiles) - a); };
+    if (n_tiles > 0) {
+        load_tile(0);
+        load_tile(1);
+        if (!v_role) {
+            load_tile(2);
+            wait_vmcnt_dyn(n_issued(1, 3));
+        }
+    }
+    __syncthreads();
+    if (grp == 1) __syncthreads();
+
+    const float c2 = p.scale_log2;
+    int v_h0, v_h1;
+    Tile::tr_bases(lane, v_h0, v_h1);
+    const int k_row = Tile::row_base(l32, g);
+    f32x16_t s_acc[2];
+    elem8_t pf[4];
+    bool pending = false;
+    constexpr int PV_STEPS = 4 * DT, S_STEPS = 2 * KS, kDepth = 3;
+    auto mfma_phase = [&](auto mode, const char* vt, const char* ks) {
+        constexpr bool kPV = (decltype(mode)::value & 1) != 0, kS = (decltype(mode)::value & 2) != 0;
+        constexpr int first = kPV ? 0 : PV_STEPS, last_step = kS ? PV_STEPS + S_STEPS : PV_STEPS;
+        elem8_t operands[kDepth];                          // requested three products ahead
+        auto fetch = [&](int i) -> elem8_t {
+            if (i < PV_STEPS) {
+                const int m = i / DT, dt = i % DT;
+                return tr_pair(vt + (v_h0 ^ (dt << 6)) + 16 * m * RB, vt + (v_h1 ^ (dt << 6)) + 16 * m * RB);
+            }
+            const int ksi = (i - PV_STEPS) >> 1, t = (i - PV_STEPS) & 1;
+            return *reinterpret_cast<const elem8_t*>(ks + (k_row ^ (ksi << 5)) + 32 * t * RB);
+        };
+        if constexpr (kS) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s_acc[t][r] = 0.f;
+        }
+#pragma unroll
+        for (int i = first; i < first + kDepth && i < last_step; ++i) operands[(i - first) % kDepth] = fetch(i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = first; i < last_step; ++i) {
+            const elem8_t a = operands[(i - first) % kDepth];
+            if (i < PV_STEPS) {
+                const int m = i / DT, dt = i % DT;
+                o_acc[dt] = mfma_32x32x16(a, pf[m], o_acc[dt]);
+            } else {
+                const int ksi = (i - PV_STEPS) >> 1, t = (i - PV_STEPS) & 1;
+                s_acc[t] = mfma_32x32x16(a, qf[ksi], s_acc[t]);
+            }
+            if (i + kDepth < last_step) operands[(i - first) % kDepth] = fetch(i + kDepth);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    for (int it = 0; it <= n_tiles; ++it) {
+        const int kt = s0 + it * BN;
+        const bool wave_active = it < n_tiles && kt < wmax;
+        {
+            const char* vt = v_lds + ((it + NS - 1) % NS) * TILE;
+            const char* ks = k_lds + (it % NS) * TILE;
+            if (pending && wave_active) mfma_phase(std::integral_constant<int, 3>{}, vt, ks);
+            else if (pending) mfma_phase(std::integral_constant<int, 1>{}, vt, ks);
+            else if (wave_active) mfma_phase(std::integral_constant<int, 2>{}, vt, ks);
+        }
+        if (it == n_tiles) break;
+        if (!v_role) wait_vmcnt_dyn(n_issued(it + 2, it + 3));        // K tile it + 1 is read behind this barrier
+        __syncthreads();
+        pending = wave_active;
+        if (wave_active) {
+            if (__any(kt + BN > limit)) {
+                int rel = kt + 4 * g - limit;
+                asm volatile("" : "+v"(rel));              // keeps the 32 compares inside this branch
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (rel + 32 * t + 8 * (r >> 2) + (r & 3) >= 0) s_acc[t][r] = -INFINITY;
+            }
+            float mx = fmaxf(s_acc[0][0], s_acc[1][0]);
+#pragma unroll
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, fmaxf(s_acc[0][r], s_acc[1][r]));
+            mx = pair_max(mx);
+            const float m_cand = mx * c2;
+            if (__any(m_cand > m_i + kRescaleGap)) {
+                const float m_new = fmaxf(m_i, m_cand);
+                float alpha = (m_new == -INFINITY) ? 1.0f : fast_exp2(m_i - m_new);
+                asm volatile("" : "+v"(alpha));            // keeps the multiplies below inside this rarely taken branch
+                m_i = m_new;
+                l_i *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o_acc[dt][r] *= alpha;
+            }
+            const float m_use = (m_i == -INFINITY) ? 0.f : m_i;
+            float rs0 = 0.f, rs1 = 0.f;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const int t = m >> 1, r0 = 8 * (m & 1);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float ev = fast_exp2(s_acc[t][r0 + e] * c2 - m_use);
+                    if (e & 1) rs1 += ev; else rs0 += ev;
+                    pf[m][e] = (elem_t)ev;
+                }
+            }
+            l_i += rs0 + rs1;
+        }
+        load_tile(it + (v_role ? 2 : 3));
+        if (v_role) wait_vmcnt_dyn(n_issued(it + 1, it + 3));         // V tile it is read behind this barrier
+        __syncthreads();
+    }
+    if (grp == 0) __syncthreads();
+
+    const float l_tot = pair_sum(l_i);
+    const int64_t partial = ((int64_t)(f.partial + split * f.work.blocks + block) * p.nkv + kvh) * kTileRows + wave * 32;     // of the wavefront's first row
+    uint64_t redo = 0;
+    const int filled = (s1 + BN - 1) & -BN;                // tiles are filled up to here: with keys that a row may not see, or with others once more
+    if (__any(row < n_rows && limit < filled)) {
+        uint32_t bad = not_finite(l_tot);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) bad |= (uint32_t)not_finite(o_acc[dt][r]);
+        redo = __ballot(bad != 0 && row < n_rows && limit < filled);
+        redo = (redo | redo >> 32) & 0xffffffffu;
+    }
+    if (row < n_rows && (redo >> l32 & 1) == 0) {
+        if (f.splits == 1) {
+            const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;
+            elem_t* orow = p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)head * p.o_sh + 4 * g;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int a = 0; a < 4; ++a)
+                    *reinterpret_cast<uint2*>(orow + 32 * dt + 8 * a) = make_uint2(pack_elem2(o_acc[dt][4 * a] * inv, o_acc[dt][4 * a + 1] * inv),
+                                                                                   pack_elem2(o_acc[dt][4 * a + 2] * inv, o_acc[dt][4 * a + 3] * inv));
+        } else {
+            float* orow = p.tiles_o + (partial + l32) * D + 4 * g;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int a = 0; a < 4; ++a)
+                    *reinterpret_cast<float4*>(orow + 32 * dt + 8 * a) = make_float4(o_acc[dt][4 * a], o_acc[dt][4 * a + 1], o_acc[dt][4 * a + 2], o_acc[dt][4 * a + 3]);
+            if (g == 0) *reinterpret_cast<float2*>(p.tiles_ml + (partial + l32) * 2) = make_float2(m_i, l_tot);
+        }
+    }
+    for (; redo != 0; redo &= redo - 1) {
+        const int r = __builtin_ctzll(redo), t = __builtin_amdgcn_readlane(token, r), h = __builtin_amdgcn_readlane(head, r), d = 2 * lane;
+        float M, L, O0, O1;
+        own_keys_only<D>(p, table, kvh, p.q + (int64_t)(f.seq.first + t) * p.q_st + (int64_t)h * p.q_sh, s0, __builtin_amdgcn_readlane(limit, r), M, L, O0, O1);
+        if (d >= D) continue;
+        if (f.splits == 1) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            *reinterpret_cast<uint32_t*>(p.o + (int64_t)(f.seq.first + t) * p.o_st + (int64_t)h * p.o_sh + d) = pack_elem2(O0 * inv, O1 * inv);
+        } else {
+            *reinterpret_cast<float2*>(p.tiles_o + (partial + r) * D + d) = make_float2(O0, O1);
+            if (d == 0) *reinterpret_cast<float2*>(p.tiles_ml + (partial + r) * 2) = make_float2(M, L);
+        }
+    }
+}
+
+// ---- merge of the splits ------------------------------------------------------------------------------------------------------------------------------
+// A workgroup looks at partial result blockIdx.x of a KV head; that of a first split stands for its block of rows, of which it merges 16 (blockIdx.z-th),
+// a wavefront one after the other with two features to a lane.  `kind` 0: of paged_rows, 1: of paged_tiles.
+constexpr int kMergeWaves = 4;
+template <int D>
+__global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const PagedParams p, int kind) {
+    const PagedPlan& plan = kind ? p.tiles : p.rows;
+    const float *from_o = kind ? p.tiles_o : p.rows_o, *from_ml = kind ? p.tiles_ml : p.rows_ml;
+    const int partial = blockIdx.x, kvh = blockIdx.y, d = 2 * (threadIdx.x & 63);
+    const Found f = find_work(p, plan, [&](int, int, int first, int n) { return partial >= first && partial < first + n; });
+    const int block = partial - f.partial;
+    if (f.b < 0 || block >= f.work.blocks || f.partial + f.work.blocks * f.splits > (kind ? p.tiles_partials : p.rows_partials)) return;
+    const int64_t step = (int64_t)f.work.blocks * p.nkv * plan.block_rows;
+    for (int in = 16 * blockIdx.z + (threadIdx.x >> 6); in < 16 * ((int)blockIdx.z + 1); in += kMergeWaves) {
+        const int row = block * plan.block_rows + in;
+        if (row >= f.seq.n * p.n_rep) return;
+        const int64_t first = ((int64_t)partial * p.nkv + kvh) * plan.block_rows + in;
+        float M = -INFINITY, L = 0.f, O0 = 0.f, O1 = 0.f;
+        constexpr int kStep = 8;
+        for (int s0 = 0; s0 < f.splits; s0 += kStep) {
+            float2 ml[kStep], o[kStep];
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {              // past the last split: its values again, with no weight below
+                const int64_t at = first + min(s0 + i, f.splits - 1) * step;
+                ml[i] = *reinterpret_cast<const float2*>(from_ml + at * 2);
+                o[i] = d < D ? *reinterpret_cast<const float2*>(from_o + at * D + d) : make_float2(0.f, 0.f);
+                if (s0 + i >= f.splits) o[i] = make_float2(0.f, 0.f);      // (no weight would not do for an infinite output)
+            }
+            float m = M;
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) m = fmaxf(m, ml[i].x);
+            const float a = M == -INFINITY ? 0.f : fast_exp2(M - m);
+            L *= a; O0 *= a; O1 *= a;
+            M = m;
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {
+                const float w = s0 + i >= f.splits || ml[i].x == -INFINITY ? 0.f : fast_exp2(ml[i].x - M);
+                L += w * ml[i].y;
+                O0 += w * o[i].x;
+                O1 += w * o[i].y;
+            }
+        }
+        if (d < D) {
+            const int token = divide(row, p.n_rep, p.rep_m);
+            const float inv = L == 0.f ? 0.f : 1.f / L;
+            *reinterpret_cast<uint32_t*>(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh + d) =
+                pack_elem2(O0 * inv, O1 * inv);
+        }
+    }
+}
+
+template <int D> int launch(const PagedParams& p, int64_t row_slots, int64_t tile_slots, hipStream_t st) {
+    if (row_slots > 0) {
+        paged_rows_kernel<D><<<dim3((unsigned)(row_slots * p.nkv)), dim3(64 * kRowWaves), 0, st>>>(p);
+        if (const int rc = mi_check_launch("paged_rows"); rc != MI_OK) return rc;
+    }
+    if (tile_slots > 0) {
+        paged_tiles_kernel<D><<<dim3((unsigned)(tile_slots * p.nkv)), dim3(512), 0, st>>>(p);
+        if (const int rc = mi_check_launch("paged_tiles"); rc != MI_OK) return rc;
+    }
+    if (p.rows_o != nullptr) paged_merge_kernel<D><<<dim3(p.rows_partials, p.nkv, kRowBlock / 16), dim3(64 * kMergeWaves), 0, st>>>(p, 0);
+    if (p.tiles_o != nullptr) paged_merge_kernel<D><<<dim3(p.tiles_partials, p.nkv, kTileRows / 16), dim3(64 * kMergeWaves), 0, st>>>(p, 1);
+    return mi_check_launch("paged_merge");
+}
+
+// Plans of both kernels for a call of these sizes.
+void make_plans(int64_t tokens, int n_rep, int nkv, PagedPlan& rows, PagedPlan& tiles) {
+    const int cus = mi_compute_units();
+    rows = PagedPlan{0, kRowLimit, kRowBlock, kRowWaves * kRowChunk, 4 * cus, nkv};
+    // Enough blocks for every compute unit: no splits, no merge.
+    const bool many = tokens * n_rep / kTileRows * nkv >= cus;
+    tiles = PagedPlan{kRowLimit, 0x7fffffff, kTileRows, kTileKeys, many ? 0 : cus, nkv};
+}
+
+size_t partial_bytes(const PagedPlan& p, int head_dim) { return (size_t)paged_max_partials(p) * p.nkv * p.block_rows * (size_t)(head_dim + 2) * sizeof(float); }
+
+}  // namespace
+
+#ifndef MI_ELEM_F16
+extern "C" size_t mi_paged_attn_workspace_bytes(int64_t tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
+    if (tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || head_dim <= 0) return 0;
+    PagedPlan rows, tiles;
+    const int n_rep = n_q_heads / n_kv_heads;
+    make_plans(0, n_rep, n_kv_heads, rows, tiles);         // for so many tokens or fewer
+    return partial_bytes(rows, head_dim) + (tokens * n_rep > kRowLimit ? partial_bytes(tiles, head_dim) : 0);
+}
+#endif
+
+int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
+    if (a->total_q < 0 || a->batch < 1 || a->n_pages < 1 || a->max_pages < 1 || a->page_size < 16 || a->page_size % 16 != 0 ||
+        (int64_t)a->max_pages * a->page_size > (1 << 30) || a->max_q_len < 0 || a->total_q > 0x7fffffffLL)
+        return mi_fail(MI_E_SHAPE, "paged_attn: %lld tokens of %d sequences, at most %d each, %d pages of %d keys (a multiple of 16), up to %d a sequence", (long long)a->total_q,
+                       a->batch, a->max_q_len, a->n_pages, a->page_size, a->max_pages);
+    if (a->n_q_heads <= 0 || a->n_kv_heads <= 0 || a->n_q_heads % a->n_kv_heads != 0)
+        return mi_fail(MI_E_SHAPE, "paged_attn: n_q_heads=%d must be a positive multiple of n_kv_heads=%d", a->n_q_heads, a->n_kv_heads);
+    if (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 96 && a->head_dim != 128)
+        return mi_fail(MI_E_SHAPE, "paged_attn: head_dim %d unsupported (32, 64, 96, 128)", a->head_dim);
+    if (!a->q || !a->k_pages || !a->v_pages || !a->o || !a->page_table || !a->cu_seqlens || !a->ctx_len) return mi_fail(MI_E_NULL, "paged_attn: null pointer");
+    if (a->softmax_scale <= 0.f || mi_is_nan(a->softmax_scale)) return mi_fail(MI_E_SHAPE, "paged_attn: softmax_scale must be positive");
+    if (!mi_aligned16(a->q) || !mi_aligned16(a->k_pages) || !mi_aligned16(a->v_pages) || !mi_aligned16(a->o)) return mi_fail(MI_E_ALIGN, "paged_attn: tensors must be 16-byte aligned");
+    for (const int64_t s : {a->q_stride_token, a->q_stride_head, a->o_stride_token, a->o_stride_head, a->page_stride, a->page_stride_token, a->page_stride_head})
+        if (s % 8 != 0) return mi_fail(MI_E_ALIGN, "paged_attn: strides must be multiples of 8 elements");
+    if (a->page_stride_token < 0 || a->page_stride_token > (1 << 26)) return mi_fail(MI_E_SHAPE, "paged_attn: a token stride of %lld elements", (long long)a->page_stride_token);
+    PagedParams p{};
+    p.q = (const elem_t*)a->q; p.kp = (const elem_t*)a->k_pages; p.vp = (const elem_t*)a->v_pages; p.o = (elem_t*)a->o;
+    p.table = a->page_table; p.cu = a->cu_seqlens; p.ctx = a->ctx_len; p.table_stride = a->page_table_stride;
+    p.q_st = a->q_stride_token; p.q_sh = a->q_stride_head; p.o_st = a->o_stride_token; p.o_sh = a->o_stride_head;
+    p.p_sp = a->page_stride; p.p_st = a->page_stride_token; p.p_sh = a->page_stride_head;
+    p.batch = a->batch; p.total = (int)a->total_q; p.n_pages = a->n_pages; p.page = a->page_size; p.max_pages = a->max_pages;
+    p.capacity = a->max_pages * a->page_size; p.nq = a->n_q_heads; p.nkv = a->n_kv_heads; p.n_rep = a->n_q_heads / a->n_kv_heads; p.causal = a->causal != 0;
+    p.page_m = divide_m(p.page); p.rep_m = divide_m(p.n_rep); p.nkv_m = divide_m(p.nkv);
+    p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+    make_plans(p.total, p.n_rep, p.nkv, p.rows, p.tiles);
+    const int64_t longest = a->max_q_len > 0 && a->max_q_len < p.total ? a->max_q_len : p.total;
+    const int64_t row_blocks = paged_max_blocks(p.rows, p.total, p.batch, longest, p.n_rep), tile_blocks = paged_max_blocks(p.tiles, p.total, p.batch, longest, p.n_rep);
+    if (p.nkv > 0xffff) return mi_fail(MI_E_SHAPE, "paged_attn: more than 65535 KV heads");
+    // Sums of blocks x tiles and of rows are kept in 32 bits, and a grid has fewer than 2^31 workgroups.
+    const int64_t tiles_most = (int64_t)p.capacity / kTileKeys + 1;
+    if ((int64_t)p.total * p.n_rep > 0x7fffffffLL || (row_blocks + tile_blocks) * tiles_most > 0x7fffffffLL || (int64_t)p.total * p.nkv > 0x7fffffffLL ||
+        (row_blocks + tile_blocks + 8LL * mi_compute_units()) * p.nkv > 0x7fffffffLL)
+        return mi_fail(MI_E_SHAPE, "paged_attn: %lld tokens of %d heads over up to %d keys are too many for one call", (long long)a->total_q, a->n_q_heads, p.capacity);
+    const size_t rows_bytes = partial_bytes(p.rows, a->head_dim), need = mi_paged_attn_workspace_bytes(p.total, p.nq, p.nkv, a->head_dim);
+    if (!a->workspace || a->workspace_bytes < need || !mi_aligned16(a->workspace))
+        return mi_fail(MI_E_WORKSPACE, "paged_attn: workspace needs %zu bytes (16-byte aligned), got %zu", need, a->workspace_bytes);
+    // A sequence of up to a tile of keys has one split, whatever the plan.
+    if (p.capacity <= p.rows.tile_keys || row_blocks == 0) p.rows.target = 0;
+    if (p.capacity <= p.tiles.tile_keys || tile_blocks == 0) p.tiles.target = 0;
+    const auto place = [&](const PagedPlan& plan, char* at, float*& o, float*& ml) {
+        if (plan.target == 0) return;
+        o = (float*)at;
+        ml = o + (size_t)paged_max_partials(plan) * plan.nkv * plan.block_rows * a->head_dim;
+    };
+    p.rows_partials = (int)paged_max_partials(p.rows);
+    p.tiles_partials = (int)paged_max_partials(p.tiles);
+    place(p.rows, (char*)a->workspace, p.rows_o, p.rows_ml);
+    place(p.tiles, (char*)a->workspace + rows_bytes, p.tiles_o, p.tiles_ml);
+    const int64_t row_slots = paged_max_slots(p.rows, row_blocks), tile_slots = paged_max_slots(p.tiles, tile_blocks);
+    const hipStream_t st = (hipStream_t)a->stream;
+    switch (a->head_dim) {
+        case 32: return launch<32>(p, row_slots, tile_slots, st);
+        case 64: return launch<64>(p, row_slots, tile_slots, st);
+        case 96: return launch<96>(p, row_slots, tile_slots, st);
+        default: return launch<128>(p, row_slots, tile_slots, st);
+    }
+}

@@ -22,6 +22,8 @@ void mi_set_error(const char* fmt, ...);
 int mi_fail(int status, const char* fmt, ...);
 int mi_check_launch(const char* what);
 
+// (comparisons with NaN are compiled away, on the host too)
+static inline bool mi_is_nan(float x) { return (__builtin_bit_cast(uint32_t, x) & 0x7fffffffu) > 0x7f800000u; }
 static inline bool mi_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // ---- element type traits: 8 x 16-bit or 4 x fp32 per 128-bit access --------------------------

@@ -426,6 +426,198 @@ struct RotaryTwo : Function<RotaryTwo> {
     static variable_list backward(AutogradContext* ctx, variable_list g) { return gradients(ctx, g); }
 };
 
+// ---- rows of one head: norms with the rotary embedding, and the append to a paged cache --------------------------------
+// Norm weights and rotary of q and k; undefined tensors where there are none.
+struct HeadRows {
+    Tensor q_weight, k_weight, q_bias, k_bias, cos, sin, ids;
+    double eps;
+    bool layer_norm, interleaved;
+};
+
+void check_head_rows(const Tensor& x, const Tensor& weight, const Tensor& bias) {
+    need_gpu(x);
+    TORCH_CHECK(x.dim() == 3 && (x.stride(2) == 1 || x.size(2) <= 1), "head rows: q, k and v must be [tokens, heads, head_dim] with contiguous features");
+    for (const Tensor& w : {weight, bias})
+        TORCH_CHECK(!w.defined() || (w.dim() == 1 && w.size(0) == x.size(2) && w.scalar_type() == x.scalar_type() && w.device() == x.device()),
+                    "head rows: norm weights and biases are [head_dim] tensors of the rows' type and device");
+}
+
+// Arguments but for the outputs and the stream; q may be undefined.  The tensors that `o` holds have to be contiguous.
+mi_norm_rotary_args head_rows_args(const Tensor& q, const Tensor& k, const HeadRows& o) {
+    mi_norm_rotary_args a{};
+    const Tensor& x = k.defined() ? k : q;
+    if (q.defined()) {
+        check_head_rows(q, o.q_weight, o.q_bias);
+        a.q = ptr(q); a.q_weight = ptr(o.q_weight); a.q_bias = ptr(o.q_bias);
+        a.q_stride_token = q.stride(0); a.q_stride_head = q.stride(1); a.n_q_heads = (int32_t)q.size(1);
+    }
+    if (k.defined()) {
+        check_head_rows(k, o.k_weight, o.k_bias);
+        a.k = ptr(k); a.k_weight = ptr(o.k_weight); a.k_bias = ptr(o.k_bias);
+        a.k_stride_token = k.stride(0); a.k_stride_head = k.stride(1); a.n_kv_heads = (int32_t)k.size(1);
+    }
+    TORCH_CHECK(!q.defined() || !k.defined() || (q.size(0) == k.size(0) && q.size(2) == k.size(2) && q.scalar_type() == k.scalar_type() && q.device() == k.device()),
+                "head rows: q and k do not match");
+    a.n_tokens = x.size(0); a.head_dim = (int32_t)x.size(2); a.dtype = code_of(x); a.layer_norm = o.layer_norm; a.eps = (float)o.eps;
+    if (o.cos.defined()) {
+        TORCH_CHECK(o.sin.defined() && o.ids.defined() && o.cos.dim() == 2 && o.cos.sizes() == o.sin.sizes() && o.cos.scalar_type() == o.sin.scalar_type() &&
+                        o.cos.device() == x.device() && o.sin.device() == x.device() && o.ids.device() == x.device() && o.ids.scalar_type() == at::kLong &&
+                        o.ids.numel() == x.size(0),
+                    "head rows: rotary takes two tables [rows, features] and one int64 position id per token, on the rows' device");
+        TORCH_CHECK(!o.interleaved || (o.cos.scalar_type() == at::kFloat && o.cos.size(1) * 2 == x.size(2)), "head rows: interleaved pairs take float32 tables [rows, head_dim / 2]");
+        a.rotary_cos = ptr(o.cos); a.rotary_sin = ptr(o.sin); a.position_ids = static_cast<const int64_t*>(ptr(o.ids));
+        a.table_rows = o.cos.size(0); a.rot_dim = (int32_t)(o.interleaved ? x.size(2) : o.cos.size(1)); a.rotary_interleaved = o.interleaved;
+        a.table_dtype = code_of(o.cos);
+    }
+    return a;
+}
+
+Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+
+struct NormRotary : Function<NormRotary> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& q_weight, const Tensor& k_weight, const OptTensor& q_bias,
+                                 const OptTensor& k_bias, const OptTensor& cos, const OptTensor& sin, const OptTensor& ids, double eps, bool layer_norm,
+                                 bool interleaved) {
+        need_gpu(q);
+        const HeadRows o{dense(q_weight), dense(k_weight), dense(opt(q_bias)), dense(opt(k_bias)), dense(opt(cos)), dense(opt(sin)), dense(opt(ids)), eps, layer_norm,
+                         interleaved};
+        Launch l(q);
+        mi_norm_rotary_args a = head_rows_args(q, k, o);
+        const Tensor q_out = at::empty(q.sizes(), q.options()), k_out = at::empty(k.sizes(), k.options());
+        a.q_out = ptr(q_out); a.q_out_stride_token = q_out.stride(0); a.q_out_stride_head = q_out.stride(1);
+        a.k_out = ptr(k_out); a.k_out_stride_token = k_out.stride(0); a.k_out_stride_head = k_out.stride(1);
+        a.stream = l.stream;
+        check(mi_norm_rotary_fwd(&a), "mi_norm_rotary_fwd");
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({q, k, q_weight, k_weight, o.cos, o.sin, o.ids});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["layer_norm"] = layer_norm;
+        ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["q_bias"] = o.q_bias.defined();
+        ctx->saved_data["k_bias"] = o.k_bias.defined();
+        return {q_out, k_out};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list g) {
+        const variable_list saved = ctx->get_saved_variables();
+        variable_list d(12);
+        if (!g[0].defined() && !g[1].defined()) return d;
+        // a tensor that does not reach the loss is left out
+        const auto rows = [](const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.contiguous(); };
+        const Tensor q = g[0].defined() ? rows(saved[0]) : Tensor(), k = g[1].defined() ? rows(saved[1]) : Tensor();
+        const Tensor dq_out = g[0].defined() ? rows(g[0]) : Tensor(), dk_out = g[1].defined() ? rows(g[1]) : Tensor();
+        const Tensor& x = q.defined() ? q : k;
+        Launch l(x);
+        const HeadRows o{dense(saved[2]), dense(saved[3]), Tensor(), Tensor(), dense(saved[4]), dense(saved[5]), dense(saved[6]), ctx->saved_data["eps"].toDouble(),
+                         ctx->saved_data["layer_norm"].toBool(), ctx->saved_data["interleaved"].toBool()};
+        mi_norm_rotary_bwd_args b{};
+        b.fwd = head_rows_args(q, k, o);
+        b.fwd.stream = l.stream;
+        const bool none = x.size(0) == 0;                  // no rows: the weights' gradients are sums over nothing
+        const auto like = [&](const Tensor& t) { return none ? at::zeros_like(t) : at::empty_like(t); };
+        if (q.defined()) {
+            d[0] = at::empty(q.sizes(), q.options());
+            d[2] = like(o.q_weight);
+            if (ctx->saved_data["q_bias"].toBool()) d[4] = like(o.q_weight);
+            b.d_q_out = ptr(dq_out); b.d_q_out_stride_token = dq_out.stride(0); b.d_q_out_stride_head = dq_out.stride(1);
+            b.dq = ptr(d[0]); b.dq_stride_token = d[0].stride(0); b.dq_stride_head = d[0].stride(1);
+            b.dq_weight = ptr(d[2]); b.dq_bias = ptr(d[4]);
+        }
+        if (k.defined()) {
+            d[1] = at::empty(k.sizes(), k.options());
+            d[3] = like(o.k_weight);
+            if (ctx->saved_data["k_bias"].toBool()) d[5] = like(o.k_weight);
+            b.d_k_out = ptr(dk_out); b.d_k_out_stride_token = dk_out.stride(0); b.d_k_out_stride_head = dk_out.stride(1);
+            b.dk = ptr(d[1]); b.dk_stride_token = d[1].stride(0); b.dk_stride_head = d[1].stride(1);
+            b.dk_weight = ptr(d[3]); b.dk_bias = ptr(d[5]);
+        }
+        if (none) return d;
+        b.workspace_bytes = mi_norm_rotary_bwd_workspace_bytes(b.fwd.head_dim);
+        const Tensor ws = float_buffer(b.workspace_bytes, x);
+        b.workspace = ptr(ws);
+        check(mi_norm_rotary_bwd(&b), "mi_norm_rotary_bwd");
+        return d;
+    }
+};
+
+std::tuple<Tensor, Tensor> op_norm_rotary(const Tensor& q, const Tensor& k, const Tensor& q_weight, const Tensor& k_weight, const OptTensor& q_bias,
+                                          const OptTensor& k_bias, const OptTensor& cos, const OptTensor& sin, const OptTensor& ids, double eps, bool layer_norm,
+                                          bool interleaved) {
+    const auto out = NormRotary::apply(q, k, q_weight, k_weight, q_bias, k_bias, cos, sin, ids, eps, layer_norm, interleaved);
+    return {out[0], out[1]};
+}
+
+// What the kernels read of a paged cache; the callers have checked it.
+struct Pages {
+    int32_t batch, n_pages, page_size, max_pages;
+};
+Pages check_pages(const Tensor& like, int64_t n_kv_heads, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu, const Tensor& ctx_len) {
+    for (const Tensor* t : {&k_pages, &v_pages, &table, &cu, &ctx_len}) TORCH_CHECK(t->device() == like.device(), "paged cache: tensors on several devices");
+    TORCH_CHECK(k_pages.dim() == 4 && k_pages.sizes() == v_pages.sizes() && k_pages.strides() == v_pages.strides() && k_pages.stride(3) == 1 &&
+                    k_pages.scalar_type() == like.scalar_type() && v_pages.scalar_type() == like.scalar_type() && k_pages.size(2) == n_kv_heads &&
+                    k_pages.size(3) == like.size(2),
+                "paged cache: k_pages and v_pages are [pages, page_size, n_kv, head_dim] tensors of the rows' type with one layout and contiguous features");
+    TORCH_CHECK(table.dim() == 2 && table.scalar_type() == at::kInt && (table.stride(1) == 1 || table.size(1) <= 1) && cu.dim() == 1 && cu.scalar_type() == at::kInt &&
+                    cu.is_contiguous() && ctx_len.dim() == 1 && ctx_len.scalar_type() == at::kInt && ctx_len.is_contiguous() && table.size(0) == ctx_len.size(0) &&
+                    cu.size(0) == ctx_len.size(0) + 1,
+                "paged cache: int32 page_table [batch, max_pages], cu_seqlens [batch + 1] and ctx_len [batch]");
+    for (const int64_t n : {table.size(0), table.size(1), k_pages.size(0), k_pages.size(1)}) TORCH_CHECK(n <= INT32_MAX, "paged cache: a size over 2^31");
+    return {(int32_t)table.size(0), (int32_t)k_pages.size(0), (int32_t)k_pages.size(1), (int32_t)table.size(1)};
+}
+
+OptTensor op_paged_append(const OptTensor& q_, const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu,
+                          const Tensor& ctx_len, const OptTensor& q_weight, const OptTensor& k_weight, const OptTensor& q_bias, const OptTensor& k_bias,
+                          const OptTensor& cos, const OptTensor& sin, const OptTensor& ids, double eps, bool layer_norm, bool interleaved) {
+    need_gpu(k);
+    const Tensor q = opt(q_);
+    const HeadRows o{dense(opt(q_weight)), dense(opt(k_weight)), dense(opt(q_bias)), dense(opt(k_bias)), dense(opt(cos)), dense(opt(sin)), dense(opt(ids)), eps, layer_norm,
+                     interleaved};
+    Launch l(k);
+    mi_paged_append_args a{};
+    a.rows = head_rows_args(q, k, o);
+    check_head_rows(v, Tensor(), Tensor());
+    TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type() && v.device() == k.device(), "paged_append: k and v do not match");
+    const Pages pages = check_pages(k, k.size(1), k_pages, v_pages, table, cu, ctx_len);
+    a.v = ptr(v); a.v_stride_token = v.stride(0); a.v_stride_head = v.stride(1);
+    a.k_pages = ptr(k_pages); a.v_pages = ptr(v_pages);
+    a.page_stride = k_pages.stride(0); a.page_stride_token = k_pages.stride(1); a.page_stride_head = k_pages.stride(2);
+    a.page_table = static_cast<const int32_t*>(ptr(table)); a.page_table_stride = table.stride(0);
+    a.cu_seqlens = static_cast<const int32_t*>(ptr(cu)); a.ctx_len = static_cast<const int32_t*>(ptr(ctx_len));
+    a.batch = pages.batch; a.n_pages = pages.n_pages; a.page_size = pages.page_size; a.max_pages = pages.max_pages;
+    Tensor q_out;
+    if (q.defined()) {
+        q_out = at::empty(q.sizes(), q.options());
+        a.rows.q_out = ptr(q_out); a.rows.q_out_stride_token = q_out.stride(0); a.rows.q_out_stride_head = q_out.stride(1);
+    }
+    a.rows.stream = l.stream;
+    check(mi_paged_append(&a), "mi_paged_append");
+    return q.defined() ? OptTensor(q_out) : std::nullopt;
+}
+
+void op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu, const Tensor& ctx_len, bool causal,
+                        double scale, int64_t max_q_len, const OptTensor& workspace_, const Tensor& out) {
+    check_head_rows(q, Tensor(), Tensor());
+    TORCH_CHECK(out.is_cuda() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device() && out.stride(2) == 1,
+                "paged_attention: out does not match q");
+    Launch l(q);
+    TORCH_CHECK(k_pages.dim() == 4, "paged cache: k_pages and v_pages are [pages, page_size, n_kv, head_dim] tensors");
+    const Pages pages = check_pages(q, k_pages.size(2), k_pages, v_pages, table, cu, ctx_len);
+    mi_paged_attn_args a{};
+    a.q = ptr(q); a.k_pages = ptr(k_pages); a.v_pages = ptr(v_pages); a.o = ptr(out);
+    a.page_table = static_cast<const int32_t*>(ptr(table)); a.page_table_stride = table.stride(0);
+    a.cu_seqlens = static_cast<const int32_t*>(ptr(cu)); a.ctx_len = static_cast<const int32_t*>(ptr(ctx_len));
+    a.total_q = q.size(0); a.q_stride_token = q.stride(0); a.q_stride_head = q.stride(1); a.o_stride_token = out.stride(0); a.o_stride_head = out.stride(1);
+    a.page_stride = k_pages.stride(0); a.page_stride_token = k_pages.stride(1); a.page_stride_head = k_pages.stride(2);
+    a.batch = pages.batch; a.n_pages = pages.n_pages; a.page_size = pages.page_size; a.max_pages = pages.max_pages;
+    a.n_q_heads = (int32_t)q.size(1); a.n_kv_heads = (int32_t)k_pages.size(2); a.head_dim = (int32_t)q.size(2); a.dtype = code_of(q);
+    a.causal = causal; a.max_q_len = (int32_t)std::min<int64_t>(max_q_len, INT32_MAX); a.softmax_scale = (float)scale;
+    Tensor workspace = opt(workspace_);
+    if (!workspace.defined()) workspace = float_buffer(mi_paged_attn_workspace_bytes(a.total_q, a.n_q_heads, a.n_kv_heads, a.head_dim), q);
+    TORCH_CHECK(workspace.device() == q.device() && workspace.is_contiguous(), "paged_attention: the workspace is a contiguous tensor on the device of q");
+    a.workspace = ptr(workspace); a.workspace_bytes = (size_t)workspace.numel() * workspace.element_size();
+    a.stream = l.stream;
+    check(mi_paged_attn(&a), "mi_paged_attn");
+}
+
 // ---- linear projections ------------------------------------------------------------------------------------------------
 // Whether a product of m x n x k multiply-adds goes to mi_gemm.  A library call costs the host 18 us whatever its size (the
 // heuristic lookup), mi_gemm 3; on the device the two meet near 3 GFLOP (16-bit: 1024 x 1024 x 1024, forward + both
@@ -1759,6 +1951,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     def("rotary", [](const Tensor& x, const Tensor& cos, const Tensor& sin, const OptTensor& ids, int64_t seq_len, bool interleaved) {
         return Rotary::apply(x, cos, sin, ids, seq_len, interleaved);
     });
+    def("norm_rotary", &op_norm_rotary);
+    def("paged_append", &op_paged_append);
+    def("paged_attention", &op_paged_attention);
     def("linear", &op_linear);
     def("projections", &op_projections);
     def("attention_forward", &op_attention_forward);

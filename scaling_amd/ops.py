@@ -22,6 +22,7 @@ __all__ = [
     "rms_norm", "swiglu", "rotary_embedding", "rotary_embedding_complex", "attention", "attention_forward", "attention_backward",
     "decode_attention", "rms_norm_forward", "rms_norm_backward", "swiglu_forward", "swiglu_backward",
     "cross_entropy", "cross_entropy_forward", "linear_cross_entropy", "weighted_cross_entropy", "add_rms_norm",
+    "norm_rotary", "paged_append", "paged_attention", "paged_workspace",
 ]
 
 
@@ -198,6 +199,82 @@ def rotary_embedding_complex(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tens
     _check_rotary(x, cos, sin, position_ids)
     assert cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.shape[1] * 2 == x.shape[2]
     return _lib.host().rotary(x, cos, sin, position_ids, int(seq_len_for_null_ids), True)
+
+
+# ------------------------------------------------------------------------------------------------
+# rows of one head: norms with the rotary embedding, and the append to a paged cache
+# ------------------------------------------------------------------------------------------------
+def _check_head_norm(q_weight, k_weight, q_bias, k_bias, layer_norm):
+    if (q_bias is not None or k_bias is not None) and not layer_norm:
+        raise ValueError("RMSNorm has no bias")
+
+
+def norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float = 1e-5,
+                q_bias: Optional[torch.Tensor] = None, k_bias: Optional[torch.Tensor] = None, layer_norm: bool = False,
+                rotary: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None, interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Norm over each head of q [tokens, n_q, d] and k [tokens, n_kv, d] (RMSNorm, or LayerNorm with optional biases; weights [d]), followed by the
+    rotary embedding, in one launch; differentiable in q, k, weights and biases.  The arithmetic is float32 with one rounding at the end (`rms_norm` or
+    `layer_norm` followed by `rotary_embedding` rounds the normed rows too).
+
+    rotary = (cos, sin, position_ids): tables [rows, r] in the tensors' type or float32 rotate the first r features in halves; with `interleaved`
+    float32 tables [rows, d / 2] rotate the whole head in neighbouring pairs.  position_ids int64 [tokens]; ids outside the tables are clamped.  None:
+    norms alone.  q and k may be views with contiguous features (slices of one projection); any d up to 256, rows of whole 16-byte vectors fastest."""
+    _need_cuda(q, k, q_weight, k_weight, q_bias, k_bias)
+    _check_head_norm(q_weight, k_weight, q_bias, k_bias, layer_norm)
+    cos, sin, ids = rotary if rotary is not None else (None, None, None)
+    return _lib.host().norm_rotary(q, k, q_weight, k_weight, q_bias, k_bias, cos, sin, ids, float(eps), bool(layer_norm), bool(interleaved))
+
+
+def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                 ctx_len: torch.Tensor, q: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                 eps: float = 1e-5, q_bias: Optional[torch.Tensor] = None, k_bias: Optional[torch.Tensor] = None, layer_norm: bool = False,
+                 rotary: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None, interleaved: bool = False) -> Optional[torch.Tensor]:
+    """Stores new keys and values (k, v [tokens, n_kv, d], bfloat16 or float16) into the pages of a cache, in one launch (inference; no autograd).
+
+    k_pages, v_pages [n_pages, page_size, n_kv, d] (any strides with contiguous features; page_size a multiple of 16); page_table int32
+    [batch, max_pages]: the pages of each sequence in the order of its positions; cu_seqlens int32 [batch + 1]: sequence b brings tokens
+    cu_seqlens[b] .. cu_seqlens[b + 1] (none is fine); ctx_len int32 [batch]: its keys INCLUDING these.  Token i of n goes to position ctx_len - n + i.  Tokens
+    behind the last sequence, and positions or pages outside the table or the cache, are not stored.  No two tokens may go to one slot.
+
+    With `rotary` and / or weights, k is normed and rotated on its way as by `norm_rotary`, and with `q` [tokens, n_q, d] the same of q is returned."""
+    _need_cuda(k, v, k_pages, v_pages, page_table, cu_seqlens, ctx_len, q, q_weight, k_weight, q_bias, k_bias)
+    _check_head_norm(q_weight, k_weight, q_bias, k_bias, layer_norm)
+    if (k_bias is not None and k_weight is None) or (q_bias is not None and q_weight is None) or (q is None and q_weight is not None):
+        raise ValueError("paged_append: a bias goes with a weight, q_weight with q")
+    if q is not None and (q_weight is None) != (k_weight is None):
+        raise ValueError("paged_append: q_weight and k_weight go together")
+    cos, sin, ids = rotary if rotary is not None else (None, None, None)
+    with torch.no_grad():
+        return _lib.host().paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, ctx_len, q_weight, k_weight, q_bias, k_bias, cos, sin, ids,
+                                        float(eps), bool(layer_norm), bool(interleaved))
+
+
+def paged_workspace(batch: int, tokens: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """Scratch of `paged_attention` for calls of up to `batch` sequences and `tokens` new tokens that do not overlap (calls on different streams, and graphs
+    that may be replayed at the same time, need one each)."""
+    nbytes = _lib.load().mi_paged_attn_workspace_bytes(tokens, n_q_heads, n_kv_heads, head_dim)
+    return torch.empty(nbytes // 4, dtype=torch.float32, device=device)
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                    ctx_len: torch.Tensor, causal: bool = True, softmax_scale: Optional[float] = None, max_q_len: Optional[int] = None,
+                    workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of new tokens over a paged cache that holds their keys and values already (`paged_append`, which describes the cache); any number of new
+    tokens per sequence, one (a decode step) and none included (inference; no autograd).
+
+    q [tokens, n_q, d] (bfloat16 or float16; d 32, 64, 96 or 128), query head h reading KV head h // (n_q / n_kv).  Token i of the n of a sequence sees keys
+    u < ctx_len and, with `causal`, u <= ctx_len - n + i; without any its row is zeros.  Rows behind the last sequence are left as they are in `out` (of a new
+    tensor: undefined).  max_q_len: an upper bound of the tokens of a sequence, where the caller knows one (1: no launches for chunks); longer ones
+    may be left out.  Lengths beyond the page table count its room.  workspace: see `paged_workspace`; without one it is allocated per call."""
+    _need_cuda(q, k_pages, v_pages, page_table, cu_seqlens, ctx_len, workspace, out)
+    if max_q_len is not None and max_q_len < 1 and q.shape[0] > 0:
+        raise ValueError("paged_attention: max_q_len must be positive")
+    with torch.no_grad():
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _lib.host().paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, ctx_len, bool(causal),
+                                    1.0 / math.sqrt(q.shape[2]) if softmax_scale is None else float(softmax_scale), max_q_len or 0, workspace, out)
+    return out
 
 
 # ------------------------------------------------------------------------------------------------

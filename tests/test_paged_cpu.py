@@ -1,0 +1,216 @@
+"""CPU checks of the paged cache: how work is cut (the header compiled for the host), and refusals of the C entry points."""
+
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+from scaling_amd import _lib
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+PROGRAM = r"""
+#include "%s/scaling_amd/csrc/paged_plan.h"
+#include <stdio.h>
+#include <stdlib.h>
+#include <vector>
+static unsigned long long state = 88172645463325252ull;
+static unsigned rnd() { state ^= state << 13; state ^= state >> 7; state ^= state << 17; return (unsigned)(state >> 11); }
+static int fail(const char* what, int i) { printf("case %%d: %%s\n", i, what); return 1; }
+int main() {
+    for (int c = 0; c < 4000; ++c) {
+        const int batch = 1 + rnd() %% (c %% 5 == 0 ? 300 : 9), n_rep = 1 + rnd() %% 40, nkv = 1 + rnd() %% 9, pages = 1 + rnd() %% 70, page = 16 * (1 + rnd() %% 9);
+        const int capacity = pages * page;
+        const bool good = c %% 3 != 0, causal = rnd() & 1;
+        std::vector<int> cu(batch + 1), ctx(batch);
+        int total = 0;
+        for (int b = 0; b < batch; ++b) {
+            const int n = rnd() %% 4 == 0 ? rnd() %% 700 : rnd() %% 3;
+            cu[b] = total;
+            total += n;
+            ctx[b] = (int)(rnd() %% (capacity + 40));
+            if (!good) { if (rnd() %% 3 == 0) cu[b] = (int)(rnd() - 2147483648u); if (rnd() %% 3 == 0) ctx[b] = (int)(rnd() - 2147483648u); }
+        }
+        cu[batch] = good ? total : (int)(rnd() - 2147483648u);
+        int longest = 0;
+        const int tile_keys[2] = {128, 64}, block[2] = {16, 256};
+        std::vector<int> taken(good ? total : 0, 0);
+        for (int b = 0; b < batch; ++b) { const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity); if (s.n > longest) longest = s.n; }
+        for (int k = 0; k < 2; ++k) {
+            const PagedPlan p = {k == 0 ? 0 : 16, k == 0 ? 16 : 0x7fffffff, block[k], tile_keys[k], rnd() %% 4 == 0 ? 0 : 1 << rnd() %% 11, nkv};
+            int64_t units = 0, slots = 0, partials = 0, blocks = 0;
+            for (int b = 0; b < batch; ++b) {
+                const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity);
+                if (s.first < 0 || s.n < 0 || s.first + s.n > total || s.len < 0 || s.len > capacity) return fail("a sequence outside the tokens or the table", c);
+                const PagedWork w = paged_work(p, s, n_rep);
+                units += (int64_t)w.blocks * w.tiles;
+            }
+            const int S = paged_split_tiles(p, units);
+            if (S < 1) return fail("no tiles to a split", c);
+            for (int b = 0; b < batch; ++b) {
+                const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity);
+                const PagedWork w = paged_work(p, s, n_rep);
+                const int splits = paged_splits(w, S);
+                if (splits < 1) return fail("no split", c);
+                blocks += w.blocks;
+                slots += (int64_t)w.blocks * splits;
+                if (splits > 1) partials += (int64_t)w.blocks * splits;
+                if (w.blocks > 0 && good) for (int i = 0; i < s.n; ++i) ++taken[s.first + i];
+                int at = 0;
+                for (int i = 0; i < splits; ++i) {         // splits cover the keys once, in order, in whole tiles
+                    int k0, k1;
+                    paged_split_keys(p, s, w, splits, i, k0, k1);
+                    if (k0 != at || k1 < k0 || k1 > s.len || (k0 %% p.tile_keys != 0 && k0 != s.len) || (k1 - k0 + p.tile_keys - 1) / p.tile_keys > S) return fail("keys of a split", c);
+                    at = k1;
+                }
+                if (at != s.len) return fail("keys left out", c);
+                for (int i = 0; i < s.n; i += 1 + s.n / 5) {
+                    const int64_t want = causal ? (int64_t)s.ctx - s.n + i + 1 : s.len;
+                    const int got = paged_limit(s, i, causal);
+                    if (got != (want < 0 ? 0 : want > s.len ? s.len : (int)want)) return fail("limit of a row", c);
+                }
+            }
+            if (good) {
+                const int64_t most = paged_max_blocks(p, total, batch, longest, n_rep);
+                if (blocks > most || (blocks == 0) < (most == 0)) return fail("more blocks than the bound", c);
+                if (slots > paged_max_slots(p, most)) return fail("more workgroups than the bound", c);
+                if (partials > paged_max_partials(p)) return fail("more partial results than the bound", c);
+            }
+        }
+        for (int t : taken) if (t != 1) return fail("a token that is not exactly one kernel's", c);
+    }
+    printf("ok\n");
+    return 0;
+}
+"""
+
+
+def test_work_is_cut_within_its_bounds(tmp_path):
+    src = tmp_path / "plan.cpp"
+    src.write_text(PROGRAM % ROOT)
+    exe = tmp_path / "plan"
+    subprocess.run(["g++", "-O1", "-std=c++17", "-Wall", "-fsanitize=undefined", "-fno-sanitize-recover=all", str(src), "-o", str(exe)], check=True)
+    done = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert done.returncode == 0 and done.stdout == "ok\n", done.stdout + done.stderr
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(_lib.LIB_PATH):
+        import __graft_entry__
+        __graft_entry__.build()
+    return _lib.load()
+
+
+@pytest.fixture()
+def base():
+    buf = (ctypes.c_char * 4096)()
+    at = ctypes.addressof(buf)
+    yield at + (-at) % 16
+    del buf
+
+
+def test_struct_layouts(tmp_path):
+    header = os.path.join(ROOT, "include", "mi355_layer.h")
+    names = {"mi_norm_rotary_args": (_lib.MiNormRotaryArgs, "stream"), "mi_norm_rotary_bwd_args": (_lib.MiNormRotaryBwdArgs, "workspace"),
+             "mi_paged_append_args": (_lib.MiPagedAppendArgs, "max_pages"), "mi_paged_attn_args": (_lib.MiPagedAttnArgs, "stream")}
+    lines = "".join(f'printf("%zu %zu\\n",sizeof({n}),offsetof({n},{f}));' for n, (_, f) in names.items())
+    src = tmp_path / "sz.c"
+    src.write_text(f'#include "{header}"\n#include <stdio.h>\n#include <stddef.h>\nint main(){{{lines}return 0;}}\n')
+    subprocess.run(["gcc", str(src), "-o", str(tmp_path / "sz")], check=True)
+    out = subprocess.run([str(tmp_path / "sz")], check=True, capture_output=True, text=True).stdout.split()
+    assert [int(v) for v in out] == [v for s, f in names.values() for v in (ctypes.sizeof(s), getattr(s, f).offset)]
+
+
+def _rows(base):
+    a = _lib.MiNormRotaryArgs()
+    a.q = a.k = a.q_out = a.k_out = a.q_weight = a.k_weight = a.rotary_cos = a.rotary_sin = a.position_ids = base
+    a.n_tokens, a.table_rows, a.n_q_heads, a.n_kv_heads, a.head_dim, a.rot_dim, a.eps = 4, 4, 2, 2, 64, 64, 1e-5
+    a.q_stride_token = a.k_stride_token = a.q_out_stride_token = a.k_out_stride_token = 128
+    a.q_stride_head = a.k_stride_head = a.q_out_stride_head = a.k_out_stride_head = 64
+    return a
+
+
+def _set(a, **fields):
+    for name, value in fields.items():
+        setattr(a, name, value)
+    return a
+
+
+ROWS_REFUSED = [
+    (dict(n_tokens=-1), -3), (dict(n_q_heads=-1), -3), (dict(n_q_heads=0, n_kv_heads=0), -3), (dict(head_dim=0), -3), (dict(head_dim=257), -3),
+    (dict(n_tokens=2 ** 30), -3), (dict(n_q_heads=70000), -3), (dict(dtype=7), -2), (dict(q=None), -1), (dict(k=None), -1), (dict(eps=-1.0), -3),
+    (dict(eps=float("nan")), -3), (dict(rotary_sin=None), -1), (dict(rotary_cos=None), -1), (dict(position_ids=None), -1), (dict(table_rows=0), -3),
+    (dict(rot_dim=63), -3), (dict(rot_dim=66), -3), (dict(rot_dim=0), -3), (dict(rotary_interleaved=1), -3), (dict(rotary_interleaved=1, table_dtype=2, rot_dim=32), -3),
+    (dict(table_dtype=1), -2),
+]
+
+
+def test_norm_rotary_refusals(lib, base):
+    assert lib.mi_norm_rotary_fwd(None) == -1 and lib.mi_norm_rotary_bwd(None) == -1
+    for fields, status in ROWS_REFUSED + [(dict(q_out=None), -1), (dict(k_out=None), -1), (dict(q_weight=None), -1), (dict(k_weight=None), -1)]:
+        assert lib.mi_norm_rotary_fwd(ctypes.byref(_set(_rows(base), **fields))) == status, fields
+    assert lib.mi_norm_rotary_fwd(ctypes.byref(_set(_rows(base), n_tokens=0, q=None))) == 0            # nothing to do
+    b = _lib.MiNormRotaryBwdArgs()
+    b.d_q_out = b.d_k_out = b.dq = b.dk = b.dq_weight = b.dk_weight = b.workspace = base
+    b.workspace_bytes = lib.mi_norm_rotary_bwd_workspace_bytes(64)
+    assert b.workspace_bytes >= 64 * 8 and lib.mi_norm_rotary_bwd_workspace_bytes(0) == 0
+    for fields, status in ROWS_REFUSED + [(dict(q_weight=None), -1), (dict(n_tokens=0), -3)]:
+        b.fwd = _set(_rows(base), **fields)
+        assert lib.mi_norm_rotary_bwd(ctypes.byref(b)) == status, fields
+    b.fwd = _rows(base)
+    for field in ("d_q_out", "d_k_out", "dq", "dk"):
+        setattr(b, field, None)
+        assert lib.mi_norm_rotary_bwd(ctypes.byref(b)) == -1, field
+        setattr(b, field, base)
+    for fields in (dict(workspace=None), dict(workspace=base + 4), dict(workspace_bytes=16)):
+        kept = {n: getattr(b, n) for n in fields}
+        assert lib.mi_norm_rotary_bwd(ctypes.byref(_set(b, **fields))) == -5, fields
+        _set(b, **kept)
+
+
+def test_paged_append_refusals(lib, base):
+    assert lib.mi_paged_append(None) == -1
+
+    def args(**fields):
+        a = _lib.MiPagedAppendArgs()
+        a.rows = _set(_rows(base), **{n: v for n, v in fields.items() if hasattr(_lib.MiNormRotaryArgs, n)})
+        a.v = a.k_pages = a.v_pages = a.page_table = a.cu_seqlens = a.ctx_len = base
+        a.v_stride_token, a.v_stride_head, a.page_stride, a.page_stride_token, a.page_stride_head = 128, 64, 16 * 128, 128, 64
+        a.page_table_stride = a.max_pages = 3
+        a.batch, a.n_pages, a.page_size = 1, 5, 16
+        return _set(a, **{n: v for n, v in fields.items() if hasattr(_lib.MiPagedAppendArgs, n)})
+    for fields, status in ROWS_REFUSED + [
+            (dict(dtype=2, table_dtype=2), -2), (dict(n_kv_heads=0), -3), (dict(batch=0), -3), (dict(n_pages=0), -3), (dict(max_pages=0), -3), (dict(page_size=8), -3), (dict(page_size=24), -3),
+            (dict(max_pages=2 ** 28), -3), (dict(v=None), -1), (dict(k_pages=None), -1), (dict(v_pages=None), -1), (dict(page_table=None), -1), (dict(cu_seqlens=None), -1),
+            (dict(ctx_len=None), -1), (dict(q_out=None), -1), (dict(k_pages=base + 2), -4), (dict(page_stride=4), -4), (dict(page_stride_token=4), -4), (dict(page_stride_head=4), -4)]:
+        assert lib.mi_paged_append(ctypes.byref(args(**fields))) == status, fields
+    assert lib.mi_paged_append(ctypes.byref(args(n_tokens=0))) == 0
+
+
+def test_paged_attention_refusals(lib, base):
+    assert lib.mi_paged_attn(None) == -1
+
+    def args(**fields):
+        a = _lib.MiPagedAttnArgs()
+        a.q = a.k_pages = a.v_pages = a.o = a.page_table = a.cu_seqlens = a.ctx_len = a.workspace = base
+        a.total_q, a.batch, a.n_pages, a.page_size, a.max_pages, a.page_table_stride = 5, 2, 9, 16, 40, 40
+        a.n_q_heads, a.n_kv_heads, a.head_dim, a.causal, a.softmax_scale = 4, 2, 64, 1, 0.125
+        a.q_stride_token = a.o_stride_token = 256
+        a.q_stride_head = a.o_stride_head = 64
+        a.page_stride, a.page_stride_token, a.page_stride_head = 16 * 128, 128, 64
+        a.workspace_bytes = lib.mi_paged_attn_workspace_bytes(5, 4, 2, 64)
+        return _set(a, **fields)
+    for fields, status in [
+            (dict(total_q=-1), -3), (dict(total_q=2 ** 31), -3), (dict(batch=0), -3), (dict(n_pages=0), -3), (dict(max_pages=0), -3), (dict(max_pages=2 ** 27), -3), (dict(page_size=0), -3),
+            (dict(page_size=20), -3), (dict(max_q_len=-1), -3), (dict(n_kv_heads=3), -3), (dict(n_q_heads=0), -3), (dict(n_kv_heads=0), -3), (dict(head_dim=80), -3), (dict(dtype=2), -2),
+            (dict(q=None), -1), (dict(k_pages=None), -1), (dict(v_pages=None), -1), (dict(o=None), -1), (dict(page_table=None), -1), (dict(cu_seqlens=None), -1), (dict(ctx_len=None), -1),
+            (dict(softmax_scale=0.0), -3), (dict(softmax_scale=float("nan")), -3), (dict(q=base + 2), -4), (dict(o=base + 8), -4), (dict(q_stride_token=4), -4), (dict(o_stride_head=2), -4),
+            (dict(page_stride=4), -4), (dict(page_stride_token=2 ** 27), -3), (dict(page_stride_token=-128), -3), (dict(workspace=None), -5), (dict(workspace=base + 4), -5),
+            (dict(workspace_bytes=64), -5), (dict(total_q=2 ** 30), -3), (dict(n_q_heads=70000, n_kv_heads=70000), -3)]:
+        assert lib.mi_paged_attn(ctypes.byref(args(**fields))) == status, fields
+    assert lib.mi_paged_attn(ctypes.byref(args(total_q=0, q=None))) == 0
+    sizes = [lib.mi_paged_attn_workspace_bytes(t, 32, 8, 128) for t in (1, 4, 5, 1000, 10 ** 6)]
+    assert sizes == sorted(sizes) and sizes[0] > 0
+    assert lib.mi_paged_attn_workspace_bytes(0, 32, 8, 128) == 0 and lib.mi_paged_attn_workspace_bytes(5, 32, 7, 128) == 0
