@@ -49,9 +49,13 @@ struct HeadParams {
     uint32_t heads_q_m, heads_k_m;
 };
 
-template <typename T, int VW> __device__ __forceinline__ void store_vec(T* p, const float* f) {
-    if constexpr (VW * sizeof(T) == 16) *reinterpret_cast<uint4*>(p) = Elem<T>::pack(f);
-    else Elem<T>::store1(p, *f);
+template <typename T, int VW, bool NT> __device__ __forceinline__ void store_vec(T* p, const float* f) {
+    if constexpr (VW * sizeof(T) == 16) {
+        if constexpr (NT) stg_nt(reinterpret_cast<uint4*>(p), Elem<T>::pack(f));
+        else *reinterpret_cast<uint4*>(p) = Elem<T>::pack(f);
+    } else {
+        Elem<T>::store1(p, *f);
+    }
 }
 // What turns a slot's features: rotate-half with tables of the rows' type or float32, or neighbouring pairs (of single elements: the slot's two).
 enum Turn { kHalf, kHalfF32, kPairs };
@@ -184,13 +188,30 @@ __device__ __forceinline__ float normalise(const HeadParams& p, const Slot (&s)[
 
 // Offset of token t's row in the pages, or -1 where the cache has no place for it: behind the last sequence, a position outside the page table, a page
 // outside the cache.  (Reads may be clamped, as the attention kernels clamp them; a write would land in somebody else's page.)
-__device__ __forceinline__ int64_t page_row(const HeadParams& p, int64_t t, int64_t token_stride) {
-    int lo = 0, hi = p.batch;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.cu[mid] <= t) lo = mid; else hi = mid;
+template <int L> __device__ __forceinline__ int64_t page_row(const HeadParams& p, int64_t t, int64_t token_stride) {
+    // The sequence: by counting ends that lie at or before t, lane i holding the end of sequence i: one trip to memory.  Of more than 64 by halving, a trip
+    // each.
+    int lo = 0, end, ctx;
+    if (p.batch <= 64) {
+        const int i = min((int)(threadIdx.x & 63), p.batch - 1), ends = p.cu[i + 1], lengths = p.ctx[i];
+        const bool counts = (int)(threadIdx.x & 63) < p.batch - 1;
+#pragma unroll
+        for (int g = 0; g < 64 / L; ++g) {                 // the items of the wavefront
+            const int before = __popcll(__ballot(counts && ends <= __builtin_amdgcn_readlane((int)t, g * L)));
+            lo = (int)(threadIdx.x & 63) / L == g ? before : lo;
+        }
+        end = __shfl(ends, lo);
+        ctx = __shfl(lengths, lo);
+    } else {
+        int hi = p.batch;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (p.cu[mid] <= t) lo = mid; else hi = mid;
+        }
+        end = p.cu[lo + 1];
+        ctx = p.ctx[lo];
     }
-    const int64_t first = p.cu[lo], end = p.cu[lo + 1], at = (int64_t)p.ctx[lo] - end + t;
+    const int64_t first = p.cu[lo], at = (int64_t)ctx - end + t;
     if (t < first || t >= end || at < 0 || at >= (int64_t)p.max_pages * p.page) return -1;
     const int in_table = divide((uint32_t)at, p.page, p.page_m), page = p.page_table[(int64_t)lo * p.table_stride + in_table];
     if (page < 0 || page >= p.n_pages) return -1;
@@ -229,9 +250,10 @@ template <typename T, int VW> struct Raw {
         }
     }
 };
-template <typename T, int VW> __device__ __forceinline__ void store_row(T* out, const Slot& s, const float (&a)[VW], const float (&b)[VW]) {
-    if (s.has_a) store_vec<T, VW>(out + s.a * VW, a);
-    if (s.has_b) store_vec<T, VW>(out + s.b * VW, b);
+// NT: past the caches (for rows of 8192 x 40 heads of 128: forward 31.1 -> 30.8 us, backward 52.0 -> 49.5; with loads past them too 57)
+template <typename T, int VW, bool NT> __device__ __forceinline__ void store_row(T* out, const Slot& s, const float (&a)[VW], const float (&b)[VW]) {
+    if (s.has_a) store_vec<T, VW, NT>(out + s.a * VW, a);
+    if (s.has_b) store_vec<T, VW, NT>(out + s.b * VW, b);
 }
 
 // A work item: some heads of one tensor at one token.  Positions' angles and the weights are loaded once for all of them; row by row they were two thirds of
@@ -277,9 +299,10 @@ template <bool PAGED> __device__ __forceinline__ RowsOf rows_of(const HeadParams
 // L lanes to a row, R slots to a lane
 template <typename T, int VW, int L, int R, int TURN, bool PAGED>
 __global__ __launch_bounds__(kBlock) void head_rows_kernel(const HeadParams p) {
-    const int64_t index = (int64_t)blockIdx.x * (kBlock / L) + threadIdx.x / L;
-    if (index >= p.n_tokens * p.blocks_all) return;        // the same for the lanes of a row
-    const Item it = item_of<PAGED>(p, (uint32_t)index);
+    const int64_t last = p.n_tokens * p.blocks_all - 1, index = (int64_t)blockIdx.x * (kBlock / L) + threadIdx.x / L;
+    if (!PAGED && index > last) return;                    // the same for the lanes of a row
+    Item it = item_of<PAGED>(p, (uint32_t)(index < last ? index : last));
+    if (index > last) it.h1 = it.h0;                       // nothing but a part in looking for places
     const RowsOf w = rows_of<PAGED>(p, it.which);
     const T* x = (const T*)w.x + it.t * w.xs_t;
     T* out = (T*)w.out;
@@ -295,12 +318,13 @@ __global__ __launch_bounds__(kBlock) void head_rows_kernel(const HeadParams p) {
         if (w.weight != nullptr) weight[r].load((const T*)w.weight, s[r]);
         if (w.bias != nullptr) bias[r].load((const T*)w.bias, s[r]);
     }
-    if (PAGED && it.which != 0) {
-        const int64_t at = page_row(p, it.t, w.os_t);
-        if (at < 0) return;
-        out += at;
-    } else {
-        out += it.t * w.os_t;
+    out += it.t * w.os_t;
+    if constexpr (PAGED) {
+        const int64_t at = page_row<L>(p, it.t, w.os_t);   // by all lanes together
+        if (it.which != 0) {
+            if (at < 0) return;
+            out = (T*)w.out + at;
+        }
     }
     for (int h = it.h0; h < it.h1; ++h) {
         float a[R][VW], b[R][VW];
@@ -335,7 +359,7 @@ __global__ __launch_bounds__(kBlock) void head_rows_kernel(const HeadParams p) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             rotate<T, VW, TURN, false>(p, s[r], angles[r], a[r], b[r]);
-            store_row<T, VW>(out + (int64_t)h * w.os_h, s[r], a[r], b[r]);
+            store_row<T, VW, !PAGED>(out + (int64_t)h * w.os_h, s[r], a[r], b[r]);
         }
     }
 }
@@ -417,7 +441,7 @@ __global__ __launch_bounds__(kBlock) void head_rows_grad_kernel(const HeadParams
                     da[r][i] = rstd * (da[r][i] - a[r][i] * dot - sum);
                     db[r][i] = rstd * (db[r][i] - b[r][i] * dot - sum);
                 }
-                store_row<T, VW>(out + (int64_t)h * w.os_h, s[r], da[r], db[r]);
+                store_row<T, VW, true>(out + (int64_t)h * w.os_h, s[r], da[r], db[r]);
             }
         }
     }
@@ -546,10 +570,11 @@ int fill(const mi_norm_rotary_args* a, const char* who, HeadParams& p) {
     return MI_OK;
 }
 
-// Heads of a work item: as many (up to kHeadsPerItem) as leave every compute unit `waves` wavefronts.
-constexpr int kHeadsPerItem = 8;
-void set_items(HeadParams& p, int lanes, int waves) {
-    const int64_t groups = (int64_t)mi_compute_units() * waves * 64 / lanes;
+// Heads of a work item: as many (up to 4) as leave every compute unit 8 wavefronts.  (8192 x 40 heads of 128, forward / backward with 1, 2, 4, 8, 32 heads to an
+// item: 58.8 / 110.6, 33.0 / 55.8, 31.2 / 51.9, 33.5 / 55.8, 33.7 / 55.9 us.)
+constexpr int kHeadsPerItem = 4;
+void set_items(HeadParams& p, int lanes) {
+    const int64_t groups = (int64_t)mi_compute_units() * 8 * 64 / lanes;
     const int64_t rows = p.n_tokens * (p.rows[0].heads + p.rows[1].heads + p.rows[2].heads);
     int n = kHeadsPerItem;
     while (n > 1 && rows < groups * n) n /= 2;
@@ -569,7 +594,7 @@ template <bool PAGED> int launch_rows(HeadParams& p, int dtype, const char* who,
         } else {
             with_shape<T>(p, whole<T>(p, false), [&](auto vec, auto lanes, auto slots, auto turn) {
                 constexpr int VW = decltype(vec)::value, L = decltype(lanes)::value, R = decltype(slots)::value, TURN = decltype(turn)::value;
-                set_items(p, L, 16);
+                set_items(p, L);
                 const dim3 grid((unsigned)((p.n_tokens * p.blocks_all + kBlock / L - 1) / (kBlock / L)));
                 head_rows_kernel<T, VW, L, R, TURN, PAGED><<<grid, dim3(kBlock), 0, st>>>(p);
             });
@@ -612,7 +637,7 @@ extern "C" int mi_norm_rotary_bwd(const mi_norm_rotary_bwd_args* b) {
     const hipStream_t st = (hipStream_t)a->stream;
     // workgroups in proportion to the items, no more than have one each
     const auto split = [&](int lanes) {
-        set_items(p, lanes, 16);
+        set_items(p, lanes);
         p.heads_q_m = divide_m(p.head_blocks[0]); p.heads_k_m = divide_m(p.head_blocks[1]);
         const int64_t rows_q = p.n_tokens * p.head_blocks[0], rows_k = p.n_tokens * p.head_blocks[1];
         const int64_t per = kBlock / lanes, all_q = (rows_q + per - 1) / per, all_k = (rows_k + per - 1) / per;
