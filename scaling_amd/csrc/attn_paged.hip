@@ -18,6 +18,7 @@ constexpr int kRowLimit = 16;        // rows of a sequence up to which paged_row
 constexpr int kRowBlock = 16;
 constexpr int kRowChunk = 32;        // keys per wavefront and step of paged_rows
 constexpr int kRowWaves = 4;
+constexpr int kRowTile = kRowChunk * kRowWaves;
 constexpr int kTileRows = 256;
 constexpr int kTileKeys = 64;
 constexpr float kRescaleGap = 8.0f;  // log2 units by which a row's maximum may lag before its output is rescaled
@@ -28,10 +29,9 @@ struct PagedParams {
     const int32_t *table, *cu, *ctx;
     int64_t table_stride, q_st, q_sh, o_st, o_sh, p_sp, p_st, p_sh;
     int batch, total, n_pages, page, max_pages, capacity, nq, nkv, n_rep, causal;
-    uint32_t page_m, rep_m, nkv_m;
+    uint32_t page_m, rep_m, nkv_m, share_m[2];        // for divide(); share_m: of rows and tiles
     float scale_log2;
     PagedPlan rows, tiles;
-    int rows_partials, tiles_partials;                // how many per KV head
     float *rows_o, *rows_ml, *tiles_o, *tiles_ml;     // partial results: [partial][KV head][row of the block][feature], and (maximum in log2 units, sum)
 };
 
@@ -65,29 +65,30 @@ struct Found {
 };
 
 // The sequence that `hit(first slot, slots, first partial result, partial results)` names, lane i looking at sequences i, i + 64, ...
-template <class Hit> __device__ __forceinline__ Found find_work(const PagedParams& p, const PagedPlan& plan, Hit hit) {
+template <int BLOCK, int TILE, class Hit> __device__ __forceinline__ Found find_work(const PagedParams& p, const PagedPlan& plan, uint32_t share_m, Hit hit) {
     const int lane = threadIdx.x & 63;
     PagedSeq seq{};
     PagedWork work{};
     auto look = [&](int base) {
         const int b = base + lane, i = min(b, p.batch - 1);
         seq = paged_seq(p.cu[i], p.cu[i + 1], p.ctx[i], p.total, p.capacity);
-        work = paged_work(plan, seq, p.n_rep);
+        work = paged_work<BLOCK, TILE>(plan, seq, p.n_rep);
         if (b >= p.batch) work.blocks = seq.n = 0;
     };
     int64_t units = 0;
-    if (plan.target > 0) {
+    if (plan.share > 0) {
         for (int base = 0; base < p.batch; base += 64) {
             look(base);
             units += (uint32_t)__builtin_amdgcn_readlane(prefix_sum(work.blocks * work.tiles), 63);
         }
     }
-    const int split_tiles = paged_split_tiles(plan, units);
+    // paged_split_tiles
+    const int split_tiles = plan.share == 0 ? 0x7fffff : divide((uint32_t)(units < 0x7fffffff ? units : 0x7fffffff), plan.share, share_m) + 1;
     int slots = 0, partials = 0;
     Found f;
     f.b = -1;
     for (int base = 0; base < p.batch; base += 64) {
-        if (p.batch > 64 || plan.target == 0) look(base);
+        if (p.batch > 64 || plan.share == 0) look(base);
         const int splits = paged_splits(work, split_tiles), n = work.blocks * splits, part = splits > 1 ? n : 0;
         const int upto = slots + prefix_sum(n), part_upto = partials + prefix_sum(part);
         const uint64_t found = __ballot(work.blocks > 0 && hit(upto - n, n, part_upto - part, part));
@@ -103,6 +104,7 @@ template <class Hit> __device__ __forceinline__ Found find_work(const PagedParam
             f.seq.len = __builtin_amdgcn_readlane(seq.len, l);
             f.work.blocks = __builtin_amdgcn_readlane(work.blocks, l);
             f.work.tiles = __builtin_amdgcn_readlane(work.tiles, l);
+            if (!paged_fits(plan, f.work, f.splits, f.slot, f.partial)) f.b = -1;
             return f;
         }
         slots = __builtin_amdgcn_readlane(upto, 63);
@@ -188,12 +190,11 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, G = lane >> 4;
     const int slot = divide(blockIdx.x, p.nkv, p.nkv_m), kvh = blockIdx.x - slot * p.nkv;
-    const Found f = find_work(p, p.rows, [&](int first, int n, int, int) { return slot >= first && slot < first + n; });
+    const Found f = find_work<kRowBlock, kRowTile>(p, p.rows, p.share_m[0], [&](int first, int n, int, int) { return slot >= first && slot < first + n; });
     if (f.b < 0) return;
-    const int in = slot - f.slot, split = in / f.work.blocks, block = in - split * f.work.blocks;
-    if (split >= f.splits || (f.splits > 1 && (uint32_t)(f.partial + in) >= (uint32_t)p.rows_partials)) return;
+    const int in = slot - f.slot, split = paged_quotient(in, f.work.blocks), block = in - split * f.work.blocks;
     int s0, s1;
-    paged_split_keys(p.rows, f.seq, f.work, f.splits, split, s0, s1);
+    paged_split_keys<kRowTile>(f.seq, f.work, f.splits, split, s0, s1);
     const int n_rows = min(kRowBlock, f.seq.n * p.n_rep - block * kRowBlock);
     // this lane's row
     const int row = block * kRowBlock + min(l16, n_rows - 1), token = divide(row, p.n_rep, p.rep_m), head = kvh * p.n_rep + row - token * p.n_rep;
@@ -224,6 +225,8 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
         const int group = (s0 + (NWV * (from + lane) + wave) * kRowChunk) >> 4;
 #pragma unroll
         for (int t = 0; t < 2; ++t) ids[t] = page_of(p, table, min(group + t, last_group));
+        // waited for here: where they are used the wait would be for everything that is under way, in every step
+        asm volatile("" : "+v"(ids[0]), "+v"(ids[1]));
     };
 
     struct ChunkRegs {
@@ -261,18 +264,12 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
         }
     };
     elem8_t qf[KS];
-    auto load_chunk = [&](ChunkRegs& c, int it) {
-        if (it >= n_iter) return;
-        if (it - ids_from >= 64) look_up(it);
-        request(c, it);
-    };
     auto process_chunk = [&](ChunkRegs& c, int it) {
         const int key0 = s0 + (NWV * it + wave) * kRowChunk;
-        const bool active = key0 < end;                    // wave-uniform
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         elem8_t pf;
-        float alpha = 1.f;
-        if (active) {
+        float alpha;
+        {
             f32x4v s_acc[2];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
@@ -312,13 +309,11 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (active) {
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const elem8_t a = tr_pair(vt_lane + 32 * dt, vt_lane + 16 * VSTR + 32 * dt);
-                o_acc[dt] = o_acc[dt] * alpha;
-                o_acc[dt] = mfma_16x16x32(a, pf, o_acc[dt]);
-            }
+        for (int dt = 0; dt < DT; ++dt) {
+            const elem8_t a = tr_pair(vt_lane + 32 * dt, vt_lane + 16 * VSTR + 32 * dt);
+            o_acc[dt] = o_acc[dt] * alpha;
+            o_acc[dt] = mfma_16x16x32(a, pf, o_acc[dt]);
         }
     };
 
@@ -329,20 +324,24 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
     }
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) qf[ks] = __builtin_bit_cast(elem8_t, raw[ks]);
-    for (int it = 0; it < n_iter; it += 2) {
-        load_chunk(rb, it + 1);
+    // No branch around a request or a chunk: where paths meet, the wait for a chunk would be for the next one too.  So chunks past the split's keys are
+    // requested (its last key over and over) and computed, with nothing in them, where other wavefronts still have some.
+    for (int it = 0; n_iter > 0;) {
+        if (it + 1 - ids_from >= 64) look_up(it + 1);
+        request(rb, it + 1);
         process_chunk(ra, it);
-        if (it + 1 < n_iter) {
-            load_chunk(ra, it + 2);
-            process_chunk(rb, it + 1);
-        }
+        if (++it >= n_iter) break;
+        if (it + 1 - ids_from >= 64) look_up(it + 1);
+        request(ra, it + 1);
+        process_chunk(rb, it);
+        if (++it >= n_iter) break;
     }
 
     // ---- the wavefronts' results together; of a single split the output, else a partial result ----
     l_i = quad_sum(l_i);
     if (G == 0) { wm_lds[wave][l16] = m_i; wl_lds[wave][l16] = l_i; }
     if (tid < 16) redo_lds[tid] = 0;
-    const int filled = (s1 + kRowChunk - 1) & -kRowChunk;  // chunks are filled up to here: with keys that a row may not see, or with others once more
+    const int filled = s0 + n_iter * kRowTile;             // chunks reach up to here: with keys that a row may not see, or with others once more
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -450,12 +449,11 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63, l32 = lane & 31, g = lane >> 5;
     const int slot = divide(blockIdx.x, p.nkv, p.nkv_m), kvh = blockIdx.x - slot * p.nkv;
-    const Found f = find_work(p, p.tiles, [&](int first, int n, int, int) { return slot >= first && slot < first + n; });
+    const Found f = find_work<kTileRows, kTileKeys>(p, p.tiles, p.share_m[1], [&](int first, int n, int, int) { return slot >= first && slot < first + n; });
     if (f.b < 0) return;                                   // the same for the whole workgroup
-    const int in = slot - f.slot, split = in / f.work.blocks, block = f.work.blocks - 1 - (in - split * f.work.blocks);      // longest first
-    if (split >= f.splits || (f.splits > 1 && (uint32_t)(f.partial + in) >= (uint32_t)p.tiles_partials)) return;
+    const int in = slot - f.slot, split = paged_quotient(in, f.work.blocks), block = f.work.blocks - 1 - (in - split * f.work.blocks);      // longest first
     int s0, s1;
-    paged_split_keys(p.tiles, f.seq, f.work, f.splits, split, s0, s1);
+    paged_split_keys<kTileKeys>(f.seq, f.work, f.splits, split, s0, s1);
 
     // ---- this lane's row, its keys [s0, limit), its part of Q ----
     const int n_rows = f.seq.n * p.n_rep, row = block * kTileRows + wave * 32 + l32;
@@ -497,7 +495,10 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
     auto load_tile = [&](int tile) {
         if (tile >= n_tiles) return;
         const int group0 = (s0 >> 4) + lw;
-        if ((tile & 63) == 0) ids = page_of(p, table, min(group0 + 4 * (tile + lane), last_group));
+        if ((tile & 63) == 0) {
+            ids = page_of(p, table, min(group0 + 4 * (tile + lane), last_group));
+            asm volatile("" : "+v"(ids));                  // waited for here, not (with all that is under way) at its use in every step
+        }
         const int group = min(group0 + 4 * tile, last_group);
         const int page = __builtin_amdgcn_readlane(ids, tile & 63);
         const elem_t* from = base + (int64_t)page * p.p_sp + (int64_t)row_in_page(p, group) * p.p_st;
@@ -672,17 +673,19 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
 constexpr int kMergeWaves = 4;
 template <int D>
 __global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const PagedParams p, int kind) {
-    const PagedPlan& plan = kind ? p.tiles : p.rows;
+    constexpr int kRows[2] = {kRowBlock, kTileRows};
+    const int block_rows = kRows[kind];
     const float *from_o = kind ? p.tiles_o : p.rows_o, *from_ml = kind ? p.tiles_ml : p.rows_ml;
     const int partial = blockIdx.x, kvh = blockIdx.y, d = 2 * (threadIdx.x & 63);
-    const Found f = find_work(p, plan, [&](int, int, int first, int n) { return partial >= first && partial < first + n; });
+    const auto holds = [&](int, int, int first, int n) { return partial >= first && partial < first + n; };
+    const Found f = kind ? find_work<kTileRows, kTileKeys>(p, p.tiles, p.share_m[1], holds) : find_work<kRowBlock, kRowTile>(p, p.rows, p.share_m[0], holds);
     const int block = partial - f.partial;
-    if (f.b < 0 || block >= f.work.blocks || f.partial + f.work.blocks * f.splits > (kind ? p.tiles_partials : p.rows_partials)) return;
-    const int64_t step = (int64_t)f.work.blocks * p.nkv * plan.block_rows;
+    if (f.b < 0 || block >= f.work.blocks) return;
+    const int64_t step = (int64_t)f.work.blocks * p.nkv * block_rows;
     for (int in = 16 * blockIdx.z + (threadIdx.x >> 6); in < 16 * ((int)blockIdx.z + 1); in += kMergeWaves) {
-        const int row = block * plan.block_rows + in;
+        const int row = block * block_rows + in;
         if (row >= f.seq.n * p.n_rep) return;
-        const int64_t first = ((int64_t)partial * p.nkv + kvh) * plan.block_rows + in;
+        const int64_t first = ((int64_t)partial * p.nkv + kvh) * block_rows + in;
         float M = -INFINITY, L = 0.f, O0 = 0.f, O1 = 0.f;
         constexpr int kStep = 8;
         for (int s0 = 0; s0 < f.splits; s0 += kStep) {
@@ -726,21 +729,23 @@ template <int D> int launch(const PagedParams& p, int64_t row_slots, int64_t til
         paged_tiles_kernel<D><<<dim3((unsigned)(tile_slots * p.nkv)), dim3(512), 0, st>>>(p);
         if (const int rc = mi_check_launch("paged_tiles"); rc != MI_OK) return rc;
     }
-    if (p.rows_o != nullptr) paged_merge_kernel<D><<<dim3(p.rows_partials, p.nkv, kRowBlock / 16), dim3(64 * kMergeWaves), 0, st>>>(p, 0);
-    if (p.tiles_o != nullptr) paged_merge_kernel<D><<<dim3(p.tiles_partials, p.nkv, kTileRows / 16), dim3(64 * kMergeWaves), 0, st>>>(p, 1);
+    if (p.rows.max_partials > 0) paged_merge_kernel<D><<<dim3(p.rows.max_partials, p.nkv, kRowBlock / 16), dim3(64 * kMergeWaves), 0, st>>>(p, 0);
+    if (p.tiles.max_partials > 0) paged_merge_kernel<D><<<dim3(p.tiles.max_partials, p.nkv, kTileRows / 16), dim3(64 * kMergeWaves), 0, st>>>(p, 1);
     return mi_check_launch("paged_merge");
 }
 
-// Plans of both kernels for a call of these sizes.
+// Workgroups per KV head that either kernel's work is cut for.
+int share_of(int workgroups, int nkv) { return workgroups / nkv > 0 ? workgroups / nkv : 1; }
 void make_plans(int64_t tokens, int n_rep, int nkv, PagedPlan& rows, PagedPlan& tiles) {
     const int cus = mi_compute_units();
-    rows = PagedPlan{0, kRowLimit, kRowBlock, kRowWaves * kRowChunk, 4 * cus, nkv};
+    rows = PagedPlan{0, kRowLimit, 0x7fffffff, share_of(4 * cus, nkv), 0, 0};
     // Enough blocks for every compute unit: no splits, no merge.
     const bool many = tokens * n_rep / kTileRows * nkv >= cus;
-    tiles = PagedPlan{kRowLimit, 0x7fffffff, kTileRows, kTileKeys, many ? 0 : cus, nkv};
+    tiles = PagedPlan{kRowLimit, 0x7fffffff, 0x7fffffff, many ? 0 : share_of(cus, nkv), 0, 0};
 }
 
-size_t partial_bytes(const PagedPlan& p, int head_dim) { return (size_t)paged_max_partials(p) * p.nkv * p.block_rows * (size_t)(head_dim + 2) * sizeof(float); }
+size_t partial_bytes(int64_t partials, int nkv, int block_rows, int head_dim) { return (size_t)partials * nkv * block_rows * (size_t)(head_dim + 2) * sizeof(float); }
+constexpr int64_t kMaxTiles = (1 << 24) + 1;              // of a sequence
 
 }  // namespace
 
@@ -750,7 +755,8 @@ extern "C" size_t mi_paged_attn_workspace_bytes(int64_t tokens, int32_t n_q_head
     PagedPlan rows, tiles;
     const int n_rep = n_q_heads / n_kv_heads;
     make_plans(0, n_rep, n_kv_heads, rows, tiles);         // for so many tokens or fewer
-    return partial_bytes(rows, head_dim) + (tokens * n_rep > kRowLimit ? partial_bytes(tiles, head_dim) : 0);
+    return partial_bytes(paged_max_partials(rows, kMaxTiles, kMaxTiles), n_kv_heads, kRowBlock, head_dim) +
+           (tokens * n_rep > kRowLimit ? partial_bytes(paged_max_partials(tiles, kMaxTiles, kMaxTiles), n_kv_heads, kTileRows, head_dim) : 0);
 }
 #endif
 
@@ -780,29 +786,31 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
     p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
     make_plans(p.total, p.n_rep, p.nkv, p.rows, p.tiles);
     const int64_t longest = a->max_q_len > 0 && a->max_q_len < p.total ? a->max_q_len : p.total;
-    const int64_t row_blocks = paged_max_blocks(p.rows, p.total, p.batch, longest, p.n_rep), tile_blocks = paged_max_blocks(p.tiles, p.total, p.batch, longest, p.n_rep);
-    if (p.nkv > 0xffff) return mi_fail(MI_E_SHAPE, "paged_attn: more than 65535 KV heads");
+    p.rows.max_n = p.tiles.max_n = (int)longest;
+    const int64_t row_blocks = paged_max_blocks<kRowBlock>(p.rows, p.total, p.batch, longest, p.n_rep);
+    const int64_t tile_blocks = paged_max_blocks<kTileRows>(p.tiles, p.total, p.batch, longest, p.n_rep);
+    const int64_t row_tiles = ((int64_t)p.capacity + kRowTile - 1) / kRowTile, tile_tiles = ((int64_t)p.capacity + kTileKeys - 1) / kTileKeys;
     // Sums of blocks x tiles and of rows are kept in 32 bits, and a grid has fewer than 2^31 workgroups.
-    const int64_t tiles_most = (int64_t)p.capacity / kTileKeys + 1;
-    if ((int64_t)p.total * p.n_rep > 0x7fffffffLL || (row_blocks + tile_blocks) * tiles_most > 0x7fffffffLL || (int64_t)p.total * p.nkv > 0x7fffffffLL ||
+    if (p.nkv > 0xffff) return mi_fail(MI_E_SHAPE, "paged_attn: more than 65535 KV heads");
+    if ((int64_t)p.total * p.n_rep > 0x7fffffffLL - kTileRows || row_blocks * row_tiles > 0x7fffffffLL || tile_blocks * tile_tiles > 0x7fffffffLL ||
         (row_blocks + tile_blocks + 8LL * mi_compute_units()) * p.nkv > 0x7fffffffLL)
         return mi_fail(MI_E_SHAPE, "paged_attn: %lld tokens of %d heads over up to %d keys are too many for one call", (long long)a->total_q, a->n_q_heads, p.capacity);
-    const size_t rows_bytes = partial_bytes(p.rows, a->head_dim), need = mi_paged_attn_workspace_bytes(p.total, p.nq, p.nkv, a->head_dim);
+    const size_t need = mi_paged_attn_workspace_bytes(p.total, p.nq, p.nkv, a->head_dim);
     if (!a->workspace || a->workspace_bytes < need || !mi_aligned16(a->workspace))
         return mi_fail(MI_E_WORKSPACE, "paged_attn: workspace needs %zu bytes (16-byte aligned), got %zu", need, a->workspace_bytes);
     // A sequence of up to a tile of keys has one split, whatever the plan.
-    if (p.capacity <= p.rows.tile_keys || row_blocks == 0) p.rows.target = 0;
-    if (p.capacity <= p.tiles.tile_keys || tile_blocks == 0) p.tiles.target = 0;
-    const auto place = [&](const PagedPlan& plan, char* at, float*& o, float*& ml) {
-        if (plan.target == 0) return;
-        o = (float*)at;
-        ml = o + (size_t)paged_max_partials(plan) * plan.nkv * plan.block_rows * a->head_dim;
-    };
-    p.rows_partials = (int)paged_max_partials(p.rows);
-    p.tiles_partials = (int)paged_max_partials(p.tiles);
-    place(p.rows, (char*)a->workspace, p.rows_o, p.rows_ml);
-    place(p.tiles, (char*)a->workspace + rows_bytes, p.tiles_o, p.tiles_ml);
-    const int64_t row_slots = paged_max_slots(p.rows, row_blocks), tile_slots = paged_max_slots(p.tiles, tile_blocks);
+    if (row_tiles == 1 || row_blocks == 0) p.rows.share = 0;
+    if (tile_tiles == 1 || tile_blocks == 0) p.tiles.share = 0;
+    p.share_m[0] = divide_m(p.rows.share); p.share_m[1] = divide_m(p.tiles.share);
+    p.rows.max_slots = (int)paged_max_slots(p.rows, row_blocks, row_tiles);
+    p.tiles.max_slots = (int)paged_max_slots(p.tiles, tile_blocks, tile_tiles);
+    p.rows.max_partials = (int)paged_max_partials(p.rows, row_blocks, row_tiles);
+    p.tiles.max_partials = (int)paged_max_partials(p.tiles, tile_blocks, tile_tiles);
+    p.rows_o = (float*)a->workspace;
+    p.rows_ml = p.rows_o + (size_t)p.rows.max_partials * p.nkv * kRowBlock * a->head_dim;
+    p.tiles_o = p.rows_o + partial_bytes(p.rows.max_partials, p.nkv, kRowBlock, a->head_dim) / sizeof(float);
+    p.tiles_ml = p.tiles_o + (size_t)p.tiles.max_partials * p.nkv * kTileRows * a->head_dim;
+    const int64_t row_slots = p.rows.max_slots, tile_slots = p.tiles.max_slots;
     const hipStream_t st = (hipStream_t)a->stream;
     switch (a->head_dim) {
         case 32: return launch<32>(p, row_slots, tile_slots, st);

@@ -2,12 +2,12 @@
 // arithmetic, the same for every workgroup of a launch and for the launch that merges; compiles for the host alone too.
 //
 // A sequence's rows are (new token, query head of a group): token i of n and head r of n_rep make row i * n_rep + r, so all heads that share keys share a
-// block of rows.  A kernel takes the sequences whose number of rows it suits, in blocks of `block_rows`, with keys in tiles of `tile_keys`.  Where blocks are
-// few, the keys of a sequence are cut into splits of at most S tiles each, with S such that all splits together are about `target` workgroups:
-//     W = sum over sequences of blocks * tiles (per KV head),   S = floor(W * nkv / target) + 1,   splits_b = ceil(tiles_b / S)
-// Then splits of all blocks are at most target / nkv + blocks in number, and those of sequences with more than one split at most 2 * target / nkv (tiles > S
-// gives ceil(tiles / S) < 2 tiles / S).  Lengths may be anything: sequences are clamped to the tokens and the page table that there are, and where lengths that
-// overlap make more partial results than the workspace holds, those are left out.
+// block of rows.  A kernel takes the sequences whose number of rows it suits, in blocks of rows, with keys in tiles.  The keys of a sequence are cut into
+// splits of at most S tiles each, with S such that all splits together are about `share` workgroups per KV head:
+//     W = sum over sequences of blocks * tiles,   S = floor(W / share) + 1,   splits_b = ceil(tiles_b / S)
+// Then splits of all blocks are at most share + blocks in number, and those of sequences with more than one split at most 2 * share (tiles > S gives
+// ceil(tiles / S) < 2 tiles / S).  Lengths may be anything: sequences are clamped to the tokens and the page table that there are, and where lengths that
+// overlap make more workgroups or partial results than there are, sequences are left out as a whole.
 #pragma once
 #include <stdint.h>
 
@@ -38,45 +38,77 @@ MI_PLAN_FN int paged_limit(const PagedSeq& s, int i, bool causal) {
     return causal ? paged_clamp((int64_t)s.ctx - s.n + i + 1, 0, s.len) : s.len;
 }
 
+// a / b for a < 2^24, 0 < b, by a reciprocal and corrections (the compiler's division is five times as long, and a workgroup's first steps wait for it)
+MI_PLAN_FN int paged_quotient(int a, int b) {
+#ifdef __HIP_DEVICE_COMPILE__
+    int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));      // two units in the last place of up to 24 bits: off by at most 2
+    int r = a - q * b;
+    for (int i = 0; i < 2; ++i) {
+        const int by = r < 0 ? -1 : r >= b ? 1 : 0;
+        q += by;
+        r -= by * b;
+    }
+    return q;
+#else
+    return a / b;
+#endif
+}
+
 struct PagedPlan {
     int rows_over, rows_up_to;    // sequences with more than rows_over and at most rows_up_to rows
-    int block_rows, tile_keys;
-    int target;                   // workgroups aimed at; 0: never split
-    int nkv;
+    int max_n;                    // ... and at most so many new tokens
+    int share;                    // workgroups per KV head aimed at; 0: never split
+    int max_slots, max_partials;  // (set by the host) workgroups and partial results per KV head that there are
 };
 
 struct PagedWork {
     int blocks, tiles;            // blocks 0: not this kernel's
 };
-MI_PLAN_FN PagedWork paged_work(const PagedPlan& p, const PagedSeq& s, int n_rep) {
-    const int64_t rows = (int64_t)s.n * n_rep;
+// BLOCK rows to a block, TILE keys to a tile: powers of two
+template <int BLOCK, int TILE> MI_PLAN_FN PagedWork paged_work(const PagedPlan& p, const PagedSeq& s, int n_rep) {
+    const int rows = s.n * n_rep;                           // of all tokens: fewer than 2^31
     PagedWork w;
-    w.blocks = rows > p.rows_over && rows <= p.rows_up_to ? (int)((rows + p.block_rows - 1) / p.block_rows) : 0;
-    w.tiles = s.len > 0 ? (int)(((int64_t)s.len + p.tile_keys - 1) / p.tile_keys) : 1;      // rows without keys are written too
+    w.blocks = rows > p.rows_over && rows <= p.rows_up_to && s.n <= p.max_n ? (int)(((uint32_t)rows + BLOCK - 1) / BLOCK) : 0;
+    w.tiles = s.len > 0 ? (s.len + TILE - 1) / TILE : 1;    // rows without keys are written too
     return w;
 }
 // tiles of a split; `units` is W
-MI_PLAN_FN int paged_split_tiles(const PagedPlan& p, int64_t units) { return p.target > 0 ? paged_clamp(units * p.nkv / p.target + 1, 1, 0x7fffffff) : 0x7fffffff; }
-MI_PLAN_FN int paged_splits(const PagedWork& w, int split_tiles) { return (w.tiles - 1) / split_tiles + 1; }
+MI_PLAN_FN int paged_split_tiles(const PagedPlan& p, int64_t units) {
+    if (p.share == 0) return 0x7fffff;                      // no sequence has more
+    const uint32_t u = (uint32_t)(units < 0x7fffffff ? units : 0x7fffffff);
+    return (int)(u / (uint32_t)p.share) + 1;
+}
+MI_PLAN_FN int paged_splits(const PagedWork& w, int split_tiles) { return paged_quotient(w.tiles - 1, split_tiles) + 1; }
 // keys [k0, k1) of split i
-MI_PLAN_FN void paged_split_keys(const PagedPlan& p, const PagedSeq& s, const PagedWork& w, int splits, int i, int& k0, int& k1) {
-    const int64_t per = (int64_t)((w.tiles + splits - 1) / splits) * p.tile_keys;
-    const int64_t a = per * i, b = a + per;
-    k0 = a < s.len ? (int)a : s.len;
-    k1 = b < s.len ? (int)b : s.len;
+template <int TILE> MI_PLAN_FN void paged_split_keys(const PagedSeq& s, const PagedWork& w, int splits, int i, int& k0, int& k1) {
+    const int64_t per = (int64_t)(paged_quotient(w.tiles - 1, splits) + 1) * TILE;
+    k0 = paged_clamp(per * i, 0, s.len);
+    k1 = paged_clamp(per * i + per, 0, s.len);
+}
+// Whether a launch computes a sequence whose first slot and first partial result are these: all of its splits or none.
+MI_PLAN_FN bool paged_fits(const PagedPlan& p, const PagedWork& w, int splits, int slot, int partial) {
+    const int64_t n = (int64_t)w.blocks * splits;
+    return slot >= 0 && slot + n <= p.max_slots && (splits == 1 || (partial >= 0 && partial + n <= p.max_partials));
 }
 
 // Upper bounds for the host: blocks of rows that `tokens` tokens of `batch` sequences make, at most max_q_len of them in one; workgroups per KV head; and
-// partial results per KV head.
-MI_PLAN_FN int64_t paged_max_blocks(const PagedPlan& p, int64_t tokens, int64_t batch, int64_t max_q_len, int n_rep) {
+// partial results per KV head, of sequences of up to max_tiles tiles.
+template <int BLOCK> MI_PLAN_FN int64_t paged_max_blocks(const PagedPlan& p, int64_t tokens, int64_t batch, int64_t max_q_len, int n_rep) {
     int64_t rows = max_q_len * n_rep;                       // of one sequence
     if (rows <= p.rows_over) return 0;
     if (rows > p.rows_up_to) rows = p.rows_up_to;
-    const int64_t each = (rows + p.block_rows - 1) / p.block_rows * batch;
+    const int64_t each = (rows + BLOCK - 1) / BLOCK * batch;
     const int64_t least = (int64_t)p.rows_over + 1;         // rows of a sequence that is this kernel's
     const int64_t sequences = tokens * n_rep / least < batch ? tokens * n_rep / least : batch;
-    const int64_t together = tokens * n_rep / p.block_rows + sequences;
+    const int64_t together = tokens * n_rep / BLOCK + sequences;
     return each < together ? each : together;
 }
-MI_PLAN_FN int64_t paged_max_slots(const PagedPlan& p, int64_t blocks) { return blocks == 0 ? 0 : blocks + (p.target > 0 ? p.target / p.nkv + 1 : 0); }
-MI_PLAN_FN int64_t paged_max_partials(const PagedPlan& p) { return p.target > 0 ? 2 * (int64_t)p.target / p.nkv + 2 : 0; }
+MI_PLAN_FN int64_t paged_max_slots(const PagedPlan& p, int64_t blocks, int64_t max_tiles) {
+    const int64_t each = blocks * max_tiles, together = blocks + p.share + 1;
+    return p.share == 0 || blocks == 0 ? blocks : each < together ? each : together;
+}
+MI_PLAN_FN int64_t paged_max_partials(const PagedPlan& p, int64_t blocks, int64_t max_tiles) {
+    if (p.share == 0) return 0;
+    const int64_t each = blocks * max_tiles, together = 2 * (int64_t)p.share + 2;
+    return each < together ? each : together;
+}

@@ -18,6 +18,54 @@ PROGRAM = r"""
 static unsigned long long state = 88172645463325252ull;
 static unsigned rnd() { state ^= state << 13; state ^= state >> 7; state ^= state << 17; return (unsigned)(state >> 11); }
 static int fail(const char* what, int i) { printf("case %%d: %%s\n", i, what); return 1; }
+template <int BLOCK, int TILE>
+static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, int capacity, int longest, bool good, bool causal, const std::vector<int>& cu,
+                  const std::vector<int>& ctx, std::vector<int>& taken) {
+    PagedPlan p = {over, up_to, longest, rnd() %% 4 == 0 ? 0 : 1 << rnd() %% 9, 0, 0};
+    const int max_tiles = (capacity + TILE - 1) / TILE;
+    const int64_t most = paged_max_blocks<BLOCK>(p, total, batch, longest, n_rep);
+    p.max_slots = (int)paged_max_slots(p, most, max_tiles);
+    p.max_partials = (int)paged_max_partials(p, most, max_tiles);
+    int64_t units = 0, slots = 0, partials = 0, blocks = 0;
+    for (int b = 0; b < batch; ++b) {
+        const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity);
+        if (s.first < 0 || s.n < 0 || s.first + s.n > total || s.len < 0 || s.len > capacity) return fail("a sequence outside the tokens or the table", c);
+        const PagedWork w = paged_work<BLOCK, TILE>(p, s, n_rep);
+        units += (int64_t)w.blocks * w.tiles;
+    }
+    const int S = paged_split_tiles(p, units);
+    if (S < 1) return fail("no tiles to a split", c);
+    for (int b = 0; b < batch; ++b) {
+        const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity);
+        const PagedWork w = paged_work<BLOCK, TILE>(p, s, n_rep);
+        const int splits = paged_splits(w, S);
+        if (splits < 1) return fail("no split", c);
+        const bool fits = paged_fits(p, w, splits, (int)slots, (int)partials);
+        if (good && w.blocks > 0 && !fits) return fail("a sequence left out", c);
+        if (fits && w.blocks > 0 && slots + (int64_t)w.blocks * splits > p.max_slots) return fail("a workgroup that is not there", c);
+        blocks += w.blocks;
+        slots += (int64_t)w.blocks * splits;
+        if (splits > 1) partials += (int64_t)w.blocks * splits;
+        if (fits && splits > 1 && w.blocks > 0 && partials > p.max_partials) return fail("a partial result outside the workspace", c);
+        if (w.blocks > 0 && good) for (int i = 0; i < s.n; ++i) ++taken[s.first + i];
+        int at = 0;
+        for (int i = 0; i < splits; ++i) {                 // splits cover the keys once, in order, in whole tiles
+            int k0, k1;
+            paged_split_keys<TILE>(s, w, splits, i, k0, k1);
+            if (k0 != at || k1 < k0 || k1 > s.len || (k0 %% TILE != 0 && k0 != s.len) || (k1 - k0 + TILE - 1) / TILE > S) return fail("keys of a split", c);
+            at = k1;
+        }
+        if (at != s.len) return fail("keys left out", c);
+        for (int i = 0; i < s.n; i += 1 + s.n / 5) {
+            const int64_t want = causal ? (int64_t)s.ctx - s.n + i + 1 : s.len;
+            const int got = paged_limit(s, i, causal);
+            if (got != (want < 0 ? 0 : want > s.len ? s.len : (int)want)) return fail("limit of a row", c);
+        }
+    }
+    if (good && (blocks > most || (blocks == 0) < (most == 0))) return fail("more blocks than the bound", c);
+    if (good && (slots > p.max_slots || partials > p.max_partials)) return fail("more workgroups or partial results than the bound", c);
+    return 0;
+}
 int main() {
     for (int c = 0; c < 4000; ++c) {
         const int batch = 1 + rnd() %% (c %% 5 == 0 ? 300 : 9), n_rep = 1 + rnd() %% 40, nkv = 1 + rnd() %% 9, pages = 1 + rnd() %% 70, page = 16 * (1 + rnd() %% 9);
@@ -34,50 +82,10 @@ int main() {
         }
         cu[batch] = good ? total : (int)(rnd() - 2147483648u);
         int longest = 0;
-        const int tile_keys[2] = {128, 64}, block[2] = {16, 256};
         std::vector<int> taken(good ? total : 0, 0);
         for (int b = 0; b < batch; ++b) { const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity); if (s.n > longest) longest = s.n; }
-        for (int k = 0; k < 2; ++k) {
-            const PagedPlan p = {k == 0 ? 0 : 16, k == 0 ? 16 : 0x7fffffff, block[k], tile_keys[k], rnd() %% 4 == 0 ? 0 : 1 << rnd() %% 11, nkv};
-            int64_t units = 0, slots = 0, partials = 0, blocks = 0;
-            for (int b = 0; b < batch; ++b) {
-                const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity);
-                if (s.first < 0 || s.n < 0 || s.first + s.n > total || s.len < 0 || s.len > capacity) return fail("a sequence outside the tokens or the table", c);
-                const PagedWork w = paged_work(p, s, n_rep);
-                units += (int64_t)w.blocks * w.tiles;
-            }
-            const int S = paged_split_tiles(p, units);
-            if (S < 1) return fail("no tiles to a split", c);
-            for (int b = 0; b < batch; ++b) {
-                const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity);
-                const PagedWork w = paged_work(p, s, n_rep);
-                const int splits = paged_splits(w, S);
-                if (splits < 1) return fail("no split", c);
-                blocks += w.blocks;
-                slots += (int64_t)w.blocks * splits;
-                if (splits > 1) partials += (int64_t)w.blocks * splits;
-                if (w.blocks > 0 && good) for (int i = 0; i < s.n; ++i) ++taken[s.first + i];
-                int at = 0;
-                for (int i = 0; i < splits; ++i) {         // splits cover the keys once, in order, in whole tiles
-                    int k0, k1;
-                    paged_split_keys(p, s, w, splits, i, k0, k1);
-                    if (k0 != at || k1 < k0 || k1 > s.len || (k0 %% p.tile_keys != 0 && k0 != s.len) || (k1 - k0 + p.tile_keys - 1) / p.tile_keys > S) return fail("keys of a split", c);
-                    at = k1;
-                }
-                if (at != s.len) return fail("keys left out", c);
-                for (int i = 0; i < s.n; i += 1 + s.n / 5) {
-                    const int64_t want = causal ? (int64_t)s.ctx - s.n + i + 1 : s.len;
-                    const int got = paged_limit(s, i, causal);
-                    if (got != (want < 0 ? 0 : want > s.len ? s.len : (int)want)) return fail("limit of a row", c);
-                }
-            }
-            if (good) {
-                const int64_t most = paged_max_blocks(p, total, batch, longest, n_rep);
-                if (blocks > most || (blocks == 0) < (most == 0)) return fail("more blocks than the bound", c);
-                if (slots > paged_max_slots(p, most)) return fail("more workgroups than the bound", c);
-                if (partials > paged_max_partials(p)) return fail("more partial results than the bound", c);
-            }
-        }
+        if (kernel<16, 128>(c, 0, 16, batch, n_rep, total, capacity, longest, good, causal, cu, ctx, taken)) return 1;
+        if (kernel<256, 64>(c, 16, 0x7fffffff, batch, n_rep, total, capacity, longest, good, causal, cu, ctx, taken)) return 1;
         for (int t : taken) if (t != 1) return fail("a token that is not exactly one kernel's", c);
     }
     printf("ok\n");
