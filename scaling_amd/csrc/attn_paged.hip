@@ -10,6 +10,8 @@
 #include "attn_common.h"
 #include "paged_plan.h"
 
+#include <algorithm>
+
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 
 namespace {
@@ -54,18 +56,19 @@ __device__ __forceinline__ int prefix_sum(int v) {
     return v;
 }
 
-// A sequence as one workgroup or row meets it; the same in every lane.
+// A sequence as one workgroup meets it; the same in every lane.
 struct Found {
     int b;             // -1: none
-    int slot;          // of the sequence's blocks * splits, where it was looked for by a slot
+    int at;            // first slot of the sequence's blocks * splits; of a search for split blocks the first of these
     int splits;
     int partial;       // first partial result of the sequence (splits > 1)
     PagedSeq seq;
     PagedWork work;
 };
 
-// The sequence that `hit(first slot, slots, first partial result, partial results)` names, lane i looking at sequences i, i + 64, ...
-template <int BLOCK, int TILE, class Hit> __device__ __forceinline__ Found find_work(const PagedParams& p, const PagedPlan& plan, uint32_t share_m, Hit hit) {
+// The sequence that holds slot `wanted` or, with OF_BLOCKS, the one that holds block `wanted` of all blocks with several splits; lane i looks at sequences
+// i, i + 64, ...
+template <int BLOCK, int TILE, bool OF_BLOCKS> __device__ __forceinline__ Found find_work(const PagedParams& p, const PagedPlan& plan, uint32_t share_m, int wanted) {
     const int lane = threadIdx.x & 63;
     PagedSeq seq{};
     PagedWork work{};
@@ -75,27 +78,39 @@ template <int BLOCK, int TILE, class Hit> __device__ __forceinline__ Found find_
         work = paged_work<BLOCK, TILE>(plan, seq, p.n_rep);
         if (b >= p.batch) work.blocks = seq.n = 0;
     };
-    int64_t units = 0;
+    const auto total = [](int v) { return (int64_t)(uint32_t)__builtin_amdgcn_readlane(prefix_sum(v), 63); };
+    int split_tiles = 0x1000000;                          // no sequence has more
     if (plan.share > 0) {
+        int64_t units = 0, blocks = 0;
         for (int base = 0; base < p.batch; base += 64) {
             look(base);
-            units += (uint32_t)__builtin_amdgcn_readlane(prefix_sum(work.blocks * work.tiles), 63);
+            units += total(work.blocks * work.tiles);
+            if (plan.fit) blocks += total(work.blocks);
+        }
+        // paged_split_tiles
+        split_tiles = divide((uint32_t)(units < 0x7fffffff ? units : 0x7fffffff), plan.share, share_m) + 1;
+        for (int step = 0; plan.fit && blocks <= plan.share && step < kPagedSteps; ++step) {
+            int64_t slots = 0;
+            for (int base = 0; base < p.batch; base += 64) {
+                if (p.batch > 64) look(base);
+                slots += total(work.blocks * paged_splits(work, split_tiles));
+            }
+            split_tiles = paged_next_tiles(plan, split_tiles, blocks, slots);
         }
     }
-    // paged_split_tiles
-    const int split_tiles = plan.share == 0 ? 0x7fffff : divide((uint32_t)(units < 0x7fffffff ? units : 0x7fffffff), plan.share, share_m) + 1;
-    int slots = 0, partials = 0;
+    int at = 0, slots = 0, partials = 0;
     Found f;
     f.b = -1;
     for (int base = 0; base < p.batch; base += 64) {
         if (p.batch > 64 || plan.share == 0) look(base);
         const int splits = paged_splits(work, split_tiles), n = work.blocks * splits, part = splits > 1 ? n : 0;
-        const int upto = slots + prefix_sum(n), part_upto = partials + prefix_sum(part);
-        const uint64_t found = __ballot(work.blocks > 0 && hit(upto - n, n, part_upto - part, part));
+        const int slots_upto = slots + prefix_sum(n), part_upto = partials + prefix_sum(part);
+        const int width = OF_BLOCKS ? (splits > 1 ? work.blocks : 0) : n, upto = OF_BLOCKS ? at + prefix_sum(width) : slots_upto;
+        const uint64_t found = __ballot(work.blocks > 0 && wanted >= upto - width && wanted < upto);
         if (found != 0) {
             const int l = __builtin_ctzll(found);
             f.b = base + l;
-            f.slot = __builtin_amdgcn_readlane(upto - n, l);
+            f.at = __builtin_amdgcn_readlane(upto - width, l);
             f.splits = __builtin_amdgcn_readlane(splits, l);
             f.partial = __builtin_amdgcn_readlane(part_upto - part, l);
             f.seq.first = __builtin_amdgcn_readlane(seq.first, l);
@@ -104,11 +119,12 @@ template <int BLOCK, int TILE, class Hit> __device__ __forceinline__ Found find_
             f.seq.len = __builtin_amdgcn_readlane(seq.len, l);
             f.work.blocks = __builtin_amdgcn_readlane(work.blocks, l);
             f.work.tiles = __builtin_amdgcn_readlane(work.tiles, l);
-            if (!paged_fits(plan, f.work, f.splits, f.slot, f.partial)) f.b = -1;
+            if (!paged_fits(plan, f.work, f.splits, __builtin_amdgcn_readlane(slots_upto - n, l), f.partial)) f.b = -1;
             return f;
         }
-        slots = __builtin_amdgcn_readlane(upto, 63);
+        slots = __builtin_amdgcn_readlane(slots_upto, 63);
         partials = __builtin_amdgcn_readlane(part_upto, 63);
+        if constexpr (OF_BLOCKS) at = __builtin_amdgcn_readlane(upto, 63);
     }
     return f;
 }
@@ -190,9 +206,9 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, G = lane >> 4;
     const int slot = divide(blockIdx.x, p.nkv, p.nkv_m), kvh = blockIdx.x - slot * p.nkv;
-    const Found f = find_work<kRowBlock, kRowTile>(p, p.rows, p.share_m[0], [&](int first, int n, int, int) { return slot >= first && slot < first + n; });
+    const Found f = find_work<kRowBlock, kRowTile, false>(p, p.rows, p.share_m[0], slot);
     if (f.b < 0) return;
-    const int in = slot - f.slot, split = paged_quotient(in, f.work.blocks), block = in - split * f.work.blocks;
+    const int in = slot - f.at, split = paged_quotient(in, f.work.blocks), block = in - split * f.work.blocks;
     int s0, s1;
     paged_split_keys<kRowTile>(f.seq, f.work, f.splits, split, s0, s1);
     const int n_rows = min(kRowBlock, f.seq.n * p.n_rep - block * kRowBlock);
@@ -329,10 +345,12 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
     for (int it = 0; n_iter > 0;) {
         if (it + 1 - ids_from >= 64) look_up(it + 1);
         request(rb, it + 1);
+        __builtin_amdgcn_sched_barrier(0);                 // under way before the wait for the chunk in front of it
         process_chunk(ra, it);
         if (++it >= n_iter) break;
         if (it + 1 - ids_from >= 64) look_up(it + 1);
         request(ra, it + 1);
+        __builtin_amdgcn_sched_barrier(0);
         process_chunk(rb, it);
         if (++it >= n_iter) break;
     }
@@ -449,9 +467,9 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63, l32 = lane & 31, g = lane >> 5;
     const int slot = divide(blockIdx.x, p.nkv, p.nkv_m), kvh = blockIdx.x - slot * p.nkv;
-    const Found f = find_work<kTileRows, kTileKeys>(p, p.tiles, p.share_m[1], [&](int first, int n, int, int) { return slot >= first && slot < first + n; });
+    const Found f = find_work<kTileRows, kTileKeys, false>(p, p.tiles, p.share_m[1], slot);
     if (f.b < 0) return;                                   // the same for the whole workgroup
-    const int in = slot - f.slot, split = paged_quotient(in, f.work.blocks), block = f.work.blocks - 1 - (in - split * f.work.blocks);      // longest first
+    const int in = slot - f.at, split = paged_quotient(in, f.work.blocks), block = f.work.blocks - 1 - (in - split * f.work.blocks);      // longest first
     int s0, s1;
     paged_split_keys<kTileKeys>(f.seq, f.work, f.splits, split, s0, s1);
 
@@ -668,80 +686,96 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
 }
 
 // ---- merge of the splits ------------------------------------------------------------------------------------------------------------------------------
-// A workgroup looks at partial result blockIdx.x of a KV head; that of a first split stands for its block of rows, of which it merges 16 (blockIdx.z-th),
-// a wavefront one after the other with two features to a lane.  `kind` 0: of paged_rows, 1: of paged_tiles.
-constexpr int kMergeWaves = 4;
-template <int D>
-__global__ __launch_bounds__(64 * kMergeWaves) void paged_merge_kernel(const PagedParams p, int kind) {
-    constexpr int kRows[2] = {kRowBlock, kTileRows};
-    const int block_rows = kRows[kind];
-    const float *from_o = kind ? p.tiles_o : p.rows_o, *from_ml = kind ? p.tiles_ml : p.rows_ml;
-    const int partial = blockIdx.x, kvh = blockIdx.y, d = 2 * (threadIdx.x & 63);
-    const auto holds = [&](int, int, int first, int n) { return partial >= first && partial < first + n; };
-    const Found f = kind ? find_work<kTileRows, kTileKeys>(p, p.tiles, p.share_m[1], holds) : find_work<kRowBlock, kRowTile>(p, p.rows, p.share_m[0], holds);
-    const int block = partial - f.partial;
-    if (f.b < 0 || block >= f.work.blocks) return;
-    const int64_t step = (int64_t)f.work.blocks * p.nkv * block_rows;
-    for (int in = 16 * blockIdx.z + (threadIdx.x >> 6); in < 16 * ((int)blockIdx.z + 1); in += kMergeWaves) {
-        const int row = block * block_rows + in;
-        if (row >= f.seq.n * p.n_rep) return;
-        const int64_t first = ((int64_t)partial * p.nkv + kvh) * block_rows + in;
-        float M = -INFINITY, L = 0.f, O0 = 0.f, O1 = 0.f;
+// A row's partial results of splits partial, partial + step, ... by 16 lanes with D / 16 features each, 2 (i + 16 k) and the next for k = 0, 1, ...; those
+// of eight splits are requested before the first is used.
+template <int D> struct RowSum {
+    static constexpr int kPairs = D / 32;
+    float M = -INFINITY, L = 0.f;
+    float2 O[kPairs];
+    __device__ __forceinline__ void add(const float* from_o, const float* from_ml, int64_t first, int64_t step, int splits) {
         constexpr int kStep = 8;
-        for (int s0 = 0; s0 < f.splits; s0 += kStep) {
-            float2 ml[kStep], o[kStep];
+        const int lane = threadIdx.x & 15;
 #pragma unroll
-            for (int i = 0; i < kStep; ++i) {              // past the last split: its values again, with no weight below
-                const int64_t at = first + min(s0 + i, f.splits - 1) * step;
+        for (int k = 0; k < kPairs; ++k) O[k] = make_float2(0.f, 0.f);
+        for (int s0 = 0; s0 < splits; s0 += kStep) {
+            float2 ml[kStep], o[kStep][kPairs];
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {              // past the last split: its values again, without effect below
+                const int64_t at = first + min(s0 + i, splits - 1) * step;
                 ml[i] = *reinterpret_cast<const float2*>(from_ml + at * 2);
-                o[i] = d < D ? *reinterpret_cast<const float2*>(from_o + at * D + d) : make_float2(0.f, 0.f);
-                if (s0 + i >= f.splits) o[i] = make_float2(0.f, 0.f);      // (no weight would not do for an infinite output)
+#pragma unroll
+                for (int k = 0; k < kPairs; ++k) o[i][k] = *reinterpret_cast<const float2*>(from_o + at * D + 2 * (lane + 16 * k));
             }
             float m = M;
 #pragma unroll
             for (int i = 0; i < kStep; ++i) m = fmaxf(m, ml[i].x);
             const float a = M == -INFINITY ? 0.f : fast_exp2(M - m);
-            L *= a; O0 *= a; O1 *= a;
+            L *= a;
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) { O[k].x *= a; O[k].y *= a; }
             M = m;
 #pragma unroll
             for (int i = 0; i < kStep; ++i) {
-                const float w = s0 + i >= f.splits || ml[i].x == -INFINITY ? 0.f : fast_exp2(ml[i].x - M);
+                if (s0 + i >= splits) break;               // (no weight would not do for an infinite output)
+                const float w = ml[i].x == -INFINITY ? 0.f : fast_exp2(ml[i].x - M);
                 L += w * ml[i].y;
-                O0 += w * o[i].x;
-                O1 += w * o[i].y;
+#pragma unroll
+                for (int k = 0; k < kPairs; ++k) { O[k].x += w * o[i][k].x; O[k].y += w * o[i][k].y; }
             }
         }
-        if (d < D) {
-            const int token = divide(row, p.n_rep, p.rep_m);
-            const float inv = L == 0.f ? 0.f : 1.f / L;
-            *reinterpret_cast<uint32_t*>(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh + d) =
-                pack_elem2(O0 * inv, O1 * inv);
-        }
     }
+    __device__ __forceinline__ void store(elem_t* row) const {
+        const int lane = threadIdx.x & 15;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) *reinterpret_cast<uint32_t*>(row + 2 * (lane + 16 * k)) = pack_elem2(O[k].x * inv, O[k].y * inv);
+    }
+};
+
+// A workgroup per (split block, KV head, 16 rows of the block).  KIND 0: of paged_rows, 1: of paged_tiles.  (Two lanes to a pair of features and rows one after the
+// other, with a workgroup for every partial result, most of them idle: 19 us for 64 blocks of 256 rows in four splits.)
+template <int D, int KIND>
+__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
+    constexpr int kRows = KIND ? kTileRows : kRowBlock;
+    const Found f = KIND ? find_work<kTileRows, kTileKeys, true>(p, p.tiles, p.share_m[1], blockIdx.x) : find_work<kRowBlock, kRowTile, true>(p, p.rows, p.share_m[0], blockIdx.x);
+    const int block = (int)blockIdx.x - f.at, kvh = blockIdx.y, in = 16 * blockIdx.z + (threadIdx.x >> 4), row = block * kRows + in;
+    if (f.b < 0 || row >= f.seq.n * p.n_rep) return;
+    RowSum<D> sum;
+    sum.add(KIND ? p.tiles_o : p.rows_o, KIND ? p.tiles_ml : p.rows_ml, ((int64_t)(f.partial + block) * p.nkv + kvh) * kRows + in, (int64_t)f.work.blocks * p.nkv * kRows, f.splits);
+    const int token = divide(row, p.n_rep, p.rep_m);
+    sum.store(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh);
 }
 
-template <int D> int launch(const PagedParams& p, int64_t row_slots, int64_t tile_slots, hipStream_t st) {
-    if (row_slots > 0) {
-        paged_rows_kernel<D><<<dim3((unsigned)(row_slots * p.nkv)), dim3(64 * kRowWaves), 0, st>>>(p);
+template <int D> int launch(const PagedParams& p, int64_t row_blocks, int64_t tile_blocks, hipStream_t st) {
+    if (row_blocks > 0) {
+        paged_rows_kernel<D><<<dim3((unsigned)p.rows.max_slots * p.nkv), dim3(64 * kRowWaves), 0, st>>>(p);
         if (const int rc = mi_check_launch("paged_rows"); rc != MI_OK) return rc;
     }
-    if (tile_slots > 0) {
-        paged_tiles_kernel<D><<<dim3((unsigned)(tile_slots * p.nkv)), dim3(512), 0, st>>>(p);
+    if (tile_blocks > 0) {
+        paged_tiles_kernel<D><<<dim3((unsigned)p.tiles.max_slots * p.nkv), dim3(512), 0, st>>>(p);
         if (const int rc = mi_check_launch("paged_tiles"); rc != MI_OK) return rc;
     }
-    if (p.rows.max_partials > 0) paged_merge_kernel<D><<<dim3(p.rows.max_partials, p.nkv, kRowBlock / 16), dim3(64 * kMergeWaves), 0, st>>>(p, 0);
-    if (p.tiles.max_partials > 0) paged_merge_kernel<D><<<dim3(p.tiles.max_partials, p.nkv, kTileRows / 16), dim3(64 * kMergeWaves), 0, st>>>(p, 1);
+    const auto rows_of = [&](const PagedPlan& plan, int block) {          // of the longest sequence that there may be, in sixteens
+        const int64_t rows = std::min<int64_t>((int64_t)plan.max_n * p.n_rep, std::min(plan.rows_up_to, block));
+        return (unsigned)((rows + 15) / 16);
+    };
+    if (p.rows.share > 0) paged_merge_kernel<D, 0><<<dim3((unsigned)paged_max_split_blocks(p.rows, row_blocks), p.nkv, rows_of(p.rows, kRowBlock)), dim3(256), 0, st>>>(p);
+    if (p.tiles.share > 0) paged_merge_kernel<D, 1><<<dim3((unsigned)paged_max_split_blocks(p.tiles, tile_blocks), p.nkv, rows_of(p.tiles, kTileRows)), dim3(256), 0, st>>>(p);
     return mi_check_launch("paged_merge");
 }
 
-// Workgroups per KV head that either kernel's work is cut for.
-int share_of(int workgroups, int nkv) { return workgroups / nkv > 0 ? workgroups / nkv : 1; }
-void make_plans(int64_t tokens, int n_rep, int nkv, PagedPlan& rows, PagedPlan& tiles) {
+// Workgroups per KV head that either kernel's work is cut for.  `items`: blocks of rows x KV heads of the calls, as many as there may be.
+// paged_rows, of which two to four share a compute unit: where items are many, lengths differ and small pieces keep the units even; where they are few, more
+// splits of each only make the merge longer.  (Kernel / merge, us, of 512, 1024, 2048 workgroups: 32 x 8 items of 200 - 8192 keys 98.9 / 4.4, 89.5 / 5.2, 85 /
+// 7.5; 3 x 4 items of 20000 - 32768 keys of 64 features 18.6 / 7.5, 19.2 / 12.7, 19.3 / 18.7.)
+constexpr int kRowsLeast = 2, kRowsMost = 8;             // per compute unit
+int share_of(int64_t workgroups, int nkv) { return workgroups / nkv > 0 ? (int)(workgroups / nkv) : 1; }
+void make_plans(int64_t tokens, int64_t items, int n_rep, int nkv, PagedPlan& rows, PagedPlan& tiles) {
     const int cus = mi_compute_units();
-    rows = PagedPlan{0, kRowLimit, 0x7fffffff, share_of(4 * cus, nkv), 0, 0};
+    rows = PagedPlan{0, kRowLimit, 0x7fffffff, share_of(std::clamp<int64_t>(8 * items, kRowsLeast * cus, kRowsMost * cus), nkv), 0, 0, 0};
     // Enough blocks for every compute unit: no splits, no merge.
     const bool many = tokens * n_rep / kTileRows * nkv >= cus;
-    tiles = PagedPlan{kRowLimit, 0x7fffffff, 0x7fffffff, many ? 0 : share_of(cus, nkv), 0, 0};
+    tiles = PagedPlan{kRowLimit, 0x7fffffff, 0x7fffffff, many ? 0 : share_of(cus, nkv), 1, 0, 0};
 }
 
 size_t partial_bytes(int64_t partials, int nkv, int block_rows, int head_dim) { return (size_t)partials * nkv * block_rows * (size_t)(head_dim + 2) * sizeof(float); }
@@ -754,7 +788,7 @@ extern "C" size_t mi_paged_attn_workspace_bytes(int64_t tokens, int32_t n_q_head
     if (tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || head_dim <= 0) return 0;
     PagedPlan rows, tiles;
     const int n_rep = n_q_heads / n_kv_heads;
-    make_plans(0, n_rep, n_kv_heads, rows, tiles);         // for so many tokens or fewer
+    make_plans(0, 0x7fffffff, n_rep, n_kv_heads, rows, tiles);         // for so many tokens or fewer, of any number of sequences
     return partial_bytes(paged_max_partials(rows, kMaxTiles, kMaxTiles), n_kv_heads, kRowBlock, head_dim) +
            (tokens * n_rep > kRowLimit ? partial_bytes(paged_max_partials(tiles, kMaxTiles, kMaxTiles), n_kv_heads, kTileRows, head_dim) : 0);
 }
@@ -784,7 +818,7 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
     p.capacity = a->max_pages * a->page_size; p.nq = a->n_q_heads; p.nkv = a->n_kv_heads; p.n_rep = a->n_q_heads / a->n_kv_heads; p.causal = a->causal != 0;
     p.page_m = divide_m(p.page); p.rep_m = divide_m(p.n_rep); p.nkv_m = divide_m(p.nkv);
     p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
-    make_plans(p.total, p.n_rep, p.nkv, p.rows, p.tiles);
+    make_plans(p.total, std::min<int64_t>(p.batch, p.total) * p.nkv, p.n_rep, p.nkv, p.rows, p.tiles);
     const int64_t longest = a->max_q_len > 0 && a->max_q_len < p.total ? a->max_q_len : p.total;
     p.rows.max_n = p.tiles.max_n = (int)longest;
     const int64_t row_blocks = paged_max_blocks<kRowBlock>(p.rows, p.total, p.batch, longest, p.n_rep);
@@ -810,12 +844,11 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
     p.rows_ml = p.rows_o + (size_t)p.rows.max_partials * p.nkv * kRowBlock * a->head_dim;
     p.tiles_o = p.rows_o + partial_bytes(p.rows.max_partials, p.nkv, kRowBlock, a->head_dim) / sizeof(float);
     p.tiles_ml = p.tiles_o + (size_t)p.tiles.max_partials * p.nkv * kTileRows * a->head_dim;
-    const int64_t row_slots = p.rows.max_slots, tile_slots = p.tiles.max_slots;
     const hipStream_t st = (hipStream_t)a->stream;
     switch (a->head_dim) {
-        case 32: return launch<32>(p, row_slots, tile_slots, st);
-        case 64: return launch<64>(p, row_slots, tile_slots, st);
-        case 96: return launch<96>(p, row_slots, tile_slots, st);
-        default: return launch<128>(p, row_slots, tile_slots, st);
+        case 32: return launch<32>(p, row_blocks, tile_blocks, st);
+        case 64: return launch<64>(p, row_blocks, tile_blocks, st);
+        case 96: return launch<96>(p, row_blocks, tile_blocks, st);
+        default: return launch<128>(p, row_blocks, tile_blocks, st);
     }
 }

@@ -58,6 +58,7 @@ struct PagedPlan {
     int rows_over, rows_up_to;    // sequences with more than rows_over and at most rows_up_to rows
     int max_n;                    // ... and at most so many new tokens
     int share;                    // workgroups per KV head aimed at; 0: never split
+    int fit;                      // whether a workgroup has a compute unit for itself, and more of them than that are to be avoided
     int max_slots, max_partials;  // (set by the host) workgroups and partial results per KV head that there are
 };
 
@@ -74,9 +75,17 @@ template <int BLOCK, int TILE> MI_PLAN_FN PagedWork paged_work(const PagedPlan& 
 }
 // tiles of a split; `units` is W
 MI_PLAN_FN int paged_split_tiles(const PagedPlan& p, int64_t units) {
-    if (p.share == 0) return 0x7fffff;                      // no sequence has more
+    if (p.share == 0) return 0x1000000;                    // no sequence has more
     const uint32_t u = (uint32_t)(units < 0x7fffffff ? units : 0x7fffffff);
     return (int)(u / (uint32_t)p.share) + 1;
+}
+// Where all blocks together fit, S grows until their splits do too: one workgroup more than there is room for at once would take as long as all others.
+// `slots`: splits of all blocks at S.  S / slots only shrinks towards the room, so a few steps do.
+constexpr int kPagedSteps = 3;
+MI_PLAN_FN int paged_next_tiles(const PagedPlan& p, int split_tiles, int64_t blocks, int64_t slots) {
+    if (!p.fit || blocks > p.share || slots <= p.share) return split_tiles;
+    const int64_t next = (int64_t)((float)split_tiles * (float)slots / (float)p.share);
+    return paged_clamp(next > split_tiles ? next : (int64_t)split_tiles + 1, 1, 0x1000000);
 }
 MI_PLAN_FN int paged_splits(const PagedWork& w, int split_tiles) { return paged_quotient(w.tiles - 1, split_tiles) + 1; }
 // keys [k0, k1) of split i
@@ -107,6 +116,8 @@ MI_PLAN_FN int64_t paged_max_slots(const PagedPlan& p, int64_t blocks, int64_t m
     const int64_t each = blocks * max_tiles, together = blocks + p.share + 1;
     return p.share == 0 || blocks == 0 ? blocks : each < together ? each : together;
 }
+// blocks of sequences with more than one split
+MI_PLAN_FN int64_t paged_max_split_blocks(const PagedPlan& p, int64_t blocks) { return p.share == 0 ? 0 : blocks < p.share + 1 ? blocks : p.share + 1; }
 MI_PLAN_FN int64_t paged_max_partials(const PagedPlan& p, int64_t blocks, int64_t max_tiles) {
     if (p.share == 0) return 0;
     const int64_t each = blocks * max_tiles, together = 2 * (int64_t)p.share + 2;

@@ -21,19 +21,31 @@ static int fail(const char* what, int i) { printf("case %%d: %%s\n", i, what); r
 template <int BLOCK, int TILE>
 static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, int capacity, int longest, bool good, bool causal, const std::vector<int>& cu,
                   const std::vector<int>& ctx, std::vector<int>& taken) {
-    PagedPlan p = {over, up_to, longest, rnd() %% 4 == 0 ? 0 : 1 << rnd() %% 9, 0, 0};
+    PagedPlan p = {over, up_to, longest, rnd() %% 4 == 0 ? 0 : 1 << rnd() %% 9, (int)(rnd() & 1), 0, 0};
     const int max_tiles = (capacity + TILE - 1) / TILE;
     const int64_t most = paged_max_blocks<BLOCK>(p, total, batch, longest, n_rep);
     p.max_slots = (int)paged_max_slots(p, most, max_tiles);
     p.max_partials = (int)paged_max_partials(p, most, max_tiles);
-    int64_t units = 0, slots = 0, partials = 0, blocks = 0;
+    int64_t units = 0, slots = 0, partials = 0, blocks = 0, split_blocks = 0;
     for (int b = 0; b < batch; ++b) {
         const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity);
         if (s.first < 0 || s.n < 0 || s.first + s.n > total || s.len < 0 || s.len > capacity) return fail("a sequence outside the tokens or the table", c);
         const PagedWork w = paged_work<BLOCK, TILE>(p, s, n_rep);
         units += (int64_t)w.blocks * w.tiles;
     }
-    const int S = paged_split_tiles(p, units);
+    int S = paged_split_tiles(p, units);
+    int64_t all = 0;
+    for (int b = 0; b < batch; ++b) all += paged_work<BLOCK, TILE>(p, paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity), n_rep).blocks;
+    for (int step = 0; p.share > 0 && step < kPagedSteps; ++step) {
+        int64_t n = 0;
+        for (int b = 0; b < batch; ++b) {
+            const PagedWork w = paged_work<BLOCK, TILE>(p, paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity), n_rep);
+            n += (int64_t)w.blocks * paged_splits(w, S);
+        }
+        const int next = paged_next_tiles(p, S, all, n);
+        if (next < S || ((next == S) != (!p.fit || all > p.share || n <= p.share))) return fail("tiles of a split do not grow", c);
+        S = next;
+    }
     if (S < 1) return fail("no tiles to a split", c);
     for (int b = 0; b < batch; ++b) {
         const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity);
@@ -45,7 +57,7 @@ static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, i
         if (fits && w.blocks > 0 && slots + (int64_t)w.blocks * splits > p.max_slots) return fail("a workgroup that is not there", c);
         blocks += w.blocks;
         slots += (int64_t)w.blocks * splits;
-        if (splits > 1) partials += (int64_t)w.blocks * splits;
+        if (splits > 1) { partials += (int64_t)w.blocks * splits; split_blocks += w.blocks; }
         if (fits && splits > 1 && w.blocks > 0 && partials > p.max_partials) return fail("a partial result outside the workspace", c);
         if (w.blocks > 0 && good) for (int i = 0; i < s.n; ++i) ++taken[s.first + i];
         int at = 0;
@@ -63,7 +75,7 @@ static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, i
         }
     }
     if (good && (blocks > most || (blocks == 0) < (most == 0))) return fail("more blocks than the bound", c);
-    if (good && (slots > p.max_slots || partials > p.max_partials)) return fail("more workgroups or partial results than the bound", c);
+    if (good && (slots > p.max_slots || partials > p.max_partials || split_blocks > paged_max_split_blocks(p, most))) return fail("more workgroups or partial results than the bound", c);
     return 0;
 }
 int main() {
