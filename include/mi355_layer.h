@@ -367,6 +367,9 @@ int mi_paged_append(const mi_paged_append_args* args);
  * max_q_len: an upper bound of the new tokens of a sequence, 0 if unknown (the launches for longer ones are then made too; sequences over the bound may be
  * left out).  Lengths beyond the page table count its room; a page number outside the cache reads the nearest page inside.
  * workspace: mi_paged_attn_workspace_bytes() bytes for calls of up to `tokens` tokens, 16-byte aligned, one call at a time; nothing in it has to be cleared.
+ * tickets: mi_paged_attn_tickets() int32 of device memory, all zero before the first call, which every call leaves zero: with them the splits of sequences
+ * with few new rows are merged in the launch that computes them instead of by one more, to the same bits.  They belong to one call at a time as the workspace does, and
+ * unlike it outlive a mistake: after calls that overlapped on them, later ones merge too early or never until they are cleared.
  * The key axis is cut by the lengths on the device, so that the work of a ragged batch is even; the order of the sums depends on the lengths of all
  * sequences of the call, and on nothing else.
  * Algorithmic work: 4 * head_dim * n_q_heads * pairs flop; HBM bytes 2 * sum ctx_len * n_kv_heads * head_dim * e + 2 * total_q * n_q_heads * head_dim * e. */
@@ -387,8 +390,11 @@ typedef struct mi_paged_attn_args {
     float softmax_scale;
     void* workspace;
     size_t workspace_bytes;
+    int32_t* tickets;              /* or NULL */
+    int64_t n_tickets;
     void* stream;
 } mi_paged_attn_args;
+int64_t mi_paged_attn_tickets(int32_t n_kv_heads);
 size_t mi_paged_attn_workspace_bytes(int64_t tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim);
 int mi_paged_attn(const mi_paged_attn_args* args);
 

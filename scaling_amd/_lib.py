@@ -28,7 +28,7 @@ EXPORTS = (
     "mi_attn_fwd", "mi_attn_bwd_workspace_bytes", "mi_attn_bwd_workspace_bytes_kv", "mi_attn_bwd_workspace_bytes_for", "mi_attn_bwd",
     "mi_gemm", "mi_gemm_workspace_bytes", "mi_gemm_with_workspace", "mi_rows_product", "mi_transpose16", "mi_column_sum", "mi_add_rmsnorm_bwd", "mi_add_layernorm_fwd", "mi_add_layernorm_bwd", "mi_attn_decode_workspace_bytes", "mi_attn_decode", "mi_attn_decode_with_tickets", "mi_fill_cache", "mi_attn_decode_static_scratch_bytes", "mi_attn_decode_static",
     "mi_norm_rotary_fwd", "mi_norm_rotary_bwd_workspace_bytes", "mi_norm_rotary_bwd", "mi_paged_append",
-    "mi_paged_attn_workspace_bytes", "mi_paged_attn",
+    "mi_paged_attn_workspace_bytes", "mi_paged_attn_tickets", "mi_paged_attn",
 )
 
 
@@ -144,7 +144,8 @@ class MiPagedAttnArgs(Structure):
         ("o_stride_head", c_int64), ("page_stride", c_int64), ("page_stride_token", c_int64), ("page_stride_head", c_int64),
         ("page_table_stride", c_int64), ("batch", c_int32), ("n_pages", c_int32), ("page_size", c_int32), ("max_pages", c_int32),
         ("n_q_heads", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32), ("dtype", c_int32), ("causal", c_int32), ("max_q_len", c_int32),
-        ("softmax_scale", c_float), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("stream", c_void_p),
+        ("softmax_scale", c_float), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("tickets", c_void_p), ("n_tickets", c_int64),
+        ("stream", c_void_p),
     ]
 
 
@@ -239,6 +240,8 @@ def _declare(lib):
     lib.mi_paged_append.argtypes = [POINTER(MiPagedAppendArgs)]
     lib.mi_paged_attn_workspace_bytes.restype = c_size_t
     lib.mi_paged_attn_workspace_bytes.argtypes = [c_int64, c_int32, c_int32, c_int32]
+    lib.mi_paged_attn_tickets.restype = c_int64
+    lib.mi_paged_attn_tickets.argtypes = [c_int32]
     lib.mi_paged_attn.restype = c_int
     lib.mi_paged_attn.argtypes = [POINTER(MiPagedAttnArgs)]
     lib.mi_attn_fwd.restype = c_int

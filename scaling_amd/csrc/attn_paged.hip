@@ -34,6 +34,7 @@ struct PagedParams {
     uint32_t page_m, rep_m, nkv_m, share_m[2];        // for divide(); share_m: of rows and tiles
     float scale_log2;
     PagedPlan rows, tiles;
+    int32_t* tickets;                                 // nullable: arrivals of the splits of paged_rows, [partial][KV head], zero between launches
     float *rows_o, *rows_ml, *tiles_o, *tiles_ml;     // partial results: [partial][KV head][row of the block][feature], and (maximum in log2 units, sum)
 };
 
@@ -138,6 +139,103 @@ __device__ __forceinline__ int page_of(const PagedParams& p, const int32_t* tabl
 __device__ __forceinline__ int row_in_page(const PagedParams& p, int group) {
     const int key = group * 16;
     return key - divide((uint32_t)key, p.page, p.page_m) * p.page;
+}
+
+// ---- partial results ----------------------------------------------------------------------------------------------------------------------------------
+// SHARED: between workgroups of one launch, past the L2s (those of the XCDs are not coherent).
+template <bool SHARED> __device__ __forceinline__ float2 load_partial(const float* at) {
+    if constexpr (!SHARED) return *reinterpret_cast<const float2*>(at);
+    const uint64_t x = __hip_atomic_load(reinterpret_cast<const uint64_t*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)));
+}
+__device__ __forceinline__ void store_partial(float* at, float a, float b, bool shared) {
+    if (shared) __hip_atomic_store(reinterpret_cast<uint64_t*>(at), (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else *reinterpret_cast<float2*>(at) = make_float2(a, b);
+}
+
+// A row's partial results of `splits` splits, `step` rows of results apart, by 16 lanes with D / 16 features each, 2 (i + 16 k) and the next for
+// k = 0, 1, ...; those of eight splits are requested before the first is used.
+template <int D> struct RowSum {
+    static constexpr int kPairs = D / 32;
+    float M = -INFINITY, L = 0.f;
+    float2 O[kPairs];
+    __device__ __forceinline__ RowSum() {
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) O[k] = make_float2(0.f, 0.f);
+    }
+    // N more results, the first `there` of them
+    template <int N> __device__ __forceinline__ void add(const float2 (&ml)[N], const float2 (&o)[N][kPairs], int there) {
+        float m = M;
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = fmaxf(m, i < there ? ml[i].x : -INFINITY);
+        const float a = M == -INFINITY ? 0.f : fast_exp2(M - m);
+        L *= a;
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) { O[k].x *= a; O[k].y *= a; }
+        M = m;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (i >= there) break;                         // (no weight would not do for an infinite output)
+            const float w = ml[i].x == -INFINITY ? 0.f : fast_exp2(ml[i].x - M);
+            // (named: of two products in a sum the compiler takes either into the fma, and both launches that merge have to leave the same bits)
+            L = __builtin_fmaf(w, ml[i].y, L);
+#pragma unroll
+            for (int k = 0; k < kPairs; ++k) {
+                O[k].x = __builtin_fmaf(w, o[i][k].x, O[k].x);
+                O[k].y = __builtin_fmaf(w, o[i][k].y, O[k].y);
+            }
+        }
+    }
+    template <bool SHARED> __device__ __forceinline__ void add(const float* from_o, const float* from_ml, int64_t first, int64_t step, int splits) {
+        constexpr int kStep = 8;
+        const int lane = threadIdx.x & 15;
+        for (int s0 = 0; s0 < splits; s0 += kStep) {
+            float2 ml[kStep], o[kStep][kPairs];
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {              // past the last split: its values again
+                const int64_t at = first + min(s0 + i, splits - 1) * step;
+                ml[i] = load_partial<SHARED>(from_ml + at * 2);
+#pragma unroll
+                for (int k = 0; k < kPairs; ++k) o[i][k] = load_partial<SHARED>(from_o + at * D + 2 * (lane + 16 * k));
+            }
+            add(ml, o, splits - s0);
+        }
+    }
+    __device__ __forceinline__ void store(elem_t* row) const {
+        const int lane = threadIdx.x & 15;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+        for (int k = 0; k < kPairs; ++k) *reinterpret_cast<uint32_t*>(row + 2 * (lane + 16 * k)) = pack_elem2(O[k].x * inv, O[k].y * inv);
+    }
+};
+
+// Block `block` of few rows, its splits merged by 256 threads: 16 / rows groups of 16 lanes to a row, a share of the splits each, together through LDS.
+template <int D, bool SHARED> __device__ __forceinline__ void merge_rows(const PagedParams& p, const Found& f, int block, int kvh, float* lds) {
+    const int n_rows = min(kRowBlock, f.seq.n * p.n_rep - block * kRowBlock), group = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    int per_row = 16;                                      // groups to a row
+    while (per_row * n_rows > 16) per_row /= 2;
+    const int r = group / per_row, part = group - r * per_row;
+    RowSum<D> sum;
+    if (r < n_rows && part < f.splits) {
+        const int64_t step = (int64_t)f.work.blocks * p.nkv * kRowBlock, first = ((int64_t)(f.partial + block) * p.nkv + kvh) * kRowBlock + r;
+        sum.template add<SHARED>(p.rows_o, p.rows_ml, first + part * step, step * per_row, (f.splits - part + per_row - 1) / per_row);
+    }
+    float* mine = lds + group * (D + 2);
+    if (lane == 0) { mine[0] = sum.M; mine[1] = sum.L; }
+#pragma unroll
+    for (int k = 0; k < RowSum<D>::kPairs; ++k) *reinterpret_cast<float2*>(mine + 2 + 2 * (lane + 16 * k)) = sum.O[k];
+    __syncthreads();
+    if (part != 0 || r >= n_rows) return;
+    for (int i = 1; i < per_row; ++i) {
+        const float* other = mine + i * (D + 2);
+        float2 ml[1], o[1][RowSum<D>::kPairs];
+        ml[0] = make_float2(other[0], other[1]);
+#pragma unroll
+        for (int k = 0; k < RowSum<D>::kPairs; ++k) o[0][k] = *reinterpret_cast<const float2*>(other + 2 + 2 * (lane + 16 * k));
+        sum.add(ml, o, 1);
+    }
+    const int row = block * kRowBlock + r, token = divide(row, p.n_rep, p.rep_m);
+    sum.store(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh);
 }
 
 // ---- rows whose products met values that are not finite -----------------------------------------------------------------------------------------------
@@ -372,8 +470,8 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
             *reinterpret_cast<uint32_t*>(p.o + (int64_t)(f.seq.first + i) * p.o_st + (int64_t)(kvh * p.n_rep + rr - i * p.n_rep) * p.o_sh + d) = pack_elem2(O0 * inv, O1 * inv);
         } else {
             const int64_t at = ((int64_t)(f.partial + in) * p.nkv + kvh) * kRowBlock + r;
-            *reinterpret_cast<float2*>(p.rows_o + at * D + d) = make_float2(O0, O1);
-            if (d == 0) *reinterpret_cast<float2*>(p.rows_ml + at * 2) = make_float2(M, L);
+            store_partial(p.rows_o + at * D + d, O0, O1, p.tickets != nullptr);
+            if (d == 0) store_partial(p.rows_ml + at * 2, M, L, p.tickets != nullptr);
         }
     };
     for (int idx = tid; idx < n_rows * (D / 2); idx += kThreads) {
@@ -392,16 +490,34 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
         if (not_finite(O0) || not_finite(O1) || not_finite(L)) redo_lds[r] = 1;
         emit(r, d, M, L, O0, O1);
     }
-    if (__ballot(l16 < n_rows && limit < filled) == 0) return;     // the same for the workgroup
-    __syncthreads();
-    for (int r = wave; r < n_rows; r += NWV) {
-        const int lim = __builtin_amdgcn_readlane(limit, r);
-        if (redo_lds[r] == 0 || lim >= filled) continue;
-        const int rr = block * kRowBlock + r, i = divide(rr, p.n_rep, p.rep_m);
-        float M, L, O0, O1;
-        own_keys_only<D>(p, table, kvh, p.q + (int64_t)(f.seq.first + i) * p.q_st + (int64_t)(kvh * p.n_rep + rr - i * p.n_rep) * p.q_sh, s0, lim, M, L, O0, O1);
-        if (2 * lane < D) emit(r, 2 * lane, M, L, O0, O1);
+    if (__ballot(l16 < n_rows && limit < filled) != 0) {   // the same for the workgroup
+        __syncthreads();
+        for (int r = wave; r < n_rows; r += NWV) {
+            const int lim = __builtin_amdgcn_readlane(limit, r);
+            if (redo_lds[r] == 0 || lim >= filled) continue;
+            const int rr = block * kRowBlock + r, i = divide(rr, p.n_rep, p.rep_m);
+            float M, L, O0, O1;
+            own_keys_only<D>(p, table, kvh, p.q + (int64_t)(f.seq.first + i) * p.q_st + (int64_t)(kvh * p.n_rep + rr - i * p.n_rep) * p.q_sh, s0, lim, M, L, O0, O1);
+            if (2 * lane < D) emit(r, 2 * lane, M, L, O0, O1);
+        }
     }
+    // With tickets the workgroup of a block that is last to get here merges its splits; nobody waits for anybody.  Partial results are stored past the L2 and
+    // every wavefront has waited for its own before the barrier, so the count that thread 0 raises behind it comes after them in memory, and the loads of
+    // the workgroup that reads the highest count come after all.  (Two launches, the second one merging, of 1500 keys of 32 / 8 heads: 11.5 us one call after the
+    // other; 32 sequences of 200 - 8192 keys: 94.)
+    if (f.splits == 1 || p.tickets == nullptr) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (tid == 0) {
+        int32_t* ticket = p.tickets + (int64_t)(f.partial + block) * p.nkv + kvh;
+        const int arrived = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        redo_lds[0] = arrived == f.splits - 1;
+        if (arrived == f.splits - 1) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);     // for the next launch
+    }
+    __syncthreads();
+    if (redo_lds[0] == 0) return;
+    static_assert(NWV == 4 && sizeof(wo_lds) >= 16 * (D + 2) * sizeof(float), "merge_rows: 256 threads, and room in LDS");
+    merge_rows<D, true>(p, f, block, kvh, &wo_lds[0][0][0]);
 }
 
 // ---- chunks -------------------------------------------------------------------------------------------------------------------------------------------
@@ -686,64 +802,24 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
 }
 
 // ---- merge of the splits ------------------------------------------------------------------------------------------------------------------------------
-// A row's partial results of splits partial, partial + step, ... by 16 lanes with D / 16 features each, 2 (i + 16 k) and the next for k = 0, 1, ...; those
-// of eight splits are requested before the first is used.
-template <int D> struct RowSum {
-    static constexpr int kPairs = D / 32;
-    float M = -INFINITY, L = 0.f;
-    float2 O[kPairs];
-    __device__ __forceinline__ void add(const float* from_o, const float* from_ml, int64_t first, int64_t step, int splits) {
-        constexpr int kStep = 8;
-        const int lane = threadIdx.x & 15;
-#pragma unroll
-        for (int k = 0; k < kPairs; ++k) O[k] = make_float2(0.f, 0.f);
-        for (int s0 = 0; s0 < splits; s0 += kStep) {
-            float2 ml[kStep], o[kStep][kPairs];
-#pragma unroll
-            for (int i = 0; i < kStep; ++i) {              // past the last split: its values again, without effect below
-                const int64_t at = first + min(s0 + i, splits - 1) * step;
-                ml[i] = *reinterpret_cast<const float2*>(from_ml + at * 2);
-#pragma unroll
-                for (int k = 0; k < kPairs; ++k) o[i][k] = *reinterpret_cast<const float2*>(from_o + at * D + 2 * (lane + 16 * k));
-            }
-            float m = M;
-#pragma unroll
-            for (int i = 0; i < kStep; ++i) m = fmaxf(m, ml[i].x);
-            const float a = M == -INFINITY ? 0.f : fast_exp2(M - m);
-            L *= a;
-#pragma unroll
-            for (int k = 0; k < kPairs; ++k) { O[k].x *= a; O[k].y *= a; }
-            M = m;
-#pragma unroll
-            for (int i = 0; i < kStep; ++i) {
-                if (s0 + i >= splits) break;               // (no weight would not do for an infinite output)
-                const float w = ml[i].x == -INFINITY ? 0.f : fast_exp2(ml[i].x - M);
-                L += w * ml[i].y;
-#pragma unroll
-                for (int k = 0; k < kPairs; ++k) { O[k].x += w * o[i][k].x; O[k].y += w * o[i][k].y; }
-            }
-        }
-    }
-    __device__ __forceinline__ void store(elem_t* row) const {
-        const int lane = threadIdx.x & 15;
-        const float inv = L == 0.f ? 0.f : 1.f / L;
-#pragma unroll
-        for (int k = 0; k < kPairs; ++k) *reinterpret_cast<uint32_t*>(row + 2 * (lane + 16 * k)) = pack_elem2(O[k].x * inv, O[k].y * inv);
-    }
-};
-
-// A workgroup per (split block, KV head, 16 rows of the block).  KIND 0: of paged_rows, 1: of paged_tiles.  (Two lanes to a pair of features and rows one after the
-// other, with a workgroup for every partial result, most of them idle: 19 us for 64 blocks of 256 rows in four splits.)
+// A workgroup per (split block, KV head, 16 rows of the block).  KIND 0: of paged_rows where the caller has no tickets, 1: of paged_tiles.  (Two lanes to a pair
+// of features and rows one after the other, with a workgroup for every partial result, most of them idle: 19 us for 64 blocks of 256 rows in four splits.)
 template <int D, int KIND>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
-    constexpr int kRows = KIND ? kTileRows : kRowBlock;
-    const Found f = KIND ? find_work<kTileRows, kTileKeys, true>(p, p.tiles, p.share_m[1], blockIdx.x) : find_work<kRowBlock, kRowTile, true>(p, p.rows, p.share_m[0], blockIdx.x);
-    const int block = (int)blockIdx.x - f.at, kvh = blockIdx.y, in = 16 * blockIdx.z + (threadIdx.x >> 4), row = block * kRows + in;
-    if (f.b < 0 || row >= f.seq.n * p.n_rep) return;
-    RowSum<D> sum;
-    sum.add(KIND ? p.tiles_o : p.rows_o, KIND ? p.tiles_ml : p.rows_ml, ((int64_t)(f.partial + block) * p.nkv + kvh) * kRows + in, (int64_t)f.work.blocks * p.nkv * kRows, f.splits);
-    const int token = divide(row, p.n_rep, p.rep_m);
-    sum.store(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh);
+    const int kvh = blockIdx.y;
+    if constexpr (KIND == 0) {
+        __shared__ float lds[16 * (D + 2)];
+        const Found f = find_work<kRowBlock, kRowTile, true>(p, p.rows, p.share_m[0], blockIdx.x);
+        if (f.b >= 0) merge_rows<D, false>(p, f, (int)blockIdx.x - f.at, kvh, lds);
+    } else {
+        const Found f = find_work<kTileRows, kTileKeys, true>(p, p.tiles, p.share_m[1], blockIdx.x);
+        const int block = (int)blockIdx.x - f.at, in = 16 * blockIdx.z + (threadIdx.x >> 4), row = block * kTileRows + in;
+        if (f.b < 0 || row >= f.seq.n * p.n_rep) return;
+        RowSum<D> sum;
+        sum.template add<false>(p.tiles_o, p.tiles_ml, ((int64_t)(f.partial + block) * p.nkv + kvh) * kTileRows + in, (int64_t)f.work.blocks * p.nkv * kTileRows, f.splits);
+        const int token = divide(row, p.n_rep, p.rep_m);
+        sum.store(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh);
+    }
 }
 
 template <int D> int launch(const PagedParams& p, int64_t row_blocks, int64_t tile_blocks, hipStream_t st) {
@@ -755,12 +831,11 @@ template <int D> int launch(const PagedParams& p, int64_t row_blocks, int64_t ti
         paged_tiles_kernel<D><<<dim3((unsigned)p.tiles.max_slots * p.nkv), dim3(512), 0, st>>>(p);
         if (const int rc = mi_check_launch("paged_tiles"); rc != MI_OK) return rc;
     }
-    const auto rows_of = [&](const PagedPlan& plan, int block) {          // of the longest sequence that there may be, in sixteens
-        const int64_t rows = std::min<int64_t>((int64_t)plan.max_n * p.n_rep, std::min(plan.rows_up_to, block));
-        return (unsigned)((rows + 15) / 16);
-    };
-    if (p.rows.share > 0) paged_merge_kernel<D, 0><<<dim3((unsigned)paged_max_split_blocks(p.rows, row_blocks), p.nkv, rows_of(p.rows, kRowBlock)), dim3(256), 0, st>>>(p);
-    if (p.tiles.share > 0) paged_merge_kernel<D, 1><<<dim3((unsigned)paged_max_split_blocks(p.tiles, tile_blocks), p.nkv, rows_of(p.tiles, kTileRows)), dim3(256), 0, st>>>(p);
+    if (p.rows.share > 0 && p.tickets == nullptr) paged_merge_kernel<D, 0><<<dim3((unsigned)paged_max_split_blocks(p.rows, row_blocks), p.nkv), dim3(256), 0, st>>>(p);
+    if (p.tiles.share > 0) {
+        const int64_t rows = std::min<int64_t>((int64_t)p.tiles.max_n * p.n_rep, kTileRows);          // of a block, as many as there may be
+        paged_merge_kernel<D, 1><<<dim3((unsigned)paged_max_split_blocks(p.tiles, tile_blocks), p.nkv, (unsigned)((rows + 15) / 16)), dim3(256), 0, st>>>(p);
+    }
     return mi_check_launch("paged_merge");
 }
 
@@ -784,6 +859,13 @@ constexpr int64_t kMaxTiles = (1 << 24) + 1;              // of a sequence
 }  // namespace
 
 #ifndef MI_ELEM_F16
+extern "C" int64_t mi_paged_attn_tickets(int32_t n_kv_heads) {
+    if (n_kv_heads <= 0) return 0;
+    PagedPlan rows, tiles;
+    make_plans(0, 0x7fffffff, 1, n_kv_heads, rows, tiles);
+    return paged_max_partials(rows, kMaxTiles, kMaxTiles) * n_kv_heads;
+}
+
 extern "C" size_t mi_paged_attn_workspace_bytes(int64_t tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
     if (tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || head_dim <= 0) return 0;
     PagedPlan rows, tiles;
@@ -832,6 +914,9 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
     const size_t need = mi_paged_attn_workspace_bytes(p.total, p.nq, p.nkv, a->head_dim);
     if (!a->workspace || a->workspace_bytes < need || !mi_aligned16(a->workspace))
         return mi_fail(MI_E_WORKSPACE, "paged_attn: workspace needs %zu bytes (16-byte aligned), got %zu", need, a->workspace_bytes);
+    if (a->tickets && (a->n_tickets < mi_paged_attn_tickets(p.nkv) || (reinterpret_cast<uintptr_t>(a->tickets) & 3u) != 0))
+        return mi_fail(MI_E_WORKSPACE, "paged_attn: %lld tickets (4-byte aligned), got %lld", (long long)mi_paged_attn_tickets(p.nkv), (long long)a->n_tickets);
+    p.tickets = a->tickets;
     // A sequence of up to a tile of keys has one split, whatever the plan.
     if (row_tiles == 1 || row_blocks == 0) p.rows.share = 0;
     if (tile_tiles == 1 || tile_blocks == 0) p.tiles.share = 0;

@@ -594,7 +594,7 @@ OptTensor op_paged_append(const OptTensor& q_, const Tensor& k, const Tensor& v,
 }
 
 void op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu, const Tensor& ctx_len, bool causal,
-                        double scale, int64_t max_q_len, const OptTensor& workspace_, const Tensor& out) {
+                        double scale, int64_t max_q_len, const OptTensor& workspace_, const OptTensor& tickets, const Tensor& out) {
     check_head_rows(q, Tensor(), Tensor());
     TORCH_CHECK(out.is_cuda() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device() && out.stride(2) == 1,
                 "paged_attention: out does not match q");
@@ -614,6 +614,11 @@ void op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_
     if (!workspace.defined()) workspace = float_buffer(mi_paged_attn_workspace_bytes(a.total_q, a.n_q_heads, a.n_kv_heads, a.head_dim), q);
     TORCH_CHECK(workspace.device() == q.device() && workspace.is_contiguous(), "paged_attention: the workspace is a contiguous tensor on the device of q");
     a.workspace = ptr(workspace); a.workspace_bytes = (size_t)workspace.numel() * workspace.element_size();
+    if (tickets.has_value() && tickets->scalar_type() == at::kInt && tickets->is_contiguous() && tickets->device() == q.device() &&
+        tickets->numel() >= mi_paged_attn_tickets(a.n_kv_heads)) {
+        a.tickets = static_cast<int32_t*>(ptr(*tickets));
+        a.n_tickets = tickets->numel();
+    }
     a.stream = l.stream;
     check(mi_paged_attn(&a), "mi_paged_attn");
 }

@@ -251,9 +251,15 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
 
 def paged_workspace(batch: int, tokens: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
     """Scratch of `paged_attention` for calls of up to `batch` sequences and `tokens` new tokens that do not overlap (calls on different streams, and graphs
-    that may be replayed at the same time, need one each)."""
-    nbytes = _lib.load().mi_paged_attn_workspace_bytes(tokens, n_q_heads, n_kv_heads, head_dim)
-    return torch.empty(nbytes // 4, dtype=torch.float32, device=device)
+    that may be replayed at the same time, need one each).  With it come the arrival counts (attribute `tickets`, int32, zero between calls) by which the
+    last workgroup of a block merges the splits of its keys in the same launch; a workspace without them (a slice, a tensor of the caller's own) takes one more
+    launch for the same result.  They are cleared on the current stream, so a first call on another stream waits for this one; after calls that
+    overlapped all the same they may not be zero, and spoil later ones until `workspace.tickets.zero_()`."""
+    lib = _lib.load()
+    nbytes = lib.mi_paged_attn_workspace_bytes(tokens, n_q_heads, n_kv_heads, head_dim) if batch > 0 else 0
+    workspace = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
+    workspace.tickets = torch.zeros(lib.mi_paged_attn_tickets(n_kv_heads), dtype=torch.int32, device=device)
+    return workspace
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -273,7 +279,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         _lib.host().paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, ctx_len, bool(causal),
-                                    1.0 / math.sqrt(q.shape[2]) if softmax_scale is None else float(softmax_scale), max_q_len or 0, workspace, out)
+                                    1.0 / math.sqrt(q.shape[2]) if softmax_scale is None else float(softmax_scale), max_q_len or 0, workspace,
+                                    getattr(workspace, "tickets", None), out)
     return out
 
 

@@ -97,9 +97,11 @@ def test_attention(case, causal, dtype):
     _check("o", out, q, k, v, table, cu, ctx, causal, 1 / math.sqrt(d))
     # a bound of the lengths and a workspace do not change the result; neither does a second call
     ws = ops.paged_workspace(len(ctx), cu[-1], nq, nkv, d, DEV)
-    for kwargs in (dict(max_q_len=max(new)), dict(workspace=ws), dict(workspace=ws, max_q_len=max(new))):
+    bare = ws.clone()                                       # without tickets
+    for kwargs in (dict(max_q_len=max(new)), dict(workspace=ws), dict(workspace=ws, max_q_len=max(new)), dict(workspace=bare)):
         assert torch.equal(out, ops.paged_attention(*args, causal=causal, **kwargs)), kwargs
     torch.cuda.synchronize()
+    assert not hasattr(bare, "tickets") and int(ws.tickets.abs().sum()) == 0
 
 
 @pytest.mark.parametrize("nq,nkv,d,page,n,length", [(8, 2, 128, 64, 1, 30000), (4, 4, 64, 16, 1, 20000), (8, 2, 128, 16, 100, 9000), (2, 1, 64, 128, 700, 5000)])
@@ -112,6 +114,13 @@ def test_long_caches_are_split(nq, nkv, d, page, n, length):
     out = ops.paged_attention(*args)
     names = launched(lambda: ops.paged_attention(*args, max_q_len=n))
     assert any("merge" in x for x in names), names
+    ws = ops.paged_workspace(3, cu[-1], nq, nkv, d, DEV)
+    names = launched(lambda: ops.paged_attention(*args, max_q_len=n, workspace=ws))
+    assert any("merge" in x for x in names) == (n > 1), names
+    for _ in range(3):                                      # whoever is last
+        assert torch.equal(out, ops.paged_attention(*args, max_q_len=n, workspace=ws))
+    torch.cuda.synchronize()
+    assert int(ws.tickets.abs().sum()) == 0
     # a few tokens of the long one, all of the others
     keep = [0, 1, n // 2 + 1, n, n + 1]
     for t in sorted(set(keep)):

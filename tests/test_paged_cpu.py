@@ -228,9 +228,10 @@ def test_paged_attention_refusals(lib, base):
             (dict(q=None), -1), (dict(k_pages=None), -1), (dict(v_pages=None), -1), (dict(o=None), -1), (dict(page_table=None), -1), (dict(cu_seqlens=None), -1), (dict(ctx_len=None), -1),
             (dict(softmax_scale=0.0), -3), (dict(softmax_scale=float("nan")), -3), (dict(q=base + 2), -4), (dict(o=base + 8), -4), (dict(q_stride_token=4), -4), (dict(o_stride_head=2), -4),
             (dict(page_stride=4), -4), (dict(page_stride_token=2 ** 27), -3), (dict(page_stride_token=-128), -3), (dict(workspace=None), -5), (dict(workspace=base + 4), -5),
-            (dict(workspace_bytes=64), -5), (dict(total_q=2 ** 30), -3), (dict(n_q_heads=70000, n_kv_heads=70000), -3)]:
+            (dict(workspace_bytes=64), -5), (dict(tickets=base, n_tickets=3), -5), (dict(tickets=base + 2, n_tickets=10 ** 6), -5), (dict(total_q=2 ** 30), -3), (dict(n_q_heads=70000, n_kv_heads=70000), -3)]:
         assert lib.mi_paged_attn(ctypes.byref(args(**fields))) == status, fields
     assert lib.mi_paged_attn(ctypes.byref(args(total_q=0, q=None))) == 0
     sizes = [lib.mi_paged_attn_workspace_bytes(t, 32, 8, 128) for t in (1, 4, 5, 1000, 10 ** 6)]
     assert sizes == sorted(sizes) and sizes[0] > 0
+    assert lib.mi_paged_attn_tickets(0) == 0 and lib.mi_paged_attn_tickets(8) > 0
     assert lib.mi_paged_attn_workspace_bytes(0, 32, 8, 128) == 0 and lib.mi_paged_attn_workspace_bytes(5, 32, 7, 128) == 0
