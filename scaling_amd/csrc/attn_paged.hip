@@ -83,13 +83,14 @@ template <int BLOCK, int TILE, bool OF_BLOCKS> __device__ __forceinline__ Found 
     int split_tiles = 0x1000000;                          // no sequence has more
     if (plan.share > 0) {
         int64_t units = 0, blocks = 0;
+        int most = 0;
         for (int base = 0; base < p.batch; base += 64) {
             look(base);
             units += total(work.blocks * work.tiles);
-            if (plan.fit) blocks += total(work.blocks);
+            if (plan.fit || plan.even) blocks += total(work.blocks);
+            if (plan.even) most = max(most, group_max<64>(work.blocks > 0 ? work.tiles : 0));
         }
-        // paged_split_tiles
-        split_tiles = divide((uint32_t)(units < 0x7fffffff ? units : 0x7fffffff), plan.share, share_m) + 1;
+        split_tiles = divide(paged_units(plan, units, blocks, most), plan.share, share_m) + 1;      // paged_split_tiles
         for (int step = 0; plan.fit && blocks <= plan.share && step < kPagedSteps; ++step) {
             int64_t slots = 0;
             for (int base = 0; base < p.batch; base += 64) {
@@ -154,7 +155,7 @@ __device__ __forceinline__ void store_partial(float* at, float a, float b, bool 
 }
 
 // A row's partial results of `splits` splits, `step` rows of results apart, by 16 lanes with D / 16 features each, 2 (i + 16 k) and the next for
-// k = 0, 1, ...; those of eight splits are requested before the first is used.
+// k = 0, 1, ...; those of STEP splits are requested before the first is used.
 template <int D> struct RowSum {
     static constexpr int kPairs = D / 32;
     float M = -INFINITY, L = 0.f;
@@ -163,11 +164,11 @@ template <int D> struct RowSum {
 #pragma unroll
         for (int k = 0; k < kPairs; ++k) O[k] = make_float2(0.f, 0.f);
     }
-    // N more results, the first `there` of them
-    template <int N> __device__ __forceinline__ void add(const float2 (&ml)[N], const float2 (&o)[N][kPairs], int there) {
+    // N more results
+    template <int N> __device__ __forceinline__ void add(const float2 (&ml)[N], const float2 (&o)[N][kPairs]) {
         float m = M;
 #pragma unroll
-        for (int i = 0; i < N; ++i) m = fmaxf(m, i < there ? ml[i].x : -INFINITY);
+        for (int i = 0; i < N; ++i) m = fmaxf(m, ml[i].x);
         const float a = M == -INFINITY ? 0.f : fast_exp2(M - m);
         L *= a;
 #pragma unroll
@@ -175,7 +176,6 @@ template <int D> struct RowSum {
         M = m;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            if (i >= there) break;                         // (no weight would not do for an infinite output)
             const float w = ml[i].x == -INFINITY ? 0.f : fast_exp2(ml[i].x - M);
             // (named: of two products in a sum the compiler takes either into the fma, and both launches that merge have to leave the same bits)
             L = __builtin_fmaf(w, ml[i].y, L);
@@ -186,8 +186,8 @@ template <int D> struct RowSum {
             }
         }
     }
-    template <bool SHARED> __device__ __forceinline__ void add(const float* from_o, const float* from_ml, int64_t first, int64_t step, int splits) {
-        constexpr int kStep = 8;
+    template <bool SHARED, int STEP> __device__ __forceinline__ void add(const float* from_o, const float* from_ml, int64_t first, int64_t step, int splits) {
+        constexpr int kStep = STEP;
         const int lane = threadIdx.x & 15;
         for (int s0 = 0; s0 < splits; s0 += kStep) {
             float2 ml[kStep], o[kStep][kPairs];
@@ -198,7 +198,14 @@ template <int D> struct RowSum {
 #pragma unroll
                 for (int k = 0; k < kPairs; ++k) o[i][k] = load_partial<SHARED>(from_o + at * D + 2 * (lane + 16 * k));
             }
-            add(ml, o, splits - s0);
+#pragma unroll
+            for (int i = 0; i < kStep; ++i) {
+                if (s0 + i < splits) continue;             // ... with nothing in them (no weight would not do for an infinite output)
+                ml[i] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int k = 0; k < kPairs; ++k) o[i][k] = make_float2(0.f, 0.f);
+            }
+            add(ml, o);
         }
     }
     __device__ __forceinline__ void store(elem_t* row) const {
@@ -218,7 +225,7 @@ template <int D, bool SHARED> __device__ __forceinline__ void merge_rows(const P
     RowSum<D> sum;
     if (r < n_rows && part < f.splits) {
         const int64_t step = (int64_t)f.work.blocks * p.nkv * kRowBlock, first = ((int64_t)(f.partial + block) * p.nkv + kvh) * kRowBlock + r;
-        sum.template add<SHARED>(p.rows_o, p.rows_ml, first + part * step, step * per_row, (f.splits - part + per_row - 1) / per_row);
+        sum.template add<SHARED, 8>(p.rows_o, p.rows_ml, first + part * step, step * per_row, (f.splits - part + per_row - 1) / per_row);
     }
     float* mine = lds + group * (D + 2);
     if (lane == 0) { mine[0] = sum.M; mine[1] = sum.L; }
@@ -232,7 +239,7 @@ template <int D, bool SHARED> __device__ __forceinline__ void merge_rows(const P
         ml[0] = make_float2(other[0], other[1]);
 #pragma unroll
         for (int k = 0; k < RowSum<D>::kPairs; ++k) o[0][k] = *reinterpret_cast<const float2*>(other + 2 + 2 * (lane + 16 * k));
-        sum.add(ml, o, 1);
+        sum.add(ml, o);
     }
     const int row = block * kRowBlock + r, token = divide(row, p.n_rep, p.rep_m);
     sum.store(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh);
@@ -802,7 +809,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
 }
 
 // ---- merge of the splits ------------------------------------------------------------------------------------------------------------------------------
-// A workgroup per (split block, KV head, 16 rows of the block).  KIND 0: of paged_rows where the caller has no tickets, 1: of paged_tiles.  (Two lanes to a pair
+// A workgroup per (split block, KV head) or, of chunks, per 16 of its rows.  KIND 0: of paged_rows where the caller has no tickets, 1: of paged_tiles.  (Two lanes to a pair
 // of features and rows one after the other, with a workgroup for every partial result, most of them idle: 19 us for 64 blocks of 256 rows in four splits.)
 template <int D, int KIND>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
@@ -813,10 +820,11 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
         if (f.b >= 0) merge_rows<D, false>(p, f, (int)blockIdx.x - f.at, kvh, lds);
     } else {
         const Found f = find_work<kTileRows, kTileKeys, true>(p, p.tiles, p.share_m[1], blockIdx.x);
+        if (f.b < 0) return;
         const int block = (int)blockIdx.x - f.at, in = 16 * blockIdx.z + (threadIdx.x >> 4), row = block * kTileRows + in;
-        if (f.b < 0 || row >= f.seq.n * p.n_rep) return;
+        if (row >= f.seq.n * p.n_rep) return;
         RowSum<D> sum;
-        sum.template add<false>(p.tiles_o, p.tiles_ml, ((int64_t)(f.partial + block) * p.nkv + kvh) * kTileRows + in, (int64_t)f.work.blocks * p.nkv * kTileRows, f.splits);
+        sum.template add<false, 4>(p.tiles_o, p.tiles_ml, ((int64_t)(f.partial + block) * p.nkv + kvh) * kTileRows + in, (int64_t)f.work.blocks * p.nkv * kTileRows, f.splits);
         const int token = divide(row, p.n_rep, p.rep_m);
         sum.store(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh);
     }
@@ -840,18 +848,22 @@ template <int D> int launch(const PagedParams& p, int64_t row_blocks, int64_t ti
 }
 
 // Workgroups per KV head that either kernel's work is cut for.  `items`: blocks of rows x KV heads of the calls, as many as there may be.
-// paged_rows, of which two to four share a compute unit: where items are many, lengths differ and small pieces keep the units even; where they are few, more
-// splits of each only make the merge longer.  (Kernel / merge, us, of 512, 1024, 2048 workgroups: 32 x 8 items of 200 - 8192 keys 98.9 / 4.4, 89.5 / 5.2, 85 /
-// 7.5; 3 x 4 items of 20000 - 32768 keys of 64 features 18.6 / 7.5, 19.2 / 12.7, 19.3 / 18.7.)
+// paged_rows, of which two to four share a compute unit: of many items small pieces keep the units even where lengths differ (8 workgroups to a unit), and 2 do
+// where they do not; of few items more splits of each only make the merge longer.  (us of 512, 1024, 2048 workgroups, d 128: 32 x 8 items of 200 - 8192
+// keys 98, 93, 87, all of 4096 keys 85, 85, 92; 3 x 4 items of 20000 - 32768 keys of 64 features 18.6, 19.2, 19.3 and for the merge 7, 13, 19.)
 constexpr int kRowsLeast = 2, kRowsMost = 8;             // per compute unit
 int share_of(int64_t workgroups, int nkv) { return workgroups / nkv > 0 ? (int)(workgroups / nkv) : 1; }
 void make_plans(int64_t tokens, int64_t items, int n_rep, int nkv, PagedPlan& rows, PagedPlan& tiles) {
     const int cus = mi_compute_units();
-    rows = PagedPlan{0, kRowLimit, 0x7fffffff, share_of(std::clamp<int64_t>(8 * items, kRowsLeast * cus, kRowsMost * cus), nkv), 0, 0, 0};
+    const bool few = 8 * items <= kRowsLeast * cus;
+    rows = PagedPlan{0, kRowLimit, 0x7fffffff, share_of(few ? kRowsLeast * cus : std::min<int64_t>(8 * items, kRowsMost * cus), nkv), 8 * items >= kRowsMost * cus, 0, 0, 0};
     // Enough blocks for every compute unit: no splits, no merge.
     const bool many = tokens * n_rep / kTileRows * nkv >= cus;
-    tiles = PagedPlan{kRowLimit, 0x7fffffff, 0x7fffffff, many ? 0 : share_of(cus, nkv), 1, 0, 0};
+    tiles = PagedPlan{kRowLimit, 0x7fffffff, 0x7fffffff, many ? 0 : share_of(cus, nkv), 0, 1, 0, 0};
 }
+// Whether the last workgroup of a block merges, given tickets: no more workgroups than run at once.  Each waits for its results to be in memory, which more of them
+// cannot hide: 32 x 8 items of 200 - 8192 keys in pieces for 2048 workgroups 100 us, with a launch of its own for the merge 92.
+bool merges_in_launch(const PagedPlan& rows, int nkv) { return (int64_t)rows.share * nkv <= kRowsLeast * mi_compute_units(); }
 
 size_t partial_bytes(int64_t partials, int nkv, int block_rows, int head_dim) { return (size_t)partials * nkv * block_rows * (size_t)(head_dim + 2) * sizeof(float); }
 constexpr int64_t kMaxTiles = (1 << 24) + 1;              // of a sequence
@@ -916,7 +928,7 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
         return mi_fail(MI_E_WORKSPACE, "paged_attn: workspace needs %zu bytes (16-byte aligned), got %zu", need, a->workspace_bytes);
     if (a->tickets && (a->n_tickets < mi_paged_attn_tickets(p.nkv) || (reinterpret_cast<uintptr_t>(a->tickets) & 3u) != 0))
         return mi_fail(MI_E_WORKSPACE, "paged_attn: %lld tickets (4-byte aligned), got %lld", (long long)mi_paged_attn_tickets(p.nkv), (long long)a->n_tickets);
-    p.tickets = a->tickets;
+    p.tickets = merges_in_launch(p.rows, p.nkv) ? a->tickets : nullptr;
     // A sequence of up to a tile of keys has one split, whatever the plan.
     if (row_tiles == 1 || row_blocks == 0) p.rows.share = 0;
     if (tile_tiles == 1 || tile_blocks == 0) p.tiles.share = 0;

@@ -58,6 +58,7 @@ struct PagedPlan {
     int rows_over, rows_up_to;    // sequences with more than rows_over and at most rows_up_to rows
     int max_n;                    // ... and at most so many new tokens
     int share;                    // workgroups per KV head aimed at; 0: never split
+    int even;                     // sequences of about one length: cut for a quarter of the share
     int fit;                      // whether a workgroup has a compute unit for itself, and more of them than that are to be avoided
     int max_slots, max_partials;  // (set by the host) workgroups and partial results per KV head that there are
 };
@@ -73,11 +74,14 @@ template <int BLOCK, int TILE> MI_PLAN_FN PagedWork paged_work(const PagedPlan& 
     w.tiles = s.len > 0 ? (s.len + TILE - 1) / TILE : 1;    // rows without keys are written too
     return w;
 }
-// tiles of a split; `units` is W
-MI_PLAN_FN int paged_split_tiles(const PagedPlan& p, int64_t units) {
+// What is divided by the share for the tiles of a split, less one.  units: W; blocks: of all sequences; most: tiles of the longest
+MI_PLAN_FN uint32_t paged_units(const PagedPlan& p, int64_t units, int64_t blocks, int most) {
+    if (p.even && most * blocks * 4 <= units * 5) units *= 4;
+    return (uint32_t)(units < 0x7fffffff ? units : 0x7fffffff);
+}
+MI_PLAN_FN int paged_split_tiles(const PagedPlan& p, int64_t units, int64_t blocks, int most) {
     if (p.share == 0) return 0x1000000;                    // no sequence has more
-    const uint32_t u = (uint32_t)(units < 0x7fffffff ? units : 0x7fffffff);
-    return (int)(u / (uint32_t)p.share) + 1;
+    return (int)(paged_units(p, units, blocks, most) / (uint32_t)p.share) + 1;
 }
 // Where all blocks together fit, S grows until their splits do too: one workgroup more than there is room for at once would take as long as all others.
 // `slots`: splits of all blocks at S.  S / slots only shrinks towards the room, so a few steps do.

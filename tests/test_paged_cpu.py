@@ -21,7 +21,7 @@ static int fail(const char* what, int i) { printf("case %%d: %%s\n", i, what); r
 template <int BLOCK, int TILE>
 static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, int capacity, int longest, bool good, bool causal, const std::vector<int>& cu,
                   const std::vector<int>& ctx, std::vector<int>& taken) {
-    PagedPlan p = {over, up_to, longest, rnd() %% 4 == 0 ? 0 : 1 << rnd() %% 9, (int)(rnd() & 1), 0, 0};
+    PagedPlan p = {over, up_to, longest, rnd() %% 4 == 0 ? 0 : 1 << rnd() %% 9, (int)(rnd() & 1), (int)(rnd() & 1), 0, 0};
     const int max_tiles = (capacity + TILE - 1) / TILE;
     const int64_t most = paged_max_blocks<BLOCK>(p, total, batch, longest, n_rep);
     p.max_slots = (int)paged_max_slots(p, most, max_tiles);
@@ -33,9 +33,14 @@ static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, i
         const PagedWork w = paged_work<BLOCK, TILE>(p, s, n_rep);
         units += (int64_t)w.blocks * w.tiles;
     }
-    int S = paged_split_tiles(p, units);
     int64_t all = 0;
-    for (int b = 0; b < batch; ++b) all += paged_work<BLOCK, TILE>(p, paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity), n_rep).blocks;
+    int longest_tiles = 0;
+    for (int b = 0; b < batch; ++b) {
+        const PagedWork w = paged_work<BLOCK, TILE>(p, paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity), n_rep);
+        all += w.blocks;
+        if (w.blocks > 0 && w.tiles > longest_tiles) longest_tiles = w.tiles;
+    }
+    int S = paged_split_tiles(p, units, all, longest_tiles);
     for (int step = 0; p.share > 0 && step < kPagedSteps; ++step) {
         int64_t n = 0;
         for (int b = 0; b < batch; ++b) {
