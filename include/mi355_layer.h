@@ -371,7 +371,7 @@ int mi_paged_append(const mi_paged_append_args* args);
  * with few new rows are merged in the launch that computes them instead of by one more, to the same bits.  They belong to one call at a time as the workspace does, and
  * unlike it outlive a mistake: after calls that overlapped on them, later ones merge too early or never until they are cleared.
  * The key axis is cut by the lengths on the device, so that the work of a ragged batch is even; the order of the sums depends on the lengths of all
- * sequences of the call, and on nothing else.
+ * sequences of the call and on max_q_len, and on nothing else.
  * Algorithmic work: 4 * head_dim * n_q_heads * pairs flop; HBM bytes 2 * sum ctx_len * n_kv_heads * head_dim * e + 2 * total_q * n_q_heads * head_dim * e. */
 typedef struct mi_paged_attn_args {
     const void* q;

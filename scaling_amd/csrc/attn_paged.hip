@@ -16,8 +16,12 @@ typedef float f32x4v __attribute__((ext_vector_type(4)));
 
 namespace {
 
-constexpr int kRowLimit = 16;        // rows of a sequence up to which paged_rows computes it
-constexpr int kRowBlock = 16;
+// Rows (tokens x query heads of a KV head) of a sequence up to which paged_rows computes it: one block, or two where items are few and none has more, so that
+// paged_tiles is not launched.  (us, rows / tiles, 4 query heads to a KV head, d 128: 32 sequences of 5 tokens 123 / 157, of 9 tokens 215 / 170; 8 of
+// 3 - 9 tokens 39.9 / 53; one of 16 tokens 15.8 / 20.7.  32 sequences of one token of 32 heads and one KV head: 28 / 27.)
+constexpr int kRowBlock = 16;        // rows of a block, or twice as many where a sequence may have more
+constexpr int kRowLimit = 32;
+constexpr int kRowsAlone = 64;
 constexpr int kRowChunk = 32;        // keys per wavefront and step of paged_rows
 constexpr int kRowWaves = 4;
 constexpr int kRowTile = kRowChunk * kRowWaves;
@@ -34,6 +38,7 @@ struct PagedParams {
     uint32_t page_m, rep_m, nkv_m, share_m[2];        // for divide(); share_m: of rows and tiles
     float scale_log2;
     PagedPlan rows, tiles;
+    int tile_rows;                                    // rows kept per partial result of paged_tiles
     int32_t* tickets;                                 // nullable: arrivals of the splits of paged_rows, [partial][KV head], zero between launches
     float *rows_o, *rows_ml, *tiles_o, *tiles_ml;     // partial results: [partial][KV head][row of the block][feature], and (maximum in log2 units, sum)
 };
@@ -91,13 +96,14 @@ template <int BLOCK, int TILE, bool OF_BLOCKS> __device__ __forceinline__ Found 
             if (plan.even) most = max(most, group_max<64>(work.blocks > 0 ? work.tiles : 0));
         }
         split_tiles = divide(paged_units(plan, units, blocks, most), plan.share, share_m) + 1;      // paged_split_tiles
-        for (int step = 0; plan.fit && blocks <= plan.share && step < kPagedSteps; ++step) {
+        for (int step = 0; paged_few(plan, blocks) && step <= kPagedSteps; ++step) {
             int64_t slots = 0;
             for (int base = 0; base < p.batch; base += 64) {
                 if (p.batch > 64) look(base);
                 slots += total(work.blocks * paged_splits(work, split_tiles));
             }
-            split_tiles = paged_next_tiles(plan, split_tiles, blocks, slots);
+            if (slots <= plan.fit) break;
+            split_tiles = paged_next_tiles(plan, split_tiles, units, blocks, slots, step);
         }
     }
     int at = 0, slots = 0, partials = 0;
@@ -216,15 +222,17 @@ template <int D> struct RowSum {
     }
 };
 
-// Block `block` of few rows, its splits merged by 256 threads: 16 / rows groups of 16 lanes to a row, a share of the splits each, together through LDS.
-template <int D, bool SHARED> __device__ __forceinline__ void merge_rows(const PagedParams& p, const Found& f, int block, int kvh, float* lds) {
-    const int n_rows = min(kRowBlock, f.seq.n * p.n_rep - block * kRowBlock), group = threadIdx.x >> 4, lane = threadIdx.x & 15;
-    int per_row = 16;                                      // groups to a row
-    while (per_row * n_rows > 16) per_row /= 2;
+// Rows r0 to r0 + n - 1 of block `block` of few rows, its splits merged by 256 threads: per row 16 / n groups of 16 lanes with a share of the splits each,
+// together through LDS (16 x (D + 2) floats).
+template <int D, int BLOCK, bool SHARED>
+__device__ __forceinline__ void merge_rows(const PagedParams& p, const Found& f, int block, int kvh, int r0, int n, float* lds) {
+    const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    int per_row = 16;
+    while (per_row * n > 16) per_row /= 2;
     const int r = group / per_row, part = group - r * per_row;
     RowSum<D> sum;
-    if (r < n_rows && part < f.splits) {
-        const int64_t step = (int64_t)f.work.blocks * p.nkv * kRowBlock, first = ((int64_t)(f.partial + block) * p.nkv + kvh) * kRowBlock + r;
+    if (r < n && part < f.splits) {
+        const int64_t step = (int64_t)f.work.blocks * p.nkv * BLOCK, first = ((int64_t)(f.partial + block) * p.nkv + kvh) * BLOCK + r0 + r;
         sum.template add<SHARED, 8>(p.rows_o, p.rows_ml, first + part * step, step * per_row, (f.splits - part + per_row - 1) / per_row);
     }
     float* mine = lds + group * (D + 2);
@@ -232,7 +240,7 @@ template <int D, bool SHARED> __device__ __forceinline__ void merge_rows(const P
 #pragma unroll
     for (int k = 0; k < RowSum<D>::kPairs; ++k) *reinterpret_cast<float2*>(mine + 2 + 2 * (lane + 16 * k)) = sum.O[k];
     __syncthreads();
-    if (part != 0 || r >= n_rows) return;
+    if (part != 0 || r >= n) return;
     for (int i = 1; i < per_row; ++i) {
         const float* other = mine + i * (D + 2);
         float2 ml[1], o[1][RowSum<D>::kPairs];
@@ -241,7 +249,7 @@ template <int D, bool SHARED> __device__ __forceinline__ void merge_rows(const P
         for (int k = 0; k < RowSum<D>::kPairs; ++k) o[0][k] = *reinterpret_cast<const float2*>(other + 2 + 2 * (lane + 16 * k));
         sum.add(ml, o);
     }
-    const int row = block * kRowBlock + r, token = divide(row, p.n_rep, p.rep_m);
+    const int row = block * BLOCK + r0 + r, token = divide(row, p.n_rep, p.rep_m);
     sum.store(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh);
 }
 
@@ -292,52 +300,63 @@ __device__ __forceinline__ void own_keys_only(const PagedParams& p, const int32_
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------------------------------------
-// One workgroup per (block of 16 rows, KV head, split); its wavefronts take chunks of 32 keys in turn:
+// One workgroup per (block of 16 NB rows, KV head, split); its wavefronts take chunks of 32 keys in turn:
 //     S^T[key][row] = K Q^T      v_mfma_f32_16x16x32, A = K rows straight from global memory in operand layout, B = Q^T
 //     online softmax over keys   a lane's column is a row: eight keys in the lane, two lane exchanges
 //     O^T[feature][row] += V^T P^T    V passes through a wavefront's own LDS and is read back transposed
-// Every cached element is read from memory once per block of rows.  The next chunk's loads are under way while a chunk is computed.
-template <int D>
-__global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const PagedParams p) {
-    constexpr int NWV = kRowWaves, kThreads = 64 * NWV;
+// Every cached element is read from memory once per block of rows.  The next chunk's K is requested as soon as the scores are computed and its V as soon as this
+// chunk's is in LDS, into the same registers: 16 KB a wavefront (d 128) are always under way, and 12 wavefronts fit a compute unit.  (Two sets of registers, a
+// whole chunk ahead: 8 wavefronts, 16 rows to a block at the most.)
+template <int D, int NB>
+__global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_kernel(const PagedParams p) {
+    constexpr int NWV = kRowWaves, kThreads = 64 * NWV, BLOCK = 16 * NB;
     constexpr int KS = D / 32, DT = D / 16;
     constexpr int VSTR = 2 * D + 32;          // bytes per key row of a staged V chunk: transposed reads of 8 rows x 32 bytes hit 256 distinct bytes
     constexpr int V_ITEMS = 8 * (D / 8);      // (four keys, eight features) of a chunk
     constexpr int V_PER_LANE = (V_ITEMS + 63) / 64;
-    __shared__ __attribute__((aligned(16))) char v_lds[NWV][kRowChunk * VSTR];
-    __shared__ float wm_lds[NWV][16], wl_lds[NWV][16], wo_lds[NWV][16][D + 1];
-    __shared__ int redo_lds[16];
+    constexpr int kStaged = NWV * kRowChunk * VSTR, kResults = NWV * BLOCK * (D + 1) * 4;
+    __shared__ __attribute__((aligned(16))) char pool[kStaged > kResults ? kStaged : kResults];     // V chunks, then the wavefronts' results
+    __shared__ float wm_lds[NWV][BLOCK], wl_lds[NWV][BLOCK];
+    __shared__ int redo_lds[BLOCK];
 
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, G = lane >> 4;
     const int slot = divide(blockIdx.x, p.nkv, p.nkv_m), kvh = blockIdx.x - slot * p.nkv;
-    const Found f = find_work<kRowBlock, kRowTile, false>(p, p.rows, p.share_m[0], slot);
+    const Found f = find_work<BLOCK, kRowTile, false>(p, p.rows, p.share_m[0], slot);
     if (f.b < 0) return;
     const int in = slot - f.at, split = paged_quotient(in, f.work.blocks), block = in - split * f.work.blocks;
     int s0, s1;
     paged_split_keys<kRowTile>(f.seq, f.work, f.splits, split, s0, s1);
-    const int n_rows = min(kRowBlock, f.seq.n * p.n_rep - block * kRowBlock);
-    // this lane's row
-    const int row = block * kRowBlock + min(l16, n_rows - 1), token = divide(row, p.n_rep, p.rep_m), head = kvh * p.n_rep + row - token * p.n_rep;
-    const int limit = l16 < n_rows ? min(paged_limit(f.seq, token, p.causal), s1) : 0;
-    const int end = group_max<16>(limit);                  // the same for the four groups of 16 lanes
-    const int n_iter = __builtin_amdgcn_readfirstlane(end > s0 ? (end - s0 + NWV * kRowChunk - 1) / (NWV * kRowChunk) : 0);
-    const int last = max(s1 - 1, 0), last_group = last >> 4;      // keys past the split repeat its last one
+    const int n_rows = min(BLOCK, f.seq.n * p.n_rep - block * BLOCK);
 
-    uint4 raw[KS];
-    {
+    // this lane's rows, l16 and 16 further on
+    uint4 raw[NB][KS];
+    int limit[NB], end = 0;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const int r = 16 * nb + l16, row = block * BLOCK + min(r, n_rows - 1), token = divide(row, p.n_rep, p.rep_m), head = kvh * p.n_rep + row - token * p.n_rep;
+        limit[nb] = r < n_rows ? min(paged_limit(f.seq, token, p.causal), s1) : 0;
+        end = max(end, group_max<16>(limit[nb]));          // the same for the four groups of 16 lanes
         const elem_t* qr = p.q + (int64_t)(f.seq.first + token) * p.q_st + (int64_t)head * p.q_sh + 8 * G;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) raw[ks] = ld128(qr + 32 * ks);
+        for (int ks = 0; ks < KS; ++ks) raw[nb][ks] = ld128(qr + 32 * ks);
     }
-    f32x4v o_acc[DT];
+    const int n_iter = __builtin_amdgcn_readfirstlane(end > s0 ? (end - s0 + kRowTile - 1) / kRowTile : 0);
+    const int last = max(s1 - 1, 0), last_group = last >> 4;      // keys past the split repeat its last one
+
+    f32x4v o_acc[NB][DT];
+    float m_i[NB], l_i[NB];
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) o_acc[dt] = f32x4v{0.f, 0.f, 0.f, 0.f};
-    float m_i = -INFINITY, l_i = 0.f;
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o_acc[nb][dt] = f32x4v{0.f, 0.f, 0.f, 0.f};
+        m_i[nb] = -INFINITY;
+        l_i[nb] = 0.f;
+    }
 
     const int32_t* table = p.table + (int64_t)f.b * p.table_stride;
     const elem_t *kbase = p.kp + (int64_t)kvh * p.p_sh, *vbase = p.vp + (int64_t)kvh * p.p_sh;
-    char* vt = v_lds[wave];
+    char* vt = pool + wave * kRowChunk * VSTR;
     const char* vt_lane = vt + (4 * G + (l16 >> 2)) * VSTR + 8 * (l16 & 3);
     // lane i: pages of both groups of this wavefront's chunk i of the 64 from `ids_from` on
     int ids[2], ids_from = 0;
@@ -349,27 +368,29 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
         // waited for here: where they are used the wait would be for everything that is under way, in every step
         asm volatile("" : "+v"(ids[0]), "+v"(ids[1]));
     };
-
-    struct ChunkRegs {
-        elem8_t kf[2][KS];
-        uint4 vraw[V_PER_LANE][4];
-    };
-    auto request = [&](ChunkRegs& c, int it) {
-        const int key0 = s0 + (NWV * it + wave) * kRowChunk;
-        int64_t at[2];                                     // of key 16 * group in the pages
-        int group[2];
+    // the chunk that is requested next: its first key, its two groups of 16 keys and where these start in the pages
+    int key_next, group[2];
+    int64_t at[2];
+    auto place = [&](int it) {
+        key_next = s0 + (NWV * it + wave) * kRowChunk;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            group[t] = min((key0 >> 4) + t, last_group);
+            group[t] = min((key_next >> 4) + t, last_group);
             at[t] = (int64_t)__builtin_amdgcn_readlane(ids[t], it - ids_from) * p.p_sp + (int64_t)row_in_page(p, group[t]) * p.p_st;
         }
+    };
+    elem8_t kf[2][KS];
+    uint4 vraw[V_PER_LANE][4];
+    auto request_k = [&]() {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int r = min(key0 + 16 * t + l16, last) - 16 * group[t];
+            const int r = min(key_next + 16 * t + l16, last) - 16 * group[t];
             const elem_t* kr = kbase + at[t] + (int64_t)r * p.p_st + 8 * G;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) c.kf[t][ks] = __builtin_bit_cast(elem8_t, ldg_nt(reinterpret_cast<const uint4*>(kr + 32 * ks)));
+            for (int ks = 0; ks < KS; ++ks) kf[t][ks] = __builtin_bit_cast(elem8_t, ldg_nt(reinterpret_cast<const uint4*>(kr + 32 * ks)));
         }
+    };
+    auto request_v = [&]() {
 #pragma unroll
         for (int j = 0; j < V_PER_LANE; ++j) {
             const int item = lane + 64 * j;
@@ -379,106 +400,117 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
             const elem_t* vr = vbase + (quad < 4 ? at[0] : at[1]) + 8 * dg;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int rr = min(key0 + 4 * quad + r, last) - 16 * g;
-                c.vraw[j][r] = ldg_nt(reinterpret_cast<const uint4*>(vr + (int64_t)rr * p.p_st));
+                const int rr = min(key_next + 4 * quad + r, last) - 16 * g;
+                vraw[j][r] = ldg_nt(reinterpret_cast<const uint4*>(vr + (int64_t)rr * p.p_st));
             }
         }
     };
-    elem8_t qf[KS];
-    auto process_chunk = [&](ChunkRegs& c, int it) {
-        const int key0 = s0 + (NWV * it + wave) * kRowChunk;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        elem8_t pf;
-        float alpha;
-        {
-            f32x4v s_acc[2];
+
+    if (n_iter > 0) {
+        look_up(0);
+        place(0);
+        request_k();
+        request_v();
+    }
+    elem8_t qf[NB][KS];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                s_acc[t] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) s_acc[t] = mfma_16x16x32(c.kf[t][ks], qf[ks], s_acc[t]);
+        for (int ks = 0; ks < KS; ++ks) qf[nb][ks] = __builtin_bit_cast(elem8_t, raw[nb][ks]);
+    // No branch around a request or a chunk: where paths meet, the wait for a chunk would be for the next one too.  So the chunk behind the last is requested
+    // as well (the split's last key over and over), and a wavefront without keys computes along with the others, with nothing in its chunk.
+    for (int it = 0; it < n_iter; ++it) {
+        const int key0 = key_next;
+        f32x4v s_acc[NB][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                s_acc[nb][t] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) s_acc[nb][t] = mfma_16x16x32(kf[t][ks], qf[nb][ks], s_acc[nb][t]);
             }
+        if (it + 1 - ids_from >= 64) look_up(it + 1);
+        place(it + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        request_k();
+        __builtin_amdgcn_sched_barrier(0);
+        elem8_t pf[NB];
+        float alpha[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
             float mx = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    if (key0 + 16 * t + 4 * G + r >= limit) s_acc[t][r] = -INFINITY;
-                    mx = fmaxf(mx, s_acc[t][r]);
+                    if (key0 + 16 * t + 4 * G + r >= limit[nb]) s_acc[nb][t][r] = -INFINITY;
+                    mx = fmaxf(mx, s_acc[nb][t][r]);
                 }
             mx = quad_max(mx);
-            const float m_new = fmaxf(m_i, mx * p.scale_log2), m_use = m_new == -INFINITY ? 0.f : m_new;   // a row may have no key here, or none at all
-            alpha = fast_exp2(m_i - m_use);
-            m_i = m_new;
+            const float m_new = fmaxf(m_i[nb], mx * p.scale_log2), m_use = m_new == -INFINITY ? 0.f : m_new;     // a row may have no key here, or none at all
+            alpha[nb] = fast_exp2(m_i[nb] - m_use);
+            m_i[nb] = m_new;
             float rs = 0.f;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float e = fast_exp2(s_acc[t][r] * p.scale_log2 - m_use);
+                    const float e = fast_exp2(s_acc[nb][t][r] * p.scale_log2 - m_use);
                     rs += e;
-                    pf[4 * t + r] = (elem_t)e;             // slot (G, i): key 16 * (i / 4) + 4 * G + i % 4
+                    pf[nb][4 * t + r] = (elem_t)e;         // slot (G, i): key 16 * (i / 4) + 4 * G + i % 4; rounded for the product, as P is in mi_attn_fwd
                 }
-            l_i = l_i * alpha + rs;
-#pragma unroll
-            for (int j = 0; j < V_PER_LANE; ++j) {
-                const int item = lane + 64 * j;
-                if (V_ITEMS % 64 != 0 && item >= V_ITEMS) break;
-                const int quad = item / (D / 8), dg = item % (D / 8);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) st128(vt + (4 * quad + r) * VSTR + 16 * dg, c.vraw[j][r]);
-            }
+            l_i[nb] = l_i[nb] * alpha[nb] + rs;
         }
+        // A wavefront's own LDS, whose accesses run in program order: fences order the compiler, and the wavefronts never wait for each other in here.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int j = 0; j < V_PER_LANE; ++j) {
+            const int item = lane + 64 * j;
+            if (V_ITEMS % 64 != 0 && item >= V_ITEMS) break;
+            const int quad = item / (D / 8), dg = item % (D / 8);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) st128(vt + (4 * quad + r) * VSTR + 16 * dg, vraw[j][r]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        request_v();
+        __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             const elem8_t a = tr_pair(vt_lane + 32 * dt, vt_lane + 16 * VSTR + 32 * dt);
-            o_acc[dt] = o_acc[dt] * alpha;
-            o_acc[dt] = mfma_16x16x32(a, pf, o_acc[dt]);
-        }
-    };
-
-    ChunkRegs ra, rb;
-    if (n_iter > 0) {
-        look_up(0);
-        request(ra, 0);
-    }
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) qf[ks] = __builtin_bit_cast(elem8_t, raw[ks]);
-    // No branch around a request or a chunk: where paths meet, the wait for a chunk would be for the next one too.  So chunks past the split's keys are
-    // requested (its last key over and over) and computed, with nothing in them, where other wavefronts still have some.
-    for (int it = 0; n_iter > 0;) {
-        if (it + 1 - ids_from >= 64) look_up(it + 1);
-        request(rb, it + 1);
-        __builtin_amdgcn_sched_barrier(0);                 // under way before the wait for the chunk in front of it
-        process_chunk(ra, it);
-        if (++it >= n_iter) break;
-        if (it + 1 - ids_from >= 64) look_up(it + 1);
-        request(ra, it + 1);
-        __builtin_amdgcn_sched_barrier(0);
-        process_chunk(rb, it);
-        if (++it >= n_iter) break;
+            for (int nb = 0; nb < NB; ++nb) {
+                o_acc[nb][dt] = o_acc[nb][dt] * alpha[nb];
+                o_acc[nb][dt] = mfma_16x16x32(a, pf[nb], o_acc[nb][dt]);
+            }
+        }
     }
 
     // ---- the wavefronts' results together; of a single split the output, else a partial result ----
-    l_i = quad_sum(l_i);
-    if (G == 0) { wm_lds[wave][l16] = m_i; wl_lds[wave][l16] = l_i; }
-    if (tid < 16) redo_lds[tid] = 0;
+    float* wo = reinterpret_cast<float*>(pool);            // [wavefront][row][feature], rows D + 1 apart
+    if (tid < BLOCK) redo_lds[tid] = 0;
     const int filled = s0 + n_iter * kRowTile;             // chunks reach up to here: with keys that a row may not see, or with others once more
+    __syncthreads();                                       // nobody reads V any more
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
+    for (int nb = 0; nb < NB; ++nb) {
+        const float l = quad_sum(l_i[nb]);
+        if (G == 0) { wm_lds[wave][16 * nb + l16] = m_i[nb]; wl_lds[wave][16 * nb + l16] = l; }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) wo_lds[wave][l16][16 * dt + 4 * G + r] = o_acc[dt][r];
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) wo[(wave * BLOCK + 16 * nb + l16) * (D + 1) + 16 * dt + 4 * G + r] = o_acc[nb][dt][r];
+    }
     __syncthreads();
     const auto emit = [&](int r, int d, float M, float L, float O0, float O1) {
         if (f.splits == 1) {
-            const int rr = block * kRowBlock + r, i = divide(rr, p.n_rep, p.rep_m);
+            const int rr = block * BLOCK + r, i = divide(rr, p.n_rep, p.rep_m);
             const float inv = L == 0.f ? 0.f : 1.f / L;
             *reinterpret_cast<uint32_t*>(p.o + (int64_t)(f.seq.first + i) * p.o_st + (int64_t)(kvh * p.n_rep + rr - i * p.n_rep) * p.o_sh + d) = pack_elem2(O0 * inv, O1 * inv);
         } else {
-            const int64_t at = ((int64_t)(f.partial + in) * p.nkv + kvh) * kRowBlock + r;
-            store_partial(p.rows_o + at * D + d, O0, O1, p.tickets != nullptr);
-            if (d == 0) store_partial(p.rows_ml + at * 2, M, L, p.tickets != nullptr);
+            const int64_t to = ((int64_t)(f.partial + in) * p.nkv + kvh) * BLOCK + r;
+            store_partial(p.rows_o + to * D + d, O0, O1, p.tickets != nullptr);
+            if (d == 0) store_partial(p.rows_ml + to * 2, M, L, p.tickets != nullptr);
         }
     };
     for (int idx = tid; idx < n_rows * (D / 2); idx += kThreads) {
@@ -490,19 +522,23 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
 #pragma unroll
         for (int w = 0; w < NWV; ++w) {
             const float wm = wm_lds[w][r], scale = wm == -INFINITY ? 0.f : fast_exp2(wm - M);
+            const float* from = wo + (w * BLOCK + r) * (D + 1) + d;
             L += scale * wl_lds[w][r];
-            O0 += scale * wo_lds[w][r][d];
-            O1 += scale * wo_lds[w][r][d + 1];
+            O0 += scale * from[0];
+            O1 += scale * from[1];
         }
         if (not_finite(O0) || not_finite(O1) || not_finite(L)) redo_lds[r] = 1;
         emit(r, d, M, L, O0, O1);
     }
-    if (__ballot(l16 < n_rows && limit < filled) != 0) {   // the same for the workgroup
+    bool uneven = false;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) uneven |= 16 * nb + l16 < n_rows && limit[nb] < filled;
+    if (__ballot(uneven) != 0) {                           // the same for the workgroup
         __syncthreads();
         for (int r = wave; r < n_rows; r += NWV) {
-            const int lim = __builtin_amdgcn_readlane(limit, r);
+            const int lim = NB == 2 && r >= 16 ? __builtin_amdgcn_readlane(limit[NB - 1], r & 15) : __builtin_amdgcn_readlane(limit[0], r & 15);
             if (redo_lds[r] == 0 || lim >= filled) continue;
-            const int rr = block * kRowBlock + r, i = divide(rr, p.n_rep, p.rep_m);
+            const int rr = block * BLOCK + r, i = divide(rr, p.n_rep, p.rep_m);
             float M, L, O0, O1;
             own_keys_only<D>(p, table, kvh, p.q + (int64_t)(f.seq.first + i) * p.q_st + (int64_t)(kvh * p.n_rep + rr - i * p.n_rep) * p.q_sh, s0, lim, M, L, O0, O1);
             if (2 * lane < D) emit(r, 2 * lane, M, L, O0, O1);
@@ -511,7 +547,8 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
     // With tickets the workgroup of a block that is last to get here merges its splits; nobody waits for anybody.  Partial results are stored past the L2 and
     // every wavefront has waited for its own before the barrier, so the count that thread 0 raises behind it comes after them in memory, and the loads of
     // the workgroup that reads the highest count come after all.  (Two launches, the second one merging, of 1500 keys of 32 / 8 heads: 11.5 us one call after the
-    // other; 32 sequences of 200 - 8192 keys: 94.)
+    // other, one launch 9.6.)
+    if constexpr (NB > 1) return;
     if (f.splits == 1 || p.tickets == nullptr) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -523,8 +560,8 @@ __global__ __launch_bounds__(64 * kRowWaves, 2) void paged_rows_kernel(const Pag
     }
     __syncthreads();
     if (redo_lds[0] == 0) return;
-    static_assert(NWV == 4 && sizeof(wo_lds) >= 16 * (D + 2) * sizeof(float), "merge_rows: 256 threads, and room in LDS");
-    merge_rows<D, true>(p, f, block, kvh, &wo_lds[0][0][0]);
+    static_assert(NWV == 4 && sizeof(pool) >= 16 * (D + 2) * sizeof(float), "merge_rows: 256 threads, and room in LDS");
+    merge_rows<D, BLOCK, true>(p, f, block, kvh, 0, n_rows, wo);
 }
 
 // ---- chunks -------------------------------------------------------------------------------------------------------------------------------------------
@@ -761,7 +798,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
     if (grp == 0) __syncthreads();
 
     const float l_tot = pair_sum(l_i);
-    const int64_t partial = ((int64_t)(f.partial + split * f.work.blocks + block) * p.nkv + kvh) * kTileRows + wave * 32;     // of the wavefront's first row
+    const int64_t partial = ((int64_t)(f.partial + split * f.work.blocks + block) * p.nkv + kvh) * p.tile_rows + wave * 32;     // of the wavefront's first row
     uint64_t redo = 0;
     const int filled = (s1 + BN - 1) & -BN;                // tiles are filled up to here: with keys that a row may not see, or with others once more
     if (__any(row < n_rows && limit < filled)) {
@@ -809,57 +846,79 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
 }
 
 // ---- merge of the splits ------------------------------------------------------------------------------------------------------------------------------
-// A workgroup per (split block, KV head) or, of chunks, per 16 of its rows.  KIND 0: of paged_rows where the caller has no tickets, 1: of paged_tiles.  (Two lanes to a pair
-// of features and rows one after the other, with a workgroup for every partial result, most of them idle: 19 us for 64 blocks of 256 rows in four splits.)
-template <int D, int KIND>
-__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p) {
-    const int kvh = blockIdx.y;
-    if constexpr (KIND == 0) {
-        __shared__ float lds[16 * (D + 2)];
-        const Found f = find_work<kRowBlock, kRowTile, true>(p, p.rows, p.share_m[0], blockIdx.x);
-        if (f.b >= 0) merge_rows<D, false>(p, f, (int)blockIdx.x - f.at, kvh, lds);
-    } else {
-        const Found f = find_work<kTileRows, kTileKeys, true>(p, p.tiles, p.share_m[1], blockIdx.x);
+// A workgroup per split block and KV head of paged_rows (the first n_rows_groups; of blocks of 32 rows per 8 of them), where they are not merged in their own
+// launch, and per 16 rows of a block of paged_tiles.
+// (Two lanes to a pair of features and rows one after the other, with a workgroup for every partial result, most of them idle: 19 us for 64 blocks of 256 rows
+// in four splits, 8 so.  32 rows to a workgroup: the same, or 2 us more where rows are few.)
+template <int NB> constexpr int merged_rows() { return NB == 1 ? 16 : 8; }
+template <int D, int NB>
+__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p, int n_rows_groups, int sixteens) {
+    __shared__ float lds[16 * (D + 2)];
+    if ((int)blockIdx.x < n_rows_groups) {
+        constexpr int BLOCK = 16 * NB, EACH = merged_rows<NB>();
+        const int at_kv = blockIdx.x / (BLOCK / EACH), r0 = blockIdx.x % (BLOCK / EACH) * EACH, at = divide(at_kv, p.nkv, p.nkv_m), kvh = at_kv - at * p.nkv;
+        const Found f = find_work<BLOCK, kRowTile, true>(p, p.rows, p.share_m[0], at);
         if (f.b < 0) return;
-        const int block = (int)blockIdx.x - f.at, in = 16 * blockIdx.z + (threadIdx.x >> 4), row = block * kTileRows + in;
-        if (row >= f.seq.n * p.n_rep) return;
-        RowSum<D> sum;
-        sum.template add<false, 4>(p.tiles_o, p.tiles_ml, ((int64_t)(f.partial + block) * p.nkv + kvh) * kTileRows + in, (int64_t)f.work.blocks * p.nkv * kTileRows, f.splits);
-        const int token = divide(row, p.n_rep, p.rep_m);
-        sum.store(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh);
+        const int n = min(EACH, f.seq.n * p.n_rep - (at - f.at) * BLOCK - r0);
+        if (n > 0) merge_rows<D, BLOCK, false>(p, f, at - f.at, kvh, r0, n, lds);
+        return;
     }
+    const int group = blockIdx.x - n_rows_groups, at_kv = group / sixteens, z = group - at_kv * sixteens;
+    const int at = divide(at_kv, p.nkv, p.nkv_m), kvh = at_kv - at * p.nkv;
+    const Found f = find_work<kTileRows, kTileKeys, true>(p, p.tiles, p.share_m[1], at);
+    const int block = at - f.at, in = 16 * z + (threadIdx.x >> 4), row = block * kTileRows + in;
+    if (f.b < 0 || row >= f.seq.n * p.n_rep) return;
+    RowSum<D> sum;
+    sum.template add<false, 4>(p.tiles_o, p.tiles_ml, ((int64_t)(f.partial + block) * p.nkv + kvh) * p.tile_rows + in, (int64_t)f.work.blocks * p.nkv * p.tile_rows, f.splits);
+    const int token = divide(row, p.n_rep, p.rep_m);
+    sum.store(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh);
 }
 
-template <int D> int launch(const PagedParams& p, int64_t row_blocks, int64_t tile_blocks, hipStream_t st) {
+template <int D, int NB> int launch(const PagedParams& p, int64_t row_blocks, int64_t tile_blocks, hipStream_t st) {
     if (row_blocks > 0) {
-        paged_rows_kernel<D><<<dim3((unsigned)p.rows.max_slots * p.nkv), dim3(64 * kRowWaves), 0, st>>>(p);
+        paged_rows_kernel<D, NB><<<dim3((unsigned)p.rows.max_slots * p.nkv), dim3(64 * kRowWaves), 0, st>>>(p);
         if (const int rc = mi_check_launch("paged_rows"); rc != MI_OK) return rc;
     }
     if (tile_blocks > 0) {
         paged_tiles_kernel<D><<<dim3((unsigned)p.tiles.max_slots * p.nkv), dim3(512), 0, st>>>(p);
         if (const int rc = mi_check_launch("paged_tiles"); rc != MI_OK) return rc;
     }
-    if (p.rows.share > 0 && p.tickets == nullptr) paged_merge_kernel<D, 0><<<dim3((unsigned)paged_max_split_blocks(p.rows, row_blocks), p.nkv), dim3(256), 0, st>>>(p);
-    if (p.tiles.share > 0) {
-        const int64_t rows = std::min<int64_t>((int64_t)p.tiles.max_n * p.n_rep, kTileRows);          // of a block, as many as there may be
-        paged_merge_kernel<D, 1><<<dim3((unsigned)paged_max_split_blocks(p.tiles, tile_blocks), p.nkv, (unsigned)((rows + 15) / 16)), dim3(256), 0, st>>>(p);
-    }
+    const int64_t of_rows = p.rows.share > 0 && p.tickets == nullptr ? paged_max_split_blocks(p.rows, row_blocks) * p.nkv * (16 * NB / merged_rows<NB>()) : 0;
+    const int sixteens = (std::min<int>(p.tile_rows, kTileRows) + 15) / 16;
+    const int64_t groups = of_rows + paged_max_split_blocks(p.tiles, tile_blocks) * p.nkv * sixteens;
+    if (groups == 0) return MI_OK;
+    paged_merge_kernel<D, NB><<<dim3((unsigned)groups), dim3(256), 0, st>>>(p, (int)of_rows, sixteens);
     return mi_check_launch("paged_merge");
 }
 
-// Workgroups per KV head that either kernel's work is cut for.  `items`: blocks of rows x KV heads of the calls, as many as there may be.
-// paged_rows, of which two to four share a compute unit: of many items small pieces keep the units even where lengths differ (8 workgroups to a unit), and 2 do
-// where they do not; of few items more splits of each only make the merge longer.  (us of 512, 1024, 2048 workgroups, d 128: 32 x 8 items of 200 - 8192
-// keys 98, 93, 87, all of 4096 keys 85, 85, 92; 3 x 4 items of 20000 - 32768 keys of 64 features 18.6, 19.2, 19.3 and for the merge 7, 13, 19.)
-constexpr int kRowsLeast = 2, kRowsMost = 8;             // per compute unit
+// Workgroups per KV head that either kernel's work is cut for.  `items`: sequences x KV heads of the calls, as many as there may be.
+// paged_rows, of which two or three share a compute unit: of many items small pieces keep the units even where lengths differ (8 workgroups to a unit, 6 of
+// blocks of 32 rows), and 2 do where they do not; of few items more splits of each only make the merge longer.  (us of 512, 1024, 2048 workgroups, d 128: 32 x 8
+// items of 200 - 8192 keys 98, 93, 87, all of 4096 keys 85, 85, 92; 8 x 8 items of 900 - 5000 keys and 3 - 9 tokens
+// of 4 heads 39.9, 46.6 of 1024; 3 x 4 items of 20000 - 32768 keys of 64 features 23.9, 27.4 of 1024.  32 x 8 items of 20 rows, 200 - 8192 keys: 6 to a unit 123, 8 to a unit 130.)
+constexpr int kRowsLeast = 2, kRowsMost = 8, kRowsMostWide = 6;     // per compute unit
 int share_of(int64_t workgroups, int nkv) { return workgroups / nkv > 0 ? (int)(workgroups / nkv) : 1; }
-void make_plans(int64_t tokens, int64_t items, int n_rep, int nkv, PagedPlan& rows, PagedPlan& tiles) {
+// paged_tiles, one to a compute unit: few blocks are cut into what runs at once.  Of many blocks of few rows (`longest` tokens to a sequence, whose partial
+// results are small) pieces are up to four times smaller, as above.
+struct Plans {
+    PagedPlan rows, tiles;
+    int row_block, tile_rows;                              // rows of a block of paged_rows; rows kept per partial result of paged_tiles
+};
+Plans make_plans(int64_t tokens, int64_t items, int64_t longest, int n_rep, int nkv) {
     const int cus = mi_compute_units();
     const bool few = 8 * items <= kRowsLeast * cus;
-    rows = PagedPlan{0, kRowLimit, 0x7fffffff, share_of(few ? kRowsLeast * cus : std::min<int64_t>(8 * items, kRowsMost * cus), nkv), 8 * items >= kRowsMost * cus, 0, 0, 0};
+    const int64_t most = longest * n_rep;
+    Plans o;
+    o.row_block = most <= kRowBlock ? kRowBlock : 2 * kRowBlock;
+    const int limit = few && most <= kRowsAlone ? kRowsAlone : kRowLimit;
+    const int64_t rows_most = (o.row_block == kRowBlock ? kRowsMost : kRowsMostWide) * cus;
+    o.rows = PagedPlan{0, limit, 0x7fffffff, share_of(few ? kRowsLeast * cus : std::min<int64_t>(8 * items, rows_most), nkv), 8 * items >= rows_most, 0, 0, 0};
     // Enough blocks for every compute unit: no splits, no merge.
     const bool many = tokens * n_rep / kTileRows * nkv >= cus;
-    tiles = PagedPlan{kRowLimit, 0x7fffffff, 0x7fffffff, many ? 0 : share_of(cus, nkv), 0, 1, 0, 0};
+    o.tile_rows = (int)std::min<int64_t>((most + 15) / 16 * 16, kTileRows);
+    const int pieces = o.tile_rows * 4 <= kTileRows ? 4 : o.tile_rows * 2 <= kTileRows ? 2 : 1, at_once = share_of(cus, nkv);
+    o.tiles = PagedPlan{limit, 0x7fffffff, 0x7fffffff, many ? 0 : pieces * at_once, 0, many ? 0 : at_once, 0, 0};
+    return o;
 }
 // Whether the last workgroup of a block merges, given tickets: no more workgroups than run at once.  Each waits for its results to be in memory, which more of them
 // cannot hide: 32 x 8 items of 200 - 8192 keys in pieces for 2048 workgroups 100 us, with a launch of its own for the merge 92.
@@ -873,18 +932,17 @@ constexpr int64_t kMaxTiles = (1 << 24) + 1;              // of a sequence
 #ifndef MI_ELEM_F16
 extern "C" int64_t mi_paged_attn_tickets(int32_t n_kv_heads) {
     if (n_kv_heads <= 0) return 0;
-    PagedPlan rows, tiles;
-    make_plans(0, 0x7fffffff, 1, n_kv_heads, rows, tiles);
-    return paged_max_partials(rows, kMaxTiles, kMaxTiles) * n_kv_heads;
+    return paged_max_partials(make_plans(0, 0x7fffffff, 1, 1, n_kv_heads).rows, kMaxTiles, kMaxTiles) * n_kv_heads;
 }
 
 extern "C" size_t mi_paged_attn_workspace_bytes(int64_t tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
     if (tokens <= 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || head_dim <= 0) return 0;
-    PagedPlan rows, tiles;
     const int n_rep = n_q_heads / n_kv_heads;
-    make_plans(0, 0x7fffffff, n_rep, n_kv_heads, rows, tiles);         // for so many tokens or fewer, of any number of sequences
-    return partial_bytes(paged_max_partials(rows, kMaxTiles, kMaxTiles), n_kv_heads, kRowBlock, head_dim) +
-           (tokens * n_rep > kRowLimit ? partial_bytes(paged_max_partials(tiles, kMaxTiles, kMaxTiles), n_kv_heads, kTileRows, head_dim) : 0);
+    const bool chunks = tokens * n_rep > kRowLimit;
+    // of any number of sequences, with chunks of any length: of shorter ones there are more pieces of fewer rows, no more together
+    const Plans o = make_plans(0, 0x7fffffff, chunks ? kTileRows : tokens, n_rep, n_kv_heads);
+    return partial_bytes(paged_max_partials(o.rows, kMaxTiles, kMaxTiles), n_kv_heads, o.row_block, head_dim) +
+           (chunks ? partial_bytes(paged_max_partials(o.tiles, kMaxTiles, kMaxTiles), n_kv_heads, kTileRows, head_dim) : 0);
 }
 #endif
 
@@ -912,23 +970,27 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
     p.capacity = a->max_pages * a->page_size; p.nq = a->n_q_heads; p.nkv = a->n_kv_heads; p.n_rep = a->n_q_heads / a->n_kv_heads; p.causal = a->causal != 0;
     p.page_m = divide_m(p.page); p.rep_m = divide_m(p.n_rep); p.nkv_m = divide_m(p.nkv);
     p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
-    make_plans(p.total, std::min<int64_t>(p.batch, p.total) * p.nkv, p.n_rep, p.nkv, p.rows, p.tiles);
     const int64_t longest = a->max_q_len > 0 && a->max_q_len < p.total ? a->max_q_len : p.total;
+    const Plans plans = make_plans(p.total, std::min<int64_t>(p.batch, p.total) * p.nkv, longest, p.n_rep, p.nkv);
+    p.rows = plans.rows;
+    p.tiles = plans.tiles;
+    p.tile_rows = plans.tile_rows;
+    const bool two = plans.row_block == 2 * kRowBlock;
     p.rows.max_n = p.tiles.max_n = (int)longest;
-    const int64_t row_blocks = paged_max_blocks<kRowBlock>(p.rows, p.total, p.batch, longest, p.n_rep);
+    const int64_t row_blocks = two ? paged_max_blocks<2 * kRowBlock>(p.rows, p.total, p.batch, longest, p.n_rep) : paged_max_blocks<kRowBlock>(p.rows, p.total, p.batch, longest, p.n_rep);
     const int64_t tile_blocks = paged_max_blocks<kTileRows>(p.tiles, p.total, p.batch, longest, p.n_rep);
     const int64_t row_tiles = ((int64_t)p.capacity + kRowTile - 1) / kRowTile, tile_tiles = ((int64_t)p.capacity + kTileKeys - 1) / kTileKeys;
     // Sums of blocks x tiles and of rows are kept in 32 bits, and a grid has fewer than 2^31 workgroups.
     if (p.nkv > 0xffff) return mi_fail(MI_E_SHAPE, "paged_attn: more than 65535 KV heads");
     if ((int64_t)p.total * p.n_rep > 0x7fffffffLL - kTileRows || row_blocks * row_tiles > 0x7fffffffLL || tile_blocks * tile_tiles > 0x7fffffffLL ||
-        (row_blocks + tile_blocks + 8LL * mi_compute_units()) * p.nkv > 0x7fffffffLL)
+        (4 * row_blocks + 17 * tile_blocks + 8LL * mi_compute_units()) * p.nkv > 0x7fffffffLL)
         return mi_fail(MI_E_SHAPE, "paged_attn: %lld tokens of %d heads over up to %d keys are too many for one call", (long long)a->total_q, a->n_q_heads, p.capacity);
     const size_t need = mi_paged_attn_workspace_bytes(p.total, p.nq, p.nkv, a->head_dim);
     if (!a->workspace || a->workspace_bytes < need || !mi_aligned16(a->workspace))
         return mi_fail(MI_E_WORKSPACE, "paged_attn: workspace needs %zu bytes (16-byte aligned), got %zu", need, a->workspace_bytes);
     if (a->tickets && (a->n_tickets < mi_paged_attn_tickets(p.nkv) || (reinterpret_cast<uintptr_t>(a->tickets) & 3u) != 0))
         return mi_fail(MI_E_WORKSPACE, "paged_attn: %lld tickets (4-byte aligned), got %lld", (long long)mi_paged_attn_tickets(p.nkv), (long long)a->n_tickets);
-    p.tickets = merges_in_launch(p.rows, p.nkv) ? a->tickets : nullptr;
+    p.tickets = !two && merges_in_launch(p.rows, p.nkv) ? a->tickets : nullptr;
     // A sequence of up to a tile of keys has one split, whatever the plan.
     if (row_tiles == 1 || row_blocks == 0) p.rows.share = 0;
     if (tile_tiles == 1 || tile_blocks == 0) p.tiles.share = 0;
@@ -938,14 +1000,18 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
     p.rows.max_partials = (int)paged_max_partials(p.rows, row_blocks, row_tiles);
     p.tiles.max_partials = (int)paged_max_partials(p.tiles, tile_blocks, tile_tiles);
     p.rows_o = (float*)a->workspace;
-    p.rows_ml = p.rows_o + (size_t)p.rows.max_partials * p.nkv * kRowBlock * a->head_dim;
-    p.tiles_o = p.rows_o + partial_bytes(p.rows.max_partials, p.nkv, kRowBlock, a->head_dim) / sizeof(float);
-    p.tiles_ml = p.tiles_o + (size_t)p.tiles.max_partials * p.nkv * kTileRows * a->head_dim;
+    p.rows_ml = p.rows_o + (size_t)p.rows.max_partials * p.nkv * plans.row_block * a->head_dim;
+    p.tiles_o = p.rows_o + partial_bytes(p.rows.max_partials, p.nkv, plans.row_block, a->head_dim) / sizeof(float);
+    p.tiles_ml = p.tiles_o + (size_t)p.tiles.max_partials * p.nkv * p.tile_rows * a->head_dim;
     const hipStream_t st = (hipStream_t)a->stream;
+    const auto go = [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        return two ? launch<D, 2>(p, row_blocks, tile_blocks, st) : launch<D, 1>(p, row_blocks, tile_blocks, st);
+    };
     switch (a->head_dim) {
-        case 32: return launch<32>(p, row_blocks, tile_blocks, st);
-        case 64: return launch<64>(p, row_blocks, tile_blocks, st);
-        case 96: return launch<96>(p, row_blocks, tile_blocks, st);
-        default: return launch<128>(p, row_blocks, tile_blocks, st);
+        case 32: return go(std::integral_constant<int, 32>{});
+        case 64: return go(std::integral_constant<int, 64>{});
+        case 96: return go(std::integral_constant<int, 96>{});
+        default: return go(std::integral_constant<int, 128>{});
     }
 }

@@ -59,7 +59,7 @@ struct PagedPlan {
     int max_n;                    // ... and at most so many new tokens
     int share;                    // workgroups per KV head aimed at; 0: never split
     int even;                     // sequences of about one length: cut for a quarter of the share
-    int fit;                      // whether a workgroup has a compute unit for itself, and more of them than that are to be avoided
+    int fit;                      // workgroups per KV head that run at once: few blocks are cut for no more of them; 0: no such line
     int max_slots, max_partials;  // (set by the host) workgroups and partial results per KV head that there are
 };
 
@@ -75,20 +75,23 @@ template <int BLOCK, int TILE> MI_PLAN_FN PagedWork paged_work(const PagedPlan& 
     return w;
 }
 // What is divided by the share for the tiles of a split, less one.  units: W; blocks: of all sequences; most: tiles of the longest
+MI_PLAN_FN bool paged_few(const PagedPlan& p, int64_t blocks) { return p.fit > 0 && 2 * blocks <= p.fit; }
 MI_PLAN_FN uint32_t paged_units(const PagedPlan& p, int64_t units, int64_t blocks, int most) {
     if (p.even && most * blocks * 4 <= units * 5) units *= 4;
+    if (paged_few(p, blocks)) units *= p.share / p.fit;
     return (uint32_t)(units < 0x7fffffff ? units : 0x7fffffff);
 }
 MI_PLAN_FN int paged_split_tiles(const PagedPlan& p, int64_t units, int64_t blocks, int most) {
     if (p.share == 0) return 0x1000000;                    // no sequence has more
     return (int)(paged_units(p, units, blocks, most) / (uint32_t)p.share) + 1;
 }
-// Where all blocks together fit, S grows until their splits do too: one workgroup more than there is room for at once would take as long as all others.
-// `slots`: splits of all blocks at S.  S / slots only shrinks towards the room, so a few steps do.
+// Of few blocks S grows until their splits run at once: one workgroup more would take as long as all others.  `slots`: splits of all blocks at S.  After
+// kPagedSteps steps S is W / (fit - blocks) + 1, which sum(ceil(tiles / S)) < W / S + blocks leaves no more than fit of.
 constexpr int kPagedSteps = 3;
-MI_PLAN_FN int paged_next_tiles(const PagedPlan& p, int split_tiles, int64_t blocks, int64_t slots) {
-    if (!p.fit || blocks > p.share || slots <= p.share) return split_tiles;
-    const int64_t next = (int64_t)((float)split_tiles * (float)slots / (float)p.share);
+MI_PLAN_FN int paged_next_tiles(const PagedPlan& p, int split_tiles, int64_t units, int64_t blocks, int64_t slots, int step) {
+    if (!paged_few(p, blocks) || slots <= p.fit) return split_tiles;
+    if (step == kPagedSteps) return paged_clamp((int64_t)((float)units / (float)(p.fit - blocks) * 1.000001f) + 1, 1, 0x1000000);
+    const int64_t next = (int64_t)((float)split_tiles * (float)slots / (float)p.fit);
     return paged_clamp(next > split_tiles ? next : (int64_t)split_tiles + 1, 1, 0x1000000);
 }
 MI_PLAN_FN int paged_splits(const PagedWork& w, int split_tiles) { return paged_quotient(w.tiles - 1, split_tiles) + 1; }
@@ -117,7 +120,7 @@ template <int BLOCK> MI_PLAN_FN int64_t paged_max_blocks(const PagedPlan& p, int
     return each < together ? each : together;
 }
 MI_PLAN_FN int64_t paged_max_slots(const PagedPlan& p, int64_t blocks, int64_t max_tiles) {
-    const int64_t each = blocks * max_tiles, together = blocks + p.share + 1;
+    const int64_t each = blocks * max_tiles, together = paged_few(p, blocks) ? p.fit : blocks + p.share + 1;
     return p.share == 0 || blocks == 0 ? blocks : each < together ? each : together;
 }
 // blocks of sequences with more than one split

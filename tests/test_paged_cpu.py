@@ -21,7 +21,9 @@ static int fail(const char* what, int i) { printf("case %%d: %%s\n", i, what); r
 template <int BLOCK, int TILE>
 static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, int capacity, int longest, bool good, bool causal, const std::vector<int>& cu,
                   const std::vector<int>& ctx, std::vector<int>& taken) {
-    PagedPlan p = {over, up_to, longest, rnd() %% 4 == 0 ? 0 : 1 << rnd() %% 9, (int)(rnd() & 1), (int)(rnd() & 1), 0, 0};
+    PagedPlan p = {over, up_to, longest, rnd() %% 4 == 0 ? 0 : 1 << rnd() %% 9, 0, 0, 0, 0};
+    if (rnd() & 1) p.even = rnd() & 1;
+    else if (rnd() & 1) p.fit = p.share >> rnd() %% 3;
     const int max_tiles = (capacity + TILE - 1) / TILE;
     const int64_t most = paged_max_blocks<BLOCK>(p, total, batch, longest, n_rep);
     p.max_slots = (int)paged_max_slots(p, most, max_tiles);
@@ -41,14 +43,17 @@ static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, i
         if (w.blocks > 0 && w.tiles > longest_tiles) longest_tiles = w.tiles;
     }
     int S = paged_split_tiles(p, units, all, longest_tiles);
-    for (int step = 0; p.share > 0 && step < kPagedSteps; ++step) {
+    for (int step = 0; p.share > 0 && step <= kPagedSteps; ++step) {
         int64_t n = 0;
         for (int b = 0; b < batch; ++b) {
             const PagedWork w = paged_work<BLOCK, TILE>(p, paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity), n_rep);
             n += (int64_t)w.blocks * paged_splits(w, S);
         }
-        const int next = paged_next_tiles(p, S, all, n);
-        if (next < S || ((next == S) != (!p.fit || all > p.share || n <= p.share))) return fail("tiles of a split do not grow", c);
+        const int next = paged_next_tiles(p, S, units, all, n, step);
+        if (next == S || (step < kPagedSteps && next < S)) {
+            if (next != S || (paged_few(p, all) && n > p.fit && next < 0x1000000)) return fail("tiles of a split do not grow", c);
+            break;
+        }
         S = next;
     }
     if (S < 1) return fail("no tiles to a split", c);
@@ -101,8 +106,10 @@ int main() {
         int longest = 0;
         std::vector<int> taken(good ? total : 0, 0);
         for (int b = 0; b < batch; ++b) { const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity); if (s.n > longest) longest = s.n; }
-        if (kernel<16, 128>(c, 0, 16, batch, n_rep, total, capacity, longest, good, causal, cu, ctx, taken)) return 1;
-        if (kernel<256, 64>(c, 16, 0x7fffffff, batch, n_rep, total, capacity, longest, good, causal, cu, ctx, taken)) return 1;
+        if (c & 1) {
+            if (kernel<16, 128>(c, 0, 32, batch, n_rep, total, capacity, longest, good, causal, cu, ctx, taken)) return 1;
+        } else if (kernel<32, 128>(c, 0, 32, batch, n_rep, total, capacity, longest, good, causal, cu, ctx, taken)) return 1;
+        if (kernel<256, 64>(c, 32, 0x7fffffff, batch, n_rep, total, capacity, longest, good, causal, cu, ctx, taken)) return 1;
         for (int t : taken) if (t != 1) return fail("a token that is not exactly one kernel's", c);
     }
     printf("ok\n");
