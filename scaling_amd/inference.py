@@ -6,7 +6,8 @@ layer loop (core/nn/parallel_module/inference_module.py:100-109), prefill + one-
 decoding with greedy sampling (transformer/inference/inference_model.py:223-263, inference/sample.py:5-6)
 and the per-layer checkpoint files `model_state_layer_{i}_{Class}.pt`
 (core/nn/parallel_module/partitioned_module.py:246-408).  Unlike the reference the cached path accepts
-a batch of prompts of equal length (the reference asserts batch size 1, attention.py:855-857).
+a batch of prompts of equal length (the reference asserts batch size 1, attention.py:855-857), and
+`generate_ragged` one of different lengths over a paged cache.
 Embedding lookup, LM head matmul and arg-max stay on PyTorch-ROCm.
 """
 
@@ -23,7 +24,7 @@ from .data import get_cumulative_seq_lengths, get_position_ids
 from . import ops
 from .layer import InferenceSettings, LayerNormWrapper, TransformerLayer, TransformerLayerIO
 from .loss import TransformerLMHead
-from .nn import RMSNorm, _unhooked, decode_arguments
+from .nn import PagedKVCache, PagedStep, RMSNorm, _unhooked, decode_arguments
 
 # class names written by older versions of the reference (partitioned_module.py:25-32)
 LEGACY_CLASS_NAMES = {"LuminousEmbeddingInput": "EmbeddingInput", "LuminousLayer": "TransformerLayer",
@@ -328,3 +329,62 @@ class TransformerInferenceModule(torch.nn.Module):
                 if b == 1 and completions[0][-1] in stop:
                     break
         return completions, torch.stack(step_logits, dim=1)
+
+    # ---- sequences of different lengths ------------------------------------------------------------------
+    def paged_cache(self, max_sequences: int, max_ctx: Optional[int] = None, num_pages: Optional[int] = None, page_size: int = 64) -> PagedKVCache:
+        """A paged cache for all layers: up to `max_sequences` sequences of up to `max_ctx` tokens (default: what the layers' own caches hold), `num_pages` pages in
+        all (default: enough for every sequence at its longest)."""
+        layers = list(self._layers[1:-2])
+        att = layers[0].self_attention
+        max_ctx = att._cache_capacity() if max_ctx is None else max_ctx
+        num_pages = max_sequences * -(-max_ctx // page_size) if num_pages is None else num_pages
+        return PagedKVCache(len(layers), num_pages, max_sequences, max_ctx, att.num_attention_heads, att.num_kv_heads_per_partition,
+                            att.hidden_size_per_attention_head, att.dtype, self.device, page_size)
+
+    @torch.no_grad()
+    def paged_forward(self, token_ids: torch.Tensor, cache: PagedKVCache, step: PagedStep) -> torch.Tensor:
+        """token_ids [tokens]: the new tokens of `step`, sequence after sequence -> logits [n, vocab] behind the last new token of each of the n sequences
+        that have any."""
+        h = self._layers[0](token_ids.to(self.device).view(1, -1))
+        for layer in self._layers[1:-2]:
+            h = layer.paged_step(h, cache, step)
+        h = h[0].index_select(0, step.last).unsqueeze(1)
+        logits = self._last_logits(h)
+        if logits is None:
+            logits = self._layers[-1].linear(self._layers[-2](TransformerLayerIO(activations=h, position_ids=None)).activations)
+        return logits[:, -1, :]
+
+    @torch.no_grad()
+    def generate_ragged(self, max_tokens: int, prompts: Sequence[Sequence[int]], stop_tokens: Optional[Sequence[int]] = None,
+                        page_size: int = 64) -> List[List[int]]:
+        """Greedy completions of prompts of different lengths, in one batch over a paged cache: `max_tokens` ids per prompt, or up to and with the first one in
+        `stop_tokens`, after which the sequence leaves the batch and gives its pages back.  A prompt is one document, whatever ids it has."""
+        prompts = [[int(t) for t in p] for p in prompts]
+        if max_tokens < 1 or not prompts or not all(prompts):
+            raise ValueError("at least one prompt, no empty one, and at least one token to generate")
+        longest = max(len(p) for p in prompts) + max_tokens - 1
+        cache = self.paged_cache(len(prompts), longest, sum(-(-(len(p) + max_tokens - 1) // page_size) for p in prompts), page_size)
+        stop = set(stop_tokens or [])
+        completions: List[List[int]] = [[] for _ in prompts]
+        active = list(range(len(prompts)))
+        logits = self.paged_forward(torch.tensor([t for p in prompts for t in p]), cache, cache.step([len(p) for p in prompts]))
+        kept = []                                        # without stop tokens the ids are read back once, at the end
+        for k in range(max_tokens):
+            tokens = sample_argmax(logits.unsqueeze(1))
+            if stop:
+                ids = tokens.tolist()
+                for b, t in zip(active, ids):
+                    completions[b].append(t)
+                stays = [i for i, t in enumerate(ids) if t not in stop]
+                for i in set(range(len(ids))) - set(stays):
+                    cache.release(active[i])
+                if len(stays) < len(ids):
+                    active = [active[i] for i in stays]
+                    tokens = tokens[torch.tensor(stays, dtype=torch.int64, device=tokens.device)]
+            else:
+                kept.append(tokens)
+            if k + 1 == max_tokens or not active:
+                break
+            going = set(active)
+            logits = self.paged_forward(tokens, cache, cache.step([int(b in going) for b in range(len(prompts))]))
+        return completions if stop else torch.stack(kept, dim=1).tolist()

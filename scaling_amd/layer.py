@@ -10,7 +10,7 @@ from typing import Callable, List, Optional
 import torch
 
 from .config import MLPType, TransformerArchitectureConfig
-from .nn import ParallelMLP, ParallelSelfAttention, ParallelSwiGLUMLP, RMSNorm, _direct, _unhooked, decode_layer, fuses_residual, get_norm, idle_dropout, layer_in_one_call, one_token_each
+from .nn import PagedKVCache, PagedStep, ParallelMLP, ParallelSelfAttention, ParallelSwiGLUMLP, RMSNorm, _direct, _unhooked, decode_layer, fuses_residual, get_norm, idle_dropout, layer_in_one_call, one_token_each
 
 
 class InferenceSettings:
@@ -108,6 +108,16 @@ class TransformerLayer(torch.nn.Module):
         """Cached single-token step on plain tensors, free of host synchronisation (HIP-graph capturable)."""
         h = hidden_state + self.self_attention.decode_forward(self.input_layernorm(hidden_state), position_ids, cache_index,
                                                               advance=advance)
+        return h + self.mlp(self.post_attention_layernorm(h))
+
+    def paged_step(self, hidden_state: torch.Tensor, cache: PagedKVCache, step: PagedStep) -> torch.Tensor:
+        """The layer on the new tokens of a step over a paged cache, whose layer `layer_index` is this one's (inference; see
+        ParallelSelfAttention.paged_forward)."""
+        if self._own_blocks() and fuses_residual(self.input_layernorm) and fuses_residual(self.post_attention_layernorm):
+            h, n = self.input_layernorm.with_residual(hidden_state)
+            h, n = self.post_attention_layernorm.with_residual(self.self_attention.paged_forward(n, cache, self.layer_index, step), h)
+            return self.mlp(n, h) if fuses_residual(self.mlp) else self.mlp(n) + h
+        h = hidden_state + self.self_attention.paged_forward(self.input_layernorm(hidden_state), cache, self.layer_index, step)
         return h + self.mlp(self.post_attention_layernorm(h))
 
     def forward(self, x: TransformerLayerIO) -> TransformerLayerIO:

@@ -8,7 +8,7 @@ do not cover raise `NotImplementedError` instead of silently taking another path
 """
 
 import math
-from typing import Callable, Dict, Optional, Tuple
+from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import torch
 
@@ -407,6 +407,98 @@ class KVCache:
         self.workspace: Optional[torch.Tensor] = None
 
 
+class PagedStep:
+    """What one call over a PagedKVCache brings (PagedKVCache.step makes it): the new tokens of all sequences behind each other.  On the device: `cu_seqlens`
+    int32 [sequences + 1], `ctx_len` int32 [sequences] including the new tokens, `position_ids` int64 [tokens], `last` int64: the last new token of each sequence
+    that has any.  On the host: `tokens`, `max_q_len` (new tokens of one sequence at the most) and `longest` (its keys)."""
+
+    def __init__(self, new: Sequence[int], lengths: Sequence[int], device: torch.device) -> None:
+        n, self.tokens = len(new), sum(new)
+        self.max_q_len, self.longest = max(new), max(lengths)
+        ends = torch.tensor([0] + list(new), device="cpu").cumsum(0)
+        last = [int(e) - 1 for e, count in zip(ends[1:], new) if count > 0]
+        positions = [torch.arange(length - count, length, device="cpu") for count, length in zip(new, lengths)]
+        # one copy to the device: int64 parts first, which keeps them aligned
+        sizes = [2 * self.tokens, 2 * len(last), n + 1, n]
+        packed = torch.empty(sum(sizes), dtype=torch.int32, device="cpu", pin_memory=device.type == "cuda")
+        parts = packed.split(sizes)
+        torch.cat(positions, out=parts[0].view(torch.int64))
+        parts[1].view(torch.int64).copy_(torch.tensor(last, dtype=torch.int64, device="cpu"))
+        parts[2].copy_(ends)
+        parts[3].copy_(torch.tensor(lengths, device="cpu"))
+        parts = packed.to(device, non_blocking=True).split(sizes)
+        self.position_ids, self.last, self.cu_seqlens, self.ctx_len = parts[0].view(torch.int64), parts[1].view(torch.int64), parts[2], parts[3]
+
+
+class PagedKVCache:
+    """Keys and values of up to `max_sequences` sequences of different lengths for `num_layers` layers, in `num_pages` pages of `page_size` keys (a multiple of 16)
+    that sequences take as they grow and give back when they end.  Where KVCache has max_ctx keys for every sequence of a batch, here only the pages that are in
+    use count, sequences come and go, and a call brings any number of tokens of each: `step`, then ParallelSelfAttention.paged_forward of every layer.
+
+    Pages are stored head-major ([page, kv head, key, d]), as KVCache is.  The host keeps lengths and pages; nothing is read back from the device.  The calls over one
+    cache belong on one stream at a time: table, pages and workspace are shared."""
+
+    def __init__(self, num_layers: int, num_pages: int, max_sequences: int, max_ctx: int, n_q: int, n_kv: int, head_dim: int, dtype, device,
+                 page_size: int = 64) -> None:
+        if page_size < 16 or page_size % 16 != 0:
+            raise ValueError(f"page_size {page_size} is no multiple of 16")
+        if min(num_layers, num_pages, max_sequences, max_ctx) < 1:
+            raise ValueError("a paged cache has at least one layer, page, sequence and key")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise NotImplementedError("the paged attention kernels take bfloat16 or float16 tensors")
+        self.device, self.page_size, self.max_ctx, self.max_sequences = torch.device(device), page_size, max_ctx, max_sequences
+        self.n_q, self.n_kv, self.head_dim = n_q, n_kv, head_dim
+        shape = (num_pages, n_kv, page_size, head_dim)
+        self.k_pages = [torch.zeros(shape, dtype=dtype, device=device).transpose(1, 2) for _ in range(num_layers)]
+        self.v_pages = [torch.zeros(shape, dtype=dtype, device=device).transpose(1, 2) for _ in range(num_layers)]
+        self.lengths = [0] * max_sequences
+        self._pages: List[List[int]] = [[] for _ in range(max_sequences)]
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._table = torch.zeros(max_sequences, -(-max_ctx // page_size), dtype=torch.int32, device="cpu")
+        self.page_table = self._table.to(device, copy=True)
+        self._workspace: Optional[Tuple[int, torch.Tensor]] = None
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def step(self, new: Sequence[int]) -> PagedStep:
+        """Takes pages for new[b] more tokens of sequence b (0: none; one entry per sequence the cache has room for, or fewer: the first ones) and returns what the
+        layers' calls need.  Raises, with nothing taken, if a sequence would pass max_ctx or the pages run out."""
+        new = [int(count) for count in new]
+        if not 0 < len(new) <= self.max_sequences or min(new) < 0 or sum(new) == 0:
+            raise ValueError(f"new tokens of 1 to {self.max_sequences} sequences, at least one token in all, got {new}")
+        lengths = [length + count for length, count in zip(self.lengths, new)]
+        if max(lengths) > self.max_ctx:
+            raise ValueError(f"a sequence of {max(lengths)} tokens does not fit a cache of {self.max_ctx}")
+        wanted = [-(-length // self.page_size) - len(pages) for length, pages in zip(lengths, self._pages)]
+        if sum(wanted) > len(self._free):
+            raise RuntimeError(f"{sum(wanted)} more pages are needed, {len(self._free)} are free")
+        for b, count in enumerate(wanted):
+            for _ in range(count):
+                self._table[b, len(self._pages[b])] = self._free[-1]
+                self._pages[b].append(self._free.pop())
+        if sum(wanted) > 0:
+            host = torch.empty(self._table.shape, dtype=torch.int32, device="cpu", pin_memory=True).copy_(self._table) if self.device.type == "cuda" else self._table
+            self.page_table.copy_(host, non_blocking=True)
+        self.lengths[:len(new)] = lengths
+        return PagedStep(new, lengths, self.device)
+
+    def release(self, sequence: int) -> None:
+        """The sequence ends: its pages are free for others (behind the calls that are on the stream), and its place starts again at length 0."""
+        if not 0 <= sequence < self.max_sequences:
+            raise IndexError(f"sequence {sequence} of {self.max_sequences}")
+        self._free.extend(reversed(self._pages[sequence]))
+        self._pages[sequence] = []
+        self.lengths[sequence] = 0
+
+    def workspace(self, tokens: int) -> torch.Tensor:
+        """Scratch of ops.paged_attention, kept from call to call."""
+        if self._workspace is None or self._workspace[0] < tokens:
+            self._workspace = tokens, ops.paged_workspace(self.max_sequences, tokens, self.n_q, self.n_kv, self.head_dim, self.device)
+        return self._workspace[1]
+
+
 class ParallelSelfAttention(torch.nn.Module):
     """Mirror of core/nn/attention/attention.py:509-969 for `masked_softmax.kernel = hip`.
 
@@ -416,7 +508,10 @@ class ParallelSelfAttention(torch.nn.Module):
     from a counter-based hash, not from torch's generator stream, and its rate is quantised to 1/256);
     float32 (the reference's default precision) runs separate exact-fp32 kernels without dropout, fused rotary or
     KV cache.  The KV cache is pre-allocated (see `KVCache`), supports batches of
-    single-document rows and is filled/extended in place.
+    single-document rows and is filled/extended in place; for sequences of different lengths see `PagedKVCache` and `paged_forward`.
+
+    `norm_rotary_in_one` (an argument of its own, off by default; may be set later): with `key_query_norm`, `forward` norms and rotates
+    queries and keys in one launch (ops.norm_rotary) instead of two norms and a rotary, which rounds once where they round after each.
     """
 
     def __init__(self, hidden_size: int, num_attention_heads: int, masked_softmax_config: MaskedSoftmaxConfig,
@@ -431,7 +526,8 @@ class ParallelSelfAttention(torch.nn.Module):
                  qkv_in_one: bool = True, num_kv_heads: Optional[int] = None, use_matmul: bool = False,
                  umup_mult: Optional[float] = None, umup_is_first_layer: Optional[bool] = None,
                  umup_is_last_layer: Optional[bool] = None, umup_on_residual: Optional[bool] = None,
-                 fp8_config=None, fp8_config_dense_out=None, max_cache_length: Optional[int] = None) -> None:
+                 fp8_config=None, fp8_config_dense_out=None, max_cache_length: Optional[int] = None,
+                 norm_rotary_in_one: bool = False) -> None:
         super().__init__()
         self._device = _default_device(device, topology)
         assert hidden_size % num_attention_heads == 0, \
@@ -493,6 +589,7 @@ class ParallelSelfAttention(torch.nn.Module):
             rotary_config.dimensions == self.hidden_size_per_attention_head and self.hidden_size_per_attention_head in (64, 128)
 
         self.key_query_norm = key_query_norm
+        self.norm_rotary_in_one = norm_rotary_in_one
         self.norm_query = self.norm_key = None
         if key_query_norm:
             self.norm_query = get_norm(norm_type, layernorm_config, d, self._device, dtype)
@@ -601,9 +698,13 @@ class ParallelSelfAttention(torch.nn.Module):
                 ctx = sdpa.forward_tokens(qkv[..., :d], qkv[..., d:2 * d], qkv[..., 2 * d:], cu, cu_k, rotary=rotary)
             return self.dense(ctx.view(b, s, nq * d))
         q, k, v = self._project(x)
+        norms, rotated = None, False
         if self.key_query_norm:
-            q = self.norm_query(q)
-            k = self.norm_key(k)
+            if self.norm_rotary_in_one and not (use_cache and not reset_cache) and (self.rotary_embedding is None or pos is not None):
+                norms = self._own_norms()
+            if norms is None:
+                q = self.norm_query(q)
+                k = self.norm_key(k)
 
         if use_cache:
             if not self.causal:
@@ -618,18 +719,74 @@ class ParallelSelfAttention(torch.nn.Module):
         self._check_positions(pos)
         cu_k = None if cumulative_seq_lengths_key is None else cumulative_seq_lengths_key.to(torch.int32)
 
-        if self._fusable_rotary and pos is not None and not use_cache:
+        if norms is not None:
+            rotary, interleaved = self._own_rotary(pos)
+            rotated = rotary is not None
+            q, k = ops.norm_rotary(q, k, **norms, rotary=rotary, interleaved=interleaved)
+        if self._fusable_rotary and pos is not None and not use_cache and not rotated:
             # rotary is applied while the kernels load Q and K (forward and backward); nothing rotated is stored
             cos, sin = self.rotary_embedding.tables()
             ctx = sdpa.forward_tokens(q, k, v, cu, cu_k, rotary=(cos, sin, pos, pos))
             return self.dense(ctx.view(b, s, nq * d))
-        if self.rotary_embedding is not None:
+        if self.rotary_embedding is not None and not rotated:
             q = self.rotary_embedding.rotate_tokens(q, pos, s)
             k = self.rotary_embedding.rotate_tokens(k, pos, s)
         if use_cache:  # prefill: keep post-rotary K and V (attention.py:861-862)
             self._fill_cache(k, v, b, s, cache_index)
         ctx = sdpa.forward_tokens(q, k, v, cu, cu_k)
         return self.dense(ctx.view(b, s, nq * d))
+
+    # ---- norms and rotary in one launch ---------------------------------------------------------------
+    def _own_norms(self) -> Optional[dict]:
+        """The norms over heads as arguments of ops.norm_rotary and ops.paged_append; None unless both are the package's, unhooked, and alike."""
+        norms = (self.norm_query, self.norm_key)
+        kind = type(norms[0])
+        if kind not in (RMSNorm, LayerNorm) or type(norms[1]) is not kind or norms[0].eps != norms[1].eps or not _unhooked(*norms):
+            return None
+        weights, biases = _weights(norms)
+        return dict(q_weight=weights[0], k_weight=weights[1], eps=norms[0].eps, q_bias=biases[0], k_bias=biases[1], layer_norm=kind is LayerNorm)
+
+    def _own_rotary(self, pos: Optional[torch.Tensor]) -> Tuple[Optional[tuple], bool]:
+        """(tables and positions, interleaved) as those take them; None where there is no rotary, or not the package's own."""
+        rot = self.rotary_embedding
+        if type(rot) not in (RotaryEmbedding, RotaryEmbeddingComplex) or "rotate_tokens" in rot.__dict__ or "tables" in rot.__dict__:
+            return None, False
+        interleaved = type(rot) is RotaryEmbeddingComplex
+        assert not interleaved or rot.dimensions == self.hidden_size_per_attention_head, "the interleaved variant rotates the whole head (rotary.py:69-70)"
+        return (*rot.tables(), pos), interleaved
+
+    # ---- paged KV cache ------------------------------------------------------------------------------
+    def paged_forward(self, x: torch.Tensor, cache: PagedKVCache, layer: int, step: PagedStep) -> torch.Tensor:
+        """Attention of the new tokens that `step` (of cache.step) brings, x [b, s, H] with b * s of them, sequence after sequence: keys and values go into the
+        pages of layer `layer` (normed and rotated on the way, in one launch), and every token sees the keys of its sequence up to itself.
+        For inference: no gradients, no dropout.  The same call takes prompts, single tokens and drafts of several tokens, mixed as they come."""
+        b, s, _ = x.shape
+        nq, d = self.num_attention_heads, self.hidden_size_per_attention_head
+        if not self.causal:
+            raise ValueError("KV caching is only supported for causal attention.")
+        if self.dtype == torch.float32:
+            raise NotImplementedError("the paged attention kernels take bfloat16 or float16 tensors")
+        if b * s != step.tokens:
+            raise ValueError(f"{b * s} tokens in x, {step.tokens} in the step")
+        if self.rotary_embedding is not None and step.longest > self.rotary_embedding.max_seq_length:
+            raise IndexError(f"position {step.longest - 1} is outside the rotary table of {self.rotary_embedding.max_seq_length} rows")
+        pages = (cache.k_pages[layer], cache.v_pages[layer], cache.page_table[:step.ctx_len.numel()], step.cu_seqlens, step.ctx_len)
+        with torch.no_grad():
+            q, k, v = self._project(x)
+            norms = self._own_norms() if self.key_query_norm else None
+            if self.key_query_norm and norms is None:
+                q, k = self.norm_query(q), self.norm_key(k)
+            rotary, interleaved = self._own_rotary(step.position_ids)
+            if self.rotary_embedding is not None and rotary is None:
+                if norms is not None:                    # the norms come first
+                    q, k, norms = self.norm_query(q), self.norm_key(k), None
+                q, k = (self.rotary_embedding.rotate_tokens(t, step.position_ids, s) for t in (q, k))
+            if norms is None and rotary is None:
+                ops.paged_append(k, v, *pages)
+            else:
+                q = ops.paged_append(k, v, *pages, q=q, rotary=rotary, interleaved=interleaved, **(norms or {}))
+            ctx = ops.paged_attention(q, *pages, softmax_scale=self.softmax_scale, max_q_len=step.max_q_len, workspace=cache.workspace(step.tokens))
+            return self.dense(ctx.view(b, s, nq * d))
 
     # ---- KV cache ----------------------------------------------------------------------------------
     def merge_lora_weights(self) -> None:
