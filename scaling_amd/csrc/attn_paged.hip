@@ -26,6 +26,7 @@ constexpr int kRowChunk = 32;        // keys per wavefront and step of paged_row
 constexpr int kRowWaves = 4;
 constexpr int kRowTile = kRowChunk * kRowWaves;
 constexpr int kTileRows = 256;
+constexpr int kMergeMost = 4;        // workgroups of paged_merge with 16 rows each per compute unit, more than which take 32 each
 constexpr int kTileKeys = 64;
 constexpr float kRescaleGap = 8.0f;  // log2 units by which a row's maximum may lag before its output is rescaled
 
@@ -846,32 +847,33 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
 }
 
 // ---- merge of the splits ------------------------------------------------------------------------------------------------------------------------------
-// A workgroup per split block and KV head of paged_rows (the first n_rows_groups; of blocks of 32 rows per 8 of them), where they are not merged in their own
-// launch, and per 16 rows of a block of paged_tiles.
-// (Two lanes to a pair of features and rows one after the other, with a workgroup for every partial result, most of them idle: 19 us for 64 blocks of 256 rows
-// in four splits, 8 so.  32 rows to a workgroup: the same, or 2 us more where rows are few.)
-template <int NB> constexpr int merged_rows() { return NB == 1 ? 16 : 8; }
+// A workgroup per 16 rows of a split block and KV head of paged_rows (the first n_rows_groups), where they are not merged in their own launch, and per
+// `per_group` rows of a block of paged_tiles: 16, or 32 where there may be so many workgroups that most of them, which find nothing, set the time.  (us of 16 and 32:
+// up to 6000 workgroups 15.0 and 10.1, 256 of 32 splits each 9.8 and 15.4.  Two lanes to a pair of features and rows one after the other, with a workgroup
+// for every partial result, most of them idle: 19 for 64 blocks of 256 rows in four splits, 8.7 so.)
 template <int D, int NB>
-__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p, int n_rows_groups, int sixteens) {
+__global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p, int n_rows_groups, int per_block, int per_group) {
     __shared__ float lds[16 * (D + 2)];
     if ((int)blockIdx.x < n_rows_groups) {
-        constexpr int BLOCK = 16 * NB, EACH = merged_rows<NB>();
-        const int at_kv = blockIdx.x / (BLOCK / EACH), r0 = blockIdx.x % (BLOCK / EACH) * EACH, at = divide(at_kv, p.nkv, p.nkv_m), kvh = at_kv - at * p.nkv;
+        constexpr int BLOCK = 16 * NB;
+        const int at_kv = blockIdx.x / NB, r0 = blockIdx.x % NB * 16, at = divide(at_kv, p.nkv, p.nkv_m), kvh = at_kv - at * p.nkv;
         const Found f = find_work<BLOCK, kRowTile, true>(p, p.rows, p.share_m[0], at);
         if (f.b < 0) return;
-        const int n = min(EACH, f.seq.n * p.n_rep - (at - f.at) * BLOCK - r0);
+        const int n = min(16, f.seq.n * p.n_rep - (at - f.at) * BLOCK - r0);
         if (n > 0) merge_rows<D, BLOCK, false>(p, f, at - f.at, kvh, r0, n, lds);
         return;
     }
-    const int group = blockIdx.x - n_rows_groups, at_kv = group / sixteens, z = group - at_kv * sixteens;
+    const int group = blockIdx.x - n_rows_groups, at_kv = group / per_block, z = group - at_kv * per_block;
     const int at = divide(at_kv, p.nkv, p.nkv_m), kvh = at_kv - at * p.nkv;
     const Found f = find_work<kTileRows, kTileKeys, true>(p, p.tiles, p.share_m[1], at);
-    const int block = at - f.at, in = 16 * z + (threadIdx.x >> 4), row = block * kTileRows + in;
-    if (f.b < 0 || row >= f.seq.n * p.n_rep) return;
-    RowSum<D> sum;
-    sum.template add<false, 4>(p.tiles_o, p.tiles_ml, ((int64_t)(f.partial + block) * p.nkv + kvh) * p.tile_rows + in, (int64_t)f.work.blocks * p.nkv * p.tile_rows, f.splits);
-    const int token = divide(row, p.n_rep, p.rep_m);
-    sum.store(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh);
+    if (f.b < 0) return;
+    const int block = at - f.at, n_rows = min(f.seq.n * p.n_rep - block * kTileRows, per_group * (z + 1));
+    for (int in = per_group * z + (threadIdx.x >> 4); in < n_rows; in += 16) {
+        RowSum<D> sum;
+        sum.template add<false, 4>(p.tiles_o, p.tiles_ml, ((int64_t)(f.partial + block) * p.nkv + kvh) * p.tile_rows + in, (int64_t)f.work.blocks * p.nkv * p.tile_rows, f.splits);
+        const int row = block * kTileRows + in, token = divide(row, p.n_rep, p.rep_m);
+        sum.store(p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)(kvh * p.n_rep + row - token * p.n_rep) * p.o_sh);
+    }
 }
 
 template <int D, int NB> int launch(const PagedParams& p, int64_t row_blocks, int64_t tile_blocks, hipStream_t st) {
@@ -883,11 +885,12 @@ template <int D, int NB> int launch(const PagedParams& p, int64_t row_blocks, in
         paged_tiles_kernel<D><<<dim3((unsigned)p.tiles.max_slots * p.nkv), dim3(512), 0, st>>>(p);
         if (const int rc = mi_check_launch("paged_tiles"); rc != MI_OK) return rc;
     }
-    const int64_t of_rows = p.rows.share > 0 && p.tickets == nullptr ? paged_max_split_blocks(p.rows, row_blocks) * p.nkv * (16 * NB / merged_rows<NB>()) : 0;
-    const int sixteens = (std::min<int>(p.tile_rows, kTileRows) + 15) / 16;
-    const int64_t groups = of_rows + paged_max_split_blocks(p.tiles, tile_blocks) * p.nkv * sixteens;
+    const int64_t of_rows = p.rows.share > 0 && p.tickets == nullptr ? paged_max_split_blocks(p.rows, row_blocks) * p.nkv * NB : 0;
+    const int64_t tile_groups = paged_max_split_blocks(p.tiles, tile_blocks) * p.nkv;
+    const int per_group = tile_groups * p.tile_rows > 16 * kMergeMost * mi_compute_units() ? 32 : 16, per_block = (p.tile_rows + per_group - 1) / per_group;
+    const int64_t groups = of_rows + tile_groups * per_block;
     if (groups == 0) return MI_OK;
-    paged_merge_kernel<D, NB><<<dim3((unsigned)groups), dim3(256), 0, st>>>(p, (int)of_rows, sixteens);
+    paged_merge_kernel<D, NB><<<dim3((unsigned)groups), dim3(256), 0, st>>>(p, (int)of_rows, per_block, per_group);
     return mi_check_launch("paged_merge");
 }
 
@@ -983,7 +986,7 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
     // Sums of blocks x tiles and of rows are kept in 32 bits, and a grid has fewer than 2^31 workgroups.
     if (p.nkv > 0xffff) return mi_fail(MI_E_SHAPE, "paged_attn: more than 65535 KV heads");
     if ((int64_t)p.total * p.n_rep > 0x7fffffffLL - kTileRows || row_blocks * row_tiles > 0x7fffffffLL || tile_blocks * tile_tiles > 0x7fffffffLL ||
-        (4 * row_blocks + 17 * tile_blocks + 8LL * mi_compute_units()) * p.nkv > 0x7fffffffLL)
+        (2 * row_blocks + 17 * tile_blocks + 8LL * mi_compute_units()) * p.nkv > 0x7fffffffLL)
         return mi_fail(MI_E_SHAPE, "paged_attn: %lld tokens of %d heads over up to %d keys are too many for one call", (long long)a->total_q, a->n_q_heads, p.capacity);
     const size_t need = mi_paged_attn_workspace_bytes(p.total, p.nq, p.nkv, a->head_dim);
     if (!a->workspace || a->workspace_bytes < need || !mi_aligned16(a->workspace))
