@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/SavedTensorHooks.h>
 #include <ATen/hip/HIPContext.h>
 #include <ATen/autocast_mode.h>
@@ -530,12 +531,20 @@ struct NormRotary : Function<NormRotary> {
             b.dk = ptr(d[1]); b.dk_stride_token = d[1].stride(0); b.dk_stride_head = d[1].stride(1);
             b.dk_weight = ptr(d[3]); b.dk_bias = ptr(d[5]);
         }
-        if (none) return d;
+        if (none) return once(d);
         b.workspace_bytes = mi_norm_rotary_bwd_workspace_bytes(b.fwd.head_dim);
         const Tensor ws = float_buffer(b.workspace_bytes, x);
         b.workspace = ptr(ws);
         check(mi_norm_rotary_bwd(&b), "mi_norm_rotary_bwd");
-        return d;
+        return once(d);
+    }
+    // Of a pass that records a graph the gradients are handed out with a node that says, if asked, that they cannot be differentiated: without one they would
+    // count as constants.
+    static variable_list once(variable_list d) {
+        if (!at::GradMode::is_enabled()) return d;
+        for (Tensor& t : d)
+            if (t.defined()) t.requires_grad_();
+        return torch::autograd::DelayedError("norm_rotary: the gradients cannot be differentiated again", (int64_t)d.size()).apply(std::move(d));
     }
 };
 
@@ -598,6 +607,7 @@ void op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_
     check_head_rows(q, Tensor(), Tensor());
     TORCH_CHECK(out.is_cuda() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device() && out.stride(2) == 1,
                 "paged_attention: out does not match q");
+    at::assert_no_overlap(out, q);                         // rows of q are read again after others were written
     Launch l(q);
     TORCH_CHECK(k_pages.dim() == 4, "paged cache: k_pages and v_pages are [pages, page_size, n_kv, head_dim] tensors");
     const Pages pages = check_pages(q, k_pages.size(2), k_pages, v_pages, table, cu, ctx_len);

@@ -363,6 +363,9 @@ class TransformerInferenceModule(torch.nn.Module):
         if max_tokens < 1 or not prompts or not all(prompts):
             raise ValueError("at least one prompt, no empty one, and at least one token to generate")
         longest = max(len(p) for p in prompts) + max_tokens - 1
+        rotary = self._layers[1].self_attention.rotary_embedding
+        if rotary is not None and longest > rotary.max_seq_length:
+            raise IndexError(f"position {longest - 1} is outside the rotary table of {rotary.max_seq_length} rows")
         cache = self.paged_cache(len(prompts), longest, sum(-(-(len(p) + max_tokens - 1) // page_size) for p in prompts), page_size)
         stop = set(stop_tokens or [])
         completions: List[List[int]] = [[] for _ in prompts]

@@ -110,6 +110,7 @@ class TransformerLayer(torch.nn.Module):
                                                               advance=advance)
         return h + self.mlp(self.post_attention_layernorm(h))
 
+    @torch.no_grad()
     def paged_step(self, hidden_state: torch.Tensor, cache: PagedKVCache, step: PagedStep) -> torch.Tensor:
         """The layer on the new tokens of a step over a paged cache, whose layer `layer_index` is this one's (inference; see
         ParallelSelfAttention.paged_forward)."""

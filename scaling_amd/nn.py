@@ -456,7 +456,7 @@ class PagedKVCache:
         self._free = list(range(num_pages - 1, -1, -1))
         self._table = torch.zeros(max_sequences, -(-max_ctx // page_size), dtype=torch.int32, device="cpu")
         self.page_table = self._table.to(device, copy=True)
-        self._workspace: Optional[Tuple[int, torch.Tensor]] = None
+        self._workspace: Optional[torch.Tensor] = None
 
     @property
     def free_pages(self) -> int:
@@ -492,11 +492,12 @@ class PagedKVCache:
         self._pages[sequence] = []
         self.lengths[sequence] = 0
 
-    def workspace(self, tokens: int) -> torch.Tensor:
-        """Scratch of ops.paged_attention, kept from call to call."""
-        if self._workspace is None or self._workspace[0] < tokens:
-            self._workspace = tokens, ops.paged_workspace(self.max_sequences, tokens, self.n_q, self.n_kv, self.head_dim, self.device)
-        return self._workspace[1]
+    def workspace(self) -> torch.Tensor:
+        """Scratch of ops.paged_attention for calls of any size: one for the cache's life, so that a captured call keeps its own."""
+        if self._workspace is None:
+            # what a call needs stops to grow at a few rows
+            self._workspace = ops.paged_workspace(self.max_sequences, 2 ** 20, self.n_q, self.n_kv, self.head_dim, self.device)
+        return self._workspace
 
 
 class ParallelSelfAttention(torch.nn.Module):
@@ -785,7 +786,7 @@ class ParallelSelfAttention(torch.nn.Module):
                 ops.paged_append(k, v, *pages)
             else:
                 q = ops.paged_append(k, v, *pages, q=q, rotary=rotary, interleaved=interleaved, **(norms or {}))
-            ctx = ops.paged_attention(q, *pages, softmax_scale=self.softmax_scale, max_q_len=step.max_q_len, workspace=cache.workspace(step.tokens))
+            ctx = ops.paged_attention(q, *pages, softmax_scale=self.softmax_scale, max_q_len=step.max_q_len, workspace=cache.workspace())
             return self.dense(ctx.view(b, s, nq * d))
 
     # ---- KV cache ----------------------------------------------------------------------------------

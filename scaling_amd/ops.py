@@ -213,7 +213,7 @@ def norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weig
                 q_bias: Optional[torch.Tensor] = None, k_bias: Optional[torch.Tensor] = None, layer_norm: bool = False,
                 rotary: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None, interleaved: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """Norm over each head of q [tokens, n_q, d] and k [tokens, n_kv, d] (RMSNorm, or LayerNorm with optional biases; weights [d]), followed by the
-    rotary embedding, in one launch; differentiable in q, k, weights and biases.  The arithmetic is float32 with one rounding at the end (`rms_norm` or
+    rotary embedding, in one launch; differentiable (once) in q, k, weights and biases.  The arithmetic is float32 with one rounding at the end (`rms_norm` or
     `layer_norm` followed by `rotary_embedding` rounds the normed rows too).
 
     rotary = (cos, sin, position_ids): tables [rows, r] in the tensors' type or float32 rotate the first r features in halves; with `interleaved`
@@ -270,7 +270,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     q [tokens, n_q, d] (bfloat16 or float16; d 32, 64, 96 or 128), query head h reading KV head h // (n_q / n_kv).  Token i of the n of a sequence sees keys
     u < ctx_len and, with `causal`, u <= ctx_len - n + i; without any its row is zeros.  Rows behind the last sequence are left as they are in `out` (of a new
-    tensor: undefined).  max_q_len: an upper bound of the tokens of a sequence, where the caller knows one (1: no launches for chunks); longer ones
+    tensor: undefined), which shares no memory with q.  max_q_len: an upper bound of the tokens of a sequence, where the caller knows one (1: no launches for chunks); longer ones
     may be left out.  Lengths beyond the page table count its room.  workspace: see `paged_workspace`; without one it is allocated per call."""
     _need_cuda(q, k_pages, v_pages, page_table, cu_seqlens, ctx_len, workspace, out)
     if max_q_len is not None and max_q_len < 1 and q.shape[0] > 0:

@@ -284,3 +284,19 @@ def test_refusals():
             ops.norm_rotary(*bad, **kwargs)
     ops.norm_rotary(q, k, w[0], w[1], 1e-5, w[2], w[3], layer_norm=True, **ok)
     torch.cuda.synchronize()
+
+
+def test_gradients_are_differentiated_once():
+    """A pass that records a graph gives the same gradients, and differentiating those raises instead of taking them for constants."""
+    g = torch.Generator().manual_seed(0)
+    q, k, w = (torch.randn(*s, generator=g).to(DEV).requires_grad_() for s in ((6, 2, 64), (6, 1, 64), (64,)))
+    out = ops.norm_rotary(q, k, w, w)
+    dy = [torch.randn_like(o) for o in out]
+    plain = torch.autograd.grad(out, (q, k, w), dy, retain_graph=True)
+    recorded = torch.autograd.grad(out, (q, k, w), dy, create_graph=True)
+    for a, b in zip(plain, recorded):
+        assert torch.equal(a, b) and b.requires_grad
+    with pytest.raises(RuntimeError):                        # torch's own: the graph of the gradients does not reach q
+        torch.autograd.grad(recorded[0].sum(), q, retain_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        recorded[0].sum().backward()

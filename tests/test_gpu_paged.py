@@ -436,3 +436,28 @@ def test_refusals():
     assert ops.paged_append(rows["k"][:0], rows["v"][:0], good["k_pages"], good["v_pages"], good["page_table"], _ints([0, 0, 0]), good["ctx_len"], q=q[:0]).shape == (0, nq, d)
     torch.cuda.synchronize()
     assert torch.equal(good["k_pages"], before)
+
+
+@pytest.mark.parametrize("new,ctx", [([6], [300]), ([8], [3000]), ([9, 2], [500, 40]), ([5, 1] * 9, [40 * i + 6 for i in range(18)])], ids=["block", "splits", "blocks", "many"])
+def test_non_finite_values_behind_the_mask_of_drafts(new, ctx):
+    """Blocks of 32 rows: keys that a row must not see do not reach it, in either half of the block."""
+    nq, nkv, d, page = 8, 2, 64, 16
+    k, v, table, cu = _cache(new, ctx, nkv, d, page, torch.bfloat16, seed=9)
+    q = torch.randn(cu[-1], nq, d, generator=torch.Generator().manual_seed(2)).bfloat16()
+    at = ctx[0] - 2
+    for value in (math.nan, math.inf, -math.inf):
+        for which in range(2):
+            pages = [k.clone(), v.clone()]
+            pages[which][int(table[0, at // page]), at % page, 0, 3] = value
+            out = ops.paged_attention(q.to(DEV), _device(pages[0]), _device(pages[1]), table.to(DEV), _ints(cu), _ints(ctx), max_q_len=max(new))
+            torch.cuda.synchronize()
+            _check(f"{value} {which}", out, q, *pages, table, cu, ctx, True, 1 / math.sqrt(d))
+
+
+def test_an_output_that_shares_memory_with_q_is_refused():
+    new, ctx, nq, nkv, d, page = [2, 1], [20, 9], 4, 2, 64, 16
+    k, v, table, cu = _cache(new, ctx, nkv, d, page, torch.bfloat16, seed=1, stale=1.0)
+    memory = torch.zeros(4, nq, d, dtype=torch.bfloat16, device=DEV)
+    for q, out in ((memory[:3], memory[:3]), (memory[:3], memory[1:])):
+        with pytest.raises(RuntimeError):
+            ops.paged_attention(q, _device(k), _device(v), table.to(DEV), _ints(cu), _ints(ctx), out=out)

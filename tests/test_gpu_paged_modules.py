@@ -201,6 +201,9 @@ def test_another_stream_and_a_captured_step():
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             y = layer.paged_step(x, cache, step)
+        held = cache.workspace()
+        cache.workspace()
+        assert cache.workspace() is held                     # what the graph reads stays where it is
         for _ in range(3):
             x.zero_()
             graph.replay()

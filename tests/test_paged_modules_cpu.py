@@ -110,6 +110,8 @@ def test_refused_generation():
     for tokens, prompts in ((0, [[1]]), (1, []), (1, [[1], []])):
         with pytest.raises(ValueError):
             model.generate_ragged(tokens, prompts)
+    with pytest.raises(IndexError):
+        model.generate_ragged(100, [[1], [2] * 30])                                          # position 128 of a table of 128
     cache = model.paged_cache(3, page_size=32)
     assert len(cache.k_pages) == 2 and cache.max_ctx == 128 and cache.free_pages == 12
     assert cache.k_pages[0].shape == (12, 32, 2, 64) and cache.k_pages[0].stride() == (4096, 64, 2048, 1)
