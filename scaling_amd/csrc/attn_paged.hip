@@ -307,7 +307,8 @@ __device__ __forceinline__ void own_keys_only(const PagedParams& p, const int32_
 //     O^T[feature][row] += V^T P^T    V passes through a wavefront's own LDS and is read back transposed
 // Every cached element is read from memory once per block of rows.  The next chunk's K is requested as soon as the scores are computed and its V as soon as this
 // chunk's is in LDS, into the same registers: 16 KB a wavefront (d 128) are always under way, and 12 wavefronts fit a compute unit.  (Two sets of registers, a
-// whole chunk ahead: 8 wavefronts, 16 rows to a block at the most.)
+// whole chunk ahead: 8 wavefronts, 16 rows to a block at the most.)  Bound by memory: 32 x 8 items of 200 - 8192 keys of 128 features 84.7 us, 6.1 TB/s; few items
+// by the start and the merge besides, ~10 us: 8 x 8 items of 4096 keys 32.7, a single one of 1500 9.7 (6.5 and a second launch of 5.5 without the merge in it).
 template <int D, int NB>
 __global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_kernel(const PagedParams p) {
     constexpr int NWV = kRowWaves, kThreads = 64 * NWV, BLOCK = 16 * NB;
@@ -614,6 +615,9 @@ template <int D> struct PageDma {
 //     S^T = K Q^T      A = K rows from LDS, B = Q in registers
 //     softmax          a lane's column is a row of the block; the maximum is raised only when it lags by 2^8, so most tiles rescale nothing
 //     O^T += V^T P^T   B = P^T as the accumulators of S^T hold it, A = V^T by transposing LDS reads
+// Bound by the matrix pipe (busy half of the time) and the power that it draws: 4 x 2048 tokens behind 2048 - 14336 others, 32 / 8 heads of 128, 1083 us, 1.07 PFLOP/s, as
+// mi_attn_fwd over contiguous keys; without its softmax 951, without its operand reads 890.  (Operands 2, 4, 8 products ahead instead of 3: 1104, 1076, 1093; the
+// first of them before the barrier: 1150.)
 template <int D>
 __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p) {
     constexpr int NW = 8, BN = kTileKeys;
