@@ -983,8 +983,12 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
     p.tiles = plans.tiles;
     p.tile_rows = plans.tile_rows;
     const bool two = plans.row_block == 2 * kRowBlock;
+    // Where every sequence is a chunk, if no rows are behind the last one, there is no launch that would only find that out: a shorter one is computed as a chunk.
+    // (4 x 2048 tokens behind others: 1112 -> 1088 us, the launch and its merge.)
+    const bool chunks_only = std::min(longest, p.total - (p.batch - 1) * longest) * p.n_rep > plans.rows.rows_up_to;
+    if (chunks_only) p.tiles.rows_over = 0;
     p.rows.max_n = p.tiles.max_n = (int)longest;
-    const int64_t row_blocks = two ? paged_max_blocks<2 * kRowBlock>(p.rows, p.total, p.batch, longest, p.n_rep) : paged_max_blocks<kRowBlock>(p.rows, p.total, p.batch, longest, p.n_rep);
+    const int64_t row_blocks = chunks_only ? 0 : two ? paged_max_blocks<2 * kRowBlock>(p.rows, p.total, p.batch, longest, p.n_rep) : paged_max_blocks<kRowBlock>(p.rows, p.total, p.batch, longest, p.n_rep);
     const int64_t tile_blocks = paged_max_blocks<kTileRows>(p.tiles, p.total, p.batch, longest, p.n_rep);
     const int64_t row_tiles = ((int64_t)p.capacity + kRowTile - 1) / kRowTile, tile_tiles = ((int64_t)p.capacity + kTileKeys - 1) / kTileKeys;
     // Sums of blocks x tiles and of rows are kept in 32 bits, and a grid has fewer than 2^31 workgroups.

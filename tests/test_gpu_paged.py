@@ -461,3 +461,21 @@ def test_an_output_that_shares_memory_with_q_is_refused():
     for q, out in ((memory[:3], memory[:3]), (memory[:3], memory[1:])):
         with pytest.raises(RuntimeError):
             ops.paged_attention(q, _device(k), _device(v), table.to(DEV), _ints(cu), _ints(ctx), out=out)
+
+
+@pytest.mark.parametrize("new,ctx,total,max_q_len", [
+    ([3], [700], 200, 200),                                  # a buffer for a chunk with a few tokens in it
+    ([100, 2, 64], [130, 900, 64], 300, 100),                # tokens for three chunks, one of them short
+    ([1, 1, 1], [40, 300, 17], 64, 1),                       # a buffer of 64 for single tokens
+    ([0, 90], [50, 90], 180, 90),
+], ids=str)
+def test_fewer_tokens_than_the_buffer_has(new, ctx, total, max_q_len):
+    """Sequences shorter than the numbers of tokens and sequences let one expect; rows behind the last one stay as they are."""
+    nq, nkv, d, page = 8, 2, 128, 16
+    k, v, table, cu = _cache(new, ctx, nkv, d, page, torch.bfloat16, seed=12)
+    q = torch.randn(total, nq, d, generator=torch.Generator().manual_seed(2)).bfloat16()
+    out = torch.full_like(q, 7.0, device=DEV)
+    ops.paged_attention(q.to(DEV), _device(k), _device(v), table.to(DEV), _ints(cu), _ints(ctx), max_q_len=max_q_len, out=out)
+    torch.cuda.synchronize()
+    _check("o", out, q, k, v, table, cu, ctx, True, 1 / math.sqrt(d))
+    assert bool((out[cu[-1]:] == 7.0).all())
