@@ -101,6 +101,16 @@ template <int TILE> MI_PLAN_FN void paged_split_keys(const PagedSeq& s, const Pa
     k0 = paged_clamp(per * i, 0, s.len);
     k1 = paged_clamp(per * i + per, 0, s.len);
 }
+// Of work that is not split: how many blocks of a sequence, the last ones, reach keys beyond x tiles (about: by the tokens that whole blocks have); all for x < 0.
+// The order of blocks is by the most x that they reach beyond, longest first, so that no long one starts when others are done.
+template <int BLOCK, int TILE> MI_PLAN_FN int paged_above(const PagedSeq& s, const PagedWork& w, int n_rep, bool causal, int x) {
+    if (x < 0) return w.blocks;
+    if ((int64_t)x * TILE >= s.len) return 0;
+    const int64_t over = (int64_t)x * TILE - ((int64_t)s.ctx - s.n);      // keys of new tokens below
+    if (!causal || over <= 0) return w.blocks;
+    const int64_t below = over * n_rep / BLOCK;
+    return below >= w.blocks ? 0 : w.blocks - (int)below;
+}
 // Whether a launch computes a sequence whose first slot and first partial result are these: all of its splits or none.
 MI_PLAN_FN bool paged_fits(const PagedPlan& p, const PagedWork& w, int splits, int slot, int partial) {
     const int64_t n = (int64_t)w.blocks * splits;

@@ -84,6 +84,32 @@ static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, i
             if (got != (want < 0 ? 0 : want > s.len ? s.len : (int)want)) return fail("limit of a row", c);
         }
     }
+    if (good && BLOCK == 256 && batch <= 64) {             // longest first: every block once
+        std::vector<int> seen(all, 0), before(batch, 0);
+        for (int b = 1; b < batch; ++b) before[b] = before[b - 1] + paged_work<BLOCK, TILE>(p, paged_seq(cu[b - 1], cu[b], ctx[b - 1], total, capacity), n_rep).blocks;
+        int previous = 0x7fffffff;
+        for (int wanted = 0; wanted < all; ++wanted) {
+            int lo = -1, hi = 0;
+            const auto above = [&](int b, int x) {
+                const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity);
+                return paged_above<BLOCK, TILE>(s, paged_work<BLOCK, TILE>(p, s, n_rep), n_rep, causal, x);
+            };
+            const auto sum = [&](int x) { int64_t n = 0; for (int b = 0; b < batch; ++b) n += above(b, x); return n; };
+            for (int b = 0; b < batch; ++b) { const int t = (paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity).len + TILE - 1) / TILE; if (t > hi) hi = t; }
+            if (sum(-1) != all || sum(hi) != 0) return fail("blocks above the ends", c);
+            while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (sum(mid) > wanted) lo = mid; else hi = mid; }
+            if (lo > previous) return fail("a longer block later", c);
+            previous = lo;
+            int in = wanted - (int)sum(hi), at = -1;
+            for (int b = 0; b < batch && at < 0; ++b) {
+                const int width = above(b, lo) - above(b, hi);
+                if (width < 0) return fail("blocks beyond more keys that are not beyond fewer", c);
+                if (in < width) at = before[b] + above(b, hi) + in;
+                else in -= width;
+            }
+            if (at < 0 || at >= all || seen[at]++) return fail("a block twice", c);
+        }
+    }
     if (good && (blocks > most || (blocks == 0) < (most == 0))) return fail("more blocks than the bound", c);
     if (good && (slots > p.max_slots || partials > p.max_partials || split_blocks > paged_max_split_blocks(p, most))) return fail("more workgroups or partial results than the bound", c);
     return 0;
