@@ -132,7 +132,7 @@ template <int BLOCK, int TILE, bool OF_BLOCKS> __device__ __forceinline__ Found 
             int64_t slots = 0;
             for (int base = 0; base < p.batch; base += 64) {
                 if (p.batch > 64) look(base);
-                slots += total(work.blocks * paged_splits(work, split_tiles));
+                slots += total(work.blocks * paged_splits(plan, work, split_tiles));
             }
             if (slots <= plan.fit) break;
             split_tiles = paged_next_tiles(plan, split_tiles, units, blocks, slots, step);
@@ -141,7 +141,7 @@ template <int BLOCK, int TILE, bool OF_BLOCKS> __device__ __forceinline__ Found 
     int at = 0, slots = 0, partials = 0;
     for (int base = 0; base < p.batch; base += 64) {
         if (p.batch > 64 || plan.share == 0) look(base);
-        const int splits = paged_splits(work, split_tiles), n = work.blocks * splits, part = splits > 1 ? n : 0;
+        const int splits = paged_splits(plan, work, split_tiles), n = work.blocks * splits, part = splits > 1 ? n : 0;
         const int slots_upto = slots + prefix_sum(n), part_upto = partials + prefix_sum(part);
         const int width = OF_BLOCKS ? (splits > 1 ? work.blocks : 0) : n, upto = OF_BLOCKS ? at + prefix_sum(width) : slots_upto;
         const uint64_t found = __ballot(work.blocks > 0 && wanted >= upto - width && wanted < upto);
@@ -928,6 +928,9 @@ template <int D, int NB> int launch(const PagedParams& p, int64_t row_blocks, in
 // items of 200 - 8192 keys 98, 93, 87, all of 4096 keys 85, 85, 92; 8 x 8 items of 900 - 5000 keys and 3 - 9 tokens
 // of 4 heads 39.9, 46.6 of 1024; 3 x 4 items of 20000 - 32768 keys of 64 features 23.9, 27.4 of 1024.  32 x 8 items of 20 rows, 200 - 8192 keys: 6 to a unit 123, 8 to a unit 130.)
 constexpr int kRowsLeast = 2, kRowsMost = 8, kRowsMostWide = 6;     // per compute unit
+// Up to so many keys a sequence is not split: a merge costs more.  (us, split and not, one call after the other.  Single tokens of 4 sequences, 32 / 8 heads of 128: 150 keys 9.6, 6.9, 300 keys 9.9, 9.2,
+// 500 keys 10.3, 11.8; 120 tokens of 120 keys 18.7, 13.3, of 300 keys 22.4, 18.3, of 500 keys 21.7, 22.9; 6 x 200 tokens of 300 keys, 16 / 4 heads: 28.5, 20.7.)
+constexpr int kUnsplitKeys = 384;
 int share_of(int64_t workgroups, int nkv) { return workgroups / nkv > 0 ? (int)(workgroups / nkv) : 1; }
 // paged_tiles, one to a compute unit: few blocks are cut into what runs at once.  Of many blocks of few rows (`longest` tokens to a sequence, whose partial
 // results are small) pieces are up to four times smaller, as above.
@@ -943,12 +946,12 @@ Plans make_plans(int64_t tokens, int64_t items, int64_t longest, int n_rep, int 
     o.row_block = most <= kRowBlock ? kRowBlock : 2 * kRowBlock;
     const int limit = few && most <= kRowsAlone ? kRowsAlone : kRowLimit;
     const int64_t rows_most = (o.row_block == kRowBlock ? kRowsMost : kRowsMostWide) * cus;
-    o.rows = PagedPlan{0, limit, 0x7fffffff, share_of(few ? kRowsLeast * cus : std::min<int64_t>(8 * items, rows_most), nkv), 8 * items >= rows_most, 0, 0, 0};
+    o.rows = PagedPlan{0, limit, 0x7fffffff, share_of(few ? kRowsLeast * cus : std::min<int64_t>(8 * items, rows_most), nkv), 8 * items >= rows_most, 0, kUnsplitKeys / kRowTile, 0, 0};
     // Enough blocks for every compute unit: no splits, no merge.
     const bool many = tokens * n_rep / kTileRows * nkv >= cus;
     o.tile_rows = (int)std::min<int64_t>((most + 15) / 16 * 16, kTileRows);
     const int pieces = o.tile_rows * 4 <= kTileRows ? 4 : o.tile_rows * 2 <= kTileRows ? 2 : 1, at_once = share_of(cus, nkv);
-    o.tiles = PagedPlan{limit, 0x7fffffff, 0x7fffffff, many ? 0 : pieces * at_once, 0, many ? 0 : at_once, 0, 0};
+    o.tiles = PagedPlan{limit, 0x7fffffff, 0x7fffffff, many ? 0 : pieces * at_once, 0, many ? 0 : at_once, kUnsplitKeys / kTileKeys, 0, 0};
     return o;
 }
 // Whether the last workgroup of a block merges, given tickets: no more workgroups than run at once.  Each waits for its results to be in memory, which more of them
@@ -1026,9 +1029,9 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
     if (a->tickets && (a->n_tickets < mi_paged_attn_tickets(p.nkv) || (reinterpret_cast<uintptr_t>(a->tickets) & 3u) != 0))
         return mi_fail(MI_E_WORKSPACE, "paged_attn: %lld tickets (4-byte aligned), got %lld", (long long)mi_paged_attn_tickets(p.nkv), (long long)a->n_tickets);
     p.tickets = !two && merges_in_launch(p.rows, p.nkv) ? a->tickets : nullptr;
-    // A sequence of up to a tile of keys has one split, whatever the plan.
-    if (row_tiles == 1 || row_blocks == 0) p.rows.share = 0;
-    if (tile_tiles == 1 || tile_blocks == 0) p.tiles.share = 0;
+    // A page table without room for more: no splits, whatever the plan.
+    if (row_tiles <= p.rows.least || row_blocks == 0) p.rows.share = 0;
+    if (tile_tiles <= p.tiles.least || tile_blocks == 0) p.tiles.share = 0;
     p.share_m[0] = divide_m(p.rows.share); p.share_m[1] = divide_m(p.tiles.share);
     p.rows.max_slots = (int)paged_max_slots(p.rows, row_blocks, row_tiles);
     p.tiles.max_slots = (int)paged_max_slots(p.tiles, tile_blocks, tile_tiles);

@@ -4,7 +4,7 @@
 // A sequence's rows are (new token, query head of a group): token i of n and head r of n_rep make row i * n_rep + r, so all heads that share keys share a
 // block of rows.  A kernel takes the sequences whose number of rows it suits, in blocks of rows, with keys in tiles.  The keys of a sequence are cut into
 // splits of at most S tiles each, with S such that all splits together are about `share` workgroups per KV head:
-//     W = sum over sequences of blocks * tiles,   S = floor(W / share) + 1,   splits_b = ceil(tiles_b / S)
+//     W = sum over sequences of blocks * tiles,   S = floor(W / share) + 1,   splits_b = ceil(tiles_b / S), of short sequences 1
 // Then splits of all blocks are at most share + blocks in number, and those of sequences with more than one split at most 2 * share (tiles > S gives
 // ceil(tiles / S) < 2 tiles / S).  Lengths may be anything: sequences are clamped to the tokens and the page table that there are, and where lengths that
 // overlap make more workgroups or partial results than there are, sequences are left out as a whole.
@@ -60,6 +60,7 @@ struct PagedPlan {
     int share;                    // workgroups per KV head aimed at; 0: never split
     int even;                     // sequences of about one length: cut for a quarter of the share
     int fit;                      // workgroups per KV head that run at once: few blocks are cut for no more of them; 0: no such line
+    int least;                    // sequences of no more tiles are not split
     int max_slots, max_partials;  // (set by the host) workgroups and partial results per KV head that there are
 };
 
@@ -94,7 +95,7 @@ MI_PLAN_FN int paged_next_tiles(const PagedPlan& p, int split_tiles, int64_t uni
     const int64_t next = (int64_t)((float)split_tiles * (float)slots / (float)p.fit);
     return paged_clamp(next > split_tiles ? next : (int64_t)split_tiles + 1, 1, 0x1000000);
 }
-MI_PLAN_FN int paged_splits(const PagedWork& w, int split_tiles) { return paged_quotient(w.tiles - 1, split_tiles) + 1; }
+MI_PLAN_FN int paged_splits(const PagedPlan& p, const PagedWork& w, int split_tiles) { return w.tiles <= p.least ? 1 : paged_quotient(w.tiles - 1, split_tiles) + 1; }
 // keys [k0, k1) of split i
 template <int TILE> MI_PLAN_FN void paged_split_keys(const PagedSeq& s, const PagedWork& w, int splits, int i, int& k0, int& k1) {
     const int64_t per = (int64_t)(paged_quotient(w.tiles - 1, splits) + 1) * TILE;

@@ -21,7 +21,7 @@ static int fail(const char* what, int i) { printf("case %%d: %%s\n", i, what); r
 template <int BLOCK, int TILE>
 static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, int capacity, int longest, bool good, bool causal, const std::vector<int>& cu,
                   const std::vector<int>& ctx, std::vector<int>& taken) {
-    PagedPlan p = {over, up_to, longest, rnd() %% 4 == 0 ? 0 : 1 << rnd() %% 9, 0, 0, 0, 0};
+    PagedPlan p = {over, up_to, longest, rnd() %% 4 == 0 ? 0 : 1 << rnd() %% 9, 0, 0, 1 + (int)(rnd() %% 6), 0, 0};
     if (rnd() & 1) p.even = rnd() & 1;
     else if (rnd() & 1) p.fit = p.share >> rnd() %% 3;
     const int max_tiles = (capacity + TILE - 1) / TILE;
@@ -47,7 +47,7 @@ static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, i
         int64_t n = 0;
         for (int b = 0; b < batch; ++b) {
             const PagedWork w = paged_work<BLOCK, TILE>(p, paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity), n_rep);
-            n += (int64_t)w.blocks * paged_splits(w, S);
+            n += (int64_t)w.blocks * paged_splits(p, w, S);
         }
         const int next = paged_next_tiles(p, S, units, all, n, step);
         if (next == S || (step < kPagedSteps && next < S)) {
@@ -60,7 +60,7 @@ static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, i
     for (int b = 0; b < batch; ++b) {
         const PagedSeq s = paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity);
         const PagedWork w = paged_work<BLOCK, TILE>(p, s, n_rep);
-        const int splits = paged_splits(w, S);
+        const int splits = paged_splits(p, w, S);
         if (splits < 1) return fail("no split", c);
         const bool fits = paged_fits(p, w, splits, (int)slots, (int)partials);
         if (good && w.blocks > 0 && !fits) return fail("a sequence left out", c);
@@ -74,7 +74,7 @@ static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, i
         for (int i = 0; i < splits; ++i) {                 // splits cover the keys once, in order, in whole tiles
             int k0, k1;
             paged_split_keys<TILE>(s, w, splits, i, k0, k1);
-            if (k0 != at || k1 < k0 || k1 > s.len || (k0 %% TILE != 0 && k0 != s.len) || (k1 - k0 + TILE - 1) / TILE > S) return fail("keys of a split", c);
+            if (k0 != at || k1 < k0 || k1 > s.len || (k0 %% TILE != 0 && k0 != s.len) || (k1 - k0 + TILE - 1) / TILE > (S > p.least ? S : p.least)) return fail("keys of a split", c);
             at = k1;
         }
         if (at != s.len) return fail("keys left out", c);
