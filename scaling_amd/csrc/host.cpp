@@ -602,12 +602,14 @@ OptTensor op_paged_append(const OptTensor& q_, const Tensor& k, const Tensor& v,
     return q.defined() ? OptTensor(q_out) : std::nullopt;
 }
 
-void op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu, const Tensor& ctx_len, bool causal,
-                        double scale, int64_t max_q_len, const OptTensor& workspace_, const OptTensor& tickets, const Tensor& out) {
+Tensor op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu, const Tensor& ctx_len, bool causal,
+                          double scale, int64_t max_q_len, const OptTensor& workspace_, const OptTensor& tickets, const OptTensor& out_) {
+    need_gpu(q);
     check_head_rows(q, Tensor(), Tensor());
+    const Tensor out = out_.has_value() ? *out_ : at::empty(q.sizes(), q.options());
     TORCH_CHECK(out.is_cuda() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device() && out.stride(2) == 1,
                 "paged_attention: out does not match q");
-    at::assert_no_overlap(out, q);                         // rows of q are read again after others were written
+    if (out_.has_value()) at::assert_no_overlap(out, q);                         // rows of q are read again after others were written
     Launch l(q);
     TORCH_CHECK(k_pages.dim() == 4, "paged cache: k_pages and v_pages are [pages, page_size, n_kv, head_dim] tensors");
     const Pages pages = check_pages(q, k_pages.size(2), k_pages, v_pages, table, cu, ctx_len);
@@ -631,6 +633,7 @@ void op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_
     }
     a.stream = l.stream;
     check(mi_paged_attn(&a), "mi_paged_attn");
+    return out;
 }
 
 // ---- linear projections ------------------------------------------------------------------------------------------------

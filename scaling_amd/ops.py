@@ -244,9 +244,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
     if q is not None and (q_weight is None) != (k_weight is None):
         raise ValueError("paged_append: q_weight and k_weight go together")
     cos, sin, ids = rotary if rotary is not None else (None, None, None)
-    with torch.no_grad():
-        return _lib.host().paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, ctx_len, q_weight, k_weight, q_bias, k_bias, cos, sin, ids,
-                                        float(eps), bool(layer_norm), bool(interleaved))
+    return _lib.host().paged_append(q, k, v, k_pages, v_pages, page_table, cu_seqlens, ctx_len, q_weight, k_weight, q_bias, k_bias, cos, sin, ids,
+                                    float(eps), bool(layer_norm), bool(interleaved))
 
 
 def paged_workspace(batch: int, tokens: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
@@ -275,13 +274,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _need_cuda(q, k_pages, v_pages, page_table, cu_seqlens, ctx_len, workspace, out)
     if max_q_len is not None and max_q_len < 1 and q.shape[0] > 0:
         raise ValueError("paged_attention: max_q_len must be positive")
-    with torch.no_grad():
-        if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _lib.host().paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, ctx_len, bool(causal),
-                                    1.0 / math.sqrt(q.shape[2]) if softmax_scale is None else float(softmax_scale), max_q_len or 0, workspace,
-                                    getattr(workspace, "tickets", None), out)
-    return out
+    return _lib.host().paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, ctx_len, bool(causal),
+                                       1.0 / math.sqrt(q.shape[2]) if softmax_scale is None else float(softmax_scale), max_q_len or 0, workspace,
+                                       getattr(workspace, "tickets", None), out)
 
 
 # ------------------------------------------------------------------------------------------------
