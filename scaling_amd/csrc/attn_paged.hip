@@ -22,6 +22,9 @@ namespace {
 constexpr int kRowBlock = 16;        // rows of a block, or twice as many where a sequence may have more
 constexpr int kRowLimit = 32;
 constexpr int kRowsAlone = 64;
+// Where the page tables have no room for more keys, calls whose blocks all run at once are paged_rows' with any number of rows.  (us, tiles / rows: 128 tokens of 32 / 8 heads
+// of 128 over 256 keys 16.9 / 11.8, 8 x 30 - 50 tokens of 16 / 4 heads of 64 over 300 keys 18.0 / 9.7; over 1000 keys 23.8 / 25.6 and 23.3 / 22.3.)
+constexpr int kRowsAloneKeys = 512;
 constexpr int kRowChunk = 32;        // keys per wavefront and step of paged_rows
 constexpr int kRowWaves = 4;
 constexpr int kRowTile = kRowChunk * kRowWaves;
@@ -938,13 +941,14 @@ struct Plans {
     PagedPlan rows, tiles;
     int row_block, tile_rows;                              // rows of a block of paged_rows; rows kept per partial result of paged_tiles
 };
-Plans make_plans(int64_t tokens, int64_t items, int64_t longest, int n_rep, int nkv) {
+Plans make_plans(int64_t tokens, int64_t batch, int64_t items, int64_t longest, int64_t capacity, int n_rep, int nkv) {
     const int cus = mi_compute_units();
-    const bool few = 8 * items <= kRowsLeast * cus;
     const int64_t most = longest * n_rep;
+    const bool few = 8 * items <= kRowsLeast * cus;
+    const bool short_keys = capacity <= kRowsAloneKeys && (tokens * n_rep / (2 * kRowBlock) + batch) * nkv <= kRowsLeast * cus;
     Plans o;
     o.row_block = most <= kRowBlock ? kRowBlock : 2 * kRowBlock;
-    const int limit = few && most <= kRowsAlone ? kRowsAlone : kRowLimit;
+    const int limit = short_keys ? 0x7fffffff : few && most <= kRowsAlone ? kRowsAlone : kRowLimit;
     const int64_t rows_most = (o.row_block == kRowBlock ? kRowsMost : kRowsMostWide) * cus;
     o.rows = PagedPlan{0, limit, 0x7fffffff, share_of(few ? kRowsLeast * cus : std::min<int64_t>(8 * items, rows_most), nkv), 8 * items >= rows_most, 0, kUnsplitKeys / kRowTile, 0, 0};
     // Enough blocks for every compute unit: no splits, no merge.
@@ -966,7 +970,7 @@ constexpr int64_t kMaxTiles = (1 << 24) + 1;              // of a sequence
 #ifndef MI_ELEM_F16
 extern "C" int64_t mi_paged_attn_tickets(int32_t n_kv_heads) {
     if (n_kv_heads <= 0) return 0;
-    return paged_max_partials(make_plans(0, 0x7fffffff, 1, 1, n_kv_heads).rows, kMaxTiles, kMaxTiles) * n_kv_heads;
+    return paged_max_partials(make_plans(0, 1, 0x7fffffff, 1, 1 << 30, 1, n_kv_heads).rows, kMaxTiles, kMaxTiles) * n_kv_heads;
 }
 
 extern "C" size_t mi_paged_attn_workspace_bytes(int64_t tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
@@ -974,7 +978,7 @@ extern "C" size_t mi_paged_attn_workspace_bytes(int64_t tokens, int32_t n_q_head
     const int n_rep = n_q_heads / n_kv_heads;
     const bool chunks = tokens * n_rep > kRowLimit;
     // of any number of sequences, with chunks of any length: of shorter ones there are more pieces of fewer rows, no more together
-    const Plans o = make_plans(0, 0x7fffffff, chunks ? kTileRows : tokens, n_rep, n_kv_heads);
+    const Plans o = make_plans(0, 1, 0x7fffffff, chunks ? kTileRows : tokens, 1 << 30, n_rep, n_kv_heads);
     return partial_bytes(paged_max_partials(o.rows, kMaxTiles, kMaxTiles), n_kv_heads, o.row_block, head_dim) +
            (chunks ? partial_bytes(paged_max_partials(o.tiles, kMaxTiles, kMaxTiles), n_kv_heads, kTileRows, head_dim) : 0);
 }
@@ -1005,7 +1009,7 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
     p.page_m = divide_m(p.page); p.rep_m = divide_m(p.n_rep); p.nkv_m = divide_m(p.nkv);
     p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
     const int64_t longest = a->max_q_len > 0 && a->max_q_len < p.total ? a->max_q_len : p.total;
-    const Plans plans = make_plans(p.total, std::min<int64_t>(p.batch, p.total) * p.nkv, longest, p.n_rep, p.nkv);
+    const Plans plans = make_plans(p.total, p.batch, std::min<int64_t>(p.batch, p.total) * p.nkv, longest, p.capacity, p.n_rep, p.nkv);
     p.rows = plans.rows;
     p.tiles = plans.tiles;
     p.tile_rows = plans.tile_rows;
