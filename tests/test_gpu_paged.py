@@ -479,3 +479,52 @@ def test_fewer_tokens_than_the_buffer_has(new, ctx, total, max_q_len):
     torch.cuda.synchronize()
     _check("o", out, q, k, v, table, cu, ctx, True, 1 / math.sqrt(d))
     assert bool((out[cu[-1]:] == 7.0).all())
+
+
+# Page tables with room for more than 512 keys, whatever the lengths: sequences of many rows are computed as chunks.
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("case", ATTENTION, ids=lambda c: f"{len(c[0])}x{max(c[0])}-{max(c[1])}-{c[2]}-{c[3]}-{c[4]}-{c[5]}")
+def test_attention_over_wide_page_tables(case, causal):
+    new, ctx, nq, nkv, d, page = case
+    dtype = torch.bfloat16
+    k, v, table, cu = _cache(new, ctx, nkv, d, page, dtype, seed=sum(ctx) + d + 1, layout="heads" if d != 64 else "tokens", spare=640 // page)
+    q = (1.5 * torch.randn(cu[-1], nq, d, generator=torch.Generator().manual_seed(d + nq))).to(dtype)
+    args = (q.to(DEV), _device(k), _device(v), table.to(DEV), _ints(cu), _ints(ctx))
+    out = ops.paged_attention(*args, causal=causal)
+    torch.cuda.synchronize()
+    _check("o", out, q, k, v, table, cu, ctx, causal, 1 / math.sqrt(d))
+
+
+@pytest.mark.parametrize("new,ctx,nq,nkv", [([100], [150], 4, 2), ([100], [700], 4, 1), ([65, 3], [700, 40], 8, 2)], ids=["tile", "splits", "mixed"])
+def test_non_finite_values_behind_the_mask_of_chunks(new, ctx, nq, nkv):
+    """As for short page tables: keys that a row must not see do not reach it."""
+    d, page = 64, 16
+    k, v, table, cu = _cache(new, ctx, nkv, d, page, torch.float16, seed=4, spare=40)
+    q = torch.randn(cu[-1], nq, d, generator=torch.Generator().manual_seed(2)).half()
+    rest = (table.to(DEV), _ints(cu), _ints(ctx))
+    clean = ops.paged_attention(q.to(DEV), _device(k), _device(v), *rest)
+    at = ctx[0] - 2
+    for value in (math.nan, math.inf, -math.inf):
+        for which in range(2):
+            pages = [k.clone(), v.clone()]
+            pages[which][int(table[0, at // page]), at % page, 0, 3] = value
+            out = ops.paged_attention(q.to(DEV), _device(pages[0]), _device(pages[1]), *rest)
+            torch.cuda.synchronize()
+            _check(f"{value} {which}", out, q, *pages, table, cu, ctx, True, 1 / math.sqrt(d))
+            heads = nq // nkv
+            assert torch.equal(out[:, heads:], clean[:, heads:])
+
+
+def test_which_launches_a_call_makes():
+    """Short page tables: blocks of few rows alone; wide ones: chunks beside them; chunks only: nothing else; short sequences: no merge."""
+    nq, nkv, d, page = 8, 2, 128, 16
+
+    def names(new, ctx, spare, **kwargs):
+        k, v, table, cu = _cache(new, ctx, nkv, d, page, torch.bfloat16, seed=2, spare=spare)
+        q = torch.randn(cu[-1], nq, d).bfloat16().to(DEV)
+        args = (q, _device(k), _device(v), table.to(DEV), _ints(cu), _ints(ctx))
+        return [n for n in ("paged_rows", "paged_tiles", "paged_merge") for m in launched(lambda: ops.paged_attention(*args, **kwargs)) if n in m]
+    assert names([100, 1], [300, 40], 1) == ["paged_rows"]
+    assert names([100, 1], [300, 40], 40) == ["paged_rows", "paged_tiles", "paged_merge"]
+    assert names([100, 80], [700, 600], 1, max_q_len=100) == ["paged_tiles", "paged_merge"]
+    assert names([1, 1], [300, 200], 0, max_q_len=1) == ["paged_rows"]
