@@ -1,7 +1,7 @@
 // Attention of ragged chunks of new tokens over a paged KV cache for gfx950.
 //
 // Two kernels share a call by the number of rows (new tokens x query heads of a group) of a sequence: `paged_rows` for up to kRowLimit of them (single
-// tokens, drafts), bound by the cache's bytes, and `paged_tiles` for chunks, bound by the matrix pipe.  Either cuts its work by paged_plan.h, which every
+// tokens, drafts; more in small calls), bound by the cache's bytes, and `paged_tiles` for chunks, bound by the matrix pipe.  Either cuts its work by paged_plan.h, which every
 // workgroup evaluates on the lengths by itself; partial results (running maximum, sum, unscaled output) of sequences with several splits go to the
 // workspace and are merged by `paged_merge`.
 //
