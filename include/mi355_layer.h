@@ -362,7 +362,7 @@ int mi_paged_append(const mi_paged_append_args* args);
 
 /* Attention of the new tokens over the pages (mi_paged_append first): token i of the n of sequence b attends to its keys at positions u < ctx_len[b] and, when
  * causal, u <= ctx_len[b] - n + i.  Softmax in fp32 of scores scaled by softmax_scale, probabilities rounded to `dtype` before P V as in mi_attn_fwd; a row
- * without keys yields zeros.  q, o [total_q, n_q_heads, head_dim] by element strides; query head h reads KV head h / (n_q_heads / n_kv_heads).  Rows of o
+ * without keys yields zeros.  q, o (which share no memory) [total_q, n_q_heads, head_dim] by element strides; query head h reads KV head h / (n_q_heads / n_kv_heads).  Rows of o
  * behind the last sequence are left as they are.  head_dim in {32, 64, 96, 128}, bf16 or f16, max_pages * page_size <= 2^30.
  * max_q_len: an upper bound of the new tokens of a sequence, 0 if unknown (the launches for longer ones are then made too; sequences over the bound may be
  * left out).  Lengths beyond the page table count its room; a page number outside the cache reads the nearest page inside.
@@ -371,7 +371,7 @@ int mi_paged_append(const mi_paged_append_args* args);
  * with few new rows are merged in the launch that computes them instead of by one more, to the same bits.  They belong to one call at a time as the workspace does, and
  * unlike it outlive a mistake: after calls that overlapped on them, later ones merge too early or never until they are cleared.
  * The key axis is cut by the lengths on the device, so that the work of a ragged batch is even; the order of the sums depends on the lengths of all
- * sequences of the call and on max_q_len, and on nothing else.
+ * sequences of the call, its sizes (the page table's width among them) and max_q_len, and on nothing else.
  * Algorithmic work: 4 * head_dim * n_q_heads * pairs flop; HBM bytes 2 * sum ctx_len * n_kv_heads * head_dim * e + 2 * total_q * n_q_heads * head_dim * e. */
 typedef struct mi_paged_attn_args {
     const void* q;
