@@ -122,15 +122,17 @@ template <int BLOCK, int TILE, bool OF_BLOCKS> __device__ __forceinline__ Found 
     }
     int split_tiles = 0x1000000;                          // no sequence has more
     if (plan.share > 0) {
-        int64_t units = 0, blocks = 0;
+        int64_t units = 0, blocks = 0, reached = 0;
         int most = 0;
         for (int base = 0; base < p.batch; base += 64) {
             look(base);
             units += total(work.blocks * work.tiles);
             if (plan.fit || plan.even) blocks += total(work.blocks);
-            if (plan.even) most = max(most, group_max<64>(work.blocks > 0 ? work.tiles : 0));
+            if (plan.fit || plan.even) most = max(most, group_max<64>(work.blocks > 0 ? work.tiles : 0));
+            if (plan.fit) reached += total(paged_reached<TILE>(seq, work, p.causal));
         }
         split_tiles = divide(paged_units(plan, units, blocks, most), plan.share, share_m) + 1;      // paged_split_tiles
+        if (paged_level(plan, blocks, most, reached)) split_tiles = 0x1000000;
         for (int step = 0; paged_few(plan, blocks) && step <= kPagedSteps; ++step) {
             int64_t slots = 0;
             for (int base = 0; base < p.batch; base += 64) {

@@ -86,6 +86,16 @@ MI_PLAN_FN int paged_split_tiles(const PagedPlan& p, int64_t units, int64_t bloc
     if (p.share == 0) return 0x1000000;                    // no sequence has more
     return (int)(paged_units(p, units, blocks, most) / (uint32_t)p.share) + 1;
 }
+// Tiles that a sequence's blocks have, by the middle one of them
+template <int TILE> MI_PLAN_FN int paged_reached(const PagedSeq& s, const PagedWork& w, bool causal) {
+    return w.blocks * w.tiles - (causal ? (int)((int64_t)w.blocks * s.n / (2 * TILE)) : 0);
+}
+// Blocks that run at once, more than half of what does, of which the longest is no more than half again a workgroup's share of all: not split, as twice the
+// pieces of half the length would take two rounds, and a merge.  (6 x 500 tokens of 3000 keys, 16 / 4 heads of 128, 192 blocks: 123 us split, 105 not; one prompt of 3900 tokens, whose
+// blocks reach from 4 to 61 tiles: 103 split, 130 not.)
+MI_PLAN_FN bool paged_level(const PagedPlan& p, int64_t blocks, int most, int64_t reached) {
+    return p.fit > 0 && !paged_few(p, blocks) && blocks <= p.fit && 2 * most * (int64_t)p.fit <= 3 * reached;
+}
 // Of few blocks S grows until their splits run at once: one workgroup more would take as long as all others.  `slots`: splits of all blocks at S.  After
 // kPagedSteps steps S is W / (fit - blocks) + 1, which sum(ceil(tiles / S)) < W / S + blocks leaves no more than fit of.
 constexpr int kPagedSteps = 3;

@@ -35,14 +35,19 @@ static int kernel(int c, int over, int up_to, int batch, int n_rep, int total, i
         const PagedWork w = paged_work<BLOCK, TILE>(p, s, n_rep);
         units += (int64_t)w.blocks * w.tiles;
     }
-    int64_t all = 0;
+    int64_t all = 0, reached = 0;
     int longest_tiles = 0;
     for (int b = 0; b < batch; ++b) {
         const PagedWork w = paged_work<BLOCK, TILE>(p, paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity), n_rep);
         all += w.blocks;
+        const int r = paged_reached<TILE>(paged_seq(cu[b], cu[b + 1], ctx[b], total, capacity), w, causal);
+        if (r > (int64_t)w.blocks * w.tiles) return fail("tiles of the middle block", c);
+        reached += r;
         if (w.blocks > 0 && w.tiles > longest_tiles) longest_tiles = w.tiles;
     }
-    int S = paged_split_tiles(p, units, all, longest_tiles);
+    const bool level = paged_level(p, all, longest_tiles, reached);
+    if (level && (all > p.fit || paged_few(p, all))) return fail("level", c);
+    int S = level ? 0x1000000 : paged_split_tiles(p, units, all, longest_tiles);
     for (int step = 0; p.share > 0 && step <= kPagedSteps; ++step) {
         int64_t n = 0;
         for (int b = 0; b < batch; ++b) {
