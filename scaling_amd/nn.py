@@ -515,6 +515,8 @@ class ParallelSelfAttention(torch.nn.Module):
     queries and keys in one launch (ops.norm_rotary) instead of two norms and a rotary, which rounds once where they round after each.
     """
 
+    norm_rotary_in_one = False               # of modules that were stored without it
+
     def __init__(self, hidden_size: int, num_attention_heads: int, masked_softmax_config: MaskedSoftmaxConfig,
                  causal: bool = True, num_local_attention_heads: int = 0,
                  local_attention_window_size: Optional[int] = None, dropout_attention_probs: float = 0.0,

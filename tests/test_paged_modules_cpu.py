@@ -121,6 +121,8 @@ def test_refused_generation():
 def test_norms_and_rotary_in_one_go_through_own_unhooked_modules_only():
     att = _attention(key_query_norm=True)
     assert att.norm_rotary_in_one is False and _attention(norm_rotary_in_one=True).norm_rotary_in_one
+    del att.__dict__["norm_rotary_in_one"]                                                   # a module stored before there was the setting
+    assert att.norm_rotary_in_one is False
     assert att._own_norms()["layer_norm"] and att._own_norms()["q_bias"] is att.norm_query.bias
     rotary, interleaved = att._own_rotary(None)
     assert rotary[0].shape == (32, 64) and not interleaved
