@@ -457,6 +457,8 @@ class PagedKVCache:
         self._table = torch.zeros(max_sequences, -(-max_ctx // page_size), dtype=torch.int32, device="cpu")
         self.page_table = self._table.to(device, copy=True)
         self._workspace: Optional[torch.Tensor] = None
+        if self.device.type == "cuda":
+            self.workspace()                             # now: the first call over the cache may be one that is captured
 
     @property
     def free_pages(self) -> int:

@@ -253,10 +253,15 @@ def paged_workspace(batch: int, tokens: int, n_q_heads: int, n_kv_heads: int, he
     that may be replayed at the same time, need one each).  With it come the arrival counts (attribute `tickets`, int32, zero between calls) by which the
     last workgroup of a block merges the splits of its keys in the same launch; a workspace without them (a slice, a tensor of the caller's own) takes one more
     launch for the same result.  They are cleared on the current stream, so a first call on another stream waits for this one; after calls that
-    overlapped all the same they may not be zero, and spoil later ones until `workspace.tickets.zero_()`."""
+    overlapped all the same they may not be zero, and spoil later ones until `workspace.tickets.zero_()`.  A workspace that is made while a graph is
+    captured has none: they would not be cleared before the graph's first replay."""
     lib = _lib.load()
     nbytes = lib.mi_paged_attn_workspace_bytes(tokens, n_q_heads, n_kv_heads, head_dim) if batch > 0 else 0
     workspace = torch.empty(nbytes // 4, dtype=torch.float32, device=device)
+    if workspace.is_cuda:
+        with torch.cuda.device(workspace.device):
+            if torch.cuda.is_current_stream_capturing():
+                return workspace
     workspace.tickets = torch.zeros(lib.mi_paged_attn_tickets(n_kv_heads), dtype=torch.int32, device=device)
     return workspace
 

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import oracle
+from scaling_amd import ops
 from scaling_amd.inference import TransformerInferenceModule
 from scaling_amd.layer import TransformerLayer, TransformerLayerIO
 from scaling_amd.nn import PagedKVCache
@@ -212,3 +213,36 @@ def test_another_stream_and_a_captured_step():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(y, want)
+
+
+def test_the_first_call_over_a_cache_may_be_a_captured_one():
+    """What the calls over a cache share is ready before any of them: an eager call in front of the graph's first replay, and the replays."""
+    cfg = _arch(hidden_size=512, num_attention_heads=8, attention_num_kv_heads=2, key_query_norm=True, sequence_length=1024)
+    layer = _seeded_layer(cfg, seed=0).eval()
+    g = torch.Generator().manual_seed(3)
+    fill = [torch.randn(24, 2, 64, 64, generator=g).bfloat16().to(DEV).transpose(1, 2) for _ in range(2)]
+    x = torch.randn(1, 2, 512, generator=g).bfloat16().to(DEV)
+
+    def make():
+        cache = PagedKVCache(1, 24, 2, 1024, 8, 2, 64, torch.bfloat16, DEV, page_size=64)
+        cache.k_pages[0].copy_(fill[0])
+        cache.v_pages[0].copy_(fill[1])
+        cache.step([700, 500])
+        return cache, cache.step([1, 1])
+
+    with torch.no_grad():
+        want = layer.paged_step(x, *make())                  # (the projections' libraries are ready, too)
+        cache, step = make()
+        assert cache._workspace is not None and int(cache._workspace.tickets.abs().sum()) == 0
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = layer.paged_step(x, cache, step)
+            made_inside = ops.paged_workspace(2, 2, 8, 2, 64, DEV)
+        assert not hasattr(made_inside, "tickets")
+        for _ in range(3):
+            assert torch.equal(layer.paged_step(x, cache, step), want)
+            y.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want)
+        assert int(cache.workspace().tickets.abs().sum()) == 0
