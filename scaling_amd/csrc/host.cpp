@@ -602,6 +602,25 @@ OptTensor op_paged_append(const OptTensor& q_, const Tensor& k, const Tensor& v,
     return q.defined() ? OptTensor(q_out) : std::nullopt;
 }
 
+// Whether two [tokens, heads, features] tensors of one shape with contiguous features share memory.  Slices of one tensor lie between each other's rows: of equal
+// strides the offset tells.  Others share where the memory that they span does.
+bool rows_meet(const Tensor& a, const Tensor& b) {
+    if (a.numel() == 0) return false;
+    const int64_t n[2] = {a.size(0), a.size(1)}, d = a.size(2);
+    const auto stride = [&](const Tensor& t, int i) { return n[i] > 1 ? t.stride(i) : 0; };
+    const auto span = [&](const Tensor& t) { return (n[0] - 1) * stride(t, 0) + (n[1] - 1) * stride(t, 1) + d; };
+    const int64_t bytes = (int64_t)(reinterpret_cast<uintptr_t>(b.data_ptr()) - reinterpret_cast<uintptr_t>(a.data_ptr())), e = (int64_t)a.element_size();
+    if (bytes >= span(a) * e || -bytes >= span(b) * e) return false;
+    if (bytes % e != 0 || stride(a, 0) != stride(b, 0) || stride(a, 1) != stride(b, 1)) return true;
+    for (int i = 0; i < 2; ++i) {                          // the places of a and b in every period of stride s
+        const int64_t s = stride(a, i), o = stride(a, 1 - i);
+        if (s == 0) continue;
+        const int64_t at = (bytes / e % s + s) % s, width = o % s == 0 ? d : (n[1 - i] - 1) * o + d;
+        if (at >= width && at + width <= s) return false;
+    }
+    return true;
+}
+
 Tensor op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu, const Tensor& ctx_len, bool causal,
                           double scale, int64_t max_q_len, const OptTensor& workspace_, const OptTensor& tickets, const OptTensor& out_) {
     need_gpu(q);
@@ -609,7 +628,10 @@ Tensor op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& 
     const Tensor out = out_.has_value() ? *out_ : at::empty(q.sizes(), q.options());
     TORCH_CHECK(out.is_cuda() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type() && out.device() == q.device() && out.stride(2) == 1,
                 "paged_attention: out does not match q");
-    if (out_.has_value()) at::assert_no_overlap(out, q);                         // rows of q are read again after others were written
+    if (out_.has_value()) {
+        at::assert_no_internal_overlap(out);
+        TORCH_CHECK(!rows_meet(q, out), "paged_attention: out shares memory with q");     // rows of q are read again after others were written
+    }
     Launch l(q);
     TORCH_CHECK(k_pages.dim() == 4, "paged cache: k_pages and v_pages are [pages, page_size, n_kv, head_dim] tensors");
     const Pages pages = check_pages(q, k_pages.size(2), k_pages, v_pages, table, cu, ctx_len);

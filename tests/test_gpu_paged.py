@@ -528,3 +528,27 @@ def test_which_launches_a_call_makes():
     assert names([100, 1], [300, 40], 40) == ["paged_rows", "paged_tiles", "paged_merge"]
     assert names([100, 80], [700, 600], 1, max_q_len=100) == ["paged_tiles", "paged_merge"]
     assert names([1, 1], [300, 200], 0, max_q_len=1) == ["paged_rows"]
+
+
+def test_an_output_between_the_rows_of_q():
+    """Slices of one tensor: an output that shares elements with q is refused however it is strided, one beside it is not."""
+    new, ctx, nq, nkv, d, page = [40, 1], [90, 30], 4, 2, 64, 16
+    k, v, table, cu = _cache(new, ctx, nkv, d, page, torch.bfloat16, seed=21, stale=1.0)
+    q = torch.randn(41, nq, d, generator=torch.Generator().manual_seed(3)).bfloat16().to(DEV)
+    rest = (_device(k), _device(v), table.to(DEV), _ints(cu), _ints(ctx))
+    want = ops.paged_attention(q, *rest)
+    one = torch.zeros(42, 3 * nq * d, dtype=torch.bfloat16, device=DEV)                          # a projection's output: q, then others
+    part = lambda i, rows=slice(0, 41): one[rows, i * nq * d:(i + 1) * nq * d].view(41, nq, d)     # noqa: E731
+    per_head = torch.zeros(41, nq, 3, d, dtype=torch.bfloat16, device=DEV)                       # per head q, then others
+    outermost = torch.zeros(nq, 2 * 41, d, dtype=torch.bfloat16, device=DEV).transpose(0, 1)     # heads outermost
+    for a, b in ((part(0), part(0)), (part(0), part(0, slice(1, 42))), (part(0), one[:41, d:(nq + 1) * d].view(41, nq, d)), (per_head[:, :, 1], per_head[:, :, 1]),
+                 (outermost[:41], outermost[1:42]), (one[:41, :nq * d].view(41, nq, d), one.view(-1)[:41 * nq * d].view(41, nq, d))):
+        a.copy_(q)
+        with pytest.raises(RuntimeError, match="memory"):
+            ops.paged_attention(a, *rest, out=b)
+    for a, b in ((part(0), part(1)), (part(2), part(0)), (part(0, slice(1, 42)), part(1)), (per_head[:, :, 0], per_head[:, :, 2]), (per_head[:, :, 2], per_head[:, :, 1]),
+                 (outermost[:41], outermost[41:])):
+        a.copy_(q)
+        assert torch.equal(ops.paged_attention(a, *rest, out=b), want) and torch.equal(b, want) and torch.equal(a, q)
+    with pytest.raises(RuntimeError):                        # rows of an output that are one
+        ops.paged_attention(q, *rest, out=one[:1, :nq * d].view(1, nq, d).expand(41, nq, d))
