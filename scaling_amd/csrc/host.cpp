@@ -513,25 +513,25 @@ struct NormRotary : Function<NormRotary> {
         mi_norm_rotary_bwd_args b{};
         b.fwd = head_rows_args(q, k, o);
         b.fwd.stream = l.stream;
-        const bool none = x.size(0) == 0;                  // no rows: the weights' gradients are sums over nothing
-        const auto like = [&](const Tensor& t) { return none ? at::zeros_like(t) : at::empty_like(t); };
+        // without rows (no tokens, or no heads) a tensor's weight gradients are sums over nothing, which no kernel writes
+        const auto like = [](const Tensor& t, const Tensor& of) { return of.numel() == 0 ? at::zeros_like(t) : at::empty_like(t); };
         if (q.defined()) {
             d[0] = at::empty(q.sizes(), q.options());
-            d[2] = like(o.q_weight);
-            if (ctx->saved_data["q_bias"].toBool()) d[4] = like(o.q_weight);
+            d[2] = like(o.q_weight, q);
+            if (ctx->saved_data["q_bias"].toBool()) d[4] = like(o.q_weight, q);
             b.d_q_out = ptr(dq_out); b.d_q_out_stride_token = dq_out.stride(0); b.d_q_out_stride_head = dq_out.stride(1);
             b.dq = ptr(d[0]); b.dq_stride_token = d[0].stride(0); b.dq_stride_head = d[0].stride(1);
             b.dq_weight = ptr(d[2]); b.dq_bias = ptr(d[4]);
         }
         if (k.defined()) {
             d[1] = at::empty(k.sizes(), k.options());
-            d[3] = like(o.k_weight);
-            if (ctx->saved_data["k_bias"].toBool()) d[5] = like(o.k_weight);
+            d[3] = like(o.k_weight, k);
+            if (ctx->saved_data["k_bias"].toBool()) d[5] = like(o.k_weight, k);
             b.d_k_out = ptr(dk_out); b.d_k_out_stride_token = dk_out.stride(0); b.d_k_out_stride_head = dk_out.stride(1);
             b.dk = ptr(d[1]); b.dk_stride_token = d[1].stride(0); b.dk_stride_head = d[1].stride(1);
             b.dk_weight = ptr(d[3]); b.dk_bias = ptr(d[5]);
         }
-        if (none) return once(d);
+        if ((!q.defined() || q.numel() == 0) && (!k.defined() || k.numel() == 0)) return once(d);
         b.workspace_bytes = mi_norm_rotary_bwd_workspace_bytes(b.fwd.head_dim);
         const Tensor ws = float_buffer(b.workspace_bytes, x);
         b.workspace = ptr(ws);

@@ -300,3 +300,34 @@ def test_gradients_are_differentiated_once():
         torch.autograd.grad(recorded[0].sum(), q, retain_graph=True)
     with pytest.raises(RuntimeError, match="differentiated again"):
         recorded[0].sum().backward()
+
+
+@pytest.mark.parametrize("nq,nkv", [(0, 2), (3, 0)])
+def test_a_tensor_without_heads(nq, nkv):
+    """Its weights' gradients are sums over nothing; the other tensor's are what they are."""
+    t, d, dtype = 9, 64, torch.bfloat16
+    q, k, w, dy, _ = _inputs(t, 3, 2, d, dtype, True, seed=13)
+    q, k, dy = q[:, :nq], k[:, :nkv], [dy[0][:, :nq], dy[1][:, :nkv]]
+    leaves = [x.contiguous().to(DEV).requires_grad_(True) for x in (q, k, *w)]
+    full = [torch.full((d,), float("nan"), dtype=dtype, device=DEV) for _ in range(64)]          # what memory holds that nobody wrote
+    del full
+
+    def call():
+        return ops.norm_rotary(leaves[0], leaves[1], leaves[2], leaves[3], 1e-5, leaves[4], leaves[5], layer_norm=True)
+    out = call()
+    assert out[0].shape == (t, nq, d) and out[1].shape == (t, nkv, d)
+    up = [x.contiguous().to(DEV) for x in dy]
+    grads = torch.autograd.grad(out, leaves, up)
+    empty = 0 if nq == 0 else 1
+    alone = torch.autograd.grad(call()[empty], leaves, up[empty], allow_unused=True)             # the tensor without heads alone
+    for i, x in enumerate(grads):
+        if i % 2 == empty:
+            assert x.shape == leaves[i].shape and float(x.float().abs().sum()) == 0.0 and float(alone[i].float().abs().sum()) == 0.0, i
+        else:
+            assert alone[i] is None
+    one = 1 - empty
+    dx, dw, db = oracle.norm_rotary_grad((q, k)[one], w[one], 1e-5, True, oracle.no_rotation, dy[one])
+    sums = ROUNDINGS + t * 3 // 8 + 16 + 128
+    _close("dx", grads[one], *dx, roundings=3 * ROUNDINGS)
+    _close("dw", grads[2 + one], *dw, roundings=sums)
+    _close("db", grads[4 + one], *db, roundings=sums)
