@@ -515,6 +515,7 @@ class ParallelSelfAttention(torch.nn.Module):
 
     `norm_rotary_in_one` (an argument of its own, off by default; may be set later): with `key_query_norm`, `forward` norms and rotates
     queries and keys in one launch (ops.norm_rotary) instead of two norms and a rotary, which rounds once where they round after each.
+    Calls with `use_cache` take the two norms and the rotary all the same: all keys of a cache are rounded alike.
     """
 
     norm_rotary_in_one = False               # of modules that were stored without it
@@ -705,7 +706,7 @@ class ParallelSelfAttention(torch.nn.Module):
         q, k, v = self._project(x)
         norms, rotated = None, False
         if self.key_query_norm:
-            if self.norm_rotary_in_one and not (use_cache and not reset_cache) and (self.rotary_embedding is None or pos is not None):
+            if self.norm_rotary_in_one and not use_cache and (self.rotary_embedding is None or pos is not None):
                 norms = self._own_norms()
             if norms is None:
                 q = self.norm_query(q)

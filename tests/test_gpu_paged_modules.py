@@ -6,7 +6,7 @@ import torch
 import oracle
 from scaling_amd import ops
 from scaling_amd.inference import TransformerInferenceModule
-from scaling_amd.layer import TransformerLayer, TransformerLayerIO
+from scaling_amd.layer import InferenceSettings, TransformerLayer, TransformerLayerIO
 from scaling_amd.nn import PagedKVCache
 from tests.kernels import launched
 from tests.parity import check
@@ -246,3 +246,29 @@ def test_the_first_call_over_a_cache_may_be_a_captured_one():
             torch.cuda.synchronize()
             assert torch.equal(y, want)
         assert int(cache.workspace().tickets.abs().sum()) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(norm_type="layernorm", mlp_type="default", mlp_factor=4.0), dict(relative_position_embedding_type="rotary_complex")], ids=["layernorm", "complex"])
+def test_cached_calls_round_their_keys_alike(kw):
+    """With the setting on, a prompt and the tokens behind it go into a KVCache as they do without it; a call without a cache is the one that takes the launch."""
+    cfg = _arch(key_query_norm=True, **kw)
+    layer = _seeded_layer(cfg, seed=0).eval()
+    att, g = layer.self_attention, torch.Generator().manual_seed(4)
+    x = torch.randn(2, 21, cfg.hidden_size, generator=g).to(cfg.precision.dtype).to(DEV)
+
+    def io(a, b, settings):
+        s = b - a
+        return TransformerLayerIO(activations=x[:, a:b], position_ids=torch.arange(a, b, device=DEV).repeat(2, 1), cumulative_seq_lengths=torch.tensor([0, s, 2 * s], dtype=torch.int32, device=DEV),
+                                  inference_settings=settings)
+
+    def generate():
+        with torch.no_grad():
+            out = [layer(io(0, 19, InferenceSettings(use_cache=True, reset_cache=True))).activations] + \
+                [layer(io(i, i + 1, InferenceSettings(use_cache=True, reset_cache=False))).activations for i in (19, 20)]
+        return (*out, att.cache[0].k[:, :21].clone(), att.cache[0].v[:, :21].clone())
+    plain = generate()
+    att.norm_rotary_in_one = True
+    assert not any("head_rows" in n for n in launched(generate))
+    for a, b in zip(plain, generate()):
+        assert torch.equal(a, b)
+    assert sum("head_rows" in n for n in launched(lambda: layer(io(0, 19, None)))) == 1
