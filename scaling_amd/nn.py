@@ -466,7 +466,10 @@ class PagedKVCache:
 
     def step(self, new: Sequence[int]) -> PagedStep:
         """Takes pages for new[b] more tokens of sequence b (0: none; one entry per sequence the cache has room for, or fewer: the first ones) and returns what the
-        layers' calls need.  Raises, with nothing taken, if a sequence would pass max_ctx or the pages run out.  Copies to the device: not while a graph is captured."""
+        layers' calls need.  Raises, with nothing taken, if a sequence would pass max_ctx or the pages run out, and while a graph is captured (it copies from host memory
+        that would be another's when the graph is replayed)."""
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a step of a paged cache is made in front of the capture that uses it")
         new = [int(count) for count in new]
         if not 0 < len(new) <= self.max_sequences or min(new) < 0 or sum(new) == 0:
             raise ValueError(f"new tokens of 1 to {self.max_sequences} sequences, at least one token in all, got {new}")

@@ -272,3 +272,16 @@ def test_cached_calls_round_their_keys_alike(kw):
     for a, b in zip(plain, generate()):
         assert torch.equal(a, b)
     assert sum("head_rows" in n for n in launched(lambda: layer(io(0, 19, None)))) == 1
+
+
+def test_a_step_is_not_captured():
+    cache = PagedKVCache(1, 12, 3, 64, 8, 2, 64, torch.bfloat16, DEV, page_size=16)
+    cache.step([5, 1])
+    x = torch.zeros(8, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="capture"):
+            cache.step([20, 1])
+    assert cache.lengths == [5, 1, 0] and cache.free_pages == 10
+    assert cache.step([20, 1]).ctx_len.tolist() == [25, 2]
