@@ -110,3 +110,37 @@ def attention(q, k_pages, v_pages, page_table, cu, ctx, causal, scale):
                 tiny = 2.0 ** -25 * (v[:limit, g].abs().sum(0) + 1) if q.dtype == torch.float16 else 0.0
                 out[row, h], bound[row, h] = o, (half * o.abs() + (1 + half) * (relative * size + tiny)) * (1 + 2.0 ** -20)
     return out, bound, owned
+
+
+def attention_by_sequence(q, k_pages, v_pages, page_table, cu, ctx, causal, scale):
+    """What `attention` gives, with the rows of a sequence and KV head together: for calls of thousands of rows."""
+    t, nq, d = q.shape
+    half = torch.finfo(q.dtype).eps / 2
+    page, nkv, n_pages = k_pages.shape[1], k_pages.shape[2], k_pages.shape[0]
+    rep = nq // nkv
+    owned = torch.zeros(t, dtype=torch.bool)
+    out, bound = torch.full((t, nq, d), math.nan, dtype=torch.float64), torch.full((t, nq, d), math.nan, dtype=torch.float64)
+    for b in range(len(ctx)):
+        n, rows = cu[b + 1] - cu[b], slice(cu[b], cu[b + 1])
+        length = max(0, min(ctx[b], page_table.shape[1] * page))
+        owned[rows] = True
+        if n == 0:
+            continue
+        ids = page_table[b, :-(-length // page)].long().clamp(0, n_pages - 1)
+        k, v = (x[ids].reshape(-1, nkv, d)[:length].double() for x in (k_pages, v_pages))
+        limit = (max(ctx[b], 0) - n + 1 + torch.arange(n)).clamp(0, length) if causal else torch.full((n,), length)
+        hidden = torch.arange(length) >= limit.repeat_interleave(rep)[:, None]
+        for g in range(nkv):
+            qs = q[rows, g * rep:(g + 1) * rep].double().reshape(n * rep, d)
+            if length == 0:
+                out[rows, g * rep:(g + 1) * rep] = bound[rows, g * rep:(g + 1) * rep] = 0.0
+                continue
+            p = torch.nan_to_num(torch.softmax((qs @ k[:, g].T * scale).masked_fill(hidden, -math.inf), 1))     # rows without keys: zeros
+            o, size = p @ v[:, g], p @ v[:, g].abs()
+            score = (qs.abs() @ k[:, g].abs().T * scale).masked_fill(hidden, 0.0).amax(1, keepdim=True)
+            relative = half + 2 * (d + 8) * 2.0 ** -24 * score + (length / 32 + 96) * 2.0 ** -24
+            tiny = 2.0 ** -25 * ((~hidden).double() @ v[:, g].abs() + 1) if q.dtype == torch.float16 else 0.0
+            b_rows = (half * o.abs() + (1 + half) * (relative * size + tiny)) * (1 + 2.0 ** -20)
+            b_rows[limit.repeat_interleave(rep) == 0] = 0.0
+            out[rows, g * rep:(g + 1) * rep], bound[rows, g * rep:(g + 1) * rep] = o.view(n, rep, d), b_rows.view(n, rep, d)
+    return out, bound, owned

@@ -1,0 +1,87 @@
+"""Attention over a paged cache where many sequences, blocks or splits decide how the work is cut: every row against float64."""
+
+import math
+
+import pytest
+import torch
+
+from scaling_amd import ops
+from tests import paged_oracle as oracle
+from tests.kernels import launched
+from tests.test_gpu_paged import DEV, _cache, _device, _ints
+
+pytestmark = pytest.mark.gpu
+
+ROWS, TILES, MERGE = "paged_rows", "paged_tiles", "paged_merge"
+ONE = [1]
+
+
+def _spread(n, lo, hi):
+    """n lengths between lo and hi, in no order"""
+    return [lo + (i * 7919) % n * (hi - lo) // max(n - 1, 1) for i in range(n)]
+
+
+# name: new tokens, keys with them, q heads, kv heads, d, page, type, whether max_q_len is given, launches (without tickets)
+CALLS = {
+    # Blocks for every compute unit (tokens x heads of a group / 256 x KV heads >= 256): chunks are not split.  17 x 16 blocks, longest first.
+    "many_blocks": ([1100, 1050, 1200, 1001], [1100, 1400, 1210, 2950], 16, 16, 32, 16, torch.bfloat16, True, [TILES]),
+    "many_blocks_f16": ([1100, 1050, 1200, 1001], [1300, 1050, 1210, 1700], 16, 16, 32, 64, torch.float16, True, [TILES]),
+    "many_blocks_gqa": ([700, 820, 690], [900, 2000, 690], 32, 8, 64, 32, torch.bfloat16, True, [TILES]),
+    # ... of more sequences than lanes, one after the other (21 x 16), short ones among them in blocks of few rows
+    "many_blocks_70_sequences": (_spread(70, 20, 140), _spread(70, 140, 700), 16, 16, 32, 16, torch.bfloat16, True, [ROWS, TILES, MERGE]),
+    # ... of as many sequences as lanes
+    "many_blocks_64_chunks": ([66] * 64, _spread(64, 66, 700), 16, 16, 32, 16, torch.bfloat16, True, [TILES]),
+    # ... and chunks alone (66 x 64 / 256 x 16 = 256)
+    "many_blocks_66_chunks": ([64] * 66, _spread(66, 64, 700), 16, 16, 32, 16, torch.bfloat16, True, [TILES]),
+    # 48 blocks of 64 that run at once, of one length: not split; of lengths far apart: split, with merges of 32 rows to a workgroup (48 x 4 blocks of 256 rows)
+    "level": ([500] * 6, [3000] * 6, 16, 4, 32, 64, torch.bfloat16, True, [TILES, MERGE]),
+    "not_level": ([500] * 6, [500, 600, 3000, 700, 900, 3900], 16, 4, 32, 64, torch.bfloat16, True, [TILES, MERGE]),
+    "not_level_70_sequences": ([1] * 40 + [500, 1, 500, 480] + [1] * 24 + [500, 490], [60] * 40 + [500, 40, 3000, 700] + [90] * 24 + [900, 3900], 16, 4, 32, 64, torch.bfloat16, True,
+                               [ROWS, TILES, MERGE]),
+    # chunks behind the 64th sequence; 40 blocks of the 128 that run at once, whose splits are cut until they do
+    "chunks_behind_64": ([1] * 66 + [300, 1, 290, 300, 1, 300, 270, 300, 1, 300, 260], [50 + i for i in range(66)] + [3000, 40, 3500, 900, 10, 3900, 2000, 3000, 700, 3100, 260], 8, 2, 64,
+                         16, torch.bfloat16, True, [ROWS, TILES, MERGE]),
+    "chunks_of_8": ([300, 290, 300, 270, 300, 260, 300, 300], [3000, 3500, 900, 3900, 2000, 3000, 3100, 260], 8, 2, 64, 16, torch.float16, True, [TILES, MERGE]),
+    # few blocks of few rows each: pieces of a half and a quarter of the blocks' rows
+    "short_chunks": ([20, 9, 24], [3000, 2000, 700], 16, 4, 128, 64, torch.bfloat16, True, [ROWS, TILES, MERGE]),
+    "shorter_chunks": (_spread(20, 8, 16), _spread(20, 500, 3000), 16, 4, 128, 64, torch.float16, True, [ROWS, TILES, MERGE]),
+    "two_blocks_of_few_rows": ([10, 9, 16], [3000, 2000, 700], 16, 4, 128, 64, torch.float16, True, [ROWS, MERGE]),
+    # 32 x 8 items: cut for a quarter of the workgroups where they are of one length
+    "even_tokens": (ONE * 32, [1500] * 32, 32, 8, 64, 16, torch.bfloat16, True, [ROWS, MERGE]),
+    "uneven_tokens": (ONE * 32, _spread(32, 20, 3000), 32, 8, 64, 16, torch.float16, True, [ROWS, MERGE]),
+    "even_drafts": ([5] * 32, [1200] * 32, 32, 8, 64, 32, torch.bfloat16, True, [ROWS, MERGE]),
+    "uneven_drafts": ([i % 8 + 1 for i in range(32)], _spread(32, 20, 2500), 32, 8, 64, 32, torch.bfloat16, True, [ROWS, MERGE]),
+    "tokens_of_200_sequences": (ONE * 200, _spread(200, 1, 1500), 8, 2, 64, 16, torch.bfloat16, True, [ROWS, MERGE]),
+    "even_tokens_of_130_sequences": (ONE * 130, [1100] * 130, 8, 2, 32, 16, torch.bfloat16, True, [ROWS, MERGE]),
+    "drafts_of_100_sequences": ([i % 6 for i in range(100)], _spread(100, 6, 1800), 16, 4, 32, 16, torch.bfloat16, True, [ROWS, MERGE]),
+    # no bound of the lengths: all kernels, whatever there is for them
+    "many_blocks_unbounded": ([1100, 1050, 1200, 1001], [1100, 1400, 1210, 2950], 16, 16, 32, 16, torch.bfloat16, False, [ROWS, TILES, MERGE]),
+    # more tokens than keys, in some of many blocks: rows without keys
+    "more_tokens_than_keys": ([1100, 1050, 1200, 1001], [500, 0, 1210, 3], 16, 16, 32, 16, torch.bfloat16, True, [TILES]),
+    "more_tokens_than_keys_level": ([500] * 6, [1500, 20, 300, 1500, 0, 1500], 16, 4, 32, 64, torch.bfloat16, True, [TILES, MERGE]),
+}
+
+
+@pytest.mark.parametrize("causal", [True, False], ids=["causal", "full"])
+@pytest.mark.parametrize("name", CALLS)
+def test_every_row(name, causal):
+    new, ctx, nq, nkv, d, page, dtype, bounded, launches = CALLS[name]
+    print(f"case {name} {causal}", flush=True)
+    k, v, table, cu = _cache(new, ctx, nkv, d, page, dtype, seed=sum(ctx) + d, spare=-(-max(0, 640 - max(ctx)) // page) + 1)
+    q = (1.5 * torch.randn(cu[-1], nq, d, generator=torch.Generator().manual_seed(d + nq))).to(dtype)
+    args = (q.to(DEV), _device(k), _device(v), table.to(DEV), _ints(cu), _ints(ctx))
+    kwargs = dict(causal=causal, max_q_len=max(new) if bounded else None)
+    out = torch.full_like(args[0], math.nan)
+    names = launched(lambda: ops.paged_attention(*args, out=out, **kwargs))
+    assert [n for n in (ROWS, TILES, MERGE) if any(n in x for x in names)] == launches, names
+    ref, bound, _ = oracle.attention_by_sequence(q, k, v, table, cu, ctx, causal, 1 / math.sqrt(d))
+    diff = (out.cpu().double() - ref).abs()
+    worst = diff / bound.clamp_min(1e-300)
+    print(f"max error / bound {float(worst.max()):.2f}", flush=True)
+    assert bool((diff <= bound).all()), f"over the bound in {int((~(diff <= bound)).any(-1).sum())} of {diff.shape[0] * nq} rows, by up to {float(worst.max())}"
+    ws = ops.paged_workspace(len(new), cu[-1], nq, nkv, d, DEV)
+    again = torch.full_like(out, math.nan)
+    for _ in range(2):                                      # with tickets: the same bits
+        assert torch.equal(ops.paged_attention(*args, out=again, workspace=ws, **kwargs), out)
+    torch.cuda.synchronize()
+    assert int(ws.tickets.abs().sum()) == 0
