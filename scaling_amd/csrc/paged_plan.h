@@ -86,9 +86,10 @@ MI_PLAN_FN int paged_split_tiles(const PagedPlan& p, int64_t units, int64_t bloc
     if (p.share == 0) return 0x1000000;                    // no sequence has more
     return (int)(paged_units(p, units, blocks, most) / (uint32_t)p.share) + 1;
 }
-// Tiles that a sequence's blocks have, by the middle one of them
+// Tiles that a sequence's blocks have, by the middle one of them (which of more tokens than keys may have none)
 template <int TILE> MI_PLAN_FN int paged_reached(const PagedSeq& s, const PagedWork& w, bool causal) {
-    return w.blocks * w.tiles - (causal ? (int)((int64_t)w.blocks * s.n / (2 * TILE)) : 0);
+    const int64_t all = (int64_t)w.blocks * w.tiles, hidden = causal ? (int64_t)w.blocks * s.n / (2 * TILE) : 0;
+    return all > hidden ? (int)(all - hidden) : 0;
 }
 // Blocks that run at once, more than half of what does, of which the longest is no more than half again a workgroup's share of all: not split, as twice the
 // pieces of half the length would take two rounds, and a merge.  (6 x 500 tokens of 3000 keys, 16 / 4 heads of 128, 192 blocks: 123 us split, 105 not; one prompt of 3900 tokens, whose
