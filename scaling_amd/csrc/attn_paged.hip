@@ -66,105 +66,35 @@ __device__ __forceinline__ int prefix_sum(int v) {
     return v;
 }
 
-// A sequence as one workgroup meets it; the same in every lane.
-struct Found {
-    int b;             // -1: none
-    int at;            // first slot of the sequence's blocks * splits; of a search for split blocks the first of these; longest first: as if it were one
-    int splits;
-    int partial;       // first partial result of the sequence (splits > 1)
-    PagedSeq seq;
-    PagedWork work;
+// The sequences of paged_find, lane by lane of a wavefront.  (Chunks that are not split, prompts of 2048 tokens, us by sequence and longest block first: 4, 16 heads
+// of 64: 97, 74; 16 of 500 - 4096, 8 heads of 64: 458, 412.)
+template <int BLOCK, int TILE> struct Wavefront {
+    const PagedParams& p;
+    const PagedPlan& plan;
+    PagedSeq s;
+    PagedWork w;
+    __device__ __forceinline__ void look(int base) {
+        const int b = base + (int)(threadIdx.x & 63), i = min(b, p.batch - 1);
+        s = paged_seq(p.cu[i], p.cu[i + 1], p.ctx[i], p.total, p.capacity);
+        w = paged_work<BLOCK, TILE>(plan, s, p.n_rep);
+        if (b >= p.batch) w.blocks = s.n = 0;
+    }
+    template <class F> __device__ __forceinline__ int of(const F& f) const { return f(s, w); }
+    template <class F> __device__ __forceinline__ int of(int v, const F& f) const { return f(w, v); }
+    __device__ __forceinline__ int value(int v, int l) const { return __builtin_amdgcn_readlane(v, l); }
+    __device__ __forceinline__ int64_t total(int v) const { return (int64_t)(uint32_t)value(prefix_sum(v), 63); }
+    __device__ __forceinline__ int most(int v) const { return group_max<64>(v); }
+    __device__ __forceinline__ int upto(int v) const { return prefix_sum(v); }
+    __device__ __forceinline__ int holder(int v, int upto, int x) const {
+        const uint64_t found = __ballot(x >= upto - v && x < upto);
+        return found != 0 ? __builtin_ctzll(found) : -1;
+    }
+    __device__ __forceinline__ PagedSeq seq(int l) const { return PagedSeq{value(s.first, l), value(s.n, l), value(s.ctx, l), value(s.len, l)}; }
+    __device__ __forceinline__ PagedWork work(int l) const { return PagedWork{value(w.blocks, l), value(w.tiles, l)}; }
 };
-
-// The sequence that holds slot `wanted` or, with OF_BLOCKS, the one that holds block `wanted` of all blocks with several splits; lane i looks at sequences
-// i, i + 64, ...
-template <int BLOCK, int TILE, bool OF_BLOCKS> __device__ __forceinline__ Found find_work(const PagedParams& p, const PagedPlan& plan, uint32_t share_m, int wanted) {
-    const int lane = threadIdx.x & 63;
-    PagedSeq seq{};
-    PagedWork work{};
-    auto look = [&](int base) {
-        const int b = base + lane, i = min(b, p.batch - 1);
-        seq = paged_seq(p.cu[i], p.cu[i + 1], p.ctx[i], p.total, p.capacity);
-        work = paged_work<BLOCK, TILE>(plan, seq, p.n_rep);
-        if (b >= p.batch) work.blocks = seq.n = 0;
-    };
-    const auto total = [](int v) { return (int64_t)(uint32_t)__builtin_amdgcn_readlane(prefix_sum(v), 63); };
-    Found f;
-    f.b = -1;
-    const auto take = [&](int l) {
-        f.seq.first = __builtin_amdgcn_readlane(seq.first, l);
-        f.seq.n = __builtin_amdgcn_readlane(seq.n, l);
-        f.seq.ctx = __builtin_amdgcn_readlane(seq.ctx, l);
-        f.seq.len = __builtin_amdgcn_readlane(seq.len, l);
-        f.work.blocks = __builtin_amdgcn_readlane(work.blocks, l);
-        f.work.tiles = __builtin_amdgcn_readlane(work.tiles, l);
-    };
-    if constexpr (BLOCK == kTileRows && !OF_BLOCKS) {
-        // Chunks that are not split: longest block first.  (Prompts of 2048 tokens, us by sequence and so: 4, 16 heads of 64: 97, 74; 16 of 500 - 4096, 8 heads of 64:
-        // 458, 412.)
-        if (plan.share == 0 && p.batch <= 64) {
-            look(0);
-            if (wanted >= total(work.blocks)) return f;
-            int lo = -1, hi = (group_max<64>(seq.len) + TILE - 1) / TILE, above_lo = work.blocks, above_hi = 0;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1, above = paged_above<BLOCK, TILE>(seq, work, p.n_rep, p.causal, mid);
-                if (total(above) > wanted) { lo = mid; above_lo = above; } else { hi = mid; above_hi = above; }
-            }
-            const int width = above_lo - above_hi, upto = prefix_sum(width), in = wanted - (int)total(above_hi);
-            const int l = __builtin_ctzll(__ballot(in >= upto - width && in < upto));
-            take(l);
-            f.b = l;
-            f.splits = 1;
-            f.partial = 0;
-            f.at = wanted - (__builtin_amdgcn_readlane(above_hi, l) + in - __builtin_amdgcn_readlane(upto - width, l));       // the block, counted from the last one, is wanted - at
-            return f;
-        }
-    }
-    int split_tiles = 0x1000000;                          // no sequence has more
-    if (plan.share > 0) {
-        int64_t units = 0, blocks = 0, reached = 0;
-        int most = 0;
-        for (int base = 0; base < p.batch; base += 64) {
-            look(base);
-            units += total(work.blocks * work.tiles);
-            if (plan.fit || plan.even) blocks += total(work.blocks);
-            if (plan.fit || plan.even) most = max(most, group_max<64>(work.blocks > 0 ? work.tiles : 0));
-            if (plan.fit) reached += total(paged_reached<TILE>(seq, work, p.causal));
-        }
-        split_tiles = divide(paged_units(plan, units, blocks, most), plan.share, share_m) + 1;      // paged_split_tiles
-        if (paged_level(plan, blocks, most, reached)) split_tiles = 0x1000000;
-        for (int step = 0; paged_few(plan, blocks) && step <= kPagedSteps; ++step) {
-            int64_t slots = 0;
-            for (int base = 0; base < p.batch; base += 64) {
-                if (p.batch > 64) look(base);
-                slots += total(work.blocks * paged_splits(plan, work, split_tiles));
-            }
-            if (slots <= plan.fit) break;
-            split_tiles = paged_next_tiles(plan, split_tiles, units, blocks, slots, step);
-        }
-    }
-    int at = 0, slots = 0, partials = 0;
-    for (int base = 0; base < p.batch; base += 64) {
-        if (p.batch > 64 || plan.share == 0) look(base);
-        const int splits = paged_splits(plan, work, split_tiles), n = work.blocks * splits, part = splits > 1 ? n : 0;
-        const int slots_upto = slots + prefix_sum(n), part_upto = partials + prefix_sum(part);
-        const int width = OF_BLOCKS ? (splits > 1 ? work.blocks : 0) : n, upto = OF_BLOCKS ? at + prefix_sum(width) : slots_upto;
-        const uint64_t found = __ballot(work.blocks > 0 && wanted >= upto - width && wanted < upto);
-        if (found != 0) {
-            const int l = __builtin_ctzll(found);
-            f.b = base + l;
-            f.at = __builtin_amdgcn_readlane(upto - width, l);
-            f.splits = __builtin_amdgcn_readlane(splits, l);
-            f.partial = __builtin_amdgcn_readlane(part_upto - part, l);
-            take(l);
-            if (!paged_fits(plan, f.work, f.splits, __builtin_amdgcn_readlane(slots_upto - n, l), f.partial)) f.b = -1;
-            return f;
-        }
-        slots = __builtin_amdgcn_readlane(slots_upto, 63);
-        partials = __builtin_amdgcn_readlane(part_upto, 63);
-        if constexpr (OF_BLOCKS) at = __builtin_amdgcn_readlane(upto, 63);
-    }
-    return f;
+template <int BLOCK, int TILE, PagedOrder ORDER> __device__ __forceinline__ PagedFound find_work(const PagedParams& p, const PagedPlan& plan, uint32_t share_m, int wanted) {
+    Wavefront<BLOCK, TILE> lanes{p, plan, {}, {}};
+    return paged_find<BLOCK, TILE, ORDER>(lanes, plan, share_m, p.batch, p.n_rep, p.causal, wanted);
 }
 
 // Page of the 16 keys from 16 * group on.  A number outside the cache is taken for the nearest inside.
@@ -255,7 +185,7 @@ template <int D> struct RowSum {
 // Rows r0 to r0 + n - 1 of block `block` of few rows, its splits merged by 256 threads: per row 16 / n groups of 16 lanes with a share of the splits each,
 // together through LDS (16 x (D + 2) floats).
 template <int D, int BLOCK, bool SHARED>
-__device__ __forceinline__ void merge_rows(const PagedParams& p, const Found& f, int block, int kvh, int r0, int n, float* lds) {
+__device__ __forceinline__ void merge_rows(const PagedParams& p, const PagedFound& f, int block, int kvh, int r0, int n, float* lds) {
     const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
     int per_row = 16;
     while (per_row * n > 16) per_row /= 2;
@@ -353,7 +283,7 @@ __global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_ke
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, G = lane >> 4;
     const int slot = divide(blockIdx.x, p.nkv, p.nkv_m), kvh = blockIdx.x - slot * p.nkv;
-    const Found f = find_work<BLOCK, kRowTile, false>(p, p.rows, p.share_m[0], slot);
+    const PagedFound f = find_work<BLOCK, kRowTile, kSlots>(p, p.rows, p.share_m[0], slot);
     if (f.b < 0) return;
     const int in = slot - f.at, split = paged_quotient(in, f.work.blocks), block = in - split * f.work.blocks;
     int s0, s1;
@@ -661,7 +591,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63, l32 = lane & 31, g = lane >> 5;
     const int slot = divide(blockIdx.x, p.nkv, p.nkv_m), kvh = blockIdx.x - slot * p.nkv;
-    const Found f = find_work<kTileRows, kTileKeys, false>(p, p.tiles, p.share_m[1], slot);
+    const PagedFound f = find_work<kTileRows, kTileKeys, kLongestFirst>(p, p.tiles, p.share_m[1], slot);
     if (f.b < 0) return;                                   // the same for the whole workgroup
     const int in = slot - f.at, split = paged_quotient(in, f.work.blocks), block = f.work.blocks - 1 - (in - split * f.work.blocks);      // longest first
     int s0, s1;
@@ -890,7 +820,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p, i
     if ((int)blockIdx.x < n_rows_groups) {
         constexpr int BLOCK = 16 * NB;
         const int at_kv = blockIdx.x / NB, r0 = blockIdx.x % NB * 16, at = divide(at_kv, p.nkv, p.nkv_m), kvh = at_kv - at * p.nkv;
-        const Found f = find_work<BLOCK, kRowTile, true>(p, p.rows, p.share_m[0], at);
+        const PagedFound f = find_work<BLOCK, kRowTile, kSplitBlocks>(p, p.rows, p.share_m[0], at);
         if (f.b < 0) return;
         const int n = min(16, f.seq.n * p.n_rep - (at - f.at) * BLOCK - r0);
         if (n > 0) merge_rows<D, BLOCK, false>(p, f, at - f.at, kvh, r0, n, lds);
@@ -898,7 +828,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p, i
     }
     const int group = blockIdx.x - n_rows_groups, at_kv = group / per_block, z = group - at_kv * per_block;
     const int at = divide(at_kv, p.nkv, p.nkv_m), kvh = at_kv - at * p.nkv;
-    const Found f = find_work<kTileRows, kTileKeys, true>(p, p.tiles, p.share_m[1], at);
+    const PagedFound f = find_work<kTileRows, kTileKeys, kSplitBlocks>(p, p.tiles, p.share_m[1], at);
     if (f.b < 0) return;
     const int block = at - f.at, n_rows = min(f.seq.n * p.n_rep - block * kTileRows, per_group * (z + 1));
     for (int in = per_group * z + (threadIdx.x >> 4); in < n_rows; in += 16) {

@@ -38,10 +38,8 @@ MI_PLAN_FN int paged_limit(const PagedSeq& s, int i, bool causal) {
     return causal ? paged_clamp((int64_t)s.ctx - s.n + i + 1, 0, s.len) : s.len;
 }
 
-// a / b for a < 2^24, 0 < b, by a reciprocal and corrections (the compiler's division is five times as long, and a workgroup's first steps wait for it)
-MI_PLAN_FN int paged_quotient(int a, int b) {
-#ifdef __HIP_DEVICE_COMPILE__
-    int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));      // two units in the last place of up to 24 bits: off by at most 2
+// a / b, of a q that is off by at most 2
+MI_PLAN_FN int paged_corrected(int a, int b, int q) {
     int r = a - q * b;
     for (int i = 0; i < 2; ++i) {
         const int by = r < 0 ? -1 : r >= b ? 1 : 0;
@@ -49,6 +47,11 @@ MI_PLAN_FN int paged_quotient(int a, int b) {
         r -= by * b;
     }
     return q;
+}
+// a / b for a < 2^24, 0 < b, by a reciprocal and corrections (the compiler's division is five times as long, and a workgroup's first steps wait for it)
+MI_PLAN_FN int paged_quotient(int a, int b) {
+#ifdef __HIP_DEVICE_COMPILE__
+    return paged_corrected(a, b, (int)((float)a * __builtin_amdgcn_rcpf((float)b)));      // two units in the last place of up to 24 bits
 #else
     return a / b;
 #endif
@@ -63,6 +66,11 @@ struct PagedPlan {
     int least;                    // sequences of no more tiles are not split
     int max_slots, max_partials;  // (set by the host) workgroups and partial results per KV head that there are
 };
+// u / share for u < 2^31: with m = 2^32 / share + 1 (of a share of 1: 0) the high half of a product is the quotient or one more
+MI_PLAN_FN int paged_by_share(const PagedPlan& p, uint32_t u, uint32_t m) {
+    const uint32_t q = (uint32_t)((uint64_t)u * m >> 32);
+    return (int)(m == 0 ? u : q * (uint32_t)p.share > u ? q - 1 : q);
+}
 
 struct PagedWork {
     int blocks, tiles;            // blocks 0: not this kernel's
@@ -82,9 +90,12 @@ MI_PLAN_FN uint32_t paged_units(const PagedPlan& p, int64_t units, int64_t block
     if (paged_few(p, blocks)) units *= p.share / p.fit;
     return (uint32_t)(units < 0x7fffffff ? units : 0x7fffffff);
 }
+MI_PLAN_FN int paged_split_tiles(const PagedPlan& p, int64_t units, int64_t blocks, int most, uint32_t share_m) {
+    return paged_by_share(p, paged_units(p, units, blocks, most), share_m) + 1;
+}
 MI_PLAN_FN int paged_split_tiles(const PagedPlan& p, int64_t units, int64_t blocks, int most) {
     if (p.share == 0) return 0x1000000;                    // no sequence has more
-    return (int)(paged_units(p, units, blocks, most) / (uint32_t)p.share) + 1;
+    return paged_split_tiles(p, units, blocks, most, p.share > 1 ? (uint32_t)((1ull << 32) / (uint32_t)p.share + 1) : 0);
 }
 // Tiles that a sequence's blocks have, by the middle one of them (which of more tokens than keys may have none)
 template <int TILE> MI_PLAN_FN int paged_reached(const PagedSeq& s, const PagedWork& w, bool causal) {
@@ -127,6 +138,110 @@ template <int BLOCK, int TILE> MI_PLAN_FN int paged_above(const PagedSeq& s, con
 MI_PLAN_FN bool paged_fits(const PagedPlan& p, const PagedWork& w, int splits, int slot, int partial) {
     const int64_t n = (int64_t)w.blocks * splits;
     return slot >= 0 && slot + n <= p.max_slots && (splits == 1 || (partial >= 0 && partial + n <= p.max_partials));
+}
+
+// A sequence as one workgroup meets it.
+struct PagedFound {
+    int b;             // -1: none
+    int at;            // first slot of the sequence's blocks * splits; of split blocks the first of these; longest first: as if it were one
+    int splits;
+    int partial;       // first partial result of the sequence (splits > 1)
+    PagedSeq seq;
+    PagedWork work;
+};
+// What is looked for: a slot, i.e. one of the blocks * splits of a sequence; a slot, where nothing is split longest block first; or one of all blocks that
+// have several splits.
+enum PagedOrder { kSlots, kLongestFirst, kSplitBlocks };
+
+// The sequence that holds `wanted`.  share_m: of paged_by_share.  It is looked for in groups of 64 sequences, one to a lane of LANES (a wavefront, or an array), which has
+//     look(base)          takes up sequences base .. base + 63; behind the last one they have no blocks
+//     of(f), of(v, f)     f(sequence, work), f(work, v's) of every lane: a Value, of which two can be subtracted
+//     total(v), most(v)   the sum (less than 2^32) and the maximum over the lanes
+//     upto(v)             of every lane the sum over the lanes up to it
+//     holder(v, upto, x)  of the lanes' parts laid end to end the lane that holds place x, or -1
+//     value(v, l), seq(l), work(l) of lane l
+template <int BLOCK, int TILE, PagedOrder ORDER, class LANES>
+MI_PLAN_FN PagedFound paged_find(LANES& lanes, const PagedPlan& p, uint32_t share_m, int batch, int n_rep, bool causal, int wanted) {
+    PagedFound f;
+    f.b = -1;
+    f.at = f.splits = f.partial = 0;
+    f.seq = PagedSeq{0, 0, 0, 0};
+    f.work = PagedWork{0, 0};
+    const auto blocks_of = [](const PagedSeq&, const PagedWork& w) { return w.blocks; };
+    if (ORDER == kLongestFirst && p.share == 0 && batch <= 64) {
+        lanes.look(0);
+        auto above_lo = lanes.of(blocks_of), above_hi = lanes.of([](const PagedSeq&, const PagedWork&) { return 0; });
+        if (wanted >= lanes.total(above_lo)) return f;
+        int lo = -1, hi = (lanes.most(lanes.of([](const PagedSeq& s, const PagedWork&) { return s.len; })) + TILE - 1) / TILE;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            const auto above = lanes.of([&](const PagedSeq& s, const PagedWork& w) { return paged_above<BLOCK, TILE>(s, w, n_rep, causal, mid); });
+            if (lanes.total(above) > wanted) { lo = mid; above_lo = above; } else { hi = mid; above_hi = above; }
+        }
+        const auto width = above_lo - above_hi, upto = lanes.upto(width);
+        const int in = wanted - (int)lanes.total(above_hi), l = lanes.holder(width, upto, in);
+        f.b = l;
+        f.splits = 1;
+        f.seq = lanes.seq(l);
+        f.work = lanes.work(l);
+        f.at = wanted - (lanes.value(above_hi, l) + in - lanes.value(upto - width, l));        // the block, counted from the last one, is wanted - at
+        return f;
+    }
+    int split_tiles = 0x1000000;                           // no sequence has more
+    if (p.share > 0) {
+        int64_t units = 0, blocks = 0, reached = 0;
+        int most = 0;
+        for (int base = 0; base < batch; base += 64) {
+            lanes.look(base);
+            units += lanes.total(lanes.of([](const PagedSeq&, const PagedWork& w) { return w.blocks * w.tiles; }));
+            if (p.fit || p.even) {
+                blocks += lanes.total(lanes.of(blocks_of));
+                const int longest = lanes.most(lanes.of([](const PagedSeq&, const PagedWork& w) { return w.blocks > 0 ? w.tiles : 0; }));
+                most = longest > most ? longest : most;
+            }
+            if (p.fit) reached += lanes.total(lanes.of([&](const PagedSeq& s, const PagedWork& w) { return paged_reached<TILE>(s, w, causal); }));
+        }
+        split_tiles = paged_split_tiles(p, units, blocks, most, share_m);
+        if (paged_level(p, blocks, most, reached)) split_tiles = 0x1000000;
+#ifdef __HIPCC__
+#pragma unroll 1
+#endif
+        for (int step = 0; paged_few(p, blocks) && step <= kPagedSteps; ++step) {
+            int64_t slots = 0;
+            for (int base = 0; base < batch; base += 64) {
+                if (batch > 64) lanes.look(base);
+                slots += lanes.total(lanes.of([&](const PagedSeq&, const PagedWork& w) { return w.blocks * paged_splits(p, w, split_tiles); }));
+            }
+            if (slots <= p.fit) break;
+            split_tiles = paged_next_tiles(p, split_tiles, units, blocks, slots, step);
+        }
+    }
+    int slots = 0, partials = 0, split_blocks = 0;
+    for (int base = 0; base < batch; base += 64) {
+        if (batch > 64 || p.share == 0) lanes.look(base);
+        const auto splits = lanes.of([&](const PagedSeq&, const PagedWork& w) { return paged_splits(p, w, split_tiles); });
+        const auto n = lanes.of(splits, [](const PagedWork& w, int i) { return w.blocks * i; });
+        const auto part = lanes.of(splits, [](const PagedWork& w, int i) { return i > 1 ? w.blocks * i : 0; });
+        const auto split = lanes.of(splits, [](const PagedWork& w, int i) { return i > 1 ? w.blocks : 0; });
+        // (all sums before they are asked for: none waits for another's)
+        const auto n_upto = lanes.upto(n), part_upto = lanes.upto(part), split_upto = ORDER == kSplitBlocks ? lanes.upto(split) : split;
+        const int l = ORDER == kSplitBlocks ? lanes.holder(split, split_upto, wanted - split_blocks) : lanes.holder(n, n_upto, wanted - slots);
+        if (l >= 0) {
+            const int slot = slots + lanes.value(n_upto - n, l);
+            f.b = base + l;
+            f.at = ORDER == kSplitBlocks ? split_blocks + lanes.value(split_upto - split, l) : slot;
+            f.splits = lanes.value(splits, l);
+            f.partial = partials + lanes.value(part_upto - part, l);
+            f.seq = lanes.seq(l);
+            f.work = lanes.work(l);
+            if (!paged_fits(p, f.work, f.splits, slot, f.partial)) f.b = -1;
+            return f;
+        }
+        slots += lanes.value(n_upto, 63);
+        partials += lanes.value(part_upto, 63);
+        if (ORDER == kSplitBlocks) split_blocks += lanes.value(split_upto, 63);
+    }
+    return f;
 }
 
 // Upper bounds for the host: blocks of rows that `tokens` tokens of `batch` sequences make, at most max_q_len of them in one; workgroups per KV head; and
