@@ -85,3 +85,46 @@ def test_every_row(name, causal):
         assert torch.equal(ops.paged_attention(*args, out=again, workspace=ws, **kwargs), out)
     torch.cuda.synchronize()
     assert int(ws.tickets.abs().sum()) == 0
+
+
+# Rows whose leading key is ahead of every other by 64 in the exponent: their output is the leader's value, which the sum of at most 4000 weights of
+# exp(-64) does not reach, times its weight over itself: both roundings of the weight's type (half a step each, of the result and of the weight for the product),
+# and float32 ones of the exponential, the sums and the division.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("new,ctx,nq,nkv,d,spare,launches", [
+    ([1, 40], [300, 80], 4, 2, 64, 0, [ROWS]),                          # blocks of few rows alone
+    ([1, 7], [1000, 900], 8, 2, 128, 1, [ROWS, MERGE]),                 # split
+    ([700, 90], [1000, 600], 4, 2, 32, 40, [TILES, MERGE]),             # chunks
+    ([300], [4000], 8, 2, 128, 1, [TILES, MERGE]),
+    ([1100, 1050, 1200, 1001], [1100, 1400, 1210, 1700], 16, 16, 32, 1, [TILES]),      # chunks that are not split
+], ids=["rows", "splits", "chunks", "chunk-splits", "unsplit"])
+def test_the_leading_key_wins(new, ctx, nq, nkv, d, spare, launches, dtype):
+    """Scores that rise along the keys by 64 each (the maximum moves in every tile), that fall (the first key leads), and rows of both in one block."""
+    page = 16
+    k, v, table, cu = _cache(new, ctx, nkv, d, page, dtype, seed=sum(ctx), spare=spare)
+    per_page = torch.zeros(k.shape[0], page, dtype=torch.int64)         # positions of the slots
+    for b, length in enumerate(ctx):
+        for i in range(-(-length // page)):
+            per_page[table[b, i]] = page * i + torch.arange(page)
+    stale = torch.isnan(k)
+    k.zero_()
+    k[..., 0], k[..., 1] = (per_page // 64)[..., None].to(dtype), (per_page % 64)[..., None].to(dtype)     # whole numbers below 64: exact in either type
+    k[stale] = math.nan
+    sign = torch.where(torch.randint(0, 2, (cu[-1], nq), generator=torch.Generator().manual_seed(1)) == 0, -1.0, 1.0)
+    q = torch.zeros(cu[-1], nq, d)
+    q[..., 0], q[..., 1] = 64 * 64 * sign, 64 * sign                    # score: 64 x position x sign, a whole number below 2^24
+    q = q.to(dtype)
+    args = (q.to(DEV), _device(k), _device(v), table.to(DEV), _ints(cu), _ints(ctx))
+    names = launched(lambda: ops.paged_attention(*args, softmax_scale=1.0, max_q_len=max(new)))
+    assert [n for n in (ROWS, TILES, MERGE) if any(n in x for x in names)] == launches, names
+    out = ops.paged_attention(*args, softmax_scale=1.0, max_q_len=max(new)).cpu().double()
+    half = torch.finfo(dtype).eps / 2
+    for b, n in enumerate(new):
+        pages = table[b, :-(-ctx[b] // page)].long()
+        values = v[pages].reshape(-1, nkv, d)[:ctx[b]].double().repeat_interleave(nq // nkv, 1)
+        rows = slice(cu[b], cu[b + 1])
+        leader = torch.where(sign[rows] > 0, (ctx[b] - n + torch.arange(n))[:, None], 0)
+        want = values[leader, torch.arange(nq)[None, :]]
+        diff = (out[rows] - want).abs()
+        bound = ((1 + half) ** 2 - 1 + 2.0 ** -18) * want.abs() + 4000 * math.exp(-64) * float(values.abs().max()) + 2.0 ** -24
+        assert bool((diff <= bound).all()), (b, float((diff / bound).max()))
