@@ -7,7 +7,7 @@ import oracle
 from scaling_amd import ops
 from scaling_amd.inference import TransformerInferenceModule
 from scaling_amd.layer import InferenceSettings, TransformerLayer, TransformerLayerIO
-from scaling_amd.nn import PagedKVCache
+from scaling_amd.nn import PagedKVCache, RotaryEmbedding
 from tests.kernels import launched
 from tests.parity import check
 from tests.test_gpu_modules import _arch, _oracle_layer, _seeded_layer
@@ -285,3 +285,46 @@ def test_a_step_is_not_captured():
             cache.step([20, 1])
     assert cache.lengths == [5, 1, 0] and cache.free_pages == 10
     assert cache.step([20, 1]).ctx_len.tolist() == [25, 2]
+
+
+class _Rotary(RotaryEmbedding):
+    """A rotary of somebody's own: the package's arithmetic, in another class."""
+
+    def rotate_tokens(self, *args, **kwargs):
+        self.calls = getattr(self, "calls", 0) + 1
+        return super().rotate_tokens(*args, **kwargs)
+
+
+@pytest.mark.parametrize("hooked,replaced", [(True, False), (False, True), (True, True)], ids=["hooked-norm", "replaced-rotary", "both"])
+def test_norms_and_rotary_of_somebodys_own(hooked, replaced):
+    """Over pages and, with the setting on, in a training step: what was hooked or replaced is called, and the outputs are the layer's."""
+    cfg = _arch(key_query_norm=True, rotary_percentage=0.5)     # (the rotary of a whole head is the attention kernels', by its tables)
+    layer = _seeded_layer(cfg, seed=0)
+    att, dtype, g = layer.self_attention, cfg.precision.dtype, torch.Generator().manual_seed(6)
+    att.norm_rotary_in_one = True
+    seen = []
+    if hooked:
+        att.norm_key.register_forward_hook(lambda module, args, out: seen.append(out.shape[0]))
+    if replaced:
+        att.rotary_embedding.__class__ = _Rotary
+    n = 37
+    x, dy = (torch.randn(1, n, cfg.hidden_size, generator=g).to(dtype) for _ in range(2))
+    cu, pos = torch.tensor([0, n], dtype=torch.int32), torch.arange(n).view(1, n)
+    ref, order = (_oracle_layer(cfg, layer.state_dict(), x, cu, pos, dy, t) for t in (torch.float32, dtype))
+
+    def train():
+        xg = x.to(DEV).requires_grad_()
+        y = layer(TransformerLayerIO(activations=xg, position_ids=pos.to(DEV), cumulative_seq_lengths=cu.to(DEV))).activations
+        y.backward(dy.to(DEV))
+        return y.detach(), xg.grad
+    names = launched(train)
+    assert any("head_rows" in name for name in names) == (not hooked), names       # norms alone where the rotary is another's
+    y, dx = train()
+    check("y", y, ref[0], order[0], module_level=True)
+    check("dx", dx, ref[1], order[1], module_level=True)
+    assert (not hooked or seen == [n, n]) and (not replaced or att.rotary_embedding.calls == 4)
+    layer.eval()
+    cache = PagedKVCache(1, 8, 1, 64, 4, 4, 64, dtype, DEV, page_size=16)
+    out = [layer.paged_step(x[:, a:b].to(DEV), cache, cache.step([b - a])) for a, b in ((0, 20), (20, 36), (36, n))]
+    check("paged", torch.cat(out, 1), ref[0], order[0], module_level=True)
+    assert (not hooked or seen[2:] == [20, 16, 1]) and (not replaced or att.rotary_embedding.calls == 10)
