@@ -331,3 +331,33 @@ def test_a_tensor_without_heads(nq, nkv):
     _close("dx", grads[one], *dx, roundings=3 * ROUNDINGS)
     _close("dw", grads[2 + one], *dw, roundings=sums)
     _close("db", grads[4 + one], *db, roundings=sums)
+
+
+def test_one_bias_and_leaves_without_gradients():
+    """A bias of one tensor alone; gradients of some of the leaves: the same as with all of them."""
+    t, nq, nkv, d, dtype = 21, 4, 2, 64, torch.bfloat16
+    q, k, w, dy, ids = _inputs(t, nq, nkv, d, dtype, True, seed=17)
+    cos, sin = _tables(64, d, dtype, False)
+    rotate, rotary = oracle.rotation(cos, sin, ids, d, False), (cos.to(DEV), sin.to(DEV), ids.to(DEV))
+    up = [x.to(DEV) for x in dy]
+    for given in (2, 3):
+        bias = [w[2] if given == 2 else None, w[3] if given == 3 else None]
+        leaves = {i: x.to(DEV).requires_grad_(True) for i, x in enumerate((q, k, w[0], w[1], *bias)) if x is not None}
+
+        def call(wanted):
+            at = [leaves[i] if i in wanted else None if i not in leaves else leaves[i].detach() for i in range(6)]
+            y = ops.norm_rotary(at[0], at[1], at[2], at[3], 1e-5, at[4], at[5], layer_norm=True, rotary=rotary)
+            return y, torch.autograd.grad(y, [leaves[i] for i in wanted], up)
+        y, grads = call(list(leaves))
+        grads = dict(zip(leaves, grads))
+        sums = ROUNDINGS + t * nq // 8 + 16 + 128
+        for i, x in enumerate((q, k)):
+            _close("y", y[i], *oracle.norm_rotary(x, w[i], bias[i], 1e-5, True, rotate))
+            dx, dw, db = oracle.norm_rotary_grad(x, w[i], 1e-5, True, rotate, dy[i])
+            _close("dx", grads[i], *dx, roundings=3 * ROUNDINGS)
+            _close("dw", grads[2 + i], *dw, roundings=sums)
+            if bias[i] is not None:
+                _close("db", grads[4 + i], *db, roundings=sums)
+        for wanted in ([0], [3], [given + 2], [1, 2]):
+            for i, x in zip(wanted, call(wanted)[1]):
+                assert torch.equal(x, grads[i]), (wanted, i)

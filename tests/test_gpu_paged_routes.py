@@ -8,6 +8,7 @@ import torch
 from scaling_amd import ops
 from tests import paged_oracle as oracle
 from tests.kernels import launched
+from tests.test_gpu_head_rows import _close, _tables
 from tests.test_gpu_paged import DEV, _cache, _device, _ints
 
 pytestmark = pytest.mark.gpu
@@ -128,3 +129,52 @@ def test_the_leading_key_wins(new, ctx, nq, nkv, d, spare, launches, dtype):
         diff = (out[rows] - want).abs()
         bound = ((1 + half) ** 2 - 1 + 2.0 ** -18) * want.abs() + 4000 * math.exp(-64) * float(values.abs().max()) + 2.0 ** -24
         assert bool((diff <= bound).all()), (b, float((diff / bound).max()))
+
+
+@pytest.mark.parametrize("new,ctx,nq,nkv,d,spare", [([3, 2], [40, 900], 8, 2, 64, 1), ([1, 1], [700, 90], 4, 2, 128, 1), ([100, 9], [150, 30], 4, 2, 64, 40), ([100], [3000], 4, 2, 64, 1),
+                                                   ([1100, 1050, 1200, 1001], [1100, 1400, 1210, 1700], 16, 16, 32, 1)], ids=["drafts", "tokens", "chunks", "splits", "unsplit"])
+def test_a_query_of_nan_stays_in_its_row(new, ctx, nq, nkv, d, spare):
+    k, v, table, cu = _cache(new, ctx, nkv, d, 16, torch.bfloat16, seed=5, spare=spare)
+    q = torch.randn(cu[-1], nq, d, generator=torch.Generator().manual_seed(2)).bfloat16().to(DEV)
+    rest = (_device(k), _device(v), table.to(DEV), _ints(cu), _ints(ctx))
+    clean = ops.paged_attention(q, *rest, max_q_len=max(new))
+    hit = torch.zeros(cu[-1], nq, dtype=torch.bool, device=DEV)
+    for i in range(len(new)):
+        hit[cu[i] + new[i] // 2, i % nq] = hit[cu[i + 1] - 1, nq - 1] = True
+    q[..., 5].masked_fill_(hit, math.nan)
+    out = ops.paged_attention(q, *rest, max_q_len=max(new))
+    assert bool(torch.isfinite(clean).all()) and bool(torch.isnan(out[hit]).all()) and torch.equal(out[~hit], clean[~hit])
+
+
+@pytest.mark.parametrize("name", ["sequences_150", "sequences_65", "float32_tables", "first_token_later"])
+def test_appends_by_other_ways(name):
+    """More sequences than lanes, empty ones among them; float32 tables; tokens in front of the first sequence."""
+    nq, nkv, d, page, dtype = 4, 2, 64, 16, torch.bfloat16
+    n = int(name.split("_")[1]) if name.startswith("sequences") else 5
+    new = [(i * 5) % 4 for i in range(n)]
+    new[0], new[-1] = 0, 2
+    ctx = [c + (i * 37) % 90 for i, c in enumerate(new)]
+    k_pages, v_pages, table, cu = _cache(new, ctx, nkv, d, page, dtype, seed=n, stale=2.0)
+    front = 3 if name == "first_token_later" else 0
+    cu = [c + front for c in cu]
+    total, g = cu[-1] + 2, torch.Generator().manual_seed(11)
+    q, k, v = (torch.randn(total, h, d, generator=g).to(dtype) for h in (nq, nkv, nkv))
+    w = [(1 + 0.3 * torch.randn(d, generator=g)).to(dtype) for _ in range(2)]
+    ids = torch.randint(0, 64, (total,), generator=g)
+    cos, sin = _tables(64, d, dtype, False, torch.float32 if name == "float32_tables" else None)
+    rotate = oracle.rotation(cos, sin, ids, d, False)
+    kp, vp = _device(k_pages), _device(v_pages)
+    out = ops.paged_append(k.to(DEV), v.to(DEV), kp, vp, table.to(DEV), _ints(cu), _ints(ctx), q=q.to(DEV), q_weight=w[0].to(DEV), k_weight=w[1].to(DEV),
+                           rotary=(cos.to(DEV), sin.to(DEV), ids.to(DEV)))
+    torch.cuda.synchronize()
+    _close("q", out, *oracle.norm_rotary(q, w[0], None, 1e-5, False, rotate))
+    where = oracle.slots(table, cu, ctx, page, k_pages.shape[0], total)
+    stored = [t for t in range(total) if where[t] is not None]
+    assert stored == list(range(cu[0], cu[-1]))
+    at = tuple(torch.tensor(i) for i in zip(*(where[t] for t in stored)))
+    ref, size = oracle.norm_rotary(k, w[1], None, 1e-5, False, rotate)
+    _close("k", kp.cpu()[at], ref[stored], size[stored])
+    assert torch.equal(vp.cpu()[at], v[stored])
+    written = torch.zeros(k_pages.shape[:2], dtype=torch.bool)
+    written[at] = True
+    assert torch.equal(kp.cpu()[~written], k_pages[~written]) and torch.equal(vp.cpu()[~written], v_pages[~written])
