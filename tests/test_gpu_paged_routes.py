@@ -178,3 +178,18 @@ def test_appends_by_other_ways(name):
     written = torch.zeros(k_pages.shape[:2], dtype=torch.bool)
     written[at] = True
     assert torch.equal(kp.cpu()[~written], k_pages[~written]) and torch.equal(vp.cpu()[~written], v_pages[~written])
+
+
+@pytest.mark.parametrize("new,ctx,spare", [([3, 1], [40, 900], 1), ([100, 9], [150, 30], 40), ([100], [3000], 1)], ids=["rows", "chunks", "splits"])
+def test_keys_that_all_score_minus_infinity_give_zeros(new, ctx, spare):
+    """As a row without keys does; a score of plus infinity among them gives NaN."""
+    nq, nkv, d = 4, 2, 64
+    k, v, table, cu = _cache(new, ctx, nkv, d, 16, torch.bfloat16, seed=6, spare=spare, stale=0.5)
+    k[..., 7] = -math.inf
+    q = torch.randn(cu[-1], nq, d, generator=torch.Generator().manual_seed(2)).bfloat16().to(DEV)
+    q[..., 7] = 1.0
+    q[cu[-1] - 1, 1, 7] = -1.0
+    out = ops.paged_attention(q, _device(k), _device(v), table.to(DEV), _ints(cu), _ints(ctx), max_q_len=max(new))
+    assert bool(torch.isnan(out[-1, 1]).all())
+    out[-1, 1] = 0.0
+    assert float(out.abs().max()) == 0.0
