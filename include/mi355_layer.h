@@ -362,7 +362,7 @@ int mi_paged_append(const mi_paged_append_args* args);
 
 /* Attention of the new tokens over the pages (mi_paged_append first): token i of the n of sequence b attends to its keys at positions u < ctx_len[b] and, when
  * causal, u <= ctx_len[b] - n + i.  Softmax in fp32 of scores scaled by softmax_scale, probabilities rounded to `dtype` before P V as in mi_attn_fwd; a row
- * without keys yields zeros.  q, o (which share no memory) [total_q, n_q_heads, head_dim] by element strides; query head h reads KV head h / (n_q_heads / n_kv_heads).  Rows of o
+ * without keys yields zeros, and so does one whose keys all score -inf (mi_attn_fwd's choice too; the quotient would be 0 / 0).  q, o (which share no memory) [total_q, n_q_heads, head_dim] by element strides; query head h reads KV head h / (n_q_heads / n_kv_heads).  Rows of o
  * behind the last sequence are left as they are.  head_dim in {32, 64, 96, 128}, bf16 or f16, max_pages * page_size <= 2^30.
  * max_q_len: an upper bound of the new tokens of a sequence, 0 if unknown (the launches for longer ones are then made too; sequences over the bound may be
  * left out).  Lengths beyond the page table count its room; a page number outside the cache reads the nearest page inside.

@@ -242,7 +242,7 @@ __device__ __forceinline__ void own_keys_only(const PagedParams& p, const int32_
         }
         s = lane < n ? s * p.scale_log2 : -INFINITY;
         const float m = fmaxf(M, group_max<64>(s)), use = m == -INFINITY ? 0.f : m, alpha = M == -INFINITY ? 0.f : fast_exp2(M - use);
-        const float e = lane < n ? fast_exp2(s - use) : 0.f, e_rounded = (float)(elem_t)e;
+        const float e = lane < n ? fast_exp2(s - use) : 0.f, e_rounded = (float)(elem_t)e;      // as the kernels' products have it
         L = L * alpha + group_sum<64>(e);
         O0 *= alpha;
         O1 *= alpha;
@@ -266,8 +266,8 @@ __device__ __forceinline__ void own_keys_only(const PagedParams& p, const int32_
 //     O^T[feature][row] += V^T P^T    V passes through a wavefront's own LDS and is read back transposed
 // Every cached element is read from memory once per block of rows.  The next chunk's K is requested as soon as the scores are computed and its V as soon as this
 // chunk's is in LDS, into the same registers: 16 KB a wavefront (d 128) are always under way, and 12 wavefronts fit a compute unit.  (Two sets of registers, a
-// whole chunk ahead: 8 wavefronts, 16 rows to a block at the most.)  Bound by memory: 32 x 8 items of 200 - 8192 keys of 128 features 84.7 us, 6.1 TB/s; few items
-// by the start and the merge besides, ~10 us: 8 x 8 items of 4096 keys 32.7, a single one of 1500 9.7 (6.5 and a second launch of 5.5 without the merge in it).
+// whole chunk ahead: 8 wavefronts, 16 rows to a block at the most.)  Bound by memory: 32 x 8 items of 200 - 8192 keys of 128 features 83.8 - 85.6 us, 6.1 TB/s; few items
+// by the start and the merge besides, ~10 us: 8 x 8 items of 4096 keys 32.7, a single one of 1500 9.8 (6.5 and a second launch of 5.5 without the merge in it).
 template <int D, int NB>
 __global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_kernel(const PagedParams p) {
     constexpr int NWV = kRowWaves, kThreads = 64 * NWV, BLOCK = 16 * NB;
@@ -572,9 +572,12 @@ template <int D> struct PageDma {
 // K requested three tiles ahead by the second four wavefronts and V two by the first.  The two groups of four run half a tile apart (enforced by the
 // barriers), so on every SIMD one wavefront issues products while the other computes its softmax:
 //     S^T = K Q^T      A = K rows from LDS, B = Q in registers
-//     softmax          a lane's column is a row of the block; the maximum is raised only when it lags by 2^8, so most tiles rescale nothing
+//     softmax          a lane's column is a row of the block; the maximum is raised only when it lags by 2^8, so most tiles rescale nothing; probabilities (up
+//                      to 2^8 then) are rounded to the element type for the product, as in mi_attn_fwd: half a step of each, where P in two
+//                      terms would be twice the products of P V.  (Relative error of the outputs against 64 bits: 0.0023 bf16, 0.00029 f16, of which one rounding
+//                      of the output alone leaves 0.0017, 0.00021)
 //     O^T += V^T P^T   B = P^T as the accumulators of S^T hold it, A = V^T by transposing LDS reads
-// Bound by the matrix pipe (busy half of the time) and the power that it draws: 4 x 2048 tokens behind 2048 - 14336 others, 32 / 8 heads of 128, 1083 us, 1.07 PFLOP/s, as
+// Bound by the matrix pipe (busy half of the time) and the power that it draws: 4 x 2048 tokens behind 2048 - 14336 others, 32 / 8 heads of 128, 1055 - 1106 us by the card's clock, 1.05 - 1.10 PFLOP/s, as
 // mi_attn_fwd over contiguous keys; without its softmax 951, without its operand reads 890.  (Operands 2, 4, 8 products ahead instead of 3: 1104, 1076, 1093; the
 // first of them before the barrier: 1150.)
 template <int D>

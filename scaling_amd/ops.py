@@ -273,7 +273,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     tokens per sequence, one (a decode step) and none included (inference; no autograd).
 
     q [tokens, n_q, d] (bfloat16 or float16; d 32, 64, 96 or 128), query head h reading KV head h // (n_q / n_kv).  Token i of the n of a sequence sees keys
-    u < ctx_len and, with `causal`, u <= ctx_len - n + i; without any its row is zeros.  Rows behind the last sequence are left as they are in `out` (of a new
+    u < ctx_len and, with `causal`, u <= ctx_len - n + i; without any, and where all of them score -inf, its row is zeros.  Rows behind the last sequence are left as they are in `out` (of a new
     tensor: undefined), which shares no memory with q.  max_q_len: an upper bound of the tokens of a sequence, where the caller knows one (1: no launches for chunks); longer ones
     may be left out.  Lengths beyond the page table count its room.  workspace: see `paged_workspace`; without one it is allocated per call."""
     _need_cuda(q, k_pages, v_pages, page_table, cu_seqlens, ctx_len, workspace, out)
