@@ -7,7 +7,7 @@
 //     W = sum over sequences of blocks * tiles,   S = floor(W / share) + 1,   splits_b = ceil(tiles_b / S), of short sequences 1
 // Then splits of all blocks are at most share + blocks in number, and those of sequences with more than one split at most 2 * share (tiles > S gives
 // ceil(tiles / S) < 2 tiles / S).  Lengths may be anything: sequences are clamped to the tokens and the page table that there are, and where lengths that
-// overlap make more workgroups or partial results than there are, sequences are left out as a whole.
+// overlap make more workgroups or partial results than there are, what is too many is left out (of work that is split: sequences as a whole).
 #pragma once
 #include <stdint.h>
 

@@ -361,3 +361,23 @@ def test_one_bias_and_leaves_without_gradients():
         for wanted in ([0], [3], [given + 2], [1, 2]):
             for i, x in zip(wanted, call(wanted)[1]):
                 assert torch.equal(x, grads[i]), (wanted, i)
+
+
+@pytest.mark.parametrize("nq,nkv,layer_norm", [(40, 1, True), (3, 38, False)], ids=["layernorm", "rms"])
+def test_more_rows_than_the_workgroups_of_the_backward_pass(nq, nkv, layer_norm):
+    """Workgroups take several items each, divided between the tensors by their rows."""
+    t, d, dtype = 3500, 128, torch.bfloat16
+    q, k, w, dy, ids = _inputs(t, nq, nkv, d, dtype, layer_norm, seed=23)
+    cos, sin = _tables(64, d, dtype, False)
+    rotate, rotary = oracle.rotation(cos, sin, ids, d, False), (cos.to(DEV), sin.to(DEV), ids.to(DEV))
+    leaves = [None if x is None else x.to(DEV).requires_grad_(True) for x in (q, k, *w)]
+    y = ops.norm_rotary(leaves[0], leaves[1], leaves[2], leaves[3], 1e-5, leaves[4], leaves[5], layer_norm=layer_norm, rotary=rotary)
+    grads = torch.autograd.grad(y, [x for x in leaves if x is not None], [x.to(DEV) for x in dy])
+    sums = ROUNDINGS + t * max(nq, nkv) // 8 + 16 + 128
+    for i, x in enumerate((q, k)):
+        _close("y", y[i], *oracle.norm_rotary(x, w[i], w[i + 2], 1e-5, layer_norm, rotate))
+        dx, dw, db = oracle.norm_rotary_grad(x, w[i], 1e-5, layer_norm, rotate, dy[i])
+        _close("dx", grads[i], *dx, roundings=3 * ROUNDINGS)
+        _close("dw", grads[2 + i], *dw, roundings=sums)
+        if layer_norm:
+            _close("db", grads[4 + i], *db, roundings=sums)
