@@ -222,6 +222,37 @@ int mi_argmax(const void* x, int64_t n_rows, int64_t vocab, int64_t row_stride, 
  * hidden and table_stride multiples of 8 elements (4 for fp32). */
 int mi_argmax_embed(const void* x, int64_t n_rows, int64_t vocab, int64_t row_stride, int64_t* index, const void* table, int64_t table_rows,
                     int64_t table_stride, int64_t hidden, void* out, int dtype, void* stream);
+/* ------------------------------------------------------------------------------------------
+ * A token of every row of logits from one random number a row (no counterpart in the reference, which samples greedily: inference/sample.py:5-6).
+ * The tokens of a row in the order of their values, largest first, equal ones by index; weights w = exp((x - max) / temperature).  Each of
+ *   top_k (> 0)        the first top_k
+ *   top_p (< 1)        the fewest, of those top_k leaves, whose weights are at least top_p of these together; one at least
+ *   min_p (> 0)        those of a weight of at least min_p (the largest weighs 1); one at least
+ * keeps the first so many.  ids[r] is the first token at which the running sum of the weights exceeds uniforms[r] times the sum of what is kept; logprobs[r] (may be
+ * NULL) the natural logarithm of its weight over that sum.  temperature <= 0 or NaN: the first token (and 0).  NaN and -inf logits have no weight; where the largest
+ * is +inf, those alone have one; a row without any gives token 0 (and -inf).  uniforms outside [0, 1) are taken for the nearest inside, NaN for 0.
+ * Weights are rounded from 64 bits to parts of 2^51 (of more than 2048 tokens: so that all fit 62 bits) and summed as whole numbers.
+ * Each parameter is an array of a value per row or, where that is NULL, one value.  row_stride in elements; rows need not be 16-byte aligned.
+ * Algorithmic HBM bytes: n_rows * vocab * e.
+ * ------------------------------------------------------------------------------------------ */
+#define MI_SAMPLE_VOCAB_MAX 4194304
+typedef struct mi_sample_args {
+    const void* logits;
+    int64_t n_rows, vocab, row_stride;
+    const float* uniforms;         /* [n_rows] */
+    const float* temperatures;
+    const int32_t* top_ks;
+    const float* top_ps;
+    const float* min_ps;
+    float temperature;
+    int32_t top_k;
+    float top_p, min_p;
+    int64_t* ids;                  /* [n_rows] */
+    float* logprobs;               /* [n_rows] or NULL */
+    int32_t dtype;
+    void* stream;
+} mi_sample_args;
+int mi_sample(const mi_sample_args* args);
 /* The weighted mean of cross_entropy.py:30 and the accuracy of :81-86 in one launch:
  *   loss = sum(losses * weights) / sum(weights),  total = sum(weights),
  *   accuracy = share of the rows with weights > 0 whose argmax is the target

@@ -28,7 +28,7 @@ EXPORTS = (
     "mi_attn_fwd", "mi_attn_bwd_workspace_bytes", "mi_attn_bwd_workspace_bytes_kv", "mi_attn_bwd_workspace_bytes_for", "mi_attn_bwd",
     "mi_gemm", "mi_gemm_workspace_bytes", "mi_gemm_with_workspace", "mi_rows_product", "mi_transpose16", "mi_column_sum", "mi_add_rmsnorm_bwd", "mi_add_layernorm_fwd", "mi_add_layernorm_bwd", "mi_attn_decode_workspace_bytes", "mi_attn_decode", "mi_attn_decode_with_tickets", "mi_fill_cache", "mi_attn_decode_static_scratch_bytes", "mi_attn_decode_static",
     "mi_norm_rotary_fwd", "mi_norm_rotary_bwd_workspace_bytes", "mi_norm_rotary_bwd", "mi_paged_append",
-    "mi_paged_attn_workspace_bytes", "mi_paged_attn_tickets", "mi_paged_attn",
+    "mi_paged_attn_workspace_bytes", "mi_paged_attn_tickets", "mi_paged_attn", "mi_sample",
 )
 
 
@@ -149,6 +149,14 @@ class MiPagedAttnArgs(Structure):
     ]
 
 
+class MiSampleArgs(Structure):
+    _fields_ = [
+        ("logits", c_void_p), ("n_rows", c_int64), ("vocab", c_int64), ("row_stride", c_int64), ("uniforms", c_void_p), ("temperatures", c_void_p),
+        ("top_ks", c_void_p), ("top_ps", c_void_p), ("min_ps", c_void_p), ("temperature", c_float), ("top_k", c_int32), ("top_p", c_float), ("min_p", c_float),
+        ("ids", c_void_p), ("logprobs", c_void_p), ("dtype", c_int32), ("stream", c_void_p),
+    ]
+
+
 _lib = None
 _host = None
 _device_checked = False
@@ -244,6 +252,8 @@ def _declare(lib):
     lib.mi_paged_attn_tickets.argtypes = [c_int32]
     lib.mi_paged_attn.restype = c_int
     lib.mi_paged_attn.argtypes = [POINTER(MiPagedAttnArgs)]
+    lib.mi_sample.restype = c_int
+    lib.mi_sample.argtypes = [POINTER(MiSampleArgs)]
     lib.mi_attn_fwd.restype = c_int
     lib.mi_attn_fwd.argtypes = [POINTER(MiAttnArgs)]
     lib.mi_attn_bwd_workspace_bytes.restype = c_size_t

@@ -1908,6 +1908,34 @@ std::optional<std::tuple<Tensor, Tensor>> op_argmax_embed(const Tensor& x, const
     return std::make_tuple(index, out);
 }
 
+// A token of each row of x [rows, n] and its log-probability.  Parameters: a tensor of one value per row, or one value.
+std::tuple<Tensor, OptTensor> op_sample_rows(const Tensor& x, const Tensor& uniforms, const OptTensor& temperatures, const OptTensor& top_ks, const OptTensor& top_ps,
+                                             const OptTensor& min_ps, double temperature, int64_t top_k, double top_p, double min_p, bool logprobs) {
+    need_gpu(x);
+    TORCH_CHECK(x.dim() == 2 && (x.size(1) <= 1 || x.stride(1) == 1), "sample_rows: logits are [rows, vocab] with contiguous rows");
+    const auto per_row = [&](const OptTensor& t, at::ScalarType type, const char* name) -> void* {
+        if (!t.has_value()) return nullptr;
+        TORCH_CHECK(t->device() == x.device() && t->scalar_type() == type && t->dim() == 1 && t->size(0) == x.size(0) && t->is_contiguous(), "sample_rows: ", name,
+                    " is a contiguous ", c10::toString(type), " tensor [rows] on the device of the logits");
+        return ptr(*t);
+    };
+    mi_sample_args a{};
+    a.logits = ptr(x); a.n_rows = x.size(0); a.vocab = x.size(1); a.row_stride = x.stride(0); a.dtype = code_of(x);
+    a.uniforms = static_cast<const float*>(per_row(uniforms, at::kFloat, "uniforms"));
+    a.temperatures = static_cast<const float*>(per_row(temperatures, at::kFloat, "temperature"));
+    a.top_ks = static_cast<const int32_t*>(per_row(top_ks, at::kInt, "top_k"));
+    a.top_ps = static_cast<const float*>(per_row(top_ps, at::kFloat, "top_p"));
+    a.min_ps = static_cast<const float*>(per_row(min_ps, at::kFloat, "min_p"));
+    a.temperature = (float)temperature; a.top_k = (int32_t)std::clamp<int64_t>(top_k, 0, INT32_MAX); a.top_p = (float)top_p; a.min_p = (float)min_p;
+    Launch l(x);
+    const Tensor ids = at::empty({x.size(0)}, x.options().dtype(at::kLong));
+    OptTensor lp;
+    if (logprobs) lp = at::empty({x.size(0)}, x.options().dtype(at::kFloat));
+    a.ids = ids.data_ptr<int64_t>(); a.logprobs = logprobs ? lp->data_ptr<float>() : nullptr; a.stream = l.stream;
+    check(mi_sample(&a), "mi_sample");
+    return {ids, lp};
+}
+
 // One token per sequence through a pre-norm layer (RMSNorm, separate q / k / v, SwiGLU, no biases): five launches, plus the merge of
 // the decode attention and the norms in front of wide products.  x [batch, 1, hidden]; raises ctx_len by one and appends to the caches.  Nothing happens, and nothing
 // is returned, where a shape, type or alignment does not suit the kernels.
@@ -2009,5 +2037,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     def("norm_linear_rows", &op_norm_linear_rows);
     def("argmax_rows", &op_argmax_rows);
     def("argmax_embed", &op_argmax_embed);
+    def("sample_rows", &op_sample_rows);
     def("decode_layer", &op_decode_layer);
 }

@@ -9,7 +9,7 @@ under saved-tensor hooks (activation checkpointing) and are deterministic under 
 
 import ctypes  # noqa: F401 - for callers that fill an argument block with _fill_attn_args and hand it to the C ABI
 import math
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 from torch.overrides import _get_current_function_mode_stack, has_torch_function
@@ -22,7 +22,7 @@ __all__ = [
     "rms_norm", "swiglu", "rotary_embedding", "rotary_embedding_complex", "attention", "attention_forward", "attention_backward",
     "decode_attention", "rms_norm_forward", "rms_norm_backward", "swiglu_forward", "swiglu_backward",
     "cross_entropy", "cross_entropy_forward", "linear_cross_entropy", "weighted_cross_entropy", "add_rms_norm",
-    "norm_rotary", "paged_append", "paged_attention", "paged_workspace",
+    "norm_rotary", "paged_append", "paged_attention", "paged_workspace", "sample_rows",
 ]
 
 
@@ -651,6 +651,31 @@ def argmax_rows(x: torch.Tensor) -> torch.Tensor:
 def argmax_embed(x: torch.Tensor, table: torch.Tensor) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
     """(argmax_rows(x), table[argmax_rows(x)]) of x [rows, n] and table [at least n, hidden] in one launch (inference); None where the kernel does not apply."""
     return None if _taken_over((x, table)) or not x.is_cuda else _lib.host().argmax_embed(x, table)
+
+
+def sample_rows(logits: torch.Tensor, uniforms: torch.Tensor, temperature: Union[float, torch.Tensor] = 1.0, top_k: Union[int, torch.Tensor] = 0,
+                top_p: Union[float, torch.Tensor] = 1.0, min_p: Union[float, torch.Tensor] = 0.0, return_logprobs: bool = False):
+    """A token of each row of logits [rows, vocab] (bfloat16, float16 or float32; contiguous rows, any stride) by uniforms float32 [rows] in [0, 1): int64 [rows], and
+    with `return_logprobs` also float32 [rows], the logarithm of the probability that the token had (inference; one launch, no autograd).
+
+    Tokens are ordered by value, largest first, equal ones by index, and weigh exp((x - max) / temperature).  top_k > 0 keeps the first top_k; top_p < 1 of these
+    the fewest with at least top_p of their weight, one at least; min_p > 0 those of at least min_p times the largest weight.  The token is the first of the order at
+    which the running sum of weights exceeds u times the sum of what is kept, so the same numbers give the same tokens, whatever else is in the batch.
+    temperature <= 0: the first token of the order, with logarithm 0.  Each parameter is a number (taken as float32) or a tensor of a value per row (float32, top_k int32)
+    on the logits' device.  -inf and NaN logits are never drawn; a row of nothing else gives token 0 and -inf."""
+    _need_cuda(logits, uniforms)
+    tensors, numbers = [], []
+    for name, value, off in (("temperature", temperature, 1.0), ("top_k", top_k, 0), ("top_p", top_p, 1.0), ("min_p", min_p, 0.0)):
+        if isinstance(value, torch.Tensor):
+            _need_cuda(value)
+        elif isinstance(value, bool) or not isinstance(value, (int, float)) or (name == "top_k" and not isinstance(value, int)):
+            raise TypeError(f"sample_rows: {name} is a number or a tensor, got {value!r}")
+        elif value != value:
+            raise ValueError(f"sample_rows: {name} is NaN")
+        tensors.append(value if isinstance(value, torch.Tensor) else None)
+        numbers.append(off if isinstance(value, torch.Tensor) else value)
+    ids, logprobs = _lib.host().sample_rows(logits, uniforms, *tensors, float(numbers[0]), numbers[1], float(numbers[2]), float(numbers[3]), bool(return_logprobs))
+    return (ids, logprobs) if return_logprobs else ids
 
 
 def decode_layer_arguments(norm1, eps1, qkv_weights, dense, norm2, eps2, w_in, w_gate, w_out, head_dim, k_cache, v_cache, ctx_len, tables,
