@@ -391,6 +391,39 @@ typedef struct mi_paged_append_args {
 } mi_paged_append_args;
 int mi_paged_append(const mi_paged_append_args* args);
 
+/* The next step of a paged cache whose lengths lie on the device (the reference has no paged cache): takes pages and lays the new tokens out, so that no host has to
+ * know how long the sequences are.  new_tokens[b] > 0: so many more tokens of sequence b; 0: none; < 0: the sequence ends, its pages go back and its length is 0.
+ *   lengths [batch]         keys before the step;  ctx_len [batch]: with it, may be lengths itself
+ *   state [2]               free pages on the stack, and the status;  state_out [2]: after the step, may be state itself
+ *   free_pages [n_free]     the stack, the next page to take last
+ *   page_table              [batch, max_pages] by stride: the pages taken are written behind those that a sequence has
+ *   cu_seqlens [batch + 1], last [batch]: rows of the sequences in the step, and of their last new tokens (0 of those without any)
+ *   position_ids, slots, sequences [tokens]: of each row its position (plus position_offset[b] where that is given), page * page_size + row in the page, and
+ *                           sequence; of rows behind the last sequence 0, -1 and 0
+ * Pages that are given back (last page first, sequence by sequence) are there to be taken.  Where pages do not suffice (1), a sequence would pass max_ctx keys (0: what
+ * the table has room for) (2), or there are more than `tokens` new tokens (4), nothing is taken by anybody, cu_seqlens is all zeros, and the
+ * number is set in the status, which nothing here clears.  Lengths outside the table's room count the nearest inside; pages that would pass the end of the stack are
+ * dropped.  batch, max_pages, tokens up to 2^24, max_pages * page_size up to 2^30. */
+typedef struct mi_paged_step_args {
+    const int32_t* new_tokens;
+    const int32_t* lengths;
+    const int32_t* state;
+    const int32_t* position_offset;    /* [batch] or NULL */
+    int32_t* ctx_len;
+    int32_t* state_out;
+    int32_t* page_table;
+    int32_t* free_pages;
+    int32_t* cu_seqlens;
+    int64_t* position_ids;
+    int64_t* slots;
+    int64_t* sequences;
+    int64_t* last;
+    int64_t page_table_stride;
+    int32_t batch, max_pages, page_size, n_free, tokens, max_ctx;
+    void* stream;
+} mi_paged_step_args;
+int mi_paged_step(const mi_paged_step_args* args);
+
 /* Attention of the new tokens over the pages (mi_paged_append first): token i of the n of sequence b attends to its keys at positions u < ctx_len[b] and, when
  * causal, u <= ctx_len[b] - n + i.  Softmax in fp32 of scores scaled by softmax_scale, probabilities rounded to `dtype` before P V as in mi_attn_fwd; a row
  * without keys yields zeros, and so does one whose keys all score -inf (mi_attn_fwd's choice too; the quotient would be 0 / 0).  q, o (which share no memory) [total_q, n_q_heads, head_dim] by element strides; query head h reads KV head h / (n_q_heads / n_kv_heads).  Rows of o
@@ -428,6 +461,26 @@ typedef struct mi_paged_attn_args {
 int64_t mi_paged_attn_tickets(int32_t n_kv_heads);
 size_t mi_paged_attn_workspace_bytes(int64_t tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim);
 int mi_paged_attn(const mi_paged_attn_args* args);
+
+/* Attention of the new tokens of sequences that share a prefix in groups (several answers to one prompt; the reference computes each by itself): sequences
+ * group_seqs[g] .. group_seqs[g + 1] - 1 (neighbours, any number, none included) all see the keys 0 .. prefix_len[g] - 1 of pages prefix_table[g], in the same pool as theirs, in
+ * front of their own, which are those of mi_paged_attn: attn.page_table, ctx_len and causal are about own keys alone.  Sequences outside all groups
+ * have no prefix.  A group's keys are read once for its new tokens together, not once a sequence.  Softmax over both parts; a row without any key yields zeros.
+ * prefix_table [n_groups, max_prefix_pages] by stride; group_seqs [n_groups + 1] ascending; lengths, pages and sizes as above.
+ * attn.max_q_len is about sequences, not groups; attn.tickets are not looked at.
+ * workspace: mi_paged_prefix_attn_workspace_bytes() bytes for so many tokens, sequences and groups or more, 16-byte aligned, one call at a time; nothing in it has to be
+ * cleared.
+ * Algorithmic work: 4 * head_dim * n_q_heads * pairs flop; HBM bytes 2 * (sum prefix_len + sum ctx_len) * n_kv_heads * head_dim * e + 2 * total_q * n_q_heads * head_dim * e. */
+typedef struct mi_paged_prefix_attn_args {
+    mi_paged_attn_args attn;
+    const int32_t* prefix_table;
+    const int32_t* prefix_len;     /* [n_groups] */
+    const int32_t* group_seqs;     /* [n_groups + 1] */
+    int64_t prefix_table_stride;
+    int32_t n_groups, max_prefix_pages;
+} mi_paged_prefix_attn_args;
+size_t mi_paged_prefix_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim);
+int mi_paged_prefix_attn(const mi_paged_prefix_attn_args* args);
 
 /* ------------------------------------------------------------------------------------------
  * Attention core.  Replaces core/nn/attention/attention.py:108-213 (multi_head_attention) with

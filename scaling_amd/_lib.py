@@ -28,7 +28,8 @@ EXPORTS = (
     "mi_attn_fwd", "mi_attn_bwd_workspace_bytes", "mi_attn_bwd_workspace_bytes_kv", "mi_attn_bwd_workspace_bytes_for", "mi_attn_bwd",
     "mi_gemm", "mi_gemm_workspace_bytes", "mi_gemm_with_workspace", "mi_rows_product", "mi_transpose16", "mi_column_sum", "mi_add_rmsnorm_bwd", "mi_add_layernorm_fwd", "mi_add_layernorm_bwd", "mi_attn_decode_workspace_bytes", "mi_attn_decode", "mi_attn_decode_with_tickets", "mi_fill_cache", "mi_attn_decode_static_scratch_bytes", "mi_attn_decode_static",
     "mi_norm_rotary_fwd", "mi_norm_rotary_bwd_workspace_bytes", "mi_norm_rotary_bwd", "mi_paged_append",
-    "mi_paged_attn_workspace_bytes", "mi_paged_attn_tickets", "mi_paged_attn", "mi_sample",
+    "mi_paged_attn_workspace_bytes", "mi_paged_attn_tickets", "mi_paged_attn", "mi_sample", "mi_paged_step",
+    "mi_paged_prefix_attn_workspace_bytes", "mi_paged_prefix_attn",
 )
 
 
@@ -149,11 +150,27 @@ class MiPagedAttnArgs(Structure):
     ]
 
 
+class MiPagedPrefixAttnArgs(Structure):
+    _fields_ = [
+        ("attn", MiPagedAttnArgs), ("prefix_table", c_void_p), ("prefix_len", c_void_p), ("group_seqs", c_void_p), ("prefix_table_stride", c_int64),
+        ("n_groups", c_int32), ("max_prefix_pages", c_int32),
+    ]
+
+
 class MiSampleArgs(Structure):
     _fields_ = [
         ("logits", c_void_p), ("n_rows", c_int64), ("vocab", c_int64), ("row_stride", c_int64), ("uniforms", c_void_p), ("temperatures", c_void_p),
         ("top_ks", c_void_p), ("top_ps", c_void_p), ("min_ps", c_void_p), ("temperature", c_float), ("top_k", c_int32), ("top_p", c_float), ("min_p", c_float),
         ("ids", c_void_p), ("logprobs", c_void_p), ("dtype", c_int32), ("stream", c_void_p),
+    ]
+
+
+class MiPagedStepArgs(Structure):
+    _fields_ = [
+        ("new_tokens", c_void_p), ("lengths", c_void_p), ("state", c_void_p), ("position_offset", c_void_p), ("ctx_len", c_void_p), ("state_out", c_void_p),
+        ("page_table", c_void_p), ("free_pages", c_void_p), ("cu_seqlens", c_void_p), ("position_ids", c_void_p), ("slots", c_void_p), ("sequences", c_void_p),
+        ("last", c_void_p), ("page_table_stride", c_int64), ("batch", c_int32), ("max_pages", c_int32), ("page_size", c_int32), ("n_free", c_int32),
+        ("tokens", c_int32), ("max_ctx", c_int32), ("stream", c_void_p),
     ]
 
 
@@ -252,6 +269,12 @@ def _declare(lib):
     lib.mi_paged_attn_tickets.argtypes = [c_int32]
     lib.mi_paged_attn.restype = c_int
     lib.mi_paged_attn.argtypes = [POINTER(MiPagedAttnArgs)]
+    lib.mi_paged_prefix_attn_workspace_bytes.restype = c_size_t
+    lib.mi_paged_prefix_attn_workspace_bytes.argtypes = [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32]
+    lib.mi_paged_prefix_attn.restype = c_int
+    lib.mi_paged_prefix_attn.argtypes = [POINTER(MiPagedPrefixAttnArgs)]
+    lib.mi_paged_step.restype = c_int
+    lib.mi_paged_step.argtypes = [POINTER(MiPagedStepArgs)]
     lib.mi_sample.restype = c_int
     lib.mi_sample.argtypes = [POINTER(MiSampleArgs)]
     lib.mi_attn_fwd.restype = c_int

@@ -15,6 +15,8 @@ int mi_attn_decode_impl_bf16(const mi_decode_args* a, bool static_ws, int32_t* t
 int mi_attn_decode_impl_f16(const mi_decode_args* a, bool static_ws, int32_t* tickets, int64_t n_tickets);
 int mi_paged_attn_impl_bf16(const mi_paged_attn_args* a);
 int mi_paged_attn_impl_f16(const mi_paged_attn_args* a);
+int mi_paged_prefix_attn_impl_bf16(const mi_paged_prefix_attn_args* a);
+int mi_paged_prefix_attn_impl_f16(const mi_paged_prefix_attn_args* a);
 
 extern "C" int mi_attn_fwd(const mi_attn_args* a) {
     if (!a) return mi_fail(MI_E_NULL, "attn_fwd: args is null");
@@ -56,6 +58,14 @@ extern "C" int mi_paged_attn(const mi_paged_attn_args* a) {
     if (a->dtype != MI_BF16 && a->dtype != MI_F16) return mi_fail(MI_E_DTYPE, "paged_attn: the caches hold bf16 or f16 elements (dtype code %d)", a->dtype);
     if (a->total_q == 0) return MI_OK;                     // no tokens (an empty tensor may come with a null pointer)
     return a->dtype == MI_F16 ? mi_paged_attn_impl_f16(a) : mi_paged_attn_impl_bf16(a);
+}
+
+extern "C" int mi_paged_prefix_attn(const mi_paged_prefix_attn_args* a) {
+    if (!a) return mi_fail(MI_E_NULL, "paged_prefix_attn: args is null");
+    if (a->attn.dtype != MI_BF16 && a->attn.dtype != MI_F16)
+        return mi_fail(MI_E_DTYPE, "paged_prefix_attn: the caches hold bf16 or f16 elements (dtype code %d)", a->attn.dtype);
+    if (a->attn.total_q == 0) return MI_OK;
+    return a->attn.dtype == MI_F16 ? mi_paged_prefix_attn_impl_f16(a) : mi_paged_prefix_attn_impl_bf16(a);
 }
 
 // ---- scratch of the entry point that allocates nothing -----------------------------------------------------------

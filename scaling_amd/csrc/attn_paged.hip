@@ -28,7 +28,8 @@ constexpr int kRowsAloneKeys = 512;
 constexpr int kRowChunk = 32;        // keys per wavefront and step of paged_rows
 constexpr int kRowWaves = 4;
 constexpr int kRowTile = kRowChunk * kRowWaves;
-constexpr int kTileRows = 256;
+constexpr int kTileRows = 256, kTileShift = 8;
+static_assert(kRowBlock == 16 && kTileRows == 1 << kTileShift);
 constexpr int kMergeMost = 4;        // workgroups of paged_merge with 16 rows each per compute unit, more than which take 32 each
 constexpr int kTileKeys = 64;
 constexpr float kRescaleGap = 8.0f;  // log2 units by which a row's maximum may lag before its output is rescaled
@@ -47,23 +48,23 @@ struct PagedParams {
     float *rows_o, *rows_ml, *tiles_o, *tiles_ml;     // partial results: [partial][KV head][row of the block][feature], and (maximum in log2 units, sum)
 };
 
+// Sequences in groups that share a prefix.  The kernels compute `batch + n_groups` entries: every sequence over its own keys, and every group's new tokens together over
+// the keys of its prefix, which are so read once per block of rows of the whole group and not once a sequence.  All results are partial; paged_prefix_merge joins those
+// of a row.
+struct PrefixParams : PagedParams {
+    const int32_t *prefix_table, *prefix_len, *groups;
+    int64_t prefix_stride;
+    int n_groups, prefix_capacity, row_block;
+    int4* places;                                         // of every token its sequence's partial results, and behind these its group's: see Place
+};
+template <class P> constexpr bool kPrefix = std::is_same_v<P, PrefixParams>;
+
 __device__ __forceinline__ f32x4v mfma_16x16x32(elem8_t a, elem8_t b, f32x4v c) {
 #ifdef MI_ELEM_F16
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 #else
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 #endif
-}
-
-// sums over lanes 0 .. this one
-__device__ __forceinline__ int prefix_sum(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);      // row_shr 1, 2, 4, 8, then the last lanes of the rows in front
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-    return v;
 }
 
 // The sequences of paged_find, lane by lane of a wavefront.  (Chunks that are not split, prompts of 2048 tokens, us by sequence and longest block first: 4, 16 heads
@@ -95,6 +96,38 @@ template <int BLOCK, int TILE> struct Wavefront {
 template <int BLOCK, int TILE, PagedOrder ORDER> __device__ __forceinline__ PagedFound find_work(const PagedParams& p, const PagedPlan& plan, uint32_t share_m, int wanted) {
     Wavefront<BLOCK, TILE> lanes{p, plan, {}, {}};
     return paged_find<BLOCK, TILE, ORDER>(lanes, plan, share_m, p.batch, p.n_rep, p.causal, wanted);
+}
+// The same of sequences and, behind them, groups.
+template <int BLOCK, int TILE> struct PrefixWavefront : Wavefront<BLOCK, TILE> {
+    const PrefixParams& x;
+    __device__ __forceinline__ PrefixWavefront(const PrefixParams& p, const PagedPlan& plan) : Wavefront<BLOCK, TILE>{p, plan, {}, {}}, x(p) {}
+    __device__ __forceinline__ void look(int base) {
+        const int e = base + (int)(threadIdx.x & 63), i = min(e, x.batch + x.n_groups - 1), g = i - x.batch;
+        const bool group = g >= 0;
+        const int first = group ? paged_clamp(x.groups[g], 0, x.batch) : i, end = group ? paged_clamp(x.groups[g + 1], first, x.batch) : i + 1;
+        this->s = paged_seq(x.cu[first], x.cu[end], group ? x.prefix_len[g] : x.ctx[i], x.total, group ? x.prefix_capacity : x.capacity);
+        this->w = paged_work<BLOCK, TILE>(this->plan, this->s, x.n_rep);
+        if (e >= x.batch + x.n_groups) this->w.blocks = this->s.n = 0;
+    }
+};
+template <int BLOCK, int TILE, PagedOrder ORDER> __device__ __forceinline__ PagedFound find_work(const PrefixParams& p, const PagedPlan& plan, uint32_t share_m, int wanted) {
+    PrefixWavefront<BLOCK, TILE> lanes(p, plan);
+    return paged_find<BLOCK, TILE, kAllKept>(lanes, plan, share_m, p.batch + p.n_groups, p.n_rep, p.causal, wanted);
+}
+__device__ __forceinline__ const int32_t* table_of(const PagedParams& p, int b) { return p.table + (int64_t)b * p.table_stride; }
+__device__ __forceinline__ const int32_t* table_of(const PrefixParams& p, int e) {
+    return e < p.batch ? p.table + (int64_t)e * p.table_stride : p.prefix_table + (int64_t)(e - p.batch) * p.prefix_stride;
+}
+__device__ __forceinline__ bool causal_of(const PagedParams& p, int) { return p.causal; }
+__device__ __forceinline__ bool causal_of(const PrefixParams& p, int e) { return e < p.batch && p.causal; }
+// Where the partial results of an entry's tokens are, left for the merge by the workgroups of its first split and KV head: (first partial result, blocks,
+// splits * 2 + 1 if paged_tiles', first token).
+__device__ __forceinline__ void note_places(const PagedParams&, const PagedFound&, int, int, int, int, bool) {}
+__device__ __forceinline__ void note_places(const PrefixParams& p, const PagedFound& f, int kvh, int split, int row0, int n_rows, bool tiles) {
+    if (kvh != 0 || split != 0) return;
+    const int t0 = divide(row0, p.n_rep, p.rep_m), t1 = divide(row0 + n_rows - 1, p.n_rep, p.rep_m);
+    int4* to = p.places + (f.b < p.batch ? 0 : p.total) + f.seq.first;
+    for (int t = t0 + threadIdx.x; t <= t1; t += blockDim.x) to[t] = make_int4(f.partial, f.work.blocks, 2 * f.splits + tiles, f.seq.first);
 }
 
 // Page of the 16 keys from 16 * group on.  A number outside the cache is taken for the nearest inside.
@@ -268,8 +301,8 @@ __device__ __forceinline__ void own_keys_only(const PagedParams& p, const int32_
 // chunk's is in LDS, into the same registers: 16 KB a wavefront (d 128) are always under way, and 12 wavefronts fit a compute unit.  (Two sets of registers, a
 // whole chunk ahead: 8 wavefronts, 16 rows to a block at the most.)  Bound by memory: 32 x 8 items of 200 - 8192 keys of 128 features 83.8 - 85.6 us, 6.1 TB/s; few items
 // by the start and the merge besides, ~10 us: 8 x 8 items of 4096 keys 32.7, a single one of 1500 9.8 (6.5 and a second launch of 5.5 without the merge in it).
-template <int D, int NB>
-__global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_kernel(const PagedParams p) {
+template <int D, int NB, class P>
+__global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_kernel(const P p) {
     constexpr int NWV = kRowWaves, kThreads = 64 * NWV, BLOCK = 16 * NB;
     constexpr int KS = D / 32, DT = D / 16;
     constexpr int VSTR = 2 * D + 32;          // bytes per key row of a staged V chunk: transposed reads of 8 rows x 32 bytes hit 256 distinct bytes
@@ -289,6 +322,8 @@ __global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_ke
     int s0, s1;
     paged_split_keys<kRowTile>(f.seq, f.work, f.splits, split, s0, s1);
     const int n_rows = min(BLOCK, f.seq.n * p.n_rep - block * BLOCK);
+    const bool causal = causal_of(p, f.b);
+    note_places(p, f, kvh, split, block * BLOCK, n_rows, false);
 
     // this lane's rows, l16 and 16 further on
     uint4 raw[NB][KS];
@@ -296,7 +331,7 @@ __global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_ke
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
         const int r = 16 * nb + l16, row = block * BLOCK + min(r, n_rows - 1), token = divide(row, p.n_rep, p.rep_m), head = kvh * p.n_rep + row - token * p.n_rep;
-        limit[nb] = r < n_rows ? min(paged_limit(f.seq, token, p.causal), s1) : 0;
+        limit[nb] = r < n_rows ? min(paged_limit(f.seq, token, causal), s1) : 0;
         end = max(end, group_max<16>(limit[nb]));          // the same for the four groups of 16 lanes
         const elem_t* qr = p.q + (int64_t)(f.seq.first + token) * p.q_st + (int64_t)head * p.q_sh + 8 * G;
 #pragma unroll
@@ -315,7 +350,7 @@ __global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_ke
         l_i[nb] = 0.f;
     }
 
-    const int32_t* table = p.table + (int64_t)f.b * p.table_stride;
+    const int32_t* table = table_of(p, f.b);
     const elem_t *kbase = p.kp + (int64_t)kvh * p.p_sh, *vbase = p.vp + (int64_t)kvh * p.p_sh;
     char* vt = pool + wave * kRowChunk * VSTR;
     const char* vt_lane = vt + (4 * G + (l16 >> 2)) * VSTR + 8 * (l16 & 3);
@@ -464,7 +499,7 @@ __global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_ke
     }
     __syncthreads();
     const auto emit = [&](int r, int d, float M, float L, float O0, float O1) {
-        if (f.splits == 1) {
+        if (!kPrefix<P> && f.splits == 1) {
             const int rr = block * BLOCK + r, i = divide(rr, p.n_rep, p.rep_m);
             const float inv = L == 0.f ? 0.f : 1.f / L;
             *reinterpret_cast<uint32_t*>(p.o + (int64_t)(f.seq.first + i) * p.o_st + (int64_t)(kvh * p.n_rep + rr - i * p.n_rep) * p.o_sh + d) = pack_elem2(O0 * inv, O1 * inv);
@@ -509,7 +544,7 @@ __global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_ke
     // every wavefront has waited for its own before the barrier, so the count that thread 0 raises behind it comes after them in memory, and the loads of
     // the workgroup that reads the highest count come after all.  (Two launches, the second one merging, of 1500 keys of 32 / 8 heads: 11.5 us one call after the
     // other, one launch 9.6.)
-    if constexpr (NB > 1) return;
+    if constexpr (NB > 1 || kPrefix<P>) return;
     if (f.splits == 1 || p.tickets == nullptr) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -580,8 +615,8 @@ template <int D> struct PageDma {
 // Bound by the matrix pipe (busy half of the time) and the power that it draws: 4 x 2048 tokens behind 2048 - 14336 others, 32 / 8 heads of 128, 1055 - 1106 us by the card's clock, 1.05 - 1.10 PFLOP/s, as
 // mi_attn_fwd over contiguous keys; without its softmax 951, without its operand reads 890.  (Operands 2, 4, 8 products ahead instead of 3: 1104, 1076, 1093; the
 // first of them before the barrier: 1150.)
-template <int D>
-__global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p) {
+template <int D, class P>
+__global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const P p) {
     constexpr int NW = 8, BN = kTileKeys;
     constexpr int KS = D / 16, DT = D / 32, NS = 4;
     using Tile = LdsTile<D>;
@@ -603,7 +638,8 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
     // ---- this lane's row, its keys [s0, limit), its part of Q ----
     const int n_rows = f.seq.n * p.n_rep, row = block * kTileRows + wave * 32 + l32;
     const int rr = min(row, n_rows - 1), token = divide(rr, p.n_rep, p.rep_m), head = kvh * p.n_rep + rr - token * p.n_rep;
-    const int limit = row < n_rows ? min(paged_limit(f.seq, token, p.causal), s1) : 0;
+    const int limit = row < n_rows ? min(paged_limit(f.seq, token, causal_of(p, f.b)), s1) : 0;
+    note_places(p, f, kvh, split, block * kTileRows, min(kTileRows, n_rows - block * kTileRows), true);
     elem8_t qf[KS];
     {
         const elem_t* qrow = p.q + (int64_t)(f.seq.first + token) * p.q_st + (int64_t)head * p.q_sh + 8 * g;
@@ -630,7 +666,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
     // ---- direct loads: wavefronts 0 - 3 of V, 4 - 7 of K; wavefront lw of either of keys 16 lw .. + 15 of a tile ----
     const bool v_role = wave < 4;
     const int lw = wave & 3, grp = wave >> 2;
-    const int32_t* table = p.table + (int64_t)f.b * p.table_stride;
+    const int32_t* table = table_of(p, f.b);
     const elem_t* base = (v_role ? p.vp : p.kp) + (int64_t)kvh * p.p_sh;
     char* ring = v_role ? v_lds : k_lds;
     const int last = max(s1 - 1, 0), last_group = last >> 4;
@@ -778,7 +814,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
         redo = (redo | redo >> 32) & 0xffffffffu;
     }
     if (row < n_rows && (redo >> l32 & 1) == 0) {
-        if (f.splits == 1) {
+        if (!kPrefix<P> && f.splits == 1) {
             const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;
             elem_t* orow = p.o + (int64_t)(f.seq.first + token) * p.o_st + (int64_t)head * p.o_sh + 4 * g;
 #pragma unroll
@@ -802,7 +838,7 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const PagedParams p
         float M, L, O0, O1;
         own_keys_only<D>(p, table, kvh, p.q + (int64_t)(f.seq.first + t) * p.q_st + (int64_t)h * p.q_sh, s0, __builtin_amdgcn_readlane(limit, r), M, L, O0, O1);
         if (d >= D) continue;
-        if (f.splits == 1) {
+        if (!kPrefix<P> && f.splits == 1) {
             const float inv = L == 0.f ? 0.f : 1.f / L;
             *reinterpret_cast<uint32_t*>(p.o + (int64_t)(f.seq.first + t) * p.o_st + (int64_t)h * p.o_sh + d) = pack_elem2(O0 * inv, O1 * inv);
         } else {
@@ -842,15 +878,20 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const PagedParams p, i
     }
 }
 
-template <int D, int NB> int launch(const PagedParams& p, int64_t row_blocks, int64_t tile_blocks, hipStream_t st) {
+template <int D, int NB, class P> int launch_blocks(const P& p, int64_t row_blocks, int64_t tile_blocks, hipStream_t st) {
     if (row_blocks > 0) {
-        paged_rows_kernel<D, NB><<<dim3((unsigned)p.rows.max_slots * p.nkv), dim3(64 * kRowWaves), 0, st>>>(p);
+        paged_rows_kernel<D, NB, P><<<dim3((unsigned)p.rows.max_slots * p.nkv), dim3(64 * kRowWaves), 0, st>>>(p);
         if (const int rc = mi_check_launch("paged_rows"); rc != MI_OK) return rc;
     }
     if (tile_blocks > 0) {
-        paged_tiles_kernel<D><<<dim3((unsigned)p.tiles.max_slots * p.nkv), dim3(512), 0, st>>>(p);
+        paged_tiles_kernel<D, P><<<dim3((unsigned)p.tiles.max_slots * p.nkv), dim3(512), 0, st>>>(p);
         if (const int rc = mi_check_launch("paged_tiles"); rc != MI_OK) return rc;
     }
+    return MI_OK;
+}
+
+template <int D, int NB> int launch(const PagedParams& p, int64_t row_blocks, int64_t tile_blocks, hipStream_t st) {
+    if (const int rc = launch_blocks<D, NB>(p, row_blocks, tile_blocks, st); rc != MI_OK) return rc;
     const int64_t of_rows = p.rows.share > 0 && p.tickets == nullptr ? paged_max_split_blocks(p.rows, row_blocks) * p.nkv * NB : 0;
     const int64_t tile_groups = paged_max_split_blocks(p.tiles, tile_blocks) * p.nkv;
     const int per_group = tile_groups * p.tile_rows > 16 * kMergeMost * mi_compute_units() ? 32 : 16, per_block = (p.tile_rows + per_group - 1) / per_group;
@@ -858,6 +899,30 @@ template <int D, int NB> int launch(const PagedParams& p, int64_t row_blocks, in
     if (groups == 0) return MI_OK;
     paged_merge_kernel<D, NB><<<dim3((unsigned)groups), dim3(256), 0, st>>>(p, (int)of_rows, per_block, per_group);
     return mi_check_launch("paged_merge");
+}
+
+// Rows of sequences with a prefix: the partial results of their own keys and of their group's together, 16 lanes to a row of a KV head.
+template <int D>
+__global__ __launch_bounds__(256) void paged_prefix_merge_kernel(const PrefixParams p) {
+    const int row = blockIdx.x * 16 + (int)(threadIdx.x >> 4), kvh = blockIdx.y, token = divide(row, p.n_rep, p.rep_m), rep = row - token * p.n_rep;
+    if (token >= p.total || token < p.cu[0] || token >= p.cu[p.batch]) return;
+    const int g0 = paged_clamp(p.groups[0], 0, p.batch), g1 = paged_clamp(p.groups[p.n_groups], g0, p.batch);
+    const bool grouped = token >= p.cu[g0] && token < p.cu[g1];
+    RowSum<D> sum;
+    int4 place[2];
+    place[0] = p.places[token];
+    place[1] = grouped ? p.places[p.total + token] : make_int4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int partial = place[i].x, blocks = place[i].y, splits = place[i].z >> 1, in = (token - place[i].w) * p.n_rep + rep;
+        const bool tiles = (place[i].z & 1) != 0;
+        const int shift = tiles ? kTileShift : p.row_block == kRowBlock ? 4 : 5, kept = tiles ? p.tile_rows : p.row_block, block = in >> shift;
+        // (of lengths that overlap: sequences that were left out have nobody's places here)
+        if (splits < 1 || partial < 0 || in < 0 || block >= blocks || in - (block << shift) >= kept || (int64_t)partial + (int64_t)blocks * splits > (tiles ? p.tiles.max_partials : p.rows.max_partials)) continue;
+        const int64_t first = ((int64_t)(partial + block) * p.nkv + kvh) * kept + (in - (block << shift)), step = (int64_t)blocks * p.nkv * kept;
+        sum.template add<false, 8>(tiles ? p.tiles_o : p.rows_o, tiles ? p.tiles_ml : p.rows_ml, first, step, splits);
+    }
+    sum.store(p.o + (int64_t)token * p.o_st + (int64_t)(kvh * p.n_rep + rep) * p.o_sh);
 }
 
 // Workgroups per KV head that either kernel's work is cut for.  `items`: sequences x KV heads of the calls, as many as there may be.
@@ -919,22 +984,22 @@ extern "C" size_t mi_paged_attn_workspace_bytes(int64_t tokens, int32_t n_q_head
 }
 #endif
 
-int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
+// What both entries take, checked, and laid out for the kernels.
+static int paged_params(const mi_paged_attn_args* a, const char* name, PagedParams& p) {
     if (a->total_q < 0 || a->batch < 1 || a->n_pages < 1 || a->max_pages < 1 || a->page_size < 16 || a->page_size % 16 != 0 ||
         (int64_t)a->max_pages * a->page_size > (1 << 30) || a->max_q_len < 0 || a->total_q > 0x7fffffffLL)
-        return mi_fail(MI_E_SHAPE, "paged_attn: %lld tokens of %d sequences, at most %d each, %d pages of %d keys (a multiple of 16), up to %d a sequence", (long long)a->total_q,
+        return mi_fail(MI_E_SHAPE, "%s: %lld tokens of %d sequences, at most %d each, %d pages of %d keys (a multiple of 16), up to %d a sequence", name, (long long)a->total_q,
                        a->batch, a->max_q_len, a->n_pages, a->page_size, a->max_pages);
     if (a->n_q_heads <= 0 || a->n_kv_heads <= 0 || a->n_q_heads % a->n_kv_heads != 0)
-        return mi_fail(MI_E_SHAPE, "paged_attn: n_q_heads=%d must be a positive multiple of n_kv_heads=%d", a->n_q_heads, a->n_kv_heads);
+        return mi_fail(MI_E_SHAPE, "%s: n_q_heads=%d must be a positive multiple of n_kv_heads=%d", name, a->n_q_heads, a->n_kv_heads);
     if (a->head_dim != 32 && a->head_dim != 64 && a->head_dim != 96 && a->head_dim != 128)
-        return mi_fail(MI_E_SHAPE, "paged_attn: head_dim %d unsupported (32, 64, 96, 128)", a->head_dim);
-    if (!a->q || !a->k_pages || !a->v_pages || !a->o || !a->page_table || !a->cu_seqlens || !a->ctx_len) return mi_fail(MI_E_NULL, "paged_attn: null pointer");
-    if (a->softmax_scale <= 0.f || mi_is_nan(a->softmax_scale)) return mi_fail(MI_E_SHAPE, "paged_attn: softmax_scale must be positive");
-    if (!mi_aligned16(a->q) || !mi_aligned16(a->k_pages) || !mi_aligned16(a->v_pages) || !mi_aligned16(a->o)) return mi_fail(MI_E_ALIGN, "paged_attn: tensors must be 16-byte aligned");
+        return mi_fail(MI_E_SHAPE, "%s: head_dim %d unsupported (32, 64, 96, 128)", name, a->head_dim);
+    if (!a->q || !a->k_pages || !a->v_pages || !a->o || !a->page_table || !a->cu_seqlens || !a->ctx_len) return mi_fail(MI_E_NULL, "%s: null pointer", name);
+    if (a->softmax_scale <= 0.f || mi_is_nan(a->softmax_scale)) return mi_fail(MI_E_SHAPE, "%s: softmax_scale must be positive", name);
+    if (!mi_aligned16(a->q) || !mi_aligned16(a->k_pages) || !mi_aligned16(a->v_pages) || !mi_aligned16(a->o)) return mi_fail(MI_E_ALIGN, "%s: tensors must be 16-byte aligned", name);
     for (const int64_t s : {a->q_stride_token, a->q_stride_head, a->o_stride_token, a->o_stride_head, a->page_stride, a->page_stride_token, a->page_stride_head})
-        if (s % 8 != 0) return mi_fail(MI_E_ALIGN, "paged_attn: strides must be multiples of 8 elements");
-    if (a->page_stride_token < 0 || a->page_stride_token > (1 << 26)) return mi_fail(MI_E_SHAPE, "paged_attn: a token stride of %lld elements", (long long)a->page_stride_token);
-    PagedParams p{};
+        if (s % 8 != 0) return mi_fail(MI_E_ALIGN, "%s: strides must be multiples of 8 elements", name);
+    if (a->page_stride_token < 0 || a->page_stride_token > (1 << 26)) return mi_fail(MI_E_SHAPE, "%s: a token stride of %lld elements", name, (long long)a->page_stride_token);
     p.q = (const elem_t*)a->q; p.kp = (const elem_t*)a->k_pages; p.vp = (const elem_t*)a->v_pages; p.o = (elem_t*)a->o;
     p.table = a->page_table; p.cu = a->cu_seqlens; p.ctx = a->ctx_len; p.table_stride = a->page_table_stride;
     p.q_st = a->q_stride_token; p.q_sh = a->q_stride_head; p.o_st = a->o_stride_token; p.o_sh = a->o_stride_head;
@@ -943,6 +1008,12 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
     p.capacity = a->max_pages * a->page_size; p.nq = a->n_q_heads; p.nkv = a->n_kv_heads; p.n_rep = a->n_q_heads / a->n_kv_heads; p.causal = a->causal != 0;
     p.page_m = divide_m(p.page); p.rep_m = divide_m(p.n_rep); p.nkv_m = divide_m(p.nkv);
     p.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+    return MI_OK;
+}
+
+int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
+    PagedParams p{};
+    if (const int rc = paged_params(a, "paged_attn", p); rc != MI_OK) return rc;
     const int64_t longest = a->max_q_len > 0 && a->max_q_len < p.total ? a->max_q_len : p.total;
     const Plans plans = make_plans(p.total, p.batch, std::min<int64_t>(p.batch, p.total) * p.nkv, longest, p.capacity, p.n_rep, p.nkv);
     p.rows = plans.rows;
@@ -984,6 +1055,95 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
     const auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
         return two ? launch<D, 2>(p, row_blocks, tile_blocks, st) : launch<D, 1>(p, row_blocks, tile_blocks, st);
+    };
+    switch (a->head_dim) {
+        case 32: return go(std::integral_constant<int, 32>{});
+        case 64: return go(std::integral_constant<int, 64>{});
+        case 96: return go(std::integral_constant<int, 96>{});
+        default: return go(std::integral_constant<int, 128>{});
+    }
+}
+
+// ---- sequences with a shared prefix -------------------------------------------------------------------------------------------------------------------
+namespace {
+
+// The plans of a call, and upper bounds of its blocks.  Of `tokens` new tokens, up to `longest` to a sequence.
+struct PrefixPlans {
+    Plans plans;
+    int64_t row_blocks, tile_blocks;
+};
+PrefixPlans prefix_plans(int64_t tokens, int64_t batch, int64_t groups, int64_t longest, int n_rep, int nkv) {
+    PrefixPlans o;
+    o.plans = make_plans(tokens, batch, std::min(batch, tokens) * nkv, longest, 1 << 30, n_rep, nkv);
+    PagedPlan &rows = o.plans.rows, &tiles = o.plans.tiles;
+    rows.rows_up_to = tiles.rows_over = o.plans.row_block;                 // an entry of more rows than a block is paged_tiles'
+    rows.max_n = tiles.max_n = 0x7fffffff;
+    o.plans.tile_rows = (int)std::min<int64_t>((tokens * n_rep + 15) / 16 * 16, kTileRows);
+    if (tiles.share > 0) tiles.share = tiles.fit;
+    o.row_blocks = std::min(batch, tokens) + std::min(groups, tokens);     // one of each entry with tokens
+    o.tile_blocks = paged_max_blocks<kTileRows>(tiles, tokens, batch, longest, n_rep) + paged_max_blocks<kTileRows>(tiles, tokens, groups, tokens, n_rep);
+    return o;
+}
+size_t prefix_bytes(int64_t tokens, int64_t row_partials, int row_block, int64_t tile_partials, int tile_rows, int nkv, int head_dim) {
+    return 2 * (size_t)tokens * sizeof(int4) + partial_bytes(row_partials, nkv, row_block, head_dim) + partial_bytes(tile_partials, nkv, tile_rows, head_dim);
+}
+
+}  // namespace
+
+#ifndef MI_ELEM_F16
+// For every max_q_len: entries with a block of rows each, blocks of 256 of those with more than 16, and the splits that either share adds.
+extern "C" size_t mi_paged_prefix_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
+    if (tokens <= 0 || tokens > 0x7fffffffLL || batch < 1 || n_groups < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || head_dim <= 0) return 0;
+    const int64_t rows = tokens * (n_q_heads / n_kv_heads), cus = mi_compute_units(), many = rows / (kRowBlock + 1);
+    const int64_t row_partials = std::min<int64_t>(batch, tokens) + std::min<int64_t>(n_groups, tokens) + share_of(kRowsMost * cus, n_kv_heads) + 1;
+    const int64_t tile_partials = std::min<int64_t>(batch, many) + std::min<int64_t>(n_groups, many) + 2 * (rows / kTileRows) + share_of(cus, n_kv_heads) + 1;
+    return prefix_bytes(tokens, row_partials, 2 * kRowBlock, many > 0 ? tile_partials : 0, (int)std::min<int64_t>((rows + 15) / 16 * 16, kTileRows), n_kv_heads, head_dim);
+}
+#endif
+
+int MI_ENTRY(mi_paged_prefix_attn_impl)(const mi_paged_prefix_attn_args* x) {
+    const mi_paged_attn_args* a = &x->attn;
+    PrefixParams p{};
+    if (const int rc = paged_params(a, "paged_prefix_attn", p); rc != MI_OK) return rc;
+    if (x->n_groups < 0 || x->max_prefix_pages < 1 || (int64_t)x->max_prefix_pages * a->page_size > (1 << 30) || p.nkv > 0xffff)
+        return mi_fail(MI_E_SHAPE, "paged_prefix_attn: %d groups with prefixes of up to %d pages, %d KV heads", x->n_groups, x->max_prefix_pages, p.nkv);
+    if (!x->prefix_table || !x->prefix_len || !x->group_seqs) return mi_fail(MI_E_NULL, "paged_prefix_attn: null pointer");
+    p.prefix_table = x->prefix_table; p.prefix_len = x->prefix_len; p.groups = x->group_seqs; p.prefix_stride = x->prefix_table_stride;
+    p.n_groups = x->n_groups; p.prefix_capacity = x->max_prefix_pages * a->page_size;
+    const int64_t longest = a->max_q_len > 0 && a->max_q_len < p.total ? a->max_q_len : p.total;
+    if ((int64_t)p.total * p.n_rep > 0x7fffffffLL - kTileRows || (int64_t)p.batch + p.n_groups > 0x7fffff00LL)
+        return mi_fail(MI_E_SHAPE, "paged_prefix_attn: %d tokens of %d heads, %d sequences", p.total, p.nq, p.batch);
+    const PrefixPlans o = prefix_plans(p.total, p.batch, p.n_groups, longest, p.n_rep, p.nkv);
+    p.rows = o.plans.rows;
+    p.tiles = o.plans.tiles;
+    p.tile_rows = o.plans.tile_rows;
+    p.row_block = o.plans.row_block;
+    const int64_t keys = std::max(p.capacity, p.prefix_capacity), row_tiles = (keys + kRowTile - 1) / kRowTile, tile_tiles = (keys + kTileKeys - 1) / kTileKeys;
+    if (o.row_blocks * row_tiles > 0x7fffffffLL || o.tile_blocks * tile_tiles > 0x7fffffffLL ||
+        (o.row_blocks + o.tile_blocks + 10LL * mi_compute_units()) * p.nkv > 0x7fffffffLL)
+        return mi_fail(MI_E_SHAPE, "paged_prefix_attn: %lld tokens of %d heads over up to %lld keys are too many for one call", (long long)a->total_q, a->n_q_heads, (long long)keys);
+    if (row_tiles <= p.rows.least || o.row_blocks == 0) p.rows.share = 0;
+    if (tile_tiles <= p.tiles.least || o.tile_blocks == 0) p.tiles.share = 0;
+    p.share_m[0] = divide_m(p.rows.share); p.share_m[1] = divide_m(p.tiles.share);
+    p.rows.max_slots = (int)paged_max_slots(p.rows, o.row_blocks, row_tiles);
+    p.tiles.max_slots = (int)paged_max_slots(p.tiles, o.tile_blocks, tile_tiles);
+    p.rows.max_partials = p.rows.max_slots;                // every split of an entry has partial results
+    p.tiles.max_partials = p.tiles.max_slots;
+    const size_t need = prefix_bytes(p.total, p.rows.max_partials, p.row_block, p.tiles.max_partials, p.tile_rows, p.nkv, a->head_dim);
+    if (!a->workspace || a->workspace_bytes < need || !mi_aligned16(a->workspace))
+        return mi_fail(MI_E_WORKSPACE, "paged_prefix_attn: workspace needs %zu bytes (16-byte aligned), got %zu", need, a->workspace_bytes);
+    p.places = (int4*)a->workspace;
+    p.rows_o = (float*)(p.places + 2 * (size_t)p.total);
+    p.rows_ml = p.rows_o + (size_t)p.rows.max_partials * p.nkv * p.row_block * a->head_dim;
+    p.tiles_o = p.rows_ml + (size_t)p.rows.max_partials * p.nkv * p.row_block * 2;
+    p.tiles_ml = p.tiles_o + (size_t)p.tiles.max_partials * p.nkv * p.tile_rows * a->head_dim;
+    const hipStream_t st = (hipStream_t)a->stream;
+    const auto go = [&](auto d) {
+        constexpr int D = decltype(d)::value;
+        const int rc = p.row_block == kRowBlock ? launch_blocks<D, 1>(p, o.row_blocks, o.tile_blocks, st) : launch_blocks<D, 2>(p, o.row_blocks, o.tile_blocks, st);
+        if (rc != MI_OK) return rc;
+        paged_prefix_merge_kernel<D><<<dim3((unsigned)((p.total * (int64_t)p.n_rep + 15) / 16), (unsigned)p.nkv), dim3(256), 0, st>>>(p);
+        return mi_check_launch("paged_prefix_merge");
     };
     switch (a->head_dim) {
         case 32: return go(std::integral_constant<int, 32>{});

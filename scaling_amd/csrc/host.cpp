@@ -602,6 +602,49 @@ OptTensor op_paged_append(const OptTensor& q_, const Tensor& k, const Tensor& v,
     return q.defined() ? OptTensor(q_out) : std::nullopt;
 }
 
+// (cu_seqlens, position_ids, slots, sequences, last) of the next step of a paged cache; takes its pages.
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> op_paged_step(const Tensor& new_tokens, const Tensor& lengths, const Tensor& table, const Tensor& free_pages,
+                                                                 const Tensor& state, int64_t page_size, int64_t tokens, int64_t max_ctx, const OptTensor& offset,
+                                                                 const Tensor& ctx_len, const Tensor& state_out) {
+    need_gpu(new_tokens);
+    const int64_t batch = new_tokens.size(0);
+    const auto ints = [&](const Tensor& t, int64_t n, const char* name) {
+        TORCH_CHECK(t.is_cuda() && t.device() == new_tokens.device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && (n < 0 || t.size(0) == n),
+                    "paged_step: ", name, " is a contiguous int32 tensor", n < 0 ? std::string() : " [" + std::to_string(n) + "]", " on the device of the others");
+        return static_cast<int32_t*>(ptr(t));
+    };
+    TORCH_CHECK(new_tokens.dim() == 1, "paged_step: new is [batch]");
+    mi_paged_step_args a{};
+    a.new_tokens = ints(new_tokens, batch, "new"); a.lengths = ints(lengths, batch, "lengths"); a.state = ints(state, 2, "state");
+    a.position_offset = offset.has_value() ? ints(*offset, batch, "position_offset") : nullptr;
+    a.ctx_len = ints(ctx_len, batch, "ctx_len"); a.state_out = ints(state_out, 2, "state_out"); a.free_pages = ints(free_pages, -1, "free_pages");
+    TORCH_CHECK(table.dim() == 2 && table.size(0) == batch && table.scalar_type() == at::kInt && table.device() == new_tokens.device() &&
+                    (table.stride(1) == 1 || table.size(1) <= 1) && (table.stride(0) >= table.size(1) || batch <= 1),
+                "paged_step: page_table is int32 [batch, max_pages] with contiguous rows of its own memory");
+    for (const int64_t n : {batch, table.size(1), page_size, free_pages.size(0), tokens, max_ctx}) TORCH_CHECK(n >= 0 && n <= INT32_MAX, "paged_step: a size of ", n);
+    // what is written besides lengths and state themselves has to be memory of its own
+    const Tensor* const read[] = {&new_tokens, &lengths, &state, offset.has_value() ? &*offset : &new_tokens};
+    const Tensor* const written[] = {&ctx_len, &state_out, &table, &free_pages};
+    for (const Tensor* w : written)
+        for (const Tensor* r : read) {
+            if ((w == &ctx_len && r == &lengths && ptr(*w) == ptr(*r)) || (w == &state_out && r == &state && ptr(*w) == ptr(*r))) continue;
+            at::assert_no_overlap(*w, *r);
+        }
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < i; ++j) at::assert_no_overlap(*written[i], *written[j]);
+    a.page_table = static_cast<int32_t*>(ptr(table)); a.page_table_stride = table.stride(0);
+    a.batch = (int32_t)batch; a.max_pages = (int32_t)table.size(1); a.page_size = (int32_t)page_size; a.n_free = (int32_t)free_pages.size(0);
+    a.tokens = (int32_t)tokens; a.max_ctx = (int32_t)max_ctx;
+    Launch l(new_tokens);
+    const auto longs = new_tokens.options().dtype(at::kLong);
+    const Tensor cu = at::empty({batch + 1}, new_tokens.options()), of_tokens = at::empty({3, tokens}, longs), last = at::empty({batch}, longs);
+    a.cu_seqlens = static_cast<int32_t*>(ptr(cu)); a.last = last.data_ptr<int64_t>();
+    a.position_ids = of_tokens.data_ptr<int64_t>(); a.slots = a.position_ids + tokens; a.sequences = a.slots + tokens;
+    a.stream = l.stream;
+    check(mi_paged_step(&a), "mi_paged_step");
+    return {cu, of_tokens[0], of_tokens[1], of_tokens[2], last};
+}
+
 // Whether two [tokens, heads, features] tensors of one shape with contiguous features share memory.  Slices of one tensor lie between each other's rows: of equal
 // strides the offset tells.  Others share where the memory that they span does.
 bool rows_meet(const Tensor& a, const Tensor& b) {
@@ -621,8 +664,9 @@ bool rows_meet(const Tensor& a, const Tensor& b) {
     return true;
 }
 
-Tensor op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu, const Tensor& ctx_len, bool causal,
-                          double scale, int64_t max_q_len, const OptTensor& workspace_, const OptTensor& tickets, const OptTensor& out_) {
+// Arguments of attention over pages, without workspace and stream; makes the output where none is given.
+std::pair<mi_paged_attn_args, Tensor> paged_attn_args(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu, const Tensor& ctx_len,
+                                                      bool causal, double scale, int64_t max_q_len, const OptTensor& out_) {
     need_gpu(q);
     check_head_rows(q, Tensor(), Tensor());
     const Tensor out = out_.has_value() ? *out_ : at::empty(q.sizes(), q.options());
@@ -632,7 +676,6 @@ Tensor op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& 
         at::assert_no_internal_overlap(out);
         TORCH_CHECK(!rows_meet(q, out), "paged_attention: out shares memory with q");     // rows of q are read again after others were written
     }
-    Launch l(q);
     TORCH_CHECK(k_pages.dim() == 4, "paged cache: k_pages and v_pages are [pages, page_size, n_kv, head_dim] tensors");
     const Pages pages = check_pages(q, k_pages.size(2), k_pages, v_pages, table, cu, ctx_len);
     mi_paged_attn_args a{};
@@ -644,6 +687,14 @@ Tensor op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& 
     a.batch = pages.batch; a.n_pages = pages.n_pages; a.page_size = pages.page_size; a.max_pages = pages.max_pages;
     a.n_q_heads = (int32_t)q.size(1); a.n_kv_heads = (int32_t)k_pages.size(2); a.head_dim = (int32_t)q.size(2); a.dtype = code_of(q);
     a.causal = causal; a.max_q_len = (int32_t)std::min<int64_t>(max_q_len, INT32_MAX); a.softmax_scale = (float)scale;
+    return {a, out};
+}
+
+Tensor op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu, const Tensor& ctx_len, bool causal,
+                          double scale, int64_t max_q_len, const OptTensor& workspace_, const OptTensor& tickets, const OptTensor& out_) {
+    need_gpu(q);
+    Launch l(q);
+    auto [a, out] = paged_attn_args(q, k_pages, v_pages, table, cu, ctx_len, causal, scale, max_q_len, out_);
     Tensor workspace = opt(workspace_);
     if (!workspace.defined()) workspace = float_buffer(mi_paged_attn_workspace_bytes(a.total_q, a.n_q_heads, a.n_kv_heads, a.head_dim), q);
     TORCH_CHECK(workspace.device() == q.device() && workspace.is_contiguous(), "paged_attention: the workspace is a contiguous tensor on the device of q");
@@ -655,6 +706,33 @@ Tensor op_paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& 
     }
     a.stream = l.stream;
     check(mi_paged_attn(&a), "mi_paged_attn");
+    return out;
+}
+
+// The same of sequences in groups with a prefix each.
+Tensor op_paged_prefix_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& cu, const Tensor& ctx_len,
+                                 const Tensor& prefix_table, const Tensor& prefix_len, const Tensor& group_seqs, bool causal, double scale, int64_t max_q_len,
+                                 const OptTensor& workspace_, const OptTensor& out_) {
+    need_gpu(q);
+    Launch l(q);
+    auto [attn, out] = paged_attn_args(q, k_pages, v_pages, table, cu, ctx_len, causal, scale, max_q_len, out_);
+    const auto ints = [&](const Tensor& t, int64_t dims) { return t.device() == q.device() && t.scalar_type() == at::kInt && t.dim() == dims; };
+    TORCH_CHECK(ints(prefix_table, 2) && (prefix_table.stride(1) == 1 || prefix_table.size(1) <= 1) && ints(prefix_len, 1) && prefix_len.is_contiguous() &&
+                    ints(group_seqs, 1) && group_seqs.is_contiguous() && prefix_table.size(0) == prefix_len.size(0) && group_seqs.size(0) == prefix_len.size(0) + 1,
+                "paged_prefix_attention: int32 prefix_table [groups, max_prefix_pages], prefix_len [groups] and group_seqs [groups + 1] on the device of q");
+    for (const int64_t n : {prefix_table.size(0), prefix_table.size(1)}) TORCH_CHECK(n >= 1 && n <= INT32_MAX, "paged_prefix_attention: a size of ", n);
+    mi_paged_prefix_attn_args a{};
+    a.attn = attn;
+    a.prefix_table = static_cast<const int32_t*>(ptr(prefix_table)); a.prefix_table_stride = prefix_table.stride(0);
+    a.prefix_len = static_cast<const int32_t*>(ptr(prefix_len)); a.group_seqs = static_cast<const int32_t*>(ptr(group_seqs));
+    a.n_groups = (int32_t)prefix_table.size(0); a.max_prefix_pages = (int32_t)prefix_table.size(1);
+    Tensor workspace = opt(workspace_);
+    if (!workspace.defined())
+        workspace = float_buffer(mi_paged_prefix_attn_workspace_bytes(attn.total_q, attn.batch, a.n_groups, attn.n_q_heads, attn.n_kv_heads, attn.head_dim), q);
+    TORCH_CHECK(workspace.device() == q.device() && workspace.is_contiguous(), "paged_prefix_attention: the workspace is a contiguous tensor on the device of q");
+    a.attn.workspace = ptr(workspace); a.attn.workspace_bytes = (size_t)workspace.numel() * workspace.element_size();
+    a.attn.stream = l.stream;
+    check(mi_paged_prefix_attn(&a), "mi_paged_prefix_attn");
     return out;
 }
 
@@ -2021,7 +2099,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     });
     def("norm_rotary", &op_norm_rotary);
     def("paged_append", &op_paged_append);
+    def("paged_step", &op_paged_step);
     def("paged_attention", &op_paged_attention);
+    def("paged_prefix_attention", &op_paged_prefix_attention);
     def("linear", &op_linear);
     def("projections", &op_projections);
     def("attention_forward", &op_attention_forward);

@@ -9,7 +9,7 @@ under saved-tensor hooks (activation checkpointing) and are deterministic under 
 
 import ctypes  # noqa: F401 - for callers that fill an argument block with _fill_attn_args and hand it to the C ABI
 import math
-from typing import Optional, Tuple, Union
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 from torch.overrides import _get_current_function_mode_stack, has_torch_function
@@ -22,7 +22,8 @@ __all__ = [
     "rms_norm", "swiglu", "rotary_embedding", "rotary_embedding_complex", "attention", "attention_forward", "attention_backward",
     "decode_attention", "rms_norm_forward", "rms_norm_backward", "swiglu_forward", "swiglu_backward",
     "cross_entropy", "cross_entropy_forward", "linear_cross_entropy", "weighted_cross_entropy", "add_rms_norm",
-    "norm_rotary", "paged_append", "paged_attention", "paged_workspace", "sample_rows",
+    "norm_rotary", "paged_append", "paged_attention", "paged_workspace", "sample_rows", "paged_step", "StepTensors", "paged_prefix_attention",
+    "paged_prefix_workspace",
 ]
 
 
@@ -248,6 +249,39 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_page
                                     float(eps), bool(layer_norm), bool(interleaved))
 
 
+class StepTensors(NamedTuple):
+    """What `paged_step` lays out, on the device: the rows of each sequence, and of each row its position, its slot (page * page_size + row in the page) and its sequence;
+    `last`: the row of each sequence's last new token (0 where it has none)."""
+    cu_seqlens: torch.Tensor
+    position_ids: torch.Tensor
+    slots: torch.Tensor
+    sequences: torch.Tensor
+    last: torch.Tensor
+
+
+def paged_step(new: torch.Tensor, lengths: torch.Tensor, page_table: torch.Tensor, free_pages: torch.Tensor, state: torch.Tensor, page_size: int, tokens: int,
+               max_ctx: Optional[int] = None, position_offset: Optional[torch.Tensor] = None, ctx_len: Optional[torch.Tensor] = None,
+               state_out: Optional[torch.Tensor] = None) -> StepTensors:
+    """The next step of a paged cache whose lengths lie on the device, without the host: takes pages for new[b] more tokens of sequence b and lays the tokens out, sequence after
+    sequence, as `paged_append` and `paged_attention` take them; capturable, and replayed on whatever new, lengths and state then hold.
+
+    new, lengths int32 [batch]: new tokens (0: none; negative: the sequence ends, its pages go back to be taken, its length is 0) and the keys before;
+    page_table int32 [batch, max_pages]; free_pages int32 [n]: a stack whose first state[0] entries are free pages, the next one to take last; state int32 [2]: that
+    count, and a status.  tokens: rows of the result; rows behind the last sequence are position 0, slot -1, sequence 0.  position_offset int32 [batch]: added to the
+    positions.  lengths and state are updated in place, or left alone and their successors written to ctx_len and state_out where these are given (then table and stack
+    hold the pages all the same, but nobody counts them yet).
+
+    Where the pages do not suffice (1), a sequence would have more than max_ctx keys (default: the table's room) (2) or there are more than `tokens` tokens (4), no sequence
+    takes or brings anything, and the number is set in state[1], which the caller reads when it suits and clears; pages given back are given back all the same."""
+    _need_cuda(new, lengths, page_table, free_pages, state, position_offset, ctx_len, state_out)
+    if page_size < 16 or page_size % 16 != 0:
+        raise ValueError(f"page_size {page_size} is no multiple of 16")
+    if max_ctx is not None and not 0 < max_ctx <= page_table.shape[1] * page_size:
+        raise ValueError(f"max_ctx {max_ctx} of a table with room for {page_table.shape[1] * page_size} keys")
+    return StepTensors(*_lib.host().paged_step(new, lengths, page_table, free_pages, state, int(page_size), int(tokens), max_ctx or 0, position_offset,
+                                               lengths if ctx_len is None else ctx_len, state if state_out is None else state_out))
+
+
 def paged_workspace(batch: int, tokens: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
     """Scratch of `paged_attention` for calls of up to `batch` sequences and `tokens` new tokens that do not overlap (calls on different streams, and graphs
     that may be replayed at the same time, need one each).  With it come the arrival counts (attribute `tickets`, int32, zero between calls) by which the
@@ -282,6 +316,32 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     return _lib.host().paged_attention(q, k_pages, v_pages, page_table, cu_seqlens, ctx_len, bool(causal),
                                        1.0 / math.sqrt(q.shape[2]) if softmax_scale is None else float(softmax_scale), max_q_len or 0, workspace,
                                        getattr(workspace, "tickets", None), out)
+
+
+def paged_prefix_workspace(batch: int, groups: int, tokens: int, n_q_heads: int, n_kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """Scratch of `paged_prefix_attention` for calls of up to `batch` sequences in `groups` groups with `tokens` new tokens that do not overlap (calls on different streams, and
+    graphs that may be replayed at the same time, need one each)."""
+    nbytes = _lib.load().mi_paged_prefix_attn_workspace_bytes(tokens, batch, groups, n_q_heads, n_kv_heads, head_dim)
+    return torch.empty(nbytes // 4, dtype=torch.float32, device=device)
+
+
+def paged_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor, ctx_len: torch.Tensor,
+                           prefix_table: torch.Tensor, prefix_len: torch.Tensor, group_seqs: torch.Tensor, causal: bool = True,
+                           softmax_scale: Optional[float] = None, max_q_len: Optional[int] = None, workspace: Optional[torch.Tensor] = None,
+                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """`paged_attention` of sequences that share a prefix in groups, as several answers to one prompt do (inference; no autograd): the keys of a prefix are read once
+    for all new tokens of its group.
+
+    Sequences group_seqs[g] .. group_seqs[g + 1] - 1 form group g (group_seqs int32 [groups + 1], ascending; sequences outside have no prefix).  All their new tokens see
+    the first prefix_len[g] (int32 [groups]) keys of the pages prefix_table[g] (int32 [groups, max_prefix_pages], in the same pool), and behind these the keys of
+    their own sequence as in `paged_attention`: page_table, ctx_len, causal and max_q_len are about own keys alone, so position p of an answer stands at
+    slot p - prefix_len of its sequence.  A row without any key is zeros; rows behind the last sequence are left as they are in `out` (of a new tensor: undefined).
+    workspace: see `paged_prefix_workspace`; without one it is allocated per call."""
+    _need_cuda(q, k_pages, v_pages, page_table, cu_seqlens, ctx_len, prefix_table, prefix_len, group_seqs, workspace, out)
+    if max_q_len is not None and max_q_len < 1 and q.shape[0] > 0:
+        raise ValueError("paged_prefix_attention: max_q_len must be positive")
+    return _lib.host().paged_prefix_attention(q, k_pages, v_pages, page_table, cu_seqlens, ctx_len, prefix_table, prefix_len, group_seqs, bool(causal),
+                                              1.0 / math.sqrt(q.shape[2]) if softmax_scale is None else float(softmax_scale), max_q_len or 0, workspace, out)
 
 
 # ------------------------------------------------------------------------------------------------
