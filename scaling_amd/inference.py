@@ -6,8 +6,9 @@ layer loop (core/nn/parallel_module/inference_module.py:100-109), prefill + one-
 decoding with greedy sampling (transformer/inference/inference_model.py:223-263, inference/sample.py:5-6)
 and the per-layer checkpoint files `model_state_layer_{i}_{Class}.pt`
 (core/nn/parallel_module/partitioned_module.py:246-408).  Unlike the reference the cached path accepts
-a batch of prompts of equal length (the reference asserts batch size 1, attention.py:855-857), and
-`generate_ragged` one of different lengths over a paged cache.
+a batch of prompts of equal length (the reference asserts batch size 1, attention.py:855-857),
+`generate_ragged` one of different lengths over a paged cache, and `generate_samples` draws several answers to each of
+such prompts, whose keys all of them share.
 Embedding lookup, LM head matmul and arg-max stay on PyTorch-ROCm.
 """
 
@@ -24,7 +25,7 @@ from .data import get_cumulative_seq_lengths, get_position_ids
 from . import ops
 from .layer import InferenceSettings, LayerNormWrapper, TransformerLayer, TransformerLayerIO
 from .loss import TransformerLMHead
-from .nn import PagedKVCache, PagedStep, RMSNorm, _unhooked, decode_arguments
+from .nn import BranchStep, PagedBranches, PagedKVCache, PagedStep, RMSNorm, _unhooked, decode_arguments
 
 # class names written by older versions of the reference (partitioned_module.py:25-32)
 LEGACY_CLASS_NAMES = {"LuminousEmbeddingInput": "EmbeddingInput", "LuminousLayer": "TransformerLayer",
@@ -342,9 +343,9 @@ class TransformerInferenceModule(torch.nn.Module):
                             att.hidden_size_per_attention_head, att.dtype, self.device, page_size)
 
     @torch.no_grad()
-    def paged_forward(self, token_ids: torch.Tensor, cache: PagedKVCache, step: PagedStep) -> torch.Tensor:
+    def paged_forward(self, token_ids: torch.Tensor, cache: PagedKVCache, step: Union[PagedStep, BranchStep]) -> torch.Tensor:
         """token_ids [tokens]: the new tokens of `step`, sequence after sequence -> logits [n, vocab] behind the last new token of each of the n sequences
-        that have any."""
+        that have any; of a step of branches, of every branch (of one without new tokens: some row's)."""
         h = self._layers[0](token_ids.to(self.device).view(1, -1))
         for layer in self._layers[1:-2]:
             h = layer.paged_step(h, cache, step)
@@ -391,3 +392,83 @@ class TransformerInferenceModule(torch.nn.Module):
             going = set(active)
             logits = self.paged_forward(tokens, cache, cache.step([int(b in going) for b in range(len(prompts))]))
         return completions if stop else torch.stack(kept, dim=1).tolist()
+
+    @torch.no_grad()
+    def generate_samples(self, max_tokens: int, prompts: Sequence[Sequence[int]], samples: int, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                         min_p: float = 0.0, uniforms: Optional[torch.Tensor] = None, generator: Optional[torch.Generator] = None,
+                         stop_tokens: Optional[Sequence[int]] = None, page_size: int = 64, graph: bool = True) -> Tuple[List[List[List[int]]], List[List[List[float]]]]:
+        """`samples` answers to each of some prompts of different lengths, drawn by ops.sample_rows (which describes the parameters): (token ids, their log-probabilities),
+        [prompt][sample][up to max_tokens], up to and with the first id in `stop_tokens`.
+
+        A prompt is computed once and its keys are read once a step for all of its answers.  The loop runs on the device: tokens are drawn there, steps planned there, answers that have
+        ended give their pages back and take no more rows there; with `graph` a step is captured once and replayed.  uniforms float32 [max_tokens, prompts *
+        samples] (answer j of prompt i: column i * samples + j): the numbers to draw by; without it `generator`'s, on the module's device.  The same numbers give the
+        same answers as long as the logits have the same bits, which also depend on the batch."""
+        prompts = [[int(t) for t in p] for p in prompts]
+        if max_tokens < 1 or samples < 1 or not prompts or not all(prompts):
+            raise ValueError("at least one prompt, no empty one, and at least one answer of one token to generate")
+        total, dev = samples * len(prompts), self.device
+        if uniforms is None:
+            uniforms = torch.rand(max_tokens, total, device=dev, generator=generator)
+        elif uniforms.shape != (max_tokens, total) or uniforms.dtype != torch.float32:
+            raise ValueError(f"uniforms are float32 [{max_tokens}, {total}], got {uniforms.dtype} {list(uniforms.shape)}")
+        uniforms = uniforms.to(dev)
+        longest = max(len(p) for p in prompts) + max_tokens - 1
+        rotary = self._layers[1].self_attention.rotary_embedding
+        if rotary is not None and longest > rotary.max_seq_length:
+            raise IndexError(f"position {longest - 1} is outside the rotary table of {rotary.max_seq_length} rows")
+        own = max(max_tokens - 1, 1)
+        of_branches = total * -(-own // page_size)
+        cache = self.paged_cache(len(prompts), max(len(p) for p in prompts), sum(-(-len(p) // page_size) for p in prompts) + of_branches, page_size)
+        logits = self.paged_forward(torch.tensor([t for p in prompts for t in p]), cache, cache.step([len(p) for p in prompts]))
+        branches = PagedBranches(cache, range(len(prompts)), samples, own, of_branches)
+        stop = None if not stop_tokens else torch.tensor(sorted(set(stop_tokens)), dtype=torch.int64, device=dev)
+        ids = torch.full((max_tokens, total), -1, dtype=torch.int64, device=dev)
+        logprobs = torch.zeros(max_tokens, total, device=dev)
+        new = torch.ones(total, dtype=torch.int32, device=dev)              # 1: goes on, -1: ends in this step, 0: has ended
+        tokens = torch.zeros(total, dtype=torch.int64, device=dev)
+        at = torch.zeros(1, dtype=torch.int64, device=dev)                  # the step that is drawn next
+
+        def draw(logits: torch.Tensor) -> None:
+            drawn, logprob = ops.sample_rows(logits, uniforms.index_select(0, at)[0], temperature, top_k, top_p, min_p, return_logprobs=True)
+            going = new > 0
+            ids.index_copy_(0, at, torch.where(going, drawn, -1).unsqueeze(0))
+            logprobs.index_copy_(0, at, logprob.unsqueeze(0))
+            tokens.copy_(drawn)
+            if stop is not None:
+                ends = (drawn.unsqueeze(1) == stop).any(dim=1)
+                new.copy_(torch.where(going, torch.where(ends, -1, 1), 0))
+            at.add_(1)
+
+        def step() -> None:
+            plan = branches.step(new, total, 1)
+            draw(self.paged_forward(tokens.index_select(0, plan.sequences), cache, plan))
+
+        draw(logits.repeat_interleave(samples, dim=0))
+        steps = max_tokens - 1
+        eager = steps if not graph else min(2, steps)                       # the first ones warm the libraries up
+        captured = None
+        if steps > eager:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                for _ in range(eager):
+                    step()
+            torch.cuda.current_stream().wait_stream(side)
+            captured = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(captured):
+                step()
+        for k in range(0 if captured is None else eager, steps):
+            if stop is not None and k % 16 == 15 and not bool((new > 0).any()):
+                break                                                       # all have ended, which is looked at now and then
+            if captured is None:
+                step()
+            else:
+                captured.replay()
+        branches.check()
+        branches.close()
+        ids, logprobs = ids.t().tolist(), logprobs.t().tolist()
+        lengths = [next((i for i, t in enumerate(row) if t < 0), max_tokens) for row in ids]
+        each = [(row[:n], lp[:n]) for row, lp, n in zip(ids, logprobs, lengths)]
+        of = lambda part: [[each[i * samples + j][part] for j in range(samples)] for i in range(len(prompts))]
+        return of(0), of(1)

@@ -5,12 +5,12 @@ at tensor-parallel size 1 with u-muP off (the residual split / add are then iden
 core/nn/residual.py:49-65).
 """
 
-from typing import Callable, List, Optional
+from typing import Callable, List, Optional, Union
 
 import torch
 
 from .config import MLPType, TransformerArchitectureConfig
-from .nn import PagedKVCache, PagedStep, ParallelMLP, ParallelSelfAttention, ParallelSwiGLUMLP, RMSNorm, _direct, _unhooked, decode_layer, fuses_residual, get_norm, idle_dropout, layer_in_one_call, one_token_each
+from .nn import BranchStep, PagedKVCache, PagedStep, ParallelMLP, ParallelSelfAttention, ParallelSwiGLUMLP, RMSNorm, _direct, _unhooked, decode_layer, fuses_residual, get_norm, idle_dropout, layer_in_one_call, one_token_each
 
 
 class InferenceSettings:
@@ -111,7 +111,7 @@ class TransformerLayer(torch.nn.Module):
         return h + self.mlp(self.post_attention_layernorm(h))
 
     @torch.no_grad()
-    def paged_step(self, hidden_state: torch.Tensor, cache: PagedKVCache, step: PagedStep) -> torch.Tensor:
+    def paged_step(self, hidden_state: torch.Tensor, cache: PagedKVCache, step: Union[PagedStep, BranchStep]) -> torch.Tensor:
         """The layer on the new tokens of a step over a paged cache, whose layer `layer_index` is this one's (inference; see
         ParallelSelfAttention.paged_forward)."""
         if self._own_blocks() and fuses_residual(self.input_layernorm) and fuses_residual(self.post_attention_layernorm):

@@ -8,7 +8,7 @@ do not cover raise `NotImplementedError` instead of silently taking another path
 """
 
 import math
-from typing import Callable, Dict, List, Optional, Sequence, Tuple
+from typing import Callable, Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -497,12 +497,88 @@ class PagedKVCache:
         self._pages[sequence] = []
         self.lengths[sequence] = 0
 
+    def take(self, pages: int) -> List[int]:
+        """Pages that somebody else manages, until they are given back."""
+        if not 0 <= pages <= len(self._free):
+            raise RuntimeError(f"{pages} pages are wanted, {len(self._free)} are free")
+        taken, self._free = self._free[len(self._free) - pages:], self._free[:len(self._free) - pages]
+        return taken
+
+    def give(self, pages: Sequence[int]) -> None:
+        self._free.extend(pages)
+
     def workspace(self) -> torch.Tensor:
         """Scratch of ops.paged_attention for calls of any size: one for the cache's life, so that a captured call keeps its own."""
         if self._workspace is None:
             # what a call needs stops to grow at a few rows
             self._workspace = ops.paged_workspace(self.max_sequences, 2 ** 20, self.n_q, self.n_kv, self.head_dim, self.device)
         return self._workspace
+
+
+class BranchStep:
+    """What one call over PagedBranches brings (PagedBranches.step makes it), as PagedStep, laid out on the device: `tokens` rows, of which as many belong to a
+    branch as have something new; `sequences` int64 [tokens]: the branch of a row; `last` int64 [branches]: its last row (0 of those without any)."""
+
+    def __init__(self, branches: "PagedBranches", tensors: ops.StepTensors, tokens: int, max_q_len: int) -> None:
+        self.branches, self.tokens, self.max_q_len, self.longest = branches, tokens, max_q_len, branches.longest
+        self.cu_seqlens, self.position_ids, self.slots, self.sequences, self.last = tensors
+        self.ctx_len = branches.ctx_len
+
+
+class PagedBranches:
+    """Branches of sequences of a PagedKVCache, `count` of each, that go on from what the sequence holds: several answers to a prompt.  A sequence's keys are the shared prefix
+    of its branches (read once for all of them, ops.paged_prefix_attention) and stay where they are; a branch has own keys alone, up to `max_ctx`, in pages
+    that the branches take from `num_pages` of the cache's.  Branch i of the j-th of `sequences` is number j * count + i.
+
+    Lengths and free pages lie on the device, and a step is planned there (ops.paged_step): the host neither knows nor waits for how long the branches are or which have ended, and
+    a step may be captured with the layers' calls and replayed.  Until `close` the sequences have to stay as they are in the cache."""
+
+    def __init__(self, cache: PagedKVCache, sequences: Sequence[int], count: int, max_ctx: int, num_pages: Optional[int] = None) -> None:
+        sequences = [int(b) for b in sequences]
+        if not sequences or count < 1 or max_ctx < 1 or not all(0 <= b < cache.max_sequences for b in sequences):
+            raise ValueError(f"branches of sequences 0 to {cache.max_sequences - 1}, at least one of each, of at least one token, got {count} of {sequences}")
+        self.cache, self.count, self.max_ctx, self.total = cache, count, max_ctx, count * len(sequences)
+        width = -(-max_ctx // cache.page_size)
+        self.pages = cache.take(self.total * width if num_pages is None else num_pages)
+        prefix = [cache.lengths[b] for b in sequences]
+        self.longest = max(prefix) + max_ctx
+
+        def ints(values):
+            return torch.tensor(values, dtype=torch.int32, device=cache.device)
+        self.prefix_table = cache.page_table.index_select(0, torch.tensor(sequences, dtype=torch.int64, device=cache.device))
+        self.prefix_len, self.group_seqs = ints(prefix), ints(list(range(0, self.total + 1, count)))
+        self.position_offset = ints([n for n in prefix for _ in range(count)])
+        self.ctx_len, self.page_table = ints([0] * self.total), torch.zeros(self.total, width, dtype=torch.int32, device=cache.device)
+        self.free_pages, self.state = ints(self.pages), ints([len(self.pages), 0])
+        self._workspaces: Dict[int, torch.Tensor] = {}
+
+    def step(self, new: torch.Tensor, tokens: int, max_q_len: int) -> BranchStep:
+        """Takes pages for new[i] more tokens of branch i (int32 [branches] on the device; 0: none, negative: the branch ends and gives its pages back), at most `tokens` in all and
+        max_q_len of one.  If they do not fit, nobody has any in this step, and `check` raises."""
+        tensors = ops.paged_step(new, self.ctx_len, self.page_table, self.free_pages, self.state, self.cache.page_size, tokens, self.max_ctx, self.position_offset)
+        return BranchStep(self, tensors, tokens, max_q_len)
+
+    def workspace(self, tokens: int) -> torch.Tensor:
+        """Scratch of ops.paged_prefix_attention for steps of `tokens` rows, kept for the branches' life (one that is made while a graph is captured is the graph's alone)."""
+        workspace = self._workspaces.get(tokens)
+        if workspace is None:
+            cache = self.cache
+            workspace = ops.paged_prefix_workspace(self.total, len(self.prefix_len), tokens, cache.n_q, cache.n_kv, cache.head_dim, cache.device)
+            if not (workspace.is_cuda and torch.cuda.is_current_stream_capturing()):
+                self._workspaces[tokens] = workspace
+        return workspace
+
+    def check(self) -> None:
+        """Raises if a step did not fit (waits for the device)."""
+        status = int(self.state[1])
+        if status != 0:
+            what = [text for bit, text in ((1, "the pages ran out"), (2, f"a branch would pass {self.max_ctx} tokens"), (4, "more tokens than rows")) if status & bit]
+            raise RuntimeError("a step of the branches did not fit: " + ", ".join(what))
+
+    def close(self) -> None:
+        """The branches end: their pages are the cache's again (behind the calls that are on the stream)."""
+        self.cache.give(self.pages)
+        self.pages = []
 
 
 class ParallelSelfAttention(torch.nn.Module):
@@ -765,8 +841,8 @@ class ParallelSelfAttention(torch.nn.Module):
         return (*rot.tables(), pos), interleaved
 
     # ---- paged KV cache ------------------------------------------------------------------------------
-    def paged_forward(self, x: torch.Tensor, cache: PagedKVCache, layer: int, step: PagedStep) -> torch.Tensor:
-        """Attention of the new tokens that `step` (of cache.step) brings, x [b, s, H] with b * s of them, sequence after sequence: keys and values go into the
+    def paged_forward(self, x: torch.Tensor, cache: PagedKVCache, layer: int, step: Union[PagedStep, BranchStep]) -> torch.Tensor:
+        """Attention of the new tokens that `step` (of cache.step, or of the step of branches of its sequences) brings, x [b, s, H] with b * s of them, sequence after sequence: keys and values go into the
         pages of layer `layer` (normed and rotated on the way, in one launch), and every token sees the keys of its sequence up to itself.
         For inference: no gradients, no dropout.  The same call takes prompts, single tokens and drafts of several tokens, mixed as they come."""
         b, s, _ = x.shape
@@ -779,7 +855,11 @@ class ParallelSelfAttention(torch.nn.Module):
             raise ValueError(f"{b * s} tokens in x, {step.tokens} in the step")
         if self.rotary_embedding is not None and step.longest > self.rotary_embedding.max_seq_length:
             raise IndexError(f"position {step.longest - 1} is outside the rotary table of {self.rotary_embedding.max_seq_length} rows")
-        pages = (cache.k_pages[layer], cache.v_pages[layer], cache.page_table[:step.ctx_len.numel()], step.cu_seqlens, step.ctx_len)
+        branches = getattr(step, "branches", None)
+        if branches is not None and branches.cache is not cache:
+            raise ValueError("a step of branches of another cache")
+        table = cache.page_table[:step.ctx_len.numel()] if branches is None else branches.page_table
+        pages = (cache.k_pages[layer], cache.v_pages[layer], table, step.cu_seqlens, step.ctx_len)
         with torch.no_grad():
             q, k, v = self._project(x)
             norms = self._own_norms() if self.key_query_norm else None
@@ -794,7 +874,11 @@ class ParallelSelfAttention(torch.nn.Module):
                 ops.paged_append(k, v, *pages)
             else:
                 q = ops.paged_append(k, v, *pages, q=q, rotary=rotary, interleaved=interleaved, **(norms or {}))
-            ctx = ops.paged_attention(q, *pages, softmax_scale=self.softmax_scale, max_q_len=step.max_q_len, workspace=cache.workspace())
+            if branches is None:
+                ctx = ops.paged_attention(q, *pages, softmax_scale=self.softmax_scale, max_q_len=step.max_q_len, workspace=cache.workspace())
+            else:
+                ctx = ops.paged_prefix_attention(q, *pages, branches.prefix_table, branches.prefix_len, branches.group_seqs, softmax_scale=self.softmax_scale,
+                                                 max_q_len=step.max_q_len, workspace=branches.workspace(step.tokens))
             return self.dense(ctx.view(b, s, nq * d))
 
     # ---- KV cache ----------------------------------------------------------------------------------

@@ -1,0 +1,168 @@
+"""Sampling, steps planned on the GPU and attention over shared prefixes together, as the modules use them."""
+
+import pytest
+import torch
+
+from scaling_amd import ops
+from scaling_amd.nn import PagedBranches, PagedKVCache
+from tests.parity import check
+from tests.test_gpu_modules import _arch, _oracle_layer, _seeded_layer
+from tests.test_gpu_paged_modules import PROMPTS, _margin, _model, _uncached
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("name,kw", [("gqa_norms", dict(hidden_size=512, num_attention_heads=8, attention_num_kv_heads=2, mlp_factor=2.5, key_query_norm=True)),
+                                     ("complex_float16", dict(precision="float16", relative_position_embedding_type="rotary_complex")),
+                                     ("no_rotary_fused_qkv", dict(relative_position_embedding_type="none", attention_qkv_in_one=True, attention_bias=True))],
+                         ids=lambda x: x if isinstance(x, str) else "")
+def test_layer_over_branches(name, kw):
+    """Three branches of each of two prompts, with single tokens, drafts, idle ones and one that ends and starts again: outputs against the oracle's on whole sequences."""
+    print(f"case {name}", flush=True)
+    cfg = _arch(**kw)
+    layer = _seeded_layer(cfg, seed=0).eval()
+    dtype, g, att = cfg.precision.dtype, torch.Generator().manual_seed(2), layer.self_attention
+    prompts = [torch.randn(n, cfg.hidden_size, generator=g).to(dtype) for n in (40, 7)]
+    steps = [[1, 1, 1, 1, 1, 1], [3, 0, 20, 1, 2, 0], [1, -1, 1, 0, 1, 1], [1, 4, 0, 1, 1, 18]]
+    total = [sum(max(s[b], 0) for s in steps) for b in range(6)]
+    x = [torch.randn(n, cfg.hidden_size, generator=g).to(dtype) for n in total]
+    cache = PagedKVCache(1, 30, 2, 64, att.num_attention_heads, att.num_kv_heads_per_partition, att.hidden_size_per_attention_head, dtype, DEV, page_size=16)
+    h = layer.paged_step(torch.cat(prompts).to(DEV).view(1, -1, cfg.hidden_size), cache, cache.step([40, 7]))
+    free = cache.free_pages
+    branches = PagedBranches(cache, [0, 1], 3, 32, 14)
+    assert cache.free_pages == free - 14
+    done, out = [0] * 6, [[] for _ in range(6)]
+    for new in steps:
+        tokens = sum(max(n, 0) for n in new) + 2            # rows that belong to nobody
+        plan = branches.step(_ints(new), tokens, max(new))
+        h = torch.cat([x[b][done[b]:done[b] + max(n, 0)] for b, n in enumerate(new)] + [x[0][:1]] * 2).to(DEV)
+        y = layer.paged_step(h.view(1, -1, cfg.hidden_size), cache, plan)[0].cpu()
+        for b, part in enumerate(y[:tokens - 2].split([max(n, 0) for n in new])):
+            out[b].append(part)
+            done[b] += max(new[b], 0)
+    branches.check()
+    assert branches.ctx_len.tolist() == [6, 4, 22, 3, 5, 20]
+    branches.close()
+    assert cache.free_pages == free and sorted(cache._free) == sorted(set(cache._free))
+    # whole sequences: the second branch's tokens after its end follow the prompt again
+    parts, got = [], []
+    for b in range(6):
+        pieces = [x[b][:1], x[b][1:]] if b == 1 else [x[b]]
+        for piece in pieces:
+            parts.append(torch.cat((prompts[b // 3], piece)))
+        got += [torch.cat(out[b])[:1], torch.cat(out[b])[1:]] if b == 1 else [torch.cat(out[b])]
+    ends = torch.tensor([0] + [len(p) for p in parts]).cumsum(0)
+    cu, pos, whole = ends.to(torch.int32), torch.cat([torch.arange(len(p)) for p in parts]).view(1, -1), torch.cat(parts).view(1, -1, cfg.hidden_size)
+    refs = [_oracle_layer(cfg, layer.state_dict(), whole, cu, pos, torch.ones_like(whole), t)[0][0] for t in (torch.float32, dtype)]
+    ref, order = (torch.cat([r[ends[i] + len(parts[i]) - len(got[i]):ends[i + 1]] for i in range(len(parts))]) for r in refs)
+    check(f"branches {name}", torch.cat(got), ref, order, module_level=True)
+
+
+def _logprobs(model, prompt, ids):
+    return torch.log_softmax(_uncached(model, torch.tensor(prompt + ids))[len(prompt) - 1:-1].float(), dim=-1)
+
+
+def test_samples_follow_the_model():
+    """Log-probabilities are those of the uncached model, within what its logits are off by (twice: a logit and the logarithm of the sum); so are greedy choices."""
+    model = _model()
+    margin = _margin(model)
+    ids, logprobs = model.generate_samples(9, PROMPTS, 3, page_size=16, generator=torch.Generator(device=DEV).manual_seed(0))
+    assert [[len(s) for s in p] for p in ids] == [[9] * 3] * 4 == [[len(s) for s in p] for p in logprobs]
+    assert len({tuple(s) for p in ids for s in p}) > 6
+    worst = 0.0
+    for prompt, answers, lps in zip(PROMPTS, ids, logprobs):
+        for answer, lp in zip(answers, lps):
+            want = _logprobs(model, prompt, answer).gather(1, torch.tensor(answer, device=DEV).view(-1, 1))[:, 0]
+            worst = max(worst, float((torch.tensor(lp, device=DEV) - want).abs().max()))
+    print(f"log-probabilities off by {worst:.4f} of {2 * margin:.4f}", flush=True)
+    assert worst <= 2 * margin
+    greedy, zeros = model.generate_samples(9, PROMPTS, 2, temperature=0.0, page_size=16)
+    assert all(lp == 0.0 for p in zeros for s in p for lp in s)
+    for prompt, answers in zip(PROMPTS, greedy):
+        for answer in answers:
+            lp = _logprobs(model, prompt, answer)
+            assert float((lp.max(dim=1).values - lp.gather(1, torch.tensor(answer, device=DEV).view(-1, 1))[:, 0]).max()) <= margin
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(key_query_norm=False, norm_type="layernorm", mlp_type="default", mlp_factor=4.0, attention_qkv_in_one=True, attention_num_kv_heads=None)],
+                         ids=["rms", "layernorm"])
+def test_a_captured_loop_draws_what_an_eager_one_does(kw):
+    """With and without stop tokens, which end some answers and not others; the given numbers decide."""
+    model = _model(**kw)
+    u = torch.rand(20, 12, generator=torch.Generator().manual_seed(1))
+    parameters = dict(samples=3, temperature=0.8, top_k=40, top_p=0.95, min_p=0.001, uniforms=u, page_size=16)
+    free = model.generate_samples(20, PROMPTS, graph=False, **parameters)
+    assert model.generate_samples(20, PROMPTS, graph=True, **parameters) == free
+    assert model.generate_samples(20, PROMPTS, graph=True, **parameters) == free
+    first = model.generate_samples(1, PROMPTS, **{**parameters, "uniforms": u[:1]})
+    assert first[0] == [[s[:1] for s in p] for p in free[0]]
+    stop = [free[0][0][0][4], free[0][2][1][7], free[0][3][2][0]]
+    ended = model.generate_samples(20, PROMPTS, stop_tokens=stop, graph=False, **parameters)
+    assert model.generate_samples(20, PROMPTS, stop_tokens=stop, graph=True, **parameters) == ended
+    lengths = [len(s) for p in ended[0] for s in p]
+    assert min(lengths) < 20
+    for p, (some, every) in enumerate(zip(ended[0], free[0])):
+        for a, b in zip(some, every):
+            assert not set(a[:-1]) & set(stop) and (len(a) == 20 or a[-1] in stop)
+    assert ended[0][3][2] == free[0][3][2][:1]              # drawn before anybody left
+    assert [[len(s) for s in p] for p in ended[1]] == [[len(s) for s in p] for p in ended[0]]
+
+
+def test_everybody_ends_early():
+    model = _model()
+    every = list(range(model.architecture_config.vocab_size))
+    ids, logprobs = model.generate_samples(40, PROMPTS, 2, stop_tokens=every, page_size=16)
+    assert [[len(s) for s in p] for p in ids] == [[1] * 2] * 4
+
+
+def test_branches_refuse_and_tell():
+    cache = PagedKVCache(1, 10, 2, 64, 4, 2, 64, torch.bfloat16, DEV, page_size=16)
+    cache.step([20, 3])
+    for bad in (([], 1, 4), ([2], 1, 4), ([0], 0, 4), ([0], 1, 0)):
+        with pytest.raises(ValueError):
+            PagedBranches(cache, *bad)
+    with pytest.raises(RuntimeError):
+        PagedBranches(cache, [0], 8, 16)
+    assert cache.free_pages == 7
+    branches = PagedBranches(cache, [0, 1], 2, 40, 5)
+    branches.step(_ints([17, 1, 1, 0]), 19, 17)
+    branches.check()
+    branches.step(_ints([0, 16, 16, 16]), 48, 16)            # three pages, one is left
+    branches.step(_ints([24, 0, 0, 0]), 24, 24)              # 41 keys
+    branches.step(_ints([1, 1, 0, 0]), 1, 1)
+    with pytest.raises(RuntimeError, match="pages ran out.*pass 40 tokens.*more tokens than rows"):
+        branches.check()
+    assert branches.ctx_len.tolist() == [17, 1, 1, 0]
+    other = PagedKVCache(1, 10, 2, 64, 4, 2, 64, torch.bfloat16, DEV, page_size=16)
+    layer = _seeded_layer(_arch(num_attention_heads=4, attention_num_kv_heads=2, hidden_size=256), seed=0).eval()
+    plan = branches.step(_ints([1, 0, 0, 0]), 1, 1)
+    with pytest.raises(ValueError, match="another cache"):
+        layer.paged_step(torch.zeros(1, 1, 256, dtype=torch.bfloat16, device=DEV), other, plan)
+
+
+def test_generation_refuses():
+    model = _model()
+    for bad in (dict(max_tokens=0), dict(samples=0), dict(prompts=[]), dict(prompts=[[1], []]), dict(uniforms=torch.zeros(2, 3)), dict(uniforms=torch.zeros(3, 2).double())):
+        with pytest.raises(ValueError):
+            model.generate_samples(**{**dict(max_tokens=3, prompts=[[1, 2]], samples=2), **bad})
+    with pytest.raises(IndexError):
+        model.generate_samples(100, [[1], [2] * 30], 2)
+
+
+def test_other_numbers_other_answers_on_another_stream():
+    """Two loops at once on two streams, each with its own graph, state and scratch."""
+    model = _model()
+    u = [torch.rand(12, 6, generator=torch.Generator().manual_seed(s)) for s in (3, 4)]
+    want = [model.generate_samples(12, PROMPTS[:3], 2, uniforms=x, page_size=16) for x in u]
+    assert want[0] != want[1]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert model.generate_samples(12, PROMPTS[:3], 2, uniforms=u[1], page_size=16) == want[1]
+    torch.cuda.current_stream().wait_stream(side)
+    assert ops.sample_rows(torch.zeros(1, 4, device=DEV), torch.zeros(1, device=DEV)).tolist() == [0]
