@@ -44,6 +44,23 @@ template <typename T> struct Row {
         head = to_boundary < vocab ? to_boundary : vocab;
         vecs = (vocab - head) / V;
     }
+    // f(vector, its number, whether there is one) by all threads alike, next() behind every four vectors a thread
+    template <class F, class G> __device__ __forceinline__ void vectors(const F& f, const G& next) const {
+        const uint4* at = reinterpret_cast<const uint4*>(x + head);
+        uint4 u[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) u[a] = vecs > 0 ? at[min((int)threadIdx.x + a * kThreads, vecs - 1)] : make_uint4(0, 0, 0, 0);
+        for (int v0 = 0; v0 < vecs; v0 += kAhead * kThreads) {
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                const int v = v0 + a * kThreads + (int)threadIdx.x;
+                const uint4 now = u[a];
+                u[a] = at[min(v + kAhead * kThreads, vecs - 1)];
+                f(now, v, v < vecs);
+            }
+            next();
+        }
+    }
     // f(value, index) of every element
     template <class F> __device__ __forceinline__ void each(const F& f) const {
         const uint4* at = reinterpret_cast<const uint4*>(x + head);
@@ -81,7 +98,7 @@ struct Shared {
 __device__ __forceinline__ uint64_t shuffle_up(uint64_t v, int by) { return __shfl_up((unsigned long long)v, by, 64); }
 
 // Sums over the threads in front of this one, and over all.
-__device__ __forceinline__ Mass scan(Shared& s, Mass v, Mass& all) {
+__device__ __forceinline__ Mass scan(Mass* partial, Mass v, Mass& all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     Mass upto = v;
 #pragma unroll
@@ -90,12 +107,12 @@ __device__ __forceinline__ Mass scan(Shared& s, Mass v, Mass& all) {
         if (lane >= by) { upto.count += c; upto.weight += w; }
     }
     __syncthreads();
-    if (lane == 63) s.partial[wave] = upto;
+    if (lane == 63) partial[wave] = upto;
     __syncthreads();
     Mass before{0, 0};
     all = Mass{0, 0};
     for (int w = 0; w < kWaves; ++w) {
-        const Mass m = s.partial[w];
+        const Mass m = partial[w];
         if (w < wave) { before.count += m.count; before.weight += m.weight; }
         all.count += m.count;
         all.weight += m.weight;
@@ -162,7 +179,7 @@ template <typename T> struct Search {
         constexpr int kEach = kBins / kThreads;
         Mass mine{0, 0}, all;
         for (int i = 0; i < kEach; ++i) { mine.count += s.count[kEach * threadIdx.x + i]; mine.weight += s.weight[kEach * threadIdx.x + i]; }
-        Mass at = scan(s, mine, all);
+        Mass at = scan(s.partial, mine, all);
         at.count += before.count;
         at.weight += before.weight;
         if (threadIdx.x == 0) s.number = 0;
@@ -240,7 +257,7 @@ template <typename T> struct Search {
             index = (int)(uint32_t)s.sorted[threadIdx.x];
             mine = Mass{1, weights.whole_of(key_value(key))};
         }
-        Mass at = scan(s, mine, all);
+        Mass at = scan(s.partial, mine, all);
         at.count += before.count;
         at.weight += before.weight;
         const Mass next{at.count + mine.count, at.weight + mine.weight};
@@ -284,19 +301,70 @@ template <typename T> struct Search {
     }
 };
 
-// One workgroup per row.
+// ---- parameters -----------------------------------------------------------------------------------------------------------------------------------------
+// (compared as bits: comparisons with NaN are compiled away)
+struct Parameters {
+    bool greedy, top_p_none, top_p_one, any_min_p;         // top-p keeps everything, or one token
+    int k;
+    float u;
+    double inverse, top_p, min_p;
+    __device__ __forceinline__ Parameters(const SampleParams& p, int64_t r) {
+        const uint32_t t_bits = __float_as_uint(p.temperature ? p.temperature[r] : p.temperature0), u_bits = __float_as_uint(p.uniforms[r]);
+        const uint32_t p_bits = __float_as_uint(p.top_p ? p.top_p[r] : p.top_p0), m_bits = __float_as_uint(p.min_p ? p.min_p[r] : p.min_p0);
+        k = p.top_k ? p.top_k[r] : p.top_k0;
+        greedy = t_bits - 1u >= 0x7f800000u;               // zero, negative, NaN
+        if (greedy) k = 1;
+        inverse = greedy ? 1.0 : 1.0 / (double)__uint_as_float(t_bits);
+        u = u_bits > 0x7f800000u ? 0.f : __uint_as_float(min(u_bits, 0x3f7fffffu));     // negative, NaN: 0
+        top_p_one = p_bits >= 0x80000000u && p_bits <= 0xff800000u;
+        top_p_none = !top_p_one && p_bits >= 0x3f800000u;
+        top_p = (double)__uint_as_float(p_bits);
+        any_min_p = m_bits - 1u < 0x7f800000u;
+        min_p = (double)__uint_as_float(m_bits);
+    }
+};
+
+// What top-k and top-p leave, and with min-p the token: find(by_count, goal) gives the mass up to the first token that reaches the goal.  heavy: the weight of those
+// of at least min_p.  (One call in a loop: the compiler makes three of three, with registers for each.)
+template <class F> __device__ __forceinline__ uint64_t draw(const Parameters& p, const Mass& all, uint64_t one, uint64_t heavy, const F& find) {
+    uint64_t kept = all.weight;
+#pragma unroll 1
+    for (int step = 0; step < 3; ++step) {
+        uint64_t goal = (uint64_t)p.k;
+        if (step == 0 && !(p.k > 0 && goal < all.count)) continue;
+        if (step == 1) {
+            if (p.top_p_one) kept = one;
+            if (p.top_p_one || p.top_p_none) continue;
+            const double least = ceil((double)kept * p.top_p);
+            goal = least < 1.0 ? 1 : (uint64_t)least;
+        }
+        if (step == 2) {
+            if (p.any_min_p) kept = min(kept, max(heavy, one));
+            goal = min((uint64_t)((double)kept * (double)p.u) + 1, kept);
+        }
+        const uint64_t weight = find(step, goal).weight;
+        if (step < 2) kept = weight;
+    }
+    return kept;
+}
+
+__device__ __forceinline__ void write_nothing(const SampleParams& p, int64_t r) {
+    if (threadIdx.x != 0) return;
+    p.ids[r] = 0;
+    if (p.logprobs) p.logprobs[r] = -INFINITY;
+}
+__device__ __forceinline__ void write_logprob(const SampleParams& p, int64_t r, const Weights& w, float x, uint64_t kept) {
+    if (p.logprobs) p.logprobs[r] = (float)(w.log_of(x) - log(ldexp((double)kept, -w.bits)));
+}
+__device__ __forceinline__ int weight_bits(int vocab) { return min(51, 30 + __builtin_clz((unsigned)vocab)); }      // all tokens' sum stays under 2^62
+
+// ---- 32-bit logits --------------------------------------------------------------------------------------------------------------------------------------
+// One workgroup per row, which it reads once for the range of its values, once for the bins, and once for every bin that is looked into.
 template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) {
     __shared__ Shared s;
     const int64_t r = blockIdx.x;
     const Row<T> row(p, r);
-    // ---- parameters (compared as bits: comparisons with NaN are compiled away) ----
-    const uint32_t t_bits = __float_as_uint(p.temperature ? p.temperature[r] : p.temperature0);
-    const bool greedy = t_bits - 1u >= 0x7f800000u;        // zero, negative, NaN
-    const uint32_t u_bits = __float_as_uint(p.uniforms[r]);
-    const float u = u_bits >= 0x80000000u || u_bits > 0x7f800000u ? 0.f : __uint_as_float(min(u_bits, 0x3f7fffffu));
-    const uint32_t p_bits = __float_as_uint(p.top_p ? p.top_p[r] : p.top_p0), m_bits = __float_as_uint(p.min_p ? p.min_p[r] : p.min_p0);
-    int k = p.top_k ? p.top_k[r] : p.top_k0;
-    if (greedy) k = 1;
+    const Parameters of(p, r);
     // ---- the largest and the smallest value with a weight ----
     uint32_t lo = 0xffffffffu, hi = 0;
     row.each([&](float x, int) {
@@ -311,56 +379,288 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     lo = (uint32_t)s.word[2];
     hi = (uint32_t)s.word[3];
     __syncthreads();
-    if (hi == 0) {                                         // nothing to draw from
-        if (threadIdx.x == 0) {
-            p.ids[r] = 0;
-            if (p.logprobs) p.logprobs[r] = -INFINITY;
-        }
-        return;
-    }
-    Weights w;
-    w.largest = key_value(hi);
-    w.inverse = greedy ? 1.0 : 1.0 / (double)__uint_as_float(t_bits);
-    w.bits = min(51, 30 + __builtin_clz((unsigned)row.vocab));        // all tokens' sum stays under 2^62
+    if (hi == 0) return write_nothing(p, r);
+    const Weights w{key_value(hi), of.inverse, weight_bits(row.vocab)};
+    const uint64_t one = 1ull << w.bits;
     Search<T> search{s, row, w, Bins{lo, hi, w.largest, 0.f, 0}};
     const float range = w.largest - key_value(lo);
     search.first.scale = range > 0.f && range < INFINITY ? (float)kBins / range : 0.f;
     if (!(search.first.scale < INFINITY)) search.first.scale = 0.f;
     if (search.first.scale == 0.f) search.first.shift = hi > lo ? max(0, 32 - (int)__builtin_clz(hi - lo) - 12) : 0;
-    // ---- what is kept: so much weight ----
+    // ---- what is kept, and the token ----
     search.fill(search.first);
     search.filled = true;
     Mass mine{0, 0}, all;
     for (int i = threadIdx.x; i < kBins; i += kThreads) { mine.count += s.count[i]; mine.weight += s.weight[i]; }
-    scan(s, mine, all);
-    uint64_t kept = all.weight;
-    if (k > 0 && (uint64_t)k < all.count) kept = search.find(true, (uint64_t)k, false).upto.weight;
-    const uint64_t one = 1ull << w.bits;
-    const uint64_t of_k = kept;
-    if (p_bits >= 0x80000000u && p_bits <= 0xff800000u) {  // negative
-        kept = one;
-    } else if (p_bits < 0x3f800000u) {
-        const double goal = ceil((double)of_k * (double)__uint_as_float(p_bits));
-        kept = search.find(false, goal < 1.0 ? 1 : (uint64_t)goal, false).upto.weight;
-    }
-    if (m_bits - 1u < 0x7f800000u) {
-        const double least = (double)__uint_as_float(m_bits);
-        Mass heavy{0, 0};
+    scan(s.partial, mine, all);
+    uint64_t heavy = 0;
+    if (of.any_min_p) {
+        Mass mass{0, 0}, sum;
         row.each([&](float x, int) {
             if (value_key(x) == 0) return;
             const double v = w.of(x);
-            if (v >= least) heavy.weight += w.whole(v);
+            if (v >= of.min_p) mass.weight += w.whole(v);
         });
-        scan(s, heavy, all);
-        kept = min(kept, max(all.weight, one));
+        scan(s.partial, mass, sum);
+        heavy = sum.weight;
     }
-    // ---- the token ----
-    const uint64_t goal = (uint64_t)((double)kept * (double)u) + 1;
-    const Found f = search.find(false, min(goal, kept), true);
+    Found f;
+    const uint64_t kept = draw(of, all, one, heavy, [&](int step, uint64_t goal) { f = search.find(step == 0, goal, step == 2); return f.upto; });
     if (threadIdx.x == 0) {
         p.ids[r] = f.index;
-        if (p.logprobs) p.logprobs[r] = (float)(w.log_of(key_value(f.key)) - log(ldexp((double)kept, -w.bits)));
+        write_logprob(p, r, w, key_value(f.key), kept);
     }
+}
+
+// ---- 16-bit logits --------------------------------------------------------------------------------------------------------------------------------------
+// There are 2^16 values, so a workgroup counts how often each occurs in its row: equal tokens weigh the same, and everything else is arithmetic on the
+// few thousand values that occur, with one exponential each.  A second pass over the row
+// finds which of the tokens that equal the drawn value is meant.  Counts of 16 bits, two to a word of LDS, are 128 KB.  One of more than 65535 equal
+// tokens overflows, which shows as counts that do not add up: then once more, in pieces of 32768 tokens with counts over 32767 put aside in between.
+constexpr int kKeys = 1 << 16, kUnit = 64, kUnits = kKeys / kUnit, kAside = MI_SAMPLE_VOCAB_MAX / 32768 + 1;     // (and one more for zeros)
+
+struct KeyShared {
+    uint32_t counts[kKeys / 2];                            // of keys 2 i and 2 i + 1
+    uint64_t unit_weight[kUnits + 1];                      // of units of 64 keys that occur, largest first: sums in front; of all
+    uint32_t unit_count[kUnits + 1];
+    uint16_t units[kUnits];
+    Mass partial[kWaves];
+    uint64_t heavy, number;
+    uint32_t occupied[kWaves * 2];
+    int index, n_aside;
+    uint32_t aside_key[kAside], aside[kAside];
+};
+
+template <typename T> struct Key16 {
+    static constexpr uint32_t kInf = std::is_same_v<T, _Float16> ? 0x7c00u : 0x7f80u, kTop = kInf | 0x8000u, kNone = 0x7fffu - kInf;     // keys of +inf and -inf
+    // both halves: values to 16-bit keys of the same order; -0 is one below +0
+    static __device__ __forceinline__ uint32_t keys(uint32_t w) { return w ^ (((w >> 15) & 0x00010001u) * 0x7fffu | 0x80008000u); }
+    static __device__ __forceinline__ uint32_t bits(uint32_t key) { return (key & 0x8000u) != 0 ? key & 0x7fffu : ~key & 0xffffu; }
+    static __device__ __forceinline__ float value(uint32_t key) { return (float)__builtin_bit_cast(T, (uint16_t)bits(key)); }
+};
+typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+
+template <typename T> __global__ __launch_bounds__(kThreads) void sample_keys_kernel(const SampleParams p) {
+    using K = Key16<T>;
+    __shared__ KeyShared s;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t r = blockIdx.x;
+    const Row<T> row(p, r);
+    const int behind = row.head + row.vecs * 8, single = tid < row.head ? tid : behind + tid - row.head;
+    uint32_t single_bits = 0;
+    if (single < row.vocab) { T x = row.x[single]; single_bits = __builtin_bit_cast(uint16_t, x); }
+    const Parameters of(p, r);
+
+    // ---- how often each value occurs ----
+    const auto count_of = [&](uint32_t key) -> uint32_t {
+        if (key > K::kTop || key <= K::kNone) return 0;
+        uint32_t c = (s.counts[key >> 1] >> (16 * (key & 1))) & 0xffffu;
+        for (int i = 0; i < s.n_aside; ++i) c += s.aside_key[i] == key ? s.aside[i] : 0;
+        return c;
+    };
+    const auto put_aside = [&]() {
+        __syncthreads();
+        for (int i = tid; i < kKeys / 2; i += kThreads) {
+            const uint32_t both = s.counts[i], over = both & 0x80008000u;
+            if (over == 0) continue;
+            s.counts[i] = both & 0x7fff7fffu;
+            for (int h = 0; h < 2; ++h)
+                if ((over >> (16 * h + 15) & 1) != 0) {
+                    const int e = min(atomicAdd(&s.n_aside, 1), kAside - 1);
+                    s.aside_key[e] = 2 * i + h;
+                    s.aside[e] = 32768;
+                }
+        }
+        __syncthreads();
+    };
+    int pieces = 0;                                        // 1: counts are put aside between pieces
+    for (;;) {
+        for (int i = tid; i < kKeys / 8; i += kThreads) reinterpret_cast<uint4*>(s.counts)[i] = make_uint4(0, 0, 0, 0);
+        if (tid == 0) { s.n_aside = 0; s.heavy = 0; s.number = 0; }
+        __syncthreads();
+        uint32_t counted = 0;                              // of the wavefront
+        const auto add = [&](uint32_t key, bool there) {
+            there = there && key != K::kNone;              // (masked tokens are many)
+            counted += __popcll(__ballot(there));
+            if (there) atomicAdd(&s.counts[key >> 1], 1u << (16 * (key & 1)));
+        };
+        const auto add_vector = [&](const uint4& u, bool there) {
+            const uint32_t w[4] = {K::keys(u.x), K::keys(u.y), K::keys(u.z), K::keys(u.w)};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { add(w[i] & 0xffffu, there); add(w[i] >> 16, there); }
+        };
+        row.vectors([&](const uint4& u, int, bool there) { add_vector(u, there); }, [&]() { if (pieces != 0) put_aside(); });
+        add(K::keys(single_bits) & 0xffffu, single < row.vocab);
+        if (pieces != 0) put_aside();                      // (the last ones: fewer than a vector)
+        if (pieces != 0 || row.vocab <= 0xffff) break;
+        if (lane == 0) atomicAdd((unsigned long long*)&s.number, (unsigned long long)counted);
+        __syncthreads();
+        uint32_t found = 0;
+        for (int i = tid; i < kKeys / 2; i += kThreads) found += (s.counts[i] & 0xffffu) + (s.counts[i] >> 16);
+        found = group_reduce_bits<64>(found, [](uint32_t a, uint32_t b) { return a + b; });
+        if (lane == 0) atomicAdd((unsigned long long*)&s.number, (unsigned long long)-(long long)found);
+        __syncthreads();
+        if (s.number == 0) break;
+        pieces = 1;
+        __syncthreads();
+    }
+    __syncthreads();
+    if (tid == 0) {                                        // -0 is +0
+        const uint32_t zeros = s.counts[0x7fff >> 1] >> 16, plus = s.counts[0x8000 >> 1] & 0xffffu;
+        s.counts[0x7fff >> 1] &= 0xffffu;
+        if (zeros + plus <= 0xffffu) {
+            s.counts[0x8000 >> 1] += zeros;
+        } else {
+            const int e = min(s.n_aside, kAside - 1);
+            s.aside_key[e] = 0x8000;
+            s.aside[e] = zeros;
+            s.n_aside = e + 1;
+        }
+        for (int i = 0; i < s.n_aside; ++i) if (s.aside_key[i] == 0x7fff) s.aside_key[i] = 0x8000;
+    }
+    __syncthreads();
+
+    // ---- the units of 64 keys that occur, largest first: unit u holds keys 65535 - 64 u and the 63 below ----
+    const int u_here = tid;                                // one to a thread
+    bool any = false;
+    {
+        const uint4* of_unit = reinterpret_cast<const uint4*>(s.counts + (kUnits - 1 - u_here) * (kUnit / 2));
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { const uint4 c = of_unit[(i + lane) & 7]; bits |= c.x | c.y | c.z | c.w; }
+        any = bits != 0;
+        for (int i = 0; i < s.n_aside; ++i) any |= kUnits - 1 - (int)(s.aside_key[i] / kUnit) == u_here;
+    }
+    const uint64_t occupied = __ballot(any);
+    if (lane == 0) { s.occupied[2 * wave] = (uint32_t)__popcll(occupied); }
+    __syncthreads();
+    int n_units = 0, unit_at = 0;
+    for (int w = 0; w < kWaves; ++w) {
+        if (w < wave) unit_at += s.occupied[2 * w];
+        n_units += s.occupied[2 * w];
+    }
+    if (any) s.units[unit_at + __popcll(occupied & ((1ull << lane) - 1))] = (uint16_t)u_here;
+    __syncthreads();
+
+    // ---- the largest value, and the units' masses ----
+    const auto key_in = [&](int i) { return (uint32_t)(kKeys - 1 - kUnit * (int)s.units[i] - lane); };
+    uint32_t top = 0;
+    for (int i = 0; i < n_units && top == 0; ++i) {
+        const uint32_t key = key_in(i);
+        const uint64_t there = __ballot(count_of(key) != 0);
+        if (there != 0) top = (uint32_t)__builtin_amdgcn_readlane((int)key, __builtin_ctzll(there));
+    }
+    if (top == 0) return write_nothing(p, r);
+    const Weights w{K::value(top), of.inverse, weight_bits(row.vocab)};
+    const uint64_t one = 1ull << w.bits;
+    uint64_t heavy = 0;
+    for (int i = wave; i < n_units; i += kWaves) {
+        const uint32_t key = key_in(i), c = count_of(key);
+        const double v = c != 0 ? w.of(K::value(key)) : 0.0;
+        uint64_t mass = (uint64_t)c * w.whole(v);
+        if (of.any_min_p && v >= of.min_p) heavy += mass;
+        uint32_t n = c;
+#pragma unroll
+        for (int by = 32; by > 0; by /= 2) { mass += (uint64_t)__shfl_xor((unsigned long long)mass, by, 64); n += __shfl_xor(n, by, 64); }
+        if (lane == 0) { s.unit_count[i] = n; s.unit_weight[i] = mass; }
+    }
+    if (of.any_min_p) {
+#pragma unroll
+        for (int by = 32; by > 0; by /= 2) heavy += (uint64_t)__shfl_xor((unsigned long long)heavy, by, 64);
+        if (lane == 0) atomicAdd((unsigned long long*)&s.heavy, (unsigned long long)heavy);
+    }
+    __syncthreads();
+    Mass mine{0, 0}, all;
+    if (tid < n_units) mine = Mass{s.unit_count[tid], s.unit_weight[tid]};
+    const Mass before = scan(s.partial, mine, all);
+    if (tid < n_units) { s.unit_count[tid] = (uint32_t)before.count; s.unit_weight[tid] = before.weight; }
+    if (tid == 0) { s.unit_count[n_units] = (uint32_t)all.count; s.unit_weight[n_units] = all.weight; }
+    __syncthreads();
+
+    // ---- searches, by every wavefront for itself ----
+    uint32_t found_key = 0;
+    uint64_t found_nth = 0;                                // of the tokens of that value: 1 ...
+    const auto find = [&](bool by_count, uint64_t goal) {
+        int lo = 0, hi = n_units;                          // the unit behind whose start the goal is not reached yet
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if ((by_count ? (uint64_t)s.unit_count[mid] : s.unit_weight[mid]) < goal) lo = mid; else hi = mid;
+        }
+        const uint32_t key = key_in(lo), c = count_of(key);
+        const uint64_t each = c != 0 ? w.whole_of(K::value(key)) : 0;
+        Mass upto{c, (uint64_t)c * each};
+#pragma unroll
+        for (int by = 1; by < 64; by *= 2) {
+            const uint64_t n = shuffle_up(upto.count, by), m = shuffle_up(upto.weight, by);
+            if (lane >= by) { upto.count += n; upto.weight += m; }
+        }
+        upto.count += s.unit_count[lo];
+        upto.weight += s.unit_weight[lo];
+        const uint64_t reached = __ballot(by_count ? upto.count >= goal : upto.weight >= goal);
+        const int l = reached != 0 ? __builtin_ctzll(reached) : 63;
+        const auto of_lane = [&](uint64_t v) { return (uint64_t)__shfl((unsigned long long)v, l, 64); };
+        const uint64_t n = of_lane(c), weight = of_lane(each);
+        const Mass end{of_lane(upto.count), of_lane(upto.weight)}, start{end.count - n, end.weight - n * weight};
+        uint64_t nth = by_count ? goal - start.count : weight > 0 ? (goal - start.weight + weight - 1) / weight : 1;
+        nth = nth < 1 ? 1 : nth > n ? n : nth;
+        found_key = (uint32_t)__builtin_amdgcn_readlane((int)key, l);
+        found_nth = nth;
+        return Mass{start.count + nth, start.weight + nth * weight};
+    };
+    const uint64_t kept = draw(of, all, one, s.heavy, [&](int step, uint64_t goal) { return find(step == 0, goal); });
+
+    // ---- which of the tokens of that value ----
+    __syncthreads();                                       // nobody counts any more
+    const int shift = max(7, 32 - (int)__builtin_clz((unsigned)row.vocab) - 10);      // indexes in up to 1024 pieces of 2^shift
+    uint32_t* of_piece = s.counts;                         // [1024], and behind these a bit to each token of one piece
+    uint32_t* bitmap = s.counts + kThreads;
+    of_piece[tid] = 0;
+    __syncthreads();
+    const uint32_t raw = K::bits(found_key), other = raw == 0 ? 0x8000u : raw;
+    const uint32_t raw2 = raw * 0x10001u, mask2 = raw == 0 ? 0x7fff7fffu : 0xffffffffu;          // (of zero, both signs)
+    const auto matches = [&](const auto& f) {              // f(index) of every token of that value
+        const auto look = [&](const uint4& u, int v) {
+            const uint32_t x[4] = {(u.x ^ raw2) & mask2, (u.y ^ raw2) & mask2, (u.z ^ raw2) & mask2, (u.w ^ raw2) & mask2};
+            u16x2_t least = __builtin_bit_cast(u16x2_t, x[0]);
+#pragma unroll
+            for (int i = 1; i < 4; ++i) least = __builtin_elementwise_min(least, __builtin_bit_cast(u16x2_t, x[i]));
+            if (least[0] != 0 && least[1] != 0) return;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if ((x[i >> 1] >> (16 * (i & 1)) & 0xffffu) == 0) f(row.head + 8 * v + i);
+        };
+        row.vectors([&](const uint4& u, int v, bool there) { if (there) look(u, v); }, []() {});
+        if (single < row.vocab && (single_bits == raw || single_bits == other)) f(single);
+    };
+    matches([&](int index) { atomicAdd(&of_piece[index >> shift], 1u); });
+    __syncthreads();
+    mine = Mass{of_piece[tid], 0};
+    const uint64_t in_front = scan(s.partial, mine, all).count;
+    if (in_front < found_nth && in_front + mine.count >= found_nth) { s.index = tid; s.number = found_nth - in_front; }
+    __syncthreads();
+    const int piece = s.index;
+    for (int i = tid; i < 1 << shift; i += kThreads) {     // whole wavefronts
+        const int index = (piece << shift) + i;
+        uint32_t x = 0xffffffffu;
+        if (index < row.vocab) { const T v = row.x[index]; x = (__builtin_bit_cast(uint16_t, v) ^ raw) & (mask2 & 0xffffu); }
+        const uint64_t equal = __ballot(x == 0);
+        if (lane == 0) { bitmap[i >> 5] = (uint32_t)equal; bitmap[(i >> 5) + 1] = (uint32_t)(equal >> 32); }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        int left = (int)s.number, i = 0;
+        for (; i < (1 << (shift - 5)) - 1 && left > __popc(bitmap[i]); ++i) left -= __popc(bitmap[i]);
+        uint32_t b = bitmap[i];
+        for (; left > 1; --left) b &= b - 1;
+        p.ids[r] = (piece << shift) + 32 * i + __builtin_ctz(b | 0x80000000u);
+        write_logprob(p, r, w, K::value(found_key), kept);
+    }
+}
+
+template <typename T> void launch(const SampleParams& p, int64_t rows, hipStream_t st) {
+    const dim3 grid((unsigned)rows), block(kThreads);
+    if constexpr (sizeof(T) == 4) sample_kernel<T><<<grid, block, 0, st>>>(p);
+    else sample_keys_kernel<T><<<grid, block, 0, st>>>(p);
 }
 
 }  // namespace
@@ -374,6 +674,6 @@ extern "C" int mi_sample(const mi_sample_args* a) {
     if (!a->logits || !a->uniforms || !a->ids) return mi_fail(MI_E_NULL, "sample: null pointer");
     const SampleParams p{a->logits, a->row_stride, (int)a->vocab, a->uniforms, a->temperatures, a->top_ps, a->min_ps, a->top_ks, a->temperature, a->top_p, a->min_p,
                          a->top_k, a->ids, a->logprobs};
-    MI_DISPATCH_DTYPE(a->dtype, sample_kernel<T><<<dim3((unsigned)a->n_rows), dim3(kThreads), 0, (hipStream_t)a->stream>>>(p));
+    MI_DISPATCH_DTYPE(a->dtype, launch<T>(p, a->n_rows, (hipStream_t)a->stream));
     return mi_check_launch("sample");
 }
