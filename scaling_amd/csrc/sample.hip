@@ -95,28 +95,29 @@ struct Shared {
     uint32_t number;
 };
 
-__device__ __forceinline__ uint64_t shuffle_up(uint64_t v, int by) { return __shfl_up((unsigned long long)v, by, 64); }
+// Sums over lanes 0 .. this one of numbers that add up to less than 2^62, as three of 26 bits (64 of which fit 32): lane exchanges of 64 bits through LDS take
+// longer than the rest of a search.
+__device__ __forceinline__ uint64_t prefix_sum64(uint64_t v) {
+    constexpr uint32_t kPart = (1u << 26) - 1;
+    const uint32_t a = (uint32_t)prefix_sum((int)((uint32_t)v & kPart)), b = (uint32_t)prefix_sum((int)((uint32_t)(v >> 26) & kPart)), c = (uint32_t)prefix_sum((int)(uint32_t)(v >> 52));
+    return ((uint64_t)c << 52) + ((uint64_t)b << 26) + a;
+}
+__device__ __forceinline__ uint64_t of_lane(uint64_t v, int l) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, l);
+}
 
 // Sums over the threads in front of this one, and over all.
 __device__ __forceinline__ Mass scan(Mass* partial, Mass v, Mass& all) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    Mass upto = v;
-#pragma unroll
-    for (int by = 1; by < 64; by *= 2) {
-        const uint64_t c = shuffle_up(upto.count, by), w = shuffle_up(upto.weight, by);
-        if (lane >= by) { upto.count += c; upto.weight += w; }
-    }
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Mass upto{prefix_sum64(v.count), prefix_sum64(v.weight)};
     __syncthreads();
     if (lane == 63) partial[wave] = upto;
     __syncthreads();
-    Mass before{0, 0};
-    all = Mass{0, 0};
-    for (int w = 0; w < kWaves; ++w) {
-        const Mass m = partial[w];
-        if (w < wave) { before.count += m.count; before.weight += m.weight; }
-        all.count += m.count;
-        all.weight += m.weight;
-    }
+    Mass of_wave{0, 0};
+    if (lane < kWaves) of_wave = partial[lane];
+    of_wave = Mass{prefix_sum64(of_wave.count), prefix_sum64(of_wave.weight)};
+    all = Mass{of_lane(of_wave.count, kWaves - 1), of_lane(of_wave.weight, kWaves - 1)};
+    const Mass before = wave > 0 ? Mass{of_lane(of_wave.count, wave - 1), of_lane(of_wave.weight, wave - 1)} : Mass{0, 0};
     return Mass{before.count + upto.count - v.count, before.weight + upto.weight - v.weight};
 }
 
@@ -134,6 +135,14 @@ struct Weights {
     __device__ __forceinline__ uint64_t whole(double w) const { return (uint64_t)__double_as_longlong(ldexp(w, bits) + 0x1p52) & ((1ull << 52) - 1); }
     __device__ __forceinline__ uint64_t whole_of(float x) const { return whole(of(x)); }
 };
+
+// ceil(a / b) for 0 < a < 2^62, 0 < b <= 2^51 and a quotient under 2^31
+__device__ __forceinline__ uint64_t ceil_quotient(uint64_t a, uint64_t b) {
+    uint64_t q = (uint64_t)(uint32_t)((double)a / (double)b);              // or one off
+    q += q * b < a;
+    q += q * b < a;
+    return q > 1 && (q - 1) * b >= a ? q - 1 : q;
+}
 
 // ---- searches -------------------------------------------------------------------------------------------------------------------------------------------
 // Values of an interval of keys in kBins bins, largest first: of equal width in value, or in key.
@@ -276,7 +285,7 @@ template <typename T> struct Search {
     // ... of n equal tokens
     __device__ __forceinline__ Found equals(uint32_t key, uint32_t n, bool by_count, uint64_t goal, Mass before, bool want_index) {
         const uint64_t w = weights.whole_of(key_value(key));
-        uint64_t nth = by_count ? goal - before.count : w > 0 ? (goal - before.weight + w - 1) / w : 1;       // 1 .. n
+        uint64_t nth = by_count ? goal - before.count : w > 0 ? ceil_quotient(goal - before.weight, w) : 1;       // 1 .. n
         nth = nth < 1 ? 1 : nth > n ? n : nth;
         Found f{key, -1, Mass{before.count + nth, before.weight + nth * w}};
         if (!want_index) return f;
@@ -414,27 +423,26 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
 
 // ---- 16-bit logits --------------------------------------------------------------------------------------------------------------------------------------
 // There are 2^16 values, so a workgroup counts how often each occurs in its row: equal tokens weigh the same, and everything else is arithmetic on the
-// few thousand values that occur, with one exponential each.  A second pass over the row
-// finds which of the tokens that equal the drawn value is meant.  Counts of 16 bits, two to a word of LDS, are 128 KB.  One of more than 65535 equal
-// tokens overflows, which shows as counts that do not add up: then once more, in pieces of 32768 tokens with counts over 32767 put aside in between.
-constexpr int kKeys = 1 << 16, kUnit = 64, kUnits = kKeys / kUnit, kAside = MI_SAMPLE_VOCAB_MAX / 32768 + 1;     // (and one more for zeros)
+// few thousand values that occur, with one exponential each.  A second pass over the row finds which of the tokens that equal the drawn value is meant.  Counts of
+// 16 bits, of x and -x in one word of LDS, are 128 KB.  One of more than 65535 equal tokens overflows, which shows as counts that do not add up: then
+// once more, in pieces of 32768 tokens with counts over 32767 put aside in between.
+constexpr int kMagnitudes = 1 << 15, kUnit = 64, kUnits = 2 * kMagnitudes / kUnit, kAside = MI_SAMPLE_VOCAB_MAX / 32768;
 
 struct KeyShared {
-    uint32_t counts[kKeys / 2];                            // of keys 2 i and 2 i + 1
+    uint32_t counts[kMagnitudes];                          // of a magnitude's bits: positive values in the lower half
     uint64_t unit_weight[kUnits + 1];                      // of units of 64 keys that occur, largest first: sums in front; of all
     uint32_t unit_count[kUnits + 1];
     uint16_t units[kUnits];
     Mass partial[kWaves];
-    uint64_t heavy, number;
-    uint32_t occupied[kWaves * 2];
-    int index, n_aside;
-    uint32_t aside_key[kAside], aside[kAside];
+    uint64_t heavy;
+    uint32_t occupied[kWaves];
+    int found, index, nth, n_aside;
+    uint32_t aside[kAside];                                // bits of a value that 32768 more tokens have
 };
 
+// Bits of values to 16-bit keys of the same order; -0 is one below +0, and counted with it.
 template <typename T> struct Key16 {
     static constexpr uint32_t kInf = std::is_same_v<T, _Float16> ? 0x7c00u : 0x7f80u, kTop = kInf | 0x8000u, kNone = 0x7fffu - kInf;     // keys of +inf and -inf
-    // both halves: values to 16-bit keys of the same order; -0 is one below +0
-    static __device__ __forceinline__ uint32_t keys(uint32_t w) { return w ^ (((w >> 15) & 0x00010001u) * 0x7fffu | 0x80008000u); }
     static __device__ __forceinline__ uint32_t bits(uint32_t key) { return (key & 0x8000u) != 0 ? key & 0x7fffu : ~key & 0xffffu; }
     static __device__ __forceinline__ float value(uint32_t key) { return (float)__builtin_bit_cast(T, (uint16_t)bits(key)); }
 };
@@ -442,8 +450,9 @@ typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 
 template <typename T> __global__ __launch_bounds__(kThreads) void sample_keys_kernel(const SampleParams p) {
     using K = Key16<T>;
+    constexpr uint32_t kMinusInf = K::kInf | 0x8000u;
     __shared__ KeyShared s;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t r = blockIdx.x;
     const Row<T> row(p, r);
     const int behind = row.head + row.vecs * 8, single = tid < row.head ? tid : behind + tid - row.head;
@@ -452,98 +461,85 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_keys_ke
     const Parameters of(p, r);
 
     // ---- how often each value occurs ----
-    const auto count_of = [&](uint32_t key) -> uint32_t {
-        if (key > K::kTop || key <= K::kNone) return 0;
-        uint32_t c = (s.counts[key >> 1] >> (16 * (key & 1))) & 0xffffu;
-        for (int i = 0; i < s.n_aside; ++i) c += s.aside_key[i] == key ? s.aside[i] : 0;
-        return c;
-    };
     const auto put_aside = [&]() {
         __syncthreads();
-        for (int i = tid; i < kKeys / 2; i += kThreads) {
+        for (int i = tid; i < kMagnitudes; i += kThreads) {
             const uint32_t both = s.counts[i], over = both & 0x80008000u;
             if (over == 0) continue;
             s.counts[i] = both & 0x7fff7fffu;
             for (int h = 0; h < 2; ++h)
-                if ((over >> (16 * h + 15) & 1) != 0) {
-                    const int e = min(atomicAdd(&s.n_aside, 1), kAside - 1);
-                    s.aside_key[e] = 2 * i + h;
-                    s.aside[e] = 32768;
-                }
+                if ((over >> (16 * h + 15) & 1) != 0) s.aside[min(atomicAdd(&s.n_aside, 1), kAside - 1)] = i | h << 15;
         }
         __syncthreads();
     };
     int pieces = 0;                                        // 1: counts are put aside between pieces
     for (;;) {
-        for (int i = tid; i < kKeys / 8; i += kThreads) reinterpret_cast<uint4*>(s.counts)[i] = make_uint4(0, 0, 0, 0);
-        if (tid == 0) { s.n_aside = 0; s.heavy = 0; s.number = 0; }
+        for (int i = tid; i < kMagnitudes / 4; i += kThreads) reinterpret_cast<uint4*>(s.counts)[i] = make_uint4(0, 0, 0, 0);
+        if (tid == 0) { s.n_aside = s.found = 0; s.heavy = 0; }
         __syncthreads();
-        uint32_t counted = 0;                              // of the wavefront
-        const auto add = [&](uint32_t key, bool there) {
-            there = there && key != K::kNone;              // (masked tokens are many)
-            counted += __popcll(__ballot(there));
-            if (there) atomicAdd(&s.counts[key >> 1], 1u << (16 * (key & 1)));
+        // Masked tokens, -inf, are many: to the lanes' own places among the NaN, where nothing is looked at (the loop is bound by the words that LDS adds to).
+        const auto add = [&](uint32_t at, uint32_t what, bool minus_inf) {
+            if (minus_inf) at = 4 * (K::kInf + 1 + lane);
+            atomicAdd(reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(s.counts) + at), what);
         };
-        const auto add_vector = [&](const uint4& u, bool there) {
-            const uint32_t w[4] = {K::keys(u.x), K::keys(u.y), K::keys(u.z), K::keys(u.w)};
+        row.vectors([&](const uint4& u, int, bool there) {
+            if (!there) return;
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { add(w[i] & 0xffffu, there); add(w[i] >> 16, there); }
-        };
-        row.vectors([&](const uint4& u, int, bool there) { add_vector(u, there); }, [&]() { if (pieces != 0) put_aside(); });
-        add(K::keys(single_bits) & 0xffffu, single < row.vocab);
+            for (int i = 0; i < 4; ++i) {
+                add((w[i] << 2) & 0x1fffcu, __umul24(w[i] >> 15 & 1, 0xffff) + 1, (uint16_t)w[i] == kMinusInf);
+                add((w[i] >> 14) & 0x1fffcu, __umul24(w[i] >> 31, 0xffff) + 1, w[i] >= kMinusInf << 16);       // (and NaN)
+            }
+        }, [&]() { if (pieces != 0) put_aside(); });
+        if (single < row.vocab) add(4 * (single_bits & 0x7fffu), single_bits >> 15 ? 0x10000u : 1u, single_bits == kMinusInf);
         if (pieces != 0) put_aside();                      // (the last ones: fewer than a vector)
+        __syncthreads();
         if (pieces != 0 || row.vocab <= 0xffff) break;
-        if (lane == 0) atomicAdd((unsigned long long*)&s.number, (unsigned long long)counted);
-        __syncthreads();
         uint32_t found = 0;
-        for (int i = tid; i < kKeys / 2; i += kThreads) found += (s.counts[i] & 0xffffu) + (s.counts[i] >> 16);
+        for (int i = tid; i < kMagnitudes / 4; i += kThreads) {
+            const uint4 c = reinterpret_cast<const uint4*>(s.counts)[i];
+            found += (c.x & 0xffffu) + (c.x >> 16) + (c.y & 0xffffu) + (c.y >> 16) + (c.z & 0xffffu) + (c.z >> 16) + (c.w & 0xffffu) + (c.w >> 16);
+        }
         found = group_reduce_bits<64>(found, [](uint32_t a, uint32_t b) { return a + b; });
-        if (lane == 0) atomicAdd((unsigned long long*)&s.number, (unsigned long long)-(long long)found);
+        if (lane == 0) atomicAdd(&s.found, (int)found);
         __syncthreads();
-        if (s.number == 0) break;
+        if (s.found == row.vocab) break;
         pieces = 1;
         __syncthreads();
     }
-    __syncthreads();
-    if (tid == 0) {                                        // -0 is +0
-        const uint32_t zeros = s.counts[0x7fff >> 1] >> 16, plus = s.counts[0x8000 >> 1] & 0xffffu;
-        s.counts[0x7fff >> 1] &= 0xffffu;
-        if (zeros + plus <= 0xffffu) {
-            s.counts[0x8000 >> 1] += zeros;
-        } else {
-            const int e = min(s.n_aside, kAside - 1);
-            s.aside_key[e] = 0x8000;
-            s.aside[e] = zeros;
-            s.n_aside = e + 1;
-        }
-        for (int i = 0; i < s.n_aside; ++i) if (s.aside_key[i] == 0x7fff) s.aside_key[i] = 0x8000;
-    }
-    __syncthreads();
+    const int n_aside = s.n_aside;
+    const auto count_of = [&](uint32_t key) -> uint32_t {
+        if (key > K::kTop || key <= K::kNone || key == 0x7fffu) return 0;
+        const uint32_t bits = K::bits(key), both = s.counts[bits & 0x7fffu];
+        uint32_t c = (bits >> 15 ? 0 : both & 0xffffu) + (bits >> 15 || bits == 0 ? both >> 16 : 0);
+        for (int i = 0; i < n_aside; ++i) c += s.aside[i] == bits || (bits == 0 && s.aside[i] == 0x8000u) ? 32768 : 0;
+        return c;
+    };
 
     // ---- the units of 64 keys that occur, largest first: unit u holds keys 65535 - 64 u and the 63 below ----
-    const int u_here = tid;                                // one to a thread
     bool any = false;
     {
-        const uint4* of_unit = reinterpret_cast<const uint4*>(s.counts + (kUnits - 1 - u_here) * (kUnit / 2));
+        const int from = tid < kUnits / 2 ? kMagnitudes - kUnit * (tid + 1) : kUnit * (tid - kUnits / 2);          // their magnitudes
+        const uint4* of_unit = reinterpret_cast<const uint4*>(s.counts + from);
         uint32_t bits = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { const uint4 c = of_unit[(i + lane) & 7]; bits |= c.x | c.y | c.z | c.w; }
-        any = bits != 0;
-        for (int i = 0; i < s.n_aside; ++i) any |= kUnits - 1 - (int)(s.aside_key[i] / kUnit) == u_here;
+        for (int i = 0; i < kUnit / 4; ++i) { const uint4 c = of_unit[(i + lane) & (kUnit / 4 - 1)]; bits |= c.x | c.y | c.z | c.w; }
+        any = tid < kUnits / 2 ? (bits & 0xffffu) != 0 || (from == 0 && s.counts[0] != 0) : bits >> 16 != 0;
+        for (int i = 0; i < n_aside; ++i) {
+            const uint32_t x = s.aside[i];
+            any |= ((x >> 15 && x != 0x8000u) ? tid >= kUnits / 2 : tid < kUnits / 2) && (int)(x & 0x7fffu) >= from && (int)(x & 0x7fffu) < from + kUnit;
+        }
     }
     const uint64_t occupied = __ballot(any);
-    if (lane == 0) { s.occupied[2 * wave] = (uint32_t)__popcll(occupied); }
+    if (lane == 0) s.occupied[wave] = (uint32_t)__popcll(occupied);
     __syncthreads();
-    int n_units = 0, unit_at = 0;
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) unit_at += s.occupied[2 * w];
-        n_units += s.occupied[2 * w];
-    }
-    if (any) s.units[unit_at + __popcll(occupied & ((1ull << lane) - 1))] = (uint16_t)u_here;
+    const int upto = prefix_sum(lane < kWaves ? (int)s.occupied[lane] : 0), n_units = __builtin_amdgcn_readlane(upto, kWaves - 1);
+    const int unit_at = wave > 0 ? __builtin_amdgcn_readlane(upto, wave - 1) : 0;
+    if (any) s.units[unit_at + __popcll(occupied & ((1ull << lane) - 1))] = (uint16_t)tid;
     __syncthreads();
 
     // ---- the largest value, and the units' masses ----
-    const auto key_in = [&](int i) { return (uint32_t)(kKeys - 1 - kUnit * (int)s.units[i] - lane); };
+    const auto key_in = [&](int i) { return (uint32_t)(2 * kMagnitudes - 1 - kUnit * (int)s.units[i] - lane); };
     uint32_t top = 0;
     for (int i = 0; i < n_units && top == 0; ++i) {
         const uint32_t key = key_in(i);
@@ -554,20 +550,19 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_keys_ke
     const Weights w{K::value(top), of.inverse, weight_bits(row.vocab)};
     const uint64_t one = 1ull << w.bits;
     uint64_t heavy = 0;
+#pragma unroll 2
     for (int i = wave; i < n_units; i += kWaves) {
         const uint32_t key = key_in(i), c = count_of(key);
-        const double v = c != 0 ? w.of(K::value(key)) : 0.0;
-        uint64_t mass = (uint64_t)c * w.whole(v);
-        if (of.any_min_p && v >= of.min_p) heavy += mass;
-        uint32_t n = c;
-#pragma unroll
-        for (int by = 32; by > 0; by /= 2) { mass += (uint64_t)__shfl_xor((unsigned long long)mass, by, 64); n += __shfl_xor(n, by, 64); }
-        if (lane == 0) { s.unit_count[i] = n; s.unit_weight[i] = mass; }
+        const double v = w.of(K::value(key));
+        const uint64_t mass = c != 0 ? (uint64_t)c * w.whole(v) : 0;
+        if (of.any_min_p && c != 0 && v >= of.min_p) heavy += mass;
+        const uint64_t masses = prefix_sum64(mass);
+        const int n = prefix_sum((int)c);
+        if (lane == 63) { s.unit_count[i] = n; s.unit_weight[i] = masses; }
     }
     if (of.any_min_p) {
-#pragma unroll
-        for (int by = 32; by > 0; by /= 2) heavy += (uint64_t)__shfl_xor((unsigned long long)heavy, by, 64);
-        if (lane == 0) atomicAdd((unsigned long long*)&s.heavy, (unsigned long long)heavy);
+        heavy = prefix_sum64(heavy);
+        if (lane == 63) atomicAdd((unsigned long long*)&s.heavy, (unsigned long long)heavy);
     }
     __syncthreads();
     Mass mine{0, 0}, all;
@@ -579,32 +574,26 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_keys_ke
 
     // ---- searches, by every wavefront for itself ----
     uint32_t found_key = 0;
-    uint64_t found_nth = 0;                                // of the tokens of that value: 1 ...
+    int found_nth = 0;                                     // of the tokens of that value: 1 ...
     const auto find = [&](bool by_count, uint64_t goal) {
-        int lo = 0, hi = n_units;                          // the unit behind whose start the goal is not reached yet
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if ((by_count ? (uint64_t)s.unit_count[mid] : s.unit_weight[mid]) < goal) lo = mid; else hi = mid;
+        int unit = n_units - 1;                            // the first unit up to which the goal is reached
+        for (int base = 0; base < n_units; base += 64) {
+            const int i = min(base + lane + 1, n_units);
+            const uint64_t reached = __ballot((by_count ? (uint64_t)s.unit_count[i] : s.unit_weight[i]) >= goal);
+            if (reached != 0) { unit = min(base + (int)__builtin_ctzll(reached), n_units - 1); break; }
         }
-        const uint32_t key = key_in(lo), c = count_of(key);
+        const uint32_t key = key_in(unit), c = count_of(key);
         const uint64_t each = c != 0 ? w.whole_of(K::value(key)) : 0;
-        Mass upto{c, (uint64_t)c * each};
-#pragma unroll
-        for (int by = 1; by < 64; by *= 2) {
-            const uint64_t n = shuffle_up(upto.count, by), m = shuffle_up(upto.weight, by);
-            if (lane >= by) { upto.count += n; upto.weight += m; }
-        }
-        upto.count += s.unit_count[lo];
-        upto.weight += s.unit_weight[lo];
+        const Mass upto{s.unit_count[unit] + (uint64_t)(uint32_t)prefix_sum((int)c), s.unit_weight[unit] + prefix_sum64((uint64_t)c * each)};
         const uint64_t reached = __ballot(by_count ? upto.count >= goal : upto.weight >= goal);
         const int l = reached != 0 ? __builtin_ctzll(reached) : 63;
-        const auto of_lane = [&](uint64_t v) { return (uint64_t)__shfl((unsigned long long)v, l, 64); };
-        const uint64_t n = of_lane(c), weight = of_lane(each);
-        const Mass end{of_lane(upto.count), of_lane(upto.weight)}, start{end.count - n, end.weight - n * weight};
-        uint64_t nth = by_count ? goal - start.count : weight > 0 ? (goal - start.weight + weight - 1) / weight : 1;
+        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)c, l);
+        const uint64_t weight = of_lane(each, l);
+        const Mass start{of_lane(upto.count, l) - n, of_lane(upto.weight, l) - n * weight};
+        uint64_t nth = by_count ? goal - start.count : weight > 0 ? ceil_quotient(goal - start.weight, weight) : 1;
         nth = nth < 1 ? 1 : nth > n ? n : nth;
         found_key = (uint32_t)__builtin_amdgcn_readlane((int)key, l);
-        found_nth = nth;
+        found_nth = (int)nth;
         return Mass{start.count + nth, start.weight + nth * weight};
     };
     const uint64_t kept = draw(of, all, one, s.heavy, [&](int step, uint64_t goal) { return find(step == 0, goal); });
@@ -616,39 +605,34 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_keys_ke
     uint32_t* bitmap = s.counts + kThreads;
     of_piece[tid] = 0;
     __syncthreads();
-    const uint32_t raw = K::bits(found_key), other = raw == 0 ? 0x8000u : raw;
-    const uint32_t raw2 = raw * 0x10001u, mask2 = raw == 0 ? 0x7fff7fffu : 0xffffffffu;          // (of zero, both signs)
-    const auto matches = [&](const auto& f) {              // f(index) of every token of that value
-        const auto look = [&](const uint4& u, int v) {
-            const uint32_t x[4] = {(u.x ^ raw2) & mask2, (u.y ^ raw2) & mask2, (u.z ^ raw2) & mask2, (u.w ^ raw2) & mask2};
-            u16x2_t least = __builtin_bit_cast(u16x2_t, x[0]);
+    const uint32_t raw = K::bits(found_key), mask = raw == 0 ? 0x7fffu : 0xffffu;     // (of zero, both signs)
+    const uint32_t raw2 = raw * 0x10001u, mask2 = mask * 0x10001u;
+    row.vectors([&](const uint4& u, int v, bool there) {
+        const uint32_t x[4] = {(u.x ^ raw2) & mask2, (u.y ^ raw2) & mask2, (u.z ^ raw2) & mask2, (u.w ^ raw2) & mask2};
+        u16x2_t least = __builtin_bit_cast(u16x2_t, x[0]);
 #pragma unroll
-            for (int i = 1; i < 4; ++i) least = __builtin_elementwise_min(least, __builtin_bit_cast(u16x2_t, x[i]));
-            if (least[0] != 0 && least[1] != 0) return;
+        for (int i = 1; i < 4; ++i) least = __builtin_elementwise_min(least, __builtin_bit_cast(u16x2_t, x[i]));
+        if ((least[0] != 0 && least[1] != 0) || !there) return;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if ((x[i >> 1] >> (16 * (i & 1)) & 0xffffu) == 0) f(row.head + 8 * v + i);
-        };
-        row.vectors([&](const uint4& u, int v, bool there) { if (there) look(u, v); }, []() {});
-        if (single < row.vocab && (single_bits == raw || single_bits == other)) f(single);
-    };
-    matches([&](int index) { atomicAdd(&of_piece[index >> shift], 1u); });
+        for (int i = 0; i < 8; ++i)
+            if ((x[i >> 1] >> (16 * (i & 1)) & 0xffffu) == 0) atomicAdd(&of_piece[(row.head + 8 * v + i) >> shift], 1u);
+    }, []() {});
+    if (single < row.vocab && ((single_bits ^ raw) & mask) == 0) atomicAdd(&of_piece[single >> shift], 1u);
     __syncthreads();
-    mine = Mass{of_piece[tid], 0};
-    const uint64_t in_front = scan(s.partial, mine, all).count;
-    if (in_front < found_nth && in_front + mine.count >= found_nth) { s.index = tid; s.number = found_nth - in_front; }
+    const int here = (int)of_piece[tid], in_front = (int)scan(s.partial, Mass{(uint64_t)here, 0}, all).count;
+    if (in_front < found_nth && in_front + here >= found_nth) { s.index = tid; s.nth = found_nth - in_front; }
     __syncthreads();
     const int piece = s.index;
     for (int i = tid; i < 1 << shift; i += kThreads) {     // whole wavefronts
         const int index = (piece << shift) + i;
-        uint32_t x = 0xffffffffu;
-        if (index < row.vocab) { const T v = row.x[index]; x = (__builtin_bit_cast(uint16_t, v) ^ raw) & (mask2 & 0xffffu); }
+        uint32_t x = 1;
+        if (index < row.vocab) { const T v = row.x[index]; x = (__builtin_bit_cast(uint16_t, v) ^ raw) & mask; }
         const uint64_t equal = __ballot(x == 0);
         if (lane == 0) { bitmap[i >> 5] = (uint32_t)equal; bitmap[(i >> 5) + 1] = (uint32_t)(equal >> 32); }
     }
     __syncthreads();
     if (tid == 0) {
-        int left = (int)s.number, i = 0;
+        int left = s.nth, i = 0;
         for (; i < (1 << (shift - 5)) - 1 && left > __popc(bitmap[i]); ++i) left -= __popc(bitmap[i]);
         uint32_t b = bitmap[i];
         for (; left > 1; --left) b &= b - 1;
