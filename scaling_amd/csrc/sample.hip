@@ -44,23 +44,6 @@ template <typename T> struct Row {
         head = to_boundary < vocab ? to_boundary : vocab;
         vecs = (vocab - head) / V;
     }
-    // f(vector, its number, whether there is one) by all threads alike, next() behind every four vectors a thread
-    template <class F, class G> __device__ __forceinline__ void vectors(const F& f, const G& next) const {
-        const uint4* at = reinterpret_cast<const uint4*>(x + head);
-        uint4 u[kAhead];
-#pragma unroll
-        for (int a = 0; a < kAhead; ++a) u[a] = vecs > 0 ? at[min((int)threadIdx.x + a * kThreads, vecs - 1)] : make_uint4(0, 0, 0, 0);
-        for (int v0 = 0; v0 < vecs; v0 += kAhead * kThreads) {
-#pragma unroll
-            for (int a = 0; a < kAhead; ++a) {
-                const int v = v0 + a * kThreads + (int)threadIdx.x;
-                const uint4 now = u[a];
-                u[a] = at[min(v + kAhead * kThreads, vecs - 1)];
-                f(now, v, v < vecs);
-            }
-            next();
-        }
-    }
     // f(value, index) of every element
     template <class F> __device__ __forceinline__ void each(const F& f) const {
         const uint4* at = reinterpret_cast<const uint4*>(x + head);
@@ -106,6 +89,20 @@ __device__ __forceinline__ uint64_t of_lane(uint64_t v, int l) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, l);
 }
 
+// to[0] += v of all lanes: 16 lanes by exchanges, the four sums by LDS.
+__device__ __forceinline__ void row_sum_to(uint64_t* to, uint64_t v) {
+    const auto step = [&](auto ctrl) {
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, decltype(ctrl)::value, 0xf, 0xf, true);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), decltype(ctrl)::value, 0xf, 0xf, true);
+        v += (uint64_t)hi << 32 | lo;
+    };
+    step(std::integral_constant<int, 0xB1>{});            // quad_perm [1, 0, 3, 2]
+    step(std::integral_constant<int, 0x4E>{});            // quad_perm [2, 3, 0, 1]
+    step(std::integral_constant<int, 0x141>{});           // row_half_mirror
+    step(std::integral_constant<int, 0x140>{});           // row_mirror
+    if ((threadIdx.x & 15) == 0) atomicAdd((unsigned long long*)to, (unsigned long long)v);
+}
+
 // Sums over the threads in front of this one, and over all.
 __device__ __forceinline__ Mass scan(Mass* partial, Mass v, Mass& all) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -121,20 +118,49 @@ __device__ __forceinline__ Mass scan(Mass* partial, Mass v, Mass& all) {
     return Mass{before.count + upto.count - v.count, before.weight + upto.weight - v.weight};
 }
 
+__device__ __forceinline__ uint64_t scan(Mass* partial, uint64_t v, uint64_t& all) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint64_t upto = prefix_sum64(v);
+    __syncthreads();
+    if (lane == 63) partial[wave].count = upto;
+    __syncthreads();
+    const uint64_t of_wave = prefix_sum64(lane < kWaves ? partial[lane].count : 0);
+    all = of_lane(of_wave, kWaves - 1);
+    return (wave > 0 ? of_lane(of_wave, wave - 1) : 0) + upto - v;
+}
+
 // ---- weights --------------------------------------------------------------------------------------------------------------------------------------------
+// 2^x for x <= 0, to 2^-47 of it: a whole power of two and the Taylor series of exp(f ln 2) for the rest f, of which 12 terms leave (ln 2 / 2)^12 / 12! = 6e-15.
+// (The library's is half again as long, for the last bits and for arguments that there are none of here.)
+__device__ __forceinline__ double scaled_exp2(double x, int scale) {
+    const double whole = __builtin_rint(x), f = (x - whole) * 0.693147180559945309417;
+    double y = 1.0 / 39916800;
+    constexpr double kTerms[11] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320, 1.0 / 362880, 1.0 / 3628800};
+#pragma unroll
+    for (int i = 10; i >= 0; --i) y = __builtin_fma(y, f, kTerms[i]);
+    return ldexp(y, (int)fmax(whole, -2000.0) + scale);
+}
+
 struct Weights {
     float largest;                                         // value
-    double inverse;                                        // 1 / T
+    double inverse, slope;                                 // 1 / T, and this over ln 2
     int bits;                                              // F
+    __device__ __forceinline__ Weights(float l, double i, int b) : largest(l), inverse(i), slope(i * 1.44269504088896340736), bits(b) {}
     __device__ __forceinline__ double log_of(float x) const {
         if (x == largest) return 0.0;
         return largest == INFINITY ? -INFINITY : ((double)x - (double)largest) * inverse;
     }
-    __device__ __forceinline__ double of(float x) const { return exp(log_of(x)); }
-    // ... times 2^F as a whole number: 2^F <= 2^51, so in a sum with 2^52 it is what the mantissa holds
-    __device__ __forceinline__ uint64_t whole(double w) const { return (uint64_t)__double_as_longlong(ldexp(w, bits) + 0x1p52) & ((1ull << 52) - 1); }
+    // a token's weight times 2^F
+    __device__ __forceinline__ double of(float x) const {
+        if (largest == INFINITY) return x == largest ? ldexp(1.0, bits) : 0.0;
+        return scaled_exp2(((double)x - (double)largest) * slope, bits);
+    }
+    // ... as a whole number: 2^F <= 2^51, so in a sum with 2^52 it is what the mantissa holds
+    __device__ __forceinline__ uint64_t whole(double w) const { return (uint64_t)__double_as_longlong(w + 0x1p52) & ((1ull << 52) - 1); }
     __device__ __forceinline__ uint64_t whole_of(float x) const { return whole(of(x)); }
 };
+// count * w for w < 2^52
+__device__ __forceinline__ uint64_t times(uint32_t count, uint64_t w) { return (uint64_t)count * (uint32_t)w + ((uint64_t)(count * (uint32_t)(w >> 32)) << 32); }
 
 // ceil(a / b) for 0 < a < 2^62, 0 < b <= 2^51 and a quotient under 2^31
 __device__ __forceinline__ uint64_t ceil_quotient(uint64_t a, uint64_t b) {
@@ -404,11 +430,12 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     scan(s.partial, mine, all);
     uint64_t heavy = 0;
     if (of.any_min_p) {
+        const double least = ldexp(of.min_p, w.bits);
         Mass mass{0, 0}, sum;
         row.each([&](float x, int) {
             if (value_key(x) == 0) return;
             const double v = w.of(x);
-            if (v >= of.min_p) mass.weight += w.whole(v);
+            if (v >= least) mass.weight += w.whole(v);
         });
         scan(s.partial, mass, sum);
         heavy = sum.weight;
@@ -423,7 +450,8 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
 
 // ---- 16-bit logits --------------------------------------------------------------------------------------------------------------------------------------
 // There are 2^16 values, so a workgroup counts how often each occurs in its row: equal tokens weigh the same, and everything else is arithmetic on the
-// few thousand values that occur, with one exponential each.  A second pass over the row finds which of the tokens that equal the drawn value is meant.  Counts of
+// few thousand values that occur, with one exponential each.  Up to 16 vectors a thread of the row (131072 logits) stay in
+// registers: a second pass finds which of the tokens that equal the drawn value is meant.  Counts of
 // 16 bits, of x and -x in one word of LDS, are 128 KB.  One of more than 65535 equal tokens overflows, which shows as counts that do not add up: then
 // once more, in pieces of 32768 tokens with counts over 32767 put aside in between.
 constexpr int kMagnitudes = 1 << 15, kUnit = 64, kUnits = 2 * kMagnitudes / kUnit, kAside = MI_SAMPLE_VOCAB_MAX / 32768;
@@ -448,17 +476,41 @@ template <typename T> struct Key16 {
 };
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 
-template <typename T> __global__ __launch_bounds__(kThreads) void sample_keys_kernel(const SampleParams p) {
+template <typename T, int NV> __global__ __launch_bounds__(kThreads) void sample_keys_kernel(const SampleParams p) {
     using K = Key16<T>;
     constexpr uint32_t kMinusInf = K::kInf | 0x8000u;
+    static_assert(K::kInf % kUnit == 0 && NV % 4 == 0, "infinities begin a unit; pieces of four vectors a thread");
     __shared__ KeyShared s;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t r = blockIdx.x;
     const Row<T> row(p, r);
+    const uint4* at = reinterpret_cast<const uint4*>(row.x + row.head);
+    uint4 held[NV];
+    if (row.vecs > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) held[i] = at[min(tid + i * kThreads, row.vecs - 1)];
+    }
     const int behind = row.head + row.vecs * 8, single = tid < row.head ? tid : behind + tid - row.head;
     uint32_t single_bits = 0;
     if (single < row.vocab) { T x = row.x[single]; single_bits = __builtin_bit_cast(uint16_t, x); }
     const Parameters of(p, r);
+    // f(vector, its number) of all vectors, next() behind every four a thread.  (The compiler would otherwise take all vectors at once, and keep what it makes of each for
+    // another round.)
+    const auto vectors = [&](const auto& f, const auto& next) {
+        int n = row.vecs - tid;
+        asm volatile("" : "+v"(n));
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            asm volatile("" : "+v"(held[i].x), "+v"(held[i].y), "+v"(held[i].z), "+v"(held[i].w));
+            if (i * kThreads < n) f(held[i], tid + i * kThreads);
+            if (i % 4 == 3) next();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        for (int v0 = NV * kThreads, i = 0; v0 < row.vecs; v0 += kThreads, ++i) {
+            if (v0 < n) f(at[v0 + tid], v0 + tid);
+            if (i % 4 == 3) next();
+        }
+    };
 
     // ---- how often each value occurs ----
     const auto put_aside = [&]() {
@@ -477,21 +529,31 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_keys_ke
         for (int i = tid; i < kMagnitudes / 4; i += kThreads) reinterpret_cast<uint4*>(s.counts)[i] = make_uint4(0, 0, 0, 0);
         if (tid == 0) { s.n_aside = s.found = 0; s.heavy = 0; }
         __syncthreads();
-        // Masked tokens, -inf, are many: to the lanes' own places among the NaN, where nothing is looked at (the loop is bound by the words that LDS adds to).
-        const auto add = [&](uint32_t at, uint32_t what, bool minus_inf) {
-            if (minus_inf) at = 4 * (K::kInf + 1 + lane);
+        const auto add = [&](uint32_t at, uint32_t negative) {       // (1, or 2^16 for a negative value)
+            uint32_t what;
+            asm("v_mad_u32_u24 %0, %1, %2, 1" : "=v"(what) : "v"(negative), "s"(0xffff));
             atomicAdd(reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(s.counts) + at), what);
         };
-        row.vectors([&](const uint4& u, int, bool there) {
-            if (!there) return;
+        // Masked tokens, -inf, are many: to the lanes' own places among the NaN, where nothing is looked at (words that are added to at once take turns).
+        const auto add_vector = [&](const uint4& u, auto masked) {
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            const uint32_t own = 4 * (K::kInf + 1 + lane);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                add((w[i] << 2) & 0x1fffcu, __umul24(w[i] >> 15 & 1, 0xffff) + 1, (uint16_t)w[i] == kMinusInf);
-                add((w[i] >> 14) & 0x1fffcu, __umul24(w[i] >> 31, 0xffff) + 1, w[i] >= kMinusInf << 16);       // (and NaN)
+                const uint32_t low = (w[i] << 2) & 0x1fffcu, high = (w[i] >> 14) & 0x1fffcu;
+                add(decltype(masked)::value && (w[i] << 16) >= kMinusInf << 16 ? own : low, w[i] >> 15 & 1);
+                add(decltype(masked)::value && w[i] >= kMinusInf << 16 ? own : high, w[i] >> 31);
             }
+        };
+        vectors([&](const uint4& u, int) {
+            u16x2_t most = __builtin_bit_cast(u16x2_t, u.x);
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, u.y));
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, u.z));
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, u.w));
+            if (__any(most[0] >= kMinusInf || most[1] >= kMinusInf)) add_vector(u, std::true_type{});
+            else add_vector(u, std::false_type{});
         }, [&]() { if (pieces != 0) put_aside(); });
-        if (single < row.vocab) add(4 * (single_bits & 0x7fffu), single_bits >> 15 ? 0x10000u : 1u, single_bits == kMinusInf);
+        if (single < row.vocab) add(4 * (single_bits & 0x7fffu), single_bits >> 15);
         if (pieces != 0) put_aside();                      // (the last ones: fewer than a vector)
         __syncthreads();
         if (pieces != 0 || row.vocab <= 0xffff) break;
@@ -516,135 +578,164 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_keys_ke
         return c;
     };
 
-    // ---- the units of 64 keys that occur, largest first: unit u holds keys 65535 - 64 u and the 63 below ----
-    bool any = false;
+    // ---- the units of 64 keys that occur, largest first: unit u holds keys 65535 - 64 u and the 63 below; sums of their counts ----
+    int in_unit = 0;                                       // one unit to a thread
     {
-        const int from = tid < kUnits / 2 ? kMagnitudes - kUnit * (tid + 1) : kUnit * (tid - kUnits / 2);          // their magnitudes
+        const bool positive = tid < kUnits / 2;
+        const int from = positive ? kMagnitudes - kUnit * (tid + 1) : kUnit * (tid - kUnits / 2);                  // their magnitudes
         const uint4* of_unit = reinterpret_cast<const uint4*>(s.counts + from);
-        uint32_t bits = 0;
+        if (from < (int)K::kInf) {                         // (NaN and what stands in for masked tokens lie above)
+            const u16x2_t which = {positive, !positive};
+            for (int i = 0; i < kUnit / 4; ++i) {
+                const uint4 c = of_unit[(i + lane) & (kUnit / 4 - 1)];
+                const uint32_t each[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-        for (int i = 0; i < kUnit / 4; ++i) { const uint4 c = of_unit[(i + lane) & (kUnit / 4 - 1)]; bits |= c.x | c.y | c.z | c.w; }
-        any = tid < kUnits / 2 ? (bits & 0xffffu) != 0 || (from == 0 && s.counts[0] != 0) : bits >> 16 != 0;
+                for (int j = 0; j < 4; ++j) in_unit = (int)__builtin_amdgcn_udot2(__builtin_bit_cast(u16x2_t, each[j]), which, (uint32_t)in_unit, false);
+            }
+        } else if (from == (int)K::kInf && positive) {
+            in_unit = (int)(of_unit[0].x & 0xffffu);
+        }
+        if (from == 0) in_unit += positive ? (int)(s.counts[0] >> 16) : -(int)(s.counts[0] >> 16);                 // -0
         for (int i = 0; i < n_aside; ++i) {
-            const uint32_t x = s.aside[i];
-            any |= ((x >> 15 && x != 0x8000u) ? tid >= kUnits / 2 : tid < kUnits / 2) && (int)(x & 0x7fffu) >= from && (int)(x & 0x7fffu) < from + kUnit;
+            const uint32_t x = s.aside[i] == 0x8000u ? 0 : s.aside[i];
+            if ((x >> 15 == 0) == positive && (int)(x & 0x7fffu) >= from && (int)(x & 0x7fffu) < from + kUnit && (int)(x & 0x7fffu) <= (int)K::kInf - !positive) in_unit += 32768;
         }
     }
-    const uint64_t occupied = __ballot(any);
-    if (lane == 0) s.occupied[wave] = (uint32_t)__popcll(occupied);
+    const uint64_t occupied = __ballot(in_unit > 0);
+    const int counts_upto = prefix_sum(in_unit);
+    if (lane == 63) { s.occupied[wave] = (uint32_t)__popcll(occupied); s.partial[wave].count = (uint64_t)counts_upto; }
     __syncthreads();
-    const int upto = prefix_sum(lane < kWaves ? (int)s.occupied[lane] : 0), n_units = __builtin_amdgcn_readlane(upto, kWaves - 1);
-    const int unit_at = wave > 0 ? __builtin_amdgcn_readlane(upto, wave - 1) : 0;
-    if (any) s.units[unit_at + __popcll(occupied & ((1ull << lane) - 1))] = (uint16_t)tid;
-    __syncthreads();
-
-    // ---- the largest value, and the units' masses ----
-    const auto key_in = [&](int i) { return (uint32_t)(2 * kMagnitudes - 1 - kUnit * (int)s.units[i] - lane); };
-    uint32_t top = 0;
-    for (int i = 0; i < n_units && top == 0; ++i) {
-        const uint32_t key = key_in(i);
-        const uint64_t there = __ballot(count_of(key) != 0);
-        if (there != 0) top = (uint32_t)__builtin_amdgcn_readlane((int)key, __builtin_ctzll(there));
+    const int units_upto = prefix_sum(lane < kWaves ? (int)s.occupied[lane] : 0), counts_before = prefix_sum(lane < kWaves ? (int)s.partial[lane].count : 0);
+    int n_units = __builtin_amdgcn_readlane(units_upto, kWaves - 1);
+    const int n_tokens = __builtin_amdgcn_readlane(counts_before, kWaves - 1);
+    if (in_unit > 0) {
+        const int i = (wave > 0 ? __builtin_amdgcn_readlane(units_upto, wave - 1) : 0) + __popcll(occupied & ((1ull << lane) - 1));
+        s.units[i] = (uint16_t)tid;
+        s.unit_count[i] = counts_upto - in_unit + (wave > 0 ? __builtin_amdgcn_readlane(counts_before, wave - 1) : 0);
     }
-    if (top == 0) return write_nothing(p, r);
-    const Weights w{K::value(top), of.inverse, weight_bits(row.vocab)};
+    if (tid == 0) s.unit_count[n_units] = n_tokens;
+    s.unit_weight[tid] = 0;
+    __syncthreads();
+    if (n_units == 0) return write_nothing(p, r);
+
+    // ---- the largest value, and the units' masses as far as they are asked for ----
+    const auto key_in = [&](int i) { return (uint32_t)(2 * kMagnitudes - 1 - kUnit * (int)s.units[i] - lane); };
+    const uint32_t first = key_in(0), top = (uint32_t)__builtin_amdgcn_readlane((int)first, __builtin_ctzll(__ballot(count_of(first) != 0)));
+    const Weights w(K::value(top), of.inverse, weight_bits(row.vocab));
     const uint64_t one = 1ull << w.bits;
+    const double least = ldexp(of.min_p, w.bits);
+    const bool cut = of.k > 0 && of.k < n_tokens;
+    if (cut || (of.any_min_p && of.top_p_none)) {          // the units in front of the k-th token and, where top-p does not ask for the whole, those with a token of enough weight
+        const bool asked = tid < n_units && !(cut && (int)s.unit_count[tid] >= of.k) &&
+                           !(of.any_min_p && of.top_p_none && tid > 0 && w.of(K::value(min((uint32_t)(2 * kMagnitudes - 1 - kUnit * (int)s.units[tid]), K::kTop))) < 0.5 * least);
+        const uint64_t all = __ballot(asked);
+        if (lane == 0) s.occupied[wave] = (uint32_t)__popcll(all);
+        __syncthreads();
+        n_units = __builtin_amdgcn_readlane(prefix_sum(lane < kWaves ? (int)s.occupied[lane] : 0), kWaves - 1);
+    }
     uint64_t heavy = 0;
-#pragma unroll 2
     for (int i = wave; i < n_units; i += kWaves) {
         const uint32_t key = key_in(i), c = count_of(key);
         const double v = w.of(K::value(key));
-        const uint64_t mass = c != 0 ? (uint64_t)c * w.whole(v) : 0;
-        if (of.any_min_p && c != 0 && v >= of.min_p) heavy += mass;
-        const uint64_t masses = prefix_sum64(mass);
-        const int n = prefix_sum((int)c);
-        if (lane == 63) { s.unit_count[i] = n; s.unit_weight[i] = masses; }
+        const uint64_t mass = c != 0 ? times(c, w.whole(v)) : 0;
+        if (of.any_min_p && c != 0 && v >= least) heavy += mass;
+        row_sum_to(&s.unit_weight[i], mass);
     }
     if (of.any_min_p) {
         heavy = prefix_sum64(heavy);
         if (lane == 63) atomicAdd((unsigned long long*)&s.heavy, (unsigned long long)heavy);
     }
     __syncthreads();
-    Mass mine{0, 0}, all;
-    if (tid < n_units) mine = Mass{s.unit_count[tid], s.unit_weight[tid]};
-    const Mass before = scan(s.partial, mine, all);
-    if (tid < n_units) { s.unit_count[tid] = (uint32_t)before.count; s.unit_weight[tid] = before.weight; }
-    if (tid == 0) { s.unit_count[n_units] = (uint32_t)all.count; s.unit_weight[n_units] = all.weight; }
+    uint64_t mine = tid < n_units ? s.unit_weight[tid] : 0, all;
+    const uint64_t before = scan(s.partial, mine, all);
+    if (tid < n_units) s.unit_weight[tid] = before;
+    if (tid == 0) s.unit_weight[n_units] = all;
     __syncthreads();
 
-    // ---- searches, by every wavefront for itself ----
-    uint32_t found_key = 0;
-    int found_nth = 0;                                     // of the tokens of that value: 1 ...
-    const auto find = [&](bool by_count, uint64_t goal) {
-        int unit = n_units - 1;                            // the first unit up to which the goal is reached
-        for (int base = 0; base < n_units; base += 64) {
-            const int i = min(base + lane + 1, n_units);
-            const uint64_t reached = __ballot((by_count ? (uint64_t)s.unit_count[i] : s.unit_weight[i]) >= goal);
-            if (reached != 0) { unit = min(base + (int)__builtin_ctzll(reached), n_units - 1); break; }
+    // ---- searches, by the first wavefront (others would only take its turns) ----
+    if (wave == 0) {
+        uint32_t found_key = 0;
+        int found_nth = 0;                                 // of the tokens of that value: 1 ...
+        const auto find = [&](bool by_count, uint64_t goal) {
+            int unit = n_units - 1;                        // the first unit up to which the goal is reached
+            for (int base = 0; base < n_units; base += 64) {
+                const int i = min(base + lane + 1, n_units);
+                const uint64_t reached = __ballot((by_count ? (uint64_t)s.unit_count[i] : s.unit_weight[i]) >= goal);
+                if (reached != 0) { unit = min(base + (int)__builtin_ctzll(reached), n_units - 1); break; }
+            }
+            const uint32_t key = key_in(unit), c = count_of(key);
+            const uint64_t each = c != 0 ? w.whole_of(K::value(key)) : 0;
+            const Mass upto{s.unit_count[unit] + (uint64_t)(uint32_t)prefix_sum((int)c), s.unit_weight[unit] + prefix_sum64(times(c, each))};
+            const uint64_t reached = __ballot(by_count ? upto.count >= goal : upto.weight >= goal);
+            const int l = reached != 0 ? __builtin_ctzll(reached) : 63;
+            const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)c, l);
+            const uint64_t weight = of_lane(each, l);
+            const Mass start{of_lane(upto.count, l) - n, of_lane(upto.weight, l) - n * weight};
+            uint64_t nth = by_count ? goal - start.count : weight > 0 ? ceil_quotient(goal - start.weight, weight) : 1;
+            nth = nth < 1 ? 1 : nth > n ? n : nth;
+            found_key = (uint32_t)__builtin_amdgcn_readlane((int)key, l);
+            found_nth = (int)nth;
+            return Mass{start.count + nth, start.weight + nth * weight};
+        };
+        const uint64_t kept = draw(of, Mass{(uint64_t)n_tokens, all}, one, s.heavy, [&](int step, uint64_t goal) { return find(step == 0, goal); });
+        if (lane == 0) {
+            s.found = (int)found_key;
+            s.nth = found_nth;
+            write_logprob(p, r, w, K::value(found_key), kept);
         }
-        const uint32_t key = key_in(unit), c = count_of(key);
-        const uint64_t each = c != 0 ? w.whole_of(K::value(key)) : 0;
-        const Mass upto{s.unit_count[unit] + (uint64_t)(uint32_t)prefix_sum((int)c), s.unit_weight[unit] + prefix_sum64((uint64_t)c * each)};
-        const uint64_t reached = __ballot(by_count ? upto.count >= goal : upto.weight >= goal);
-        const int l = reached != 0 ? __builtin_ctzll(reached) : 63;
-        const uint32_t n = (uint32_t)__builtin_amdgcn_readlane((int)c, l);
-        const uint64_t weight = of_lane(each, l);
-        const Mass start{of_lane(upto.count, l) - n, of_lane(upto.weight, l) - n * weight};
-        uint64_t nth = by_count ? goal - start.count : weight > 0 ? ceil_quotient(goal - start.weight, weight) : 1;
-        nth = nth < 1 ? 1 : nth > n ? n : nth;
-        found_key = (uint32_t)__builtin_amdgcn_readlane((int)key, l);
-        found_nth = (int)nth;
-        return Mass{start.count + nth, start.weight + nth * weight};
-    };
-    const uint64_t kept = draw(of, all, one, s.heavy, [&](int step, uint64_t goal) { return find(step == 0, goal); });
+    }
+    __syncthreads();                                       // (nobody counts any more)
+    const uint32_t found_key = (uint32_t)s.found;
+    const int found_nth = s.nth;
 
     // ---- which of the tokens of that value ----
-    __syncthreads();                                       // nobody counts any more
-    const int shift = max(7, 32 - (int)__builtin_clz((unsigned)row.vocab) - 10);      // indexes in up to 1024 pieces of 2^shift
+    // Pieces of the row in its order: the elements in front of the vectors, up to 1022 pieces of 2^shift vectors, the elements behind them.
+    const int shift = max(4, 32 - (int)__builtin_clz((unsigned)row.vecs | 1) - 9), last_piece = kThreads - 1;
     uint32_t* of_piece = s.counts;                         // [1024], and behind these a bit to each token of one piece
     uint32_t* bitmap = s.counts + kThreads;
     of_piece[tid] = 0;
     __syncthreads();
     const uint32_t raw = K::bits(found_key), mask = raw == 0 ? 0x7fffu : 0xffffu;     // (of zero, both signs)
     const uint32_t raw2 = raw * 0x10001u, mask2 = mask * 0x10001u;
-    row.vectors([&](const uint4& u, int v, bool there) {
-        const uint32_t x[4] = {(u.x ^ raw2) & mask2, (u.y ^ raw2) & mask2, (u.z ^ raw2) & mask2, (u.w ^ raw2) & mask2};
-        u16x2_t least = __builtin_bit_cast(u16x2_t, x[0]);
+    vectors([&](const uint4& u, int v) {
+        const u16x2_t x[4] = {__builtin_bit_cast(u16x2_t, (u.x ^ raw2) & mask2), __builtin_bit_cast(u16x2_t, (u.y ^ raw2) & mask2),
+                              __builtin_bit_cast(u16x2_t, (u.z ^ raw2) & mask2), __builtin_bit_cast(u16x2_t, (u.w ^ raw2) & mask2)};
+        const u16x2_t nearest = __builtin_elementwise_min(__builtin_elementwise_min(x[0], x[1]), __builtin_elementwise_min(x[2], x[3]));
+        if (nearest[0] != 0 && nearest[1] != 0) return;
+        const u16x2_t ones = {1, 1};
+        u16x2_t others = {0, 0};
 #pragma unroll
-        for (int i = 1; i < 4; ++i) least = __builtin_elementwise_min(least, __builtin_bit_cast(u16x2_t, x[i]));
-        if ((least[0] != 0 && least[1] != 0) || !there) return;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if ((x[i >> 1] >> (16 * (i & 1)) & 0xffffu) == 0) atomicAdd(&of_piece[(row.head + 8 * v + i) >> shift], 1u);
+        for (int i = 0; i < 4; ++i) others += __builtin_elementwise_min(x[i], ones);
+        atomicAdd(&of_piece[1 + (v >> shift)], 8u - others[0] - others[1]);
     }, []() {});
-    if (single < row.vocab && ((single_bits ^ raw) & mask) == 0) atomicAdd(&of_piece[single >> shift], 1u);
+    if (single < row.vocab && ((single_bits ^ raw) & mask) == 0) atomicAdd(&of_piece[single < row.head ? 0 : last_piece], 1u);
     __syncthreads();
-    const int here = (int)of_piece[tid], in_front = (int)scan(s.partial, Mass{(uint64_t)here, 0}, all).count;
+    const int here = (int)of_piece[tid], in_front = (int)scan(s.partial, (uint64_t)here, all);
     if (in_front < found_nth && in_front + here >= found_nth) { s.index = tid; s.nth = found_nth - in_front; }
     __syncthreads();
-    const int piece = s.index;
-    for (int i = tid; i < 1 << shift; i += kThreads) {     // whole wavefronts
-        const int index = (piece << shift) + i;
+    const int piece = s.index, from = piece == 0 ? 0 : piece == last_piece ? behind : row.head + ((piece - 1) << (shift + 3));
+    const int upto = piece == 0 ? row.head : piece == last_piece ? row.vocab : min(behind, from + (8 << shift));
+    for (int i = tid; i < 8 << shift; i += kThreads) {     // whole wavefronts
         uint32_t x = 1;
-        if (index < row.vocab) { const T v = row.x[index]; x = (__builtin_bit_cast(uint16_t, v) ^ raw) & mask; }
+        if (from + i < upto) { const T v = row.x[from + i]; x = (__builtin_bit_cast(uint16_t, v) ^ raw) & mask; }
         const uint64_t equal = __ballot(x == 0);
         if (lane == 0) { bitmap[i >> 5] = (uint32_t)equal; bitmap[(i >> 5) + 1] = (uint32_t)(equal >> 32); }
     }
     __syncthreads();
     if (tid == 0) {
         int left = s.nth, i = 0;
-        for (; i < (1 << (shift - 5)) - 1 && left > __popc(bitmap[i]); ++i) left -= __popc(bitmap[i]);
+        for (; i < (1 << (shift - 2)) - 1 && left > __popc(bitmap[i]); ++i) left -= __popc(bitmap[i]);
         uint32_t b = bitmap[i];
         for (; left > 1; --left) b &= b - 1;
-        p.ids[r] = (piece << shift) + 32 * i + __builtin_ctz(b | 0x80000000u);
-        write_logprob(p, r, w, K::value(found_key), kept);
+        p.ids[r] = from + 32 * i + __builtin_ctz(b | 0x80000000u);
     }
 }
 
 template <typename T> void launch(const SampleParams& p, int64_t rows, hipStream_t st) {
     const dim3 grid((unsigned)rows), block(kThreads);
     if constexpr (sizeof(T) == 4) sample_kernel<T><<<grid, block, 0, st>>>(p);
-    else sample_keys_kernel<T><<<grid, block, 0, st>>>(p);
+    else if (p.vocab <= 4 * 8 * kThreads) sample_keys_kernel<T, 4><<<grid, block, 0, st>>>(p);
+    else sample_keys_kernel<T, 16><<<grid, block, 0, st>>>(p);
 }
 
 }  // namespace
