@@ -44,25 +44,45 @@ template <typename T> struct Row {
         head = to_boundary < vocab ? to_boundary : vocab;
         vecs = (vocab - head) / V;
     }
-    // f(value, index) of every element
+    // f(value, index) of every element; the next vectors are under way while these are looked at
     template <class F> __device__ __forceinline__ void each(const F& f) const {
         const uint4* at = reinterpret_cast<const uint4*>(x + head);
-        for (int v0 = threadIdx.x; v0 < vecs; v0 += kAhead * kThreads) {
-            uint4 u[kAhead];
+        const int last = vecs - 1;
+        uint4 u[kAhead];
+        if (vecs > 0) {
 #pragma unroll
-            for (int a = 0; a < kAhead; ++a) u[a] = at[min(v0 + a * kThreads, vecs - 1)];
+            for (int a = 0; a < kAhead; ++a) u[a] = at[min((int)threadIdx.x + a * kThreads, last)];
+        }
+#pragma unroll 1
+        for (int v0 = threadIdx.x; v0 < vecs; v0 += kAhead * kThreads) {
+            uint4 now[kAhead];
+#pragma unroll
+            for (int a = 0; a < kAhead; ++a) {
+                now[a] = u[a];
+                u[a] = at[min(v0 + (kAhead + a) * kThreads, last)];
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int a = 0; a < kAhead; ++a) {
                 const int v = v0 + a * kThreads;
                 if (v >= vecs) break;
                 float e[V];
-                Elem<T>::unpack(u[a], e);
+                Elem<T>::unpack(now[a], e);
 #pragma unroll
                 for (int i = 0; i < V; ++i) f(e[i], head + v * V + i);
             }
         }
         const int behind = head + vecs * V, i = (int)threadIdx.x < head ? (int)threadIdx.x : behind + (int)threadIdx.x - head;
         if (i < vocab) f(Elem<T>::load1(x + i), i);
+    }
+};
+
+// A few tokens of a row that were gathered in LDS, in any order: complements of their keys over their indexes.
+struct Gathered {
+    const uint64_t* tokens;
+    int n;
+    template <class F> __device__ __forceinline__ void each(const F& f) const {
+        for (int i = threadIdx.x; i < n; i += kThreads) f(key_value(~(uint32_t)(tokens[i] >> 32)), (int)(uint32_t)tokens[i]);
     }
 };
 
@@ -89,18 +109,18 @@ __device__ __forceinline__ uint64_t of_lane(uint64_t v, int l) {
     return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)v, l);
 }
 
-// to[0] += v of all lanes: 16 lanes by exchanges, the four sums by LDS.
-__device__ __forceinline__ void row_sum_to(uint64_t* to, uint64_t v) {
+// Sum over the lanes: 16 lanes by exchanges, then the four sums.
+__device__ __forceinline__ uint64_t sum64(uint64_t v) {
     const auto step = [&](auto ctrl) {
         const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, decltype(ctrl)::value, 0xf, 0xf, true);
         const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), decltype(ctrl)::value, 0xf, 0xf, true);
-        v += (uint64_t)hi << 32 | lo;
+        v += __builtin_bit_cast(uint64_t, make_uint2(lo, hi));
     };
     step(std::integral_constant<int, 0xB1>{});            // quad_perm [1, 0, 3, 2]
     step(std::integral_constant<int, 0x4E>{});            // quad_perm [2, 3, 0, 1]
     step(std::integral_constant<int, 0x141>{});           // row_half_mirror
     step(std::integral_constant<int, 0x140>{});           // row_mirror
-    if ((threadIdx.x & 15) == 0) atomicAdd((unsigned long long*)to, (unsigned long long)v);
+    return of_lane(v, 0) + of_lane(v, 16) + of_lane(v, 32) + of_lane(v, 48);
 }
 
 // Sums over the threads in front of this one, and over all.
@@ -170,6 +190,20 @@ __device__ __forceinline__ uint64_t ceil_quotient(uint64_t a, uint64_t b) {
     return q > 1 && (q - 1) * b >= a ? q - 1 : q;
 }
 
+// The smallest lo and the largest hi of all threads.
+__device__ __forceinline__ void range(Shared& s, uint32_t& lo, uint32_t& hi) {
+    lo = group_reduce_bits<64>(lo, [](uint32_t a, uint32_t b) { return min(a, b); });
+    hi = group_reduce_bits<64>(hi, [](uint32_t a, uint32_t b) { return max(a, b); });
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s.partial[threadIdx.x >> 6] = Mass{lo, hi};
+    __syncthreads();
+    const int w = threadIdx.x & (kWaves - 1);
+    lo = group_reduce_bits<16>((uint32_t)s.partial[w].count, [](uint32_t a, uint32_t b) { return min(a, b); });
+    hi = group_reduce_bits<16>((uint32_t)s.partial[w].weight, [](uint32_t a, uint32_t b) { return max(a, b); });
+    static_assert(kWaves == 16);
+    __syncthreads();
+}
+
 // ---- searches -------------------------------------------------------------------------------------------------------------------------------------------
 // Values of an interval of keys in kBins bins, largest first: of equal width in value, or in key.
 struct Bins {
@@ -188,12 +222,14 @@ struct Found {
     Mass upto;                                             // tokens up to it, it included
 };
 
-template <typename T> struct Search {
+template <typename T, class ROW> struct Search {
     Shared& s;
-    const Row<T>& row;
+    const ROW& row;                                        // the tokens that are looked at
+    const Row<T>& whole;
     const Weights& weights;
-    Bins first;                                            // of the whole row
-    bool filled = false;                                   // with them
+    bool weighed;                                          // bins of counts and weights, or of counts alone
+    Bins first;
+    bool filled;                                           // with the first bins
 
     __device__ __forceinline__ void fill(const Bins& bins) {
         __syncthreads();
@@ -201,12 +237,28 @@ template <typename T> struct Search {
         __syncthreads();
         row.each([&](float x, int) {
             const uint32_t key = value_key(x);
-            if (key == 0 || !bins.holds(key)) return;
+            if (!bins.holds(key)) return;
             const int b = bins.of(x, key);
             atomicAdd(&s.count[b], 1u);
-            atomicAdd((unsigned long long*)&s.weight[b], (unsigned long long)weights.whole_of(x));
+            if (weighed) atomicAdd((unsigned long long*)&s.weight[b], (unsigned long long)weights.whole_of(x));
         });
         __syncthreads();
+    }
+    // All tokens of keys lo to hi, lo at least 1, in bins of equal width where their range allows.
+    __device__ __forceinline__ void take(uint32_t lo, uint32_t hi, bool with_weights) {
+        weighed = with_weights;
+        const float top = key_value(hi), range = top - key_value(lo), scale = (float)kBins / range;
+        first = range > 0.f && range < INFINITY && scale < INFINITY ? Bins{lo, hi, top, scale, 0} : Bins{lo, hi, 0.f, 0.f, hi > lo ? max(0, 32 - (int)__builtin_clz(hi - lo) - 12) : 0};
+        fill(first);
+        filled = true;
+    }
+
+    // What all bins hold.
+    __device__ __forceinline__ Mass all() const {
+        Mass mine{0, 0}, sum;
+        for (int i = threadIdx.x; i < kBins; i += kThreads) { mine.count += s.count[i]; mine.weight += s.weight[i]; }
+        scan(s.partial, mine, sum);
+        return sum;
     }
 
     // The bin in which the count or weight reaches `goal`, with what lies in front of it.
@@ -243,22 +295,14 @@ template <typename T> struct Search {
         for (;;) {
             const int bin = bin_of(by_count, goal, before);
             const uint32_t n = s.count[bin];
-            const auto in_bin = [&](float x, uint32_t key) { return key != 0 && bins.holds(key) && bins.of(x, key) == bin; };
+            const auto in_bin = [&](float x, uint32_t key) { return bins.holds(key) && bins.of(x, key) == bin; };
             if (n <= kCandidates) return among(in_bin, (int)n, by_count, goal, before);
             uint32_t lo = 0xffffffffu, hi = 0;
             row.each([&](float x, int) {
                 const uint32_t key = value_key(x);
                 if (in_bin(x, key)) { lo = min(lo, key); hi = max(hi, key); }
             });
-            __syncthreads();
-            if (threadIdx.x == 0) { s.word[2] = 0xffffffffu; s.word[3] = 0; }
-            __syncthreads();
-            atomicMin((unsigned int*)&s.word[2], lo);
-            atomicMax((unsigned int*)&s.word[3], hi);
-            __syncthreads();
-            lo = (uint32_t)s.word[2];
-            hi = (uint32_t)s.word[3];
-            __syncthreads();
+            range(s, lo, hi);
             if (lo == hi) return equals(lo, n, by_count, goal, before, want_index);
             bins = Bins{lo, hi, 0.f, 0.f, max(0, 32 - (int)__builtin_clz(hi - lo) - 12)};
             fill(bins);
@@ -290,7 +334,7 @@ template <typename T> struct Search {
         if ((int)threadIdx.x < n) {
             key = ~(uint32_t)(s.sorted[threadIdx.x] >> 32);
             index = (int)(uint32_t)s.sorted[threadIdx.x];
-            mine = Mass{1, weights.whole_of(key_value(key))};
+            mine = Mass{1, weighed ? weights.whole_of(key_value(key)) : 0};
         }
         Mass at = scan(s.partial, mine, all);
         at.count += before.count;
@@ -316,7 +360,7 @@ template <typename T> struct Search {
         Found f{key, -1, Mass{before.count + nth, before.weight + nth * w}};
         if (!want_index) return f;
         // bins of equal width in the index
-        const int width = (row.vocab + kBins - 1) / kBins;
+        const int width = (whole.vocab + kBins - 1) / kBins;
         filled = false;
         __syncthreads();
         for (int i = threadIdx.x; i < kBins; i += kThreads) { s.count[i] = 0; s.weight[i] = 0; }
@@ -327,8 +371,8 @@ template <typename T> struct Search {
         const int bin = bin_of(true, nth, none);
         if (threadIdx.x == 0) {
             uint64_t left = nth - none.count;
-            for (int i = bin * width; i < row.vocab && i < (bin + 1) * width; ++i)
-                if (value_key(Elem<T>::load1(row.x + i)) == key && --left == 0) { s.word[3] = i; break; }
+            for (int i = bin * width; i < whole.vocab && i < (bin + 1) * width; ++i)
+                if (value_key(Elem<T>::load1(whole.x + i)) == key && --left == 0) { s.word[3] = i; break; }
         }
         __syncthreads();
         f.index = (int)s.word[3];
@@ -359,14 +403,12 @@ struct Parameters {
     }
 };
 
-// What top-k and top-p leave, and with min-p the token: find(by_count, goal) gives the mass up to the first token that reaches the goal.  heavy: the weight of those
-// of at least min_p.  (One call in a loop: the compiler makes three of three, with registers for each.)
-template <class F> __device__ __forceinline__ uint64_t draw(const Parameters& p, const Mass& all, uint64_t one, uint64_t heavy, const F& find) {
-    uint64_t kept = all.weight;
+// The token of what top-k (k > 0), top-p and min-p leave of the weight `kept`, and how much that is: find(step, goal), of step 0 by count, 
+// gives the mass up to the first token that reaches the goal.  heavy: the weight of those of at least min_p.  (One call in a loop: the compiler makes three of three, with registers for each.)
+template <class F> __device__ __forceinline__ uint64_t draw(const Parameters& p, uint64_t kept, int k, uint64_t one, uint64_t heavy, const F& find) {
 #pragma unroll 1
-    for (int step = 0; step < 3; ++step) {
-        uint64_t goal = (uint64_t)p.k;
-        if (step == 0 && !(p.k > 0 && goal < all.count)) continue;
+    for (int step = k > 0 ? 0 : 1; step < 3; ++step) {
+        uint64_t goal = (uint64_t)k;
         if (step == 1) {
             if (p.top_p_one) kept = one;
             if (p.top_p_one || p.top_p_none) continue;
@@ -394,58 +436,126 @@ __device__ __forceinline__ void write_logprob(const SampleParams& p, int64_t r, 
 __device__ __forceinline__ int weight_bits(int vocab) { return min(51, 30 + __builtin_clz((unsigned)vocab)); }      // all tokens' sum stays under 2^62
 
 // ---- 32-bit logits --------------------------------------------------------------------------------------------------------------------------------------
-// One workgroup per row, which it reads once for the range of its values, once for the bins, and once for every bin that is looked into.
+// One workgroup per row, for which every pass over it is an exchange with memory.  The first one counts the tokens by the upper 12 bits of their keys, which
+// tells from where on top-k asks for tokens; without top-p, min-p does too.  If these are few they are gathered in LDS, and all else happens there.
+constexpr int kGathered = 8192, kCoarse = 20;              // bits of a key below its first bin
+
+// All tokens of keys lo to hi in LDS, of which there are no more than fit.
+template <typename T> __device__ __forceinline__ Gathered gather(Shared& s, uint64_t* gathered, const Row<T>& row, uint32_t lo) {
+    __syncthreads();
+    if (threadIdx.x == 0) s.number = 0;
+    __syncthreads();
+    row.each([&](float x, int i) {
+        const uint32_t key = value_key(x);
+        if (key >= lo) gathered[min(atomicAdd(&s.number, 1u), (uint32_t)kGathered - 1)] = (uint64_t)~key << 32 | (uint32_t)i;
+    });
+    __syncthreads();
+    const Gathered few{gathered, min((int)s.number, kGathered)};
+    __syncthreads();
+    return few;
+}
+
+// Of the tokens of keys lo to hi, hi the largest of the row and these the first ones, all or the first k (k > 0).
+template <typename T, class ROW>
+__device__ __forceinline__ void sample_from(Shared& s, uint64_t* gathered, const SampleParams& p, int64_t r, const Parameters& of, const Row<T>& whole, const ROW& row, uint32_t lo,
+                                            uint32_t hi, int k) {
+    const Weights w(key_value(hi), of.inverse, weight_bits(whole.vocab));
+    const uint64_t one = 1ull << w.bits;
+    Search<T, ROW> search{s, row, whole, w, false, {}, false};
+    if (k > 0) {
+        search.take(lo, hi, false);
+        if (search.all().count > (uint64_t)k) lo = search.find(true, (uint64_t)k, false).key;
+        else k = 0;
+    }
+    search.take(lo, hi, true);
+    Mass all = search.all();
+    if (k > 0) all.weight -= (all.count - k) * w.whole_of(key_value(lo));      // equals of the k-th token behind it
+    const auto finish = [&](auto& search) {
+        uint64_t heavy = 0;
+        if (of.any_min_p) {
+            const double least = ldexp(of.min_p, w.bits);
+            uint64_t weight = 0;
+            search.row.each([&](float x, int) {
+                if (value_key(x) < lo) return;
+                const double v = w.of(x);
+                if (v >= least) weight += w.whole(v);
+            });
+            scan(s.partial, weight, heavy);
+        }
+        Found f;
+        const uint64_t kept = draw(of, all.weight, 0, one, heavy, [&](int step, uint64_t goal) { f = search.find(false, goal, step == 2); return f.upto; });
+        if (threadIdx.x == 0) {
+            p.ids[r] = f.index;
+            write_logprob(p, r, w, key_value(f.key), kept);
+        }
+    };
+    if constexpr (std::is_same_v<ROW, Row<T>>) {
+        if (!of.top_p_one && !of.top_p_none) {             // what top-p keeps is often few: no more passes over the row
+            Mass front{0, 0};
+            const double least = ceil((double)all.weight * of.top_p);
+            const int bin = search.bin_of(false, least < 1.0 ? 1 : (uint64_t)least, front);
+            if (front.count + s.count[bin] <= (uint64_t)kGathered) {
+                uint32_t from = 0xffffffffu, none = 0;
+                row.each([&](float x, int) {
+                    const uint32_t key = value_key(x);
+                    if (search.first.holds(key) && search.first.of(x, key) <= bin) from = min(from, key);
+                });
+                range(s, from, none);
+                const Gathered few = gather(s, gathered, whole, from);
+                Search<T, Gathered> rest{s, few, whole, w, false, {}, false};
+                rest.take(from, hi, true);
+                return finish(rest);
+            }
+        }
+    }
+    finish(search);
+}
+
 template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) {
     __shared__ Shared s;
+    __shared__ uint64_t gathered[kGathered];
     const int64_t r = blockIdx.x;
     const Row<T> row(p, r);
     const Parameters of(p, r);
-    // ---- the largest and the smallest value with a weight ----
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.count[i] = 0;
+    __syncthreads();
     uint32_t lo = 0xffffffffu, hi = 0;
     row.each([&](float x, int) {
         const uint32_t key = value_key(x);
-        if (key != 0) { lo = min(lo, key); hi = max(hi, key); }
+        if (key == 0) return;
+        lo = min(lo, key);
+        hi = max(hi, key);
+        atomicAdd(&s.count[(~key) >> kCoarse], 1u);        // largest first
     });
-    if (threadIdx.x == 0) { s.word[2] = 0xffffffffu; s.word[3] = 0; }
-    __syncthreads();
-    atomicMin((unsigned int*)&s.word[2], lo);
-    atomicMax((unsigned int*)&s.word[3], hi);
-    __syncthreads();
-    lo = (uint32_t)s.word[2];
-    hi = (uint32_t)s.word[3];
-    __syncthreads();
+    range(s, lo, hi);
     if (hi == 0) return write_nothing(p, r);
-    const Weights w{key_value(hi), of.inverse, weight_bits(row.vocab)};
-    const uint64_t one = 1ull << w.bits;
-    Search<T> search{s, row, w, Bins{lo, hi, w.largest, 0.f, 0}};
-    const float range = w.largest - key_value(lo);
-    search.first.scale = range > 0.f && range < INFINITY ? (float)kBins / range : 0.f;
-    if (!(search.first.scale < INFINITY)) search.first.scale = 0.f;
-    if (search.first.scale == 0.f) search.first.shift = hi > lo ? max(0, 32 - (int)__builtin_clz(hi - lo) - 12) : 0;
-    // ---- what is kept, and the token ----
-    search.fill(search.first);
-    search.filled = true;
-    Mass mine{0, 0}, all;
-    for (int i = threadIdx.x; i < kBins; i += kThreads) { mine.count += s.count[i]; mine.weight += s.weight[i]; }
-    scan(s.partial, mine, all);
-    uint64_t heavy = 0;
-    if (of.any_min_p) {
-        const double least = ldexp(of.min_p, w.bits);
-        Mass mass{0, 0}, sum;
-        row.each([&](float x, int) {
-            if (value_key(x) == 0) return;
-            const double v = w.of(x);
-            if (v >= least) mass.weight += w.whole(v);
-        });
-        scan(s.partial, mass, sum);
-        heavy = sum.weight;
+    // ---- from where on tokens are asked for, and how many there are ----
+    constexpr int kEach = kBins / kThreads;
+    uint64_t here = 0, n_all;
+    for (int i = 0; i < kEach; ++i) here += s.count[kEach * threadIdx.x + i];
+    const uint64_t front = scan(s.partial, here, n_all);
+    const int k = of.k > 0 && (uint64_t)of.k < n_all ? of.k : 0;
+    if (k > 0) {
+        uint64_t upto = front;
+        for (int i = 0; i < kEach; ++i) {
+            const uint64_t next = upto + s.count[kEach * threadIdx.x + i];
+            if (upto < (uint64_t)k && next >= (uint64_t)k) s.word[0] = (uint32_t)~(((uint64_t)(kEach * threadIdx.x + i + 1) << kCoarse) - 1);      // the smallest key of the bin
+            upto = next;
+        }
+        __syncthreads();
+        lo = max(lo, (uint32_t)s.word[0]);
     }
-    Found f;
-    const uint64_t kept = draw(of, all, one, heavy, [&](int step, uint64_t goal) { f = search.find(step == 0, goal, step == 2); return f.upto; });
-    if (threadIdx.x == 0) {
-        p.ids[r] = f.index;
-        write_logprob(p, r, w, key_value(f.key), kept);
+    if (of.any_min_p && of.top_p_none) {                   // a little below the value that min_p stands for
+        const double largest = (double)key_value(hi), x = largest + log(of.min_p) / of.inverse;
+        const uint32_t key = value_key((float)fmax(x - 1e-6 * fabs(x), -3e38));
+        if (key_value(hi) < INFINITY && of.inverse > 0.0 && key > lo && key <= hi) lo = key;
     }
+    uint64_t mine = 0, n_asked;                            // those of the bins down to the last one's
+    for (int i = 0; i < kEach; ++i)
+        if (kEach * (int)threadIdx.x + i <= (int)(~lo >> kCoarse)) mine += s.count[kEach * threadIdx.x + i];
+    scan(s.partial, mine, n_asked);
+    if (n_asked > kGathered) sample_from<T>(s, gathered, p, r, of, row, row, lo, hi, k);
+    else sample_from<T>(s, gathered, p, r, of, row, gather(s, gathered, row, lo), lo, hi, k);
 }
 
 // ---- 16-bit logits --------------------------------------------------------------------------------------------------------------------------------------
@@ -614,7 +724,6 @@ template <typename T, int NV> __global__ __launch_bounds__(kThreads) void sample
         s.unit_count[i] = counts_upto - in_unit + (wave > 0 ? __builtin_amdgcn_readlane(counts_before, wave - 1) : 0);
     }
     if (tid == 0) s.unit_count[n_units] = n_tokens;
-    s.unit_weight[tid] = 0;
     __syncthreads();
     if (n_units == 0) return write_nothing(p, r);
 
@@ -639,11 +748,12 @@ template <typename T, int NV> __global__ __launch_bounds__(kThreads) void sample
         const double v = w.of(K::value(key));
         const uint64_t mass = c != 0 ? times(c, w.whole(v)) : 0;
         if (of.any_min_p && c != 0 && v >= least) heavy += mass;
-        row_sum_to(&s.unit_weight[i], mass);
+        const uint64_t masses = sum64(mass);
+        if (lane == 0) s.unit_weight[i] = masses;
     }
     if (of.any_min_p) {
-        heavy = prefix_sum64(heavy);
-        if (lane == 63) atomicAdd((unsigned long long*)&s.heavy, (unsigned long long)heavy);
+        heavy = sum64(heavy);
+        if (lane == 0) atomicAdd((unsigned long long*)&s.heavy, (unsigned long long)heavy);
     }
     __syncthreads();
     uint64_t mine = tid < n_units ? s.unit_weight[tid] : 0, all;
@@ -677,7 +787,7 @@ template <typename T, int NV> __global__ __launch_bounds__(kThreads) void sample
             found_nth = (int)nth;
             return Mass{start.count + nth, start.weight + nth * weight};
         };
-        const uint64_t kept = draw(of, Mass{(uint64_t)n_tokens, all}, one, s.heavy, [&](int step, uint64_t goal) { return find(step == 0, goal); });
+        const uint64_t kept = draw(of, all, cut ? of.k : 0, one, s.heavy, [&](int step, uint64_t goal) { return find(step == 0, goal); });
         if (lane == 0) {
             s.found = (int)found_key;
             s.nth = found_nth;
