@@ -901,28 +901,42 @@ template <int D, int NB> int launch(const PagedParams& p, int64_t row_blocks, in
     return mi_check_launch("paged_merge");
 }
 
-// Rows of sequences with a prefix: the partial results of their own keys and of their group's together, 16 lanes to a row of a KV head.
+// Rows of sequences with a prefix: the partial results of their own keys and of their group's together, 16 lanes to a row of a KV head.  Nothing but exchanges with
+// memory, so those that need nothing of each other go together: places and offsets, then all results; whether the token is in a group at all is looked at last.
 template <int D>
 __global__ __launch_bounds__(256) void paged_prefix_merge_kernel(const PrefixParams p) {
-    const int row = blockIdx.x * 16 + (int)(threadIdx.x >> 4), kvh = blockIdx.y, token = divide(row, p.n_rep, p.rep_m), rep = row - token * p.n_rep;
-    if (token >= p.total || token < p.cu[0] || token >= p.cu[p.batch]) return;
-    const int g0 = paged_clamp(p.groups[0], 0, p.batch), g1 = paged_clamp(p.groups[p.n_groups], g0, p.batch);
-    const bool grouped = token >= p.cu[g0] && token < p.cu[g1];
-    RowSum<D> sum;
-    int4 place[2];
-    place[0] = p.places[token];
-    place[1] = grouped ? p.places[p.total + token] : make_int4(0, 0, 0, 0);
+    const int row = min((int)(blockIdx.x * 16 + (threadIdx.x >> 4)), p.total * p.n_rep - 1), kvh = blockIdx.y, token = divide(row, p.n_rep, p.rep_m), rep = row - token * p.n_rep;
+    const int4 place[2] = {p.places[token], p.places[p.total + token]};
+    const int first_token = p.cu[0], end_token = p.cu[p.batch], g0 = paged_clamp(p.groups[0], 0, p.batch), g1 = paged_clamp(p.groups[p.n_groups], g0, p.batch);
+    const int first_grouped = p.cu[g0], end_grouped = p.cu[g1];
+    int splits[2];
+    int64_t first[2], step[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int partial = place[i].x, blocks = place[i].y, splits = place[i].z >> 1, in = (token - place[i].w) * p.n_rep + rep;
+        const int partial = place[i].x, blocks = place[i].y, in = (token - place[i].w) * p.n_rep + rep;
         const bool tiles = (place[i].z & 1) != 0;
         const int shift = tiles ? kTileShift : p.row_block == kRowBlock ? 4 : 5, kept = tiles ? p.tile_rows : p.row_block, block = in >> shift;
-        // (of lengths that overlap: sequences that were left out have nobody's places here)
-        if (splits < 1 || partial < 0 || in < 0 || block >= blocks || in - (block << shift) >= kept || (int64_t)partial + (int64_t)blocks * splits > (tiles ? p.tiles.max_partials : p.rows.max_partials)) continue;
-        const int64_t first = ((int64_t)(partial + block) * p.nkv + kvh) * kept + (in - (block << shift)), step = (int64_t)blocks * p.nkv * kept;
-        sum.template add<false, 8>(tiles ? p.tiles_o : p.rows_o, tiles ? p.tiles_ml : p.rows_ml, first, step, splits);
+        splits[i] = place[i].z >> 1;
+        // (places that nobody left, of a token in no group or of lengths that overlap, hold anything)
+        if (splits[i] < 1 || partial < 0 || in < 0 || block >= blocks || in - (block << shift) >= kept ||
+            (int64_t)partial + (int64_t)blocks * splits[i] > (tiles ? p.tiles.max_partials : p.rows.max_partials)) splits[i] = 0;
+        first[i] = ((int64_t)(partial + block) * p.nkv + kvh) * kept + (in - (block << shift));
+        step[i] = (int64_t)blocks * p.nkv * kept;
     }
-    sum.store(p.o + (int64_t)token * p.o_st + (int64_t)(kvh * p.n_rep + rep) * p.o_sh);
+    RowSum<D> sum[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const bool tiles = (place[i].z & 1) != 0;
+        sum[i].template add<false, 8>(tiles ? p.tiles_o : p.rows_o, tiles ? p.tiles_ml : p.rows_ml, first[i], step[i], splits[i]);
+    }
+    if (blockIdx.x * 16 + (threadIdx.x >> 4) != (unsigned)row || token < first_token || token >= end_token) return;
+    if (token >= first_grouped && token < end_grouped) {
+        float2 ml[1] = {make_float2(sum[1].M, sum[1].L)}, o[1][RowSum<D>::kPairs];
+#pragma unroll
+        for (int k = 0; k < RowSum<D>::kPairs; ++k) o[0][k] = sum[1].O[k];
+        sum[0].add(ml, o);
+    }
+    sum[0].store(p.o + (int64_t)token * p.o_st + (int64_t)(kvh * p.n_rep + rep) * p.o_sh);
 }
 
 // Workgroups per KV head that either kernel's work is cut for.  `items`: sequences x KV heads of the calls, as many as there may be.
@@ -1067,6 +1081,8 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
 // ---- sequences with a shared prefix -------------------------------------------------------------------------------------------------------------------
 namespace {
 
+constexpr int kPrefixPiece = 2;      // tiles of paged_rows that a split has at least
+
 // The plans of a call, and upper bounds of its blocks.  Of `tokens` new tokens, up to `longest` to a sequence.
 struct PrefixPlans {
     Plans plans;
@@ -1076,11 +1092,15 @@ PrefixPlans prefix_plans(int64_t tokens, int64_t batch, int64_t groups, int64_t 
     PrefixPlans o;
     o.plans = make_plans(tokens, batch, std::min(batch, tokens) * nkv, longest, 1 << 30, n_rep, nkv);
     PagedPlan &rows = o.plans.rows, &tiles = o.plans.tiles;
-    rows.rows_up_to = tiles.rows_over = o.plans.row_block;                 // an entry of more rows than a block is paged_tiles'
+    // An entry of more rows than a block is paged_tiles', unless all rows together are so few that it need not be launched.
+    const bool alone = tokens * n_rep <= kRowsAlone;
+    if (alone && tokens * n_rep > kRowBlock) o.plans.row_block = 2 * kRowBlock;
+    rows.rows_up_to = tiles.rows_over = alone ? kRowsAlone : o.plans.row_block;
+    rows.shortest = kPrefixPiece;
     rows.max_n = tiles.max_n = 0x7fffffff;
     o.plans.tile_rows = (int)std::min<int64_t>((tokens * n_rep + 15) / 16 * 16, kTileRows);
     if (tiles.share > 0) tiles.share = tiles.fit;
-    o.row_blocks = std::min(batch, tokens) + std::min(groups, tokens);     // one of each entry with tokens
+    o.row_blocks = std::min(batch, tokens) + std::min(groups, tokens) + (alone ? 2 * (tokens * n_rep / o.plans.row_block) : 0);      // one of each entry with tokens, and of few rows more
     o.tile_blocks = paged_max_blocks<kTileRows>(tiles, tokens, batch, longest, n_rep) + paged_max_blocks<kTileRows>(tiles, tokens, groups, tokens, n_rep);
     return o;
 }
@@ -1095,7 +1115,7 @@ size_t prefix_bytes(int64_t tokens, int64_t row_partials, int row_block, int64_t
 extern "C" size_t mi_paged_prefix_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
     if (tokens <= 0 || tokens > 0x7fffffffLL || batch < 1 || n_groups < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || head_dim <= 0) return 0;
     const int64_t rows = tokens * (n_q_heads / n_kv_heads), cus = mi_compute_units(), many = rows / (kRowBlock + 1);
-    const int64_t row_partials = std::min<int64_t>(batch, tokens) + std::min<int64_t>(n_groups, tokens) + share_of(kRowsMost * cus, n_kv_heads) + 1;
+    const int64_t row_partials = std::min<int64_t>(batch, tokens) + std::min<int64_t>(n_groups, tokens) + 2 * kRowsAlone / kRowBlock + share_of(kRowsMost * cus, n_kv_heads) + 1;
     const int64_t tile_partials = std::min<int64_t>(batch, many) + std::min<int64_t>(n_groups, many) + 2 * (rows / kTileRows) + share_of(cus, n_kv_heads) + 1;
     return prefix_bytes(tokens, row_partials, 2 * kRowBlock, many > 0 ? tile_partials : 0, (int)std::min<int64_t>((rows + 15) / 16 * 16, kTileRows), n_kv_heads, head_dim);
 }

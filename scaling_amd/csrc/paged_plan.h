@@ -65,6 +65,7 @@ struct PagedPlan {
     int fit;                      // workgroups per KV head that run at once: few blocks are cut for no more of them; 0: no such line
     int least;                    // sequences of no more tiles are not split
     int max_slots, max_partials;  // (set by the host) workgroups and partial results per KV head that there are
+    int shortest;                 // tiles that a split has at least (0: 1)
 };
 // u / share for u < 2^31: with m = 2^32 / share + 1 (of a share of 1: 0) the high half of a product is the quotient or one more
 MI_PLAN_FN int paged_by_share(const PagedPlan& p, uint32_t u, uint32_t m) {
@@ -203,6 +204,7 @@ MI_PLAN_FN PagedFound paged_find(LANES& lanes, const PagedPlan& p, uint32_t shar
             if (p.fit) reached += lanes.total(lanes.of([&](const PagedSeq& s, const PagedWork& w) { return paged_reached<TILE>(s, w, causal); }));
         }
         split_tiles = paged_split_tiles(p, units, blocks, most, share_m);
+        split_tiles = split_tiles < p.shortest ? p.shortest : split_tiles;
         if (paged_level(p, blocks, most, reached)) split_tiles = 0x1000000;
 #ifdef __HIPCC__
 #pragma unroll 1
