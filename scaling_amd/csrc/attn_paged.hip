@@ -110,9 +110,93 @@ template <int BLOCK, int TILE> struct PrefixWavefront : Wavefront<BLOCK, TILE> {
         if (e >= x.batch + x.n_groups) this->w.blocks = this->s.n = 0;
     }
 };
-template <int BLOCK, int TILE, PagedOrder ORDER> __device__ __forceinline__ PagedFound find_work(const PrefixParams& p, const PagedPlan& plan, uint32_t share_m, int wanted) {
+// The entry that holds slot `wanted`: the slots of an entry are its blocks * splits, and every split has partial results.  S as in paged_plan.h, of kPrefixPiece tiles at
+// least.  Up to 64 entries every wavefront looks at for itself; of more they take 64 each at a time and tell each other.  (us until a workgroup knows its work, one
+// wavefront after the other over 64 at a time as in paged_find, and so: 8 sequences 2.2, 2.2; 128 sequences 6.0, 4.0 of paged_rows, 4.9, 2.9 of paged_tiles.)
+constexpr int kPrefixPiece = 2;
+struct FindShared {
+    int sums[8][4];
+    PagedFound found;
+};
+template <int BLOCK, int TILE> __device__ __forceinline__ PagedFound find_entry(FindShared& s, const PrefixParams& p, const PagedPlan& plan, uint32_t share_m, int wanted) {
+    const int entries = p.batch + p.n_groups, lane = threadIdx.x & 63;
+    const bool alone = entries <= 64;
+    const int waves = alone ? 1 : blockDim.x >> 6, wave = alone ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), step = 64 * waves;
     PrefixWavefront<BLOCK, TILE> lanes(p, plan);
-    return paged_find<BLOCK, TILE, kAllKept>(lanes, plan, share_m, p.batch + p.n_groups, p.n_rep, p.causal, wanted);
+    // sums (of the last one the maximum) over the wavefronts
+    const auto exchange = [&](int (&v)[4]) {
+        if (alone) return;
+        __syncthreads();
+        if (lane < 4) s.sums[wave][lane] = lane == 0 ? v[0] : lane == 1 ? v[1] : lane == 2 ? v[2] : v[3];
+        __syncthreads();
+        int of_wave[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) of_wave[k] = lane < waves ? s.sums[lane & 7][k] : 0;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) v[k] = __builtin_amdgcn_readlane(prefix_sum(of_wave[k]), 63);
+        v[3] = group_max<64>(of_wave[3]);
+    };
+    int split_tiles = 0x1000000;                           // no sequence has more
+    lanes.look(64 * wave);
+    if (plan.share > 0) {
+        int v[4] = {0, 0, 0, 0};                           // units, blocks, tiles reached, the most tiles
+        for (int base = 64 * wave; base < entries; base += step) {
+            if (base >= step) lanes.look(base);
+            v[0] += __builtin_amdgcn_readlane(prefix_sum(lanes.w.blocks * lanes.w.tiles), 63);
+            v[1] += __builtin_amdgcn_readlane(prefix_sum(lanes.w.blocks), 63);
+            v[2] += __builtin_amdgcn_readlane(prefix_sum(paged_reached<TILE>(lanes.s, lanes.w, p.causal)), 63);
+            v[3] = max(v[3], group_max<64>(lanes.w.blocks > 0 ? lanes.w.tiles : 0));
+        }
+        exchange(v);
+        const int64_t units = (uint32_t)v[0], blocks = v[1], reached = (uint32_t)v[2];
+        split_tiles = max(paged_split_tiles(plan, units, blocks, v[3], share_m), kPrefixPiece);
+        if (paged_level(plan, blocks, v[3], reached)) split_tiles = 0x1000000;
+        for (int i = 0; paged_few(plan, blocks) && i <= kPagedSteps; ++i) {
+            int slots[4] = {0, 0, 0, 0};
+            for (int base = 64 * wave; base < entries; base += step) {
+                if (entries > step) lanes.look(base);
+                slots[0] += __builtin_amdgcn_readlane(prefix_sum(lanes.w.blocks * paged_splits(plan, lanes.w, split_tiles)), 63);
+            }
+            exchange(slots);
+            if (slots[0] <= plan.fit) break;
+            split_tiles = paged_next_tiles(plan, split_tiles, units, blocks, slots[0], i);
+        }
+    }
+    PagedFound f;
+    if (alone) {
+        const int splits = paged_splits(plan, lanes.w, split_tiles), n = lanes.w.blocks * splits, at = prefix_sum(n) - n;
+        const uint64_t holds = __ballot(wanted >= at && wanted < at + n && paged_fits(plan, lanes.w, splits, at, at, true));
+        const int l = holds != 0 ? __builtin_ctzll(holds) : 0, first = lanes.value(at, l);
+        f = PagedFound{holds != 0 ? l : -1, first, lanes.value(splits, l), first, lanes.seq(l), lanes.work(l)};
+        return f;
+    }
+    int slots = 0;
+    for (int base = 0; base < entries; base += step) {
+        if (entries > step) lanes.look(base + 64 * wave);
+        const int splits = paged_splits(plan, lanes.w, split_tiles), n = lanes.w.blocks * splits, upto = prefix_sum(n);
+        __syncthreads();
+        if (lane == 63) s.sums[wave][0] = upto;
+        if (threadIdx.x == 0) s.found.b = -1;
+        __syncthreads();
+        int at = slots + upto - n;
+        for (int w = 0; w < waves; ++w) {
+            at += w < wave ? s.sums[w][0] : 0;
+            slots += s.sums[w][0];
+        }
+        if (wanted >= at && wanted < at + n && paged_fits(plan, lanes.w, splits, at, at, true))
+            s.found = PagedFound{base + 64 * wave + lane, at, splits, at, lanes.s, lanes.w};
+        __syncthreads();
+        if (wanted < slots) break;
+    }
+    f = s.found;
+    const auto uniform = [](int& v) { v = __builtin_amdgcn_readfirstlane(v); };
+    uniform(f.b); uniform(f.at); uniform(f.splits); uniform(f.partial); uniform(f.seq.first); uniform(f.seq.n); uniform(f.seq.ctx); uniform(f.seq.len);
+    uniform(f.work.blocks); uniform(f.work.tiles);
+    return f;
+}
+template <int BLOCK, int TILE, PagedOrder ORDER> __device__ __forceinline__ PagedFound find_work(const PrefixParams& p, const PagedPlan& plan, uint32_t share_m, int wanted) {
+    __shared__ FindShared s;
+    return find_entry<BLOCK, TILE>(s, p, plan, share_m, wanted);
 }
 __device__ __forceinline__ const int32_t* table_of(const PagedParams& p, int b) { return p.table + (int64_t)b * p.table_stride; }
 __device__ __forceinline__ const int32_t* table_of(const PrefixParams& p, int e) {
@@ -901,16 +985,21 @@ template <int D, int NB> int launch(const PagedParams& p, int64_t row_blocks, in
     return mi_check_launch("paged_merge");
 }
 
-// Rows of sequences with a prefix: the partial results of their own keys and of their group's together, 16 lanes to a row of a KV head.  Nothing but exchanges with
-// memory, so those that need nothing of each other go together: places and offsets, then all results; whether the token is in a group at all is looked at last.
+// Rows of sequences with a prefix: the partial results of their own keys and of their group's, a wavefront to a row of a KV head.  Nothing but exchanges with memory, so
+// those that need nothing of each other go together: places and offsets, then all results, 20 of them at a time by four groups of 16 lanes; whether the
+// token is in a group at all is looked at last.  (16 lanes to a row, own results and then the group's: 4096 rows of 17 - 18 results 9.4 us.)
 template <int D>
 __global__ __launch_bounds__(256) void paged_prefix_merge_kernel(const PrefixParams p) {
-    const int row = min((int)(blockIdx.x * 16 + (threadIdx.x >> 4)), p.total * p.n_rep - 1), kvh = blockIdx.y, token = divide(row, p.n_rep, p.rep_m), rep = row - token * p.n_rep;
+    constexpr int kPairs = RowSum<D>::kPairs, kAhead = 5;
+    const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kvh = blockIdx.y, token = divide(row, p.n_rep, p.rep_m), rep = row - token * p.n_rep;
+    const int lane = threadIdx.x & 15, part = (threadIdx.x >> 4) & 3;
+    if (token >= p.total) return;
     const int4 place[2] = {p.places[token], p.places[p.total + token]};
     const int first_token = p.cu[0], end_token = p.cu[p.batch], g0 = paged_clamp(p.groups[0], 0, p.batch), g1 = paged_clamp(p.groups[p.n_groups], g0, p.batch);
-    const int first_grouped = p.cu[g0], end_grouped = p.cu[g1];
+    const bool grouped = token >= p.cu[g0] && token < p.cu[g1];
     int splits[2];
     int64_t first[2], step[2];
+    const float *o[2], *ml[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int partial = place[i].x, blocks = place[i].y, in = (token - place[i].w) * p.n_rep + rep;
@@ -919,24 +1008,40 @@ __global__ __launch_bounds__(256) void paged_prefix_merge_kernel(const PrefixPar
         splits[i] = place[i].z >> 1;
         // (places that nobody left, of a token in no group or of lengths that overlap, hold anything)
         if (splits[i] < 1 || partial < 0 || in < 0 || block >= blocks || in - (block << shift) >= kept ||
-            (int64_t)partial + (int64_t)blocks * splits[i] > (tiles ? p.tiles.max_partials : p.rows.max_partials)) splits[i] = 0;
+            (int64_t)partial + (int64_t)blocks * splits[i] > (tiles ? p.tiles.max_partials : p.rows.max_partials) || (i == 1 && !grouped)) splits[i] = 0;
         first[i] = ((int64_t)(partial + block) * p.nkv + kvh) * kept + (in - (block << shift));
         step[i] = (int64_t)blocks * p.nkv * kept;
+        o[i] = tiles ? p.tiles_o : p.rows_o;
+        ml[i] = tiles ? p.tiles_ml : p.rows_ml;
     }
-    RowSum<D> sum[2];
+    const int n = splits[0] + splits[1];
+    RowSum<D> sum;
+    for (int s0 = 0; s0 < n; s0 += 4 * kAhead) {
+        float2 m[kAhead], v[kAhead][kPairs];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const bool tiles = (place[i].z & 1) != 0;
-        sum[i].template add<false, 8>(tiles ? p.tiles_o : p.rows_o, tiles ? p.tiles_ml : p.rows_ml, first[i], step[i], splits[i]);
-    }
-    if (blockIdx.x * 16 + (threadIdx.x >> 4) != (unsigned)row || token < first_token || token >= end_token) return;
-    if (token >= first_grouped && token < end_grouped) {
-        float2 ml[1] = {make_float2(sum[1].M, sum[1].L)}, o[1][RowSum<D>::kPairs];
+        for (int j = 0; j < kAhead; ++j) {
+            const int s = s0 + 4 * j + part, i = min(s, n - 1);
+            const bool own = i < splits[0];
+            const int64_t at = own ? first[0] + i * step[0] : first[1] + (i - splits[0]) * step[1];
+            m[j] = *reinterpret_cast<const float2*>((own ? ml[0] : ml[1]) + at * 2);
 #pragma unroll
-        for (int k = 0; k < RowSum<D>::kPairs; ++k) o[0][k] = sum[1].O[k];
-        sum[0].add(ml, o);
+            for (int k = 0; k < kPairs; ++k) v[j][k] = *reinterpret_cast<const float2*>((own ? o[0] : o[1]) + at * D + 2 * (lane + 16 * k));
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (s0 + 4 * j + part >= n) {                  // (no weight would not do for an infinite output)
+                m[j] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int k = 0; k < kPairs; ++k) v[j][k] = make_float2(0.f, 0.f);
+            }
+        sum.add(m, v);
     }
-    sum[0].store(p.o + (int64_t)token * p.o_st + (int64_t)(kvh * p.n_rep + rep) * p.o_sh);
+    // the four groups of lanes
+    const float most = quad_max(sum.M), scale = sum.M == -INFINITY ? 0.f : fast_exp2(sum.M - most);
+    sum.L = quad_sum(sum.L * scale);
+#pragma unroll
+    for (int k = 0; k < kPairs; ++k) sum.O[k] = make_float2(quad_sum(sum.O[k].x * scale), quad_sum(sum.O[k].y * scale));
+    if (part == 0 && token >= first_token && token < end_token) sum.store(p.o + (int64_t)token * p.o_st + (int64_t)(kvh * p.n_rep + rep) * p.o_sh);
 }
 
 // Workgroups per KV head that either kernel's work is cut for.  `items`: sequences x KV heads of the calls, as many as there may be.
@@ -1081,8 +1186,6 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
 // ---- sequences with a shared prefix -------------------------------------------------------------------------------------------------------------------
 namespace {
 
-constexpr int kPrefixPiece = 2;      // tiles of paged_rows that a split has at least
-
 // The plans of a call, and upper bounds of its blocks.  Of `tokens` new tokens, up to `longest` to a sequence.
 struct PrefixPlans {
     Plans plans;
@@ -1096,7 +1199,6 @@ PrefixPlans prefix_plans(int64_t tokens, int64_t batch, int64_t groups, int64_t 
     const bool alone = tokens * n_rep <= kRowsAlone;
     if (alone && tokens * n_rep > kRowBlock) o.plans.row_block = 2 * kRowBlock;
     rows.rows_up_to = tiles.rows_over = alone ? kRowsAlone : o.plans.row_block;
-    rows.shortest = kPrefixPiece;
     rows.max_n = tiles.max_n = 0x7fffffff;
     o.plans.tile_rows = (int)std::min<int64_t>((tokens * n_rep + 15) / 16 * 16, kTileRows);
     if (tiles.share > 0) tiles.share = tiles.fit;
@@ -1162,7 +1264,7 @@ int MI_ENTRY(mi_paged_prefix_attn_impl)(const mi_paged_prefix_attn_args* x) {
         constexpr int D = decltype(d)::value;
         const int rc = p.row_block == kRowBlock ? launch_blocks<D, 1>(p, o.row_blocks, o.tile_blocks, st) : launch_blocks<D, 2>(p, o.row_blocks, o.tile_blocks, st);
         if (rc != MI_OK) return rc;
-        paged_prefix_merge_kernel<D><<<dim3((unsigned)((p.total * (int64_t)p.n_rep + 15) / 16), (unsigned)p.nkv), dim3(256), 0, st>>>(p);
+        paged_prefix_merge_kernel<D><<<dim3((unsigned)((p.total * (int64_t)p.n_rep + 3) / 4), (unsigned)p.nkv), dim3(256), 0, st>>>(p);
         return mi_check_launch("paged_prefix_merge");
     };
     switch (a->head_dim) {

@@ -65,7 +65,6 @@ struct PagedPlan {
     int fit;                      // workgroups per KV head that run at once: few blocks are cut for no more of them; 0: no such line
     int least;                    // sequences of no more tiles are not split
     int max_slots, max_partials;  // (set by the host) workgroups and partial results per KV head that there are
-    int shortest;                 // tiles that a split has at least (0: 1)
 };
 // u / share for u < 2^31: with m = 2^32 / share + 1 (of a share of 1: 0) the high half of a product is the quotient or one more
 MI_PLAN_FN int paged_by_share(const PagedPlan& p, uint32_t u, uint32_t m) {
@@ -135,25 +134,25 @@ template <int BLOCK, int TILE> MI_PLAN_FN int paged_above(const PagedSeq& s, con
     const int64_t below = over * n_rep / BLOCK;
     return below >= w.blocks ? 0 : w.blocks - (int)below;
 }
-// Whether a launch computes a sequence whose first slot and first partial result (`kept`: has any) are these: all of its splits or none.
-MI_PLAN_FN bool paged_fits(const PagedPlan& p, const PagedWork& w, int splits, int slot, int partial, bool kept) {
+// Whether a launch computes a sequence whose first slot and first partial result are these: all of its splits or none.
+// kept: a single split has a partial result too.
+MI_PLAN_FN bool paged_fits(const PagedPlan& p, const PagedWork& w, int splits, int slot, int partial, bool kept = false) {
     const int64_t n = (int64_t)w.blocks * splits;
-    return slot >= 0 && slot + n <= p.max_slots && (!kept || (partial >= 0 && partial + n <= p.max_partials));
+    return slot >= 0 && slot + n <= p.max_slots && ((splits == 1 && !kept) || (partial >= 0 && partial + n <= p.max_partials));
 }
-MI_PLAN_FN bool paged_fits(const PagedPlan& p, const PagedWork& w, int splits, int slot, int partial) { return paged_fits(p, w, splits, slot, partial, splits > 1); }
 
 // A sequence as one workgroup meets it.
 struct PagedFound {
     int b;             // -1: none
     int at;            // first slot of the sequence's blocks * splits; of split blocks the first of these; longest first: as if it were one
     int splits;
-    int partial;       // first partial result of the sequence (splits > 1, or kAllKept)
+    int partial;       // first partial result of the sequence (splits > 1)
     PagedSeq seq;
     PagedWork work;
 };
 // What is looked for: a slot, i.e. one of the blocks * splits of a sequence; a slot, where nothing is split longest block first; or one of all blocks that
-// have several splits.  kAllKept: as kSlots, where sequences of a single split have partial results too.
-enum PagedOrder { kSlots, kLongestFirst, kSplitBlocks, kAllKept };
+// have several splits.
+enum PagedOrder { kSlots, kLongestFirst, kSplitBlocks };
 
 // The sequence that holds `wanted`.  share_m: of paged_by_share.  It is looked for in groups of 64 sequences, one to a lane of LANES (a wavefront, or an array), which has
 //     look(base)          takes up sequences base .. base + 63; behind the last one they have no blocks
@@ -204,7 +203,6 @@ MI_PLAN_FN PagedFound paged_find(LANES& lanes, const PagedPlan& p, uint32_t shar
             if (p.fit) reached += lanes.total(lanes.of([&](const PagedSeq& s, const PagedWork& w) { return paged_reached<TILE>(s, w, causal); }));
         }
         split_tiles = paged_split_tiles(p, units, blocks, most, share_m);
-        split_tiles = split_tiles < p.shortest ? p.shortest : split_tiles;
         if (paged_level(p, blocks, most, reached)) split_tiles = 0x1000000;
 #ifdef __HIPCC__
 #pragma unroll 1
@@ -224,7 +222,7 @@ MI_PLAN_FN PagedFound paged_find(LANES& lanes, const PagedPlan& p, uint32_t shar
         if (batch > 64 || p.share == 0) lanes.look(base);
         const auto splits = lanes.of([&](const PagedSeq&, const PagedWork& w) { return paged_splits(p, w, split_tiles); });
         const auto n = lanes.of(splits, [](const PagedWork& w, int i) { return w.blocks * i; });
-        const auto part = lanes.of(splits, [](const PagedWork& w, int i) { return ORDER == kAllKept || i > 1 ? w.blocks * i : 0; });
+        const auto part = lanes.of(splits, [](const PagedWork& w, int i) { return i > 1 ? w.blocks * i : 0; });
         const auto split = lanes.of(splits, [](const PagedWork& w, int i) { return i > 1 ? w.blocks : 0; });
         // (all sums before they are asked for: none waits for another's)
         const auto n_upto = lanes.upto(n), part_upto = lanes.upto(part), split_upto = ORDER == kSplitBlocks ? lanes.upto(split) : split;
@@ -237,7 +235,7 @@ MI_PLAN_FN PagedFound paged_find(LANES& lanes, const PagedPlan& p, uint32_t shar
             f.partial = partials + lanes.value(part_upto - part, l);
             f.seq = lanes.seq(l);
             f.work = lanes.work(l);
-            if (!paged_fits(p, f.work, f.splits, slot, f.partial, ORDER == kAllKept || f.splits > 1)) f.b = -1;
+            if (!paged_fits(p, f.work, f.splits, slot, f.partial)) f.b = -1;
             return f;
         }
         slots += lanes.value(n_upto, 63);
