@@ -1195,14 +1195,17 @@ PrefixPlans prefix_plans(int64_t tokens, int64_t batch, int64_t groups, int64_t 
     PrefixPlans o;
     o.plans = make_plans(tokens, batch, std::min(batch, tokens) * nkv, longest, 1 << 30, n_rep, nkv);
     PagedPlan &rows = o.plans.rows, &tiles = o.plans.tiles;
-    // An entry of more rows than a block is paged_tiles', unless all rows together are so few that it need not be launched.
+    // An entry of more rows than a block is paged_tiles', except where that launch would be for little: all rows together are few, or groups of about one size have no more
+    // than one and a half blocks.  (us: 16 groups of 16 - 20 rows over 1000 keys 46.0, with two blocks to a group 40.3; 8 of 24 over 1500 keys of 16 heads of 64, 64.8 and 60.3; 8
+    // of 32 over 4000 keys 57.4 and 74.  64 rows in 8 groups in blocks of 16 and of 32: 28.0 and 32.7, in one group 29.4 and 23.0.)
+    const int64_t average = (tokens * n_rep + groups - 1) / std::max<int64_t>(groups, 1), entries = std::min(batch, tokens) + std::min(groups, tokens);
     const bool alone = tokens * n_rep <= kRowsAlone;
-    if (alone && tokens * n_rep > kRowBlock) o.plans.row_block = 2 * kRowBlock;
-    rows.rows_up_to = tiles.rows_over = alone ? kRowsAlone : o.plans.row_block;
+    if (alone && average > kRowBlock) o.plans.row_block = 2 * kRowBlock;
+    rows.rows_up_to = tiles.rows_over = alone ? kRowsAlone : average <= 3 * kRowBlock / 2 ? 2 * kRowBlock : o.plans.row_block;
     rows.max_n = tiles.max_n = 0x7fffffff;
     o.plans.tile_rows = (int)std::min<int64_t>((tokens * n_rep + 15) / 16 * 16, kTileRows);
     if (tiles.share > 0) tiles.share = tiles.fit;
-    o.row_blocks = std::min(batch, tokens) + std::min(groups, tokens) + (alone ? 2 * (tokens * n_rep / o.plans.row_block) : 0);      // one of each entry with tokens, and of few rows more
+    o.row_blocks = alone ? entries + 2 * (tokens * n_rep / o.plans.row_block) : entries * (rows.rows_up_to / o.plans.row_block);
     o.tile_blocks = paged_max_blocks<kTileRows>(tiles, tokens, batch, longest, n_rep) + paged_max_blocks<kTileRows>(tiles, tokens, groups, tokens, n_rep);
     return o;
 }
@@ -1213,11 +1216,12 @@ size_t prefix_bytes(int64_t tokens, int64_t row_partials, int row_block, int64_t
 }  // namespace
 
 #ifndef MI_ELEM_F16
-// For every max_q_len: entries with a block of rows each, blocks of 256 of those with more than 16, and the splits that either share adds.
+// For every max_q_len: entries with two blocks of rows each (and the few of a call without paged_tiles), blocks of 256 of those with more than 16, and the splits that either
+// share adds.
 extern "C" size_t mi_paged_prefix_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
     if (tokens <= 0 || tokens > 0x7fffffffLL || batch < 1 || n_groups < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || head_dim <= 0) return 0;
     const int64_t rows = tokens * (n_q_heads / n_kv_heads), cus = mi_compute_units(), many = rows / (kRowBlock + 1);
-    const int64_t row_partials = std::min<int64_t>(batch, tokens) + std::min<int64_t>(n_groups, tokens) + 2 * kRowsAlone / kRowBlock + share_of(kRowsMost * cus, n_kv_heads) + 1;
+    const int64_t row_partials = 2 * (std::min<int64_t>(batch, tokens) + std::min<int64_t>(n_groups, tokens)) + 2 * kRowsAlone / kRowBlock + share_of(kRowsMost * cus, n_kv_heads) + 1;
     const int64_t tile_partials = std::min<int64_t>(batch, many) + std::min<int64_t>(n_groups, many) + 2 * (rows / kTileRows) + share_of(cus, n_kv_heads) + 1;
     return prefix_bytes(tokens, row_partials, 2 * kRowBlock, many > 0 ? tile_partials : 0, (int)std::min<int64_t>((rows + 15) / 16 * 16, kTileRows), n_kv_heads, head_dim);
 }
