@@ -622,27 +622,37 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> op_paged_step(const Tensor& n
                     (table.stride(1) == 1 || table.size(1) <= 1) && (table.stride(0) >= table.size(1) || batch <= 1),
                 "paged_step: page_table is int32 [batch, max_pages] with contiguous rows of its own memory");
     for (const int64_t n : {batch, table.size(1), page_size, free_pages.size(0), tokens, max_ctx}) TORCH_CHECK(n >= 0 && n <= INT32_MAX, "paged_step: a size of ", n);
-    // what is written besides lengths and state themselves has to be memory of its own
-    const Tensor* const read[] = {&new_tokens, &lengths, &state, offset.has_value() ? &*offset : &new_tokens};
-    const Tensor* const written[] = {&ctx_len, &state_out, &table, &free_pages};
-    for (const Tensor* w : written)
-        for (const Tensor* r : read) {
-            if ((w == &ctx_len && r == &lengths && ptr(*w) == ptr(*r)) || (w == &state_out && r == &state && ptr(*w) == ptr(*r))) continue;
-            at::assert_no_overlap(*w, *r);
-        }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < i; ++j) at::assert_no_overlap(*written[i], *written[j]);
+    // What is written, but lengths and state themselves, has to be memory of its own.  (By spans; at::assert_no_overlap takes longer than the kernel does.)
+    struct Span { const char *from, *to; };
+    const auto span = [](const void* p, int64_t n) { return Span{static_cast<const char*>(p), static_cast<const char*>(p) + 4 * n}; };
+    const Span read[] = {span(a.new_tokens, batch), span(a.lengths, batch), span(a.state, 2), span(a.position_offset, a.position_offset ? batch : 0)};
+    const Span written[] = {span(a.ctx_len, batch), span(a.state_out, 2), span(ptr(table), batch > 0 && table.size(1) > 0 ? (batch - 1) * table.stride(0) + table.size(1) : 0),
+                            span(a.free_pages, free_pages.size(0))};
+    const auto meet = [](const Span& x, const Span& y) { return x.from < y.to && y.from < x.to; };
+    for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < 4; ++j)
+            TORCH_CHECK(!meet(written[i], read[j]) || (i < 2 && j == i + 1 && written[i].from == read[j].from), "paged_step: tensors that are written share memory with others");
+        for (int j = 0; j < i; ++j) TORCH_CHECK(!meet(written[i], written[j]), "paged_step: tensors that are written share memory");
+    }
     a.page_table = static_cast<int32_t*>(ptr(table)); a.page_table_stride = table.stride(0);
     a.batch = (int32_t)batch; a.max_pages = (int32_t)table.size(1); a.page_size = (int32_t)page_size; a.n_free = (int32_t)free_pages.size(0);
     a.tokens = (int32_t)tokens; a.max_ctx = (int32_t)max_ctx;
     Launch l(new_tokens);
-    const auto longs = new_tokens.options().dtype(at::kLong);
-    const Tensor cu = at::empty({batch + 1}, new_tokens.options()), of_tokens = at::empty({3, tokens}, longs), last = at::empty({batch}, longs);
-    a.cu_seqlens = static_cast<int32_t*>(ptr(cu)); a.last = last.data_ptr<int64_t>();
-    a.position_ids = of_tokens.data_ptr<int64_t>(); a.slots = a.position_ids + tokens; a.sequences = a.slots + tokens;
+    // One allocation for the five results, each a tensor over its part of it (as many allocations take longer than the launch).
+    const Tensor whole = at::empty({3 * tokens + batch + (batch + 2) / 2}, new_tokens.options().dtype(at::kLong));
+    const auto part = [&](at::ScalarType type, int64_t from, int64_t n) {
+        auto t = c10::make_intrusive<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(type));
+        t->set_storage_offset(from);
+        t->set_sizes_contiguous({n});
+        return Tensor(std::move(t));
+    };
+    const Tensor positions = part(at::kLong, 0, tokens), slots = part(at::kLong, tokens, tokens), sequences = part(at::kLong, 2 * tokens, tokens);
+    const Tensor last = part(at::kLong, 3 * tokens, batch), cu = part(at::kInt, 2 * (3 * tokens + batch), batch + 1);
+    a.cu_seqlens = static_cast<int32_t*>(ptr(cu)); a.last = static_cast<int64_t*>(ptr(last));
+    a.position_ids = static_cast<int64_t*>(ptr(positions)); a.slots = static_cast<int64_t*>(ptr(slots)); a.sequences = static_cast<int64_t*>(ptr(sequences));
     a.stream = l.stream;
     check(mi_paged_step(&a), "mi_paged_step");
-    return {cu, of_tokens[0], of_tokens[1], of_tokens[2], last};
+    return {cu, positions, slots, sequences, last};
 }
 
 // Whether two [tokens, heads, features] tensors of one shape with contiguous features share memory.  Slices of one tensor lie between each other's rows: of equal

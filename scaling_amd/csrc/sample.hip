@@ -430,7 +430,7 @@ __device__ __forceinline__ void write_nothing(const SampleParams& p, int64_t r) 
     p.ids[r] = 0;
     if (p.logprobs) p.logprobs[r] = -INFINITY;
 }
-__device__ __forceinline__ void write_logprob(const SampleParams& p, int64_t r, const Weights& w, float x, uint64_t kept) {
+__device__ __forceinline__ void write_logprob(const SampleParams& p, int64_t r, const Weights& w, float x, uint64_t kept) {      // (by one thread)
     if (p.logprobs) p.logprobs[r] = (float)(w.log_of(x) - log(ldexp((double)kept, -w.bits)));
 }
 __device__ __forceinline__ int weight_bits(int vocab) { return min(51, 30 + __builtin_clz((unsigned)vocab)); }      // all tokens' sum stays under 2^62
@@ -511,6 +511,45 @@ __device__ __forceinline__ void sample_from(Shared& s, uint64_t* gathered, const
     finish(search);
 }
 
+// The same of up to kCandidates tokens that were gathered, one to a thread: in order, their running sums answer everything.
+__device__ __forceinline__ void sample_few(Shared& s, const SampleParams& p, int64_t r, const Parameters& of, int vocab, const Gathered& few, uint32_t hi, int k) {
+    const Weights w(key_value(hi), of.inverse, weight_bits(vocab));
+    const uint64_t one = 1ull << w.bits;
+    const int i = threadIdx.x;
+    const bool there = i < few.n;
+    if (there) {
+        const uint64_t c = few.tokens[i];
+        int rank = 0;
+        for (int j = 0; j < few.n; ++j) rank += few.tokens[j] < c;
+        s.sorted[rank] = c;
+    }
+    __syncthreads();
+    const uint64_t token = there ? s.sorted[i] : 0;
+    const float x = key_value(~(uint32_t)(token >> 32));
+    const double v = there ? w.of(x) : 0.0;
+    const uint64_t mine = there ? w.whole(v) : 0;
+    uint64_t all;
+    const uint64_t before = scan(s.partial, mine, all), upto = before + mine;
+    if (of.any_min_p && there && v >= ldexp(of.min_p, w.bits)) atomicMax((unsigned long long*)&s.word[1], (unsigned long long)upto);      // (cleared by the caller)
+    if (k > 0 && k <= few.n && i == k - 1) s.word[2] = upto;
+    __syncthreads();
+    const uint64_t heavy = s.word[1];
+    if (k > 0 && k <= few.n) all = s.word[2];
+    int found = 0;
+    const uint64_t kept = draw(of, all, 0, one, heavy, [&](int step, uint64_t goal) {
+        if (there && before < goal && upto >= goal) { s.word[0] = upto; s.number = i; }
+        __syncthreads();
+        found = (int)s.number;
+        const uint64_t reached = s.word[0];
+        __syncthreads();
+        return Mass{0, reached};
+    });
+    if (i == found && there) {
+        p.ids[r] = (int64_t)(uint32_t)token;
+        write_logprob(p, r, w, x, kept);
+    }
+}
+
 template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) {
     __shared__ Shared s;
     __shared__ uint64_t gathered[kGathered];
@@ -554,8 +593,11 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     for (int i = 0; i < kEach; ++i)
         if (kEach * (int)threadIdx.x + i <= (int)(~lo >> kCoarse)) mine += s.count[kEach * threadIdx.x + i];
     scan(s.partial, mine, n_asked);
-    if (n_asked > kGathered) sample_from<T>(s, gathered, p, r, of, row, row, lo, hi, k);
-    else sample_from<T>(s, gathered, p, r, of, row, gather(s, gathered, row, lo), lo, hi, k);
+    if (n_asked > kGathered) return sample_from<T>(s, gathered, p, r, of, row, row, lo, hi, k);
+    if (threadIdx.x == 0) s.word[1] = 0;
+    const Gathered few = gather(s, gathered, row, lo);
+    if (few.n <= kCandidates) sample_few(s, p, r, of, row.vocab, few, hi, k);
+    else sample_from<T>(s, gathered, p, r, of, row, few, lo, hi, k);
 }
 
 // ---- 16-bit logits --------------------------------------------------------------------------------------------------------------------------------------
