@@ -8,6 +8,8 @@
 // one row of some thousands where 32 bits are all there is.
 #include "common.h"
 
+#include <stddef.h>
+
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
@@ -210,6 +212,11 @@ struct Bins {
     uint32_t lo, hi;
     float top, scale;                                      // scale 0: by key
     int shift;
+    // of equal width in value where the range allows
+    static __device__ __forceinline__ Bins over(uint32_t lo, uint32_t hi) {
+        const float top = key_value(hi), range = top - key_value(lo), scale = (float)kBins / range;
+        return range > 0.f && range < INFINITY && scale < INFINITY ? Bins{lo, hi, top, scale, 0} : Bins{lo, hi, 0.f, 0.f, hi > lo ? max(0, 32 - (int)__builtin_clz(hi - lo) - 12) : 0};
+    }
     __device__ __forceinline__ bool holds(uint32_t key) const { return key >= lo && key <= hi; }
     __device__ __forceinline__ int of(float x, uint32_t key) const {
         return scale > 0.f ? min((int)((top - x) * scale), kBins - 1) : (int)((hi - key) >> shift);
@@ -244,11 +251,10 @@ template <typename T, class ROW> struct Search {
         });
         __syncthreads();
     }
-    // All tokens of keys lo to hi, lo at least 1, in bins of equal width where their range allows.
+    // All tokens of keys lo to hi, lo at least 1.
     __device__ __forceinline__ void take(uint32_t lo, uint32_t hi, bool with_weights) {
         weighed = with_weights;
-        const float top = key_value(hi), range = top - key_value(lo), scale = (float)kBins / range;
-        first = range > 0.f && range < INFINITY && scale < INFINITY ? Bins{lo, hi, top, scale, 0} : Bins{lo, hi, 0.f, 0.f, hi > lo ? max(0, 32 - (int)__builtin_clz(hi - lo) - 12) : 0};
+        first = Bins::over(lo, hi);
         fill(first);
         filled = true;
     }
@@ -438,7 +444,7 @@ __device__ __forceinline__ int weight_bits(int vocab) { return min(51, 30 + __bu
 // ---- 32-bit logits --------------------------------------------------------------------------------------------------------------------------------------
 // One workgroup per row, for which every pass over it is an exchange with memory.  The first one counts the tokens by the upper 12 bits of their keys, which
 // tells from where on top-k asks for tokens; without top-p, min-p does too.  If these are few they are gathered in LDS, and all else happens there.
-constexpr int kGathered = 8192, kCoarse = 20;              // bits of a key below its first bin
+constexpr int kGathered = 6144, kCoarse = 19, kCoarseBins = 1 << (32 - kCoarse), kEach = kGathered / kThreads;      // bits of a key below its first bin
 
 // All tokens of keys lo to hi in LDS, of which there are no more than fit.
 template <typename T> __device__ __forceinline__ Gathered gather(Shared& s, uint64_t* gathered, const Row<T>& row, uint32_t lo) {
@@ -453,6 +459,106 @@ template <typename T> __device__ __forceinline__ Gathered gather(Shared& s, uint
     const Gathered few{gathered, min((int)s.number, kGathered)};
     __syncthreads();
     return few;
+}
+
+// Puts gathered tokens of keys from lo on in order: by bins of their values, and in a bin, of which most hold a handful, by comparisons.  False, and nothing done, where one holds many.
+__device__ __forceinline__ bool sort(Shared& s, uint64_t* tokens, int n, uint32_t lo, uint32_t hi) {
+    uint64_t* scattered = s.weight;
+    static_assert(sizeof(s.weight) + sizeof(s.candidates) + sizeof(s.sorted) >= kGathered * sizeof(uint64_t) && offsetof(Shared, candidates) == offsetof(Shared, weight) + sizeof(s.weight) &&
+                  offsetof(Shared, sorted) == offsetof(Shared, candidates) + sizeof(s.candidates), "room for the tokens, in one piece");
+    constexpr int kMost = 128, kBinsEach = kBins / kThreads;
+    const Bins bins = Bins::over(lo, hi);
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.count[i] = 0;
+    __syncthreads();
+    uint64_t token[kEach];
+    int bin[kEach];
+    uint32_t place[kEach];                                 // among the bin's, in no order
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int i = threadIdx.x + e * kThreads;
+        if (i >= n) break;
+        token[e] = tokens[i];
+        const uint32_t key = ~(uint32_t)(token[e] >> 32);
+        bin[e] = bins.of(key_value(key), key);
+        place[e] = atomicAdd(&s.count[bin[e]], 1u);
+    }
+    __syncthreads();
+    uint32_t count[kBinsEach], most = 0;
+    uint64_t all, mine = 0;
+#pragma unroll
+    for (int e = 0; e < kBinsEach; ++e) {
+        count[e] = s.count[kBinsEach * threadIdx.x + e];
+        mine += count[e];
+        most = max(most, count[e]);
+    }
+    if (__syncthreads_or(most > kMost)) return false;
+    uint32_t front = (uint32_t)scan(s.partial, mine, all);
+#pragma unroll
+    for (int e = 0; e < kBinsEach; ++e) { s.count[kBinsEach * threadIdx.x + e] = front; front += count[e]; }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        if ((int)threadIdx.x + e * kThreads >= n) break;
+        scattered[s.count[bin[e]] + place[e]] = token[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        if ((int)threadIdx.x + e * kThreads >= n) break;
+        const int from = (int)s.count[bin[e]], end = bin[e] + 1 < kBins ? (int)s.count[bin[e] + 1] : n;
+        int rank = from;
+        for (int i = from; i < end; ++i) rank += scattered[i] < token[e];
+        tokens[rank] = token[e];
+    }
+    __syncthreads();
+    return true;
+}
+
+// The token of the first `n` of a row that lie in order, whose running sums answer everything: all of them or, of a row's `whole` weight (0: of these), the first k (k > 0).
+__device__ __forceinline__ void sample_sorted(Shared& s, const SampleParams& p, int64_t r, const Parameters& of, const Weights& w, const uint64_t* tokens, int n, int k, uint64_t whole) {
+    const uint64_t one = 1ull << w.bits;
+    const double least = ldexp(of.min_p, w.bits);
+    if (threadIdx.x == 0) s.word[1] = 0;
+    uint64_t weight[kEach], mine = 0, all, heavy = 0;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        const int i = kEach * threadIdx.x + e;
+        const double v = i < n ? w.of(key_value(~(uint32_t)(tokens[i] >> 32))) : 0.0;
+        weight[e] = i < n ? w.whole(v) : 0;
+        mine += weight[e];
+        if (of.any_min_p && i < n && v >= least) heavy = mine;
+    }
+    const uint64_t front = scan(s.partial, mine, all);
+    if (heavy > 0) atomicMax((unsigned long long*)&s.word[1], (unsigned long long)(front + heavy));
+    if (k > 0 && k <= n) {
+        uint64_t upto = front;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            upto += weight[e];
+            if (kEach * (int)threadIdx.x + e == k - 1) s.word[2] = upto;
+        }
+    }
+    __syncthreads();
+    heavy = s.word[1];
+    if (whole > 0) all = whole;
+    else if (k > 0 && k <= n) all = s.word[2];
+    const uint64_t kept = draw(of, all, 0, one, heavy, [&](int, uint64_t goal) {
+        uint64_t upto = front;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            if (upto < goal && upto + weight[e] >= goal) { s.word[0] = upto + weight[e]; s.number = kEach * threadIdx.x + e; }
+            upto += weight[e];
+        }
+        __syncthreads();
+        const Mass reached{0, s.word[0]};
+        __syncthreads();
+        return reached;
+    });
+    if (threadIdx.x == 0) {
+        const uint64_t token = tokens[s.number];
+        p.ids[r] = (int64_t)(uint32_t)token;
+        write_logprob(p, r, w, key_value(~(uint32_t)(token >> 32)), kept);
+    }
 }
 
 // Of the tokens of keys lo to hi, hi the largest of the row and these the first ones, all or the first k (k > 0).
@@ -502,6 +608,7 @@ __device__ __forceinline__ void sample_from(Shared& s, uint64_t* gathered, const
                 });
                 range(s, from, none);
                 const Gathered few = gather(s, gathered, whole, from);
+                if (sort(s, gathered, few.n, from, hi)) return sample_sorted(s, p, r, of, w, gathered, few.n, 0, all.weight);
                 Search<T, Gathered> rest{s, few, whole, w, false, {}, false};
                 rest.take(from, hi, true);
                 return finish(rest);
@@ -511,52 +618,16 @@ __device__ __forceinline__ void sample_from(Shared& s, uint64_t* gathered, const
     finish(search);
 }
 
-// The same of up to kCandidates tokens that were gathered, one to a thread: in order, their running sums answer everything.
-__device__ __forceinline__ void sample_few(Shared& s, const SampleParams& p, int64_t r, const Parameters& of, int vocab, const Gathered& few, uint32_t hi, int k) {
-    const Weights w(key_value(hi), of.inverse, weight_bits(vocab));
-    const uint64_t one = 1ull << w.bits;
-    const int i = threadIdx.x;
-    const bool there = i < few.n;
-    if (there) {
-        const uint64_t c = few.tokens[i];
-        int rank = 0;
-        for (int j = 0; j < few.n; ++j) rank += few.tokens[j] < c;
-        s.sorted[rank] = c;
-    }
-    __syncthreads();
-    const uint64_t token = there ? s.sorted[i] : 0;
-    const float x = key_value(~(uint32_t)(token >> 32));
-    const double v = there ? w.of(x) : 0.0;
-    const uint64_t mine = there ? w.whole(v) : 0;
-    uint64_t all;
-    const uint64_t before = scan(s.partial, mine, all), upto = before + mine;
-    if (of.any_min_p && there && v >= ldexp(of.min_p, w.bits)) atomicMax((unsigned long long*)&s.word[1], (unsigned long long)upto);      // (cleared by the caller)
-    if (k > 0 && k <= few.n && i == k - 1) s.word[2] = upto;
-    __syncthreads();
-    const uint64_t heavy = s.word[1];
-    if (k > 0 && k <= few.n) all = s.word[2];
-    int found = 0;
-    const uint64_t kept = draw(of, all, 0, one, heavy, [&](int step, uint64_t goal) {
-        if (there && before < goal && upto >= goal) { s.word[0] = upto; s.number = i; }
-        __syncthreads();
-        found = (int)s.number;
-        const uint64_t reached = s.word[0];
-        __syncthreads();
-        return Mass{0, reached};
-    });
-    if (i == found && there) {
-        p.ids[r] = (int64_t)(uint32_t)token;
-        write_logprob(p, r, w, x, kept);
-    }
-}
-
 template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) {
     __shared__ Shared s;
     __shared__ uint64_t gathered[kGathered];
     const int64_t r = blockIdx.x;
     const Row<T> row(p, r);
     const Parameters of(p, r);
-    for (int i = threadIdx.x; i < kBins; i += kThreads) s.count[i] = 0;
+    uint32_t* coarse = reinterpret_cast<uint32_t*>(gathered);
+    static_assert(kCoarseBins * sizeof(uint32_t) <= sizeof(gathered));
+    constexpr int kCoarseEach = kCoarseBins / kThreads;
+    for (int i = threadIdx.x; i < kCoarseBins; i += kThreads) coarse[i] = 0;
     __syncthreads();
     uint32_t lo = 0xffffffffu, hi = 0;
     row.each([&](float x, int) {
@@ -564,22 +635,23 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
         if (key == 0) return;
         lo = min(lo, key);
         hi = max(hi, key);
-        atomicAdd(&s.count[(~key) >> kCoarse], 1u);        // largest first
+        atomicAdd(&coarse[~key >> kCoarse], 1u);           // largest first
     });
     range(s, lo, hi);
     if (hi == 0) return write_nothing(p, r);
     // ---- from where on tokens are asked for, and how many there are ----
-    constexpr int kEach = kBins / kThreads;
-    uint64_t here = 0, n_all;
-    for (int i = 0; i < kEach; ++i) here += s.count[kEach * threadIdx.x + i];
-    const uint64_t front = scan(s.partial, here, n_all);
+    uint32_t here[kCoarseEach];
+    uint64_t mine = 0, n_all;
+#pragma unroll
+    for (int i = 0; i < kCoarseEach; ++i) { here[i] = coarse[kCoarseEach * threadIdx.x + i]; mine += here[i]; }
+    uint64_t upto = scan(s.partial, mine, n_all);
     const int k = of.k > 0 && (uint64_t)of.k < n_all ? of.k : 0;
     if (k > 0) {
-        uint64_t upto = front;
-        for (int i = 0; i < kEach; ++i) {
-            const uint64_t next = upto + s.count[kEach * threadIdx.x + i];
-            if (upto < (uint64_t)k && next >= (uint64_t)k) s.word[0] = (uint32_t)~(((uint64_t)(kEach * threadIdx.x + i + 1) << kCoarse) - 1);      // the smallest key of the bin
-            upto = next;
+#pragma unroll
+        for (int i = 0; i < kCoarseEach; ++i) {
+            if (upto < (uint64_t)k && upto + here[i] >= (uint64_t)k)
+                s.word[0] = (uint32_t)~(((uint64_t)(kCoarseEach * threadIdx.x + i + 1) << kCoarse) - 1);     // the smallest key of the bin
+            upto += here[i];
         }
         __syncthreads();
         lo = max(lo, (uint32_t)s.word[0]);
@@ -589,15 +661,16 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
         const uint32_t key = value_key((float)fmax(x - 1e-6 * fabs(x), -3e38));
         if (key_value(hi) < INFINITY && of.inverse > 0.0 && key > lo && key <= hi) lo = key;
     }
-    uint64_t mine = 0, n_asked;                            // those of the bins down to the last one's
-    for (int i = 0; i < kEach; ++i)
-        if (kEach * (int)threadIdx.x + i <= (int)(~lo >> kCoarse)) mine += s.count[kEach * threadIdx.x + i];
+    uint64_t n_asked;                                      // those of the bins down to the last one's
+    mine = 0;
+#pragma unroll
+    for (int i = 0; i < kCoarseEach; ++i)
+        if (kCoarseEach * (int)threadIdx.x + i <= (int)(~lo >> kCoarse)) mine += here[i];
     scan(s.partial, mine, n_asked);
     if (n_asked > kGathered) return sample_from<T>(s, gathered, p, r, of, row, row, lo, hi, k);
-    if (threadIdx.x == 0) s.word[1] = 0;
     const Gathered few = gather(s, gathered, row, lo);
-    if (few.n <= kCandidates) sample_few(s, p, r, of, row.vocab, few, hi, k);
-    else sample_from<T>(s, gathered, p, r, of, row, few, lo, hi, k);
+    if (sort(s, gathered, few.n, lo, hi)) return sample_sorted(s, p, r, of, Weights(key_value(hi), of.inverse, weight_bits(row.vocab)), gathered, few.n, k, 0);
+    sample_from<T>(s, gathered, p, r, of, row, few, lo, hi, k);
 }
 
 // ---- 16-bit logits --------------------------------------------------------------------------------------------------------------------------------------
