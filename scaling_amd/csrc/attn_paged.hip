@@ -54,7 +54,7 @@ struct PagedParams {
 struct PrefixParams : PagedParams {
     const int32_t *prefix_table, *prefix_len, *groups;
     int64_t prefix_stride;
-    int n_groups, prefix_capacity, row_block;
+    int n_groups, prefix_capacity, row_block, tile_shift;
     int4* places;                                         // of every token its sequence's partial results, and behind these its group's: see Place
 };
 template <class P> constexpr bool kPrefix = std::is_same_v<P, PrefixParams>;
@@ -110,10 +110,10 @@ template <int BLOCK, int TILE> struct PrefixWavefront : Wavefront<BLOCK, TILE> {
         if (e >= x.batch + x.n_groups) this->w.blocks = this->s.n = 0;
     }
 };
-// The entry that holds slot `wanted`: the slots of an entry are its blocks * splits, and every split has partial results.  S as in paged_plan.h, of kPrefixPiece tiles at
+// The entry that holds slot `wanted`: the slots of an entry are its blocks * splits, and every split has partial results.  S as in paged_plan.h, of a few tiles at
 // least.  Up to 64 entries every wavefront looks at for itself; of more they take 64 each at a time and tell each other.  (us until a workgroup knows its work, one
 // wavefront after the other over 64 at a time as in paged_find, and so: 8 sequences 2.2, 2.2; 128 sequences 6.0, 4.0 of paged_rows, 4.9, 2.9 of paged_tiles.)
-constexpr int kPrefixPiece = 2;
+constexpr int kPrefixPiece = 2, kPrefixPieceTiles = 4;      // of paged_rows, and of 64 keys
 struct FindShared {
     int sums[8][4];
     PagedFound found;
@@ -136,6 +136,7 @@ template <int BLOCK, int TILE> __device__ __forceinline__ PagedFound find_entry(
         for (int k = 0; k < 3; ++k) v[k] = __builtin_amdgcn_readlane(prefix_sum(of_wave[k]), 63);
         v[3] = group_max<64>(of_wave[3]);
     };
+    constexpr int piece = TILE == kTileKeys ? kPrefixPieceTiles : kPrefixPiece;
     int split_tiles = 0x1000000;                           // no sequence has more
     lanes.look(64 * wave);
     if (plan.share > 0) {
@@ -149,7 +150,7 @@ template <int BLOCK, int TILE> __device__ __forceinline__ PagedFound find_entry(
         }
         exchange(v);
         const int64_t units = (uint32_t)v[0], blocks = v[1], reached = (uint32_t)v[2];
-        split_tiles = max(paged_split_tiles(plan, units, blocks, v[3], share_m), kPrefixPiece);
+        split_tiles = max(paged_split_tiles(plan, units, blocks, v[3], share_m), piece);
         if (paged_level(plan, blocks, v[3], reached)) split_tiles = 0x1000000;
         for (int i = 0; paged_few(plan, blocks) && i <= kPagedSteps; ++i) {
             int slots[4] = {0, 0, 0, 0};
@@ -385,21 +386,24 @@ __device__ __forceinline__ void own_keys_only(const PagedParams& p, const int32_
 // chunk's is in LDS, into the same registers: 16 KB a wavefront (d 128) are always under way, and 12 wavefronts fit a compute unit.  (Two sets of registers, a
 // whole chunk ahead: 8 wavefronts, 16 rows to a block at the most.)  Bound by memory: 32 x 8 items of 200 - 8192 keys of 128 features 83.8 - 85.6 us, 6.1 TB/s; few items
 // by the start and the merge besides, ~10 us: 8 x 8 items of 4096 keys 32.7, a single one of 1500 9.8 (6.5 and a second launch of 5.5 without the merge in it).
-template <int D, int NB, class P>
-__global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_kernel(const P p) {
+template <int D, int NB> struct RowsShared {
+    static constexpr int NWV = kRowWaves, BLOCK = 16 * NB;
+    static constexpr int VSTR = 2 * D + 32;   // bytes per key row of a staged V chunk: transposed reads of 8 rows x 32 bytes hit 256 distinct bytes
+    static constexpr int kStaged = NWV * kRowChunk * VSTR, kResults = NWV * BLOCK * (D + 1) * 4;
+    __attribute__((aligned(16))) char pool[kStaged > kResults ? kStaged : kResults];     // V chunks, then the wavefronts' results
+    float wm_lds[NWV][BLOCK], wl_lds[NWV][BLOCK];
+    int redo_lds[BLOCK];
+};
+template <int D, int NB, class P> __device__ __forceinline__ void paged_rows(const P& p, int index, RowsShared<D, NB>& shared) {
     constexpr int NWV = kRowWaves, kThreads = 64 * NWV, BLOCK = 16 * NB;
-    constexpr int KS = D / 32, DT = D / 16;
-    constexpr int VSTR = 2 * D + 32;          // bytes per key row of a staged V chunk: transposed reads of 8 rows x 32 bytes hit 256 distinct bytes
+    constexpr int KS = D / 32, DT = D / 16, VSTR = RowsShared<D, NB>::VSTR;
     constexpr int V_ITEMS = 8 * (D / 8);      // (four keys, eight features) of a chunk
     constexpr int V_PER_LANE = (V_ITEMS + 63) / 64;
-    constexpr int kStaged = NWV * kRowChunk * VSTR, kResults = NWV * BLOCK * (D + 1) * 4;
-    __shared__ __attribute__((aligned(16))) char pool[kStaged > kResults ? kStaged : kResults];     // V chunks, then the wavefronts' results
-    __shared__ float wm_lds[NWV][BLOCK], wl_lds[NWV][BLOCK];
-    __shared__ int redo_lds[BLOCK];
+    auto& [pool, wm_lds, wl_lds, redo_lds] = shared;
 
     const int tid = threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, G = lane >> 4;
-    const int slot = divide(blockIdx.x, p.nkv, p.nkv_m), kvh = blockIdx.x - slot * p.nkv;
+    const int slot = divide(index, p.nkv, p.nkv_m), kvh = index - slot * p.nkv;
     const PagedFound f = find_work<BLOCK, kRowTile, kSlots>(p, p.rows, p.share_m[0], slot);
     if (f.b < 0) return;
     const int in = slot - f.at, split = paged_quotient(in, f.work.blocks), block = in - split * f.work.blocks;
@@ -642,6 +646,11 @@ __global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_ke
     if (redo_lds[0] == 0) return;
     static_assert(NWV == 4 && sizeof(pool) >= 16 * (D + 2) * sizeof(float), "merge_rows: 256 threads, and room in LDS");
     merge_rows<D, BLOCK, true>(p, f, block, kvh, 0, n_rows, wo);
+}
+template <int D, int NB, class P>
+__global__ __launch_bounds__(64 * kRowWaves, NB == 1 ? 3 : 2) void paged_rows_kernel(const P p) {
+    __shared__ RowsShared<D, NB> shared;
+    paged_rows<D, NB, P>(p, blockIdx.x, shared);
 }
 
 // ---- chunks -------------------------------------------------------------------------------------------------------------------------------------------
@@ -932,6 +941,221 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const P p) {
     }
 }
 
+// ---- groups' prefixes beside sequences' own keys --------------------------------------------------------------------------------------------------------------
+// Blocks of 128 rows in a workgroup of four wavefronts, in the form that shares a compute unit with others: rings of two tiles of K and two of V, requested one and a
+// half tiles ahead, two barriers a tile.  Products wait for the softmax here; other workgroups' fill the pipe, or their requests the time.  Tiles of BN = 64 keys, of
+// which every wavefront requests 16 keys of K and of V, or of 32 (two wavefronts K, two V), where the rings would let one workgroup less run on a compute unit.
+constexpr int kSmallRows = 128, kSmallShift = 7;
+constexpr int kSmallAtOnce = 3;      // workgroups of paged_prefix_kernel that run on a compute unit (blocks of 16 rows)
+template <int D, int BN> struct SmallShared {
+    __attribute__((aligned(1024))) char k[2 * BN * LdsTile<D>::RB], v[2 * BN * LdsTile<D>::RB];
+    int end[4];
+};
+template <int D, int BN> __device__ __forceinline__ void prefix_tiles(const PrefixParams& p, int index, SmallShared<D, BN>& shared) {
+    constexpr int NW = 4, KS = D / 16, DT = D / 32, NT = BN / 32;
+    constexpr bool kRoles = BN == 32;
+    using Tile = LdsTile<D>;
+    constexpr int RB = Tile::RB, TILE = BN * RB, IPW = PageDma<D>::COUNT;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+    const int slot = divide(index, p.nkv, p.nkv_m), kvh = index - slot * p.nkv;
+    const PagedFound f = find_work<kSmallRows, kTileKeys, kSlots>(p, p.tiles, p.share_m[1], slot);
+    if (f.b < 0) return;                                   // the same for the whole workgroup
+    const int in = slot - f.at, split = paged_quotient(in, f.work.blocks), block = f.work.blocks - 1 - (in - split * f.work.blocks);
+    int s0, s1;
+    paged_split_keys<kTileKeys>(f.seq, f.work, f.splits, split, s0, s1);
+
+    const int n_rows = f.seq.n * p.n_rep, row = block * kSmallRows + wave * 32 + l32;
+    const int rr = min(row, n_rows - 1), token = divide(rr, p.n_rep, p.rep_m), head = kvh * p.n_rep + rr - token * p.n_rep;
+    const int limit = row < n_rows ? min(paged_limit(f.seq, token, causal_of(p, f.b)), s1) : 0;
+    elem8_t qf[KS];
+    {
+        const elem_t* qrow = p.q + (int64_t)(f.seq.first + token) * p.q_st + (int64_t)head * p.q_sh + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = __builtin_bit_cast(elem8_t, ld128(qrow + 16 * ks));
+    }
+    note_places(p, f, kvh, split, block * kSmallRows, min(kSmallRows, n_rows - block * kSmallRows), true);
+    const int wmax = group_max<64>(limit);
+    if (lane == 0) shared.end[wave] = wmax;
+    __syncthreads();
+    int end = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) end = max(end, shared.end[w]);
+    const int n_tiles = __builtin_amdgcn_readfirstlane(end > s0 ? (end - s0 + BN - 1) / BN : 0);
+
+    f32x16_t o_acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o_acc[dt][r] = 0.f;
+    float m_i = -INFINITY, l_i = 0.f;
+
+    // ---- direct loads of a wavefront's 16 keys of a tile ----
+    const bool of_k = !kRoles || wave < 2, of_v = !kRoles || wave >= 2;
+    const int part = kRoles ? wave & 1 : wave;
+    const int32_t* table = table_of(p, f.b);
+    const elem_t *kbase = p.kp + (int64_t)kvh * p.p_sh, *vbase = p.vp + (int64_t)kvh * p.p_sh;
+    const int last = max(s1 - 1, 0), last_group = last >> 4, group0 = (s0 >> 4) + part;
+    PageDma<D> dma;
+    dma.init(part, lane, p.p_st);
+    int ids[2] = {0, 0};                                   // lane i: page of this wavefront's keys in tile i of 64, of the 64 that a request is in and the next ones
+    const auto look_up = [&](int from) {
+        const int id = page_of(p, table, min(group0 + BN / 16 * (from + lane), last_group));
+        ids[from >> 6 & 1] = id;
+        asm volatile("" : "+v"(ids[0]), "+v"(ids[1]));     // waited for here, not (with all that is under way) at its use in every step
+    };
+    const auto request = [&](int tile, const elem_t* base, char* ring) {
+        if (tile >= n_tiles) return;
+        const int group = min(group0 + BN / 16 * tile, last_group);
+        const int page = (tile & 64) != 0 ? __builtin_amdgcn_readlane(ids[1], tile & 63) : __builtin_amdgcn_readlane(ids[0], tile & 63);
+        dma.issue(base + (int64_t)page * p.p_sp + (int64_t)row_in_page(p, group) * p.p_st, p.p_st, last - 16 * group + 1, ring + (tile & 1) * TILE);
+    };
+    const auto n_issued = [&](int a, int b) { return IPW * max(0, min(b, n_tiles) - min(a, n_tiles)); };
+    if (n_tiles > 0) {
+        look_up(0);                                        // (Q has come with them)
+        if (of_k) request(0, kbase, shared.k);
+        if (of_v) request(0, vbase, shared.v);
+        if (of_k) request(1, kbase, shared.k);
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
+
+    const float c2 = p.scale_log2;
+    int v_h0, v_h1;
+    Tile::tr_bases(lane, v_h0, v_h1);
+    const int k_row = Tile::row_base(l32, g);
+    constexpr int kDepth = 3;                              // operands are requested three products ahead
+    for (int it = 0; it < n_tiles; ++it) {
+        const int kt = s0 + it * BN;
+        const bool active = kt < wmax;
+        const char *ks_lds = shared.k + (it & 1) * TILE, *vt = shared.v + (it & 1) * TILE;
+        if (of_k) wait_vmcnt_dyn((of_v ? n_issued(it, it + 1) : 0) + n_issued(it + 1, it + 2));         // K tile it; behind it came V tile it and K tile it + 1
+        __syncthreads();                                   // everybody's part of it; and nobody reads V tile it - 1 any more
+        if (of_v) request(it + 1, vbase, shared.v);
+        f32x16_t s_acc[NT];
+        elem8_t pf[2 * NT];
+        if (active) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s_acc[t][r] = 0.f;
+            elem8_t operands[kDepth];
+            const auto fetch = [&](int i) { return *reinterpret_cast<const elem8_t*>(ks_lds + (k_row ^ ((i / NT) << 5)) + 32 * (i % NT) * RB); };
+#pragma unroll
+            for (int i = 0; i < kDepth && i < NT * KS; ++i) operands[i] = fetch(i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < NT * KS; ++i) {
+                s_acc[i % NT] = mfma_32x32x16(operands[i % kDepth], qf[i / NT], s_acc[i % NT]);
+                if (i + kDepth < NT * KS) operands[i % kDepth] = fetch(i + kDepth);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (__any(kt + BN > limit)) {
+                int rel = kt + 4 * g - limit;
+                asm volatile("" : "+v"(rel));              // keeps the compares inside this branch
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (rel + 32 * t + 8 * (r >> 2) + (r & 3) >= 0) s_acc[t][r] = -INFINITY;
+            }
+            float mx = fmaxf(s_acc[0][0], s_acc[NT - 1][0]);
+#pragma unroll
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, fmaxf(s_acc[0][r], s_acc[NT - 1][r]));
+            mx = pair_max(mx);
+            const float m_cand = mx * c2;
+            if (__any(m_cand > m_i + kRescaleGap)) {
+                const float m_new = fmaxf(m_i, m_cand);
+                float alpha = (m_new == -INFINITY) ? 1.0f : fast_exp2(m_i - m_new);
+                asm volatile("" : "+v"(alpha));            // keeps the multiplies below inside this rarely taken branch
+                m_i = m_new;
+                l_i *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o_acc[dt][r] *= alpha;
+            }
+            const float m_use = (m_i == -INFINITY) ? 0.f : m_i;
+            float rs0 = 0.f, rs1 = 0.f;
+#pragma unroll
+            for (int m = 0; m < 2 * NT; ++m) {
+                const int t = m >> 1, r0 = 8 * (m & 1);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float ev = fast_exp2(s_acc[t][r0 + e] * c2 - m_use);
+                    if (e & 1) rs1 += ev; else rs0 += ev;
+                    pf[m][e] = (elem_t)ev;                 // rounded for the product, as in paged_tiles
+                }
+            }
+            l_i += rs0 + rs1;
+        }
+        if (it + 2 < n_tiles && ((it + 2) & 63) == 0) look_up(it + 2);
+        if (of_v) wait_vmcnt_dyn((of_k ? n_issued(it + 1, it + 2) : 0) + n_issued(it + 1, it + 2));     // V tile it; behind it came K and V tile it + 1
+        __syncthreads();                                   // everybody's part of it; and nobody reads K tile it any more
+        if (of_k) request(it + 2, kbase, shared.k);
+        if (active) {
+            elem8_t operands[kDepth];
+            const auto fetch = [&](int i) {
+                const int m = i / DT, dt = i % DT;
+                return tr_pair(vt + (v_h0 ^ (dt << 6)) + 16 * m * RB, vt + (v_h1 ^ (dt << 6)) + 16 * m * RB);
+            };
+#pragma unroll
+            for (int i = 0; i < kDepth && i < 2 * NT * DT; ++i) operands[i] = fetch(i);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < 2 * NT * DT; ++i) {
+                o_acc[i % DT] = mfma_32x32x16(operands[i % kDepth], pf[i / DT], o_acc[i % DT]);
+                if (i + kDepth < 2 * NT * DT) operands[i % kDepth] = fetch(i + kDepth);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+
+    const float l_tot = pair_sum(l_i);
+    const int64_t partial = ((int64_t)(f.partial + split * f.work.blocks + block) * p.nkv + kvh) * p.tile_rows + wave * 32;     // of the wavefront's first row
+    uint64_t redo = 0;
+    const int filled = s0 + n_tiles * BN;                  // tiles are filled up to here: with keys that a row may not see, or with others once more
+    if (__any(row < n_rows && limit < filled)) {
+        uint32_t bad = not_finite(l_tot);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) bad |= (uint32_t)not_finite(o_acc[dt][r]);
+        redo = __ballot(bad != 0 && row < n_rows && limit < filled);
+        redo = (redo | redo >> 32) & 0xffffffffu;
+    }
+    if (row < n_rows && (redo >> l32 & 1) == 0) {
+        float* orow = p.tiles_o + (partial + l32) * D + 4 * g;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+                *reinterpret_cast<float4*>(orow + 32 * dt + 8 * a) = make_float4(o_acc[dt][4 * a], o_acc[dt][4 * a + 1], o_acc[dt][4 * a + 2], o_acc[dt][4 * a + 3]);
+        if (g == 0) *reinterpret_cast<float2*>(p.tiles_ml + (partial + l32) * 2) = make_float2(m_i, l_tot);
+    }
+    for (; redo != 0; redo &= redo - 1) {
+        const int r = __builtin_ctzll(redo), t = __builtin_amdgcn_readlane(token, r), h = __builtin_amdgcn_readlane(head, r), d = 2 * lane;
+        float M, L, O0, O1;
+        own_keys_only<D>(p, table, kvh, p.q + (int64_t)(f.seq.first + t) * p.q_st + (int64_t)h * p.q_sh, s0, __builtin_amdgcn_readlane(limit, r), M, L, O0, O1);
+        if (d >= D) continue;
+        *reinterpret_cast<float2*>(p.tiles_o + (partial + r) * D + d) = make_float2(O0, O1);
+        if (d == 0) *reinterpret_cast<float2*>(p.tiles_ml + (partial + r) * 2) = make_float2(M, L);
+    }
+}
+
+// Both kinds of work in one launch: the first `tiles` workgroups are prefix_tiles', the others paged_rows'.  What either leaves idle, the matrix pipe or the memory, the
+// other one uses, and neither begins and ends alone.
+template <int D, int NB> __global__ __launch_bounds__(256, NB == 1 ? kSmallAtOnce : 2) void paged_prefix_kernel(const PrefixParams p, int tiles) {
+    static_assert(64 * kRowWaves == 256);
+    constexpr int BN = NB == 1 && D >= 96 ? 32 : 64;
+    __shared__ union Both {
+        __device__ Both() {}
+        SmallShared<D, BN> tiles;
+        RowsShared<D, NB> rows;
+    } shared;
+    if ((int)blockIdx.x < tiles) prefix_tiles<D, BN>(p, blockIdx.x, shared.tiles);
+    else paged_rows<D, NB, PrefixParams>(p, blockIdx.x - tiles, shared.rows);
+}
+
 // ---- merge of the splits ------------------------------------------------------------------------------------------------------------------------------
 // A workgroup per 16 rows of a split block and KV head of paged_rows (the first n_rows_groups), where they are not merged in their own launch, and per
 // `per_group` rows of a block of paged_tiles: 16, or 32 where there may be so many workgroups that most of them, which find nothing, set the time.  (us of 16 and 32:
@@ -1004,7 +1228,7 @@ __global__ __launch_bounds__(256) void paged_prefix_merge_kernel(const PrefixPar
     for (int i = 0; i < 2; ++i) {
         const int partial = place[i].x, blocks = place[i].y, in = (token - place[i].w) * p.n_rep + rep;
         const bool tiles = (place[i].z & 1) != 0;
-        const int shift = tiles ? kTileShift : p.row_block == kRowBlock ? 4 : 5, kept = tiles ? p.tile_rows : p.row_block, block = in >> shift;
+        const int shift = tiles ? p.tile_shift : p.row_block == kRowBlock ? 4 : 5, kept = tiles ? p.tile_rows : p.row_block, block = in >> shift;
         splits[i] = place[i].z >> 1;
         // (places that nobody left, of a token in no group or of lengths that overlap, hold anything)
         if (splits[i] < 1 || partial < 0 || in < 0 || block >= blocks || in - (block << shift) >= kept ||
@@ -1186,10 +1410,12 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
 // ---- sequences with a shared prefix -------------------------------------------------------------------------------------------------------------------
 namespace {
 
+
 // The plans of a call, and upper bounds of its blocks.  Of `tokens` new tokens, up to `longest` to a sequence.
 struct PrefixPlans {
     Plans plans;
     int64_t row_blocks, tile_blocks;
+    bool together;                                         // paged_prefix_kernel; else paged_rows and paged_tiles
 };
 PrefixPlans prefix_plans(int64_t tokens, int64_t batch, int64_t groups, int64_t longest, int n_rep, int nkv) {
     PrefixPlans o;
@@ -1203,10 +1429,18 @@ PrefixPlans prefix_plans(int64_t tokens, int64_t batch, int64_t groups, int64_t 
     if (alone && average > kRowBlock) o.plans.row_block = 2 * kRowBlock;
     rows.rows_up_to = tiles.rows_over = alone ? kRowsAlone : average <= 3 * kRowBlock / 2 ? 2 * kRowBlock : o.plans.row_block;
     rows.max_n = tiles.max_n = 0x7fffffff;
-    o.plans.tile_rows = (int)std::min<int64_t>((tokens * n_rep + 15) / 16 * 16, kTileRows);
+    // Prefixes that are cut into pieces, of more blocks than paged_rows takes, go together with the sequences' own keys, for half (two thirds, where two workgroups run on a
+    // compute unit) of what runs at once.  (us, two launches and one: 4 groups of 12 - 13 sequences over 700 - 6000 keys, 16 / 4 heads of 64, 28.6 and 20.0; 64 sequences over 4096
+    // keys, 32 / 8 heads of 128, 46.5 and 34.4, for a third 38.3 and for two thirds 38.1; 128 over 16384 keys 113 and 102, for a third 110; 4 x 16 over 8000 keys 59 and
+    // 45; 32 drafts over 8192 keys 68.8 and 62.4.  Groups that hardly ever have more rows than paged_rows takes: 16 of 16 - 20 rows 41.3 and 44.9.)
+    o.together = !alone && average > 3 * kRowBlock / 2 && tiles.share > 0;
+    o.plans.tile_rows = (int)std::min<int64_t>((tokens * n_rep + 15) / 16 * 16, o.together ? kSmallRows : kTileRows);
+    if (o.together) tiles.fit = share_of(o.plans.row_block == kRowBlock ? kSmallAtOnce * mi_compute_units() / 2 : mi_compute_units(), nkv);
     if (tiles.share > 0) tiles.share = tiles.fit;
     o.row_blocks = alone ? entries + 2 * (tokens * n_rep / o.plans.row_block) : entries * (rows.rows_up_to / o.plans.row_block);
-    o.tile_blocks = paged_max_blocks<kTileRows>(tiles, tokens, batch, longest, n_rep) + paged_max_blocks<kTileRows>(tiles, tokens, groups, tokens, n_rep);
+    if (o.together) o.tile_blocks = paged_max_blocks<kSmallRows>(tiles, tokens, batch, longest, n_rep) + paged_max_blocks<kSmallRows>(tiles, tokens, groups, tokens, n_rep);
+    else o.tile_blocks = paged_max_blocks<kTileRows>(tiles, tokens, batch, longest, n_rep) + paged_max_blocks<kTileRows>(tiles, tokens, groups, tokens, n_rep);
+    o.together = o.together && o.row_blocks > 0 && o.tile_blocks > 0;
     return o;
 }
 size_t prefix_bytes(int64_t tokens, int64_t row_partials, int row_block, int64_t tile_partials, int tile_rows, int nkv, int head_dim) {
@@ -1222,7 +1456,8 @@ extern "C" size_t mi_paged_prefix_attn_workspace_bytes(int64_t tokens, int32_t b
     if (tokens <= 0 || tokens > 0x7fffffffLL || batch < 1 || n_groups < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || head_dim <= 0) return 0;
     const int64_t rows = tokens * (n_q_heads / n_kv_heads), cus = mi_compute_units(), many = rows / (kRowBlock + 1);
     const int64_t row_partials = 2 * (std::min<int64_t>(batch, tokens) + std::min<int64_t>(n_groups, tokens)) + 2 * kRowsAlone / kRowBlock + share_of(kRowsMost * cus, n_kv_heads) + 1;
-    const int64_t tile_partials = std::min<int64_t>(batch, many) + std::min<int64_t>(n_groups, many) + 2 * (rows / kTileRows) + share_of(cus, n_kv_heads) + 1;
+    const int64_t tile_entries = std::min<int64_t>(batch, many) + std::min<int64_t>(n_groups, many), splits = share_of(kSmallAtOnce * cus / 2, n_kv_heads) + 1;
+    const int64_t tile_partials = std::max(tile_entries + 2 * (rows / kTileRows) + splits, (tile_entries + 2 * (rows / kSmallRows) + splits) / 2 + 1);      // of 256 rows, or half as many
     return prefix_bytes(tokens, row_partials, 2 * kRowBlock, many > 0 ? tile_partials : 0, (int)std::min<int64_t>((rows + 15) / 16 * 16, kTileRows), n_kv_heads, head_dim);
 }
 #endif
@@ -1244,6 +1479,7 @@ int MI_ENTRY(mi_paged_prefix_attn_impl)(const mi_paged_prefix_attn_args* x) {
     p.tiles = o.plans.tiles;
     p.tile_rows = o.plans.tile_rows;
     p.row_block = o.plans.row_block;
+    p.tile_shift = o.together ? kSmallShift : kTileShift;
     const int64_t keys = std::max(p.capacity, p.prefix_capacity), row_tiles = (keys + kRowTile - 1) / kRowTile, tile_tiles = (keys + kTileKeys - 1) / kTileKeys;
     if (o.row_blocks * row_tiles > 0x7fffffffLL || o.tile_blocks * tile_tiles > 0x7fffffffLL ||
         (o.row_blocks + o.tile_blocks + 10LL * mi_compute_units()) * p.nkv > 0x7fffffffLL)
@@ -1266,7 +1502,14 @@ int MI_ENTRY(mi_paged_prefix_attn_impl)(const mi_paged_prefix_attn_args* x) {
     const hipStream_t st = (hipStream_t)a->stream;
     const auto go = [&](auto d) {
         constexpr int D = decltype(d)::value;
-        const int rc = p.row_block == kRowBlock ? launch_blocks<D, 1>(p, o.row_blocks, o.tile_blocks, st) : launch_blocks<D, 2>(p, o.row_blocks, o.tile_blocks, st);
+        const auto blocks = [&](auto nb) {
+            constexpr int NB = decltype(nb)::value;
+            if (!o.together) return launch_blocks<D, NB>(p, o.row_blocks, o.tile_blocks, st);
+            const int tiles = p.tiles.max_slots * p.nkv;
+            paged_prefix_kernel<D, NB><<<dim3((unsigned)(tiles + p.rows.max_slots * p.nkv)), dim3(256), 0, st>>>(p, tiles);
+            return mi_check_launch("paged_prefix");
+        };
+        const int rc = p.row_block == kRowBlock ? blocks(std::integral_constant<int, 1>{}) : blocks(std::integral_constant<int, 2>{});
         if (rc != MI_OK) return rc;
         paged_prefix_merge_kernel<D><<<dim3((unsigned)((p.total * (int64_t)p.n_rep + 3) / 4), (unsigned)p.nkv), dim3(256), 0, st>>>(p);
         return mi_check_launch("paged_prefix_merge");
