@@ -232,7 +232,7 @@ int mi_argmax_embed(const void* x, int64_t n_rows, int64_t vocab, int64_t row_st
  * NULL) the natural logarithm of its weight over that sum.  temperature <= 0 or NaN: the first token (and 0).  NaN and -inf logits have no weight; where the largest
  * is +inf, those alone have one; a row without any gives token 0 (and -inf).  uniforms outside [0, 1) are taken for the nearest inside, NaN for 0.
  * Weights are rounded from 64 bits to parts of 2^51 (of more than 2048 tokens: so that all fit 62 bits) and summed as whole numbers.
- * Each parameter is an array of a value per row or, where that is NULL, one value.  row_stride in elements; rows need not be 16-byte aligned.
+ * Each parameter is an array of a value per row or, where that is NULL, one value.  row_stride in elements; rows need not be 16-byte aligned; fewer than 2^22 of them.
  * Algorithmic HBM bytes: n_rows * vocab * e.
  * ------------------------------------------------------------------------------------------ */
 #define MI_SAMPLE_VOCAB_MAX 4194304
@@ -403,7 +403,7 @@ int mi_paged_append(const mi_paged_append_args* args);
  * Pages that are given back (last page first, sequence by sequence) are there to be taken.  Where pages do not suffice (1), a sequence would pass max_ctx keys (0: what
  * the table has room for) (2), or there are more than `tokens` new tokens (4), nothing is taken by anybody, cu_seqlens is all zeros, and the
  * number is set in the status, which nothing here clears.  Lengths outside the table's room count the nearest inside; pages that would pass the end of the stack are
- * dropped.  batch, max_pages, tokens up to 2^24, max_pages * page_size up to 2^30. */
+ * dropped.  batch, max_pages, tokens up to 2^24, max_pages * page_size up to 2^30, batch * max_pages under 2^31. */
 typedef struct mi_paged_step_args {
     const int32_t* new_tokens;
     const int32_t* lengths;

@@ -245,7 +245,7 @@ __global__ __launch_bounds__(kTokenThreads) void paged_step_tokens_kernel(const 
 extern "C" int mi_paged_step(const mi_paged_step_args* a) {
     if (!a) return mi_fail(MI_E_NULL, "paged_step: args is null");
     if (a->batch < 1 || a->batch > (1 << 24) || a->max_pages < 1 || a->max_pages > (1 << 24) || a->page_size < 1 || (int64_t)a->max_pages * a->page_size > (1 << 30) ||
-        a->n_free < 0 || a->tokens < 0 || a->tokens > (1 << 24) || a->max_ctx < 0 || a->max_ctx > a->max_pages * a->page_size || a->page_table_stride < 0)
+        (int64_t)a->batch * a->max_pages > 0x7fffffffLL || a->n_free < 0 || a->tokens < 0 || a->tokens > (1 << 24) || a->max_ctx < 0 || a->max_ctx > a->max_pages * a->page_size || a->page_table_stride < 0)
         return mi_fail(MI_E_SHAPE, "paged_step: %d sequences of up to %d pages of %d keys, %d keys at most, %d tokens, a stack of %d pages", a->batch, a->max_pages,
                        a->page_size, a->max_ctx, a->tokens, a->n_free);
     if (!a->new_tokens || !a->lengths || !a->state || !a->ctx_len || !a->state_out || !a->page_table || !a->cu_seqlens || !a->last ||

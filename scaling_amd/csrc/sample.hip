@@ -409,7 +409,7 @@ struct Parameters {
     }
 };
 
-// The token of what top-k (k > 0), top-p and min-p leave of the weight `kept`, and how much that is: find(step, goal), of step 0 by count, 
+// The token of what top-k (k > 0), top-p and min-p leave of the weight `kept`, and how much that is: find(step, goal), of step 0 by count,
 // gives the mass up to the first token that reaches the goal.  heavy: the weight of those of at least min_p.  (One call in a loop: the compiler makes three of three, with registers for each.)
 template <class F> __device__ __forceinline__ uint64_t draw(const Parameters& p, uint64_t kept, int k, uint64_t one, uint64_t heavy, const F& find) {
 #pragma unroll 1
@@ -442,7 +442,7 @@ __device__ __forceinline__ void write_logprob(const SampleParams& p, int64_t r, 
 __device__ __forceinline__ int weight_bits(int vocab) { return min(51, 30 + __builtin_clz((unsigned)vocab)); }      // all tokens' sum stays under 2^62
 
 // ---- 32-bit logits --------------------------------------------------------------------------------------------------------------------------------------
-// One workgroup per row, for which every pass over it is an exchange with memory.  The first one counts the tokens by the upper 12 bits of their keys, which
+// One workgroup per row, for which every pass over it is an exchange with memory.  The first one counts the tokens by the upper 13 bits of their keys, which
 // tells from where on top-k asks for tokens; without top-p, min-p does too.  If these are few they are gathered in LDS, and all else happens there.
 constexpr int kGathered = 6144, kCoarse = 19, kCoarseBins = 1 << (32 - kCoarse), kEach = kGathered / kThreads;      // bits of a key below its first bin
 
@@ -657,9 +657,9 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
         lo = max(lo, (uint32_t)s.word[0]);
     }
     if (of.any_min_p && of.top_p_none) {                   // a little below the value that min_p stands for
-        const double largest = (double)key_value(hi), x = largest + log(of.min_p) / of.inverse;
-        const uint32_t key = value_key((float)fmax(x - 1e-6 * fabs(x), -3e38));
-        if (key_value(hi) < INFINITY && of.inverse > 0.0 && key > lo && key <= hi) lo = key;
+        const double largest = (double)key_value(hi), at = largest + log(of.min_p) / of.inverse, x = at - 1e-6 * fmax(fabs(at), fabs(largest));
+        const uint32_t key = value_key((float)fmax(x, -3e38));
+        if (key_value(hi) < INFINITY && of.inverse > 0.0 && x > -3e38 && key > lo && key <= hi) lo = key;      // (no float may be lower than x)
     }
     uint64_t n_asked;                                      // those of the bins down to the last one's
     mine = 0;
@@ -956,6 +956,8 @@ template <typename T, int NV> __global__ __launch_bounds__(kThreads) void sample
     }
 }
 
+constexpr int64_t kMostRows = (1ll << 32) / kThreads - 1;  // a launch has fewer than 2^32 threads
+
 template <typename T> void launch(const SampleParams& p, int64_t rows, hipStream_t st) {
     const dim3 grid((unsigned)rows), block(kThreads);
     if constexpr (sizeof(T) == 4) sample_kernel<T><<<grid, block, 0, st>>>(p);
@@ -968,7 +970,7 @@ template <typename T> void launch(const SampleParams& p, int64_t rows, hipStream
 extern "C" int mi_sample(const mi_sample_args* a) {
     if (!a) return mi_fail(MI_E_NULL, "sample: args is null");
     if (a->n_rows == 0) return MI_OK;
-    if (a->n_rows < 0 || a->n_rows > 0x7fffffffLL || a->vocab < 1 || a->vocab > MI_SAMPLE_VOCAB_MAX || a->row_stride < 0)
+    if (a->n_rows < 0 || a->n_rows > kMostRows || a->vocab < 1 || a->vocab > MI_SAMPLE_VOCAB_MAX || a->row_stride < 0)
         return mi_fail(MI_E_SHAPE, "sample: %lld rows of %lld logits (1 to %d), %lld apart", (long long)a->n_rows, (long long)a->vocab, MI_SAMPLE_VOCAB_MAX,
                        (long long)a->row_stride);
     if (!a->logits || !a->uniforms || !a->ids) return mi_fail(MI_E_NULL, "sample: null pointer");

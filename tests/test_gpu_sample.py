@@ -182,6 +182,18 @@ def test_one_launch_streams_and_replays():
     assert torch.equal(out, want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+def test_min_p_far_below(dtype):
+    """Temperatures at which tokens of the type's lowest value weigh more than min_p, and ones at which min_p stands for a value near zero far below the largest."""
+    vocab, low = 3000, torch.finfo(dtype).min
+    x = _logits(6, vocab, dtype, seed=20)
+    x[:3] = x[:3].masked_fill(torch.rand(3, vocab, generator=torch.Generator().manual_seed(21)) < 0.8, low)
+    x[3, ::2] = low / 2
+    x[4] *= 1e-3
+    x[4, 17] = 60000.0
+    _check(x, [0.99, 0.5, 0.2, 0.9, 0.7, 0.999], temperature=[-low / 4, -low / 3, math.inf, -low / 2, 60000.0 / math.log(1000.0), 1.0], min_p=[1e-3, 1e-3, 0.5, 0.05, 1e-3, 1e-3])
+
+
 def test_far_rows():
     """Offsets over 2^31 elements."""
     stride = (1 << 31) // 3 + 1001

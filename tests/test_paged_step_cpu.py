@@ -58,6 +58,9 @@ def test_entry_refuses():
         setattr(a, name, value)
         assert lib.mi_paged_step(ctypes.byref(a)) == -3, name
         setattr(a, name, before)
+    a.batch, a.max_pages = 1 << 10, 1 << 21                                                  # sums of pages are kept in 32 bits
+    assert lib.mi_paged_step(ctypes.byref(a)) == -3
+    a.batch, a.max_pages = 2, 4
     for name in ("new_tokens", "lengths", "state", "ctx_len", "state_out", "page_table", "free_pages", "cu_seqlens", "last", "position_ids", "slots", "sequences"):
         setattr(a, name, None)
         assert lib.mi_paged_step(ctypes.byref(a)) == -1, name

@@ -36,7 +36,7 @@ def test_entry_refuses():
     assert lib.mi_sample(ctypes.byref(a)) == -1
     buf = (ctypes.c_char * 64)()
     a.logits = a.uniforms = a.ids = ctypes.addressof(buf)
-    for name, value in (("n_rows", -1), ("n_rows", 1 << 31), ("vocab", 0), ("vocab", (1 << 22) + 1), ("row_stride", -1)):
+    for name, value in (("n_rows", -1), ("n_rows", 1 << 31), ("n_rows", 1 << 22), ("vocab", 0), ("vocab", (1 << 22) + 1), ("row_stride", -1)):
         before = getattr(a, name)
         setattr(a, name, value)
         assert lib.mi_sample(ctypes.byref(a)) == -3, name
