@@ -5,6 +5,9 @@
 // workgroup evaluates on the lengths by itself; partial results (running maximum, sum, unscaled output) of sequences with several splits go to the
 // workspace and are merged by `paged_merge`.
 //
+// Where groups of sequences share a prefix, the same kernels compute sequences and groups, or `paged_prefix` has sequences' own keys as paged_rows beside prefixes
+// in blocks of 128 rows; `paged_prefix_merge` joins the two softmax parts of a row.
+//
 // Pages hold a multiple of 16 keys, so 16 neighbouring keys (what one row of an MFMA operand tile, or one wavefront's share of a tile's direct loads, needs)
 // have one page: its number is found once per 16 keys and wavefront, and a paged cache costs next to nothing against a contiguous one.
 #include "attn_common.h"
@@ -1410,7 +1413,6 @@ int MI_ENTRY(mi_paged_attn_impl)(const mi_paged_attn_args* a) {
 // ---- sequences with a shared prefix -------------------------------------------------------------------------------------------------------------------
 namespace {
 
-
 // The plans of a call, and upper bounds of its blocks.  Of `tokens` new tokens, up to `longest` to a sequence.
 struct PrefixPlans {
     Plans plans;
@@ -1450,8 +1452,8 @@ size_t prefix_bytes(int64_t tokens, int64_t row_partials, int row_block, int64_t
 }  // namespace
 
 #ifndef MI_ELEM_F16
-// For every max_q_len: entries with two blocks of rows each (and the few of a call without paged_tiles), blocks of 256 of those with more than 16, and the splits that either
-// share adds.
+// For every max_q_len: entries with two blocks of rows each (and the few of a call without paged_tiles), blocks of 256 or of 128 rows of those with more than 16, and the
+// splits that either share adds.
 extern "C" size_t mi_paged_prefix_attn_workspace_bytes(int64_t tokens, int32_t batch, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim) {
     if (tokens <= 0 || tokens > 0x7fffffffLL || batch < 1 || n_groups < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || head_dim <= 0) return 0;
     const int64_t rows = tokens * (n_q_heads / n_kv_heads), cus = mi_compute_units(), many = rows / (kRowBlock + 1);

@@ -96,6 +96,37 @@ def test_long_prefixes_are_split(nq, nkv, d, page, batch, length):
         assert torch.equal(out, ops.paged_prefix_attention(*args, max_q_len=1))
 
 
+@DTYPES
+@pytest.mark.parametrize("nq,nkv,d,batch,groups,length,new", [(8, 2, 96, 30, 1, 700, 1), (8, 2, 32, 30, 1, 700, 1), (4, 1, 128, 62, 2, 500, 1), (8, 1, 128, 63, 2, 300, 1), (4, 2, 64, 64, 1, 400, 1),
+                                                              (8, 2, 64, 300, 3, 200, 1), (4, 1, 32, 300, 2, 90, 3), (8, 1, 96, 20, 1, 1000, 2), (4, 1, 128, 40, 1, 2000, 5),
+                                                              (128, 128, 32, 30, 1, 13000, 1), (128, 128, 32, 66, 1, 13000, 1), (128, 128, 96, 66, 1, 6500, 1), (128, 128, 32, 20, 1, 13000, 17)])
+def test_groups_of_many_rows(nq, nkv, d, batch, groups, length, new, dtype):
+    """Prefixes and own keys in one launch, by every head size, by the number of sequences that its workgroups look for their work among, and with
+    more tiles of a prefix to a workgroup than it looks up pages for at once."""
+    print(f"case {nq} {nkv} {d} {batch} {groups} {length} {new} {dtype}", flush=True)
+    sizes = [batch // groups] * groups
+    sizes[0] += batch - sum(sizes)
+    counts = [1 + i % new for i in range(batch)]
+    call = _Call(counts, [n + 13 * i % 70 for i, n in enumerate(counts)], sizes, [length + 37 * g for g in range(groups)], nq, nkv, d, 16, dtype, seed=length + d)
+    args = call.arguments()
+    names = launched(lambda: ops.paged_prefix_attention(*args, max_q_len=new))
+    assert len(names) == 2 and any("paged_prefix_kernel" in n for n in names) == (sum(counts) * nq // nkv > 64), names       # all rows together are few
+    out = ops.paged_prefix_attention(*args, max_q_len=new)
+    call.check("o", out)
+    for _ in range(3):
+        assert torch.equal(out, ops.paged_prefix_attention(*args, max_q_len=new))
+    call.check("o, tokens not bounded", ops.paged_prefix_attention(*args))
+
+
+def test_more_blocks_than_compute_units():
+    """So many rows that nothing is cut into pieces, of more sequences than a workgroup's wavefronts look at together."""
+    call = _Call([3] * 700, [3 + i % 20 for i in range(700)], [300, 400], [100, 33], 32, 32, 32, 16, torch.bfloat16, seed=21)
+    args = call.arguments()
+    names = launched(lambda: ops.paged_prefix_attention(*args, max_q_len=3))
+    assert any("paged_tiles" in n for n in names), names
+    call.check("o", ops.paged_prefix_attention(*args, max_q_len=3))
+
+
 def test_no_prefix_is_paged_attention():
     """Groups of empty prefixes, and sequences outside all groups."""
     call = _Call([1, 3, 1, 1], [50, 3, 400, 1], [1, 1], [0, 0], 8, 2, 128, 16, torch.bfloat16, seed=3, first=1)
