@@ -218,6 +218,25 @@ def test_launches_streams_and_replays():
     assert torch.equal(out, want)
 
 
+def test_replays_of_many_rows():
+    """Prefixes and own keys in one launch: lengths change between replays, eager calls with a workspace of their own between them."""
+    call = _Call([1] * 40, [60] * 40, [25, 15], [900, 500], 8, 2, 64, 16, torch.float16, seed=22)
+    args = list(call.arguments())
+    ws = ops.paged_prefix_workspace(40, 2, 40, 8, 2, 64, DEV)
+    assert any("paged_prefix_kernel" in n for n in launched(lambda: ops.paged_prefix_attention(*args, max_q_len=1, workspace=ws)))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_prefix_attention(*args, max_q_len=1, workspace=ws)
+    for ctx, prefix, groups in (([1] * 40, [1, 0], [0, 25, 40]), ([i + 1 for i in range(40)], [899, 333], [0, 1, 40]), ([60] * 40, [0, 0], [3, 3, 40]), ([60] * 40, [900, 500], [0, 25, 40])):
+        args[5].copy_(_ints(ctx))
+        args[7].copy_(_ints(prefix))
+        args[8].copy_(_ints(groups))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int16), ops.paged_prefix_attention(*args, max_q_len=1).view(torch.int16)), (ctx, prefix, groups)
+    call.check("o of the last replay", out)
+
+
 def test_far_pages():
     """Pages over 2^31 elements away."""
     pages = (1 << 31) // (16 * 2 * 64) + 40

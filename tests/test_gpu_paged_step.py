@@ -62,6 +62,41 @@ def test_steps(batch, page, most):
     assert refused > 0 or batch == 1
 
 
+@pytest.mark.parametrize("batch,page,rows", [(1, 16, 0), (2, 16, 1), (63, 32, 0), (65, 16, 9), (130, 48, 0), (1000, 16, 30), (1024, 16, 0), (1024, 16, 4000), (1025, 16, 0)])
+def test_single_tokens(batch, page, rows):
+    """Steps of a token or none of each sequence, of which some end: pages of those go to others in the same step."""
+    rng = random.Random(batch + rows)
+    cache = _Cache(batch, 3, 2 * batch, page, seed=batch + 1)
+    refused = taken = 0
+    for i in range(3 * page + 20):
+        ends = 0.3 if i % 7 == 6 else 0.02
+        new = [-1 if rng.random() < ends else int(rng.random() < 0.95) for _ in range(batch)]
+        tokens = max(1, new.count(1) + rows - (1 if i % 11 == 10 else 0))
+        if i % 16 == 0:
+            print(f"step {i}: {tokens} tokens of {batch} sequences", flush=True)
+        before = cache.count
+        cache.step(new, tokens, None if i % 3 else 2 * page + 3, [rng.randrange(1000) for _ in range(batch)] if i % 2 else None, in_place=i % 4 != 3)
+        taken += cache.count < before
+        refused += cache.status != 0
+        cache.status = 0
+        cache.on_gpu[3][1] = 0
+    assert taken > 0 and (refused > 0 or batch <= 2)
+
+
+def test_results_are_tensors_like_any():
+    """One allocation holds them; they are written to, kept and used in products as others are, also where no gradients are ever wanted."""
+    for mode in (torch.inference_mode, torch.no_grad, torch.enable_grad):
+        with mode():
+            cache = _Cache(3, 4, 12, 16, seed=9)
+            got = cache.step([2, 0, 5], 9)
+            kept = [t.clone() for t in got]
+            for i, t in enumerate(got):
+                t.add_(1 + i)
+                assert all(torch.equal(x, k + (1 + j if j <= i else 0)) for j, (x, k) in enumerate(zip(got, kept)))
+            assert torch.equal(got.position_ids.view(3, 3).t().contiguous().float().sum(), (kept[1] + 2).float().sum())
+            assert not any(t.requires_grad for t in got) and got.last.device == got.cu_seqlens.device and got.slots[2:].storage_offset() == 2 + got.slots.storage_offset()
+
+
 @pytest.mark.parametrize("new,tokens", [([4000, 96, 1], 4097), ([5000, 0, 3000], 9000), ([1, 1, 1], 6000)])
 def test_many_rows(new, tokens):
     cache = _Cache(3, 400, 900, 16, seed=1)
