@@ -232,6 +232,8 @@ template <int D> struct LdsTile {
     }
 };
 
+__device__ __forceinline__ uint32_t lds_byte(char* at) { return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)at; }
+
 // Direct global -> LDS loads of 64-token tiles by one wavefront: instructions [n0, n0 + COUNT) of each tile.
 // The per-lane byte offsets inside a tile are fixed for the kernel, so a tile costs COUNT instructions with
 // a scalar base address and no vector arithmetic; only a tile that runs past the last token recomputes its
@@ -260,10 +262,12 @@ template <int D, int COUNT> struct DmaPlan {
             off[j] = (uint32_t)(row * (int)tok_stride * 2 + unit_off);
         }
     }
-    __device__ __forceinline__ static void issue_one(uint32_t voff, const void* sbase, char* dst_lds) {
-        const uint32_t dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)dst_lds;
+    __device__ __forceinline__ static void issue_one(uint32_t voff, const void* sbase, uint32_t dst) {      // dst: byte of LDS
         asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                      :: "v"(voff), "s"(sbase), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
+    }
+    __device__ __forceinline__ static void issue_one(uint32_t voff, const void* sbase, char* dst_lds) {
+        issue_one(voff, sbase, lds_byte(dst_lds));
     }
     // All COUNT instructions of the tile whose first token is tok0, straight-line when the tile is full.
     // tile: wave-uniform LDS address of the stage; base + tok0 * tok_stride must be wave-uniform too.

@@ -681,8 +681,8 @@ template <int D> struct PageDma {
         }
     }
     // base: key 16 * group of the wavefront's group (uniform); rows: how many of the 16 there are (further ones repeat the last)
-    __device__ __forceinline__ void issue(const elem_t* base, int64_t tok_stride, int rows, char* tile) const {
-        char* dst = tile + 1024 * COUNT * lw;
+    template <class LDS> __device__ __forceinline__ void issue(const elem_t* base, int64_t tok_stride, int rows, LDS tile) const {      // (a pointer or a byte of LDS)
+        const LDS dst = tile + 1024 * COUNT * lw;
         if (rows >= 16) {
 #pragma unroll
             for (int j = 0; j < COUNT; ++j) DmaPlan<D, 1>::issue_one(off[j], base, dst + 1024 * j);
@@ -945,18 +945,25 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const P p) {
 }
 
 // ---- groups' prefixes beside sequences' own keys --------------------------------------------------------------------------------------------------------------
-// Blocks of 128 rows in a workgroup of four wavefronts, in the form that shares a compute unit with others: rings of two tiles of K and two of V, requested one and a
-// half tiles ahead, two barriers a tile.  Products wait for the softmax here; other workgroups' fill the pipe, or their requests the time.  Tiles of BN = 64 keys, of
-// which every wavefront requests 16 keys of K and of V, or of 32 (two wavefronts K, two V), where the rings would let one workgroup less run on a compute unit.
+// Blocks of 128 rows in a workgroup of four wavefronts, in the form that shares a compute unit with others: rings of two tiles of K and two of V.  A wavefront has a SIMD
+// to itself or with others' workgroups, so that all that it issues counts: a tile's place in the cache is two lane reads, waits are constants (per 64 keys 3770 cycles with the
+// page's place computed by the scalar unit and waits by how much is under way, 3200 so).  Two forms, by the registers that there are:
+//     three workgroups to a compute unit (168 registers; K one and a half tiles ahead, two barriers a tile): products wait for the softmax; other workgroups' fill the pipe, or
+//     their requests the time.  Tiles of BN = 64 keys, of which every wavefront requests 16 keys of K and of V, or of 32 (two wavefronts K, two V), where the rings would
+//     let one workgroup less run on a compute unit.
+//     AHEAD, two workgroups: the next tile's scores are computed among this one's exponentials (which take twice as long as the products), one barrier a tile.
+// (us of 32 drafts of 3 - 7 tokens over 8192 keys, 32 / 8 heads of 128: 58 without the next scores, 54 with them.  Rings of three or four tiles, requests spread over the products
+// or over the wavefronts: level or slower.)
 constexpr int kSmallRows = 128, kSmallShift = 7;
 constexpr int kSmallAtOnce = 3;      // workgroups of paged_prefix_kernel that run on a compute unit (blocks of 16 rows)
 template <int D, int BN> struct SmallShared {
     __attribute__((aligned(1024))) char k[2 * BN * LdsTile<D>::RB], v[2 * BN * LdsTile<D>::RB];
     int end[4];
 };
-template <int D, int BN> __device__ __forceinline__ void prefix_tiles(const PrefixParams& p, int index, SmallShared<D, BN>& shared) {
+template <int D, int BN, bool AHEAD> __device__ __forceinline__ void prefix_tiles(const PrefixParams& p, int index, SmallShared<D, BN>& shared) {
     constexpr int NW = 4, KS = D / 16, DT = D / 32, NT = BN / 32;
     constexpr bool kRoles = BN == 32;
+    static_assert(!(AHEAD && kRoles));
     using Tile = LdsTile<D>;
     constexpr int RB = Tile::RB, TILE = BN * RB, IPW = PageDma<D>::COUNT;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
@@ -977,7 +984,7 @@ template <int D, int BN> __device__ __forceinline__ void prefix_tiles(const Pref
         for (int ks = 0; ks < KS; ++ks) qf[ks] = __builtin_bit_cast(elem8_t, ld128(qrow + 16 * ks));
     }
     note_places(p, f, kvh, split, block * kSmallRows, min(kSmallRows, n_rows - block * kSmallRows), true);
-    const int wmax = group_max<64>(limit);
+    const int wmax = __builtin_amdgcn_readfirstlane(group_max<64>(limit));
     if (lane == 0) shared.end[wave] = wmax;
     __syncthreads();
     int end = 0;
@@ -1000,24 +1007,34 @@ template <int D, int BN> __device__ __forceinline__ void prefix_tiles(const Pref
     const int last = max(s1 - 1, 0), last_group = last >> 4, group0 = (s0 >> 4) + part;
     PageDma<D> dma;
     dma.init(part, lane, p.p_st);
-    int ids[2] = {0, 0};                                   // lane i: page of this wavefront's keys in tile i of 64, of the 64 that a request is in and the next ones
-    const auto look_up = [&](int from) {
-        const int id = page_of(p, table, min(group0 + BN / 16 * (from + lane), last_group));
-        ids[from >> 6 & 1] = id;
-        asm volatile("" : "+v"(ids[0]), "+v"(ids[1]));     // waited for here, not (with all that is under way) at its use in every step
+    // lane i: where this wavefront's keys of the tile i, i + 64, ... that is next lie from kbase and vbase on; 32 tiles more at a time
+    int at_lo = 0, at_hi = 0;
+    const auto look_up = [&](int from, int n) {
+        const int tile = from + ((lane - from) & 63), group = min(group0 + BN / 16 * tile, last_group);
+        const int64_t x = (int64_t)page_of(p, table, group) * p.p_sp + (int64_t)row_in_page(p, group) * p.p_st;
+        at_lo = tile < from + n ? (int)x : at_lo;
+        at_hi = tile < from + n ? (int)(x >> 32) : at_hi;
+        asm volatile("" : "+v"(at_lo), "+v"(at_hi));       // waited for here, not (with all that is under way) at its use in every step
     };
-    const auto request = [&](int tile, const elem_t* base, char* ring) {
+    const uint32_t k_ring = lds_byte(shared.k), v_ring = lds_byte(shared.v);
+    const auto request = [&](int tile, const elem_t* base, uint32_t ring) {
         if (tile >= n_tiles) return;
-        const int group = min(group0 + BN / 16 * tile, last_group);
-        const int page = (tile & 64) != 0 ? __builtin_amdgcn_readlane(ids[1], tile & 63) : __builtin_amdgcn_readlane(ids[0], tile & 63);
-        dma.issue(base + (int64_t)page * p.p_sp + (int64_t)row_in_page(p, group) * p.p_st, p.p_st, last - 16 * group + 1, ring + (tile & 1) * TILE);
+        const int64_t from = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, tile & 63) << 32 | (uint32_t)__builtin_amdgcn_readlane(at_lo, tile & 63));
+        dma.issue(base + from, p.p_st, last - 16 * min(group0 + BN / 16 * tile, last_group) + 1, ring + (tile & 1) * TILE);
     };
-    const auto n_issued = [&](int a, int b) { return IPW * max(0, min(b, n_tiles) - min(a, n_tiles)); };
+    // K or V of a tile has come; behind it came `more` and, if there is a next one, as much of each of that
+    const auto wait_for = [&](int it, auto more, auto next) {
+        if (it + 1 < n_tiles) wait_vmcnt<IPW * (decltype(more)::value + decltype(next)::value)>();
+        else wait_vmcnt<IPW * decltype(more)::value>();
+    };
+    using C0 = std::integral_constant<int, 0>;
+    using C1 = std::integral_constant<int, 1>;
+    using C2 = std::integral_constant<int, 2>;
     if (n_tiles > 0) {
-        look_up(0);                                        // (Q has come with them)
-        if (of_k) request(0, kbase, shared.k);
-        if (of_v) request(0, vbase, shared.v);
-        if (of_k) request(1, kbase, shared.k);
+        look_up(0, 64);                                    // (Q has come with them)
+        if (of_k) request(0, kbase, k_ring);
+        if (of_v) request(0, vbase, v_ring);
+        if (of_k) request(1, kbase, k_ring);
     }
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[ks]));
@@ -1027,89 +1044,131 @@ template <int D, int BN> __device__ __forceinline__ void prefix_tiles(const Pref
     Tile::tr_bases(lane, v_h0, v_h1);
     const int k_row = Tile::row_base(l32, g);
     constexpr int kDepth = 3;                              // operands are requested three products ahead
-    for (int it = 0; it < n_tiles; ++it) {
-        const int kt = s0 + it * BN;
-        const bool active = kt < wmax;
-        const char *ks_lds = shared.k + (it & 1) * TILE, *vt = shared.v + (it & 1) * TILE;
-        if (of_k) wait_vmcnt_dyn((of_v ? n_issued(it, it + 1) : 0) + n_issued(it + 1, it + 2));         // K tile it; behind it came V tile it and K tile it + 1
-        __syncthreads();                                   // everybody's part of it; and nobody reads V tile it - 1 any more
-        if (of_v) request(it + 1, vbase, shared.v);
-        f32x16_t s_acc[NT];
-        elem8_t pf[2 * NT];
-        if (active) {
+    // one after the other: S^T of a tile and, behind every product, whatever else
+    const auto scores = [&](const char* ks_lds, f32x16_t (&s)[NT], const auto& behind) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[t][r] = 0.f;
+        elem8_t operands[kDepth];
+        const auto fetch = [&](int i) { return *reinterpret_cast<const elem8_t*>(ks_lds + (k_row ^ ((i / NT) << 5)) + 32 * (i % NT) * RB); };
+#pragma unroll
+        for (int i = 0; i < kDepth && i < NT * KS; ++i) operands[i] = fetch(i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < NT * KS; ++i) {
+            s[i % NT] = mfma_32x32x16(operands[i % kDepth], qf[i / NT], s[i % NT]);
+            if (i + kDepth < NT * KS) operands[i % kDepth] = fetch(i + kDepth);
+            behind(i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // the maximum that a tile's weights are taken by
+    const auto maximum = [&](int kt, f32x16_t (&s)[NT]) {
+        if (__any(kt + BN > limit)) {
+            int rel = kt + 4 * g - limit;
+            asm volatile("" : "+v"(rel));                  // keeps the compares inside this branch
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s_acc[t][r] = 0.f;
-            elem8_t operands[kDepth];
-            const auto fetch = [&](int i) { return *reinterpret_cast<const elem8_t*>(ks_lds + (k_row ^ ((i / NT) << 5)) + 32 * (i % NT) * RB); };
-#pragma unroll
-            for (int i = 0; i < kDepth && i < NT * KS; ++i) operands[i] = fetch(i);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int i = 0; i < NT * KS; ++i) {
-                s_acc[i % NT] = mfma_32x32x16(operands[i % kDepth], qf[i / NT], s_acc[i % NT]);
-                if (i + kDepth < NT * KS) operands[i % kDepth] = fetch(i + kDepth);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if (__any(kt + BN > limit)) {
-                int rel = kt + 4 * g - limit;
-                asm volatile("" : "+v"(rel));              // keeps the compares inside this branch
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (rel + 32 * t + 8 * (r >> 2) + (r & 3) >= 0) s_acc[t][r] = -INFINITY;
-            }
-            float mx = fmaxf(s_acc[0][0], s_acc[NT - 1][0]);
-#pragma unroll
-            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, fmaxf(s_acc[0][r], s_acc[NT - 1][r]));
-            mx = pair_max(mx);
-            const float m_cand = mx * c2;
-            if (__any(m_cand > m_i + kRescaleGap)) {
-                const float m_new = fmaxf(m_i, m_cand);
-                float alpha = (m_new == -INFINITY) ? 1.0f : fast_exp2(m_i - m_new);
-                asm volatile("" : "+v"(alpha));            // keeps the multiplies below inside this rarely taken branch
-                m_i = m_new;
-                l_i *= alpha;
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o_acc[dt][r] *= alpha;
-            }
-            const float m_use = (m_i == -INFINITY) ? 0.f : m_i;
-            float rs0 = 0.f, rs1 = 0.f;
-#pragma unroll
-            for (int m = 0; m < 2 * NT; ++m) {
-                const int t = m >> 1, r0 = 8 * (m & 1);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float ev = fast_exp2(s_acc[t][r0 + e] * c2 - m_use);
-                    if (e & 1) rs1 += ev; else rs0 += ev;
-                    pf[m][e] = (elem_t)ev;                 // rounded for the product, as in paged_tiles
-                }
-            }
-            l_i += rs0 + rs1;
+                for (int r = 0; r < 16; ++r)
+                    if (rel + 32 * t + 8 * (r >> 2) + (r & 3) >= 0) s[t][r] = -INFINITY;
         }
-        if (it + 2 < n_tiles && ((it + 2) & 63) == 0) look_up(it + 2);
-        if (of_v) wait_vmcnt_dyn((of_k ? n_issued(it + 1, it + 2) : 0) + n_issued(it + 1, it + 2));     // V tile it; behind it came K and V tile it + 1
-        __syncthreads();                                   // everybody's part of it; and nobody reads K tile it any more
-        if (of_k) request(it + 2, kbase, shared.k);
-        if (active) {
-            elem8_t operands[kDepth];
-            const auto fetch = [&](int i) {
-                const int m = i / DT, dt = i % DT;
-                return tr_pair(vt + (v_h0 ^ (dt << 6)) + 16 * m * RB, vt + (v_h1 ^ (dt << 6)) + 16 * m * RB);
-            };
+        float mx = fmaxf(s[0][0], s[NT - 1][0]);
 #pragma unroll
-            for (int i = 0; i < kDepth && i < 2 * NT * DT; ++i) operands[i] = fetch(i);
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, fmaxf(s[0][r], s[NT - 1][r]));
+        mx = pair_max(mx);
+        const float m_cand = mx * c2;
+        if (__any(m_cand > m_i + kRescaleGap)) {
+            const float m_new = fmaxf(m_i, m_cand);
+            float alpha = (m_new == -INFINITY) ? 1.0f : fast_exp2(m_i - m_new);
+            asm volatile("" : "+v"(alpha));                // keeps the multiplies below inside this rarely taken branch
+            m_i = m_new;
+            l_i *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o_acc[dt][r] *= alpha;
+        }
+        return (m_i == -INFINITY) ? 0.f : m_i;
+    };
+    const auto add_values = [&](const char* vt, const elem8_t (&pf)[2 * NT]) {
+        elem8_t operands[kDepth];
+        const auto fetch = [&](int i) {
+            const int m = i / DT, dt = i % DT;
+            return tr_pair(vt + (v_h0 ^ (dt << 6)) + 16 * m * RB, vt + (v_h1 ^ (dt << 6)) + 16 * m * RB);
+        };
+#pragma unroll
+        for (int i = 0; i < kDepth && i < 2 * NT * DT; ++i) operands[i] = fetch(i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 2 * NT * DT; ++i) {
+            o_acc[i % DT] = mfma_32x32x16(operands[i % kDepth], pf[i / DT], o_acc[i % DT]);
+            if (i + kDepth < 2 * NT * DT) operands[i % kDepth] = fetch(i + kDepth);
             __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    float sums[2];
+    // weights n of a tile's 16 NT from e on; rounded for the product, as in paged_tiles
+    const auto weigh = [&](const f32x16_t (&s)[NT], float m_use, elem8_t (&pf)[2 * NT], int e0, int n) {
 #pragma unroll
-            for (int i = 0; i < 2 * NT * DT; ++i) {
-                o_acc[i % DT] = mfma_32x32x16(operands[i % kDepth], pf[i / DT], o_acc[i % DT]);
-                if (i + kDepth < 2 * NT * DT) operands[i % kDepth] = fetch(i + kDepth);
-                __builtin_amdgcn_sched_barrier(0);
+        for (int e = 0; e < 16 * NT; ++e) {
+            if (e < e0 || e >= e0 + n) continue;
+            const float ev = fast_exp2(s[e / 16][e % 16] * c2 - m_use);
+            sums[e & 1] += ev;
+            pf[e / 8][e % 8] = (elem_t)ev;
+        }
+    };
+    if constexpr (AHEAD) {
+        f32x16_t s_acc[2][NT];                             // of a tile and of the next one
+        if (n_tiles > 0) {
+            wait_for(0, C1{}, C1{});                       // K tile 0; behind it came V tile 0 and K tile 1
+            __syncthreads();
+            if (s0 < wmax) scores(shared.k, s_acc[0], [](int) {});
+        }
+        const auto step = [&](int it, f32x16_t (&s)[NT], f32x16_t (&s_next)[NT]) {
+            const int kt = s0 + it * BN;
+            if (it + 33 < n_tiles && ((it + 1) & 31) == 0) look_up(it + 33, 32);
+            wait_vmcnt<0>();                               // V tile it and K tile it + 1
+            __syncthreads();                               // everybody's parts of them; and nobody reads V tile it - 1 or K tile it any more
+            request(it + 1, vbase, v_ring);
+            request(it + 2, kbase, k_ring);
+            if (kt >= wmax) return;
+            const float m_use = maximum(kt, s);
+            elem8_t pf[2 * NT];
+            sums[0] = sums[1] = 0.f;
+            // (behind the last tile: products with what lies there, that nobody looks at)
+            scores(shared.k + ((it + 1) & 1) * TILE, s_next, [&](int i) { weigh(s, m_use, pf, i * ((16 + KS - 1) / KS), (16 + KS - 1) / KS); });
+            l_i += sums[0] + sums[1];
+            add_values(shared.v + (it & 1) * TILE, pf);
+        };
+        for (int it = 0; it < n_tiles; it += 2) {
+            step(it, s_acc[0], s_acc[1]);
+            if (it + 1 < n_tiles) step(it + 1, s_acc[1], s_acc[0]);
+        }
+    } else {
+        for (int it = 0; it < n_tiles; ++it) {
+            const int kt = s0 + it * BN;
+            const bool active = kt < wmax;
+            if constexpr (!kRoles) wait_for(it, C1{}, C1{});   // K tile it; behind it came V tile it and K tile it + 1
+            else if (of_k) wait_for(it, C0{}, C1{});
+            __syncthreads();                               // everybody's part of it; and nobody reads V tile it - 1 any more
+            if (of_v) request(it + 1, vbase, v_ring);
+            elem8_t pf[2 * NT];
+            if (active) {
+                f32x16_t s_acc[NT];
+                scores(shared.k + (it & 1) * TILE, s_acc, [](int) {});
+                const float m_use = maximum(kt, s_acc);
+                sums[0] = sums[1] = 0.f;
+                weigh(s_acc, m_use, pf, 0, 16 * NT);
+                l_i += sums[0] + sums[1];
             }
+            if (it + 34 < n_tiles && ((it + 2) & 31) == 0) look_up(it + 34, 32);
+            if constexpr (!kRoles) wait_for(it, C0{}, C2{});   // V tile it; behind it came K and V tile it + 1
+            else if (of_v) wait_for(it, C0{}, C1{});
+            __syncthreads();                               // everybody's part of it; and nobody reads K tile it any more
+            if (of_k) request(it + 2, kbase, k_ring);
+            if (active) add_values(shared.v + (it & 1) * TILE, pf);
         }
     }
 
@@ -1155,7 +1214,7 @@ template <int D, int NB> __global__ __launch_bounds__(256, NB == 1 ? kSmallAtOnc
         SmallShared<D, BN> tiles;
         RowsShared<D, NB> rows;
     } shared;
-    if ((int)blockIdx.x < tiles) prefix_tiles<D, BN>(p, blockIdx.x, shared.tiles);
+    if ((int)blockIdx.x < tiles) prefix_tiles<D, BN, NB == 2>(p, blockIdx.x, shared.tiles);
     else paged_rows<D, NB, PrefixParams>(p, blockIdx.x - tiles, shared.rows);
 }
 
@@ -1431,10 +1490,10 @@ PrefixPlans prefix_plans(int64_t tokens, int64_t batch, int64_t groups, int64_t 
     if (alone && average > kRowBlock) o.plans.row_block = 2 * kRowBlock;
     rows.rows_up_to = tiles.rows_over = alone ? kRowsAlone : average <= 3 * kRowBlock / 2 ? 2 * kRowBlock : o.plans.row_block;
     rows.max_n = tiles.max_n = 0x7fffffff;
-    // Prefixes that are cut into pieces, of more blocks than paged_rows takes, go together with the sequences' own keys, for half (two thirds, where two workgroups run on a
-    // compute unit) of what runs at once.  (us, two launches and one: 4 groups of 12 - 13 sequences over 700 - 6000 keys, 16 / 4 heads of 64, 28.6 and 20.0; 64 sequences over 4096
-    // keys, 32 / 8 heads of 128, 46.5 and 34.4, for a third 38.3 and for two thirds 38.1; 128 over 16384 keys 113 and 102, for a third 110; 4 x 16 over 8000 keys 59 and
-    // 45; 32 drafts over 8192 keys 68.8 and 62.4.  Groups that hardly ever have more rows than paged_rows takes: 16 of 16 - 20 rows 41.3 and 44.9.)
+    // Prefixes that are cut into pieces, of more blocks than paged_rows takes, go together with the sequences' own keys, for half of what runs at once.  (us, two launches and
+    // one: 4 groups of 12 - 13 sequences over 700 - 6000 keys, 16 / 4 heads of 64, 28.6 and 20.0; 64 sequences over 4096 keys, 32 / 8 heads of 128, 46.5 and 33.9, for a third
+    // 38.3 and for two thirds 38.1; 128 over 16384 keys 113 and 98, for a third 110; 4 x 16 over 8000 keys 59 and 45; 32 drafts over 8192 keys 68.8 and 54.  Groups
+    // that hardly ever have more rows than paged_rows takes: 16 of 16 - 20 rows 41.3 and 44.9.)
     o.together = !alone && average > 3 * kRowBlock / 2 && tiles.share > 0;
     o.plans.tile_rows = (int)std::min<int64_t>((tokens * n_rep + 15) / 16 * 16, o.together ? kSmallRows : kTileRows);
     if (o.together) tiles.fit = share_of(o.plans.row_block == kRowBlock ? kSmallAtOnce * mi_compute_units() / 2 : mi_compute_units(), nkv);
