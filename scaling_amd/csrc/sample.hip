@@ -36,6 +36,43 @@ __device__ __forceinline__ uint32_t value_key(float x) {
 }
 __device__ __forceinline__ float key_value(uint32_t key) { return __uint_as_float((key & 0x80000000u) != 0 ? key & 0x7fffffffu : ~key); }
 
+// Values of keys lo to hi as a test of a value's bits: its positive and its negative part, with both zeros where zero is in it (one of two parts that are alike, where
+// there is only one).  NaN is in none.
+struct Interval {
+    uint32_t a0, n0, a1, n1;
+    __device__ __forceinline__ Interval(uint32_t lo, uint32_t hi) {
+        constexpr uint32_t kZero = 0x80000000u;
+        if (hi == kZero - 1) --hi;                         // (no value's key; its bits are those of -0)
+        a0 = lo > kZero ? lo & 0x7fffffffu : 0;
+        n0 = (hi & 0x7fffffffu) - a0;
+        a1 = hi >= kZero ? kZero : ~hi;
+        n1 = (lo < kZero ? ~lo : kZero) - a1;
+        if (hi < kZero) { a0 = a1; n0 = n1; }
+        if (lo > kZero) { a1 = a0; n1 = n0; }
+    }
+    __device__ __forceinline__ bool holds(float x) const {
+        const uint32_t u = __float_as_uint(x);
+        return (u - a0 <= n0) | (u - a1 <= n1);
+    }
+};
+// The smallest key of lo to hi that `reached` holds for, as it does for all above and for hi: 64 keys at a time by a wavefront.
+template <class F> __device__ __forceinline__ uint32_t first_key(uint32_t lo, uint32_t hi, const F& reached) {
+    const uint32_t lane = threadIdx.x & 63;
+    while (lo < hi) {
+        const uint32_t n = hi - lo, step = n / 64 + 1, at = lane * step <= n ? lo + lane * step : hi;
+        const uint64_t those = __ballot(reached(at));
+        if (those == 0) {                                  // (lane 63 may be short of hi)
+            lo = (uint32_t)__builtin_amdgcn_readlane((int)at, 63) + 1;
+            continue;
+        }
+        const int l = __builtin_ctzll(those);
+        hi = (uint32_t)__builtin_amdgcn_readlane((int)at, l);
+        if (l == 0) break;
+        lo = (uint32_t)__builtin_amdgcn_readlane((int)at, l - 1) + 1;
+    }
+    return hi;
+}
+
 // A row as aligned 16-byte vectors, with the elements in front of the first and behind the last (at most a vector's less one each) one to a thread.
 template <typename T> struct Row {
     static constexpr int V = Elem<T>::kVec, kAhead = 4;
@@ -207,7 +244,7 @@ __device__ __forceinline__ void range(Shared& s, uint32_t& lo, uint32_t& hi) {
 }
 
 // ---- searches -------------------------------------------------------------------------------------------------------------------------------------------
-// Values of an interval of keys in kBins bins, largest first: of equal width in value, or in key.
+// Values of keys lo to hi in kBins bins, largest first: of equal width in value, or in key.
 struct Bins {
     uint32_t lo, hi;
     float top, scale;                                      // scale 0: by key
@@ -217,10 +254,13 @@ struct Bins {
         const float top = key_value(hi), range = top - key_value(lo), scale = (float)kBins / range;
         return range > 0.f && range < INFINITY && scale < INFINITY ? Bins{lo, hi, top, scale, 0} : Bins{lo, hi, 0.f, 0.f, hi > lo ? max(0, 32 - (int)__builtin_clz(hi - lo) - 12) : 0};
     }
-    __device__ __forceinline__ bool holds(uint32_t key) const { return key >= lo && key <= hi; }
-    __device__ __forceinline__ int of(float x, uint32_t key) const {
-        return scale > 0.f ? min((int)((top - x) * scale), kBins - 1) : (int)((hi - key) >> shift);
+    __device__ __forceinline__ int of(float x) const { return scale > 0.f ? min((int)((top - x) * scale), kBins - 1) : (int)((hi - value_key(x)) >> shift); }
+    // the smallest key of bins 0 to `bin`
+    __device__ __forceinline__ uint32_t from(int bin) const {
+        return first_key(lo, hi, [&](uint32_t key) { return of(key_value(key)) <= bin; });
     }
+    // what a bin, that holds something, holds
+    __device__ __forceinline__ Interval interval(int bin) const { return Interval(from(bin), bin > 0 ? from(bin - 1) - 1 : hi); }
 };
 
 struct Found {
@@ -242,10 +282,10 @@ template <typename T, class ROW> struct Search {
         __syncthreads();
         for (int i = threadIdx.x; i < kBins; i += kThreads) { s.count[i] = 0; s.weight[i] = 0; }
         __syncthreads();
+        const Interval asked(bins.lo, bins.hi);
         row.each([&](float x, int) {
-            const uint32_t key = value_key(x);
-            if (!bins.holds(key)) return;
-            const int b = bins.of(x, key);
+            if (!asked.holds(x)) return;
+            const int b = bins.of(x);
             atomicAdd(&s.count[b], 1u);
             if (weighed) atomicAdd((unsigned long long*)&s.weight[b], (unsigned long long)weights.whole_of(x));
         });
@@ -301,12 +341,14 @@ template <typename T, class ROW> struct Search {
         for (;;) {
             const int bin = bin_of(by_count, goal, before);
             const uint32_t n = s.count[bin];
-            const auto in_bin = [&](float x, uint32_t key) { return bins.holds(key) && bins.of(x, key) == bin; };
+            const Interval in_bin = bins.interval(bin);
             if (n <= kCandidates) return among(in_bin, (int)n, by_count, goal, before);
             uint32_t lo = 0xffffffffu, hi = 0;
             row.each([&](float x, int) {
+                if (!in_bin.holds(x)) return;
                 const uint32_t key = value_key(x);
-                if (in_bin(x, key)) { lo = min(lo, key); hi = max(hi, key); }
+                lo = min(lo, key);
+                hi = max(hi, key);
             });
             range(s, lo, hi);
             if (lo == hi) return equals(lo, n, by_count, goal, before, want_index);
@@ -317,14 +359,13 @@ template <typename T, class ROW> struct Search {
     }
 
     // ... of the few tokens of a bin
-    template <class F> __device__ __forceinline__ Found among(const F& in_bin, int n, bool by_count, uint64_t goal, Mass before) {
+    __device__ __forceinline__ Found among(const Interval& in_bin, int n, bool by_count, uint64_t goal, Mass before) {
         __syncthreads();
         if (threadIdx.x == 0) s.number = 0;
         __syncthreads();
         row.each([&](float x, int i) {
-            const uint32_t key = value_key(x);
-            if (!in_bin(x, key)) return;
-            s.candidates[min(atomicAdd(&s.number, 1u), (uint32_t)kCandidates - 1)] = (uint64_t)~key << 32 | (uint32_t)i;
+            if (!in_bin.holds(x)) return;
+            s.candidates[min(atomicAdd(&s.number, 1u), (uint32_t)kCandidates - 1)] = (uint64_t)~value_key(x) << 32 | (uint32_t)i;
         });
         __syncthreads();
         Mass mine{0, 0}, all;
@@ -371,7 +412,8 @@ template <typename T, class ROW> struct Search {
         __syncthreads();
         for (int i = threadIdx.x; i < kBins; i += kThreads) { s.count[i] = 0; s.weight[i] = 0; }
         __syncthreads();
-        row.each([&](float x, int i) { if (value_key(x) == key) atomicAdd(&s.count[i / width], 1u); });
+        const Interval equal(key, key);
+        row.each([&](float x, int i) { if (equal.holds(x)) atomicAdd(&s.count[i / width], 1u); });
         __syncthreads();
         Mass none{0, 0};
         const int bin = bin_of(true, nth, none);
@@ -407,6 +449,14 @@ struct Parameters {
         any_min_p = m_bits - 1u < 0x7f800000u;
         min_p = (double)__uint_as_float(m_bits);
     }
+    // Keys lo to hi, hi the largest: from where on the logarithm of a weight may be `log` or more (a little below the value that this stands for).
+    __device__ __forceinline__ uint32_t from(uint32_t lo, uint32_t hi, double log) const {
+        const double largest = (double)key_value(hi), at = largest + log / inverse, x = at - 1e-6 * fmax(fabs(at), fabs(largest));
+        if (key_value(hi) == INFINITY || !(inverse > 0.0) || !(x > -3e38)) return lo;      // (no float may be lower than x)
+        const uint32_t key = value_key((float)x);
+        return key > lo && key <= hi ? key : lo;
+    }
+    __device__ __forceinline__ uint32_t heavy_from(uint32_t lo, uint32_t hi) const { return from(lo, hi, log(min_p)); }
 };
 
 // The token of what top-k (k > 0), top-p and min-p leave of the weight `kept`, and how much that is: find(step, goal), of step 0 by count,
@@ -451,9 +501,9 @@ template <typename T> __device__ __forceinline__ Gathered gather(Shared& s, uint
     __syncthreads();
     if (threadIdx.x == 0) s.number = 0;
     __syncthreads();
+    const Interval asked(lo, 0xff800000u);
     row.each([&](float x, int i) {
-        const uint32_t key = value_key(x);
-        if (key >= lo) gathered[min(atomicAdd(&s.number, 1u), (uint32_t)kGathered - 1)] = (uint64_t)~key << 32 | (uint32_t)i;
+        if (asked.holds(x)) gathered[min(atomicAdd(&s.number, 1u), (uint32_t)kGathered - 1)] = (uint64_t)~value_key(x) << 32 | (uint32_t)i;
     });
     __syncthreads();
     const Gathered few{gathered, min((int)s.number, kGathered)};
@@ -479,7 +529,7 @@ __device__ __forceinline__ bool sort(Shared& s, uint64_t* tokens, int n, uint32_
         if (i >= n) break;
         token[e] = tokens[i];
         const uint32_t key = ~(uint32_t)(token[e] >> 32);
-        bin[e] = bins.of(key_value(key), key);
+        bin[e] = bins.of(key_value(key));
         place[e] = atomicAdd(&s.count[bin[e]], 1u);
     }
     __syncthreads();
@@ -581,8 +631,9 @@ __device__ __forceinline__ void sample_from(Shared& s, uint64_t* gathered, const
         if (of.any_min_p) {
             const double least = ldexp(of.min_p, w.bits);
             uint64_t weight = 0;
+            const Interval asked(of.heavy_from(lo, hi), hi);
             search.row.each([&](float x, int) {
-                if (value_key(x) < lo) return;
+                if (!asked.holds(x)) return;
                 const double v = w.of(x);
                 if (v >= least) weight += w.whole(v);
             });
@@ -601,12 +652,7 @@ __device__ __forceinline__ void sample_from(Shared& s, uint64_t* gathered, const
             const double least = ceil((double)all.weight * of.top_p);
             const int bin = search.bin_of(false, least < 1.0 ? 1 : (uint64_t)least, front);
             if (front.count + s.count[bin] <= (uint64_t)kGathered) {
-                uint32_t from = 0xffffffffu, none = 0;
-                row.each([&](float x, int) {
-                    const uint32_t key = value_key(x);
-                    if (search.first.holds(key) && search.first.of(x, key) <= bin) from = min(from, key);
-                });
-                range(s, from, none);
+                const uint32_t from = search.first.from(bin);
                 const Gathered few = gather(s, gathered, whole, from);
                 if (sort(s, gathered, few.n, from, hi)) return sample_sorted(s, p, r, of, w, gathered, few.n, 0, all.weight);
                 Search<T, Gathered> rest{s, few, whole, w, false, {}, false};
@@ -616,6 +662,13 @@ __device__ __forceinline__ void sample_from(Shared& s, uint64_t* gathered, const
         }
     }
     finish(search);
+}
+
+// A value's place among all: the values' order, and below the lowest finite one (kLowest) -inf and NaN.
+constexpr uint32_t kPlace = 0x007fffffu, kLowest = 0x00ffffffu;
+__device__ __forceinline__ uint32_t place_of(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return (u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u)) + kPlace;        // (NaN of either sign wraps)
 }
 
 template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) {
@@ -629,43 +682,50 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     constexpr int kCoarseEach = kCoarseBins / kThreads;
     for (int i = threadIdx.x; i < kCoarseBins; i += kThreads) coarse[i] = 0;
     __syncthreads();
-    uint32_t lo = 0xffffffffu, hi = 0;
+    uint32_t n_lowest = 0, most = 0;
     row.each([&](float x, int) {
-        const uint32_t key = value_key(x);
-        if (key == 0) return;
-        lo = min(lo, key);
-        hi = max(hi, key);
-        atomicAdd(&coarse[~key >> kCoarse], 1u);           // largest first
+        const uint32_t at = place_of(x);
+        most = max(most, at);
+        if (at > kLowest) atomicAdd(&coarse[~at >> kCoarse], 1u);              // largest first
+        else n_lowest += at == kLowest;                    // (masked tokens may be many, and adding to one word takes turns)
     });
-    range(s, lo, hi);
-    if (hi == 0) return write_nothing(p, r);
+    n_lowest = group_reduce_bits<64>(n_lowest, [](uint32_t a, uint32_t b) { return a + b; });
+    if ((threadIdx.x & 63) == 0 && n_lowest > 0) atomicAdd(&coarse[~kLowest >> kCoarse], n_lowest);
+    uint32_t none = 0;
+    range(s, none, most);
+    if (most < kLowest) return write_nothing(p, r);
+    const uint32_t hi = value_key(key_value(most - kPlace));
+    const auto edge = [](int bin) { return max((uint32_t)~(((uint64_t)(bin + 1) << kCoarse) - 1), kLowest) - kPlace; };      // the smallest key of a bin
     // ---- from where on tokens are asked for, and how many there are ----
     uint32_t here[kCoarseEach];
     uint64_t mine = 0, n_all;
+    uint32_t last = 0;
 #pragma unroll
-    for (int i = 0; i < kCoarseEach; ++i) { here[i] = coarse[kCoarseEach * threadIdx.x + i]; mine += here[i]; }
+    for (int i = 0; i < kCoarseEach; ++i) {
+        here[i] = coarse[kCoarseEach * threadIdx.x + i];
+        mine += here[i];
+        if (here[i] > 0) last = kCoarseEach * threadIdx.x + i;
+    }
     uint64_t upto = scan(s.partial, mine, n_all);
+    range(s, none, last);
+    uint32_t lo = edge((int)last);
     const int k = of.k > 0 && (uint64_t)of.k < n_all ? of.k : 0;
     if (k > 0) {
 #pragma unroll
         for (int i = 0; i < kCoarseEach; ++i) {
-            if (upto < (uint64_t)k && upto + here[i] >= (uint64_t)k)
-                s.word[0] = (uint32_t)~(((uint64_t)(kCoarseEach * threadIdx.x + i + 1) << kCoarse) - 1);     // the smallest key of the bin
+            if (upto < (uint64_t)k && upto + here[i] >= (uint64_t)k) s.word[0] = edge(kCoarseEach * threadIdx.x + i);
             upto += here[i];
         }
         __syncthreads();
         lo = max(lo, (uint32_t)s.word[0]);
     }
-    if (of.any_min_p && of.top_p_none) {                   // a little below the value that min_p stands for
-        const double largest = (double)key_value(hi), at = largest + log(of.min_p) / of.inverse, x = at - 1e-6 * fmax(fabs(at), fabs(largest));
-        const uint32_t key = value_key((float)fmax(x, -3e38));
-        if (key_value(hi) < INFINITY && of.inverse > 0.0 && x > -3e38 && key > lo && key <= hi) lo = key;      // (no float may be lower than x)
-    }
+    if (of.any_min_p && of.top_p_none) lo = of.heavy_from(lo, hi);
+    lo = of.from(lo, hi, -0.693147180559945309417 * (weight_bits(row.vocab) + 2));      // (those below weigh nothing: no sum, and no search by one, has to do with them)
     uint64_t n_asked;                                      // those of the bins down to the last one's
     mine = 0;
 #pragma unroll
     for (int i = 0; i < kCoarseEach; ++i)
-        if (kCoarseEach * (int)threadIdx.x + i <= (int)(~lo >> kCoarse)) mine += here[i];
+        if (kCoarseEach * (int)threadIdx.x + i <= (int)(~(lo + kPlace) >> kCoarse)) mine += here[i];
     scan(s.partial, mine, n_asked);
     if (n_asked > kGathered) return sample_from<T>(s, gathered, p, r, of, row, row, lo, hi, k);
     const Gathered few = gather(s, gathered, row, lo);
@@ -690,6 +750,7 @@ struct KeyShared {
     uint64_t heavy;
     uint32_t occupied[kWaves];
     int found, index, nth, n_aside;
+    uint32_t frequent, n_frequent;                         // bits of a value that many tokens have, and how many of them are not in the counts
     uint32_t aside[kAside];                                // bits of a value that 32768 more tokens have
 };
 
@@ -703,7 +764,7 @@ typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
 
 template <typename T, int NV> __global__ __launch_bounds__(kThreads) void sample_keys_kernel(const SampleParams p) {
     using K = Key16<T>;
-    constexpr uint32_t kMinusInf = K::kInf | 0x8000u;
+    constexpr uint32_t kNothing = 0x10000;                 // no value's bits
     static_assert(K::kInf % kUnit == 0 && NV % 4 == 0, "infinities begin a unit; pieces of four vectors a thread");
     __shared__ KeyShared s;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -752,37 +813,50 @@ template <typename T, int NV> __global__ __launch_bounds__(kThreads) void sample
     int pieces = 0;                                        // 1: counts are put aside between pieces
     for (;;) {
         for (int i = tid; i < kMagnitudes / 4; i += kThreads) reinterpret_cast<uint4*>(s.counts)[i] = make_uint4(0, 0, 0, 0);
-        if (tid == 0) { s.n_aside = s.found = 0; s.heavy = 0; }
+        s.unit_count[tid] = 0;                             // (a lane's place for the frequent value)
+        if (tid == 0) { s.n_aside = s.found = 0; s.heavy = 0; s.frequent = kNothing; s.n_frequent = 0; }
         __syncthreads();
         const auto add = [&](uint32_t at, uint32_t negative) {       // (1, or 2^16 for a negative value)
             uint32_t what;
             asm("v_mad_u32_u24 %0, %1, %2, 1" : "=v"(what) : "v"(negative), "s"(0xffff));
             atomicAdd(reinterpret_cast<uint32_t*>(reinterpret_cast<char*>(s.counts) + at), what);
         };
-        // Masked tokens, -inf, are many: to the lanes' own places among the NaN, where nothing is looked at (words that are added to at once take turns).
-        const auto add_vector = [&](const uint4& u, auto masked) {
+        // One value may be most of a row's, as those of masked tokens are, and words that are added to at once take turns: the lanes have places of their own for it.  It is the
+        // first one that a wavefront finds in many lanes.  (us of 64 x 128256, three quarters of which are the lowest value: 190 in one word, 21.)
+        constexpr int kMany = 16, kStillMany = 8;
+        const uint32_t own = offsetof(KeyShared, unit_count) + 4 * tid;
+#pragma unroll
+        for (int i = 0; i < 6; ++i) {
+            const int v = i / 2 * (NV - 1) / 2;            // the first, a middle and the last of a whole row's
+            const uint32_t candidate = (uint32_t)__builtin_amdgcn_readfirstlane((int)(i % 2 == 0 ? held[v].x : held[v].y)) & 0xffffu;
+            if ((v + 1) * kThreads <= row.vecs && __popcll(__ballot((held[v].z & 0xffffu) == candidate)) >= kMany && lane == 0) atomicCAS(&s.frequent, kNothing, candidate);
+        }
+        __syncthreads();
+        const uint32_t frequent = (uint32_t)__builtin_amdgcn_readfirstlane((int)s.frequent);
+        const auto add_vector = [&](const uint4& u, auto some) {
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-            const uint32_t own = 4 * (K::kInf + 1 + lane);
+            const uint32_t those = frequent << 16;
+            const auto place = [&](uint32_t high, uint32_t at) { return decltype(some)::value && (high ^ those) <= 0xffffu ? own : at; };
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t low = (w[i] << 2) & 0x1fffcu, high = (w[i] >> 14) & 0x1fffcu;
-                add(decltype(masked)::value && (w[i] << 16) >= kMinusInf << 16 ? own : low, w[i] >> 15 & 1);
-                add(decltype(masked)::value && w[i] >= kMinusInf << 16 ? own : high, w[i] >> 31);
+                add(place(w[i] << 16, low), w[i] >> 15 & 1);
+                add(place(w[i], high), w[i] >> 31);
             }
         };
         vectors([&](const uint4& u, int) {
-            u16x2_t most = __builtin_bit_cast(u16x2_t, u.x);
-            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, u.y));
-            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, u.z));
-            most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, u.w));
-            if (__any(most[0] >= kMinusInf || most[1] >= kMinusInf)) add_vector(u, std::true_type{});
+            if (frequent != kNothing && __popcll(__ballot((u.x & 0xffffu) == frequent)) >= kStillMany) add_vector(u, std::true_type{});
             else add_vector(u, std::false_type{});
         }, [&]() { if (pieces != 0) put_aside(); });
         if (single < row.vocab) add(4 * (single_bits & 0x7fffu), single_bits >> 15);
+        if (frequent != kNothing) {
+            const int n = __builtin_amdgcn_readlane(prefix_sum((int)(s.unit_count[tid] >> (frequent >> 15 << 4))), 63);
+            if (lane == 0) atomicAdd(&s.n_frequent, (uint32_t)n);
+        }
         if (pieces != 0) put_aside();                      // (the last ones: fewer than a vector)
         __syncthreads();
         if (pieces != 0 || row.vocab <= 0xffff) break;
-        uint32_t found = 0;
+        uint32_t found = tid == 0 ? s.n_frequent : 0;
         for (int i = tid; i < kMagnitudes / 4; i += kThreads) {
             const uint4 c = reinterpret_cast<const uint4*>(s.counts)[i];
             found += (c.x & 0xffffu) + (c.x >> 16) + (c.y & 0xffffu) + (c.y >> 16) + (c.z & 0xffffu) + (c.z >> 16) + (c.w & 0xffffu) + (c.w >> 16);
@@ -795,10 +869,12 @@ template <typename T, int NV> __global__ __launch_bounds__(kThreads) void sample
         __syncthreads();
     }
     const int n_aside = s.n_aside;
+    const uint32_t frequent = s.frequent, n_frequent = s.n_frequent;
     const auto count_of = [&](uint32_t key) -> uint32_t {
         if (key > K::kTop || key <= K::kNone || key == 0x7fffu) return 0;
         const uint32_t bits = K::bits(key), both = s.counts[bits & 0x7fffu];
         uint32_t c = (bits >> 15 ? 0 : both & 0xffffu) + (bits >> 15 || bits == 0 ? both >> 16 : 0);
+        c += bits == frequent || (bits == 0 && frequent == 0x8000u) ? n_frequent : 0;
         for (int i = 0; i < n_aside; ++i) c += s.aside[i] == bits || (bits == 0 && s.aside[i] == 0x8000u) ? 32768 : 0;
         return c;
     };
@@ -821,10 +897,12 @@ template <typename T, int NV> __global__ __launch_bounds__(kThreads) void sample
             in_unit = (int)(of_unit[0].x & 0xffffu);
         }
         if (from == 0) in_unit += positive ? (int)(s.counts[0] >> 16) : -(int)(s.counts[0] >> 16);                 // -0
-        for (int i = 0; i < n_aside; ++i) {
-            const uint32_t x = s.aside[i] == 0x8000u ? 0 : s.aside[i];
-            if ((x >> 15 == 0) == positive && (int)(x & 0x7fffu) >= from && (int)(x & 0x7fffu) < from + kUnit && (int)(x & 0x7fffu) <= (int)K::kInf - !positive) in_unit += 32768;
-        }
+        const auto add = [&](uint32_t bits, int n) {
+            const uint32_t x = bits == 0x8000u ? 0 : bits;
+            if ((x >> 15 == 0) == positive && (int)(x & 0x7fffu) >= from && (int)(x & 0x7fffu) < from + kUnit && (int)(x & 0x7fffu) <= (int)K::kInf - !positive) in_unit += n;
+        };
+        if (n_frequent > 0) add(frequent, (int)n_frequent);
+        for (int i = 0; i < n_aside; ++i) add(s.aside[i], 32768);
     }
     const uint64_t occupied = __ballot(in_unit > 0);
     const int counts_upto = prefix_sum(in_unit);

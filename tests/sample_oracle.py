@@ -29,7 +29,7 @@ def row(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if not temperature > 0:
         return int(order[0]), 0.0, {int(order[0])}
     u = 0.0 if math.isnan(u) else min(max(u, 0.0), 1.0 - 2.0 ** -24)
-    z = torch.where(v == v[0], 0.0, (v - v[0]) / temperature) if not math.isinf(float(v[0])) else torch.where(v == v[0], 0.0, -math.inf)
+    z = torch.where(v == v[0], 0.0, (v - v[0]) / temperature) if not math.isinf(float(v[0])) else torch.where(v == v[0], 0.0, -math.inf).double()
     w = torch.exp(z)
     S = w.cumsum(0)
     n_k = min(top_k, len(w)) if top_k > 0 else len(w)

@@ -194,6 +194,27 @@ def test_min_p_far_below(dtype):
     _check(x, [0.99, 0.5, 0.2, 0.9, 0.7, 0.999], temperature=[-low / 4, -low / 3, math.inf, -low / 2, 60000.0 / math.log(1000.0), 1.0], min_p=[1e-3, 1e-3, 0.5, 0.05, 1e-3, 1e-3])
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("value", [-math.inf, "lowest", -1e4, 0.0, -0.0, 3.5, math.inf, math.nan])
+def test_one_value_most_of_the_row(value, dtype):
+    """Masked tokens and the like: more than 65535 of one value, beside another one that is frequent, everywhere or only at an end of the row; NaN of any payload among them."""
+    vocab, value = 140003, torch.finfo(dtype).min if value == "lowest" else value
+    print(f"case {value} {dtype}", flush=True)
+    x = _logits(6, vocab, dtype, seed=30)
+    at = torch.rand(6, vocab, generator=torch.Generator().manual_seed(31))
+    x[:3] = x[:3].masked_fill(at[:3] < 0.9, value)
+    x[3, 40000:130000] = value
+    x[4] = value
+    x[5] = x[5].masked_fill(at[5] < 0.4, value).masked_fill(at[5] > 0.6, -2.25)
+    if dtype != torch.float32:
+        ints = torch.int16
+        payloads = (torch.arange(200, dtype=torch.int32) % 127 + (0x7f81 if dtype == torch.bfloat16 else 0x7c01)).to(ints)
+        x[1, 777:977], x[2, 777:977] = payloads.view(dtype), (payloads | torch.tensor(-32768, dtype=ints)).view(dtype)
+    u = [0.3, 1 - 2.0 ** -24, 0.999, 0.5, 0.77, 0.9]
+    _check(x, u, temperature=[1.0, math.inf, 3e4, 1.0, 1.0, 2.0])
+    _check(x, u, temperature=[1.0, math.inf, 1.0, 1.0, 1.0, 2.0], top_k=[0, 90000, 20000, 51000, 139000, 30000], top_p=[0.9, 1.0, 0.99, 0.5, 0.7, 0.8])
+
+
 def test_far_rows():
     """Offsets over 2^31 elements."""
     stride = (1 << 31) // 3 + 1001
