@@ -266,29 +266,39 @@ struct Bins {
 struct Found {
     uint32_t key;                                          // of the token
     int index;                                             // -1 unless asked for
-    Mass upto;                                             // tokens up to it, it included
+    uint64_t upto;                                         // tokens up to it, it included, or their weight
 };
 
+// Searches by count or by weight, in bins that hold the one or the other: adding to LDS is what a pass over a row waits for.  (us of 64 x 128256 by top-p: 111 with
+// both, 100.)
 template <typename T, class ROW> struct Search {
     Shared& s;
     const ROW& row;                                        // the tokens that are looked at
     const Row<T>& whole;
     const Weights& weights;
-    bool weighed;                                          // bins of counts and weights, or of counts alone
+    bool weighed;                                          // bins of weights, or of counts
     Bins first;
     bool filled;                                           // with the first bins
+    uint32_t passed;                                       // tokens in them, of this thread's
 
+    __device__ __forceinline__ uint64_t in(int bin) const { return weighed ? s.weight[bin] : s.count[bin]; }
     __device__ __forceinline__ void fill(const Bins& bins) {
         __syncthreads();
-        for (int i = threadIdx.x; i < kBins; i += kThreads) { s.count[i] = 0; s.weight[i] = 0; }
+        for (int i = threadIdx.x; i < kBins; i += kThreads) {
+            if (weighed) s.weight[i] = 0;
+            else s.count[i] = 0;
+        }
         __syncthreads();
         const Interval asked(bins.lo, bins.hi);
+        uint32_t n = 0;
         row.each([&](float x, int) {
             if (!asked.holds(x)) return;
             const int b = bins.of(x);
-            atomicAdd(&s.count[b], 1u);
+            ++n;
             if (weighed) atomicAdd((unsigned long long*)&s.weight[b], (unsigned long long)weights.whole_of(x));
+            else atomicAdd(&s.count[b], 1u);
         });
+        passed = n;
         __syncthreads();
     }
     // All tokens of keys lo to hi, lo at least 1.
@@ -300,49 +310,56 @@ template <typename T, class ROW> struct Search {
     }
 
     // What all bins hold.
-    __device__ __forceinline__ Mass all() const {
-        Mass mine{0, 0}, sum;
-        for (int i = threadIdx.x; i < kBins; i += kThreads) { mine.count += s.count[i]; mine.weight += s.weight[i]; }
+    __device__ __forceinline__ uint64_t all() const {
+        uint64_t mine = 0, sum;
+        for (int i = threadIdx.x; i < kBins; i += kThreads) mine += in(i);
         scan(s.partial, mine, sum);
         return sum;
     }
+    __device__ __forceinline__ uint64_t tokens() const {
+        uint64_t sum;
+        scan(s.partial, (uint64_t)passed, sum);
+        return sum;
+    }
 
-    // The bin in which the count or weight reaches `goal`, with what lies in front of it.
-    __device__ __forceinline__ int bin_of(bool by_count, uint64_t goal, Mass& before) {
+    // The bin in which what `value` gives reaches `goal`, with what lies in front of it.
+    template <class F> __device__ __forceinline__ int bin_of(const F& value, uint64_t goal, uint64_t& before) {
         constexpr int kEach = kBins / kThreads;
-        Mass mine{0, 0}, all;
-        for (int i = 0; i < kEach; ++i) { mine.count += s.count[kEach * threadIdx.x + i]; mine.weight += s.weight[kEach * threadIdx.x + i]; }
-        Mass at = scan(s.partial, mine, all);
-        at.count += before.count;
-        at.weight += before.weight;
+        uint64_t mine = 0, all;
+        for (int i = 0; i < kEach; ++i) mine += value(kEach * threadIdx.x + i);
+        uint64_t at = scan(s.partial, mine, all) + before;
         if (threadIdx.x == 0) s.number = 0;
         __syncthreads();
         for (int i = 0; i < kEach; ++i) {
             const int b = kEach * threadIdx.x + i;
-            const Mass next{at.count + s.count[b], at.weight + s.weight[b]};
-            if (by_count ? at.count < goal && next.count >= goal : at.weight < goal && next.weight >= goal) {
+            const uint64_t next = at + value(b);
+            if (at < goal && next >= goal) {
                 s.number = b;
-                s.word[0] = at.count;
-                s.word[1] = at.weight;
+                s.word[0] = at;
             }
             at = next;
         }
         __syncthreads();
-        const int b = (int)s.number;
-        before = Mass{s.word[0], s.word[1]};
-        return b;
+        before = s.word[0];
+        return (int)s.number;
+    }
+    __device__ __forceinline__ int bin_of(uint64_t goal, uint64_t& before) {
+        return bin_of([&](int b) { return in(b); }, goal, before);
     }
 
     // The first token up to which there are `goal` tokens, or there is that much weight: at least 1, at most what there is.
-    __device__ __forceinline__ Found find(bool by_count, uint64_t goal, bool want_index) {
+    __device__ __forceinline__ Found find(uint64_t goal, bool want_index) {
         Bins bins = first;
-        Mass before{0, 0};
+        uint64_t before = 0;
         if (!filled) { fill(bins); filled = true; }
         for (;;) {
-            const int bin = bin_of(by_count, goal, before);
-            const uint32_t n = s.count[bin];
+            const int bin = bin_of(goal, before);
             const Interval in_bin = bins.interval(bin);
-            if (n <= kCandidates) return among(in_bin, (int)n, by_count, goal, before);
+            uint32_t n = weighed ? 0 : s.count[bin];
+            if (n <= kCandidates) {
+                n = collect(in_bin);
+                if (n <= kCandidates) return among((int)n, goal, before);
+            }
             uint32_t lo = 0xffffffffu, hi = 0;
             row.each([&](float x, int) {
                 if (!in_bin.holds(x)) return;
@@ -351,24 +368,31 @@ template <typename T, class ROW> struct Search {
                 hi = max(hi, key);
             });
             range(s, lo, hi);
-            if (lo == hi) return equals(lo, n, by_count, goal, before, want_index);
+            if (lo == hi) return equals(lo, n, goal, before, want_index);
             bins = Bins{lo, hi, 0.f, 0.f, max(0, 32 - (int)__builtin_clz(hi - lo) - 12)};
             fill(bins);
             filled = false;
         }
     }
 
-    // ... of the few tokens of a bin
-    __device__ __forceinline__ Found among(const Interval& in_bin, int n, bool by_count, uint64_t goal, Mass before) {
+    // The tokens of an interval, as far as there is room; how many there are.
+    __device__ __forceinline__ uint32_t collect(const Interval& those) {
         __syncthreads();
         if (threadIdx.x == 0) s.number = 0;
         __syncthreads();
         row.each([&](float x, int i) {
-            if (!in_bin.holds(x)) return;
-            s.candidates[min(atomicAdd(&s.number, 1u), (uint32_t)kCandidates - 1)] = (uint64_t)~value_key(x) << 32 | (uint32_t)i;
+            if (!those.holds(x)) return;
+            const uint32_t at = atomicAdd(&s.number, 1u);
+            if (at < (uint32_t)kCandidates) s.candidates[at] = (uint64_t)~value_key(x) << 32 | (uint32_t)i;
         });
         __syncthreads();
-        Mass mine{0, 0}, all;
+        const uint32_t n = s.number;
+        __syncthreads();
+        return n;
+    }
+
+    // ... of the few tokens of a bin
+    __device__ __forceinline__ Found among(int n, uint64_t goal, uint64_t before) {
         if ((int)threadIdx.x < n) {
             const uint64_t c = s.candidates[threadIdx.x];
             int rank = 0;
@@ -378,47 +402,44 @@ template <typename T, class ROW> struct Search {
         __syncthreads();
         uint32_t key = 0;
         int index = 0;
+        uint64_t mine = 0, all;
         if ((int)threadIdx.x < n) {
             key = ~(uint32_t)(s.sorted[threadIdx.x] >> 32);
             index = (int)(uint32_t)s.sorted[threadIdx.x];
-            mine = Mass{1, weighed ? weights.whole_of(key_value(key)) : 0};
+            mine = weighed ? weights.whole_of(key_value(key)) : 1;
         }
-        Mass at = scan(s.partial, mine, all);
-        at.count += before.count;
-        at.weight += before.weight;
-        const Mass next{at.count + mine.count, at.weight + mine.weight};
-        if (by_count ? at.count < goal && next.count >= goal : at.weight < goal && next.weight >= goal) {
-            s.word[0] = next.count;
-            s.word[1] = next.weight;
+        const uint64_t at = scan(s.partial, mine, all) + before;
+        if (at < goal && at + mine >= goal) {
+            s.word[0] = at + mine;
             s.word[2] = key;
             s.word[3] = (uint32_t)index;
         }
         __syncthreads();
-        const Found f{(uint32_t)s.word[2], (int)(uint32_t)s.word[3], Mass{s.word[0], s.word[1]}};
+        const Found f{(uint32_t)s.word[2], (int)(uint32_t)s.word[3], s.word[0]};
         __syncthreads();
         return f;
     }
 
     // ... of n equal tokens
-    __device__ __forceinline__ Found equals(uint32_t key, uint32_t n, bool by_count, uint64_t goal, Mass before, bool want_index) {
-        const uint64_t w = weights.whole_of(key_value(key));
-        uint64_t nth = by_count ? goal - before.count : w > 0 ? ceil_quotient(goal - before.weight, w) : 1;       // 1 .. n
+    __device__ __forceinline__ Found equals(uint32_t key, uint32_t n, uint64_t goal, uint64_t before, bool want_index) {
+        const uint64_t w = weighed ? weights.whole_of(key_value(key)) : 1;
+        uint64_t nth = w > 0 ? ceil_quotient(goal - before, w) : 1;           // 1 .. n
         nth = nth < 1 ? 1 : nth > n ? n : nth;
-        Found f{key, -1, Mass{before.count + nth, before.weight + nth * w}};
+        Found f{key, -1, before + nth * w};
         if (!want_index) return f;
         // bins of equal width in the index
         const int width = (whole.vocab + kBins - 1) / kBins;
-        filled = false;
+        filled = filled && weighed;
         __syncthreads();
-        for (int i = threadIdx.x; i < kBins; i += kThreads) { s.count[i] = 0; s.weight[i] = 0; }
+        for (int i = threadIdx.x; i < kBins; i += kThreads) s.count[i] = 0;
         __syncthreads();
         const Interval equal(key, key);
         row.each([&](float x, int i) { if (equal.holds(x)) atomicAdd(&s.count[i / width], 1u); });
         __syncthreads();
-        Mass none{0, 0};
-        const int bin = bin_of(true, nth, none);
+        uint64_t none = 0;
+        const int bin = bin_of([&](int b) { return (uint64_t)s.count[b]; }, nth, none);
         if (threadIdx.x == 0) {
-            uint64_t left = nth - none.count;
+            uint64_t left = nth - none;
             for (int i = bin * width; i < whole.vocab && i < (bin + 1) * width; ++i)
                 if (value_key(Elem<T>::load1(whole.x + i)) == key && --left == 0) { s.word[3] = i; break; }
         }
@@ -460,7 +481,7 @@ struct Parameters {
 };
 
 // The token of what top-k (k > 0), top-p and min-p leave of the weight `kept`, and how much that is: find(step, goal), of step 0 by count,
-// gives the mass up to the first token that reaches the goal.  heavy: the weight of those of at least min_p.  (One call in a loop: the compiler makes three of three, with registers for each.)
+// gives the weight up to the first token that reaches the goal.  heavy: the weight of those of at least min_p.  (One call in a loop: the compiler makes three of three, with registers for each.)
 template <class F> __device__ __forceinline__ uint64_t draw(const Parameters& p, uint64_t kept, int k, uint64_t one, uint64_t heavy, const F& find) {
 #pragma unroll 1
     for (int step = k > 0 ? 0 : 1; step < 3; ++step) {
@@ -475,7 +496,7 @@ template <class F> __device__ __forceinline__ uint64_t draw(const Parameters& p,
             if (p.any_min_p) kept = min(kept, max(heavy, one));
             goal = min((uint64_t)((double)kept * (double)p.u) + 1, kept);
         }
-        const uint64_t weight = find(step, goal).weight;
+        const uint64_t weight = find(step, goal);
         if (step < 2) kept = weight;
     }
     return kept;
@@ -600,7 +621,7 @@ __device__ __forceinline__ void sample_sorted(Shared& s, const SampleParams& p, 
             upto += weight[e];
         }
         __syncthreads();
-        const Mass reached{0, s.word[0]};
+        const uint64_t reached = s.word[0];
         __syncthreads();
         return reached;
     });
@@ -611,21 +632,39 @@ __device__ __forceinline__ void sample_sorted(Shared& s, const SampleParams& p, 
     }
 }
 
+// A value's place among all: the values' order, and below the lowest finite one (kLowest) -inf and NaN.
+constexpr uint32_t kPlace = 0x007fffffu, kLowest = 0x00ffffffu;
+__device__ __forceinline__ uint32_t place_of(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return (u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u)) + kPlace;        // (NaN of either sign wraps)
+}
+
+// How many tokens there are in the coarse bins down to a key's.
+__device__ __forceinline__ uint64_t tokens_from(Shared& s, const uint32_t* coarse, uint32_t key) {
+    constexpr int kEachOf = kCoarseBins / kThreads;
+    uint64_t mine = 0, all;
+#pragma unroll
+    for (int i = 0; i < kEachOf; ++i)
+        if (kEachOf * (int)threadIdx.x + i <= (int)(~(key + kPlace) >> kCoarse)) mine += coarse[kEachOf * threadIdx.x + i];
+    scan(s.partial, mine, all);
+    return all;
+}
+
 // Of the tokens of keys lo to hi, hi the largest of the row and these the first ones, all or the first k (k > 0).
 template <typename T, class ROW>
 __device__ __forceinline__ void sample_from(Shared& s, uint64_t* gathered, const SampleParams& p, int64_t r, const Parameters& of, const Row<T>& whole, const ROW& row, uint32_t lo,
                                             uint32_t hi, int k) {
     const Weights w(key_value(hi), of.inverse, weight_bits(whole.vocab));
     const uint64_t one = 1ull << w.bits;
-    Search<T, ROW> search{s, row, whole, w, false, {}, false};
+    Search<T, ROW> search{s, row, whole, w, false, {}, false, 0};
     if (k > 0) {
         search.take(lo, hi, false);
-        if (search.all().count > (uint64_t)k) lo = search.find(true, (uint64_t)k, false).key;
+        if (search.all() > (uint64_t)k) lo = search.find((uint64_t)k, false).key;
         else k = 0;
     }
     search.take(lo, hi, true);
-    Mass all = search.all();
-    if (k > 0) all.weight -= (all.count - k) * w.whole_of(key_value(lo));      // equals of the k-th token behind it
+    uint64_t all = search.all();
+    if (k > 0) all -= (search.tokens() - k) * w.whole_of(key_value(lo));      // equals of the k-th token behind it
     const auto finish = [&](auto& search) {
         uint64_t heavy = 0;
         if (of.any_min_p) {
@@ -640,7 +679,7 @@ __device__ __forceinline__ void sample_from(Shared& s, uint64_t* gathered, const
             scan(s.partial, weight, heavy);
         }
         Found f;
-        const uint64_t kept = draw(of, all.weight, 0, one, heavy, [&](int step, uint64_t goal) { f = search.find(false, goal, step == 2); return f.upto; });
+        const uint64_t kept = draw(of, all, 0, one, heavy, [&](int step, uint64_t goal) { f = search.find(goal, step == 2); return f.upto; });
         if (threadIdx.x == 0) {
             p.ids[r] = f.index;
             write_logprob(p, r, w, key_value(f.key), kept);
@@ -648,27 +687,19 @@ __device__ __forceinline__ void sample_from(Shared& s, uint64_t* gathered, const
     };
     if constexpr (std::is_same_v<ROW, Row<T>>) {
         if (!of.top_p_one && !of.top_p_none) {             // what top-p keeps is often few: no more passes over the row
-            Mass front{0, 0};
-            const double least = ceil((double)all.weight * of.top_p);
-            const int bin = search.bin_of(false, least < 1.0 ? 1 : (uint64_t)least, front);
-            if (front.count + s.count[bin] <= (uint64_t)kGathered) {
-                const uint32_t from = search.first.from(bin);
+            uint64_t front = 0;
+            const double least = ceil((double)all * of.top_p);
+            const uint32_t from = search.first.from(search.bin_of(least < 1.0 ? 1 : (uint64_t)least, front));
+            if (tokens_from(s, reinterpret_cast<const uint32_t*>(gathered), from) <= (uint64_t)kGathered) {
                 const Gathered few = gather(s, gathered, whole, from);
-                if (sort(s, gathered, few.n, from, hi)) return sample_sorted(s, p, r, of, w, gathered, few.n, 0, all.weight);
-                Search<T, Gathered> rest{s, few, whole, w, false, {}, false};
+                if (sort(s, gathered, few.n, from, hi)) return sample_sorted(s, p, r, of, w, gathered, few.n, 0, all);
+                Search<T, Gathered> rest{s, few, whole, w, false, {}, false, 0};
                 rest.take(from, hi, true);
                 return finish(rest);
             }
         }
     }
     finish(search);
-}
-
-// A value's place among all: the values' order, and below the lowest finite one (kLowest) -inf and NaN.
-constexpr uint32_t kPlace = 0x007fffffu, kLowest = 0x00ffffffu;
-__device__ __forceinline__ uint32_t place_of(float x) {
-    const uint32_t u = __float_as_uint(x);
-    return (u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u)) + kPlace;        // (NaN of either sign wraps)
 }
 
 template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) {
@@ -721,13 +752,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     }
     if (of.any_min_p && of.top_p_none) lo = of.heavy_from(lo, hi);
     lo = of.from(lo, hi, -0.693147180559945309417 * (weight_bits(row.vocab) + 2));      // (those below weigh nothing: no sum, and no search by one, has to do with them)
-    uint64_t n_asked;                                      // those of the bins down to the last one's
-    mine = 0;
-#pragma unroll
-    for (int i = 0; i < kCoarseEach; ++i)
-        if (kCoarseEach * (int)threadIdx.x + i <= (int)(~(lo + kPlace) >> kCoarse)) mine += here[i];
-    scan(s.partial, mine, n_asked);
-    if (n_asked > kGathered) return sample_from<T>(s, gathered, p, r, of, row, row, lo, hi, k);
+    if (tokens_from(s, coarse, lo) > kGathered) return sample_from<T>(s, gathered, p, r, of, row, row, lo, hi, k);
     const Gathered few = gather(s, gathered, row, lo);
     if (sort(s, gathered, few.n, lo, hi)) return sample_sorted(s, p, r, of, Weights(key_value(hi), of.inverse, weight_bits(row.vocab)), gathered, few.n, k, 0);
     sample_from<T>(s, gathered, p, r, of, row, few, lo, hi, k);
@@ -978,7 +1003,7 @@ template <typename T, int NV> __global__ __launch_bounds__(kThreads) void sample
             nth = nth < 1 ? 1 : nth > n ? n : nth;
             found_key = (uint32_t)__builtin_amdgcn_readlane((int)key, l);
             found_nth = (int)nth;
-            return Mass{start.count + nth, start.weight + nth * weight};
+            return start.weight + nth * weight;
         };
         const uint64_t kept = draw(of, all, cut ? of.k : 0, one, s.heavy, [&](int step, uint64_t goal) { return find(step == 0, goal); });
         if (lane == 0) {
