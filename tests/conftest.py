@@ -1,3 +1,4 @@
+import gc
 import os
 import sys
 
@@ -22,6 +23,13 @@ def pytest_collection_modifyitems(config, items):
     for item in items:
         if "gpu" in item.keywords:
             item.add_marker(skip)
+
+
+@pytest.fixture(autouse=True)
+def no_garbage_of_others(request):
+    """Reference cycles that earlier tests left may hold device memory, which a collection in the middle of a test of memory would give back."""
+    if "memory" in request.node.name:
+        gc.collect()
 
 
 @pytest.fixture(scope="session")
