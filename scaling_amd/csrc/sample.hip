@@ -631,7 +631,6 @@ __device__ __forceinline__ bool sort(Shared& s, uint64_t* tokens, int n, uint32_
 __device__ __forceinline__ void sample_sorted(Shared& s, const SampleParams& p, int64_t r, const Parameters& of, const Weights& w, const uint64_t* tokens, int n, int k, uint64_t whole) {
     const uint64_t one = 1ull << w.bits;
     const double least = ldexp(of.min_p, w.bits);
-    if (threadIdx.x == 0) s.word[1] = 0;
     const int each = (n + kThreads - 1) / kThreads;        // tokens to a thread
     uint64_t weight[kEach], mine = 0, all, heavy = 0;
 #pragma unroll
@@ -645,7 +644,11 @@ __device__ __forceinline__ void sample_sorted(Shared& s, const SampleParams& p, 
         if (of.any_min_p && i < n && v >= least) heavy = mine;
     }
     const uint64_t front = scan(s.partial, mine, all);
-    if (heavy > 0) atomicMax((unsigned long long*)&s.word[1], (unsigned long long)(front + heavy));
+    // up to the last one of enough weight
+    const int lane = threadIdx.x & 63;
+    const uint64_t upto_heavy = of_lane(front + heavy, 63 - __builtin_clzll(__ballot(heavy > 0) | 1)), any = __ballot(heavy > 0);
+    __syncthreads();
+    if (lane == 0) s.partial[threadIdx.x >> 6].weight = any != 0 ? upto_heavy : 0;
     if (k > 0 && k <= n) {
         uint64_t upto = front;
 #pragma unroll
@@ -655,7 +658,8 @@ __device__ __forceinline__ void sample_sorted(Shared& s, const SampleParams& p, 
         }
     }
     __syncthreads();
-    heavy = s.word[1];
+    const uint64_t of_wave = s.partial[lane & (kWaves - 1)].weight;
+    heavy = of_lane(of_wave, 63 - __builtin_clzll((__ballot(of_wave > 0) & 0xffff) | 1));
     if (whole > 0) all = whole;
     else if (k > 0 && k <= n) all = s.word[2];
     const uint64_t kept = draw(of, all, 0, one, heavy, [&](int, uint64_t goal) {
@@ -684,16 +688,27 @@ __device__ __forceinline__ uint32_t place_of(float x) {
     return (u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u)) + kPlace;        // (NaN of either sign wraps)
 }
 
-// How many tokens there are in the coarse bins down to a key's.
-__device__ __forceinline__ uint64_t tokens_from(Shared& s, const uint32_t* coarse, uint32_t key) {
-    constexpr int kEachOf = kCoarseBins / kThreads;
-    uint64_t mine = 0, all;
+// A thread's coarse bins, and how many tokens there are in those down to a key's.
+constexpr int kCoarseEach = kCoarseBins / kThreads;
+struct CoarseBins {
+    uint32_t here[kCoarseEach];
+    __device__ __forceinline__ explicit CoarseBins(const uint32_t* coarse) {
+        static_assert(kCoarseEach % 4 == 0);
 #pragma unroll
-    for (int i = 0; i < kEachOf; ++i)
-        if (kEachOf * (int)threadIdx.x + i <= (int)(~(key + kPlace) >> kCoarse)) mine += coarse[kEachOf * threadIdx.x + i];
-    scan(s.partial, mine, all);
-    return all;
-}
+        for (int i = 0; i < kCoarseEach; i += 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(coarse + kCoarseEach * threadIdx.x + i);
+            here[i] = u.x; here[i + 1] = u.y; here[i + 2] = u.z; here[i + 3] = u.w;
+        }
+    }
+    __device__ __forceinline__ uint64_t from(Shared& s, uint32_t key) const {
+        uint64_t mine = 0, all;
+#pragma unroll
+        for (int i = 0; i < kCoarseEach; ++i)
+            if (kCoarseEach * (int)threadIdx.x + i <= (int)(~(key + kPlace) >> kCoarse)) mine += here[i];
+        scan(s.partial, mine, all);
+        return all;
+    }
+};
 
 // Of the tokens of keys lo to hi, hi the largest of the row and these the first ones, all or the first k (k > 0).
 template <typename T, class ROW>
@@ -735,7 +750,7 @@ __device__ __forceinline__ void sample_from(Shared& s, uint64_t* gathered, const
             uint64_t front = 0;
             const double least = ceil((double)all * of.top_p);
             const uint32_t from = search.first.from(search.bin_of(least < 1.0 ? 1 : (uint64_t)least, front));
-            if (tokens_from(s, reinterpret_cast<const uint32_t*>(gathered), from) <= (uint64_t)kGathered) {
+            if (CoarseBins(reinterpret_cast<const uint32_t*>(gathered)).from(s, from) <= (uint64_t)kGathered) {
                 const Gathered few = gather(s, gathered, whole, from);
                 if (sort(s, gathered, few.n, from, hi)) return sample_sorted(s, p, r, of, w, gathered, few.n, 0, all);
                 Search<T, Gathered> rest{s, few, whole, w, false, {}, false, 0};
@@ -749,13 +764,12 @@ __device__ __forceinline__ void sample_from(Shared& s, uint64_t* gathered, const
 
 template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(const SampleParams p) {
     __shared__ Shared s;
-    __shared__ uint64_t gathered[kGathered];
+    __shared__ __attribute__((aligned(16))) uint64_t gathered[kGathered];
     const int64_t r = blockIdx.x;
     const Row<T> row(p, r);
     const Parameters of(p, r);
     uint32_t* coarse = reinterpret_cast<uint32_t*>(gathered);
     static_assert(kCoarseBins * sizeof(uint32_t) <= sizeof(gathered));
-    constexpr int kCoarseEach = kCoarseBins / kThreads;
     for (int i = threadIdx.x; i < kCoarseBins; i += kThreads) coarse[i] = 0;
     __syncthreads();
     uint32_t n_lowest = 0, most = 0;
@@ -773,13 +787,11 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
     const uint32_t hi = value_key(key_value(most - kPlace));
     const auto edge = [](int bin) { return max((uint32_t)~(((uint64_t)(bin + 1) << kCoarse) - 1), kLowest) - kPlace; };      // the smallest key of a bin
     // ---- from where on tokens are asked for, and how many there are ----
-    uint32_t here[kCoarseEach];
+    const CoarseBins bins(coarse);
+    const auto& here = bins.here;
     uint64_t mine = 0, n_all;
 #pragma unroll
-    for (int i = 0; i < kCoarseEach; ++i) {
-        here[i] = coarse[kCoarseEach * threadIdx.x + i];
-        mine += here[i];
-    }
+    for (int i = 0; i < kCoarseEach; ++i) mine += here[i];
     uint64_t upto = scan(s.partial, mine, n_all);
     uint32_t lo = kLowest - kPlace;
     const int k = of.k > 0 && (uint64_t)of.k < n_all ? of.k : 0;
@@ -803,7 +815,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void sample_kernel(
         range(s, none, last);
         lo = edge((int)last);
     }
-    if (tokens_from(s, coarse, lo) > kGathered) return sample_from<T>(s, gathered, p, r, of, row, row, lo, hi, k);
+    if (bins.from(s, lo) > kGathered) return sample_from<T>(s, gathered, p, r, of, row, row, lo, hi, k);
     const Gathered few = gather(s, gathered, row, lo);
     if (sort(s, gathered, few.n, lo, hi)) return sample_sorted(s, p, r, of, Weights(key_value(hi), of.inverse, weight_bits(row.vocab)), gathered, few.n, k, 0);
     sample_from<T>(s, gathered, p, r, of, row, few, lo, hi, k);
