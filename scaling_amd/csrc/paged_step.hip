@@ -70,34 +70,33 @@ __device__ __forceinline__ void write_token(const StepParams& p, int row, int b,
 
 __global__ __launch_bounds__(kThreads) void paged_step_kernel(const StepParams p, bool write_tokens) {
     __shared__ Sums sums;
-    __shared__ int of_wave[3][kWaves];
-    __shared__ int64_t all[3];
-    __shared__ int long_ones;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ int of_wave[4][kWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int free_before = min(max(p.state[0], 0), p.n_free), was = p.state[1];
 
-    // sums of a chunk of sequences; of all of them in `all`
+    // sums of a chunk of sequences; what all of them have together (of more tokens than there may be: some number over it)
+    struct Totals { int given, wanted, tokens; bool too_long, several; };
     const auto add_up = [&](const Sequence& s) {
         const int given = prefix_sum(s.given), wanted = prefix_sum(s.wanted), tokens = prefix_sum(s.n);
+        const int flags = (__any(s.too_long) ? 1 : 0) | (__any(s.n > 1) ? 2 : 0);
         __syncthreads();
-        if (lane == 63) { of_wave[0][wave] = given; of_wave[1][wave] = wanted; of_wave[2][wave] = tokens; }
-        if (tid == 0) long_ones = 0;
+        if (lane == 63) { of_wave[0][wave] = given; of_wave[1][wave] = wanted; of_wave[2][wave] = min(tokens, p.tokens + 1); of_wave[3][wave] = flags; }
         __syncthreads();
-        int64_t before[3] = {0, 0, 0}, total[3] = {0, 0, 0};
-        for (int k = 0; k < 3; ++k)
-            for (int w = 0; w < kWaves; ++w) {
-                if (w < wave) before[k] += of_wave[k][w];
-                total[k] += of_wave[k][w];
-            }
-        sums.given[tid] = (int)(before[0] + given - s.given);
-        sums.wanted[tid] = (int)(before[1] + wanted - s.wanted);
-        sums.tokens[tid] = (int)(before[2] + tokens - s.n);
-        if (tid == 0) {
-            sums.given[kThreads] = (int)total[0]; sums.wanted[kThreads] = (int)total[1]; sums.tokens[kThreads] = (int)total[2];
-            for (int k = 0; k < 3; ++k) all[k] = total[k];
+        const bool there = lane < kWaves;
+        int before[3], total[3];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const int upto = prefix_sum(there ? of_wave[k][lane & (kWaves - 1)] : 0);
+            before[k] = wave > 0 ? __builtin_amdgcn_readlane(upto, wave - 1) : 0;
+            total[k] = __builtin_amdgcn_readlane(upto, kWaves - 1);
         }
-        if (s.too_long) long_ones = 1;
+        const int of_all = there ? of_wave[3][lane & (kWaves - 1)] : 0;
+        sums.given[tid] = before[0] + given - s.given;
+        sums.wanted[tid] = before[1] + wanted - s.wanted;
+        sums.tokens[tid] = before[2] + tokens - s.n;
+        if (tid == 0) { sums.given[kThreads] = total[0]; sums.wanted[kThreads] = total[1]; sums.tokens[kThreads] = total[2]; }
         __syncthreads();
+        return Totals{total[0], total[1], total[2], __any(of_all & 1) != 0, __any(of_all & 2) != 0};
     };
 
     // pages of a chunk's sequences that end onto the stack from `at` on, last page first; four at a time, so that four are under way
@@ -120,16 +119,18 @@ __global__ __launch_bounds__(kThreads) void paged_step_kernel(const StepParams p
     };
 
     // ---- a token of each sequence at most: the sequences' threads have all that is needed ----
-    if (p.batch <= kThreads) {
-        const Sequence s = sequence(p, tid, true);
+    const bool one_chunk = p.batch <= kThreads;
+    Sequence s = sequence(p, tid, true);
+    Totals all;
+    if (one_chunk) {
         const int at = divide((uint32_t)s.len, p.page, p.page_m);
         const bool there = tid < p.batch;
         int page = there && s.len < p.max_pages * p.page ? p.table[(int64_t)tid * p.table_stride + at] : 0;       // (asked for before it is known whether it is a new one)
         const int offset = there && p.offsets ? p.offsets[tid] : 0;
-        if (__syncthreads_or(s.n > 1) == 0) {
-            add_up(s);
-            const int64_t wanted = all[1], tokens = all[2], stacked = min(free_before + all[0], (int64_t)p.n_free);
-            const int status = (wanted > stacked ? kNoPages : 0) | (long_ones != 0 ? kTooLong : 0) | (tokens > p.tokens ? kTooMany : 0);
+        all = add_up(s);
+        if (!all.several) {
+            const int64_t wanted = all.wanted, tokens = all.tokens, stacked = min(free_before + (int64_t)all.given, (int64_t)p.n_free);
+            const int status = (wanted > stacked ? kNoPages : 0) | (all.too_long ? kTooLong : 0) | (tokens > p.tokens ? kTooMany : 0);
             const bool take = status == 0;
             const int row = sums.tokens[tid];
             if (there) {
@@ -165,12 +166,13 @@ __global__ __launch_bounds__(kThreads) void paged_step_kernel(const StepParams p
     // ---- whether there is room ----
     int64_t given = 0, wanted = 0, tokens = 0;
     bool too_long = false;
-    Sequence s;
     for (int base = 0; base < p.batch; base += kThreads) {
-        s = sequence(p, base + tid, true);
-        add_up(s);
-        given += all[0]; wanted += all[1]; tokens += all[2];
-        too_long |= long_ones != 0;
+        if (!one_chunk) {
+            s = sequence(p, base + tid, true);
+            all = add_up(s);
+        }
+        given += all.given; wanted += all.wanted; tokens += all.tokens;
+        too_long |= all.too_long;
     }
     const int64_t stacked = min(free_before + given, (int64_t)p.n_free);        // (more than all pages: the caller's mistake)
     const int status = (wanted > stacked ? kNoPages : 0) | (too_long ? kTooLong : 0) | (tokens > p.tokens ? kTooMany : 0);
@@ -180,7 +182,7 @@ __global__ __launch_bounds__(kThreads) void paged_step_kernel(const StepParams p
     if (given > 0) {
         int64_t done = free_before;
         for (int base = 0; base < p.batch; base += kThreads) {
-            if (p.batch > kThreads) add_up(sequence(p, base + tid, true));
+            if (!one_chunk) add_up(sequence(p, base + tid, true));
             push(base, done);
             done += sums.given[kThreads];
         }
@@ -192,7 +194,7 @@ __global__ __launch_bounds__(kThreads) void paged_step_kernel(const StepParams p
     int rows = 0;
     for (int base = 0; base < p.batch; base += kThreads) {
         const int b = base + tid;
-        if (p.batch > kThreads || !take) {
+        if (!one_chunk || !take) {
             s = sequence(p, b, take);
             add_up(s);
         }
