@@ -237,6 +237,15 @@ def test_replays_of_many_rows():
     call.check("o of the last replay", out)
 
 
+@pytest.mark.parametrize("batch", [6, 80])
+def test_one_prefix_of_two_groups(batch):
+    """Groups that name the same pages, one of them for fewer keys, and a third without any key of a prefix."""
+    sizes = [batch // 3, batch // 3, batch - 2 * (batch // 3)]
+    call = _Call([1 + i % 2 for i in range(batch)], [2 + i % 40 for i in range(batch)], sizes, [600, 600, 0], 8, 2, 128, 16, torch.bfloat16, seed=23 + batch)
+    call.prefix_table[1], call.prefix[1] = call.prefix_table[0], 411
+    call.check("o", ops.paged_prefix_attention(*call.arguments(), max_q_len=2))
+
+
 def test_far_pages():
     """Pages over 2^31 elements away."""
     pages = (1 << 31) // (16 * 2 * 64) + 40

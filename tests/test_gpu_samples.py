@@ -166,3 +166,24 @@ def test_other_numbers_other_answers_on_another_stream():
         assert model.generate_samples(12, PROMPTS[:3], 2, uniforms=u[1], page_size=16) == want[1]
     torch.cuda.current_stream().wait_stream(side)
     assert ops.sample_rows(torch.zeros(1, 4, device=DEV), torch.zeros(1, device=DEV)).tolist() == [0]
+
+
+def test_branches_of_one_sequence_twice_and_of_an_empty_one():
+    """The same sequence named twice, and one that holds nothing yet: what branches of each by itself give."""
+    cfg = _arch(hidden_size=512, num_attention_heads=8, attention_num_kv_heads=2, mlp_factor=2.5)
+    layer = _seeded_layer(cfg, seed=0).eval()
+    dtype, att, g = cfg.precision.dtype, layer.self_attention, torch.Generator().manual_seed(7)
+    prompt, x = torch.randn(37, cfg.hidden_size, generator=g).to(dtype), torch.randn(4, cfg.hidden_size, generator=g).to(dtype).to(DEV)
+
+    def outputs(sequences, rows):
+        cache = PagedKVCache(1, 40, 2, 64, att.num_attention_heads, att.num_kv_heads_per_partition, att.hidden_size_per_attention_head, dtype, DEV, page_size=16)
+        layer.paged_step(prompt.to(DEV).view(1, -1, cfg.hidden_size), cache, cache.step([37, 0]))
+        branches = PagedBranches(cache, sequences, 1, 16)
+        out = [layer.paged_step(x[rows].view(1, -1, cfg.hidden_size), cache, branches.step(_ints([1] * len(rows)), len(rows), 1))[0] for _ in range(3)]
+        branches.check()
+        return torch.stack(out, 1)
+    together = outputs([0, 0, 1, 0], [0, 1, 2, 0])
+    assert torch.equal(together[0], together[3]) and not torch.equal(together[0], together[1])
+    alone = torch.cat([outputs([0], [0]), outputs([0], [1]), outputs([1], [2])])
+    # values of about 1 through one layer of 16-bit roundings, in products and sums cut otherwise for other batches: a few steps
+    assert float((together[:3].float() - alone.float()).abs().max()) <= 16 * torch.finfo(dtype).eps * float(alone.float().abs().max())
