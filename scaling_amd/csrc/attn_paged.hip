@@ -622,9 +622,11 @@ template <int D, int NB, class P> __device__ __forceinline__ void paged_rows(con
     for (int nb = 0; nb < NB; ++nb) uneven |= 16 * nb + l16 < n_rows && limit[nb] < filled;
     if (__ballot(uneven) != 0) {                           // the same for the workgroup
         __syncthreads();
-        for (int r = wave; r < n_rows; r += NWV) {
+        uint64_t redo = __ballot(lane < n_rows && redo_lds[lane & (BLOCK - 1)] != 0);
+        for (; redo != 0; redo &= redo - 1) {
+            const int r = __builtin_ctzll(redo);
             const int lim = NB == 2 && r >= 16 ? __builtin_amdgcn_readlane(limit[NB - 1], r & 15) : __builtin_amdgcn_readlane(limit[0], r & 15);
-            if (redo_lds[r] == 0 || lim >= filled) continue;
+            if (r % NWV != wave || lim >= filled) continue;
             const int rr = block * BLOCK + r, i = divide(rr, p.n_rep, p.rep_m);
             float M, L, O0, O1;
             own_keys_only<D>(p, table, kvh, p.q + (int64_t)(f.seq.first + i) * p.q_st + (int64_t)(kvh * p.n_rep + rr - i * p.n_rep) * p.q_sh, s0, lim, M, L, O0, O1);
