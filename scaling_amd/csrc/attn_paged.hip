@@ -948,13 +948,13 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const P p) {
 
 // ---- groups' prefixes beside sequences' own keys --------------------------------------------------------------------------------------------------------------
 // Blocks of 128 rows in a workgroup of four wavefronts, in the form that shares a compute unit with others: rings of two tiles of K and two of V.  A wavefront has a SIMD
-// to itself or with others' workgroups, so that all that it issues counts: a tile's place in the cache is two lane reads, waits are constants (per 64 keys 3770 cycles with the
-// page's place computed by the scalar unit and waits by how much is under way, 3200 so).  Two forms, by the registers that there are:
+// to itself or with others' workgroups, so that all that it issues counts: a tile's place in the cache is two lane reads, waits are constants (us of
+// prefixes alone, 128 tokens behind 16384 keys: 79.5 with the place computed by the scalar unit and waits by how much is under way, 70.2 so).  Two forms, by the registers that there are:
 //     three workgroups to a compute unit (168 registers; K one and a half tiles ahead, two barriers a tile): products wait for the softmax; other workgroups' fill the pipe, or
 //     their requests the time.  Tiles of BN = 64 keys, of which every wavefront requests 16 keys of K and of V, or of 32 (two wavefronts K, two V), where the rings would
 //     let one workgroup less run on a compute unit.
 //     AHEAD, two workgroups: the next tile's scores are computed among this one's exponentials (which take twice as long as the products), one barrier a tile.
-// (us of 32 drafts of 3 - 7 tokens over 8192 keys, 32 / 8 heads of 128: 58 without the next scores, 54 with them.  Rings of three or four tiles, requests spread over the products
+// (us of 32 drafts of 3 - 7 tokens over 8192 keys, 32 / 8 heads of 128: 58 without the next scores, 54 with them, 2650 cycles to a tile.  Rings of three or four tiles, requests spread over the products
 // or over the wavefronts: level or slower.)
 constexpr int kSmallRows = 128, kSmallShift = 7;
 constexpr int kSmallAtOnce = 3;      // workgroups of paged_prefix_kernel that run on a compute unit (blocks of 16 rows)
