@@ -467,7 +467,7 @@ int mi_paged_attn(const mi_paged_attn_args* args);
  * front of their own, which are those of mi_paged_attn: attn.page_table, ctx_len and causal are about own keys alone.  Sequences outside all groups
  * have no prefix.  A group's keys are read once for its new tokens together, not once a sequence.  Softmax over both parts; a row without any key yields zeros.
  * prefix_table [n_groups, max_prefix_pages] by stride; group_seqs [n_groups + 1] ascending; lengths, pages and sizes as above.
- * attn.max_q_len is about sequences, not groups; attn.tickets are not looked at.
+ * attn.max_q_len is about sequences, not groups, and decides how the work is cut alone: sequences over the bound are computed all the same; attn.tickets are not looked at.
  * workspace: mi_paged_prefix_attn_workspace_bytes() bytes for so many tokens, sequences and groups or more, 16-byte aligned, one call at a time; nothing in it has to be
  * cleared.
  * Algorithmic work: 4 * head_dim * n_q_heads * pairs flop; HBM bytes 2 * (sum prefix_len + sum ctx_len) * n_kv_heads * head_dim * e + 2 * total_q * n_q_heads * head_dim * e. */

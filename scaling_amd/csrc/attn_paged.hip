@@ -1501,8 +1501,11 @@ PrefixPlans prefix_plans(int64_t tokens, int64_t batch, int64_t groups, int64_t 
     if (o.together) tiles.fit = share_of(o.plans.row_block == kRowBlock ? kSmallAtOnce * mi_compute_units() / 2 : mi_compute_units(), nkv);
     if (tiles.share > 0) tiles.share = tiles.fit;
     o.row_blocks = alone ? entries + 2 * (tokens * n_rep / o.plans.row_block) : entries * (rows.rows_up_to / o.plans.row_block);
-    if (o.together) o.tile_blocks = paged_max_blocks<kSmallRows>(tiles, tokens, batch, longest, n_rep) + paged_max_blocks<kSmallRows>(tiles, tokens, groups, tokens, n_rep);
-    else o.tile_blocks = paged_max_blocks<kTileRows>(tiles, tokens, batch, longest, n_rep) + paged_max_blocks<kTileRows>(tiles, tokens, groups, tokens, n_rep);
+    // Sequences are counted as groups are, by the tokens that there are and not by `longest`: one of more tokens than the caller's bound would else take the slots of others,
+    // a whole group's among them, whose places nobody would leave for the merge.  (128 single tokens over 16384 keys: 40 slots more than by the bound, 92.2 -> 94.0 us; the other
+    // sizes above level.)
+    const auto blocks = [&](auto rows_of_block) { return paged_max_blocks<decltype(rows_of_block)::value>(tiles, tokens, batch, tokens, n_rep) + paged_max_blocks<decltype(rows_of_block)::value>(tiles, tokens, groups, tokens, n_rep); };
+    o.tile_blocks = o.together ? blocks(std::integral_constant<int, kSmallRows>{}) : blocks(std::integral_constant<int, kTileRows>{});
     o.together = o.together && o.row_blocks > 0 && o.tile_blocks > 0;
     return o;
 }

@@ -553,8 +553,9 @@ class PagedBranches:
         self._workspaces: Dict[int, torch.Tensor] = {}
 
     def step(self, new: torch.Tensor, tokens: int, max_q_len: int) -> BranchStep:
-        """Takes pages for new[i] more tokens of branch i (int32 [branches] on the device; 0: none, negative: the branch ends and gives its pages back), at most `tokens` in all and
-        max_q_len of one.  If they do not fit, nobody has any in this step, and `check` raises."""
+        """Takes pages for new[i] more tokens of branch i (int32 [branches] on the device; 0: none, negative: the branch ends and gives its pages back), at most `tokens` in
+        all.  If they do not fit, nobody has any in this step, and `check` raises.  max_q_len: the most that is expected of one branch, by which attention cuts its work; more of one is
+        right as well."""
         tensors = ops.paged_step(new, self.ctx_len, self.page_table, self.free_pages, self.state, self.cache.page_size, tokens, self.max_ctx, self.position_offset)
         return BranchStep(self, tensors, tokens, max_q_len)
 

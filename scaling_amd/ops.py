@@ -334,8 +334,9 @@ def paged_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
 
     Sequences group_seqs[g] .. group_seqs[g + 1] - 1 form group g (group_seqs int32 [groups + 1], ascending; sequences outside have no prefix).  All their new tokens see
     the first prefix_len[g] (int32 [groups]) keys of the pages prefix_table[g] (int32 [groups, max_prefix_pages], in the same pool), and behind these the keys of
-    their own sequence as in `paged_attention`: page_table, ctx_len, causal and max_q_len are about own keys alone, so position p of an answer stands at
-    slot p - prefix_len of its sequence.  A row without any key is zeros; rows behind the last sequence are left as they are in `out` (of a new tensor: undefined).
+    their own sequence as in `paged_attention`: page_table, ctx_len and causal are about own keys alone, so position p of an answer stands at
+    slot p - prefix_len of its sequence.  max_q_len, an upper bound of the tokens of a sequence (not of a group), decides how the work is cut; longer sequences are computed all the
+    same, if not as fast.  A row without any key is zeros; rows behind the last sequence are left as they are in `out` (of a new tensor: undefined).
     workspace: see `paged_prefix_workspace`; without one it is allocated per call."""
     _need_cuda(q, k_pages, v_pages, page_table, cu_seqlens, ctx_len, prefix_table, prefix_len, group_seqs, workspace, out)
     if max_q_len is not None and max_q_len < 1 and q.shape[0] > 0:

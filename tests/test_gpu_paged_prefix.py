@@ -139,6 +139,20 @@ def test_no_prefix_is_paged_attention():
     call.check("sequences in front and behind", ops.paged_prefix_attention(*call.arguments()))
 
 
+@pytest.mark.parametrize("new,sizes,nq,nkv,d,prefix", [([20] + [1] * 7, [8], 8, 2, 64, [200]), ([1, 1, 40, 1, 33, 1, 1, 90], [4, 3], 32, 8, 128, [700, 30]), ([300] + [1] * 60, [30, 31], 4, 1, 96, [90, 500]),
+                                                        ([9, 1, 1], [3], 4, 2, 32, [300]), ([64, 1] * 150, [150, 150], 32, 32, 32, [60, 20])])
+def test_a_bound_that_is_too_low(new, sizes, nq, nkv, d, prefix):
+    """Sequences of more tokens than max_q_len are computed all the same, and so is everybody else; nothing is left of what an earlier call wrote to the workspace."""
+    print(f"case {new[:8]} {sizes} {nq} {nkv} {d}", flush=True)
+    call = _Call(new, [n + 11 * i % 300 for i, n in enumerate(new)], sizes, prefix, nq, nkv, d, 16, torch.bfloat16, seed=len(new) + d)
+    args = call.arguments()
+    ws = ops.paged_prefix_workspace(len(new), len(prefix), call.cu[-1], nq, nkv, d, DEV)
+    for stale in (math.nan, 0.0, 1.0):
+        ws.fill_(stale)
+        for bound in (1, 2, max(new) - 1):
+            call.check(f"o, bound {bound}", ops.paged_prefix_attention(*args, workspace=ws, max_q_len=bound))
+
+
 @DTYPES
 def test_values_that_are_not_finite(dtype):
     """Infinities and NaN reach the rows that see them and no others."""
