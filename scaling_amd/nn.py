@@ -550,12 +550,15 @@ class PagedBranches:
         self.position_offset = ints([n for n in prefix for _ in range(count)])
         self.ctx_len, self.page_table = ints([0] * self.total), torch.zeros(self.total, width, dtype=torch.int32, device=cache.device)
         self.free_pages, self.state = ints(self.pages), ints([len(self.pages), 0])
+        self.closed = False
         self._workspaces: Dict[int, torch.Tensor] = {}
 
     def step(self, new: torch.Tensor, tokens: int, max_q_len: int) -> BranchStep:
         """Takes pages for new[i] more tokens of branch i (int32 [branches] on the device; 0: none, negative: the branch ends and gives its pages back), at most `tokens` in
         all.  If they do not fit, nobody has any in this step, and `check` raises.  max_q_len: the most that is expected of one branch, by which attention cuts its work; more of one is
         right as well."""
+        if self.closed:
+            raise RuntimeError("a step of branches that are closed")
         tensors = ops.paged_step(new, self.ctx_len, self.page_table, self.free_pages, self.state, self.cache.page_size, tokens, self.max_ctx, self.position_offset)
         return BranchStep(self, tensors, tokens, max_q_len)
 
@@ -577,7 +580,17 @@ class PagedBranches:
             raise RuntimeError("a step of the branches did not fit: " + ", ".join(what))
 
     def close(self) -> None:
-        """The branches end: their pages are the cache's again (behind the calls that are on the stream)."""
+        """The branches end: their pages are the cache's again (behind the calls that are on the stream).  Steps are refused from here on, and one that was captured finds no page
+        when it is replayed: neither a free one nor one of its own."""
+        if self.closed:
+            return
+        if self.cache.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("branches are not closed while a graph is captured")
+        self.closed = True
+        with torch.inference_mode():                         # (where the branches may have been made)
+            self.state[:1].zero_()
+            self.ctx_len.zero_()
+            self.page_table.fill_(-1)
         self.cache.give(self.pages)
         self.pages = []
 
@@ -854,11 +867,13 @@ class ParallelSelfAttention(torch.nn.Module):
             raise NotImplementedError("the paged attention kernels take bfloat16 or float16 tensors")
         if b * s != step.tokens:
             raise ValueError(f"{b * s} tokens in x, {step.tokens} in the step")
-        if self.rotary_embedding is not None and step.longest > self.rotary_embedding.max_seq_length:
-            raise IndexError(f"position {step.longest - 1} is outside the rotary table of {self.rotary_embedding.max_seq_length} rows")
         branches = getattr(step, "branches", None)
         if branches is not None and branches.cache is not cache:
             raise ValueError("a step of branches of another cache")
+        if branches is not None and branches.closed:
+            raise RuntimeError("a step of branches that are closed")
+        if self.rotary_embedding is not None and step.longest > self.rotary_embedding.max_seq_length:
+            raise IndexError(f"position {step.longest - 1} is outside the rotary table of {self.rotary_embedding.max_seq_length} rows")
         table = cache.page_table[:step.ctx_len.numel()] if branches is None else branches.page_table
         pages = (cache.k_pages[layer], cache.v_pages[layer], table, step.cu_seqlens, step.ctx_len)
         with torch.no_grad():

@@ -1,0 +1,46 @@
+"""Host side of branches of sequences of a paged cache."""
+
+import pytest
+import torch
+
+from scaling_amd import ops
+from scaling_amd.nn import BranchStep, PagedBranches
+from tests.test_paged_modules_cpu import _attention, _cache
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def _plan(branches, tokens):
+    """A step's tensors, without a GPU to plan them on."""
+    long = lambda n: torch.zeros(n, dtype=torch.int64)
+    return BranchStep(branches, ops.StepTensors(_ints([0] * (branches.total + 1)), long(tokens), long(tokens), long(tokens), long(branches.total)), tokens, 1)
+
+
+def test_closed_branches_take_no_steps():
+    """Their pages are others' then, and nothing that was captured before finds any: no free ones, no keys, no page in the table."""
+    cache = _cache(num_pages=20)
+    cache.step([20, 5, 1])
+    free = sorted(cache._free)
+    branches = PagedBranches(cache, [0, 1], 2, 30)
+    branches.ctx_len.fill_(3)
+    plan = _plan(branches, 4)
+    branches.close()
+    branches.close()
+    assert sorted(cache._free) == free
+    assert branches.state.tolist() == [0, 0] and branches.ctx_len.tolist() == [0] * 4 and bool((branches.page_table == -1).all())
+    with pytest.raises(RuntimeError, match="closed"):
+        branches.step(_ints([1] * 4), 4, 1)
+    with pytest.raises(RuntimeError, match="closed"):
+        _attention().paged_forward(torch.zeros(1, 4, 256, dtype=torch.bfloat16), cache, 0, plan)
+
+
+@pytest.mark.parametrize("inference", [False, True])
+def test_close_of_branches_made_in_inference_mode(inference):
+    cache = _cache()
+    cache.step([3, 1])
+    with torch.inference_mode(inference):
+        branches = PagedBranches(cache, [0], 1, 16)
+    branches.close()
+    assert cache.free_pages == 3 and branches.state.tolist() == [0, 0]

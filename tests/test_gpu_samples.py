@@ -187,3 +187,42 @@ def test_branches_of_one_sequence_twice_and_of_an_empty_one():
     alone = torch.cat([outputs([0], [0]), outputs([0], [1]), outputs([1], [2])])
     # values of about 1 through one layer of 16-bit roundings, in products and sums cut otherwise for other batches: a few steps
     assert float((together[:3].float() - alone.float()).abs().max()) <= 16 * torch.finfo(dtype).eps * float(alone.float().abs().max())
+
+
+def test_replays_behind_the_end():
+    """A captured step of branches, replayed after they were closed and their pages went to another sequence: it takes nothing, says so, and leaves the pages alone."""
+    cfg = _arch(hidden_size=512, num_attention_heads=8, attention_num_kv_heads=2, mlp_factor=2.5)
+    layer = _seeded_layer(cfg, seed=0).eval()
+    dtype, att, g = cfg.precision.dtype, layer.self_attention, torch.Generator().manual_seed(11)
+    rows = lambda n: torch.randn(1, n, cfg.hidden_size, generator=g).to(dtype).to(DEV)
+    cache = PagedKVCache(1, 5, 2, 64, att.num_attention_heads, att.num_kv_heads_per_partition, att.hidden_size_per_attention_head, dtype, DEV, page_size=16)
+    layer.paged_step(rows(20), cache, cache.step([20, 0]))
+    branches = PagedBranches(cache, [0], 3, 16)
+    x, new = rows(3), _ints([1, 1, 1])
+    step = lambda: layer.paged_step(x, cache, branches.step(new, 3, 1))
+    for _ in range(2):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(3):
+        graph.replay()
+    branches.check()
+    assert branches.ctx_len.tolist() == [5, 5, 5]
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        x.add(1.0)
+        with pytest.raises(RuntimeError, match="captured"):
+            branches.close()
+    branches.close()
+    layer.paged_step(rows(48), cache, cache.step([0, 48]))       # all that they had
+    assert cache.free_pages == 0
+    pages = [t.clone() for t in (cache.k_pages[0], cache.v_pages[0])]
+    for now in ([1, 1, 1], [-1, 1, 0], [1, 0, -1]):
+        new.copy_(_ints(now))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(cache.k_pages[0], pages[0]) and torch.equal(cache.v_pages[0], pages[1])
+        assert branches.ctx_len.tolist() == [0, 0, 0] and branches.state.tolist() == [0, 1]
+    with pytest.raises(RuntimeError, match="pages ran out"):
+        branches.check()
