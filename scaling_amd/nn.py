@@ -8,6 +8,7 @@ do not cover raise `NotImplementedError` instead of silently taking another path
 """
 
 import math
+import weakref
 from typing import Callable, Dict, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -457,6 +458,7 @@ class PagedKVCache:
         self._table = torch.zeros(max_sequences, -(-max_ctx // page_size), dtype=torch.int32, device="cpu")
         self.page_table = self._table.to(device, copy=True)
         self._workspace: Optional[torch.Tensor] = None
+        self._branches: "weakref.WeakSet[PagedBranches]" = weakref.WeakSet()      # open ones
         if self.device.type == "cuda":
             self.workspace()                             # now: the first call over the cache may be one that is captured
 
@@ -490,9 +492,12 @@ class PagedKVCache:
         return PagedStep(new, lengths, self.device)
 
     def release(self, sequence: int) -> None:
-        """The sequence ends: its pages are free for others (behind the calls that are on the stream), and its place starts again at length 0."""
+        """The sequence ends: its pages are free for others (behind the calls that are on the stream), and its place starts again at length 0.  Refused while
+        branches of it are open, which read them."""
         if not 0 <= sequence < self.max_sequences:
             raise IndexError(f"sequence {sequence} of {self.max_sequences}")
+        if any(sequence in branches.sequences for branches in self._branches):
+            raise RuntimeError(f"sequence {sequence} has branches that are not closed")
         self._free.extend(reversed(self._pages[sequence]))
         self._pages[sequence] = []
         self.lengths[sequence] = 0
@@ -531,7 +536,7 @@ class PagedBranches:
     that the branches take from `num_pages` of the cache's.  Branch i of the j-th of `sequences` is number j * count + i.
 
     Lengths and free pages lie on the device, and a step is planned there (ops.paged_step): the host neither knows nor waits for how long the branches are or which have ended, and
-    a step may be captured with the layers' calls and replayed.  Until `close` the sequences have to stay as they are in the cache."""
+    a step may be captured with the layers' calls and replayed.  Until `close` the sequences stay in the cache, which refuses to release them."""
 
     def __init__(self, cache: PagedKVCache, sequences: Sequence[int], count: int, max_ctx: int, num_pages: Optional[int] = None) -> None:
         sequences = [int(b) for b in sequences]
@@ -550,7 +555,8 @@ class PagedBranches:
         self.position_offset = ints([n for n in prefix for _ in range(count)])
         self.ctx_len, self.page_table = ints([0] * self.total), torch.zeros(self.total, width, dtype=torch.int32, device=cache.device)
         self.free_pages, self.state = ints(self.pages), ints([len(self.pages), 0])
-        self.closed = False
+        self.sequences, self.closed = frozenset(sequences), False
+        cache._branches.add(self)
         self._workspaces: Dict[int, torch.Tensor] = {}
 
     def step(self, new: torch.Tensor, tokens: int, max_q_len: int) -> BranchStep:
@@ -591,6 +597,7 @@ class PagedBranches:
             self.state[:1].zero_()
             self.ctx_len.zero_()
             self.page_table.fill_(-1)
+        self.cache._branches.discard(self)
         self.cache.give(self.pages)
         self.pages = []
 

@@ -44,3 +44,23 @@ def test_close_of_branches_made_in_inference_mode(inference):
         branches = PagedBranches(cache, [0], 1, 16)
     branches.close()
     assert cache.free_pages == 3 and branches.state.tolist() == [0, 0]
+
+
+def test_a_prefix_stays_while_branches_read_it():
+    """A sequence is not released under branches that are open, of which there may be several; branches that nobody has any more hold nothing."""
+    cache = _cache(num_pages=20)
+    cache.step([20, 5, 1])
+    first, second = PagedBranches(cache, [0, 1], 2, 30), PagedBranches(cache, [1], 1, 30)
+    for sequence in (0, 1):
+        with pytest.raises(RuntimeError, match=f"sequence {sequence}.*branches"):
+            cache.release(sequence)
+    assert cache.lengths == [20, 5, 1] and len(cache._pages[0]) == 2
+    cache.release(2)
+    cache.step([1, 0, 0])                                        # (more keys of a sequence are behind the prefix)
+    first.close()
+    cache.release(0)
+    with pytest.raises(RuntimeError, match="sequence 1"):
+        cache.release(1)
+    del second
+    cache.release(1)
+    assert cache.lengths == [0, 0, 0]
