@@ -226,3 +226,66 @@ def test_replays_behind_the_end():
         assert branches.ctx_len.tolist() == [0, 0, 0] and branches.state.tolist() == [0, 1]
     with pytest.raises(RuntimeError, match="pages ran out"):
         branches.check()
+
+
+class _Loop:
+    """Branches of one prompt through one layer, whose outputs are the next inputs; every step's are kept."""
+
+    def __init__(self, layer, cfg, seed, prompt, count, steps):
+        att, dtype, g = layer.self_attention, cfg.precision.dtype, torch.Generator().manual_seed(seed)
+        rows = lambda n: torch.randn(1, n, cfg.hidden_size, generator=g).to(dtype).to(DEV)
+        self.layer, self.count = layer, count
+        self.cache = PagedKVCache(1, -(-prompt // 16) + count * 8, 1, prompt, att.num_attention_heads, att.num_kv_heads_per_partition, att.hidden_size_per_attention_head, dtype, DEV,
+                                  page_size=16)
+        layer.paged_step(rows(prompt), self.cache, self.cache.step([prompt]))
+        self.branches = PagedBranches(self.cache, [0], count, 128)
+        self.x, self.one, self.at = rows(count), _ints([1] * count), torch.zeros(1, dtype=torch.int64, device=DEV)
+        self.out = torch.zeros(steps, count, cfg.hidden_size, dtype=dtype, device=DEV)
+
+    def step(self):
+        y = self.layer.paged_step(self.x, self.cache, self.branches.step(self.one, self.count, 1))
+        self.out.index_copy_(0, self.at, y)
+        self.at.add_(1)
+        self.x.copy_(y / y.float().square().mean(-1, keepdim=True).sqrt().to(y.dtype))
+
+    def capture(self, stream):
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            self.step()
+        return graph
+
+
+def _wide_layer():
+    cfg = _arch(hidden_size=1024, num_attention_heads=8, attention_num_kv_heads=2, mlp_factor=2.5, sequence_length=4096)
+    return cfg, _seeded_layer(cfg, seed=0).eval()
+
+
+def test_two_captured_loops_run_at_once():
+    """Two caches, each with branches, a captured step and scratch of its own: replayed on two streams that run at the same time, they give what each gives alone."""
+    cfg, layer = _wide_layer()
+    steps, alone = 14, []
+    shapes = ((3, 700, 40), (4, 3000, 24))
+    for seed, prompt, count in shapes:
+        loop = _Loop(layer, cfg, seed, prompt, count, steps)
+        for _ in range(steps):
+            loop.step()
+        loop.branches.check()
+        alone.append(loop.out)
+    loops, streams = [_Loop(layer, cfg, *shape, steps) for shape in shapes], [torch.cuda.Stream() for _ in shapes]
+    for loop in loops:
+        loop.step()
+        loop.step()
+    graphs = [loop.capture(stream) for loop, stream in zip(loops, streams)]
+    torch.cuda.synchronize()
+    for stream in streams:                                   # both wait until everything is issued
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(20_000_000)
+    for _ in range(steps - 2):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for loop, want in zip(loops, alone):
+        loop.branches.check()
+        assert bool(torch.isfinite(want.float()).all()) and torch.equal(loop.out, want)
