@@ -557,7 +557,9 @@ class PagedBranches:
         self.free_pages, self.state = ints(self.pages), ints([len(self.pages), 0])
         self.sequences, self.closed = frozenset(sequences), False
         cache._branches.add(self)
-        self._workspaces: Dict[int, torch.Tensor] = {}
+        self._workspace: Optional[torch.Tensor] = None       # for steps of up to `_rows` tokens
+        self._rows = 0
+        self._captured: List[torch.Tensor] = []              # what captured steps have
 
     def step(self, new: torch.Tensor, tokens: int, max_q_len: int) -> BranchStep:
         """Takes pages for new[i] more tokens of branch i (int32 [branches] on the device; 0: none, negative: the branch ends and gives its pages back), at most `tokens` in
@@ -568,15 +570,31 @@ class PagedBranches:
         tensors = ops.paged_step(new, self.ctx_len, self.page_table, self.free_pages, self.state, self.cache.page_size, tokens, self.max_ctx, self.position_offset)
         return BranchStep(self, tensors, tokens, max_q_len)
 
+    def _capturing(self) -> bool:
+        if self.cache.device.type != "cuda":
+            return False
+        with torch.cuda.device(self.cache.device):
+            return torch.cuda.is_current_stream_capturing()
+
     def workspace(self, tokens: int) -> torch.Tensor:
-        """Scratch of ops.paged_prefix_attention for steps of `tokens` rows, kept for the branches' life (one that is made while a graph is captured is the graph's alone)."""
-        workspace = self._workspaces.get(tokens)
-        if workspace is None:
-            cache = self.cache
-            workspace = ops.paged_prefix_workspace(self.total, len(self.prefix_len), tokens, cache.n_q, cache.n_kv, cache.head_dim, cache.device)
-            if not (workspace.is_cuda and torch.cuda.is_current_stream_capturing()):
-                self._workspaces[tokens] = workspace
-        return workspace
+        """Scratch of ops.paged_prefix_attention for steps of `tokens` rows: one for all, which grows by a quarter at least.  What a captured step has is kept for the branches' life (or, made
+        in the capture, the graph's alone)."""
+        capturing = self._capturing()
+        if self._workspace is None or tokens > self._rows:
+            cache, rows = self.cache, tokens if capturing else max(tokens, self._rows * 5 // 4)
+            workspace = ops.paged_prefix_workspace(self.total, len(self.prefix_len), rows, cache.n_q, cache.n_kv, cache.head_dim, cache.device)
+            if capturing:
+                return workspace
+            self._drop_workspace()
+            self._workspace, self._rows = workspace, rows
+        elif capturing and not any(w is self._workspace for w in self._captured):
+            self._captured.append(self._workspace)
+        return self._workspace
+
+    def _drop_workspace(self) -> None:
+        if self._workspace is not None and self._workspace.is_cuda:
+            self._workspace.record_stream(torch.cuda.current_stream(self._workspace.device))      # calls that have it may be under way here, on a stream other than its own
+        self._workspace, self._rows = None, 0
 
     def check(self) -> None:
         """Raises if a step did not fit (waits for the device)."""
@@ -590,13 +608,14 @@ class PagedBranches:
         when it is replayed: neither a free one nor one of its own."""
         if self.closed:
             return
-        if self.cache.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        if self._capturing():
             raise RuntimeError("branches are not closed while a graph is captured")
         self.closed = True
         with torch.inference_mode():                         # (where the branches may have been made)
             self.state[:1].zero_()
             self.ctx_len.zero_()
             self.page_table.fill_(-1)
+        self._drop_workspace()
         self.cache._branches.discard(self)
         self.cache.give(self.pages)
         self.pages = []

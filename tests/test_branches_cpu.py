@@ -1,5 +1,7 @@
 """Host side of branches of sequences of a paged cache."""
 
+import gc
+
 import pytest
 import torch
 
@@ -64,3 +66,32 @@ def test_a_prefix_stays_while_branches_read_it():
     del second
     cache.release(1)
     assert cache.lengths == [0, 0, 0]
+
+
+def test_scratch_of_steps_of_many_sizes(monkeypatch):
+    """Drafts bring another number of tokens in every step: they share one scratch, not one for every number, but for those that captured steps have, which stay."""
+    cache = _cache(num_pages=20)
+    cache.step([20, 5, 1])
+    branches, capturing = PagedBranches(cache, [0, 1], 4, 30), False
+    monkeypatch.setattr(PagedBranches, "_capturing", lambda self: capturing, raising=False)
+    need = lambda tokens: ops.paged_prefix_workspace(8, 2, tokens, 4, 2, 64, "cpu").numel()
+    held = lambda: {x.data_ptr(): x.numel() for x in gc.get_objects() if type(x) is torch.Tensor and x.dtype == torch.float32 and x.numel() >= need(1)}
+    most = 0
+    for tokens in (8, 9, 5, 17, 40, 11, 39, 41, 8, 100, 64, 240, 101, 33):
+        assert branches.workspace(tokens).numel() >= need(tokens)
+        most = max(most, tokens)
+        assert len(held()) == 1 and sum(held().values()) <= need(2 * most)
+    capturing = True
+    graphs = branches.workspace(100).data_ptr()                  # the one that there is
+    assert graphs in held() and branches.workspace(3).data_ptr() == graphs
+    own = branches.workspace(1000)                               # made in the capture: the graph's alone
+    assert own.numel() >= need(1000) and set(held()) == {graphs, own.data_ptr()}
+    del own
+    capturing = False
+    assert branches.workspace(64).data_ptr() == graphs and set(held()) == {graphs}
+    eager = branches.workspace(5000).data_ptr()
+    assert set(held()) == {graphs, eager}
+    branches.close()
+    assert set(held()) == {graphs}
+    del branches
+    assert not held()

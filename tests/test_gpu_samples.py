@@ -239,7 +239,7 @@ class _Loop:
                                   page_size=16)
         layer.paged_step(rows(prompt), self.cache, self.cache.step([prompt]))
         self.branches = PagedBranches(self.cache, [0], count, 128)
-        self.x, self.one, self.at = rows(count), _ints([1] * count), torch.zeros(1, dtype=torch.int64, device=DEV)
+        self.x, self.drafts, self.one, self.at = rows(count), rows(20 * count), _ints([1] * count), torch.zeros(1, dtype=torch.int64, device=DEV)
         self.out = torch.zeros(steps, count, cfg.hidden_size, dtype=dtype, device=DEV)
 
     def step(self):
@@ -247,6 +247,9 @@ class _Loop:
         self.out.index_copy_(0, self.at, y)
         self.at.add_(1)
         self.x.copy_(y / y.float().square().mean(-1, keepdim=True).sqrt().to(y.dtype))
+
+    def draft(self, n):
+        self.layer.paged_step(self.drafts[:, :n * self.count], self.cache, self.branches.step(_ints([n] * self.count), n * self.count, n))
 
     def capture(self, stream):
         graph = torch.cuda.CUDAGraph()
@@ -289,3 +292,29 @@ def test_two_captured_loops_run_at_once():
     for loop, want in zip(loops, alone):
         loop.branches.check()
         assert bool(torch.isfinite(want.float()).all()) and torch.equal(loop.out, want)
+
+
+def test_a_captured_step_keeps_its_scratch():
+    """Drafts between replays need more scratch than the captured step has, and what they leave is others' memory then: the replays give what eager steps do."""
+    cfg, layer = _wide_layer()
+    graph, outs = None, []
+    for captured in (False, True):
+        loop = _Loop(layer, cfg, 5, 900, 30, 9)
+        loop.step()
+        first = loop.branches.workspace(30).data_ptr()
+        if captured:
+            graph = loop.capture(torch.cuda.Stream())
+        for drafts in (0, 2, 0, 20, 0, 5, 1, 0):
+            if drafts:
+                loop.draft(drafts)
+            held = [torch.full((1 << 22,), float("nan"), device=DEV) for _ in range(16)]
+            if captured:
+                graph.replay()
+            else:
+                loop.step()
+            torch.cuda.synchronize()
+            del held
+        loop.branches.check()
+        assert loop.branches.workspace(30).data_ptr() != first
+        outs.append(loop.out)
+    assert bool(torch.isfinite(outs[0].float()).all()) and torch.equal(outs[0], outs[1])
