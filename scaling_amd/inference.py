@@ -444,27 +444,28 @@ class TransformerInferenceModule(torch.nn.Module):
             plan = branches.step(new, total, 1)
             draw(self.paged_forward(tokens.index_select(0, plan.sequences), cache, plan))
 
-        draw(logits.repeat_interleave(samples, dim=0))
-        steps = max_tokens - 1
-        eager = steps if not graph else min(2, steps)                       # the first ones warm the libraries up
-        captured = None
-        if steps > eager:
-            side = torch.cuda.Stream()
-            side.wait_stream(torch.cuda.current_stream())
-            with torch.cuda.stream(side):
-                for _ in range(eager):
+        with torch.cuda.device(dev):                                        # streams and graphs are of the current device
+            draw(logits.repeat_interleave(samples, dim=0))
+            steps = max_tokens - 1
+            eager = steps if not graph else min(2, steps)                   # the first ones warm the libraries up
+            captured = None
+            if steps > eager:
+                side = torch.cuda.Stream()
+                side.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(side):
+                    for _ in range(eager):
+                        step()
+                torch.cuda.current_stream().wait_stream(side)
+                captured = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(captured):
                     step()
-            torch.cuda.current_stream().wait_stream(side)
-            captured = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(captured):
-                step()
-        for k in range(0 if captured is None else eager, steps):
-            if stop is not None and k % 16 == 15 and not bool((new > 0).any()):
-                break                                                       # all have ended, which is looked at now and then
-            if captured is None:
-                step()
-            else:
-                captured.replay()
+            for k in range(0 if captured is None else eager, steps):
+                if stop is not None and k % 16 == 15 and not bool((new > 0).any()):
+                    break                                                   # all have ended, which is looked at now and then
+                if captured is None:
+                    step()
+                else:
+                    captured.replay()
         branches.check()
         branches.close()
         ids, logprobs = ids.t().tolist(), logprobs.t().tolist()

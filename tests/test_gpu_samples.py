@@ -318,3 +318,24 @@ def test_a_captured_step_keeps_its_scratch():
         assert loop.branches.workspace(30).data_ptr() != first
         outs.append(loop.out)
     assert bool(torch.isfinite(outs[0].float()).all()) and torch.equal(outs[0], outs[1])
+
+
+def test_generation_is_on_the_module_s_device(monkeypatch):
+    """Streams and graphs belong to a device, the current one unless told otherwise: they are made where the module's is current."""
+    model, current, made = _model(), [], []
+
+    class Device(torch.cuda.device):
+        def __enter__(self):
+            current.append(self.idx)
+            return super().__enter__()
+
+        def __exit__(self, *args):
+            current.pop()
+            return super().__exit__(*args)
+    stream, graph = torch.cuda.Stream, torch.cuda.graph
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "Stream", lambda *a, **kw: made.append(list(current)) or stream(*a, **kw))
+    monkeypatch.setattr(torch.cuda, "graph", lambda *a, **kw: made.append(list(current)) or graph(*a, **kw))
+    want = model.generate_samples(6, PROMPTS, 2, uniforms=torch.full((6, 8), 0.4), page_size=16)
+    assert len(made) >= 2 and all(made), made                # (torch makes some of its own)
+    assert not current and [len(s) for p in want[0] for s in p] == [6] * 8
