@@ -409,7 +409,7 @@ class TransformerInferenceModule(torch.nn.Module):
             raise ValueError("at least one prompt, no empty one, and at least one answer of one token to generate")
         total, dev = samples * len(prompts), self.device
         if uniforms is None:
-            uniforms = torch.rand(max_tokens, total, device=dev, generator=generator)
+            uniforms = torch.rand(max_tokens, total, dtype=torch.float32, device=dev, generator=generator)
         elif uniforms.shape != (max_tokens, total) or uniforms.dtype != torch.float32:
             raise ValueError(f"uniforms are float32 [{max_tokens}, {total}], got {uniforms.dtype} {list(uniforms.shape)}")
         uniforms = uniforms.to(dev)
@@ -424,7 +424,7 @@ class TransformerInferenceModule(torch.nn.Module):
         branches = PagedBranches(cache, range(len(prompts)), samples, own, of_branches)
         stop = None if not stop_tokens else torch.tensor(sorted(set(stop_tokens)), dtype=torch.int64, device=dev)
         ids = torch.full((max_tokens, total), -1, dtype=torch.int64, device=dev)
-        logprobs = torch.zeros(max_tokens, total, device=dev)
+        logprobs = torch.zeros(max_tokens, total, dtype=torch.float32, device=dev)
         new = torch.ones(total, dtype=torch.int32, device=dev)              # 1: goes on, -1: ends in this step, 0: has ended
         tokens = torch.zeros(total, dtype=torch.int64, device=dev)
         at = torch.zeros(1, dtype=torch.int64, device=dev)                  # the step that is drawn next

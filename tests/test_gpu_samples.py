@@ -346,3 +346,18 @@ def test_generation_is_on_the_module_s_device(monkeypatch):
     want = model.generate_samples(6, PROMPTS, 2, uniforms=torch.full((6, 8), 0.4), page_size=16)
     assert len(made) >= 2 and all(made), made
     assert not current and [len(s) for p in want[0] for s in p] == [6] * 8
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64])
+def test_generation_under_another_default_type(dtype):
+    model = _model()
+    u = torch.rand(5, 8, generator=torch.Generator().manual_seed(9))
+    want = model.generate_samples(5, PROMPTS, 2, uniforms=u, page_size=16)
+    drawn = model.generate_samples(5, PROMPTS, 2, generator=torch.Generator(device=DEV).manual_seed(9), page_size=16)
+    torch.set_default_dtype(dtype)
+    try:
+        got = model.generate_samples(5, PROMPTS, 2, uniforms=u, page_size=16)
+        again = model.generate_samples(5, PROMPTS, 2, generator=torch.Generator(device=DEV).manual_seed(9), page_size=16)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert got == want and again == drawn
