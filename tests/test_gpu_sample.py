@@ -146,6 +146,26 @@ def test_shares_of_evenly_spaced_numbers(dtype):
             assert abs(int(counts[i]) - n * p.get(i, 0.0)) <= 1.001, (i, int(counts[i]), n * p.get(i, 0.0))
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=NAMES)
+@pytest.mark.parametrize("parameters", [dict(), dict(top_k=20, temperature=0.7), dict(top_p=0.8), dict(min_p=0.2), dict(top_k=40, top_p=0.9, min_p=0.1, temperature=1.5)],
+                         ids=lambda p: "-".join(p) or "all")
+def test_probabilities_of_what_is_kept_add_up(parameters, dtype):
+    """Every token that is kept is drawn by evenly spaced numbers that lie closer than the least of their probabilities, no other is, and their probabilities together are 1."""
+    n, vocab = 8192, 61
+    x = _logits(1, vocab, dtype, seed=19, spread=0.8)
+    w = torch.exp(torch.sort(x[0].double(), descending=True, stable=True)[0] / parameters.get("temperature", 1.0))
+    w = w[:parameters.get("top_k") or vocab]
+    if "top_p" in parameters:
+        w = w[:int((w.cumsum(0) < parameters["top_p"] * w.sum()).sum()) + 1]
+    w = w[w >= parameters.get("min_p", 0.0) * w[0]]
+    assert float(w[-1] / w.sum()) * n > 2.0
+    ids, logprobs = _draw(x.to(DEV).expand(n, vocab), [(i + 0.5) / n for i in range(n)], **parameters)
+    p = {int(i): float(l) for i, l in zip(ids, logprobs)}
+    assert len(p) == len(w)
+    # a float32 rounding of each logarithm, and weights in parts of 2^51
+    assert abs(sum(math.exp(l) for l in p.values()) - 1) <= max(-l for l in p.values()) * 2.0 ** -24 * 1.01 + vocab * 2.0 ** -50
+
+
 @pytest.mark.parametrize("u,same", [(-0.5, 0.0), (1.0, 1 - 2.0 ** -24), (7.0, 1 - 2.0 ** -24), (math.inf, 1 - 2.0 ** -24), (-math.inf, 0.0), (math.nan, 0.0)])
 def test_numbers_outside_are_the_nearest_inside(u, same):
     x = _logits(3, 777, torch.bfloat16, seed=11)
