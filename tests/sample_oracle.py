@@ -11,6 +11,7 @@ import torch
 
 
 def slack(vocab):
+    """(F is 39 for 2^22 tokens and 44 for 2^17, which makes the first part 2^-18 and 2^-28.)"""
     bits = min(51, 30 + 32 - vocab.bit_length())
     return vocab * 2.0 ** -(bits + 1) + vocab * 2.0 ** -50
 
