@@ -231,7 +231,8 @@ int mi_argmax_embed(const void* x, int64_t n_rows, int64_t vocab, int64_t row_st
  * keeps the first so many.  ids[r] is the first token at which the running sum of the weights exceeds uniforms[r] times the sum of what is kept; logprobs[r] (may be
  * NULL) the natural logarithm of its weight over that sum.  temperature <= 0 or NaN: the first token (and 0).  NaN and -inf logits have no weight; where the largest
  * is +inf, those alone have one; a row without any gives token 0 (and -inf).  uniforms outside [0, 1) are taken for the nearest inside, NaN for 0.
- * Weights are rounded from 64 bits to parts of 2^51 (of more than 2048 tokens: so that all fit 62 bits) and summed as whole numbers.
+ * Weights are rounded from 64 bits to parts of 2^51 (of 2048 tokens and more to as many fewer as let the sum of all stay under 2^62: of 128256 tokens to parts of 2^45) and
+ * summed as whole numbers: a sum is off by vocab halves of a part at most, and a token that weighs less than half of one is not drawn.
  * Each parameter is an array of a value per row or, where that is NULL, one value.  row_stride in elements; rows need not be 16-byte aligned; fewer than 2^22 of them.
  * Algorithmic HBM bytes: n_rows * vocab * e.
  * ------------------------------------------------------------------------------------------ */
@@ -465,7 +466,8 @@ int mi_paged_attn(const mi_paged_attn_args* args);
 /* Attention of the new tokens of sequences that share a prefix in groups (several answers to one prompt; the reference computes each by itself): sequences
  * group_seqs[g] .. group_seqs[g + 1] - 1 (neighbours, any number, none included) all see the keys 0 .. prefix_len[g] - 1 of pages prefix_table[g], in the same pool as theirs, in
  * front of their own, which are those of mi_paged_attn: attn.page_table, ctx_len and causal are about own keys alone.  Sequences outside all groups
- * have no prefix.  A group's keys are read once for its new tokens together, not once a sequence.  Softmax over both parts; a row without any key yields zeros.
+ * have no prefix.  A group's keys are read once for its new tokens together, not once a sequence.  Softmax over both parts in fp32, probabilities rounded to `dtype` before P V as
+ * in mi_paged_attn; a row without any key yields zeros.
  * prefix_table [n_groups, max_prefix_pages] by stride; group_seqs [n_groups + 1] ascending; lengths, pages and sizes as above.
  * attn.max_q_len is about sequences, not groups, and decides how the work is cut alone: sequences over the bound are computed all the same; attn.tickets are not looked at.
  * workspace: mi_paged_prefix_attn_workspace_bytes() bytes for so many tokens, sequences and groups or more, 16-byte aligned, one call at a time; nothing in it has to be

@@ -953,7 +953,9 @@ __global__ __launch_bounds__(512, 2) void paged_tiles_kernel(const P p) {
 //     three workgroups to a compute unit (168 registers; K one and a half tiles ahead, two barriers a tile): products wait for the softmax; other workgroups' fill the pipe, or
 //     their requests the time.  Tiles of BN = 64 keys, of which every wavefront requests 16 keys of K and of V, or of 32 (two wavefronts K, two V), where the rings would
 //     let one workgroup less run on a compute unit.
-//     AHEAD, two workgroups: the next tile's scores are computed among this one's exponentials (which take twice as long as the products), one barrier a tile.
+//     AHEAD, two workgroups: the next tile's scores are computed among this one's exponentials (which take twice as long as the products), one barrier a tile.  232 registers
+//     of 128 features; of 64 features 169, one too many for a third workgroup.
+// (Either spills scalar registers, 10 - 59, into lanes of a vector register.)
 // (us of 32 drafts of 3 - 7 tokens over 8192 keys, 32 / 8 heads of 128: 58 without the next scores, 54 with them, 2650 cycles to a tile.  Rings of three or four tiles, requests spread over the products
 // or over the wavefronts: level or slower.)
 constexpr int kSmallRows = 128, kSmallShift = 7;

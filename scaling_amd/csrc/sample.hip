@@ -559,6 +559,7 @@ __device__ __forceinline__ int weight_bits(int vocab) { return min(51, 30 + __bu
 // ---- 32-bit logits --------------------------------------------------------------------------------------------------------------------------------------
 // One workgroup per row, for which every pass over it is an exchange with memory.  The first one counts the tokens by the upper 13 bits of their keys, which
 // tells from where on top-k asks for tokens; without top-p, min-p does too.  If these are few they are gathered in LDS, and all else happens there.
+// 1024 threads leave 128 registers each, of which the searches over a whole row would take more: 36 are spilled (84 bytes of scratch a lane).
 constexpr int kGathered = 6144, kCoarse = 19, kCoarseBins = 1 << (32 - kCoarse), kEach = kGathered / kThreads;      // bits of a key below its first bin
 
 // All tokens of keys lo to hi in LDS, of which there are no more than fit.

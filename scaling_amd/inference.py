@@ -401,7 +401,7 @@ class TransformerInferenceModule(torch.nn.Module):
         [prompt][sample][up to max_tokens], up to and with the first id in `stop_tokens`.
 
         A prompt is computed once and its keys are read once a step for all of its answers.  The loop runs on the device: tokens are drawn there, steps planned there, answers that have
-        ended give their pages back and take no more rows there; with `graph` a step is captured once and replayed.  uniforms float32 [max_tokens, prompts *
+        ended give their pages back there, and attention has no more rows of theirs (the layers' other parts compute a row of each answer in every step); with `graph` a step is captured once and replayed.  uniforms float32 [max_tokens, prompts *
         samples] (answer j of prompt i: column i * samples + j): the numbers to draw by; without it `generator`'s, on the module's device.  The same numbers give the
         same answers as long as the logits have the same bits, which also depend on the batch."""
         prompts = [[int(t) for t in p] for p in prompts]
