@@ -332,7 +332,8 @@ def paged_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     """`paged_attention` of sequences that share a prefix in groups, as several answers to one prompt do (inference; no autograd): the keys of a prefix are read once
     for all new tokens of its group.
 
-    Sequences group_seqs[g] .. group_seqs[g + 1] - 1 form group g (group_seqs int32 [groups + 1], ascending; sequences outside have no prefix).  All their new tokens see
+    Sequences group_seqs[g] .. group_seqs[g + 1] - 1 form group g (group_seqs int32 [groups + 1], ascending; one group at least, empty or of an empty prefix if need be; sequences outside have
+    no prefix).  All their new tokens see
     the first prefix_len[g] (int32 [groups]) keys of the pages prefix_table[g] (int32 [groups, max_prefix_pages], in the same pool), and behind these the keys of
     their own sequence as in `paged_attention`: page_table, ctx_len and causal are about own keys alone, so position p of an answer stands at
     slot p - prefix_len of its sequence.  max_q_len, an upper bound of the tokens of a sequence (not of a group), decides how the work is cut; longer sequences are computed all the
