@@ -571,23 +571,26 @@ class PagedBranches:
         return BranchStep(self, tensors, tokens, max_q_len)
 
     def _capturing(self) -> bool:
-        if self.cache.device.type != "cuda":
+        device = self.cache.device
+        if device.type != "cuda":
             return False
-        with torch.cuda.device(self.cache.device):
+        if device.index is None or device.index == torch.cuda.current_device():
+            return torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(device):
             return torch.cuda.is_current_stream_capturing()
 
     def workspace(self, tokens: int) -> torch.Tensor:
         """Scratch of ops.paged_prefix_attention for steps of `tokens` rows: one for all, which grows by a quarter at least.  What a captured step has is kept for the branches' life (or, made
         in the capture, the graph's alone)."""
-        capturing = self._capturing()
         if self._workspace is None or tokens > self._rows:
+            capturing = self._capturing()
             cache, rows = self.cache, tokens if capturing else max(tokens, self._rows * 5 // 4)
             workspace = ops.paged_prefix_workspace(self.total, len(self.prefix_len), rows, cache.n_q, cache.n_kv, cache.head_dim, cache.device)
             if capturing:
                 return workspace
             self._drop_workspace()
             self._workspace, self._rows = workspace, rows
-        elif capturing and not any(w is self._workspace for w in self._captured):
+        elif not any(w is self._workspace for w in self._captured) and self._capturing():
             self._captured.append(self._workspace)
         return self._workspace
 
