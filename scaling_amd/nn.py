@@ -522,12 +522,13 @@ class PagedKVCache:
 
 class BranchStep:
     """What one call over PagedBranches brings (PagedBranches.step makes it), as PagedStep, laid out on the device: `tokens` rows, of which as many belong to a
-    branch as have something new; `sequences` int64 [tokens]: the branch of a row; `last` int64 [branches]: its last row (0 of those without any)."""
+    branch as have something new; `sequences` int64 [tokens]: the branch of a row; `last` int64 [branches]: its last row (0 of those without any).
+    Lengths and pages are the branches', so a step is for the layers' calls in front of the next one."""
 
     def __init__(self, branches: "PagedBranches", tensors: ops.StepTensors, tokens: int, max_q_len: int) -> None:
         self.branches, self.tokens, self.max_q_len, self.longest = branches, tokens, max_q_len, branches.longest
         self.cu_seqlens, self.position_ids, self.slots, self.sequences, self.last = tensors
-        self.ctx_len = branches.ctx_len
+        self.ctx_len, self.number = branches.ctx_len, branches.planned
 
 
 class PagedBranches:
@@ -555,7 +556,7 @@ class PagedBranches:
         self.position_offset = ints([n for n in prefix for _ in range(count)])
         self.ctx_len, self.page_table = ints([0] * self.total), torch.zeros(self.total, width, dtype=torch.int32, device=cache.device)
         self.free_pages, self.state = ints(self.pages), ints([len(self.pages), 0])
-        self.sequences, self.closed = frozenset(sequences), False
+        self.sequences, self.closed, self.planned = frozenset(sequences), False, 0
         cache._branches.add(self)
         self._workspace: Optional[torch.Tensor] = None       # for steps of up to `_rows` tokens
         self._rows = 0
@@ -568,6 +569,7 @@ class PagedBranches:
         if self.closed:
             raise RuntimeError("a step of branches that are closed")
         tensors = ops.paged_step(new, self.ctx_len, self.page_table, self.free_pages, self.state, self.cache.page_size, tokens, self.max_ctx, self.position_offset)
+        self.planned += 1
         return BranchStep(self, tensors, tokens, max_q_len)
 
     def _capturing(self) -> bool:
@@ -901,6 +903,8 @@ class ParallelSelfAttention(torch.nn.Module):
             raise ValueError("a step of branches of another cache")
         if branches is not None and branches.closed:
             raise RuntimeError("a step of branches that are closed")
+        if branches is not None and step.number != branches.planned:
+            raise RuntimeError("a later step of the branches is planned, which has changed their lengths")
         if self.rotary_embedding is not None and step.longest > self.rotary_embedding.max_seq_length:
             raise IndexError(f"position {step.longest - 1} is outside the rotary table of {self.rotary_embedding.max_seq_length} rows")
         table = cache.page_table[:step.ctx_len.numel()] if branches is None else branches.page_table

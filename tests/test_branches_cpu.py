@@ -14,10 +14,14 @@ def _ints(x):
     return torch.tensor(x, dtype=torch.int32)
 
 
-def _plan(branches, tokens):
-    """A step's tensors, without a GPU to plan them on."""
+def _tensors(branches, tokens):
     long = lambda n: torch.zeros(n, dtype=torch.int64)
-    return BranchStep(branches, ops.StepTensors(_ints([0] * (branches.total + 1)), long(tokens), long(tokens), long(tokens), long(branches.total)), tokens, 1)
+    return ops.StepTensors(_ints([0] * (branches.total + 1)), long(tokens), long(tokens), long(tokens), long(branches.total))
+
+
+def _plan(branches, tokens):
+    """A step, without a GPU to plan it on."""
+    return BranchStep(branches, _tensors(branches, tokens), tokens, 1)
 
 
 def test_closed_branches_take_no_steps():
@@ -95,3 +99,20 @@ def test_scratch_of_steps_of_many_sizes(monkeypatch):
     assert set(held()) == {graphs}
     del branches
     assert not held()
+
+
+def test_a_step_is_for_the_layers_in_front_of_the_next_one(monkeypatch):
+    """Lengths and pages lie on the device and are the last planned step's: an earlier one is refused from then on."""
+    cache = _cache(num_pages=20)
+    cache.step([20, 5, 1])
+    branches = PagedBranches(cache, [0], 2, 10)
+    monkeypatch.setattr(ops, "paged_step", lambda *a, **kw: _tensors(branches, 2))
+    attention, x = _attention(), torch.zeros(1, 2, 256, dtype=torch.bfloat16)
+    first = branches.step(_ints([1, 1]), 2, 1)
+    monkeypatch.setattr(ops, "paged_append", lambda k, *a, q=None, **kw: q)
+    monkeypatch.setattr(ops, "paged_prefix_attention", lambda q, *a, **kw: q)
+    assert attention.paged_forward(x, cache, 0, first).shape == x.shape
+    second = branches.step(_ints([1, 1]), 2, 1)
+    with pytest.raises(RuntimeError, match="later step"):
+        attention.paged_forward(x, cache, 0, first)
+    assert attention.paged_forward(x, cache, 1, second).shape == x.shape
